@@ -227,6 +227,103 @@ int qg_moe_status(const void *workspace, int *invalid_tokens, int *selected, int
 int qg_moe_profile(int enable);
 int qg_moe_profile_read(int phase, double *total_ms, int *launches);
 
+/* ---- speculative verification on a paged cache (no counterpart in the
+ * reference header, whose attention and verification kernels run outside the
+ * MoE path: qwen/gpu.cu:300-455,561-613) --------------------------------
+ *
+ * One verify step of `seqs` sequences with `tokens` drafted tokens each (node
+ * 0 is the last token already chosen, 1..tokens-1 the drafts; rows
+ * [seq*tokens + node]) runs, per attention layer, qg_qk_norm_rope and
+ * qg_tree_attention, then once qg_verify_tree and qg_cache_commit. tokens is
+ * 1 for plain decoding, at most 64; seqs at most 1024.
+ *
+ * The cache: per layer two pools of F16 pages [pages][page_tokens][kv_heads]
+ * [head_dim] at k and v + layer*layer_bytes, 16-byte aligned. Position p of
+ * sequence s is row p % page_tokens of page page_table[s*table_pages +
+ * p / page_tokens]. lengths[s] positions are committed; a step's nodes take
+ * the positions after them, so the caller's table covers lengths[s] + tokens
+ * positions. Entries of page_table past those are never read. page_tokens:
+ * 16, 32, 64, 128 or 256. head_dim: 64, 128 or 256.
+ *
+ * A sequence whose length is negative or leaves no room for its nodes, or
+ * whose table names a page outside the pool, gets NaN rows and no store;
+ * other sequences are not affected. */
+typedef struct {
+    void *k, *v;
+    const int *page_table;  /* device [seqs][table_pages] */
+    int *lengths;           /* device [seqs] */
+    size_t layer_bytes;     /* from one layer's pool to the next's */
+    int layers, pages, page_tokens, table_pages, kv_heads, head_dim;
+} qg_kv_cache;
+
+/* table [positions][rotary/2][2]: cos and sin of position*base^(-2i/rotary),
+ * evaluated in 64 bits and rounded once. rotary: even, 2..256. */
+int qg_rope_table(float *table, int positions, int rotary, double base);
+
+/* Queries and keys of one layer: every head x [head_dim] becomes
+ * x*rsqrt(mean(x*x) + eps)*weight, then its values i and i + rotary/2
+ * (i < rotary/2) are rotated by the table's angle for the row's position
+ * lengths[seq] + offsets[row] (offsets: the node's depth in the tree; NULL:
+ * the node's index, a chain). Queries go to q_out [row][q_heads][head_dim];
+ * keys and the values v, rounded to F16, to the cache at position
+ * lengths[seq] + node. q, k, v: rows of q_stride / k_stride / v_stride floats
+ * (so they may be parts of one projection's rows); q_out may be q when
+ * q_stride is q_heads*head_dim. rotary: 0 (no rotation, rope unused) or even
+ * and at most head_dim. A row whose position is outside the rope table gets NaN
+ * queries and no store. */
+int qg_qk_norm_rope(float *q_out, const qg_kv_cache *cache, int layer, const float *q, int q_stride, const float *k,
+                    int k_stride, const float *v, int v_stride, const float *q_weight, const float *k_weight, float eps,
+                    const float *rope, int rope_positions, int rotary, const int *offsets, int seqs, int tokens,
+                    int q_heads);
+
+/* Attention of the drafted tokens over the cache (q_heads a multiple of
+ * kv_heads; query head h reads key/value head h / (q_heads/kv_heads)):
+ *   out[row][h] = sum_j softmax_j(scale * q[row][h] . K_j) V_j
+ * over the committed positions and the nodes that the row's mask names: bit j
+ * of tree[row] is node j (its own bit is not implied). tree NULL: a chain,
+ * node i sees nodes 0..i. A row that sees nothing is zero. What a row does not
+ * see has no effect on it, whatever its bits (NaN and infinities included).
+ * q and out: [row][q_heads][head_dim] F32, 16-byte aligned. The workspace is
+ * zero-filled once; calls sharing it must not overlap on the device.
+ * Deterministic, graph-capturable, no host synchronisation. */
+int qg_attention_workspace_bytes(int seqs, int tokens, int q_heads, int kv_heads, int head_dim, size_t *bytes);
+int qg_tree_attention(float *out, const float *q, const qg_kv_cache *cache, int layer, const uint64_t *tree, float scale,
+                      int seqs, int tokens, int q_heads, void *workspace);
+
+/* Which drafts the target accepts, and its next token. logits [row][vocab] are
+ * the target's after each node, p = softmax(logits/temperature) (temperature
+ * 0: all on the largest logit, the lowest index of equals). draft[row] is the
+ * node's token, parents[row] its parent (< node; node 0 is the root, whose
+ * draft and parent are not read; -1: an unused node), uniforms [row] the given
+ * random numbers in [0, 1). From the root on, the children of the current
+ * node are tried in ascending order:
+ *  - draft_probs NULL (drafts taken as they are): child c is accepted when
+ *    uniforms[c] * (p's mass left) < p(draft[c]), otherwise draft[c] leaves p;
+ *  - draft_probs [row][vocab], the distribution each draft was drawn from
+ *    (chains: a node with two children is refused): accepted when
+ *    uniforms[c] * draft_probs[c](draft[c]) < p(draft[c]), otherwise p becomes
+ *    max(p - draft_probs[c], 0) (p itself where that is zero everywhere).
+ * When no child is accepted, next[seq] is drawn from what is left of p with
+ * uniforms[root]: the first token at which p's running sum exceeds
+ * uniforms[root] * its total. So the tokens follow the target's distribution.
+ * path [seq][tokens]: the accepted nodes from the root (0) on, then -1;
+ * accepted[seq]: their number without the root. A sequence that meets a row with a
+ * NaN or +infinite logit or no finite one, a malformed tree or a draft outside
+ * the vocabulary on its way gets accepted, next and path -1.
+ * Sums over the vocabulary are held in 64 bits: the tokens do not depend on
+ * how the work is split. vocab at most 2^24. The workspace is zero-filled once. */
+int qg_verify_workspace_bytes(int seqs, int tokens, int vocab, size_t *bytes);
+int qg_verify_tree(int *path, int *accepted, int *next, const float *logits, const int *draft, const int *parents,
+                   const float *draft_probs, const float *uniforms, double temperature, int seqs, int tokens, int vocab,
+                   void *workspace);
+
+/* Keeps the accepted nodes: in every layer the key and value rows of nodes
+ * path[seq][1..accepted[seq]] move to the positions after node 0's, and
+ * lengths_out[seq] = lengths[seq] + accepted[seq] + 1. lengths_out may be the
+ * cache's lengths. A sequence with accepted < 0 (or a path that is not
+ * ascending) keeps its length and its rows. */
+int qg_cache_commit(const qg_kv_cache *cache, int *lengths_out, const int *path, const int *accepted, int seqs, int tokens);
+
 /* ---- loading an all-resident model (no counterpart in the reference
  * header; the reference's loader is qwen/qwen.c:108-146,324-369) -------- */
 

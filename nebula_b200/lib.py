@@ -45,6 +45,13 @@ SIGNATURES = {
     "moe_layer_ep": ([P, P, P, P, I, P, P, P, I, P, I, P, I, I, P, P, I, P, I, P, I, P, I, I, I, I, I, P], I),
     "moe_status": ([P, C.POINTER(I), C.POINTER(I), C.POINTER(I)], I),
     "moe_profile": ([I], I), "moe_profile_read": ([I, C.POINTER(D), C.POINTER(I)], I),
+    "rope_table": ([P, I, I, D], I),
+    "qk_norm_rope": ([P, P, I, P, I, P, I, P, I, P, P, F, P, I, I, P, I, I, I], I),
+    "attention_workspace_bytes": ([I, I, I, I, I, C.POINTER(Z)], I),
+    "tree_attention": ([P, P, P, I, P, F, I, I, I, P], I),
+    "verify_workspace_bytes": ([I, I, I, C.POINTER(Z)], I),
+    "verify_tree": ([P, P, P, P, P, P, P, P, D, I, I, I, P], I),
+    "cache_commit": ([P, P, P, P, I, I], I),
     "synth_weights": ([P, I, I, I, U64, F], I), "synth_normal": ([P, Z, U64, F], I),
     "index_open": ([C.c_char_p, C.POINTER(P), C.c_char_p, Z], I), "index_close": ([P], None),
     "index_tensor": ([P, C.c_char_p, C.POINTER(P), C.POINTER(I), C.POINTER(U64), C.POINTER(U64)], I),
@@ -53,6 +60,14 @@ SIGNATURES = {
     "route_trace_next": ([P, C.POINTER(I), C.POINTER(I), C.POINTER(I), P, P, I], I),
     "route_trace_close": ([P], None),
 }
+
+
+class KvCache(C.Structure):
+    """qg_kv_cache: the paged key/value cache of the verify step (pass C.byref of it)."""
+
+    _fields_ = [("k", P), ("v", P), ("page_table", P), ("lengths", P), ("layer_bytes", Z), ("layers", I), ("pages", I),
+                ("page_tokens", I), ("table_pages", I), ("kv_heads", I), ("head_dim", I)]
+
 
 _LIB = None
 
@@ -196,6 +211,24 @@ def workspace(tokens: int, hidden: int, ffn: int) -> Device:
     ws = Device(nbytes=workspace_bytes(tokens, hidden, ffn))
     call("zero", ws.p, ws.nbytes)
     return ws
+
+
+def _zeroed(name: str, *sizes) -> Device:
+    n = Z(0)
+    call(name, *sizes, C.byref(n))
+    ws = Device(nbytes=n.value)
+    call("zero", ws.p, ws.nbytes)
+    return ws
+
+
+def attention_workspace(seqs: int, tokens: int, q_heads: int, kv_heads: int, head_dim: int) -> Device:
+    """A zero-filled workspace for qg_tree_attention."""
+    return _zeroed("attention_workspace_bytes", seqs, tokens, q_heads, kv_heads, head_dim)
+
+
+def verify_workspace(seqs: int, tokens: int, vocab: int) -> Device:
+    """A zero-filled workspace for qg_verify_tree."""
+    return _zeroed("verify_workspace_bytes", seqs, tokens, vocab)
 
 
 def status(ws) -> tuple[int, int, int]:
