@@ -13,7 +13,7 @@ struct CacheView {
     const int *lengths;
     int pages, shift, table_pages, kv_heads, head_dim;
 
-    __device__ int page_tokens() const { return 1 << shift; }
+    __host__ __device__ int page_tokens() const { return 1 << shift; }
     // Committed tokens of a sequence, or -1 when its length leaves no room for its nodes.
     __device__ int committed(int seq, int tokens) const {
         const int n = lengths[seq];
