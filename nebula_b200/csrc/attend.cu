@@ -2,7 +2,7 @@
 //
 // For one sequence and key/value head, the queries of all nodes and of the
 // group's heads are the rows of one matrix product: rows (node, head of the
-// group), 128 to a tile. A CTA streams 64 keys at a time:
+// group), 128 to a tile. A CTA streams 128 keys at a time:
 //     S = Q K^T          tcgen05, Q and K in shared memory, S in tensor memory
 //     P = 2^(c S - m)    one thread per row, m the row's running maximum
 //     O = P V            tcgen05, P in tensor memory, V in shared memory
@@ -10,11 +10,11 @@
 // and out = acc / sum(P). F32 results need more than one F16 product: Q is
 // scaled by a power of two per row and split into F16 hi + lo (22 bits), P
 // likewise, and both planes go into the same accumulator; K and V are F16 as
-// they are. O starts anew with every 64 keys and is added up in registers,
+// they are. O starts anew with every 128 keys and is added up in registers,
 // because an accumulation on the tensor cores does not round to nearest: one
 // accumulator over thousands of keys would drift towards zero.
 //
-// Work is cut into units of 64 keys of one (sequence, head, row tile), and the
+// Work is cut into units of 128 keys of one (sequence, head, row tile), and the
 // CTAs take equal contiguous ranges of them, so one long sequence fills the
 // GPU as well as many short ones. A range that covers an item only in part
 // leaves its unnormalised sum, maximum and total in the workspace; a second
@@ -34,7 +34,7 @@ using namespace nb;
 namespace {
 
 constexpr int kRows = 128;       // rows per tile (MMA M)
-constexpr int kKeys = 64;        // keys per unit
+constexpr int kKeys = 128;       // keys per unit (MMA N of S: with 64 the re-reads of Q bound the shared memory)
 constexpr int kMaxCtas = 148;    // SMs of a B200: one CTA each
 constexpr int kThreads = 512;
 // Registers per thread after the split; the four warpgroups' sum is what the
@@ -51,31 +51,34 @@ struct AttendArgs {
     float scale;  // |scale| * log2(e)
     float sign;   // of scale, folded into Q
     int seqs, tokens, q_heads, group, row_tiles, part_rows;
-    int box;      // rows of one TMA box: a page, at most kKeys
+    int k_box, v_box;  // rows of one TMA box: a page, at most a piece's keys
     int *err;
     float *part_acc;   // [2 * kMaxCtas][part_rows][D]
     float2 *part_ml;   // [2 * kMaxCtas][part_rows]
 };
 
+constexpr int kStage = 16384;    // one piece of the ring
+constexpr int kChunk = 32;       // keys per step of the softmax
+
 template <int D>
 struct Cfg {
-    static constexpr int kChunks = D / 64;                  // 128-byte wide column blocks
-    static constexpr int kPlane = kChunks * kRows * 128;    // one plane of Q
-    static constexpr int kStage = kChunks * kKeys * 128;    // 64 keys or values
-    static constexpr int kStages = D == 256 ? 3 : 8;
+    static constexpr int kChunks = D / 64;                // 128-byte wide column blocks
+    static constexpr int kPlane = kChunks * kRows * 128;  // one plane of Q
+    // The ring's pieces: 64 columns of 128 keys, or all columns of kVKeys values; kChunks pieces for a unit's keys or values.
+    static constexpr int kVKeys = kStage / (2 * D);
+    static constexpr int kStages = D == 256 ? 6 : 8;
     static constexpr int kSmem = 2 * kPlane + kStages * kStage + 2048 + 1024;
-    // tensor memory columns: O, two S, two P (hi and lo, two values a column)
-    static constexpr int kS = 256, kP = 384;
+    static constexpr int kS = 256;  // tensor memory columns: O, then two of S (P takes its place)
 };
 
 struct Shared {
     float val[2][kRows];    // rescaling factors, and at an item's end the totals: softmax -> accumulators
     float q_scale[kRows];
-    uint64_t full[8], empty[8], s_full[2], s_empty[2], p_full[2], p_empty[2], v_full[2], v_empty[2], o_full, o_empty, q_full, drain;
+    uint64_t full[8], empty[8], s_full[2], p_full[2][kKeys / kChunk], pv_done[2], v_full[2], v_empty[2], o_full, o_empty, q_full, drain;
     uint64_t odd_nodes;     // nodes whose values are not finite: softmax warps only
     uint64_t odd_msg[2];    // the same, posted with an item's totals
     long long unit0, unit1, base;
-    int seq0;
+    int seq0, length0;
     uint32_t tmem;
     int abort;
 };
@@ -180,27 +183,29 @@ __device__ __forceinline__ bool group_any(int id, int n, bool x) {
 
 // ---- the division of the work ---------------------------------------------
 
-// Units of one (sequence, head, row tile); 0: the sequence is refused.
-__device__ __forceinline__ int units_of(const AttendArgs &a, int seq) {
-    const int n = a.c.committed(seq, a.tokens);
-    return n < 0 ? 0 : (n + a.tokens + kKeys - 1) / kKeys;
+// Units of one (sequence, head, row tile); 0: the sequence is refused (length -1).
+__device__ __forceinline__ int units_of(const AttendArgs &a, int length) {
+    return length < 0 ? 0 : (length + a.tokens + kKeys - 1) / kKeys;
 }
-// One warp: units of all sequences, of those before `seq`, or (find) the
-// sequence that holds unit `at` and the units before it.
-__device__ long long sum_units(const AttendArgs &a, int seqs, int per) {
-    const int lane = threadIdx.x & 31;
-    long long sum = 0;
-    for (int s = lane; s < seqs; s += 32) sum += (long long)units_of(a, s) * per;
+__device__ __forceinline__ long long warp_sum(long long x) {
 #pragma unroll
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    return sum;
+    for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    return x;
 }
-__device__ int find_unit(const AttendArgs &a, int per, long long at, long long &base) {
+// One warp: units of the sequences before `seqs`.
+__device__ long long sum_units(const AttendArgs &a, int seqs, int per) {
+    long long sum = 0;
+    for (int s = threadIdx.x & 31; s < seqs; s += 32) sum += (long long)units_of(a, a.c.committed(s, a.tokens)) * per;
+    return warp_sum(sum);
+}
+// One warp: the sequence that holds unit `at`, its length and the units before it.
+__device__ int find_unit(const AttendArgs &a, int per, long long at, long long &base, int &length) {
     const int lane = threadIdx.x & 31;
     base = 0;
     for (int s0 = 0; s0 < a.seqs; s0 += 32) {
         const int s = s0 + lane;
-        const long long mine = s < a.seqs ? (long long)units_of(a, s) * per : 0;
+        const int len = s < a.seqs ? a.c.committed(s, a.tokens) : -1;
+        const long long mine = (long long)units_of(a, len) * per;
         long long upto = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -211,15 +216,20 @@ __device__ int find_unit(const AttendArgs &a, int per, long long at, long long &
         if (past) {
             const int l = __ffs(past) - 1;
             base += __shfl_sync(0xffffffffu, upto - mine, l);
+            length = __shfl_sync(0xffffffffu, len, l);
             return s0 + l;
         }
         base += __shfl_sync(0xffffffffu, upto, 31);
     }
     return a.seqs;
 }
+// Quotients that nearly always fit 32 bits.
+__device__ __forceinline__ long long quotient(long long x, long long y) {
+    return (x | y) >> 32 ? x / y : (long long)((uint32_t)x / (uint32_t)y);
+}
 // CTA c of g takes units [c*w/g, (c+1)*w/g).
-__device__ __forceinline__ long long range_start(long long c, long long w, int g) { return c * w / g; }
-__device__ __forceinline__ int cta_of(long long unit, long long w, int g) { return (int)(((unit + 1) * g + w - 1) / w) - 1; }
+__device__ __forceinline__ long long range_start(long long c, long long w, int g) { return quotient(c * w, g); }
+__device__ __forceinline__ int cta_of(long long unit, long long w, int g) { return (int)quotient((unit + 1) * g + w - 1, w) - 1; }
 
 // One CTA's part of one item.
 struct Item {
@@ -228,44 +238,53 @@ struct Item {
 };
 struct Walk {
     long long at, end, base;
-    int seq;
-    __device__ Walk(const Shared &s) : at(s.unit0), end(s.unit1), base(s.base), seq(s.seq0) {}
+    int seq, length;
+    __device__ Walk(const Shared &s) : at(s.unit0), end(s.unit1), base(s.base), seq(s.seq0), length(s.length0) {}
     __device__ bool next(const AttendArgs &a, Item &it) {
         if (at >= end) return false;
         const int per = a.c.kv_heads * a.row_tiles;
-        for (;;) {
-            it.units = units_of(a, seq);
-            if (at < base + (long long)it.units * per) break;
-            base += (long long)it.units * per;
-            seq++;
+        while (at >= base + (long long)units_of(a, length) * per) {
+            base += (long long)units_of(a, length) * per;
+            length = a.c.committed(++seq, a.tokens);
         }
+        it.units = units_of(a, length);
         const long long in = at - base;
-        const int index = (int)(in / it.units);
+        const int index = (int)quotient(in, it.units);
         it.seq = seq;
         it.kv = index / a.row_tiles;
         it.tile = index % a.row_tiles;
         it.first = (int)(in - (long long)index * it.units);
         it.count = (int)min((long long)(it.units - it.first), end - at);
-        it.length = a.c.lengths[seq];
+        it.length = length;
         it.start = at - it.first;
         at += it.count;
         return true;
     }
 };
 
-// The ring's order within an item of n units: K0, K1, V0, K2, V1, ..., V(n-1).
+// The ring's order within an item of n units: K0, K1, V0, K2, V1, ..., V(n-1),
+// `pieces` pieces each; a last unit that is not full has fewer pieces of V.
 __device__ __forceinline__ uint32_t k_index(int j) { return j ? 2 * j - 1 : 0; }
 __device__ __forceinline__ uint32_t v_index(int j, int n) { return j == n - 1 ? 2 * n - 1 : 2 * j + 2; }
+// Keys that unit j of an item's part holds.
+__device__ __forceinline__ int keys_of(const AttendArgs &a, const Item &it, int j) {
+    return min(kKeys, it.length + a.tokens - (it.first + j) * kKeys);
+}
+template <int D>
+__device__ __forceinline__ uint32_t ring_pieces(const AttendArgs &a, const Item &it) {
+    return (2 * it.count - 1) * Cfg<D>::kChunks + (keys_of(a, it, it.count - 1) + Cfg<D>::kVKeys - 1) / Cfg<D>::kVKeys;
+}
 
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __grid_constant__ AttendArgs a,
                                                                      const __grid_constant__ CUtensorMap k_map,
                                                                      const __grid_constant__ CUtensorMap v_map) {
     using C = Cfg<D>;
+    constexpr int NC = C::kChunks, NS = C::kStages, VK = C::kVKeys;
     extern __shared__ unsigned char raw[];
     unsigned char *smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
     unsigned char *q_smem = smem, *ring = smem + 2 * C::kPlane;
-    Shared &s = *reinterpret_cast<Shared *>(ring + C::kStages * C::kStage);
+    Shared &s = *reinterpret_cast<Shared *>(ring + NS * kStage);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     volatile int *abort = &s.abort;
 
@@ -274,29 +293,32 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         const long long w = sum_units(a, a.seqs, per);
         const int g = (int)min((long long)gridDim.x, w);
         long long base = 0, u0 = 0, u1 = 0;
-        int seq = 0;
+        int seq = 0, length = -1;
         if ((int)blockIdx.x < g) {
             u0 = range_start(blockIdx.x, w, g);
             u1 = range_start(blockIdx.x + 1, w, g);
-            seq = find_unit(a, per, u0, base);
+            seq = find_unit(a, per, u0, base, length);
         }
         if (lane == 0) {
-            s.unit0 = u0, s.unit1 = u1, s.base = base, s.seq0 = seq;
-            s.abort = 0;
-            s.odd_nodes = 0;
-            for (int i = 0; i < C::kStages; i++) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], 1);
-            for (int i = 0; i < 2; i++) {
-                mbar_init(&s.s_full[i], 1), mbar_init(&s.s_empty[i], 4);
-                mbar_init(&s.p_full[i], 4), mbar_init(&s.p_empty[i], 1);
-                mbar_init(&s.v_full[i], 4), mbar_init(&s.v_empty[i], 8);
-            }
-            mbar_init(&s.o_full, 1), mbar_init(&s.o_empty, 8), mbar_init(&s.q_full, 8), mbar_init(&s.drain, 2);
-            fence_mbar_init();
+            s.unit0 = u0, s.unit1 = u1, s.base = base, s.seq0 = seq, s.length0 = length;
         }
-    }
-    if (warp == 1) {
+    } else if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s.tmem)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    } else if (warp == 2 && lane == 0) {
+        s.abort = 0;
+        s.odd_nodes = 0;
+        for (int i = 0; i < NS; i++) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], 1);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&s.s_full[i], 1), mbar_init(&s.pv_done[i], 1);
+            mbar_init(&s.v_full[i], 4), mbar_init(&s.v_empty[i], 8);
+            for (int k = 0; k < kKeys / kChunk; k++) mbar_init(&s.p_full[i][k], 4);
+        }
+        mbar_init(&s.o_full, 1), mbar_init(&s.o_empty, 8), mbar_init(&s.q_full, 8), mbar_init(&s.drain, 2);
+        fence_mbar_init();
+    } else if (warp == 3 && lane == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map));
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map));
     }
     tc_fence_before();
     __syncthreads();
@@ -308,64 +330,86 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
-        if (warp == 0 && lane == 0) {
+        if (warp == 0) {
             // ------------------------------------------------ producer: pages to the ring
+            // The warp looks the pages of one unit up ahead of time (a lane each) and its lanes issue the boxes.
             uint32_t idx = 0;
             bool ok = true;
-            const int page = a.c.page_tokens();
+            const int page = a.c.page_tokens(), per_unit = max(1, kKeys >> a.c.shift);
             while (ok && walk.next(a, it)) {
                 const int n = it.length + a.tokens;
                 const int *table = a.c.table + (size_t)it.seq * a.c.table_pages;
-                for (int i = 0; ok && i < 2 * it.count; i++, idx++) {
+                auto look_up = [&](int j) {  // page of keys l*page.. of unit j, for lane l
+                    const int p = (((it.first + j) * kKeys) >> a.c.shift) + lane;
+                    const int id = lane < per_unit && p <= (n - 1) >> a.c.shift ? table[p] : 0;
+                    return (unsigned)id < (unsigned)a.c.pages ? id : 0;  // the accumulators make the row NaN
+                };
+                int next_ids = look_up(0), k_ids = 0, v_ids = 0;
+                for (int i = 0; ok && i < 2 * it.count; i++) {
                     // i-th of K0, K1, V0, K2, V1, ...
                     const bool is_k = i == 0 || (i & 1 && i != 2 * it.count - 1);
                     const int j = is_k ? (i + 1) / 2 : (i == 2 * it.count - 1 ? it.count - 1 : i / 2 - 1);
-                    const int st = idx % C::kStages;
-                    if (idx >= C::kStages) ok = wait(&s.empty[st], (idx / C::kStages - 1) & 1, abort, a.err);
-                    if (!ok) break;
-                    const int pos = (it.first + j) * kKeys;
-                    const int boxes = (min(kKeys, n - pos) + a.box - 1) / a.box;  // none past the last position
-                    mbar_arrive_expect_tx(&s.full[st], boxes * a.box * 128 * C::kChunks);
-                    for (int b = 0; b < boxes; b++) {
-                        const int p = pos + b * a.box;
-                        int id = table[p >> a.c.shift];
-                        if ((unsigned)id >= (unsigned)a.c.pages) id = 0;  // the accumulators make the row NaN
-                        const int y = (id << a.c.shift) + (p & (page - 1));
-                        for (int c = 0; c < C::kChunks; c++)
-                            tma_2d(ring + st * C::kStage + c * kKeys * 128 + b * a.box * 128, is_k ? &k_map : &v_map,
-                                   it.kv * D + c * 64, y, &s.full[st]);
+                    if (is_k) {
+                        v_ids = k_ids;
+                        k_ids = next_ids;
+                        if (j + 1 < it.count) next_ids = look_up(j + 1);
+                    } else if (j == it.count - 1) {
+                        v_ids = k_ids;
+                    }
+                    const int ids = is_k ? k_ids : v_ids;
+                    const int pos = (it.first + j) * kKeys, keys = keys_of(a, it, j);
+                    const int box = is_k ? a.k_box : a.v_box, piece = is_k ? kKeys : VK;
+                    const int pieces = is_k ? NC : (keys + VK - 1) / VK;
+                    for (int c = 0; ok && c < pieces; c++, idx++) {
+                        const int st = idx % NS;
+                        if (idx >= NS) ok = wait_warp(&s.empty[st], (idx / NS - 1) & 1, abort, a.err);
+                        if (!ok) break;
+                        const int key0 = is_k ? 0 : c * VK;  // the piece's first key within the unit
+                        const int boxes = (min(piece, keys - key0) + box - 1) / box;  // none past the last position
+                        const int blocks = is_k ? 1 : NC;                              // column blocks of the piece
+                        if (lane == 0) mbar_arrive_expect_tx(&s.full[st], boxes * blocks * box * 128);
+                        __syncwarp();
+                        const int b = is_k ? lane : lane / NC, col = is_k ? c : lane % NC;
+                        const int key = key0 + b * box, p = pos + key;
+                        const int id = __shfl_sync(0xffffffffu, ids, (p >> a.c.shift) - (pos >> a.c.shift) & 31);
+                        if (b < boxes)
+                            tma_2d(ring + st * kStage + (is_k ? 0 : col * VK * 128) + b * box * 128, is_k ? &k_map : &v_map,
+                                   it.kv * D + col * 64, (id << a.c.shift) + (p & (page - 1)), &s.full[st]);
                     }
                 }
             }
-            if (!ok)  // the copies in flight land before the CTA ends
-                for (uint32_t i = idx > C::kStages ? idx - C::kStages : 0; i < idx; i++)
-                    wait_drain(&s.full[i % C::kStages], (i / C::kStages) & 1);
+            if (!ok && lane == 0)  // the copies in flight land before the CTA ends
+                for (uint32_t i = idx > NS ? idx - NS : 0; i < idx; i++) wait_drain(&s.full[i % NS], (i / NS) & 1);
         } else if (warp == 1 && lane == 0) {
             // ------------------------------------------------ S = Q K^T
             uint32_t ring0 = 0, tile = 0, item = 0;
             bool ok = true;
+            const uint64_t q_lo = operand(smem_u32(q_smem) + C::kPlane, 16);
+            const uint64_t q_hi = operand(smem_u32(q_smem), 16);
             while (ok && walk.next(a, it)) {
                 ok = wait(&s.q_full, item & 1, abort, a.err);
                 for (int j = 0; ok && j < it.count; j++, tile++) {
-                    const uint32_t idx = ring0 + k_index(j), st = idx % C::kStages, buf = tile & 1;
-                    ok = wait(&s.full[st], (idx / C::kStages) & 1, abort, a.err) &&
-                         (tile < 2 || wait(&s.s_empty[buf], (tile / 2 - 1) & 1, abort, a.err));
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t d = tmem + C::kS + buf * kKeys;
-                    const uint32_t kb = smem_u32(ring + st * C::kStage), qb = smem_u32(q_smem);
+                    const uint32_t buf = tile & 1, d = tmem + C::kS + buf * kKeys;
+                    uint32_t idx = ring0 + k_index(j) * NC;
+                    if (tile >= 2) ok = wait(&s.pv_done[buf], (tile / 2 - 1) & 1, abort, a.err);
+#pragma unroll 1
+                    for (int c = 0; ok && c < NC; c++, idx++) {
+                        const uint32_t st = idx % NS;
+                        ok = wait(&s.full[st], (idx / NS) & 1, abort, a.err);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint64_t kd = operand(smem_u32(ring + st * kStage), 16);
 #pragma unroll
-                    for (int p = 0; p < 2; p++)
+                        for (int k = 0; k < 4; k++)
+                            mma_ss(d, q_lo + c * (kRows * 128 / 16) + 2 * k, kd + 2 * k, idesc(kKeys, false), c + k > 0);
 #pragma unroll
-                        for (int c = 0; c < C::kChunks; c++)
-#pragma unroll
-                            for (int k = 0; k < 4; k++)
-                                mma_ss(d, operand(qb + (1 - p) * C::kPlane + c * kRows * 128 + k * 32, 16),
-                                       operand(kb + c * kKeys * 128 + k * 32, 16), idesc(kKeys, false), p + c + k > 0);
-                    commit(&s.empty[st]);
-                    commit(&s.s_full[buf]);
+                        for (int k = 0; k < 4; k++)
+                            mma_ss(d, q_hi + c * (kRows * 128 / 16) + 2 * k, kd + 2 * k, idesc(kKeys, false), true);
+                        commit(&s.empty[st]);
+                    }
+                    if (ok) commit(&s.s_full[buf]);
                 }
-                ring0 += 2 * it.count;
+                ring0 += ring_pieces<D>(a, it);
                 item++;
             }
             commit(&s.drain);
@@ -376,24 +420,34 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             bool ok = true;
             while (ok && walk.next(a, it)) {
                 for (int j = 0; ok && j < it.count; j++, tile++) {
-                    const uint32_t idx = ring0 + v_index(j, it.count), st = idx % C::kStages, buf = tile & 1;
-                    ok = wait(&s.full[st], (idx / C::kStages) & 1, abort, a.err) &&
-                         (tile < 1 || wait(&s.o_empty, (tile - 1) & 1, abort, a.err)) &&
-                         wait(&s.p_full[buf], (tile / 2) & 1, abort, a.err);
+                    const uint32_t buf = tile & 1, p0 = tmem + C::kS + buf * kKeys;
+                    const int keys = keys_of(a, it, j);
+                    uint32_t idx = ring0 + v_index(j, it.count) * NC;
+                    if (tile >= 1) ok = wait(&s.o_empty, (tile - 1) & 1, abort, a.err);
+                    // 32 keys at a time, as the softmax delivers them; past the last key there is nothing
+#pragma unroll 1
+                    for (int h = 0; ok && h * kChunk < keys; h++) {
+                        const uint32_t st = idx % NS;
+                        ok = wait(&s.full[st], (idx / NS) & 1, abort, a.err) && wait(&s.p_full[buf][h], (tile / 2) & 1, abort, a.err);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const int row = h * kChunk % VK;
+                        const uint64_t vd = operand(smem_u32(ring + st * kStage) + row * 128, VK * 128);
+                        const int steps = min(2, (keys - h * kChunk + 15) / 16);
+                        for (int k = 0; k < steps; k++) {
+                            mma_ts(tmem, p0 + h * kChunk + 16 + k * 8, vd + k * 128, idesc(D, true), h + k > 0);
+                            mma_ts(tmem, p0 + h * kChunk + k * 8, vd + k * 128, idesc(D, true), true);
+                        }
+                        if (row + kChunk == VK || (h + 1) * kChunk >= keys) {
+                            commit(&s.empty[st]);
+                            idx++;
+                        }
+                    }
                     if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t p0 = tmem + C::kP + buf * kKeys, vb = smem_u32(ring + st * C::kStage);
-#pragma unroll
-                    for (int p = 0; p < 2; p++)
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            mma_ts(tmem, p0 + (1 - p) * (kKeys / 2) + k * 8, operand(vb + k * 2048, kKeys * 128), idesc(D, true),
-                                   p + k > 0);
-                    commit(&s.empty[st]);
-                    commit(&s.p_empty[buf]);
+                    commit(&s.pv_done[buf]);
                     commit(&s.o_full);
                 }
-                ring0 += 2 * it.count;
+                ring0 += ring_pieces<D>(a, it);
             }
             commit(&s.drain);
             wait_drain(&s.drain, 0);
@@ -406,46 +460,51 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         uint32_t ring0 = 0, tile = 0, item = 0, msg = 0;
         bool ok = true;
         while (ok && walk.next(a, it)) {
-            ok = wait_warp(&s.q_full, item & 1, abort, a.err);
-            const float c = s.q_scale[row];
-            const int r = it.tile * kRows + row, node = r / a.group;
+            const int node = (it.tile * kRows + row) / a.group;
             uint64_t mask = 0;
             if (node < a.tokens) {
                 mask = a.tree ? a.tree[(size_t)it.seq * a.tokens + node] : ~0ull >> (63 - node);
                 if (a.tokens < 64) mask &= (1ull << a.tokens) - 1;
             }
+            ok = wait_warp(&s.q_full, item & 1, abort, a.err);
+            const float c = s.q_scale[row];
             float m = -INFINITY, l = 0.0f, l_low = 0.0f;
             for (int j = 0; ok && j < it.count; j++, tile++) {
-                const uint32_t buf = tile & 1;
+                const uint32_t buf = tile & 1, cols = tmem + lanes + C::kS + buf * kKeys;
+                const int past = it.length - (it.first + j) * kKeys;  // keys of this unit before the nodes
+                const bool tail = past < kKeys;
+                // which of keys 32h .. 32h+31 the row sees, in a unit that holds nodes
+                auto seen = [&](int h) -> uint32_t {
+                    const int at = past - 32 * h;  // keys of the chunk before the nodes
+                    if (at >= 32) return ~0u;
+                    const uint32_t before = at > 0 ? (1u << at) - 1 : 0;
+                    return before | (uint32_t)(at > 0 ? mask << at : at > -64 ? mask >> -at : 0);
+                };
                 ok = wait_warp(&s.s_full[buf], (tile / 2) & 1, abort, a.err);
                 if (!ok) break;
                 tc_fence_after();
-                float x[2][32];
-                tmem_ld32(tmem + lanes + C::kS + buf * kKeys, x[0]);
-                tmem_ld32(tmem + lanes + C::kS + buf * kKeys + 32, x[1]);
-                tmem_wait_ld();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) arrive(&s.s_empty[buf]);
-                const int pos = (it.first + j) * kKeys, past = it.length - pos;  // keys of this unit before the nodes
-                const bool tail = past < kKeys;
-                if (tail) {
-                    const uint64_t seen = (past > 0 ? (1ull << past) - 1 : 0) |
-                                          (past > 0 ? mask << past : past > -64 ? mask >> -past : 0);
+                float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll 1
+                for (int h = 0; h < kKeys / kChunk; h += 2) {
+                    float x[2][32];
+                    tmem_ld32(cols + 32 * h, x[0]);
+                    tmem_ld32(cols + 32 * h + 32, x[1]);
+                    tmem_wait_ld();
+                    if (tail) {
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const uint32_t bits = (uint32_t)(seen >> (32 * h));
+                        for (int g = 0; g < 2; g++) {
+                            const uint32_t bits = seen(h + g);
 #pragma unroll
-                        for (int i = 0; i < 32; i++) x[h][i] = bits >> i & 1 ? x[h][i] : -INFINITY;
+                            for (int i = 0; i < 32; i++) x[g][i] = bits >> i & 1 ? x[g][i] : -INFINITY;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        top[0] = fmaxf(top[0], x[0][i]);
+                        top[1] = fmaxf(top[1], x[1][i]);
                     }
                 }
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int i = 0; i < 32; i++) {
-                    top[i & 1] = fmaxf(top[i & 1], x[0][i]);
-                    top[2 + (i & 1)] = fmaxf(top[2 + (i & 1)], x[1][i]);
-                }
-                const float m_new = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c);
+                const float m_new = fmaxf(m, fmaxf(top[0], top[1]) * c);
                 const float keep = m == -INFINITY ? 0.0f : ex2(m - m_new);
                 const float off = m_new == -INFINITY ? 0.0f : m_new;
                 m = m_new;
@@ -457,26 +516,61 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 __syncwarp();
                 if (lane == 0) arrive(&s.v_full[slot]);
                 msg++;
-                if (tile >= 2) ok = wait_warp(&s.p_empty[buf], (tile / 2 - 1) & 1, abort, a.err);
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t p_cols = tmem + lanes + C::kP + buf * kKeys;
                 float2 sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
                 const float2 c2 = {c, c}, off2 = {-off, -off}, up2 = {kPScale, kPScale};
+#pragma unroll 1
+                for (int h = 0; ok && h < kKeys / kChunk; h++) {
+                    float x[32];
+                    tmem_ld32(cols + 32 * h, x);
+                    tmem_wait_ld();
+                    if (tail) {
+                        const uint32_t bits = seen(h);
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
+                        for (int i = 0; i < 32; i++) x[i] = bits >> i & 1 ? x[i] : -INFINITY;
+                    }
+                    // P takes the place of these 32 scores: 16 columns of hi, 16 of lo
                     uint32_t hi[16], lo[16];
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        const float2 t = __ffma2_rn({x[h][2 * i], x[h][2 * i + 1]}, c2, off2);
+                        const float2 t = __ffma2_rn({x[2 * i], x[2 * i + 1]}, c2, off2);
                         const float2 p = __fmul2_rn({ex2(t.x), ex2(t.y)}, up2);
                         sum[i & 1] = __fadd2_rn(sum[i & 1], p);
                         hi[i] = pack_half(p.x, p.y);
                         const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[i]));
-                        lo[i] = pack_half(p.x - f.x, p.y - f.y);
+                        const float2 d = __fadd2_rn(p, {-f.x, -f.y});
+                        lo[i] = pack_half(d.x, d.y);
                     }
-                    tmem_st16(p_cols + 16 * h, hi);
-                    tmem_st16(p_cols + kKeys / 2 + 16 * h, lo);
+                    tmem_st16(cols + 32 * h, hi);
+                    tmem_st16(cols + 32 * h + 16, lo);
+                    const int first = 32 * h, end = past + a.tokens;  // first key of the unit that holds no value
+                    if (tail && first + 32 > past && first < end) {
+                        // Values past the last position become 0; those of nodes 0 where they are not finite.
+                        const uint32_t idx = ring0 + v_index(j, it.count) * NC + first / VK, st = idx % NS;
+                        ok = wait_warp(&s.full[st], (idx / NS) & 1, abort, a.err);
+                        if (!ok) break;
+                        unsigned char *v0 = ring + st * kStage + first % VK * 128;
+                        uint64_t odd = 0;
+#pragma unroll 1
+                        for (int u = row; u < 32 * 8 * NC; u += 128) {
+                            const int key = first + ((u >> 3) & 31);
+                            if (key < past) continue;
+                            uint4 *p = reinterpret_cast<uint4 *>(v0 + (u >> 8) * VK * 128 + (u & 255) * 16);
+                            uint4 v = key < end ? *p : make_uint4(0, 0, 0, 0);
+                            uint32_t *wd = &v.x;
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                if ((wd[e] & 0x7c00u) == 0x7c00u) wd[e] &= 0xffff0000u, odd |= 1ull << (key - past);
+                                if ((wd[e] & 0x7c000000u) == 0x7c000000u) wd[e] &= 0x0000ffffu, odd |= 1ull << (key - past);
+                            }
+                            *p = v;
+                        }
+                        if (odd) atomicOr(reinterpret_cast<unsigned long long *>(&s.odd_nodes), (unsigned long long)odd);
+                        fence_proxy_async();
+                    }
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive(&s.p_full[buf][h]);
                 }
                 // the running total, with what its rounding lost
                 const float add = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
@@ -484,33 +578,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 const float y = add - l_low * keep, next = l + y;
                 l_low = (next - l) - y;
                 l = next;
-                if (tail) {
-                    // Values past the last position become 0; those of nodes 0 where they are not finite.
-                    const uint32_t idx = ring0 + v_index(j, it.count), st = idx % C::kStages;
-                    ok = wait_warp(&s.full[st], (idx / C::kStages) & 1, abort, a.err);
-                    if (!ok) break;
-                    const int end = past + a.tokens;  // first row of the unit that holds no value
-                    uint64_t odd = 0;
-                    for (int u = row; u < kKeys * C::kChunks * 8; u += 128) {
-                        const int key = (u >> 3) & (kKeys - 1);
-                        if (key < past) continue;
-                        uint4 *p = reinterpret_cast<uint4 *>(ring + st * C::kStage) + u;
-                        uint4 v = key < end ? *p : make_uint4(0, 0, 0, 0);
-                        uint32_t *wd = &v.x;
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            if ((wd[e] & 0x7c00u) == 0x7c00u) wd[e] &= 0xffff0000u, odd |= 1ull << (key - past);
-                            if ((wd[e] & 0x7c000000u) == 0x7c000000u) wd[e] &= 0x0000ffffu, odd |= 1ull << (key - past);
-                        }
-                        *p = v;
-                    }
-                    if (odd) atomicOr(reinterpret_cast<unsigned long long *>(&s.odd_nodes), (unsigned long long)odd);
-                    fence_proxy_async();
-                }
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) arrive(&s.p_full[buf]);
             }
             // the item's totals
             const uint32_t slot = msg & 1;
@@ -527,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             __syncwarp();
             if (lane == 0) arrive(&s.v_full[slot]);
             msg++;
-            ring0 += 2 * it.count;
+            ring0 += ring_pieces<D>(a, it);
             item++;
             group_sync(2, 128);  // odd_nodes is empty again
         }
@@ -540,27 +607,37 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         uint32_t tile = 0, msg = 0;
         bool ok = true;
         while (ok && walk.next(a, it)) {
-            // ---- Q of this item: warp w prepares rows 16w .. 16w+15, lane l values V*l .. V*l+V-1
-            bool bad = false;
+            // Warp w prepares, and at the end stores, rows w, w+8, ...; lane i < 16 knows where row w+8i lies in q and
+            // out. Rows past the last are left as they are: no one reads their results.
+            const int rows = min(kRows, a.tokens * a.group - it.tile * kRows);
+            size_t where = 0;
             {
-                float x[16][V];
+                const int r = it.tile * kRows + w + 8 * (lane & 15), node = r / a.group;
+                if (node < a.tokens)
+                    where = (((size_t)it.seq * a.tokens + node) * a.q_heads + it.kv * a.group + (r - node * a.group)) * D;
+            }
+            // pages of the item, checked
+            bool bad = false;
+            const int last = min((it.first + it.count) * kKeys, it.length + a.tokens) - 1;
+#pragma unroll 1
+            for (int p = ((it.first * kKeys) >> a.c.shift) + (tid - 256); p <= last >> a.c.shift; p += 256)
+                bad |= (unsigned)a.c.table[(size_t)it.seq * a.c.table_pages + p] >= (unsigned)a.c.pages;
+#pragma unroll 1
+            for (int i0 = 0; w + 8 * i0 < rows; i0 += 8) {  // lane l holds values V*l .. V*l+V-1 of eight rows
+                float x[8][V];
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int r = it.tile * kRows + w * 16 + i, node = r / a.group;
-                    const float *src = a.q + (((size_t)it.seq * a.tokens + node) * a.q_heads + it.kv * a.group + r % a.group) * D + lane * V;
+                for (int i = 0; i < 8; i++) {
+                    const float *src = a.q + __shfl_sync(0xffffffffu, where, i0 + i) + lane * V;
+                    if constexpr (V == 2) {
+                        *reinterpret_cast<float2 *>(x[i]) = __ldg(reinterpret_cast<const float2 *>(src));
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < V; e += 2) {
-                        const float2 f = node < a.tokens ? *reinterpret_cast<const float2 *>(src + e) : make_float2(0.0f, 0.0f);
-                        x[i][e] = f.x, x[i][e + 1] = f.y;
+                        for (int e = 0; e < V; e += 4) *reinterpret_cast<float4 *>(x[i] + e) = __ldg(reinterpret_cast<const float4 *>(src + e));
                     }
                 }
-                // pages of the item, checked meanwhile
-                const int last = min((it.first + it.count) * kKeys, it.length + a.tokens) - 1;
-                for (int p = ((it.first * kKeys) >> a.c.shift) + (tid - 256); p <= last >> a.c.shift; p += 256)
-                    bad |= (unsigned)a.c.table[(size_t)it.seq * a.c.table_pages + p] >= (unsigned)a.c.pages;
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int r = w * 16 + i;
+                for (int i = 0; i < 8; i++) {
+                    const int r = w + 8 * (i0 + i);
                     float mx = 0.0f;
 #pragma unroll
                     for (int e = 0; e < V; e++) mx = fmaxf(mx, fabsf(x[i][e]));
@@ -580,19 +657,25 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     }
                     const int at = lane * V, unit = (at % 64) / 8;
                     unsigned char *dst = q_smem + (at / 64) * kRows * 128 + r * 128 + ((unit ^ (r & 7)) << 4) + (at % 8) * 2;
-#pragma unroll
-                    for (int e = 0; e < V / 2; e++) {
-                        reinterpret_cast<uint32_t *>(dst)[e] = hi[e];
-                        reinterpret_cast<uint32_t *>(dst + C::kPlane)[e] = lo[e];
+                    if constexpr (V == 8) {
+                        *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4 *>(dst + C::kPlane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    } else if constexpr (V == 4) {
+                        *reinterpret_cast<uint2 *>(dst) = make_uint2(hi[0], hi[1]);
+                        *reinterpret_cast<uint2 *>(dst + C::kPlane) = make_uint2(lo[0], lo[1]);
+                    } else {
+                        *reinterpret_cast<uint32_t *>(dst) = hi[0];
+                        *reinterpret_cast<uint32_t *>(dst + C::kPlane) = lo[0];
                     }
                 }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) arrive(&s.q_full);
             }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) arrive(&s.q_full);
             float2 acc[H / 2];
 #pragma unroll
             for (int i = 0; i < H / 2; i++) acc[i] = make_float2(0.0f, 0.0f);
+#pragma unroll 1
             for (int j = 0; ok && j < it.count; j++, tile++, msg++) {
                 const uint32_t slot = msg & 1;
                 ok = wait_warp(&s.v_full[slot], (msg / 2) & 1, abort, a.err);
@@ -618,42 +701,52 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             }
             const uint32_t slot = msg & 1;
             if (ok) ok = wait_warp(&s.v_full[slot], (msg / 2) & 1, abort, a.err);
-            ok = !group_any(3, 256, !ok);  // the eight warps stop together
+            bad = group_any(3, 256, bad);
+            ok = !group_any(4, 256, !ok);  // the eight warps stop together
             if (!ok) break;
             const float total = s.val[slot][row];
             uint64_t odd = s.odd_msg[slot];
             __syncwarp();
             if (lane == 0) arrive(&s.v_empty[slot]);
             msg++;
-            bad = group_any(4, 256, bad);
-            const int r = it.tile * kRows + row, node = r / a.group;
-            if (node < a.tokens) {
-                if (odd) {  // rare: values that are not finite, for the rows that see them
-                    odd &= a.tree ? a.tree[(size_t)it.seq * a.tokens + node] : ~0ull >> (63 - node);
-                    while (odd) {
-                        const int nd = __ffsll((long long)odd) - 1;
-                        odd &= odd - 1;
-                        const long long at = a.c.row(it.seq, it.length + nd);
-                        if (at < 0) continue;
-                        const __half *v = a.c.v + ((size_t)at * a.c.kv_heads + it.kv) * D + col0;
-    #pragma unroll
-                        for (int i = 0; i < H / 2; i++) {
-                            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(v + 2 * i));
-                            if (!(fabsf(f.x) < INFINITY)) acc[i].x += f.x;
-                            if (!(fabsf(f.y) < INFINITY)) acc[i].y += f.y;
-                        }
+            // The rows go through Q's place, 16-byte units turned by the row's low bits, so that whole rows are stored.
+            const bool whole = it.count == it.units;
+            float mul = whole ? (total == 0.0f ? 0.0f : 1.0f / total) : 1.0f;
+            if (bad) mul = __int_as_float(0x7fc00000);
+            unsigned char *mine = q_smem + (size_t)row * D * 4;
+#pragma unroll
+            for (int i = 0; i < H / 4; i++)
+                *reinterpret_cast<float4 *>(mine + (((col0 / 4 + i) ^ (row & 7)) << 4)) =
+                    make_float4(acc[2 * i].x * mul, acc[2 * i].y * mul, acc[2 * i + 1].x * mul, acc[2 * i + 1].y * mul);
+            if (odd && row < rows) {  // rare: values that are not finite, for the rows that see them
+                const int node = (it.tile * kRows + row) / a.group;
+                odd &= a.tree ? a.tree[(size_t)it.seq * a.tokens + node] : ~0ull >> (63 - node);
+                while (odd) {
+                    const int nd = __ffsll((long long)odd) - 1;
+                    odd &= odd - 1;
+                    const long long at = a.c.row(it.seq, it.length + nd);
+                    if (at < 0) continue;
+                    const __half *v = a.c.v + ((size_t)at * a.c.kv_heads + it.kv) * D + col0;
+#pragma unroll 1
+                    for (int i = 0; i < H; i++) {
+                        const float f = __half2float(v[i]);
+                        if (!(fabsf(f) < INFINITY))
+                            *reinterpret_cast<float *>(mine + (((col0 + i) / 4 ^ (row & 7)) << 4) + (i & 3) * 4) += f;
                     }
                 }
-                const bool whole = it.count == it.units;
-                float mul = whole ? (total == 0.0f ? 0.0f : 1.0f / total) : 1.0f;
-                if (bad) mul = __int_as_float(0x7fc00000);
-                float *dst = whole ? a.out + (((size_t)it.seq * a.tokens + node) * a.q_heads + it.kv * a.group + r % a.group) * D + col0
-                                   : a.part_acc + ((size_t)(2 * blockIdx.x + (it.start > s.unit0)) * a.part_rows + row) * D + col0;
-    #pragma unroll
-                for (int i = 0; i < H / 4; i++)
-                    reinterpret_cast<float4 *>(dst)[i] =
-                        make_float4(acc[2 * i].x * mul, acc[2 * i].y * mul, acc[2 * i + 1].x * mul, acc[2 * i + 1].y * mul);
             }
+            group_sync(3, 256);
+            const size_t part = (size_t)(2 * blockIdx.x + (it.start > s.unit0)) * a.part_rows;
+#pragma unroll 4
+            for (int i = 0; w + 8 * i < rows; i++) {
+                const int r = w + 8 * i;
+                const size_t at = __shfl_sync(0xffffffffu, where, i);
+                float *dst = whole ? a.out + at : a.part_acc + (part + r) * D;
+#pragma unroll
+                for (int u = lane; u < D / 4; u += 32)
+                    reinterpret_cast<float4 *>(dst)[u] = *reinterpret_cast<const float4 *>(q_smem + (size_t)r * D * 4 + ((u ^ (r & 7)) << 4));
+            }
+            group_sync(4, 256);  // Q's place is free again
         }
     }
     __syncthreads();
@@ -663,43 +756,68 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     }
 }
 
-// Joins the parts of items that several CTAs share, one warp per (row, head);
-// refused sequences, and every row after an error, become NaN.
+// Joins the parts of items that several CTAs share; refused sequences, and
+// every row after an error, become NaN. One warp per (row, head, 128 columns):
+// lanes look up a part's place, maximum and total each, then the warp adds the
+// parts' columns in order, several loads in flight.
 template <int D>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttendArgs a, int ctas) {
-    constexpr int V = D / 32;
+    constexpr int V = D == 64 ? 2 : 4, kBlocks = D / (32 * V);
     const int lane = threadIdx.x & 31;
-    const int id = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int job = blockIdx.x * 8 + (threadIdx.x >> 5), id = job / kBlocks;
     if (id >= a.seqs * a.tokens * a.q_heads) return;
     const int h = id % a.q_heads, row = id / a.q_heads, seq = row / a.tokens;
     const int kv = h / a.group, r = (row % a.tokens) * a.group + h % a.group, tile = r / kRows;
-    const int per = a.c.kv_heads * a.row_tiles;
+    const int per = a.c.kv_heads * a.row_tiles, col = (job % kBlocks) * 32 * V + lane * V;
     const long long w = sum_units(a, a.seqs, per);
-    const int units = units_of(a, seq);
-    const long long start = sum_units(a, seq, per) + (long long)(kv * a.row_tiles + tile) * units;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    float *out = a.out + (size_t)id * D + lane * V;
-    if (units == 0 || *(volatile int *)a.err) {
-        for (int e = 0; e < V; e++) out[e] = __int_as_float(0x7fc00000);
-        return;
-    }
+    const int units = units_of(a, a.c.committed(seq, a.tokens));
+    const long long start = (seq ? sum_units(a, seq, per) : 0) + (long long)(kv * a.row_tiles + tile) * units;
+    float *out = a.out + (size_t)id * D + col;
     const int g = (int)min((long long)ctas, w);
-    const int c0 = cta_of(start, w, g), c1 = cta_of(start + units - 1, w, g);
-    if (c0 == c1) return;
-    float m = -INFINITY, l = 0.0f, acc[V];
-    for (int e = 0; e < V; e++) acc[e] = 0.0f;
-    for (int c = c0; c <= c1; c++) m = fmaxf(m, __ldcg(&a.part_ml[(size_t)(2 * c + (start > range_start(c, w, g))) * a.part_rows + r % kRows].x));
-    for (int c = c0; c <= c1; c++) {
-        const size_t at = (size_t)(2 * c + (start > range_start(c, w, g))) * a.part_rows + r % kRows;
-        const float2 ml = __ldcg(a.part_ml + at);
-        const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - m);
-        l += f == 0.0f && ml.y == 0.0f ? 0.0f : f * ml.y;
-        const float *p = a.part_acc + at * D + lane * V;
+    const int c0 = units ? cta_of(start, w, g) : 0, parts = units ? cta_of(start + units - 1, w, g) - c0 + 1 : 0;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    float acc[V], m = -INFINITY, l = 0.0f;
 #pragma unroll
-        for (int e = 0; e < V; e++) acc[e] = fmaf(f, __ldcg(p + e), acc[e]);
+    for (int e = 0; e < V; e++) acc[e] = 0.0f;
+    if (parts == 0 || *(volatile int *)a.err) {
+        l = __int_as_float(0x7fc00000);
+    } else if (parts == 1) {
+        return;
+    } else {
+        for (int p = lane; p < parts; p += 32)
+            m = fmaxf(m, __ldcg(&a.part_ml[(size_t)(2 * (c0 + p) + (start > range_start(c0 + p, w, g))) * a.part_rows + r % kRows].x));
+#pragma unroll
+        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+        for (int p0 = 0; p0 < parts; p0 += 32) {
+            int at = 0;
+            float f = 0.0f;
+            if (p0 + lane < parts) {
+                const int c = c0 + p0 + lane;
+                at = (2 * c + (start > range_start(c, w, g))) * a.part_rows + r % kRows;
+                const float2 ml = __ldcg(a.part_ml + at);
+                f = ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : ml.y) : ex2(ml.x - m);
+                l += f * ml.y;
+            }
+            const int n = min(32, parts - p0);
+#pragma unroll 8
+            for (int i = 0; i < n; i++) {
+                const float fi = __shfl_sync(0xffffffffu, f, i);
+                const float *p = a.part_acc + (size_t)__shfl_sync(0xffffffffu, at, i) * D + col;
+                float x[V];
+                if constexpr (V == 4) *reinterpret_cast<float4 *>(x) = __ldcg(reinterpret_cast<const float4 *>(p));
+                else *reinterpret_cast<float2 *>(x) = __ldcg(reinterpret_cast<const float2 *>(p));
+#pragma unroll
+                for (int e = 0; e < V; e++) acc[e] = fmaf(fi, x[e], acc[e]);
+            }
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    for (int e = 0; e < V; e++) out[e] = acc[e] * inv;
+#pragma unroll
+    for (int e = 0; e < V; e++) acc[e] *= inv;
+    if constexpr (V == 4) *reinterpret_cast<float4 *>(out) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    else *reinterpret_cast<float2 *>(out) = make_float2(acc[0], acc[1]);
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
@@ -739,7 +857,7 @@ int launch(const AttendArgs &a, const CUtensorMap &k_map, const CUtensorMap &v_m
     tree_attention_kernel<D><<<ctas, kThreads, Cfg<D>::kSmem, launch_stream>>>(a, k_map, v_map);
     if (int rc = cudaGetLastError()) return rc;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((a.seqs * a.tokens * a.q_heads + 7) / 8));
+    cfg.gridDim = dim3((unsigned)(((size_t)a.seqs * a.tokens * a.q_heads * (D / (D == 64 ? 64 : 128)) + 7) / 8));
     cfg.blockDim = dim3(256);
     cfg.stream = launch_stream;
     cudaLaunchAttribute pdl[1];
@@ -780,13 +898,15 @@ extern "C" int qg_tree_attention(float *out, const float *q, const qg_kv_cache *
     a.group = q_heads / a.c.kv_heads;
     a.row_tiles = (tokens * a.group + kRows - 1) / kRows;
     a.part_rows = part_rows(tokens, a.group);
-    a.box = a.c.page_tokens() < kKeys ? a.c.page_tokens() : kKeys;
+    a.k_box = a.c.page_tokens() < kKeys ? a.c.page_tokens() : kKeys;
+    const int v_keys = kStage / (2 * a.c.head_dim);
+    a.v_box = a.c.page_tokens() < v_keys ? a.c.page_tokens() : v_keys;
     a.err = static_cast<int *>(workspace);
     a.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + 256);
     a.part_acc = reinterpret_cast<float *>(static_cast<char *>(workspace) + 256 + ml_bytes(a.part_rows));
     CUtensorMap k_map, v_map;
-    if (int rc = pool_map(&k_map, a.c, a.c.k, a.box)) return rc;
-    if (int rc = pool_map(&v_map, a.c, a.c.v, a.box)) return rc;
+    if (int rc = pool_map(&k_map, a.c, a.c.k, a.k_box)) return rc;
+    if (int rc = pool_map(&v_map, a.c, a.c.v, a.v_box)) return rc;
     if (a.c.head_dim == 64) return launch<64>(a, k_map, v_map);
     if (a.c.head_dim == 128) return launch<128>(a, k_map, v_map);
     return launch<256>(a, k_map, v_map);
