@@ -50,7 +50,7 @@ struct AttendArgs {
     const uint64_t *tree;
     float scale;  // |scale| * log2(e)
     float sign;   // of scale, folded into Q
-    int seqs, tokens, q_heads, group, row_tiles, part_rows;
+    int seqs, tokens, q_heads, group, row_tiles, part_rows, copies;
     int k_box, v_box;  // rows of one TMA box: a page, at most a piece's keys
     int *err;
     float *part_acc;   // [2 * kMaxCtas][part_rows][D]
@@ -60,25 +60,25 @@ struct AttendArgs {
 constexpr int kStage = 16384;    // one piece of the ring
 constexpr int kChunk = 32;       // keys per step of the softmax
 
-template <int D>
+template <int D, int MR>
 struct Cfg {
-    static constexpr int kChunks = D / 64;                // 128-byte wide column blocks
-    static constexpr int kPlane = kChunks * kRows * 128;  // one plane of Q
+    static constexpr int kChunks = D / 64;                  // 128-byte wide column blocks
+    static constexpr int kBlock = MR * 128;                 // one of them, of one plane of Q
+    static constexpr int kPlane = kChunks * kBlock;
     // The ring's pieces: 64 columns of 128 keys, or all columns of kVKeys values; kChunks pieces for a unit's keys or values.
     static constexpr int kVKeys = kStage / (2 * D);
-    static constexpr int kStages = D == 256 ? 6 : 8;
+    static constexpr int kStages = D == 256 ? (MR == 64 ? 10 : 6) : 8;
     static constexpr int kSmem = 2 * kPlane + kStages * kStage + 2048 + 1024;
     static constexpr int kS = 256;  // tensor memory columns: O, then two of S (P takes its place)
 };
 
 struct Shared {
     float val[2][kRows];    // rescaling factors, and at an item's end the totals: softmax -> accumulators
-    float q_scale[kRows];
-    uint64_t full[8], empty[8], s_full[2], p_full[2][kKeys / kChunk], pv_done[2], v_full[2], v_empty[2], o_full, o_empty, q_full, drain;
-    uint64_t odd_nodes;     // nodes whose values are not finite: softmax warps only
-    uint64_t odd_msg[2];    // the same, posted with an item's totals
-    long long unit0, unit1, base;
-    int seq0, length0;
+    float q_scale[kRows];   // at an item's end the maxima
+    uint64_t full[10], empty[10], s_full[2], p_full[2][kKeys / kChunk], pv_done[2], v_full[2], v_empty[2], o_full, o_empty, q_full, clean, drain;
+    uint64_t odd_nodes;     // nodes whose values are not finite
+    long long unit0, unit1;
+    int seq0, length0, kv0, tile0, first0;
     uint32_t tmem;
     int abort;
 };
@@ -198,13 +198,13 @@ __device__ long long sum_units(const AttendArgs &a, int seqs, int per) {
     for (int s = threadIdx.x & 31; s < seqs; s += 32) sum += (long long)units_of(a, a.c.committed(s, a.tokens)) * per;
     return warp_sum(sum);
 }
-// One warp: the sequence that holds unit `at`, its length and the units before it.
-__device__ int find_unit(const AttendArgs &a, int per, long long at, long long &base, int &length) {
+// One warp: the sequence that holds unit `at`, its length and the units before it. `len`: the lane's own sequence
+// among the first 32.
+__device__ int find_unit(const AttendArgs &a, int per, long long at, int len, long long &base, int &length) {
     const int lane = threadIdx.x & 31;
     base = 0;
     for (int s0 = 0; s0 < a.seqs; s0 += 32) {
-        const int s = s0 + lane;
-        const int len = s < a.seqs ? a.c.committed(s, a.tokens) : -1;
+        if (s0) len = s0 + lane < a.seqs ? a.c.committed(s0 + lane, a.tokens) : -1;
         const long long mine = (long long)units_of(a, len) * per;
         long long upto = mine;
 #pragma unroll
@@ -237,27 +237,27 @@ struct Item {
     long long start;  // the item's first unit
 };
 struct Walk {
-    long long at, end, base;
-    int seq, length;
-    __device__ Walk(const Shared &s) : at(s.unit0), end(s.unit1), base(s.base), seq(s.seq0), length(s.length0) {}
+    long long at, end;
+    int seq, length, kv, tile, first;
+    __device__ Walk(const Shared &s)
+        : at(s.unit0), end(s.unit1), seq(s.seq0), length(s.length0), kv(s.kv0), tile(s.tile0), first(s.first0) {}
     __device__ bool next(const AttendArgs &a, Item &it) {
         if (at >= end) return false;
-        const int per = a.c.kv_heads * a.row_tiles;
-        while (at >= base + (long long)units_of(a, length) * per) {
-            base += (long long)units_of(a, length) * per;
-            length = a.c.committed(++seq, a.tokens);
-        }
+        it.seq = seq, it.kv = kv, it.tile = tile, it.first = first, it.length = length;
         it.units = units_of(a, length);
-        const long long in = at - base;
-        const int index = (int)quotient(in, it.units);
-        it.seq = seq;
-        it.kv = index / a.row_tiles;
-        it.tile = index % a.row_tiles;
-        it.first = (int)(in - (long long)index * it.units);
-        it.count = (int)min((long long)(it.units - it.first), end - at);
-        it.length = length;
-        it.start = at - it.first;
+        it.count = (int)min((long long)(it.units - first), end - at);
+        it.start = at - first;
         at += it.count;
+        first = 0;  // the item after it, should there be one
+        if (++tile == a.row_tiles) {
+            tile = 0;
+            if (++kv == a.c.kv_heads) {
+                kv = 0;
+                do
+                    if (++seq < a.seqs) length = a.c.committed(seq, a.tokens);
+                while (seq < a.seqs && length < 0);
+            }
+        }
         return true;
     }
 };
@@ -270,16 +270,16 @@ __device__ __forceinline__ uint32_t v_index(int j, int n) { return j == n - 1 ? 
 __device__ __forceinline__ int keys_of(const AttendArgs &a, const Item &it, int j) {
     return min(kKeys, it.length + a.tokens - (it.first + j) * kKeys);
 }
-template <int D>
+template <class C>
 __device__ __forceinline__ uint32_t ring_pieces(const AttendArgs &a, const Item &it) {
-    return (2 * it.count - 1) * Cfg<D>::kChunks + (keys_of(a, it, it.count - 1) + Cfg<D>::kVKeys - 1) / Cfg<D>::kVKeys;
+    return (2 * it.count - 1) * C::kChunks + (keys_of(a, it, it.count - 1) + C::kVKeys - 1) / C::kVKeys;
 }
 
-template <int D>
+template <int D, int MR>
 __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __grid_constant__ AttendArgs a,
                                                                      const __grid_constant__ CUtensorMap k_map,
                                                                      const __grid_constant__ CUtensorMap v_map) {
-    using C = Cfg<D>;
+    using C = Cfg<D, MR>;
     constexpr int NC = C::kChunks, NS = C::kStages, VK = C::kVKeys;
     extern __shared__ unsigned char raw[];
     unsigned char *smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
@@ -290,17 +290,23 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
 
     if (warp == 0) {
         const int per = a.c.kv_heads * a.row_tiles;
-        const long long w = sum_units(a, a.seqs, per);
+        const int len = lane < a.seqs ? a.c.committed(lane, a.tokens) : -1;
+        long long w = (long long)units_of(a, len) * per;
+        for (int q = lane + 32; q < a.seqs; q += 32) w += (long long)units_of(a, a.c.committed(q, a.tokens)) * per;
+        w = warp_sum(w);
         const int g = (int)min((long long)gridDim.x, w);
         long long base = 0, u0 = 0, u1 = 0;
         int seq = 0, length = -1;
         if ((int)blockIdx.x < g) {
             u0 = range_start(blockIdx.x, w, g);
             u1 = range_start(blockIdx.x + 1, w, g);
-            seq = find_unit(a, per, u0, base, length);
+            seq = find_unit(a, per, u0, len, base, length);
         }
         if (lane == 0) {
-            s.unit0 = u0, s.unit1 = u1, s.base = base, s.seq0 = seq, s.length0 = length;
+            const int units = max(1, units_of(a, length)), index = (int)quotient(u0 - base, units);
+            s.unit0 = u0, s.unit1 = u1, s.seq0 = seq, s.length0 = length;
+            s.kv0 = index / a.row_tiles, s.tile0 = index % a.row_tiles;
+            s.first0 = (int)(u0 - base - (long long)index * units);
         }
     } else if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s.tmem)));
@@ -315,6 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             for (int k = 0; k < kKeys / kChunk; k++) mbar_init(&s.p_full[i][k], 4);
         }
         mbar_init(&s.o_full, 1), mbar_init(&s.o_empty, 8), mbar_init(&s.q_full, 8), mbar_init(&s.drain, 2);
+        mbar_init(&s.clean, 8);
         fence_mbar_init();
     } else if (warp == 3 && lane == 0) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map));
@@ -401,22 +408,22 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                         const uint64_t kd = operand(smem_u32(ring + st * kStage), 16);
 #pragma unroll
                         for (int k = 0; k < 4; k++)
-                            mma_ss(d, q_lo + c * (kRows * 128 / 16) + 2 * k, kd + 2 * k, idesc(kKeys, false), c + k > 0);
+                            mma_ss(d, q_lo + c * (C::kBlock / 16) + 2 * k, kd + 2 * k, idesc(kKeys, false), c + k > 0);
 #pragma unroll
                         for (int k = 0; k < 4; k++)
-                            mma_ss(d, q_hi + c * (kRows * 128 / 16) + 2 * k, kd + 2 * k, idesc(kKeys, false), true);
+                            mma_ss(d, q_hi + c * (C::kBlock / 16) + 2 * k, kd + 2 * k, idesc(kKeys, false), true);
                         commit(&s.empty[st]);
                     }
                     if (ok) commit(&s.s_full[buf]);
                 }
-                ring0 += ring_pieces<D>(a, it);
+                ring0 += ring_pieces<C>(a, it);
                 item++;
             }
             commit(&s.drain);
             wait_drain(&s.drain, 0);
         } else if (warp == 2 && lane == 0) {
             // ------------------------------------------------ O = P V
-            uint32_t ring0 = 0, tile = 0;
+            uint32_t ring0 = 0, tile = 0, tails = 0;
             bool ok = true;
             while (ok && walk.next(a, it)) {
                 for (int j = 0; ok && j < it.count; j++, tile++) {
@@ -424,6 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     const int keys = keys_of(a, it, j);
                     uint32_t idx = ring0 + v_index(j, it.count) * NC;
                     if (tile >= 1) ok = wait(&s.o_empty, (tile - 1) & 1, abort, a.err);
+                    if (ok && it.length < (it.first + j + 1) * kKeys) ok = wait(&s.clean, tails++ & 1, abort, a.err);
                     // 32 keys at a time, as the softmax delivers them; past the last key there is nothing
 #pragma unroll 1
                     for (int h = 0; ok && h * kChunk < keys; h++) {
@@ -447,20 +455,24 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     commit(&s.pv_done[buf]);
                     commit(&s.o_full);
                 }
-                ring0 += ring_pieces<D>(a, it);
+                ring0 += ring_pieces<C>(a, it);
             }
             commit(&s.drain);
             wait_drain(&s.drain, 0);
         }
     } else if (warp < 8) {
         // ---------------------------------------------------- softmax: one thread per row
+        // With few rows (a.copies 2 or 4) Q lies in the tile several times, and each copy takes its share of a unit's
+        // keys: a running maximum and total of its own, P = 0 for the others' keys, joined at the end of the item.
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-        const int row = tid - 128;
+        const int row = tid - 128, span = kRows / a.copies, copy = row / span, chunks = kKeys / kChunk / a.copies;
+        const int h0 = copy * chunks, h1 = h0 + chunks;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // tensor memory lane of the warp's first row, in bits 16+
-        uint32_t ring0 = 0, tile = 0, item = 0, msg = 0;
+        uint32_t tile = 0, item = 0, msg = 0;
         bool ok = true;
         while (ok && walk.next(a, it)) {
-            const int node = (it.tile * kRows + row) / a.group;
+            const int r = it.tile * kRows + row % span, node = r / a.group;
+            const bool live = (row & ~31) % span + it.tile * kRows < a.tokens * a.group;  // the warp has rows
             uint64_t mask = 0;
             if (node < a.tokens) {
                 mask = a.tree ? a.tree[(size_t)it.seq * a.tokens + node] : ~0ull >> (63 - node);
@@ -483,31 +495,27 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 ok = wait_warp(&s.s_full[buf], (tile / 2) & 1, abort, a.err);
                 if (!ok) break;
                 tc_fence_after();
-                float top[2] = {-INFINITY, -INFINITY};
+                float keep = 0.0f, off = 0.0f;
+                if (live) {
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
-                for (int h = 0; h < kKeys / kChunk; h += 2) {
-                    float x[2][32];
-                    tmem_ld32(cols + 32 * h, x[0]);
-                    tmem_ld32(cols + 32 * h + 32, x[1]);
-                    tmem_wait_ld();
-                    if (tail) {
+                    for (int h = h0; h < h1; h++) {
+                        float x[32];
+                        tmem_ld32(cols + 32 * h, x);
+                        tmem_wait_ld();
+                        if (tail) {
+                            const uint32_t bits = seen(h);
 #pragma unroll
-                        for (int g = 0; g < 2; g++) {
-                            const uint32_t bits = seen(h + g);
-#pragma unroll
-                            for (int i = 0; i < 32; i++) x[g][i] = bits >> i & 1 ? x[g][i] : -INFINITY;
+                            for (int i = 0; i < 32; i++) x[i] = bits >> i & 1 ? x[i] : -INFINITY;
                         }
-                    }
 #pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        top[0] = fmaxf(top[0], x[0][i]);
-                        top[1] = fmaxf(top[1], x[1][i]);
+                        for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], x[i]);
                     }
+                    const float m_new = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c);
+                    keep = m == -INFINITY ? 0.0f : ex2(m - m_new);
+                    off = m_new == -INFINITY ? 0.0f : m_new;
+                    m = m_new;
                 }
-                const float m_new = fmaxf(m, fmaxf(top[0], top[1]) * c);
-                const float keep = m == -INFINITY ? 0.0f : ex2(m - m_new);
-                const float off = m_new == -INFINITY ? 0.0f : m_new;
-                m = m_new;
                 // the factor goes to the accumulators
                 const uint32_t slot = msg & 1;
                 if (msg >= 2) ok = wait_warp(&s.v_empty[slot], (msg / 2 - 1) & 1, abort, a.err);
@@ -519,55 +527,40 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 float2 sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
                 const float2 c2 = {c, c}, off2 = {-off, -off}, up2 = {kPScale, kPScale};
 #pragma unroll 1
-                for (int h = 0; ok && h < kKeys / kChunk; h++) {
-                    float x[32];
-                    tmem_ld32(cols + 32 * h, x);
-                    tmem_wait_ld();
-                    if (tail) {
-                        const uint32_t bits = seen(h);
-#pragma unroll
-                        for (int i = 0; i < 32; i++) x[i] = bits >> i & 1 ? x[i] : -INFINITY;
-                    }
-                    // P takes the place of these 32 scores: 16 columns of hi, 16 of lo
+                for (int h = 0; h < kKeys / kChunk; h++) {
+                    // P takes the place of 32 scores: 16 columns of hi, 16 of lo
                     uint32_t hi[16], lo[16];
+                    if (h >= h0 && h < h1) {
+                        if (live) {
+                            float x[32];
+                            tmem_ld32(cols + 32 * h, x);
+                            tmem_wait_ld();
+                            if (tail) {
+                                const uint32_t bits = seen(h);
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const float2 t = __ffma2_rn({x[2 * i], x[2 * i + 1]}, c2, off2);
-                        const float2 p = __fmul2_rn({ex2(t.x), ex2(t.y)}, up2);
-                        sum[i & 1] = __fadd2_rn(sum[i & 1], p);
-                        hi[i] = pack_half(p.x, p.y);
-                        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[i]));
-                        const float2 d = __fadd2_rn(p, {-f.x, -f.y});
-                        lo[i] = pack_half(d.x, d.y);
-                    }
-                    tmem_st16(cols + 32 * h, hi);
-                    tmem_st16(cols + 32 * h + 16, lo);
-                    const int first = 32 * h, end = past + a.tokens;  // first key of the unit that holds no value
-                    if (tail && first + 32 > past && first < end) {
-                        // Values past the last position become 0; those of nodes 0 where they are not finite.
-                        const uint32_t idx = ring0 + v_index(j, it.count) * NC + first / VK, st = idx % NS;
-                        ok = wait_warp(&s.full[st], (idx / NS) & 1, abort, a.err);
-                        if (!ok) break;
-                        unsigned char *v0 = ring + st * kStage + first % VK * 128;
-                        uint64_t odd = 0;
-#pragma unroll 1
-                        for (int u = row; u < 32 * 8 * NC; u += 128) {
-                            const int key = first + ((u >> 3) & 31);
-                            if (key < past) continue;
-                            uint4 *p = reinterpret_cast<uint4 *>(v0 + (u >> 8) * VK * 128 + (u & 255) * 16);
-                            uint4 v = key < end ? *p : make_uint4(0, 0, 0, 0);
-                            uint32_t *wd = &v.x;
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                if ((wd[e] & 0x7c00u) == 0x7c00u) wd[e] &= 0xffff0000u, odd |= 1ull << (key - past);
-                                if ((wd[e] & 0x7c000000u) == 0x7c000000u) wd[e] &= 0x0000ffffu, odd |= 1ull << (key - past);
+                                for (int i = 0; i < 32; i++) x[i] = bits >> i & 1 ? x[i] : -INFINITY;
                             }
-                            *p = v;
+#pragma unroll
+                            for (int i = 0; i < 16; i++) {
+                                const float2 t = __ffma2_rn({x[2 * i], x[2 * i + 1]}, c2, off2);
+                                const float2 p = __fmul2_rn({ex2(t.x), ex2(t.y)}, up2);
+                                sum[i & 1] = __fadd2_rn(sum[i & 1], p);
+                                hi[i] = pack_half(p.x, p.y);
+                                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[i]));
+                                const float2 d = __fadd2_rn(p, {-f.x, -f.y});
+                                lo[i] = pack_half(d.x, d.y);
+                            }
+                            tmem_st16(cols + 32 * h, hi);
+                            tmem_st16(cols + 32 * h + 16, lo);
+                            tmem_wait_st();
                         }
-                        if (odd) atomicOr(reinterpret_cast<unsigned long long *>(&s.odd_nodes), (unsigned long long)odd);
-                        fence_proxy_async();
+                    } else if (live) {
+#pragma unroll
+                        for (int i = 0; i < 16; i++) hi[i] = 0;
+                        tmem_st16(cols + 32 * h, hi);
+                        tmem_st16(cols + 32 * h + 16, hi);
+                        tmem_wait_st();
                     }
-                    tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) arrive(&s.p_full[buf][h]);
@@ -582,51 +575,39 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             // the item's totals
             const uint32_t slot = msg & 1;
             if (ok && msg >= 2) ok = wait_warp(&s.v_empty[slot], (msg / 2 - 1) & 1, abort, a.err);
-            ok = !group_any(1, 128, !ok);  // the four warps stop together; odd_nodes is complete
+            ok = !group_any(1, 128, !ok);  // the four warps stop together
             if (!ok) break;
             s.val[slot][row] = l;
-            if (row == 0) {
-                s.odd_msg[slot] = s.odd_nodes;
-                s.odd_nodes = 0;
-            }
-            if (it.count != it.units && row < a.part_rows)
-                a.part_ml[(size_t)(2 * blockIdx.x + (it.start > s.unit0)) * a.part_rows + row] = make_float2(m, l);
+            s.q_scale[row] = m;
             __syncwarp();
             if (lane == 0) arrive(&s.v_full[slot]);
             msg++;
-            ring0 += ring_pieces<D>(a, it);
             item++;
-            group_sync(2, 128);  // odd_nodes is empty again
         }
     } else {
         // ---------------------------------------------------- Q, and the accumulators: rows x half of the columns
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsAcc));
         constexpr int H = D / 2, V = D / 32;
-        const int w = warp - 8, row = (warp & 3) * 32 + lane, col0 = (w >> 2) * H;
+        const int w = warp - 8, row = (warp & 3) * 32 + lane, col0 = (w >> 2) * H, span = kRows / a.copies;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
-        uint32_t tile = 0, msg = 0;
+        uint32_t ring0 = 0, tile = 0, msg = 0;
         bool ok = true;
         while (ok && walk.next(a, it)) {
             // Warp w prepares, and at the end stores, rows w, w+8, ...; lane i < 16 knows where row w+8i lies in q and
             // out. Rows past the last are left as they are: no one reads their results.
             const int rows = min(kRows, a.tokens * a.group - it.tile * kRows);
+            const bool live = (row & ~31) % span < rows;  // the warp has rows
             size_t where = 0;
             {
                 const int r = it.tile * kRows + w + 8 * (lane & 15), node = r / a.group;
                 if (node < a.tokens)
                     where = (((size_t)it.seq * a.tokens + node) * a.q_heads + it.kv * a.group + (r - node * a.group)) * D;
             }
-            // pages of the item, checked
-            bool bad = false;
-            const int last = min((it.first + it.count) * kKeys, it.length + a.tokens) - 1;
 #pragma unroll 1
-            for (int p = ((it.first * kKeys) >> a.c.shift) + (tid - 256); p <= last >> a.c.shift; p += 256)
-                bad |= (unsigned)a.c.table[(size_t)it.seq * a.c.table_pages + p] >= (unsigned)a.c.pages;
-#pragma unroll 1
-            for (int i0 = 0; w + 8 * i0 < rows; i0 += 8) {  // lane l holds values V*l .. V*l+V-1 of eight rows
-                float x[8][V];
+            for (int i0 = 0; w + 8 * i0 < rows; i0 += 4) {  // lane l holds values V*l .. V*l+V-1 of four rows
+                float x[4][V];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
+                for (int i = 0; i < 4; i++) {
                     const float *src = a.q + __shfl_sync(0xffffffffu, where, i0 + i) + lane * V;
                     if constexpr (V == 2) {
                         *reinterpret_cast<float2 *>(x[i]) = __ldg(reinterpret_cast<const float2 *>(src));
@@ -636,16 +617,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
+                for (int i = 0; i < 4; i++) {
                     const int r = w + 8 * (i0 + i);
                     float mx = 0.0f;
 #pragma unroll
                     for (int e = 0; e < V; e++) mx = fmaxf(mx, fabsf(x[i][e]));
-#pragma unroll
-                    for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                    // of values that are not negative the bit patterns have the same order
+                    mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
                     float up, inv;
                     pow2_scale(mx, up, inv);
-                    if (lane == 0) s.q_scale[r] = fmaxf(a.scale * inv, 1e-44f);  // never 0: -infinity stays what it is
                     up *= a.sign;
                     uint32_t hi[V / 2], lo[V / 2];
 #pragma unroll
@@ -655,28 +635,70 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                         const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[e]));
                         lo[e] = pack_half(p - f.x, q - f.y);
                     }
+                    if (r >= rows) continue;
                     const int at = lane * V, unit = (at % 64) / 8;
-                    unsigned char *dst = q_smem + (at / 64) * kRows * 128 + r * 128 + ((unit ^ (r & 7)) << 4) + (at % 8) * 2;
-                    if constexpr (V == 8) {
-                        *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        *reinterpret_cast<uint4 *>(dst + C::kPlane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                    } else if constexpr (V == 4) {
-                        *reinterpret_cast<uint2 *>(dst) = make_uint2(hi[0], hi[1]);
-                        *reinterpret_cast<uint2 *>(dst + C::kPlane) = make_uint2(lo[0], lo[1]);
-                    } else {
-                        *reinterpret_cast<uint32_t *>(dst) = hi[0];
-                        *reinterpret_cast<uint32_t *>(dst + C::kPlane) = lo[0];
+                    for (int rr = r; rr < kRows; rr += span) {
+                        if (lane == 0) s.q_scale[rr] = fmaxf(a.scale * inv, 1e-44f);  // never 0: -infinity stays what it is
+                        unsigned char *dst = q_smem + (at / 64) * C::kBlock + rr * 128 + ((unit ^ (rr & 7)) << 4) + (at % 8) * 2;
+                        if constexpr (V == 8) {
+                            *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                            *reinterpret_cast<uint4 *>(dst + C::kPlane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        } else if constexpr (V == 4) {
+                            *reinterpret_cast<uint2 *>(dst) = make_uint2(hi[0], hi[1]);
+                            *reinterpret_cast<uint2 *>(dst + C::kPlane) = make_uint2(lo[0], lo[1]);
+                        } else {
+                            *reinterpret_cast<uint32_t *>(dst) = hi[0];
+                            *reinterpret_cast<uint32_t *>(dst + C::kPlane) = lo[0];
+                        }
                     }
                 }
             }
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) arrive(&s.q_full);
+            // pages of the item, checked
+            bool bad = false;
+            const int last = min((it.first + it.count) * kKeys, it.length + a.tokens) - 1;
+#pragma unroll 1
+            for (int p = ((it.first * kKeys) >> a.c.shift) + (tid - 256); p <= last >> a.c.shift; p += 256)
+                bad |= (unsigned)a.c.table[(size_t)it.seq * a.c.table_pages + p] >= (unsigned)a.c.pages;
             float2 acc[H / 2];
 #pragma unroll
             for (int i = 0; i < H / 2; i++) acc[i] = make_float2(0.0f, 0.0f);
 #pragma unroll 1
             for (int j = 0; ok && j < it.count; j++, tile++, msg++) {
+                const int past = it.length - (it.first + j) * kKeys;  // keys of the unit before the nodes
+                if (past < kKeys) {
+                    // Values past the last position become 0 up to a multiple of 32; those of nodes 0 where they are
+                    // not finite.
+                    const int end = min(kKeys, past + a.tokens), from = max(past, 0);
+                    for (int k0 = from & ~31; ok && k0 < end; k0 += 32) {
+                        const uint32_t idx = ring0 + v_index(j, it.count) * NC + k0 / VK, st = idx % NS;
+                        ok = wait_warp(&s.full[st], (idx / NS) & 1, abort, a.err);
+                        if (!ok) break;
+                        unsigned char *v0 = ring + st * kStage + k0 % VK * 128;
+                        uint64_t odd = 0;
+#pragma unroll 1
+                        for (int u = tid - 256; u < 32 * 8 * NC; u += 256) {
+                            const int key = k0 + ((u >> 3) & 31);
+                            if (key < past) continue;
+                            uint4 *p = reinterpret_cast<uint4 *>(v0 + (u >> 8) * VK * 128 + (u & 255) * 16);
+                            uint4 v = key < end ? *p : make_uint4(0, 0, 0, 0);
+                            uint32_t *wd = &v.x;
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                if ((wd[e] & 0x7c00u) == 0x7c00u) wd[e] &= 0xffff0000u, odd |= 1ull << (key - past);
+                                if ((wd[e] & 0x7c000000u) == 0x7c000000u) wd[e] &= 0x0000ffffu, odd |= 1ull << (key - past);
+                            }
+                            *p = v;
+                        }
+                        if (odd) atomicOr(reinterpret_cast<unsigned long long *>(&s.odd_nodes), (unsigned long long)odd);
+                    }
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) arrive(&s.clean);
+                    if (!ok) break;
+                }
                 const uint32_t slot = msg & 1;
                 ok = wait_warp(&s.v_full[slot], (msg / 2) & 1, abort, a.err);
                 if (!ok) break;
@@ -685,69 +707,99 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 if (lane == 0) arrive(&s.v_empty[slot]);
                 ok = wait_warp(&s.o_full, tile & 1, abort, a.err);
                 if (!ok) break;
-                tc_fence_after();
-                const float2 keep2 = {keep, keep};
+                if (live) {
+                    tc_fence_after();
+                    const float2 keep2 = {keep, keep};
 #pragma unroll
-                for (int b = 0; b < H / 32; b++) {
-                    float x[32];
-                    tmem_ld32(tmem + lanes + col0 + 32 * b, x);
-                    tmem_wait_ld();
+                    for (int b = 0; b < H / 32; b++) {
+                        float x[32];
+                        tmem_ld32(tmem + lanes + col0 + 32 * b, x);
+                        tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 16; i++) acc[16 * b + i] = __ffma2_rn(acc[16 * b + i], keep2, {x[2 * i], x[2 * i + 1]});
+                        for (int i = 0; i < 16; i++) acc[16 * b + i] = __ffma2_rn(acc[16 * b + i], keep2, {x[2 * i], x[2 * i + 1]});
+                    }
+                    tc_fence_before();
                 }
-                tc_fence_before();
                 __syncwarp();
                 if (lane == 0) arrive(&s.o_empty);
             }
             const uint32_t slot = msg & 1;
             if (ok) ok = wait_warp(&s.v_full[slot], (msg / 2) & 1, abort, a.err);
-            bad = group_any(3, 256, bad);
-            ok = !group_any(4, 256, !ok);  // the eight warps stop together
-            if (!ok) break;
-            const float total = s.val[slot][row];
-            uint64_t odd = s.odd_msg[slot];
-            __syncwarp();
-            if (lane == 0) arrive(&s.v_empty[slot]);
-            msg++;
             // The rows go through Q's place, 16-byte units turned by the row's low bits, so that whole rows are stored.
-            const bool whole = it.count == it.units;
-            float mul = whole ? (total == 0.0f ? 0.0f : 1.0f / total) : 1.0f;
-            if (bad) mul = __int_as_float(0x7fc00000);
-            unsigned char *mine = q_smem + (size_t)row * D * 4;
+            if (ok && row < MR && live) {
+                unsigned char *mine = q_smem + (size_t)row * D * 4;
 #pragma unroll
-            for (int i = 0; i < H / 4; i++)
-                *reinterpret_cast<float4 *>(mine + (((col0 / 4 + i) ^ (row & 7)) << 4)) =
-                    make_float4(acc[2 * i].x * mul, acc[2 * i].y * mul, acc[2 * i + 1].x * mul, acc[2 * i + 1].y * mul);
-            if (odd && row < rows) {  // rare: values that are not finite, for the rows that see them
-                const int node = (it.tile * kRows + row) / a.group;
-                odd &= a.tree ? a.tree[(size_t)it.seq * a.tokens + node] : ~0ull >> (63 - node);
-                while (odd) {
-                    const int nd = __ffsll((long long)odd) - 1;
-                    odd &= odd - 1;
-                    const long long at = a.c.row(it.seq, it.length + nd);
-                    if (at < 0) continue;
-                    const __half *v = a.c.v + ((size_t)at * a.c.kv_heads + it.kv) * D + col0;
+                for (int i = 0; i < H / 4; i++)
+                    *reinterpret_cast<float4 *>(mine + (((col0 / 4 + i) ^ (row & 7)) << 4)) =
+                        make_float4(acc[2 * i].x, acc[2 * i].y, acc[2 * i + 1].x, acc[2 * i + 1].y);
+                uint64_t odd = row % span < rows ? *(volatile uint64_t *)&s.odd_nodes : 0;
+                if (odd) {  // rare: values that are not finite, for the rows that see them
+                    const int node = (it.tile * kRows + row % span) / a.group;
+                    odd &= a.tree ? a.tree[(size_t)it.seq * a.tokens + node] : ~0ull >> (63 - node);
+                    while (odd) {
+                        const int nd = __ffsll((long long)odd) - 1;
+                        odd &= odd - 1;
+                        const long long at = a.c.row(it.seq, it.length + nd);
+                        if (at < 0) continue;
+                        const __half *v = a.c.v + ((size_t)at * a.c.kv_heads + it.kv) * D + col0;
 #pragma unroll 1
-                    for (int i = 0; i < H; i++) {
-                        const float f = __half2float(v[i]);
-                        if (!(fabsf(f) < INFINITY))
-                            *reinterpret_cast<float *>(mine + (((col0 + i) / 4 ^ (row & 7)) << 4) + (i & 3) * 4) += f;
+                        for (int i = 0; i < H; i++) {
+                            const float f = __half2float(v[i]);
+                            if (!(fabsf(f) < INFINITY))
+                                *reinterpret_cast<float *>(mine + (((col0 + i) / 4 ^ (row & 7)) << 4) + (i & 3) * 4) += f;
+                        }
                     }
                 }
             }
-            group_sync(3, 256);
+            bad = group_any(3, 256, bad);
+            ok = !group_any(4, 256, !ok);  // the eight warps stop together
+            if (!ok) break;
+            if (tid == 256) s.odd_nodes = 0;
+            const bool whole = it.count == it.units;
             const size_t part = (size_t)(2 * blockIdx.x + (it.start > s.unit0)) * a.part_rows;
-#pragma unroll 4
+#pragma unroll 1
             for (int i = 0; w + 8 * i < rows; i++) {
                 const int r = w + 8 * i;
                 const size_t at = __shfl_sync(0xffffffffu, where, i);
-                float *dst = whole ? a.out + at : a.part_acc + (part + r) * D;
+                // the copies' maxima and totals become one
+                float m = -INFINITY, l = 0.0f, f[4];
+                for (int k = 0; k < a.copies; k++) m = fmaxf(m, s.q_scale[r + k * span]);
 #pragma unroll
-                for (int u = lane; u < D / 4; u += 32)
-                    reinterpret_cast<float4 *>(dst)[u] = *reinterpret_cast<const float4 *>(q_smem + (size_t)r * D * 4 + ((u ^ (r & 7)) << 4));
+                for (int k = 0; k < 4; k++) {
+                    f[k] = 0.0f;
+                    if (k < a.copies) {
+                        const float mk = s.q_scale[r + k * span], lk = s.val[slot][r + k * span];
+                        f[k] = mk == -INFINITY ? lk : ex2(mk - m);  // lk is 0 (nothing seen) or NaN
+                        l += f[k] * lk;
+                    }
+                }
+                float mul = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+                if (bad) mul = __int_as_float(0x7fc00000);
+                float *dst = whole ? a.out + at : a.part_acc + (part + r) * D;
+                if (!whole && lane == 0) a.part_ml[part + r] = make_float2(m, l);
+#pragma unroll
+                for (int u = lane; u < D / 4; u += 32) {
+                    float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        if (k < a.copies) {
+                            const float4 x = *reinterpret_cast<const float4 *>(q_smem + (size_t)(r + k * span) * D * 4 + ((u ^ (r & 7)) << 4));
+                            v.x += f[k] * x.x, v.y += f[k] * x.y, v.z += f[k] * x.z, v.w += f[k] * x.w;
+                        }
+                    reinterpret_cast<float4 *>(dst)[u] = make_float4(v.x * mul, v.y * mul, v.z * mul, v.w * mul);
+                }
             }
+            __syncwarp();
+            if (lane == 0) arrive(&s.v_empty[slot]);
+            msg++;
+            ring0 += ring_pieces<C>(a, it);
             group_sync(4, 256);  // Q's place is free again
         }
+        // refused sequences
+        for (int q = blockIdx.x; q < a.seqs; q += gridDim.x)
+            if (a.c.committed(q, a.tokens) < 0)
+                for (size_t i = tid - 256; i < (size_t)a.tokens * a.q_heads * D; i += 256)
+                    a.out[(size_t)q * a.tokens * a.q_heads * D + i] = __int_as_float(0x7fc00000);
     }
     __syncthreads();
     if (warp == 1) {
@@ -756,68 +808,65 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     }
 }
 
-// Joins the parts of items that several CTAs share; refused sequences, and
-// every row after an error, become NaN. One warp per (row, head, 128 columns):
-// lanes look up a part's place, maximum and total each, then the warp adds the
-// parts' columns in order, several loads in flight.
+// Joins the parts of items that several CTAs share, and makes every row NaN
+// after an error: one CTA per (row, head). Warps take every eighth part, so all
+// loads of a row are in flight at once; their sums join in order.
 template <int D>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttendArgs a, int ctas) {
-    constexpr int V = D == 64 ? 2 : 4, kBlocks = D / (32 * V);
-    const int lane = threadIdx.x & 31;
-    const int job = blockIdx.x * 8 + (threadIdx.x >> 5), id = job / kBlocks;
-    if (id >= a.seqs * a.tokens * a.q_heads) return;
-    const int h = id % a.q_heads, row = id / a.q_heads, seq = row / a.tokens;
+    constexpr int V = D / 32;
+    __shared__ float sums[8][D], totals[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int id = blockIdx.x, h = id % a.q_heads, row = id / a.q_heads, seq = row / a.tokens;
     const int kv = h / a.group, r = (row % a.tokens) * a.group + h % a.group, tile = r / kRows;
-    const int per = a.c.kv_heads * a.row_tiles, col = (job % kBlocks) * 32 * V + lane * V;
-    const long long w = sum_units(a, a.seqs, per);
+    const int per = a.c.kv_heads * a.row_tiles;
     const int units = units_of(a, a.c.committed(seq, a.tokens));
+    const long long w = sum_units(a, a.seqs, per);
     const long long start = (seq ? sum_units(a, seq, per) : 0) + (long long)(kv * a.row_tiles + tile) * units;
-    float *out = a.out + (size_t)id * D + col;
     const int g = (int)min((long long)ctas, w);
     const int c0 = units ? cta_of(start, w, g) : 0, parts = units ? cta_of(start + units - 1, w, g) - c0 + 1 : 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    float acc[V], m = -INFINITY, l = 0.0f;
+    float *out = a.out + (size_t)id * D;
+    if (*(volatile int *)a.err) {
+        for (int i = threadIdx.x; i < D; i += 256) out[i] = __int_as_float(0x7fc00000);
+        return;
+    }
+    if (parts < 2) return;
+    float m = -INFINITY, l = 0.0f, acc[V];
 #pragma unroll
     for (int e = 0; e < V; e++) acc[e] = 0.0f;
-    if (parts == 0 || *(volatile int *)a.err) {
-        l = __int_as_float(0x7fc00000);
-    } else if (parts == 1) {
-        return;
-    } else {
-        for (int p = lane; p < parts; p += 32)
-            m = fmaxf(m, __ldcg(&a.part_ml[(size_t)(2 * (c0 + p) + (start > range_start(c0 + p, w, g))) * a.part_rows + r % kRows].x));
+    auto place = [&](int p) { return (size_t)(2 * (c0 + p) + (p == 0 && start > range_start(c0, w, g))) * a.part_rows + r % kRows; };
+    for (int p = lane; p < parts; p += 32) m = fmaxf(m, __ldcg(&a.part_ml[place(p)].x));
 #pragma unroll
-        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-        for (int p0 = 0; p0 < parts; p0 += 32) {
-            int at = 0;
-            float f = 0.0f;
-            if (p0 + lane < parts) {
-                const int c = c0 + p0 + lane;
-                at = (2 * c + (start > range_start(c, w, g))) * a.part_rows + r % kRows;
-                const float2 ml = __ldcg(a.part_ml + at);
-                f = ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : ml.y) : ex2(ml.x - m);
-                l += f * ml.y;
-            }
-            const int n = min(32, parts - p0);
-#pragma unroll 8
-            for (int i = 0; i < n; i++) {
-                const float fi = __shfl_sync(0xffffffffu, f, i);
-                const float *p = a.part_acc + (size_t)__shfl_sync(0xffffffffu, at, i) * D + col;
-                float x[V];
-                if constexpr (V == 4) *reinterpret_cast<float4 *>(x) = __ldcg(reinterpret_cast<const float4 *>(p));
-                else *reinterpret_cast<float2 *>(x) = __ldcg(reinterpret_cast<const float2 *>(p));
+    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+#pragma unroll 5
+    for (int p = warp; p < parts; p += 8) {
+        const size_t at = place(p);
+        const float2 ml = __ldcg(a.part_ml + at);
+        const float f = ml.x == -INFINITY ? ml.y : ex2(ml.x - m);  // its total is 0 (nothing seen) or NaN
+        l += f * ml.y;
+        const float *src = a.part_acc + at * D + lane * V;
+        float x[V];
+        if constexpr (V == 2) {
+            *reinterpret_cast<float2 *>(x) = __ldcg(reinterpret_cast<const float2 *>(src));
+        } else {
 #pragma unroll
-                for (int e = 0; e < V; e++) acc[e] = fmaf(fi, x[e], acc[e]);
-            }
+            for (int e = 0; e < V; e += 4) *reinterpret_cast<float4 *>(x + e) = __ldcg(reinterpret_cast<const float4 *>(src + e));
         }
 #pragma unroll
-        for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+        for (int e = 0; e < V; e++) acc[e] = fmaf(f, x[e], acc[e]);
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-    for (int e = 0; e < V; e++) acc[e] *= inv;
-    if constexpr (V == 4) *reinterpret_cast<float4 *>(out) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-    else *reinterpret_cast<float2 *>(out) = make_float2(acc[0], acc[1]);
+    for (int e = 0; e < V; e++) sums[warp][lane * V + e] = acc[e];
+    if (lane == 0) totals[warp] = l;
+    __syncthreads();
+    l = 0.0f;
+    for (int k = 0; k < 8; k++) l += totals[k];
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    for (int i = threadIdx.x; i < D; i += 256) {
+        float v = 0.0f;
+        for (int k = 0; k < 8; k++) v += sums[k][i];
+        out[i] = v * inv;
+    }
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
@@ -848,16 +897,18 @@ int part_rows(int tokens, int group) { return tokens * group < kRows ? tokens * 
 
 size_t ml_bytes(int rows) { return (size_t)2 * kMaxCtas * rows * sizeof(float2); }
 
-template <int D>
+template <int D, int MR>
 int launch(const AttendArgs &a, const CUtensorMap &k_map, const CUtensorMap &v_map) {
-    if (int rc = cudaFuncSetAttribute(tree_attention_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem)) return rc;
+    using C = Cfg<D, MR>;
+    if (int rc = cudaFuncSetAttribute(tree_attention_kernel<D, MR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem)) return rc;
     // no more CTAs than the longest sequences that the table allows could use
-    const long long most = (long long)a.seqs * a.c.kv_heads * a.row_tiles * ((((long long)a.c.table_pages << a.c.shift) + kKeys - 1) / kKeys);
+    const long long units = (((long long)a.c.table_pages << a.c.shift) + kKeys - 1) / kKeys;
+    const long long most = (long long)a.seqs * a.c.kv_heads * a.row_tiles * units;
     const int ctas = (int)(most < kMaxCtas ? most : kMaxCtas);
-    tree_attention_kernel<D><<<ctas, kThreads, Cfg<D>::kSmem, launch_stream>>>(a, k_map, v_map);
+    tree_attention_kernel<D, MR><<<ctas, kThreads, C::kSmem, launch_stream>>>(a, k_map, v_map);
     if (int rc = cudaGetLastError()) return rc;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(((size_t)a.seqs * a.tokens * a.q_heads * (D / (D == 64 ? 64 : 128)) + 7) / 8));
+    cfg.gridDim = dim3((unsigned)(a.seqs * a.tokens * a.q_heads));
     cfg.blockDim = dim3(256);
     cfg.stream = launch_stream;
     cudaLaunchAttribute pdl[1];
@@ -907,7 +958,11 @@ extern "C" int qg_tree_attention(float *out, const float *q, const qg_kv_cache *
     CUtensorMap k_map, v_map;
     if (int rc = pool_map(&k_map, a.c, a.c.k, a.k_box)) return rc;
     if (int rc = pool_map(&v_map, a.c, a.c.v, a.v_box)) return rc;
-    if (a.c.head_dim == 64) return launch<64>(a, k_map, v_map);
-    if (a.c.head_dim == 128) return launch<128>(a, k_map, v_map);
-    return launch<256>(a, k_map, v_map);
+    // Few rows: heads of 64 and 128 values, whose units take little time, share a unit's keys among copies of Q; heads of
+    // 256 keep only 64 rows of Q, and the room goes to the ring.
+    const int rows = tokens * a.group;
+    a.copies = a.c.head_dim == 256 || rows > 64 ? 1 : rows > 32 ? 2 : 4;
+    if (a.c.head_dim == 64) return launch<64, 128>(a, k_map, v_map);
+    if (a.c.head_dim == 128) return launch<128, 128>(a, k_map, v_map);
+    return rows <= 64 ? launch<256, 64>(a, k_map, v_map) : launch<256, 128>(a, k_map, v_map);
 }
