@@ -75,7 +75,7 @@ struct Cfg {
 struct Shared {
     float val[2][kRows];    // rescaling factors, and at an item's end the totals: softmax -> accumulators
     float q_scale[kRows];   // at an item's end the maxima
-    uint64_t full[10], empty[10], s_full[2], p_full[2][kKeys / kChunk], pv_done[2], v_full[2], v_empty[2], o_full, o_empty, q_full, clean, drain;
+    uint64_t k_full[10], v_full[10], empty[10], s_full[2], p_full[2][kKeys / kChunk], pv_done[2], msg_full[2], msg_empty[2], o_full, o_empty, q_full, landed, clean, drain;
     uint64_t odd_nodes;     // nodes whose values are not finite
     long long unit0, unit1;
     int seq0, length0, kv0, tile0, first0;
@@ -314,14 +314,14 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     } else if (warp == 2 && lane == 0) {
         s.abort = 0;
         s.odd_nodes = 0;
-        for (int i = 0; i < NS; i++) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], 1);
+        for (int i = 0; i < NS; i++) mbar_init(&s.k_full[i], 1), mbar_init(&s.v_full[i], 1), mbar_init(&s.empty[i], 1);
         for (int i = 0; i < 2; i++) {
             mbar_init(&s.s_full[i], 1), mbar_init(&s.pv_done[i], 1);
-            mbar_init(&s.v_full[i], 4), mbar_init(&s.v_empty[i], 8);
+            mbar_init(&s.msg_full[i], 4), mbar_init(&s.msg_empty[i], 8);
             for (int k = 0; k < kKeys / kChunk; k++) mbar_init(&s.p_full[i][k], 4);
         }
         mbar_init(&s.o_full, 1), mbar_init(&s.o_empty, 8), mbar_init(&s.q_full, 8), mbar_init(&s.drain, 2);
-        mbar_init(&s.clean, 8);
+        mbar_init(&s.landed, 1), mbar_init(&s.clean, 8);
         fence_mbar_init();
     } else if (warp == 3 && lane == 0) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map));
@@ -340,7 +340,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         if (warp == 0) {
             // ------------------------------------------------ producer: pages to the ring
             // The warp looks the pages of one unit up ahead of time (a lane each) and its lanes issue the boxes.
-            uint32_t idx = 0;
+            // (k_phase, v_phase: a bit per place of the ring, the parity of the next filling with keys or values. Each kind
+            // has its barriers, so that the role that takes it sees every phase of them.)
+            uint32_t idx = 0, k_phase = 0, v_phase = 0;
             bool ok = true;
             const int page = a.c.page_tokens(), per_unit = max(1, kKeys >> a.c.shift);
             while (ok && walk.next(a, it)) {
@@ -374,22 +376,27 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                         const int key0 = is_k ? 0 : c * VK;  // the piece's first key within the unit
                         const int boxes = (min(piece, keys - key0) + box - 1) / box;  // none past the last position
                         const int blocks = is_k ? 1 : NC;                              // column blocks of the piece
-                        if (lane == 0) mbar_arrive_expect_tx(&s.full[st], boxes * blocks * box * 128);
+                        uint64_t *full = is_k ? &s.k_full[st] : &s.v_full[st];
+                        (is_k ? k_phase : v_phase) ^= 1u << st;
+                        if (lane == 0) mbar_arrive_expect_tx(full, boxes * blocks * box * 128);
                         __syncwarp();
                         const int b = is_k ? lane : lane / NC, col = is_k ? c : lane % NC;
                         const int key = key0 + b * box, p = pos + key;
                         const int id = __shfl_sync(0xffffffffu, ids, (p >> a.c.shift) - (pos >> a.c.shift) & 31);
                         if (b < boxes)
                             tma_2d(ring + st * kStage + (is_k ? 0 : col * VK * 128) + b * box * 128, is_k ? &k_map : &v_map,
-                                   it.kv * D + col * 64, (id << a.c.shift) + (p & (page - 1)), &s.full[st]);
+                                   it.kv * D + col * 64, (id << a.c.shift) + (p & (page - 1)), full);
                     }
                 }
             }
             if (!ok && lane == 0)  // the copies in flight land before the CTA ends
-                for (uint32_t i = idx > NS ? idx - NS : 0; i < idx; i++) wait_drain(&s.full[i % NS], (i / NS) & 1);
+                for (uint32_t st = 0; st < NS && st < idx; st++) {
+                    wait_drain(&s.k_full[st], ~k_phase >> st & 1);
+                    wait_drain(&s.v_full[st], ~v_phase >> st & 1);
+                }
         } else if (warp == 1 && lane == 0) {
             // ------------------------------------------------ S = Q K^T
-            uint32_t ring0 = 0, tile = 0, item = 0;
+            uint32_t ring0 = 0, tile = 0, item = 0, phase = 0;
             bool ok = true;
             const uint64_t q_lo = operand(smem_u32(q_smem) + C::kPlane, 16);
             const uint64_t q_hi = operand(smem_u32(q_smem), 16);
@@ -402,8 +409,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
 #pragma unroll 1
                     for (int c = 0; ok && c < NC; c++, idx++) {
                         const uint32_t st = idx % NS;
-                        ok = wait(&s.full[st], (idx / NS) & 1, abort, a.err);
+                        ok = wait(&s.k_full[st], phase >> st & 1, abort, a.err);
                         if (!ok) break;
+                        phase ^= 1u << st;
                         tc_fence_after();
                         const uint64_t kd = operand(smem_u32(ring + st * kStage), 16);
 #pragma unroll
@@ -423,23 +431,38 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             wait_drain(&s.drain, 0);
         } else if (warp == 2 && lane == 0) {
             // ------------------------------------------------ O = P V
-            uint32_t ring0 = 0, tile = 0, tails = 0;
+            uint32_t ring0 = 0, tile = 0, tails = 0, phase = 0;
             bool ok = true;
             while (ok && walk.next(a, it)) {
                 for (int j = 0; ok && j < it.count; j++, tile++) {
                     const uint32_t buf = tile & 1, p0 = tmem + C::kS + buf * kKeys;
                     const int keys = keys_of(a, it, j);
                     uint32_t idx = ring0 + v_index(j, it.count) * NC;
-                    if (tile >= 1) ok = wait(&s.o_empty, (tile - 1) & 1, abort, a.err);
-                    if (ok && it.length < (it.first + j + 1) * kKeys) ok = wait(&s.clean, tails++ & 1, abort, a.err);
+                    // a unit that holds nodes: the accumulator warps clean its values as soon as they are there
+                    const bool tail = it.length < (it.first + j + 1) * kKeys;
+                    if (tail) {
+                        for (int c = 0; ok && c * VK < keys; c++) {
+                            const uint32_t st = (idx + c) % NS;
+                            ok = wait(&s.v_full[st], phase >> st & 1, abort, a.err);
+                            phase ^= 1u << st;
+                        }
+                        if (!ok) break;
+                        arrive(&s.landed);
+                        ok = wait(&s.clean, tails++ & 1, abort, a.err);
+                    }
+                    if (ok && tile >= 1) ok = wait(&s.o_empty, (tile - 1) & 1, abort, a.err);
                     // 32 keys at a time, as the softmax delivers them; past the last key there is nothing
 #pragma unroll 1
                     for (int h = 0; ok && h * kChunk < keys; h++) {
                         const uint32_t st = idx % NS;
-                        ok = wait(&s.full[st], (idx / NS) & 1, abort, a.err) && wait(&s.p_full[buf][h], (tile / 2) & 1, abort, a.err);
+                        const int row = h * kChunk % VK;
+                        if (!tail && row == 0) {
+                            ok = wait(&s.v_full[st], phase >> st & 1, abort, a.err);
+                            phase ^= 1u << st;
+                        }
+                        ok = ok && wait(&s.p_full[buf][h], (tile / 2) & 1, abort, a.err);
                         if (!ok) break;
                         tc_fence_after();
-                        const int row = h * kChunk % VK;
                         const uint64_t vd = operand(smem_u32(ring + st * kStage) + row * 128, VK * 128);
                         const int steps = min(2, (keys - h * kChunk + 15) / 16);
                         for (int k = 0; k < steps; k++) {
@@ -518,11 +541,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 }
                 // the factor goes to the accumulators
                 const uint32_t slot = msg & 1;
-                if (msg >= 2) ok = wait_warp(&s.v_empty[slot], (msg / 2 - 1) & 1, abort, a.err);
+                if (msg >= 2) ok = wait_warp(&s.msg_empty[slot], (msg / 2 - 1) & 1, abort, a.err);
                 if (!ok) break;
                 s.val[slot][row] = keep;
                 __syncwarp();
-                if (lane == 0) arrive(&s.v_full[slot]);
+                if (lane == 0) arrive(&s.msg_full[slot]);
                 msg++;
                 float2 sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
                 const float2 c2 = {c, c}, off2 = {-off, -off}, up2 = {kPScale, kPScale};
@@ -574,13 +597,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             }
             // the item's totals
             const uint32_t slot = msg & 1;
-            if (ok && msg >= 2) ok = wait_warp(&s.v_empty[slot], (msg / 2 - 1) & 1, abort, a.err);
+            if (ok && msg >= 2) ok = wait_warp(&s.msg_empty[slot], (msg / 2 - 1) & 1, abort, a.err);
             ok = !group_any(1, 128, !ok);  // the four warps stop together
             if (!ok) break;
             s.val[slot][row] = l;
             s.q_scale[row] = m;
             __syncwarp();
-            if (lane == 0) arrive(&s.v_full[slot]);
+            if (lane == 0) arrive(&s.msg_full[slot]);
             msg++;
             item++;
         }
@@ -590,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         constexpr int H = D / 2, V = D / 32;
         const int w = warp - 8, row = (warp & 3) * 32 + lane, col0 = (w >> 2) * H, span = kRows / a.copies;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
-        uint32_t ring0 = 0, tile = 0, msg = 0;
+        uint32_t ring0 = 0, tile = 0, msg = 0, tails = 0;
         bool ok = true;
         while (ok && walk.next(a, it)) {
             // Warp w prepares, and at the end stores, rows w, w+8, ...; lane i < 16 knows where row w+8i lies in q and
@@ -667,15 +690,21 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             for (int i = 0; i < H / 2; i++) acc[i] = make_float2(0.0f, 0.0f);
 #pragma unroll 1
             for (int j = 0; ok && j < it.count; j++, tile++, msg++) {
+                const uint32_t slot = msg & 1;
+                ok = wait_warp(&s.msg_full[slot], (msg / 2) & 1, abort, a.err);
+                if (!ok) break;
+                const float keep = s.val[slot][row];
+                __syncwarp();
+                if (lane == 0) arrive(&s.msg_empty[slot]);
                 const int past = it.length - (it.first + j) * kKeys;  // keys of the unit before the nodes
                 if (past < kKeys) {
                     // Values past the last position become 0 up to a multiple of 32; those of nodes 0 where they are
                     // not finite.
                     const int end = min(kKeys, past + a.tokens), from = max(past, 0);
-                    for (int k0 = from & ~31; ok && k0 < end; k0 += 32) {
-                        const uint32_t idx = ring0 + v_index(j, it.count) * NC + k0 / VK, st = idx % NS;
-                        ok = wait_warp(&s.full[st], (idx / NS) & 1, abort, a.err);
-                        if (!ok) break;
+                    ok = wait_warp(&s.landed, tails++ & 1, abort, a.err);
+                    if (!ok) break;
+                    for (int k0 = from & ~31; k0 < end; k0 += 32) {
+                        const uint32_t st = (ring0 + v_index(j, it.count) * NC + k0 / VK) % NS;
                         unsigned char *v0 = ring + st * kStage + k0 % VK * 128;
                         uint64_t odd = 0;
 #pragma unroll 1
@@ -697,14 +726,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) arrive(&s.clean);
-                    if (!ok) break;
                 }
-                const uint32_t slot = msg & 1;
-                ok = wait_warp(&s.v_full[slot], (msg / 2) & 1, abort, a.err);
-                if (!ok) break;
-                const float keep = s.val[slot][row];
-                __syncwarp();
-                if (lane == 0) arrive(&s.v_empty[slot]);
                 ok = wait_warp(&s.o_full, tile & 1, abort, a.err);
                 if (!ok) break;
                 if (live) {
@@ -724,7 +746,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 if (lane == 0) arrive(&s.o_empty);
             }
             const uint32_t slot = msg & 1;
-            if (ok) ok = wait_warp(&s.v_full[slot], (msg / 2) & 1, abort, a.err);
+            if (ok) ok = wait_warp(&s.msg_full[slot], (msg / 2) & 1, abort, a.err);
             // The rows go through Q's place, 16-byte units turned by the row's low bits, so that whole rows are stored.
             if (ok && row < MR && live) {
                 unsigned char *mine = q_smem + (size_t)row * D * 4;
@@ -790,7 +812,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 }
             }
             __syncwarp();
-            if (lane == 0) arrive(&s.v_empty[slot]);
+            if (lane == 0) arrive(&s.msg_empty[slot]);
             msg++;
             ring0 += ring_pieces<C>(a, it);
             group_sync(4, 256);  // Q's place is free again
