@@ -65,24 +65,26 @@ struct Cfg {
     static constexpr int kChunks = D / 64;                  // 128-byte wide column blocks
     static constexpr int kBlock = MR * 128;                 // one of them, of one plane of Q
     static constexpr int kPlane = kChunks * kBlock;
-    // The ring's pieces: 64 columns of 128 keys, or all columns of kVKeys values; kChunks pieces for a unit's keys or values.
+    // The rings' pieces: 64 columns of 128 keys, or all columns of kVKeys values; kChunks pieces for a unit's keys or values.
     static constexpr int kVKeys = kStage / (2 * D);
-    static constexpr int kStages = D == 256 ? (MR == 64 ? 10 : 6) : 8;
-    static constexpr int kSmem = 2 * kPlane + kStages * kStage + 2048 + 1024;
+    static constexpr int kKStages = D == 256 ? (MR == 64 ? 5 : 3) : D == 128 ? 5 : 6, kVStages = kKStages;
+    static constexpr int kStages = kKStages + kVStages;
+    static constexpr int kSmem = 2 * kPlane + kStages * kStage + 3072;
     static constexpr int kS = 256;  // tensor memory columns: O, then two of S (P takes its place)
 };
 
 struct Shared {
     float val[2][kRows];    // rescaling factors, and at an item's end the totals: softmax -> accumulators
     float q_scale[kRows];   // at an item's end the maxima
-    uint64_t k_full[10], v_full[10], empty[10], s_full[2], p_full[2][kKeys / kChunk], pv_done[2], msg_full[2], msg_empty[2], o_full, o_empty, q_full, landed, clean, drain;
+    uint64_t k_full[6], k_empty[6], v_full[6], v_empty[6], s_full[2], p_full[2][kKeys / kChunk], pv_done[2], msg_full[2], msg_empty[2], o_full, o_empty, q_full, landed, clean, drain;
+    int pages[2][2][8];     // of the units that the producers are at: keys, values
     uint64_t odd_nodes;     // nodes whose values are not finite
     long long unit0, unit1;
     int seq0, length0, kv0, tile0, first0;
     uint32_t tmem;
     int abort;
 };
-static_assert(sizeof(Shared) <= 2048, "shared bookkeeping");
+static_assert(sizeof(Shared) <= 3072, "shared bookkeeping");
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -113,12 +115,19 @@ __device__ __forceinline__ void wait_drain(uint64_t *bar, uint32_t parity) {
     for (int i = 0; i < (1 << 17); i++)
         if (mbar_try_wait_sleep(bar, parity, kWaitHintNs)) return;
 }
-__device__ __forceinline__ void tma_2d(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
+// Box at pool row y, 64-column block z.
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap *map, int y, int z, uint32_t bar) {
     asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
-            "r"(smem_u32(dst)),
-        "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+            "r"(dst),
+        "l"(map), "r"(0), "r"(y), "r"(z), "r"(bar)
         : "memory");
+}
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
 }
 // Shared-memory operand with 128-byte swizzle. K-major (Q, K: rows of 64
 // values): groups of 8 rows 1024 bytes apart. MN-major (V as it lies, rows are
@@ -262,17 +271,19 @@ struct Walk {
     }
 };
 
-// The ring's order within an item of n units: K0, K1, V0, K2, V1, ..., V(n-1),
-// `pieces` pieces each; a last unit that is not full has fewer pieces of V.
-__device__ __forceinline__ uint32_t k_index(int j) { return j ? 2 * j - 1 : 0; }
-__device__ __forceinline__ uint32_t v_index(int j, int n) { return j == n - 1 ? 2 * n - 1 : 2 * j + 2; }
 // Keys that unit j of an item's part holds.
 __device__ __forceinline__ int keys_of(const AttendArgs &a, const Item &it, int j) {
     return min(kKeys, it.length + a.tokens - (it.first + j) * kKeys);
 }
+// Where key `row` of a piece of values starts: boxes of v_box keys, in each the column blocks one after the other.
+template <int NC>
+__device__ __forceinline__ uint32_t value_at(const AttendArgs &a, int row) {
+    return ((row & ~(a.v_box - 1)) * NC + (row & (a.v_box - 1))) * 128;
+}
+// Pieces of values of an item's part: a last unit that is not full has fewer.
 template <class C>
-__device__ __forceinline__ uint32_t ring_pieces(const AttendArgs &a, const Item &it) {
-    return (2 * it.count - 1) * C::kChunks + (keys_of(a, it, it.count - 1) + C::kVKeys - 1) / C::kVKeys;
+__device__ __forceinline__ uint32_t value_pieces(const AttendArgs &a, const Item &it) {
+    return (it.count - 1) * C::kChunks + (keys_of(a, it, it.count - 1) + C::kVKeys - 1) / C::kVKeys;
 }
 
 template <int D, int MR>
@@ -280,11 +291,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                                                                      const __grid_constant__ CUtensorMap k_map,
                                                                      const __grid_constant__ CUtensorMap v_map) {
     using C = Cfg<D, MR>;
-    constexpr int NC = C::kChunks, NS = C::kStages, VK = C::kVKeys;
-    extern __shared__ unsigned char raw[];
-    unsigned char *smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
-    unsigned char *q_smem = smem, *ring = smem + 2 * C::kPlane;
-    Shared &s = *reinterpret_cast<Shared *>(ring + NS * kStage);
+    constexpr int NC = C::kChunks, NK = C::kKStages, NV = C::kVStages, VK = C::kVKeys;
+    extern __shared__ __align__(1024) unsigned char smem[];  // swizzled tiles start on multiples of 1024
+    unsigned char *q_smem = smem, *k_ring = smem + 2 * C::kPlane, *v_ring = k_ring + NK * kStage;
+    Shared &s = *reinterpret_cast<Shared *>(v_ring + NV * kStage);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     volatile int *abort = &s.abort;
 
@@ -314,7 +324,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     } else if (warp == 2 && lane == 0) {
         s.abort = 0;
         s.odd_nodes = 0;
-        for (int i = 0; i < NS; i++) mbar_init(&s.k_full[i], 1), mbar_init(&s.v_full[i], 1), mbar_init(&s.empty[i], 1);
+        for (int i = 0; i < NK; i++) mbar_init(&s.k_full[i], 1), mbar_init(&s.k_empty[i], 1);
+        for (int i = 0; i < NV; i++) mbar_init(&s.v_full[i], 1), mbar_init(&s.v_empty[i], 1);
         for (int i = 0; i < 2; i++) {
             mbar_init(&s.s_full[i], 1), mbar_init(&s.pv_done[i], 1);
             mbar_init(&s.msg_full[i], 4), mbar_init(&s.msg_empty[i], 8);
@@ -337,14 +348,20 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
-        if (warp == 0) {
-            // ------------------------------------------------ producer: pages to the ring
-            // The warp looks the pages of one unit up ahead of time (a lane each) and its lanes issue the boxes.
-            // (k_phase, v_phase: a bit per place of the ring, the parity of the next filling with keys or values. Each kind
-            // has its barriers, so that the role that takes it sees every phase of them.)
-            uint32_t idx = 0, k_phase = 0, v_phase = 0;
-            bool ok = true;
+        if (warp == 0 || warp == 3) {
+            // ------------------------------------------------ producers: pages to the rings, keys (warp 0), values (warp 3)
+            // A warp issues its copies one after the other (134 cycles for a 2 KB box, 440 for 8 KB, measured), 15-23
+            // bytes per cycle and SM; HBM delivers 25, so it takes two of them.
+            // The warp looks a unit's pages up one unit ahead (a lane each); one lane issues the boxes. A box of keys has
+            // one block of 64 columns, a box of values all of them.
+            const bool is_k = warp == 0;
             const int page = a.c.page_tokens(), per_unit = max(1, kKeys >> a.c.shift);
+            const int box = is_k ? a.k_box : a.v_box, piece = is_k ? kKeys : VK, bytes = box * 128 * (is_k ? 1 : NC);
+            const uint32_t ring = smem_u32(is_k ? k_ring : v_ring), places = is_k ? NK : NV;
+            uint64_t *full = is_k ? s.k_full : s.v_full, *empty = is_k ? s.k_empty : s.v_empty;
+            const CUtensorMap *map = is_k ? &k_map : &v_map;
+            uint32_t st = 0, round = 0, unit = 0;
+            bool ok = true;
             while (ok && walk.next(a, it)) {
                 const int n = it.length + a.tokens;
                 const int *table = a.c.table + (size_t)it.seq * a.c.table_pages;
@@ -353,50 +370,39 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     const int id = lane < per_unit && p <= (n - 1) >> a.c.shift ? table[p] : 0;
                     return (unsigned)id < (unsigned)a.c.pages ? id : 0;  // the accumulators make the row NaN
                 };
-                int next_ids = look_up(0), k_ids = 0, v_ids = 0;
-                for (int i = 0; ok && i < 2 * it.count; i++) {
-                    // i-th of K0, K1, V0, K2, V1, ...
-                    const bool is_k = i == 0 || (i & 1 && i != 2 * it.count - 1);
-                    const int j = is_k ? (i + 1) / 2 : (i == 2 * it.count - 1 ? it.count - 1 : i / 2 - 1);
-                    if (is_k) {
-                        v_ids = k_ids;
-                        k_ids = next_ids;
-                        if (j + 1 < it.count) next_ids = look_up(j + 1);
-                    } else if (j == it.count - 1) {
-                        v_ids = k_ids;
-                    }
-                    const int ids = is_k ? k_ids : v_ids;
+                int ids = look_up(0);
+                for (int j = 0; ok && j < it.count; j++, unit++) {
+                    int *pages = s.pages[!is_k][unit & 1];
+                    if (lane < 8) pages[lane] = ids;
+                    __syncwarp();
+                    if (j + 1 < it.count) ids = look_up(j + 1);
                     const int pos = (it.first + j) * kKeys, keys = keys_of(a, it, j);
-                    const int box = is_k ? a.k_box : a.v_box, piece = is_k ? kKeys : VK;
                     const int pieces = is_k ? NC : (keys + VK - 1) / VK;
-                    for (int c = 0; ok && c < pieces; c++, idx++) {
-                        const int st = idx % NS;
-                        if (idx >= NS) ok = wait_warp(&s.empty[st], (idx / NS - 1) & 1, abort, a.err);
+                    for (int c = 0; c < pieces; c++) {
+                        if (round) ok = wait_warp(&empty[st], (round - 1) & 1, abort, a.err);
                         if (!ok) break;
-                        const int key0 = is_k ? 0 : c * VK;  // the piece's first key within the unit
-                        const int boxes = (min(piece, keys - key0) + box - 1) / box;  // none past the last position
-                        const int blocks = is_k ? 1 : NC;                              // column blocks of the piece
-                        uint64_t *full = is_k ? &s.k_full[st] : &s.v_full[st];
-                        (is_k ? k_phase : v_phase) ^= 1u << st;
-                        if (lane == 0) mbar_arrive_expect_tx(full, boxes * blocks * box * 128);
+                        if (elect_one()) {
+                            const int key0 = is_k ? 0 : c * VK;  // the piece's first key within the unit
+                            const int boxes = (min(piece, keys - key0) + box - 1) / box;  // none past the last position
+                            const uint32_t bar = smem_u32(&full[st]);
+                            uint32_t dst = ring + st * kStage;
+                            mbar_arrive_expect_tx(&full[st], boxes * bytes);
+                            int p = pos + key0;
+                            for (int b = 0; b < boxes; b++, p += box, dst += bytes)
+                                tma_3d(dst, map, (pages[(p >> a.c.shift) - (pos >> a.c.shift)] << a.c.shift) + (p & (page - 1)),
+                                       it.kv * NC + (is_k ? c : 0), bar);
+                        }
                         __syncwarp();
-                        const int b = is_k ? lane : lane / NC, col = is_k ? c : lane % NC;
-                        const int key = key0 + b * box, p = pos + key;
-                        const int id = __shfl_sync(0xffffffffu, ids, (p >> a.c.shift) - (pos >> a.c.shift) & 31);
-                        if (b < boxes)
-                            tma_2d(ring + st * kStage + (is_k ? 0 : col * VK * 128) + b * box * 128, is_k ? &k_map : &v_map,
-                                   it.kv * D + col * 64, (id << a.c.shift) + (p & (page - 1)), full);
+                        if (++st == places) st = 0, round++;
                     }
                 }
             }
             if (!ok && lane == 0)  // the copies in flight land before the CTA ends
-                for (uint32_t st = 0; st < NS && st < idx; st++) {
-                    wait_drain(&s.k_full[st], ~k_phase >> st & 1);
-                    wait_drain(&s.v_full[st], ~v_phase >> st & 1);
-                }
-        } else if (warp == 1 && lane == 0) {
+                for (uint32_t i = 0; i < places; i++)
+                    if (i < st || round) wait_drain(&full[i], (i < st ? round : round - 1) & 1);
+        } else if (warp == 1 && elect_one()) {
             // ------------------------------------------------ S = Q K^T
-            uint32_t ring0 = 0, tile = 0, item = 0, phase = 0;
+            uint32_t st = 0, round = 0, tile = 0, item = 0;
             bool ok = true;
             const uint64_t q_lo = operand(smem_u32(q_smem) + C::kPlane, 16);
             const uint64_t q_hi = operand(smem_u32(q_smem), 16);
@@ -404,81 +410,65 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 ok = wait(&s.q_full, item & 1, abort, a.err);
                 for (int j = 0; ok && j < it.count; j++, tile++) {
                     const uint32_t buf = tile & 1, d = tmem + C::kS + buf * kKeys;
-                    uint32_t idx = ring0 + k_index(j) * NC;
                     if (tile >= 2) ok = wait(&s.pv_done[buf], (tile / 2 - 1) & 1, abort, a.err);
 #pragma unroll 1
-                    for (int c = 0; ok && c < NC; c++, idx++) {
-                        const uint32_t st = idx % NS;
-                        ok = wait(&s.k_full[st], phase >> st & 1, abort, a.err);
+                    for (int c = 0; ok && c < NC; c++) {
+                        ok = wait(&s.k_full[st], round & 1, abort, a.err);
                         if (!ok) break;
-                        phase ^= 1u << st;
                         tc_fence_after();
-                        const uint64_t kd = operand(smem_u32(ring + st * kStage), 16);
+                        const uint64_t kd = operand(smem_u32(k_ring + st * kStage), 16);
 #pragma unroll
                         for (int k = 0; k < 4; k++)
                             mma_ss(d, q_lo + c * (C::kBlock / 16) + 2 * k, kd + 2 * k, idesc(kKeys, false), c + k > 0);
 #pragma unroll
                         for (int k = 0; k < 4; k++)
                             mma_ss(d, q_hi + c * (C::kBlock / 16) + 2 * k, kd + 2 * k, idesc(kKeys, false), true);
-                        commit(&s.empty[st]);
+                        commit(&s.k_empty[st]);
+                        if (++st == NK) st = 0, round++;
                     }
                     if (ok) commit(&s.s_full[buf]);
                 }
-                ring0 += ring_pieces<C>(a, it);
                 item++;
             }
             commit(&s.drain);
             wait_drain(&s.drain, 0);
-        } else if (warp == 2 && lane == 0) {
+        } else if (warp == 2 && elect_one()) {
             // ------------------------------------------------ O = P V
-            uint32_t ring0 = 0, tile = 0, tails = 0, phase = 0;
+            uint32_t st = 0, round = 0, tile = 0, cleans = 0;
             bool ok = true;
             while (ok && walk.next(a, it)) {
                 for (int j = 0; ok && j < it.count; j++, tile++) {
                     const uint32_t buf = tile & 1, p0 = tmem + C::kS + buf * kKeys;
-                    const int keys = keys_of(a, it, j);
-                    uint32_t idx = ring0 + v_index(j, it.count) * NC;
-                    // a unit that holds nodes: the accumulator warps clean its values as soon as they are there
-                    const bool tail = it.length < (it.first + j + 1) * kKeys;
-                    if (tail) {
-                        for (int c = 0; ok && c * VK < keys; c++) {
-                            const uint32_t st = (idx + c) % NS;
-                            ok = wait(&s.v_full[st], phase >> st & 1, abort, a.err);
-                            phase ^= 1u << st;
-                        }
-                        if (!ok) break;
-                        arrive(&s.landed);
-                        ok = wait(&s.clean, tails++ & 1, abort, a.err);
-                    }
-                    if (ok && tile >= 1) ok = wait(&s.o_empty, (tile - 1) & 1, abort, a.err);
+                    const int keys = keys_of(a, it, j), past = it.length - (it.first + j) * kKeys;
+                    if (tile >= 1) ok = wait(&s.o_empty, (tile - 1) & 1, abort, a.err);
                     // 32 keys at a time, as the softmax delivers them; past the last key there is nothing
 #pragma unroll 1
                     for (int h = 0; ok && h * kChunk < keys; h++) {
-                        const uint32_t st = idx % NS;
                         const int row = h * kChunk % VK;
-                        if (!tail && row == 0) {
-                            ok = wait(&s.v_full[st], phase >> st & 1, abort, a.err);
-                            phase ^= 1u << st;
+                        if (row == 0) ok = wait(&s.v_full[st], round & 1, abort, a.err);
+                        if (ok && (h + 1) * kChunk > past) {  // nodes: the accumulator warps clean their values
+                            arrive(&s.landed);
+                            ok = wait(&s.clean, cleans++ & 1, abort, a.err);
                         }
                         ok = ok && wait(&s.p_full[buf][h], (tile / 2) & 1, abort, a.err);
                         if (!ok) break;
                         tc_fence_after();
-                        const uint64_t vd = operand(smem_u32(ring + st * kStage) + row * 128, VK * 128);
+                        const uint32_t v0 = smem_u32(v_ring + st * kStage);
                         const int steps = min(2, (keys - h * kChunk + 15) / 16);
                         for (int k = 0; k < steps; k++) {
-                            mma_ts(tmem, p0 + h * kChunk + 16 + k * 8, vd + k * 128, idesc(D, true), h + k > 0);
-                            mma_ts(tmem, p0 + h * kChunk + k * 8, vd + k * 128, idesc(D, true), true);
+                            const uint64_t vd = operand(v0 + value_at<NC>(a, row + 16 * k), a.v_box * 128);
+                            mma_ts(tmem, p0 + h * kChunk + 16 + k * 8, vd, idesc(D, true), h + k > 0);
+                            mma_ts(tmem, p0 + h * kChunk + k * 8, vd, idesc(D, true), true);
                         }
                         if (row + kChunk == VK || (h + 1) * kChunk >= keys) {
-                            commit(&s.empty[st]);
-                            idx++;
+                            commit(&s.v_empty[st]);
+                            if (++st == NV) st = 0, round++;
                         }
                     }
                     if (!ok) break;
                     commit(&s.pv_done[buf]);
                     commit(&s.o_full);
                 }
-                ring0 += ring_pieces<C>(a, it);
             }
             commit(&s.drain);
             wait_drain(&s.drain, 0);
@@ -613,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         constexpr int H = D / 2, V = D / 32;
         const int w = warp - 8, row = (warp & 3) * 32 + lane, col0 = (w >> 2) * H, span = kRows / a.copies;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
-        uint32_t ring0 = 0, tile = 0, msg = 0, tails = 0;
+        uint32_t piece0 = 0, tile = 0, msg = 0, cleans = 0;
         bool ok = true;
         while (ok && walk.next(a, it)) {
             // Warp w prepares, and at the end stores, rows w, w+8, ...; lane i < 16 knows where row w+8i lies in q and
@@ -700,18 +690,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 if (past < kKeys) {
                     // Values past the last position become 0 up to a multiple of 32; those of nodes 0 where they are
                     // not finite.
-                    const int end = min(kKeys, past + a.tokens), from = max(past, 0);
-                    ok = wait_warp(&s.landed, tails++ & 1, abort, a.err);
-                    if (!ok) break;
-                    for (int k0 = from & ~31; k0 < end; k0 += 32) {
-                        const uint32_t st = (ring0 + v_index(j, it.count) * NC + k0 / VK) % NS;
-                        unsigned char *v0 = ring + st * kStage + k0 % VK * 128;
+                    const int end = min(kKeys, past + a.tokens);
+                    for (int k0 = max(past, 0) & ~31; ok && k0 < end; k0 += 32) {
+                        ok = wait_warp(&s.landed, cleans++ & 1, abort, a.err);
+                        if (!ok) break;
+                        unsigned char *v0 = v_ring + (piece0 + j * NC + k0 / VK) % NV * kStage;
                         uint64_t odd = 0;
 #pragma unroll 1
                         for (int u = tid - 256; u < 32 * 8 * NC; u += 256) {
                             const int key = k0 + ((u >> 3) & 31);
                             if (key < past) continue;
-                            uint4 *p = reinterpret_cast<uint4 *>(v0 + (u >> 8) * VK * 128 + (u & 255) * 16);
+                            uint4 *p = reinterpret_cast<uint4 *>(v0 + value_at<NC>(a, key % VK) + (u >> 8) * a.v_box * 128 + (u & 7) * 16);
                             uint4 v = key < end ? *p : make_uint4(0, 0, 0, 0);
                             uint32_t *wd = &v.x;
 #pragma unroll
@@ -722,10 +711,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                             *p = v;
                         }
                         if (odd) atomicOr(reinterpret_cast<unsigned long long *>(&s.odd_nodes), (unsigned long long)odd);
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) arrive(&s.clean);
                     }
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) arrive(&s.clean);
+                    if (!ok) break;
                 }
                 ok = wait_warp(&s.o_full, tile & 1, abort, a.err);
                 if (!ok) break;
@@ -814,7 +804,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             __syncwarp();
             if (lane == 0) arrive(&s.msg_empty[slot]);
             msg++;
-            ring0 += ring_pieces<C>(a, it);
+            piece0 += value_pieces<C>(a, it);
             group_sync(4, 256);  // Q's place is free again
         }
         // refused sequences
@@ -895,8 +885,8 @@ using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t,
                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// One layer's pool as rows of kv_heads*head_dim halves, read 64 values x box rows at a time.
-int pool_map(CUtensorMap *m, const CacheView &c, const __half *pool, int box) {
+// One layer's pool as [column blocks of 64 values][rows][64], read in boxes of box rows and `blocks` column blocks.
+int pool_map(CUtensorMap *m, const CacheView &c, const __half *pool, int box, int blocks) {
     static EncodeTiled fn = nullptr;
     if (!fn) {
         void *p = nullptr;
@@ -906,10 +896,10 @@ int pool_map(CUtensorMap *m, const CacheView &c, const __half *pool, int box) {
             return cudaErrorNotSupported;
         fn = reinterpret_cast<EncodeTiled>(p);
     }
-    const cuuint64_t inner = (cuuint64_t)c.kv_heads * c.head_dim;
-    const cuuint64_t dims[2] = {inner, (cuuint64_t)c.pages << c.shift}, strides[1] = {inner * sizeof(__half)};
-    const cuuint32_t boxes[2] = {64, (cuuint32_t)box}, step[2] = {1, 1};
-    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<__half *>(pool), dims, strides, boxes, step,
+    const cuuint64_t width = (cuuint64_t)c.kv_heads * c.head_dim;
+    const cuuint64_t dims[3] = {64, (cuuint64_t)c.pages << c.shift, width / 64}, strides[2] = {width * sizeof(__half), 128};
+    const cuuint32_t boxes[3] = {64, (cuuint32_t)box, (cuuint32_t)blocks}, step[3] = {1, 1, 1};
+    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half *>(pool), dims, strides, boxes, step,
                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? 0 : cudaErrorInvalidValue;
@@ -978,8 +968,8 @@ extern "C" int qg_tree_attention(float *out, const float *q, const qg_kv_cache *
     a.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + 256);
     a.part_acc = reinterpret_cast<float *>(static_cast<char *>(workspace) + 256 + ml_bytes(a.part_rows));
     CUtensorMap k_map, v_map;
-    if (int rc = pool_map(&k_map, a.c, a.c.k, a.k_box)) return rc;
-    if (int rc = pool_map(&v_map, a.c, a.c.v, a.v_box)) return rc;
+    if (int rc = pool_map(&k_map, a.c, a.c.k, a.k_box, 1)) return rc;
+    if (int rc = pool_map(&v_map, a.c, a.c.v, a.v_box, a.c.head_dim / 64)) return rc;
     // Few rows: heads of 64 and 128 values, whose units take little time, share a unit's keys among copies of Q; heads of
     // 256 keep only 64 rows of Q, and the room goes to the ring.
     const int rows = tokens * a.group;
