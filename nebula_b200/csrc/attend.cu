@@ -67,16 +67,17 @@ struct Cfg {
     static constexpr int kPlane = kChunks * kBlock;
     // The rings' pieces: 64 columns of 128 keys, or all columns of kVKeys values; kChunks pieces for a unit's keys or values.
     static constexpr int kVKeys = kStage / (2 * D);
-    static constexpr int kKStages = D == 256 ? (MR == 64 ? 5 : 3) : D == 128 ? 5 : 6, kVStages = kKStages;
-    static constexpr int kStages = kKStages + kVStages;
-    static constexpr int kSmem = 2 * kPlane + kStages * kStage + 3072;
+    // Two places for Q where there is room: the next item's is prepared while this one's is in use.
+    static constexpr int kQBufs = 4 * kPlane <= 131072 ? 2 : 1;
+    static constexpr int kKStages = (232448 - 3072 - kQBufs * 2 * kPlane) / (2 * kStage), kVStages = kKStages;
+    static constexpr int kSmem = kQBufs * 2 * kPlane + (kKStages + kVStages) * kStage + 3072;
     static constexpr int kS = 256;  // tensor memory columns: O, then two of S (P takes its place)
 };
 
 struct Shared {
     float val[2][kRows];    // rescaling factors, and at an item's end the totals: softmax -> accumulators
-    float q_scale[kRows];   // at an item's end the maxima
-    uint64_t k_full[6], k_empty[6], v_full[6], v_empty[6], s_full[2], p_full[2][kKeys / kChunk], pv_done[2], msg_full[2], msg_empty[2], o_full, o_empty, q_full, landed, clean, drain;
+    float q_scale[2][kRows];  // at an item's end the maxima
+    uint64_t k_full[7], k_empty[7], v_full[7], v_empty[7], s_full[2], p_full[2][kKeys / kChunk], pv_done[2], msg_full[2], msg_empty[2], o_full, o_empty, q_full[2], landed, clean, drain;
     int pages[2][2][8];     // of the units that the producers are at: keys, values
     uint64_t odd_nodes;     // nodes whose values are not finite
     long long unit0, unit1;
@@ -291,9 +292,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                                                                      const __grid_constant__ CUtensorMap k_map,
                                                                      const __grid_constant__ CUtensorMap v_map) {
     using C = Cfg<D, MR>;
-    constexpr int NC = C::kChunks, NK = C::kKStages, NV = C::kVStages, VK = C::kVKeys;
+    constexpr int NC = C::kChunks, NK = C::kKStages, NV = C::kVStages, VK = C::kVKeys, QB = C::kQBufs;
     extern __shared__ __align__(1024) unsigned char smem[];  // swizzled tiles start on multiples of 1024
-    unsigned char *q_smem = smem, *k_ring = smem + 2 * C::kPlane, *v_ring = k_ring + NK * kStage;
+    unsigned char *q_smem = smem, *k_ring = smem + QB * 2 * C::kPlane, *v_ring = k_ring + NK * kStage;
     Shared &s = *reinterpret_cast<Shared *>(v_ring + NV * kStage);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     volatile int *abort = &s.abort;
@@ -331,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             mbar_init(&s.msg_full[i], 4), mbar_init(&s.msg_empty[i], 8);
             for (int k = 0; k < kKeys / kChunk; k++) mbar_init(&s.p_full[i][k], 4);
         }
-        mbar_init(&s.o_full, 1), mbar_init(&s.o_empty, 8), mbar_init(&s.q_full, 8), mbar_init(&s.drain, 2);
+        mbar_init(&s.o_full, 1), mbar_init(&s.o_empty, 8), mbar_init(&s.q_full[0], 8), mbar_init(&s.q_full[1], 8), mbar_init(&s.drain, 2);
         mbar_init(&s.landed, 1), mbar_init(&s.clean, 8);
         fence_mbar_init();
     } else if (warp == 3 && lane == 0) {
@@ -407,7 +408,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             const uint64_t q_lo = operand(smem_u32(q_smem) + C::kPlane, 16);
             const uint64_t q_hi = operand(smem_u32(q_smem), 16);
             while (ok && walk.next(a, it)) {
-                ok = wait(&s.q_full, item & 1, abort, a.err);
+                const uint32_t qb = item % QB;
+                ok = wait(&s.q_full[qb], item / QB & 1, abort, a.err);
                 for (int j = 0; ok && j < it.count; j++, tile++) {
                     const uint32_t buf = tile & 1, d = tmem + C::kS + buf * kKeys;
                     if (tile >= 2) ok = wait(&s.pv_done[buf], (tile / 2 - 1) & 1, abort, a.err);
@@ -419,10 +421,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                         const uint64_t kd = operand(smem_u32(k_ring + st * kStage), 16);
 #pragma unroll
                         for (int k = 0; k < 4; k++)
-                            mma_ss(d, q_lo + c * (C::kBlock / 16) + 2 * k, kd + 2 * k, idesc(kKeys, false), c + k > 0);
+                            mma_ss(d, q_lo + qb * (2 * C::kPlane / 16) + c * (C::kBlock / 16) + 2 * k, kd + 2 * k, idesc(kKeys, false), c + k > 0);
 #pragma unroll
                         for (int k = 0; k < 4; k++)
-                            mma_ss(d, q_hi + c * (C::kBlock / 16) + 2 * k, kd + 2 * k, idesc(kKeys, false), true);
+                            mma_ss(d, q_hi + qb * (2 * C::kPlane / 16) + c * (C::kBlock / 16) + 2 * k, kd + 2 * k, idesc(kKeys, false), true);
                         commit(&s.k_empty[st]);
                         if (++st == NK) st = 0, round++;
                     }
@@ -478,21 +480,22 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         // With few rows (a.copies 2 or 4) Q lies in the tile several times, and each copy takes its share of a unit's
         // keys: a running maximum and total of its own, P = 0 for the others' keys, joined at the end of the item.
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-        const int row = tid - 128, span = kRows / a.copies, copy = row / span, chunks = kKeys / kChunk / a.copies;
+        const int row = tid - 128, span = MR / a.copies, copy = row / span, chunks = kKeys / kChunk / a.copies;
         const int h0 = copy * chunks, h1 = h0 + chunks;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // tensor memory lane of the warp's first row, in bits 16+
         uint32_t tile = 0, item = 0, msg = 0;
         bool ok = true;
         while (ok && walk.next(a, it)) {
             const int r = it.tile * kRows + row % span, node = r / a.group;
-            const bool live = (row & ~31) % span + it.tile * kRows < a.tokens * a.group;  // the warp has rows
+            const bool live = row < MR && (row & ~31) % span + it.tile * kRows < a.tokens * a.group;  // the warp has rows
             uint64_t mask = 0;
             if (node < a.tokens) {
                 mask = a.tree ? a.tree[(size_t)it.seq * a.tokens + node] : ~0ull >> (63 - node);
                 if (a.tokens < 64) mask &= (1ull << a.tokens) - 1;
             }
-            ok = wait_warp(&s.q_full, item & 1, abort, a.err);
-            const float c = s.q_scale[row];
+            const uint32_t qb = item % QB;
+            ok = wait_warp(&s.q_full[qb], item / QB & 1, abort, a.err);
+            const float c = s.q_scale[qb][row];
             float m = -INFINITY, l = 0.0f, l_low = 0.0f;
             for (int j = 0; ok && j < it.count; j++, tile++) {
                 const uint32_t buf = tile & 1, cols = tmem + lanes + C::kS + buf * kKeys;
@@ -591,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             ok = !group_any(1, 128, !ok);  // the four warps stop together
             if (!ok) break;
             s.val[slot][row] = l;
-            s.q_scale[row] = m;
+            s.q_scale[qb][row] = m;
             __syncwarp();
             if (lane == 0) arrive(&s.msg_full[slot]);
             msg++;
@@ -601,74 +604,88 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         // ---------------------------------------------------- Q, and the accumulators: rows x half of the columns
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsAcc));
         constexpr int H = D / 2, V = D / 32;
-        const int w = warp - 8, row = (warp & 3) * 32 + lane, col0 = (w >> 2) * H, span = kRows / a.copies;
+        const int w = warp - 8, row = (warp & 3) * 32 + lane, col0 = (w >> 2) * H, span = MR / a.copies;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
         uint32_t piece0 = 0, tile = 0, msg = 0, cleans = 0;
-        bool ok = true;
-        while (ok && walk.next(a, it)) {
-            // Warp w prepares, and at the end stores, rows w, w+8, ...; lane i < 16 knows where row w+8i lies in q and
-            // out. Rows past the last are left as they are: no one reads their results.
-            const int rows = min(kRows, a.tokens * a.group - it.tile * kRows);
-            const bool live = (row & ~31) % span < rows;  // the warp has rows
-            size_t where = 0;
-            {
-                const int r = it.tile * kRows + w + 8 * (lane & 15), node = r / a.group;
-                if (node < a.tokens)
-                    where = (((size_t)it.seq * a.tokens + node) * a.q_heads + it.kv * a.group + (r - node * a.group)) * D;
-            }
-#pragma unroll 1
-            for (int i0 = 0; w + 8 * i0 < rows; i0 += 4) {  // lane l holds values V*l .. V*l+V-1 of four rows
-                float x[4][V];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float *src = a.q + __shfl_sync(0xffffffffu, where, i0 + i) + lane * V;
-                    if constexpr (V == 2) {
-                        *reinterpret_cast<float2 *>(x[i]) = __ldg(reinterpret_cast<const float2 *>(src));
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < V; e += 4) *reinterpret_cast<float4 *>(x[i] + e) = __ldg(reinterpret_cast<const float4 *>(src + e));
-                    }
+        // Every round prepares Q of one item and works through one: the same, or with two places for Q the one before.
+        Item nx;
+        size_t where_nx = 0, where = 0;
+        bool ok = true, more = walk.next(a, nx), left = false;
+        for (uint32_t round = 0; ok && (more || left); round++) {
+            if (more) {
+                // Warp w prepares, and at the end stores, rows w, w+8, ...; lane i < 16 knows where row w+8i lies in q
+                // and out. Rows past the last are left as they are: no one reads their results.
+                const int rows = min(kRows, a.tokens * a.group - nx.tile * kRows);
+                {
+                    const int r = nx.tile * kRows + w + 8 * (lane & 15), node = r / a.group;
+                    where_nx = node < a.tokens ? (((size_t)nx.seq * a.tokens + node) * a.q_heads + nx.kv * a.group + (r - node * a.group)) * D : 0;
                 }
+                const uint32_t qb = round % QB;
+                unsigned char *q_to = q_smem + qb * 2 * C::kPlane;
+#pragma unroll 1
+                for (int i0 = 0; w + 8 * i0 < rows; i0 += 4) {  // lane l holds values V*l .. V*l+V-1 of four rows
+                    float x[4][V];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int r = w + 8 * (i0 + i);
-                    float mx = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < V; e++) mx = fmaxf(mx, fabsf(x[i][e]));
-                    // of values that are not negative the bit patterns have the same order
-                    mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
-                    float up, inv;
-                    pow2_scale(mx, up, inv);
-                    up *= a.sign;
-                    uint32_t hi[V / 2], lo[V / 2];
-#pragma unroll
-                    for (int e = 0; e < V / 2; e++) {
-                        const float p = x[i][2 * e] * up, q = x[i][2 * e + 1] * up;
-                        hi[e] = pack_half(p, q);
-                        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[e]));
-                        lo[e] = pack_half(p - f.x, q - f.y);
-                    }
-                    if (r >= rows) continue;
-                    const int at = lane * V, unit = (at % 64) / 8;
-                    for (int rr = r; rr < kRows; rr += span) {
-                        if (lane == 0) s.q_scale[rr] = fmaxf(a.scale * inv, 1e-44f);  // never 0: -infinity stays what it is
-                        unsigned char *dst = q_smem + (at / 64) * C::kBlock + rr * 128 + ((unit ^ (rr & 7)) << 4) + (at % 8) * 2;
-                        if constexpr (V == 8) {
-                            *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                            *reinterpret_cast<uint4 *>(dst + C::kPlane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                        } else if constexpr (V == 4) {
-                            *reinterpret_cast<uint2 *>(dst) = make_uint2(hi[0], hi[1]);
-                            *reinterpret_cast<uint2 *>(dst + C::kPlane) = make_uint2(lo[0], lo[1]);
+                    for (int i = 0; i < 4; i++) {
+                        const float *src = a.q + __shfl_sync(0xffffffffu, where_nx, i0 + i) + lane * V;
+                        if constexpr (V == 2) {
+                            *reinterpret_cast<float2 *>(x[i]) = __ldg(reinterpret_cast<const float2 *>(src));
                         } else {
-                            *reinterpret_cast<uint32_t *>(dst) = hi[0];
-                            *reinterpret_cast<uint32_t *>(dst + C::kPlane) = lo[0];
+#pragma unroll
+                            for (int e = 0; e < V; e += 4) *reinterpret_cast<float4 *>(x[i] + e) = __ldg(reinterpret_cast<const float4 *>(src + e));
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int r = w + 8 * (i0 + i);
+                        float mx = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < V; e++) mx = fmaxf(mx, fabsf(x[i][e]));
+                        // of values that are not negative the bit patterns have the same order
+                        mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
+                        float up, inv;
+                        pow2_scale(mx, up, inv);
+                        up *= a.sign;
+                        uint32_t hi[V / 2], lo[V / 2];
+#pragma unroll
+                        for (int e = 0; e < V / 2; e++) {
+                            const float p = x[i][2 * e] * up, q = x[i][2 * e + 1] * up;
+                            hi[e] = pack_half(p, q);
+                            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[e]));
+                            lo[e] = pack_half(p - f.x, q - f.y);
+                        }
+                        if (r >= rows) continue;
+                        const int at = lane * V, unit = (at % 64) / 8;
+                        for (int rr = r; rr < MR; rr += span) {
+                            if (lane == 0) s.q_scale[qb][rr] = fmaxf(a.scale * inv, 1e-44f);  // never 0: -infinity stays what it is
+                            unsigned char *dst = q_to + (at / 64) * C::kBlock + rr * 128 + ((unit ^ (rr & 7)) << 4) + (at % 8) * 2;
+                            if constexpr (V == 8) {
+                                *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                                *reinterpret_cast<uint4 *>(dst + C::kPlane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                            } else if constexpr (V == 4) {
+                                *reinterpret_cast<uint2 *>(dst) = make_uint2(hi[0], hi[1]);
+                                *reinterpret_cast<uint2 *>(dst + C::kPlane) = make_uint2(lo[0], lo[1]);
+                            } else {
+                                *reinterpret_cast<uint32_t *>(dst) = hi[0];
+                                *reinterpret_cast<uint32_t *>(dst + C::kPlane) = lo[0];
+                            }
                         }
                     }
                 }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) arrive(&s.q_full[qb]);
             }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) arrive(&s.q_full);
+            if (QB == 2 && !left) {  // the first round only prepares
+                it = nx, where = where_nx, left = more;
+                more = more && walk.next(a, nx);
+                continue;
+            }
+            if (QB == 1) it = nx, where = where_nx;
+            const uint32_t qb = QB == 2 ? (round - 1) % 2 : 0;
+            const int rows = min(kRows, a.tokens * a.group - it.tile * kRows);
+            const bool live = (row & ~31) % span < rows && row < MR;  // the warp has rows
+            unsigned char *stage = q_smem + qb * 2 * C::kPlane;
             // pages of the item, checked
             bool bad = false;
             const int last = min((it.first + it.count) * kKeys, it.length + a.tokens) - 1;
@@ -738,8 +755,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             const uint32_t slot = msg & 1;
             if (ok) ok = wait_warp(&s.msg_full[slot], (msg / 2) & 1, abort, a.err);
             // The rows go through Q's place, 16-byte units turned by the row's low bits, so that whole rows are stored.
-            if (ok && row < MR && live) {
-                unsigned char *mine = q_smem + (size_t)row * D * 4;
+            if (ok && live) {
+                unsigned char *mine = stage + (size_t)row * D * 4;
 #pragma unroll
                 for (int i = 0; i < H / 4; i++)
                     *reinterpret_cast<float4 *>(mine + (((col0 / 4 + i) ^ (row & 7)) << 4)) =
@@ -775,12 +792,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 const size_t at = __shfl_sync(0xffffffffu, where, i);
                 // the copies' maxima and totals become one
                 float m = -INFINITY, l = 0.0f, f[4];
-                for (int k = 0; k < a.copies; k++) m = fmaxf(m, s.q_scale[r + k * span]);
+                for (int k = 0; k < a.copies; k++) m = fmaxf(m, s.q_scale[qb][r + k * span]);
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     f[k] = 0.0f;
                     if (k < a.copies) {
-                        const float mk = s.q_scale[r + k * span], lk = s.val[slot][r + k * span];
+                        const float mk = s.q_scale[qb][r + k * span], lk = s.val[slot][r + k * span];
                         f[k] = mk == -INFINITY ? lk : ex2(mk - m);  // lk is 0 (nothing seen) or NaN
                         l += f[k] * lk;
                     }
@@ -795,7 +812,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
 #pragma unroll
                     for (int k = 0; k < 4; k++)
                         if (k < a.copies) {
-                            const float4 x = *reinterpret_cast<const float4 *>(q_smem + (size_t)(r + k * span) * D * 4 + ((u ^ (r & 7)) << 4));
+                            const float4 x = *reinterpret_cast<const float4 *>(stage + (size_t)(r + k * span) * D * 4 + ((u ^ (r & 7)) << 4));
                             v.x += f[k] * x.x, v.y += f[k] * x.y, v.z += f[k] * x.z, v.w += f[k] * x.w;
                         }
                     reinterpret_cast<float4 *>(dst)[u] = make_float4(v.x * mul, v.y * mul, v.z * mul, v.w * mul);
@@ -806,6 +823,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             msg++;
             piece0 += value_pieces<C>(a, it);
             group_sync(4, 256);  // Q's place is free again
+            if (QB == 2) it = nx, where = where_nx, left = more;
+            more = more && walk.next(a, nx);
         }
         // refused sequences
         for (int q = blockIdx.x; q < a.seqs; q += gridDim.x)
@@ -975,6 +994,10 @@ extern "C" int qg_tree_attention(float *out, const float *q, const qg_kv_cache *
     const int rows = tokens * a.group;
     a.copies = a.c.head_dim == 256 || rows > 64 ? 1 : rows > 32 ? 2 : 4;
     if (a.c.head_dim == 64) return launch<64, 128>(a, k_map, v_map);
+    if (a.c.head_dim == 128 && rows <= 32) {
+        a.copies = 2;
+        return launch<128, 64>(a, k_map, v_map);
+    }
     if (a.c.head_dim == 128) return launch<128, 128>(a, k_map, v_map);
     return rows <= 64 ? launch<256, 64>(a, k_map, v_map) : launch<256, 128>(a, k_map, v_map);
 }
