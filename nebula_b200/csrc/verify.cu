@@ -24,7 +24,8 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int kMaxVocab = 1 << 24;
-constexpr int kChunk = 4096, kThreads = 256, kPer = kChunk / kThreads;
+constexpr int kChunk = 4096;
+constexpr int kChunkThreads = 256, kWalkThreads = 512;
 constexpr int kDrawnCtas = 8;  // CTAs per sequence that sum max(p - q, 0)
 
 // Of a chunk, or of a row.
@@ -69,129 +70,159 @@ __device__ __forceinline__ float weight(float scale, const Stats &r, float x, in
     return weigh(f, n - r.top);
 }
 
-// Two parts of a row as one. The order of equal logits: the lower index.
-__device__ __forceinline__ Stats join(const Stats &a, const Stats &b, bool greedy) {
-    Stats r;
-    if (a.best == kBad || b.best == kBad) return {0.0, 0.0f, kBad};
-    if (a.best == kNone) return b;
-    if (b.best == kNone) return a;
-    if (greedy) return a.top > b.top || (a.top == b.top && a.best < b.best) ? a : b;
-    r.top = fmaxf(a.top, b.top);
-    r.sum = a.sum * shift_down(a.top - r.top) + b.sum * shift_down(b.top - r.top);
-    r.best = 0;
-    return r;
-}
-__device__ __forceinline__ Stats shuffled(const Stats &a, int d) {
-    return {__shfl_xor_sync(0xffffffffu, a.sum, d), __shfl_xor_sync(0xffffffffu, a.top, d), __shfl_xor_sync(0xffffffffu, a.best, d)};
-}
-__device__ __forceinline__ Stats warp_join(Stats a, bool greedy) {
-#pragma unroll
-    for (int d = 16; d; d >>= 1) a = join(a, shuffled(a, d), greedy);
-    return a;
-}
+// A part of a row brought to the row's M.
+__device__ __forceinline__ double brought(const Stats &s, float top) { return s.sum * shift_down(s.top - top); }
 
-// Chunks begin at the row's first 16-byte boundary at or before its start (when the logits are 16-byte aligned), so a
-// thread loads four values at once; `v` of the first is then up to three before the row.
+// Chunks begin at the row's last 16-byte boundary at or before its start, up to three values before the row, so that a
+// thread loads four values at once.
 __device__ __forceinline__ int chunk_lead(const float *row) { return (int)(reinterpret_cast<uintptr_t>(row) / 4 % 4); }
-
-// The thread's kPer values of chunk c; out: their positions in the row are first + 4*kThreads*(i/4) + i%4, those
-// outside the row -infinity.
-__device__ __forceinline__ void load_chunk(const float *row, int vocab, int c, float (&x)[kPer], int &first, float outside) {
-    first = c * kChunk - chunk_lead(row) + 4 * (int)threadIdx.x;
+// Four values from position v on, those outside the row -infinity.
+__device__ __forceinline__ void load4(const float *row, int vocab, int v, float (&x)[4]) {
+    if (v >= 0 && v + 4 <= vocab && !(reinterpret_cast<uintptr_t>(row + v) & 15)) {
+        *reinterpret_cast<float4 *>(x) = __ldg(reinterpret_cast<const float4 *>(row + v));
+    } else {
 #pragma unroll
-    for (int i = 0; i < kPer / 4; i++) {
-        const int v = first + 4 * kThreads * i;
-        if (v >= 0 && v + 4 <= vocab) {
-            *reinterpret_cast<float4 *>(x + 4 * i) = __ldg(reinterpret_cast<const float4 *>(row + v));
-        } else {
-#pragma unroll
-            for (int k = 0; k < 4; k++) x[4 * i + k] = v + k >= 0 && v + k < vocab ? __ldg(row + v + k) : outside;
-        }
+        for (int k = 0; k < 4; k++) x[k] = v + k >= 0 && v + k < vocab ? __ldg(row + v + k) : -INFINITY;
     }
 }
-__device__ __forceinline__ int place(int first, int i) { return first + 4 * kThreads * (i / 4) + i % 4; }
 
-template <bool GREEDY>
-__global__ void __launch_bounds__(kThreads) chunk_kernel(const VerifyArgs a) {
-    __shared__ Stats part[kThreads / 32];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int c = blockIdx.x % a.chunks, row = blockIdx.x / a.chunks;
-    float x[kPer];
-    int first;
-    load_chunk(a.logits + (size_t)row * a.vocab, a.vocab, c, x, first, -INFINITY);
-    bool bad = false;
-    Stats s = {0.0, -INFINITY, kNone};
-    if (GREEDY) {
+__device__ __forceinline__ double warp_sum(double x) {
 #pragma unroll
-        for (int i = 0; i < kPer; i++) {
-            bad |= !(x[i] < INFINITY);
-            if (x[i] > s.top) s.top = x[i], s.best = place(first, i);
-        }
-    } else {
-        float n[kPer];
+    for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    return x;
+}
+// Floats in order as integers.
+__device__ __forceinline__ int ordered(float x) {
+    const int b = __float_as_int(x);
+    return b < 0 ? b ^ 0x7fffffff : b;
+}
+__device__ __forceinline__ float warp_max(float x) {
+    const int m = __reduce_max_sync(0xffffffffu, ordered(x));
+    return __int_as_float(m < 0 ? m ^ 0x7fffffff : m);
+}
+
+// Of 8 values of a thread: the largest n, and the sum of the weights relative to it. Conversions and floor run at an
+// eighth of the rate of additions here and would bound the kernel (50 us instead of the copy's 17 for 12 x 17 x
+// 131072 logits), so for |t| < 2^21 floor comes from rounding by an addition, n is read from that sum's bits, and 2^f
+// 2^(n - top) is put together as the bits of a double.
+__device__ __forceinline__ void weigh8(const float (&x)[8], float scale, float &top, double &sum) {
+    constexpr float kMagic = 12582912.0f, kRange = 2097152.0f;  // 1.5 * 2^23, 2^21
+    float t[8], most = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kPer; i++) {
-            bad |= !(x[i] < INFINITY);
-            n[i] = -INFINITY;
-            if (x[i] > -INFINITY) n[i] = split(x[i], a.scale, x[i]);
-            s.top = fmaxf(s.top, n[i]);
-        }
-        if (s.top > -INFINITY) {
-            s.best = 0;
-#pragma unroll
-            for (int i = 0; i < kPer; i++) s.sum += (double)(n[i] > -INFINITY ? weigh(x[i], n[i] - s.top) : 0.0f);
-        }
+    for (int i = 0; i < 8; i++) {
+        t[i] = __fmul_rn(x[i], scale);
+        most = fmaxf(most, t[i]);
     }
-    if (bad) s.best = kBad;
-    s = warp_join(s, GREEDY);
-    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = s;
+    top = -INFINITY;
+    sum = 0.0;
+    if (most < kRange && most > -kRange / 2) {
+        int n[8], m = -0x7fffffff;
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float tc = fmaxf(t[i], -kRange), u = __fadd_rn(tc, kMagic), d = __fsub_rn(tc, __fsub_rn(u, kMagic));
+            const bool up = d < 0.0f;  // u rounded up
+            n[i] = __float_as_int(u) - (up ? 1 : 0);
+            f[i] = up ? __fadd_rn(d, 1.0f) : d;
+            m = max(m, n[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const unsigned g = __float_as_uint(exp2f(f[i]));  // in [1, 2]
+            const int rel = max(n[i] - m, -900);              // 2^-900 is nothing beside the largest
+            sum += __hiloint2double((int)((g >> 3) + ((1023 - 127) << 20)) + (rel << 20), (int)(g << 29));
+        }
+        top = (float)(m - __float_as_int(kMagic));
+    } else {
+        float n[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            n[i] = -INFINITY;
+            if (x[i] > -INFINITY) n[i] = split(x[i], scale, t[i]);
+            top = fmaxf(top, n[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) sum += (double)(n[i] > -INFINITY ? weigh(t[i], n[i] - top) : 0.0f);
+    }
+}
+
+// GREEDY: temperature 0, only the largest logit and its lowest index.
+template <bool GREEDY>
+__global__ void __launch_bounds__(kChunkThreads) chunk_kernel(const VerifyArgs a) {
+    constexpr int kWarps = kChunkThreads / 32;
+    __shared__ double sums[kWarps];
+    __shared__ float tops[kWarps];
+    __shared__ int bests[kWarps];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int c = blockIdx.x % a.chunks, r = blockIdx.x / a.chunks, warp = threadIdx.x / 32;
+    const float *row = a.logits + (size_t)r * a.vocab;
+    const int first = c * kChunk - chunk_lead(row) + 4 * (int)threadIdx.x;
+    float x[2][8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) load4(row, a.vocab, first + 4 * kChunkThreads * i, *reinterpret_cast<float(*)[4]>(&x[i / 2][i % 2 * 4]));
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 16; i++) bad |= !(x[i / 8][i % 8] < INFINITY);
+    bad = __any_sync(0xffffffffu, bad);
+    if constexpr (GREEDY) {
+        float top = -INFINITY;
+        int best = 0x7fffffff;
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            if (x[i / 8][i % 8] > top) top = x[i / 8][i % 8], best = first + 4 * kChunkThreads * (i / 4) + i % 4;
+        const float m = warp_max(top + 0.0f);  // -0 and 0 are equals
+        best = __reduce_min_sync(0xffffffffu, top == m && top > -INFINITY ? best : 0x7fffffff);
+        if (threadIdx.x % 32 == 0) tops[warp] = m, bests[warp] = bad ? kBad : m > -INFINITY ? best : kNone;
+    } else {
+        float t0, t1;
+        double s0, s1;
+        weigh8(x[0], a.scale, t0, s0);
+        weigh8(x[1], a.scale, t1, s1);
+        const float m = warp_max(fmaxf(t0, t1));
+        double sum = 0.0;
+        if (m > -INFINITY) sum = warp_sum(s0 * shift_down(t0 - m) + s1 * shift_down(t1 - m));
+        if (threadIdx.x % 32 == 0) tops[warp] = m, sums[warp] = sum, bests[warp] = bad ? kBad : m > -INFINITY ? 0 : kNone;
+    }
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < kThreads / 32; w++) s = join(s, part[w], GREEDY);
+        Stats s = {0.0, -INFINITY, kNone};
+        for (int w = 0; w < kWarps; w++) {
+            if (bests[w] == kBad) bad = true;
+            if (tops[w] > s.top || (tops[w] == s.top && bests[w] >= 0 && bests[w] < s.best)) s.top = tops[w], s.best = bests[w];
+        }
+        if (!GREEDY)
+            for (int w = 0; w < kWarps; w++) s.sum += sums[w] * shift_down(tops[w] - s.top);
+        if (bad) s.best = kBad;
         a.stats[blockIdx.x] = s;
     }
 }
 
-// The running sum of x over the CTA's threads, and its total.
-__device__ double block_scan(double x, double *buf, double &total) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// The running sum of x over a warp.
+__device__ __forceinline__ double warp_scan(double x) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
         const double up = __shfl_up_sync(0xffffffffu, x, d);
         if (lane >= d) x += up;
     }
-    __syncthreads();
-    if (lane == 31) buf[warp] = x;
-    __syncthreads();
-    total = 0.0;
-    double before = 0.0;
-    for (int w = 0; w < kThreads / 32; w++) {
-        before = w == warp ? total : before;
-        total += buf[w];
-    }
-    return before + x;
+    return x;
 }
-
-// The first thread whose running sum passes the aim, or where rounding leaves none the last that has any weight; -1: no
-// weight at all. (`has`: the thread has weight.)
-__device__ int claim(bool has, bool passes, int *buf) {
-    if (threadIdx.x == 0) buf[0] = kThreads, buf[1] = -1;
-    __syncthreads();
-    if (has && passes) atomicMin(&buf[0], (int)threadIdx.x);
-    if (has) atomicMax(&buf[1], (int)threadIdx.x);
-    __syncthreads();
-    return buf[0] < kThreads ? buf[0] : buf[1];
+// The lane at which a running sum (`upto`, of parts that are not negative) passes the aim; where rounding leaves none,
+// the last that has any weight. -1: no weight at all.
+__device__ __forceinline__ int claim(double part, double upto, double aim) {
+    const unsigned has = __ballot_sync(0xffffffffu, part > 0.0), passes = __ballot_sync(0xffffffffu, part > 0.0 && aim < upto);
+    return passes ? __ffs(passes) - 1 : has ? 31 - __clz(has) : -1;
 }
 
 // DRAWN: the drafts' distributions are given; a cluster of kDrawnCtas CTAs per sequence, otherwise one CTA.
 template <bool DRAWN>
-__global__ void __launch_bounds__(kThreads) walk_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) {
+    constexpr int kWarps = kWalkThreads / 32, kCtas = DRAWN ? kDrawnCtas : 1;
+    static_assert(kWalkThreads * 8 == kChunk, "eight values of a chunk to a thread");
     __shared__ Stats rows[kMaxNodes];
-    __shared__ double buf[kThreads / 32];
-    __shared__ float mine[kMaxNodes], guess[kMaxNodes], uniform[kMaxNodes], values[kChunk + kChunk / 16];
-    __shared__ int draft[kMaxNodes], parent[kMaxNodes], gone[kMaxNodes], path[kMaxNodes], n_gone, count, at_node, refused, picked, found[2];
-    __shared__ double before_chunk;
-    constexpr int kCtas = DRAWN ? kDrawnCtas : 1;
+    __shared__ double sums[kWarps];
+    __shared__ float mine[kMaxNodes], guess[kMaxNodes], uniform[kMaxNodes];
+    __shared__ int draft[kMaxNodes], parent[kMaxNodes], gone[kMaxNodes], path[kMaxNodes], n_gone, count, at_node, refused;
     const int seq = blockIdx.x / kCtas, rank = blockIdx.x % kCtas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const size_t base = (size_t)seq * a.tokens;
     const bool greedy = a.scale == 0.0f;
@@ -208,16 +239,36 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const VerifyArgs a) {
     const float x = tries ? a.logits[above * a.vocab + draft[tid]] : 0.0f;
     if (DRAWN && tries) guess[tid] = a.probs[(base + tid) * a.vocab + draft[tid]];
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (int r = warp; r < a.tokens; r += kThreads / 32) {
-        Stats s = {0.0, -INFINITY, kNone};
-        for (int c = lane; c < a.chunks; c += 32) s = join(s, a.stats[(base + r) * a.chunks + c], greedy);
-        s = warp_join(s, greedy);
-        if (greedy) s.sum = 1.0;
-        if (lane == 0) rows[r] = s;
+    // ---- the rows' M and total: a warp per row
+    for (int r = warp; r < a.tokens; r += kWarps) {
+        const Stats *part = a.stats + (base + r) * a.chunks;
+        float top = -INFINITY;
+        int best = 0x7fffffff, bad = 0;
+        double sum = 0.0;
+        for (int c = lane; c < a.chunks; c += 32) {
+            const Stats s = part[c];
+            bad |= s.best == kBad;
+            if (s.best < 0) continue;
+            if (s.top > top) {
+                sum *= shift_down(top - s.top);
+                top = s.top, best = s.best;
+            } else if (s.top == top && s.best < best) {
+                best = s.best;
+            }
+            sum += brought(s, top);
+        }
+        const float m = warp_max(top);
+        sum = m > -INFINITY ? warp_sum(sum * shift_down(top - m)) : 0.0;
+        best = __reduce_min_sync(0xffffffffu, top == m ? best : 0x7fffffff);
+        bad = __any_sync(0xffffffffu, bad);
+        if (lane == 0) rows[r] = {greedy ? 1.0 : sum, m, bad ? kBad : m > -INFINITY ? best : kNone};
     }
     __syncthreads();
-    if (tries) mine[tid] = weight(a.scale, rows[parent[tid]], x, draft[tid]);  // the target's weight of each draft
-    __syncthreads();
+    // ---- the walk
+    if (warp < kMaxNodes / 32) {
+        if (tries) mine[tid] = weight(a.scale, rows[parent[tid]], x, draft[tid]);  // the target's weight of each draft
+        asm volatile("bar.sync 1, 64;" ::: "memory");
+    }
     if (tid == 0) {
         int cur = 0, n = 0, child = -1, left_out = 0;
         bool ok = sound && rows[0].best >= 0;
@@ -231,8 +282,8 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const VerifyArgs a) {
             }
             float w = mine[c];
             bool take;
-            if (DRAWN) {
-                take = __fmul_rn(uniform[c], guess[c]) < w / (float)rows[cur].sum;
+            if constexpr (DRAWN) {
+                take = __fmul_rn(uniform[c], guess[c]) < w / (float)left;
             } else {
                 for (int g = 0; g < left_out; g++)
                     if (gone[g] == draft[c]) w = 0.0f;
@@ -247,15 +298,16 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const VerifyArgs a) {
                 left = rows[c].sum;
             } else {
                 child = c;
-                if (w > 0.0f) gone[left_out++] = draft[c];
-                left -= (double)w;
+                if constexpr (!DRAWN) {
+                    if (w > 0.0f) gone[left_out++] = draft[c];
+                    left -= (double)w;
+                }
             }
         }
         at_node = ok ? cur : -1;
         refused = child;
-        n_gone = DRAWN ? 0 : left_out;
+        n_gone = left_out;
         count = ok ? n : -1;
-        picked = -1;
     }
     __syncthreads();
     if (rank == 0) {
@@ -265,113 +317,129 @@ __global__ void __launch_bounds__(kThreads) walk_kernel(const VerifyArgs a) {
     }
     if (at_node < 0) return;  // the same in all CTAs of the cluster
 
+    // ---- what is left of the last node's row
     const float *row = a.logits + (base + at_node) * a.vocab;
     const Stats r = rows[at_node];
     const float total = (float)r.sum;
     const float *q = DRAWN && refused >= 0 ? a.probs + (base + refused) * a.vocab : nullptr;
-    // what is left of token v's weight
-    auto left = [&](float x, int v) -> float {
-        float w = weight(a.scale, r, x, v);
-        if constexpr (DRAWN) {
-            w /= total;
-            return q ? fmaxf(w - __ldg(q + v), 0.0f) : w;
-        } else {
-            for (int g = 0; g < n_gone; g++)
-                if (gone[g] == v) w = 0.0f;
-            return w;
+    const int lead = chunk_lead(row);
+    // the thread's eight neighbouring values of chunk c
+    auto left8 = [&](int c, float (&w)[8]) {
+        const int v = c * kChunk - lead + 8 * tid;
+        float y[8];
+        load4(row, a.vocab, v, *reinterpret_cast<float(*)[4]>(&w[0]));
+        load4(row, a.vocab, v + 4, *reinterpret_cast<float(*)[4]>(&w[4]));
+        if (DRAWN && q) {
+            load4(q, a.vocab, v, *reinterpret_cast<float(*)[4]>(&y[0]));
+            load4(q, a.vocab, v + 4, *reinterpret_cast<float(*)[4]>(&y[4]));
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            w[i] = weight(a.scale, r, w[i], v + i);  // none outside the row
+            if constexpr (DRAWN) {
+                w[i] /= total;
+                if (q) w[i] = v + i >= 0 && v + i < a.vocab ? fmaxf(w[i] - y[i], 0.0f) : 0.0f;
+            } else {
+                for (int g = 0; g < n_gone; g++)
+                    if (gone[g] == v + i) w[i] = 0.0f;
+            }
         }
     };
     double *rest = a.rest + (size_t)seq * a.chunks;
-    // ---- the chunks' sums, and the chunk that holds the aim
-    const int per = (a.chunks + kThreads - 1) / kThreads, c0 = tid * per, c1 = min(c0 + per, a.chunks);
-    double whole = 0.0, upto = 0.0, sum = 0.0;
     auto chunk_sum = [&](int c) -> double {
-        if constexpr (DRAWN) return __ldcg(rest + c);
-        const Stats s = a.stats[(base + at_node) * a.chunks + c];
-        if (greedy) return s.best == r.best ? 1.0 : 0.0;
-        double w = s.best >= 0 ? s.sum * shift_down(s.top - r.top) : 0.0;
-        const int lead = chunk_lead(row);
-        for (int g = 0; g < n_gone; g++)
-            if ((gone[g] + lead) / kChunk == c) w -= (double)weight(a.scale, r, row[gone[g]], gone[g]);
-        return fmax(w, 0.0);
+        if constexpr (DRAWN) {
+            return __ldcg(rest + c);
+        } else {
+            const Stats s = a.stats[(base + at_node) * a.chunks + c];
+            if (greedy) return s.best == r.best ? 1.0 : 0.0;
+            double w = s.best >= 0 ? brought(s, r.top) : 0.0;
+            for (int g = 0; g < n_gone; g++)
+                if ((gone[g] + lead) / kChunk == c) w -= (double)weight(a.scale, r, row[gone[g]], gone[g]);
+            return fmax(w, 0.0);
+        }
     };
+    // ---- the chunk that holds the aim: every warp finds it for itself, a lane takes neighbouring chunks
+    const int per = (a.chunks + 31) / 32, c0 = min(lane * per, a.chunks), c1 = min(c0 + per, a.chunks);
+    double whole = 0.0, upto = 0.0, sum = 0.0;
     for (;;) {
         if constexpr (DRAWN) {
             for (int c = rank; c < a.chunks; c += kCtas) {
-                float v[kPer];
-                int first;
-                load_chunk(row, a.vocab, c, v, first, -INFINITY);
+                float w[8];
+                left8(c, w);
                 double part = 0.0;
 #pragma unroll
-                for (int i = 0; i < kPer; i++) {
-                    const int at = place(first, i);
-                    if (at >= 0 && at < a.vocab) part += (double)left(v[i], at);
+                for (int i = 0; i < 8; i++) part += (double)w[i];
+                part = warp_sum(part);
+                __syncthreads();
+                if (lane == 0) sums[warp] = part;
+                __syncthreads();
+                if (tid == 0) {
+                    double all = 0.0;
+                    for (int k = 0; k < kWarps; k++) all += sums[k];
+                    __stcg(rest + c, all);
                 }
-                double all;
-                block_scan(part, buf, all);
-                if (tid == 0) __stcg(rest + c, all);
             }
-            cg::this_cluster().sync();  // the sums are there (and were read, before they are written again)
+            cg::this_cluster().sync();  // the sums are there
         }
         sum = 0.0;
         for (int c = c0; c < c1; c++) sum += chunk_sum(c);
-        upto = block_scan(sum, buf, whole);
+        upto = warp_scan(sum);
+        whole = __shfl_sync(0xffffffffu, upto, 31);
         if (!DRAWN || whole > 0.0 || !q) break;
         q = nullptr;  // the draft's distribution covers the target's: draw from the target's
-        cg::this_cluster().sync();
+        cg::this_cluster().sync();  // the sums were read
     }
     if (rank) return;
     const double aim = (double)uniform[0] * whole;
-    if (tid == claim(sum > 0.0, aim < upto, found)) {
-        double run = upto - sum;
-        for (int c = c0; c < c1; c++) {
-            const double w = chunk_sum(c);
-            if (w > 0.0) picked = c, before_chunk = run;
+    const int owner = claim(sum, upto, aim);
+    if (owner < 0) {  // not met: a row with a distribution has weight left, for what was refused was not all of it
+        if (tid == 0) a.next[seq] = -1;
+        return;
+    }
+    int c = c0;
+    double before = upto - sum;
+    if (lane == owner) {
+        double run = before;
+        for (int k = c0; k < c1; k++) {
+            const double w = chunk_sum(k);
+            if (w > 0.0) c = k, before = run;
             run += w;
             if (run > aim) break;
         }
     }
-    __syncthreads();
-    const int c = picked;  // a row with a distribution has weight left (what was refused was not all of it)
-    if (c < 0) {
-        if (tid == 0) a.next[seq] = -1;
-        return;
-    }
-    // ---- the place in the chunk: 16 values in a row to a thread
-    {
-        float v[kPer];
-        int first;
-        load_chunk(row, a.vocab, c, v, first, -INFINITY);
+    c = __shfl_sync(0xffffffffu, c, owner);
+    before = __shfl_sync(0xffffffffu, before, owner);
+    // ---- the place in the chunk
+    float w[8];
+    left8(c, w);
+    double part = 0.0;
 #pragma unroll
-        for (int i = 0; i < kPer; i++) {
-            const int at = place(first, i), in = at - first + 4 * tid;
-            values[in + in / 16] = at >= 0 && at < a.vocab ? left(v[i], at) : 0.0f;
-        }
-    }
+    for (int i = 0; i < 8; i++) part += (double)w[i];
+    double end = warp_scan(part);
     __syncthreads();
-    const double before = before_chunk;
-    double part = 0.0, all;
+    if (lane == 31) sums[warp] = end;
+    __syncthreads();
+    const double theirs = lane < kWarps ? sums[lane] : 0.0, ends = before + warp_scan(theirs);
+    if (claim(theirs, ends, aim) != warp) return;
+    end += __shfl_sync(0xffffffffu, ends - theirs, warp);
+    if (lane != claim(part, end, aim)) return;
+    double run = end - part;
+    int hit = 0;
+    bool past = false;
 #pragma unroll
-    for (int i = 0; i < 16; i++) part += (double)values[17 * tid + i];
-    const double end = before + block_scan(part, buf, all);
-    if (tid == claim(part > 0.0, aim < end, found)) {
-        double run = end - part;
-        int hit = 0;
-        for (int i = 0; i < 16; i++) {
-            const float w = values[17 * tid + i];
-            if (w > 0.0f) hit = i;
-            run += (double)w;
-            if (run > aim) break;
-        }
-        a.next[seq] = 16 * tid + hit + c * kChunk - chunk_lead(row);
+    for (int i = 0; i < 8; i++) {
+        if (!past && w[i] > 0.0f) hit = i;
+        run += (double)w[i];
+        past |= run > aim;
     }
+    a.next[seq] = c * kChunk - lead + 8 * tid + hit;
 }
 
 template <bool DRAWN>
 int launch_walk(const VerifyArgs &a, int seqs) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(seqs * (DRAWN ? kDrawnCtas : 1));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(kWalkThreads);
     cfg.stream = launch_stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -409,8 +477,8 @@ extern "C" int qg_verify_tree(int *path, int *accepted, int *next, const float *
     const VerifyArgs a = {path, accepted, next, logits, draft, parents, draft_probs, uniforms, scale, tokens, vocab, chunks, stats,
                           reinterpret_cast<double *>(stats + (size_t)seqs * tokens * chunks)};
     const unsigned grid = (unsigned)((size_t)seqs * tokens * chunks);
-    if (scale == 0.0f) chunk_kernel<true><<<grid, kThreads, 0, launch_stream>>>(a);
-    else chunk_kernel<false><<<grid, kThreads, 0, launch_stream>>>(a);
+    if (scale == 0.0f) chunk_kernel<true><<<grid, kChunkThreads, 0, launch_stream>>>(a);
+    else chunk_kernel<false><<<grid, kChunkThreads, 0, launch_stream>>>(a);
     if (int rc = cudaGetLastError()) return rc;
     return draft_probs ? launch_walk<true>(a, seqs) : launch_walk<false>(a, seqs);
 }
