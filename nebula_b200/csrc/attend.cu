@@ -443,9 +443,14 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     const uint32_t buf = tile & 1, p0 = tmem + C::kS + buf * kKeys;
                     const int keys = keys_of(a, it, j), past = it.length - (it.first + j) * kKeys;
                     if (tile >= 1) ok = wait(&s.o_empty, (tile - 1) & 1, abort, a.err);
-                    // 32 keys at a time, as the softmax delivers them; past the last key there is nothing
+                    // 32 keys at a time, as the softmax delivers them. Past the last key there is nothing to multiply, but
+                    // the softmax writes there too, and must be done before S takes the place again.
 #pragma unroll 1
-                    for (int h = 0; ok && h * kChunk < keys; h++) {
+                    for (int h = 0; ok && h < kKeys / kChunk; h++) {
+                        if (h * kChunk >= keys) {
+                            ok = wait(&s.p_full[buf][h], (tile / 2) & 1, abort, a.err);
+                            continue;
+                        }
                         const int row = h * kChunk % VK;
                         if (row == 0) ok = wait(&s.v_full[st], round & 1, abort, a.err);
                         if (ok && (h + 1) * kChunk > past) {  // nodes: the accumulator warps clean their values

@@ -105,6 +105,18 @@ def test_attention(L, hq, hkv, d, lengths, tokens, page, tree):
     assert_parity(got, expected(cache, q, masks, d ** -0.5))
 
 
+@pytest.mark.parametrize("hq,hkv,d,tokens", [(16, 4, 64, 25), (16, 4, 64, 32), (32, 8, 128, 25), (8, 2, 128, 9), (24, 2, 256, 5),
+                                             (24, 2, 256, 17), (8, 2, 256, 1)])
+def test_attention_many_short_sequences(L, hq, hkv, d, tokens):
+    """Several sequences to a CTA, one following the other while the last unit of the one before is still at work."""
+    rng = np.random.default_rng(d * tokens)
+    lengths = [int(n) for n in rng.integers(0, 700, 60)]
+    cache = Cache(L, rng, lengths, tokens, hkv, d, 64)
+    q = (1.5 * rng.normal(size=(len(lengths), tokens, hq, d))).astype(np.float32)
+    got = attend(L, cache, q, None, d ** -0.5, calls=3)
+    assert_parity(got, expected(cache, q, None, d ** -0.5))
+
+
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_attention_layers_and_large_scores(L, d):
     """The layer asked for is the one read; scores of some hundreds leave one key with all the weight."""
