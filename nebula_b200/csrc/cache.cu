@@ -25,72 +25,134 @@ struct PrepArgs {
     const int *offsets;
     int q_stride, k_stride, v_stride, rope_positions, half, tokens, q_heads, rows;
     float eps;
+    bool aligned;  // all rows of q, k, v, q_out and the weights start on 16-byte boundaries
 };
 
-// One warp per (row, head): query heads, then key heads, then value heads.
-// Lane l holds values l + 32j. The partner of a rotated value may sit in any
-// lane (rotary is any even number), so the normalised head goes through the
-// warp's part of shared memory.
+// W neighbouring floats; aligned: in one load. (Not through the read-only path: q may be q_out.)
+template <int W>
+__device__ __forceinline__ void load(float (&x)[W], const float *p, bool aligned) {
+    if (W == 4 && aligned) {
+        *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(p);
+    } else if (W == 2 && aligned) {
+        *reinterpret_cast<float2 *>(x) = *reinterpret_cast<const float2 *>(p);
+    } else {
+#pragma unroll
+        for (int e = 0; e < W; e++) x[e] = p[e];
+    }
+}
+
+// One warp per row and kHeads of its heads: query heads, then key heads, then
+// value heads. Lane l holds values W*l .. W*l+W-1 of each 128 (64 for heads of
+// 64) of a head. The heads' values are asked for first; the length, the page and
+// the table's angles, each of which depends on the one before, arrive meanwhile
+// and serve both heads (96 x 17 rows of 24 + 4 heads of 256: 24.6 us; one head to
+// a warp 28.9, four 24.9, each with the registers that keep five CTAs on an SM or
+// without, whichever was faster). The partner of a rotated value sits in
+// another lane, so the rotated part of the normalised head goes through the
+// warp's part of shared memory. Bound by HBM (by the launch for one verify batch).
+constexpr int kHeads = 2;
+
 template <int D>
-__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const PrepArgs a) {
-    constexpr int N = D / 32;
-    __shared__ float head[8][D];
+__global__ void __launch_bounds__(256, 5) qk_norm_rope_kernel(const __grid_constant__ PrepArgs a) {
+    constexpr int W = D == 64 ? 2 : 4, N = D / (32 * W);
+    __shared__ __align__(16) float head[8][D];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int heads = a.q_heads + 2 * a.c.kv_heads;
-    const long long item = (long long)blockIdx.x * 8 + warp;
-    if (item >= (long long)a.rows * heads) return;
-    const int row = (int)(item / heads), h = (int)(item % heads);
-    const int seq = row / a.tokens, node = row % a.tokens;
-    const bool is_q = h < a.q_heads, is_v = h >= a.q_heads + a.c.kv_heads;
-    const int kv = is_q ? 0 : (h - a.q_heads) % a.c.kv_heads;
-
+    const unsigned groups = (heads + kHeads - 1) / kHeads, item = blockIdx.x * 8 + warp;
+    if (item >= (unsigned)a.rows * groups) return;
+    const int row = item / groups, h0 = (item - row * groups) * kHeads, seq = row / a.tokens, node = row - seq * a.tokens;
+    float x[kHeads][N][W];
+#pragma unroll
+    for (int g = 0; g < kHeads; g++) {
+        const int h = min(h0 + g, heads - 1), k = h - a.q_heads, v = k - a.c.kv_heads;
+        const float *src = k < 0   ? a.q + (size_t)row * a.q_stride + (size_t)h * D
+                           : v < 0 ? a.k + (size_t)row * a.k_stride + (size_t)k * D
+                                   : a.v + (size_t)row * a.v_stride + (size_t)v * D;
+#pragma unroll
+        for (int j = 0; j < N; j++) load(x[g][j], src + 32 * W * j + W * lane, a.aligned);
+    }
     const int length = a.c.committed(seq, a.tokens);
     const int pos = length + (a.offsets ? a.offsets[row] : node);
     long long at = length < 0 ? -1 : a.c.row(seq, length + node);
     if (a.half && (unsigned)pos >= (unsigned)a.rope_positions) at = -1;
-    if (at < 0) {  // the header's refusals: NaN queries, no store
-        if (is_q)
-            for (int j = 0; j < N; j++)
-                a.q_out[((size_t)row * a.q_heads + h) * D + lane + 32 * j] = __int_as_float(0x7fc00000);
-        return;
-    }
-    const float *src = is_q ? a.q + (size_t)row * a.q_stride + (size_t)h * D
-                            : (is_v ? a.v + (size_t)row * a.v_stride : a.k + (size_t)row * a.k_stride) + (size_t)kv * D;
-    float x[N];
+    float2 turn[N][W];
 #pragma unroll
-    for (int j = 0; j < N; j++) x[j] = src[lane + 32 * j];
-    if (!is_v) {
-        float sum = 0.0f;
+    for (int j = 0; j < N; j++)
 #pragma unroll
-        for (int j = 0; j < N; j++) sum = fmaf(x[j], x[j], sum);
-#pragma unroll
-        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        const float inv = rsqrtf(sum * (1.0f / D) + a.eps);
-        const float *w = is_q ? a.q_weight : a.k_weight;
-#pragma unroll
-        for (int j = 0; j < N; j++) {
-            x[j] = x[j] * inv * w[lane + 32 * j];
-            head[warp][lane + 32 * j] = x[j];
+        for (int e = 0; e < W; e++) {
+            const int i = 32 * W * j + W * lane + e;
+            turn[j][e] = make_float2(1.0f, 0.0f);
+            if (at >= 0 && i < 2 * a.half) turn[j][e] = __ldg(a.rope + (size_t)pos * a.half + (i < a.half ? i : i - a.half));
         }
-        __syncwarp();
 #pragma unroll
-        for (int j = 0; j < N; j++) {
-            const int i = lane + 32 * j;
-            if (i < 2 * a.half) {
-                const bool low = i < a.half;
-                const float2 t = a.rope[(size_t)pos * a.half + (low ? i : i - a.half)];
-                const float other = head[warp][low ? i + a.half : i - a.half];
-                x[j] = low ? x[j] * t.x - other * t.y : x[j] * t.x + other * t.y;
+    for (int g = 0; g < kHeads; g++) {
+        const int h = h0 + g, k = h - a.q_heads, v = k - a.c.kv_heads;
+        if (h >= heads) break;
+        if (v < 0) {
+            const float *weight = (k < 0 ? a.q_weight : a.k_weight) + W * lane;
+            float w[N][W], sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                load(w[j], weight + 32 * W * j, a.aligned);
+#pragma unroll
+                for (int e = 0; e < W; e++) sum = fmaf(x[g][j][e], x[g][j][e], sum);
+            }
+#pragma unroll
+            for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            const float inv = rsqrtf(sum * (1.0f / D) + a.eps);
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < N; j++)
+#pragma unroll
+                for (int e = 0; e < W; e++) {
+                    x[g][j][e] = x[g][j][e] * inv * w[j][e];
+                }
+#pragma unroll
+            for (int j = 0; j < N; j++)
+                if (32 * W * j < 2 * a.half) {
+                    if constexpr (W == 4) *reinterpret_cast<float4 *>(&head[warp][32 * W * j + W * lane]) = *reinterpret_cast<float4 *>(x[g][j]);
+                    else *reinterpret_cast<float2 *>(&head[warp][32 * W * j + W * lane]) = *reinterpret_cast<float2 *>(x[g][j]);
+                }
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                if (32 * W * j >= 2 * a.half) continue;
+#pragma unroll
+                for (int e = 0; e < W; e++) {
+                    const int i = 32 * W * j + W * lane + e;
+                    if (i < 2 * a.half) {
+                        const bool low = i < a.half;
+                        const float other = head[warp][low ? i + a.half : i - a.half];
+                        const float2 t = turn[j][e];
+                        x[g][j][e] = low ? x[g][j][e] * t.x - other * t.y : x[g][j][e] * t.x + other * t.y;
+                    }
+                }
             }
         }
-    }
-    if (is_q) {
+        if (k < 0) {
+            float *out = a.q_out + ((size_t)row * a.q_heads + h) * D + W * lane;
 #pragma unroll
-        for (int j = 0; j < N; j++) a.q_out[((size_t)row * a.q_heads + h) * D + lane + 32 * j] = x[j];
-    } else {
-        __half *dst = (is_v ? a.c.v : a.c.k) + ((size_t)at * a.c.kv_heads + kv) * D;
+            for (int j = 0; j < N; j++) {
+                if (at < 0)  // the header's refusals: NaN queries, no store
 #pragma unroll
-        for (int j = 0; j < N; j++) dst[lane + 32 * j] = __float2half_rn(x[j]);
+                    for (int e = 0; e < W; e++) x[g][j][e] = __int_as_float(0x7fc00000);
+                if (W == 4 && a.aligned) *reinterpret_cast<float4 *>(out + 32 * W * j) = *reinterpret_cast<float4 *>(x[g][j]);
+                else
+#pragma unroll
+                    for (int e = 0; e < W; e++) out[32 * W * j + e] = x[g][j][e];
+            }
+        } else if (at >= 0) {
+            // cache rows are 16-byte aligned
+            __half2 *dst = reinterpret_cast<__half2 *>((v < 0 ? a.c.k : a.c.v) + ((size_t)at * a.c.kv_heads + (v < 0 ? k : v)) * D + W * lane);
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                __half2 y[W / 2];
+#pragma unroll
+                for (int e = 0; e < W / 2; e++) y[e] = __floats2half2_rn(x[g][j][2 * e], x[g][j][2 * e + 1]);
+                if constexpr (W == 4) *reinterpret_cast<uint2 *>(dst + 16 * W * j) = *reinterpret_cast<uint2 *>(y);
+                else dst[16 * W * j] = y[0];
+            }
+        }
     }
 }
 
@@ -108,45 +170,52 @@ constexpr int kCommitCtas = 8;  // one cluster per sequence
 // of one layer's key or value rows and moves it for every accepted node. path
 // ascends, so path[i] >= i: a destination is never a later node's source, and
 // a thread that reads nodes in ascending order before it writes them moves
-// them as if at once. The length is written after the cluster's barrier, when
-// every CTA has read it, so lengths_out may be the cache's own.
-__global__ void __cluster_dims__(kCommitCtas, 1, 1) __launch_bounds__(256) cache_commit_kernel(const CommitArgs a) {
+// them as if at once. Eight are read before they are written: with one at a
+// time each move waits for its own load (48 sequences x 24 layers: 45 us). Nodes
+// already in place are a prefix. The length is written after the cluster's
+// barrier, when every CTA has read it, so lengths_out may be the cache's own.
+// Bound by HBM for many sequences, by the chain length - page - row for one.
+__global__ void __cluster_dims__(kCommitCtas, 1, 1) __launch_bounds__(256) cache_commit_kernel(const __grid_constant__ CommitArgs a) {
     __shared__ long long from[kMaxNodes], to[kMaxNodes];
-    __shared__ int moves;
     cg::cluster_group cluster = cg::this_cluster();
-    const int seq = blockIdx.x / kCommitCtas, part = blockIdx.x % kCommitCtas;
-    const int length = a.c.committed(seq, a.tokens);
+    const int seq = blockIdx.x / kCommitCtas, part = blockIdx.x % kCommitCtas, i = threadIdx.x;
     const int n = a.accepted[seq];
-    if (threadIdx.x == 0) {
-        int m = length >= 0 && n >= 0 && n < a.tokens ? 0 : -1, last = 0;
-        for (int i = 1; m >= 0 && i <= n; i++) {
-            const int p = a.path[(size_t)seq * a.tokens + i];
-            if (p <= last || p >= a.tokens) {
-                m = -1;
-                break;
-            }
-            last = p;
-            if (p == i) continue;
-            from[m] = a.c.row(seq, length + p);
-            to[m] = a.c.row(seq, length + i);
-            if (from[m] < 0 || to[m] < 0) m = -1;
-            else m++;
+    const int p = i < a.tokens ? a.path[(size_t)seq * a.tokens + i] : 0;
+    const int before = i > 0 && i < a.tokens ? a.path[(size_t)seq * a.tokens + i - 1] : -1;
+    const int length = a.c.committed(seq, a.tokens);
+    bool sound = length >= 0 && n >= 0 && n < a.tokens, moves = false;
+    if (sound && i > 0 && i <= n) {
+        // the root is not read: the first draft only has to come after it
+        sound = p < a.tokens && p > (i == 1 ? 0 : before);
+        if (sound && p != i) {
+            from[i] = a.c.row(seq, length + p);
+            to[i] = a.c.row(seq, length + i);
+            sound = from[i] >= 0 && to[i] >= 0;
+            moves = true;
         }
-        moves = m;
     }
-    __syncthreads();
-    if (moves > 0) {
+    sound = __syncthreads_and(sound);
+    const int count = __syncthreads_count(moves);
+    if (sound && count) {
         const size_t width = (size_t)a.c.kv_heads * a.c.head_dim * sizeof(__half) / 16;  // 16-byte columns of a row
-        const size_t columns = width * 2 * a.layers;
-        for (size_t col = (size_t)part * 256 + threadIdx.x; col < columns; col += kCommitCtas * 256) {
-            const size_t pool = col / width, x = col % width;
+        const unsigned columns = (unsigned)(width * 2 * a.layers);
+        for (unsigned col = part * 256 + i; col < columns; col += kCommitCtas * 256) {
+            const unsigned pool = col / (unsigned)width, x = col % (unsigned)width;
             uint4 *base = reinterpret_cast<uint4 *>(reinterpret_cast<char *>(pool & 1 ? a.c.v : a.c.k) +
                                                     (pool >> 1) * a.layer_bytes) + x;
-            for (int i = 0; i < moves; i++) base[to[i] * width] = base[from[i] * width];
+            for (int m = n - count + 1; m <= n; m += 8) {
+                uint4 v[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (m + k <= n) v[k] = base[from[m + k] * width];
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (m + k <= n) base[to[m + k] * width] = v[k];
+            }
         }
     }
     cluster.sync();
-    if (part == 0 && threadIdx.x == 0) a.lengths_out[seq] = moves >= 0 ? length + n + 1 : a.c.lengths[seq];
+    if (part == 0 && i == 0) a.lengths_out[seq] = sound ? length + n + 1 : a.c.lengths[seq];
 }
 
 }  // namespace
@@ -183,7 +252,10 @@ extern "C" int qg_qk_norm_rope(float *q_out, const qg_kv_cache *cache, int layer
     a.half = rotary / 2;
     a.tokens = tokens, a.q_heads = q_heads, a.rows = seqs * tokens;
     a.eps = eps;
-    const long long items = (long long)a.rows * (q_heads + 2 * a.c.kv_heads);
+    a.aligned = !((reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
+                   reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(q_weight) | reinterpret_cast<uintptr_t>(k_weight)) & 15) &&
+                !((q_stride | k_stride | v_stride) & 3);
+    const long long items = (long long)a.rows * ((q_heads + 2 * a.c.kv_heads + kHeads - 1) / kHeads);
     const unsigned grid = (unsigned)((items + 7) / 8);
     if (D == 64) qk_norm_rope_kernel<64><<<grid, 256, 0, launch_stream>>>(a);
     else if (D == 128) qk_norm_rope_kernel<128><<<grid, 256, 0, launch_stream>>>(a);
