@@ -292,6 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                                                                      const __grid_constant__ CUtensorMap k_map,
                                                                      const __grid_constant__ CUtensorMap v_map) {
     using C = Cfg<D, MR>;
+    const int copies = D == 256 ? 1 : a.copies;
     constexpr int NC = C::kChunks, NK = C::kKStages, NV = C::kVStages, VK = C::kVKeys, QB = C::kQBufs;
     extern __shared__ __align__(1024) unsigned char smem[];  // swizzled tiles start on multiples of 1024
     unsigned char *q_smem = smem, *k_ring = smem + QB * 2 * C::kPlane, *v_ring = k_ring + NK * kStage;
@@ -302,16 +303,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     if (warp == 0) {
         const int per = a.c.kv_heads * a.row_tiles;
         const int len = lane < a.seqs ? a.c.committed(lane, a.tokens) : -1;
-        long long w = (long long)units_of(a, len) * per;
-        for (int q = lane + 32; q < a.seqs; q += 32) w += (long long)units_of(a, a.c.committed(q, a.tokens)) * per;
-        w = warp_sum(w);
-        const int g = (int)min((long long)gridDim.x, w);
-        long long base = 0, u0 = 0, u1 = 0;
-        int seq = 0, length = -1;
+        long long w = (long long)units_of(a, len) * per, base = 0, u0 = 0, u1 = 0;
+        int seq = 0, length = len;
+        if (a.seqs > 1) {
+            for (int q = lane + 32; q < a.seqs; q += 32) w += (long long)units_of(a, a.c.committed(q, a.tokens)) * per;
+            w = warp_sum(w);
+        }
+        const int g = (int)min((long long)gridDim.x, w);  // (one sequence: right in lane 0)
         if ((int)blockIdx.x < g) {
             u0 = range_start(blockIdx.x, w, g);
             u1 = range_start(blockIdx.x + 1, w, g);
-            seq = find_unit(a, per, u0, len, base, length);
+            if (a.seqs > 1) seq = find_unit(a, per, u0, len, base, length);
         }
         if (lane == 0) {
             const int units = max(1, units_of(a, length)), index = (int)quotient(u0 - base, units);
@@ -485,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         // With few rows (a.copies 2 or 4) Q lies in the tile several times, and each copy takes its share of a unit's
         // keys: a running maximum and total of its own, P = 0 for the others' keys, joined at the end of the item.
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-        const int row = tid - 128, span = MR / a.copies, copy = row / span, chunks = kKeys / kChunk / a.copies;
+        const int row = tid - 128, span = MR / copies, copy = row / span, chunks = kKeys / kChunk / copies;
         const int h0 = copy * chunks, h1 = h0 + chunks;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // tensor memory lane of the warp's first row, in bits 16+
         uint32_t tile = 0, item = 0, msg = 0;
@@ -609,7 +611,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         // ---------------------------------------------------- Q, and the accumulators: rows x half of the columns
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsAcc));
         constexpr int H = D / 2, V = D / 32;
-        const int w = warp - 8, row = (warp & 3) * 32 + lane, col0 = (w >> 2) * H, span = MR / a.copies;
+        const int w = warp - 8, row = (warp & 3) * 32 + lane, col0 = (w >> 2) * H, span = MR / copies;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
         uint32_t piece0 = 0, tile = 0, msg = 0, cleans = 0;
         // Every round prepares Q of one item and works through one: the same, or with two places for Q the one before.
@@ -643,6 +645,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int r = w + 8 * (i0 + i);
+                        if (r >= rows) break;
                         float mx = 0.0f;
 #pragma unroll
                         for (int e = 0; e < V; e++) mx = fmaxf(mx, fabsf(x[i][e]));
@@ -659,7 +662,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                             const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[e]));
                             lo[e] = pack_half(p - f.x, q - f.y);
                         }
-                        if (r >= rows) continue;
                         const int at = lane * V, unit = (at % 64) / 8;
                         for (int rr = r; rr < MR; rr += span) {
                             if (lane == 0) s.q_scale[qb][rr] = fmaxf(a.scale * inv, 1e-44f);  // never 0: -infinity stays what it is
@@ -791,17 +793,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             if (tid == 256) s.odd_nodes = 0;
             const bool whole = it.count == it.units;
             const size_t part = (size_t)(2 * blockIdx.x + (it.start > s.unit0)) * a.part_rows;
-#pragma unroll 1
+#pragma unroll 2
             for (int i = 0; w + 8 * i < rows; i++) {
                 const int r = w + 8 * i;
                 const size_t at = __shfl_sync(0xffffffffu, where, i);
                 // the copies' maxima and totals become one
                 float m = -INFINITY, l = 0.0f, f[4];
-                for (int k = 0; k < a.copies; k++) m = fmaxf(m, s.q_scale[qb][r + k * span]);
+                for (int k = 0; k < copies; k++) m = fmaxf(m, s.q_scale[qb][r + k * span]);
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     f[k] = 0.0f;
-                    if (k < a.copies) {
+                    if (k < copies) {
                         const float mk = s.q_scale[qb][r + k * span], lk = s.val[slot][r + k * span];
                         f[k] = mk == -INFINITY ? lk : ex2(mk - m);  // lk is 0 (nothing seen) or NaN
                         l += f[k] * lk;
@@ -816,7 +818,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int k = 0; k < 4; k++)
-                        if (k < a.copies) {
+                        if (k < copies) {
                             const float4 x = *reinterpret_cast<const float4 *>(stage + (size_t)(r + k * span) * D * 4 + ((u ^ (r & 7)) << 4));
                             v.x += f[k] * x.x, v.y += f[k] * x.y, v.z += f[k] * x.z, v.w += f[k] * x.w;
                         }
@@ -850,7 +852,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
 template <int D>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttendArgs a, int ctas) {
     constexpr int V = D / 32;
-    __shared__ float sums[8][D], totals[8];
+    __shared__ float sums[8][D];
+    __shared__ float2 totals[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int id = blockIdx.x, h = id % a.q_heads, row = id / a.q_heads, seq = row / a.tokens;
     const int kv = h / a.group, r = (row % a.tokens) * a.group + h % a.group, tile = r / kRows;
@@ -867,40 +870,65 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Atten
         return;
     }
     if (parts < 2) return;
+    // Every warp has its own maximum; kFly parts are asked for before the first is used.
+    constexpr int kFly = 5;
     float m = -INFINITY, l = 0.0f, acc[V];
 #pragma unroll
     for (int e = 0; e < V; e++) acc[e] = 0.0f;
-    auto place = [&](int p) { return (size_t)(2 * (c0 + p) + (p == 0 && start > range_start(c0, w, g))) * a.part_rows + r % kRows; };
-    for (int p = lane; p < parts; p += 32) m = fmaxf(m, __ldcg(&a.part_ml[place(p)].x));
+    const bool late = start > range_start(c0, w, g);  // the first part is its CTA's second
+    for (int p0 = warp; p0 < parts; p0 += 8 * kFly) {
+        float2 ml[kFly];
+        float x[kFly][V], top = m;
 #pragma unroll
-    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-#pragma unroll 5
-    for (int p = warp; p < parts; p += 8) {
-        const size_t at = place(p);
-        const float2 ml = __ldcg(a.part_ml + at);
-        const float f = ml.x == -INFINITY ? ml.y : ex2(ml.x - m);  // its total is 0 (nothing seen) or NaN
-        l += f * ml.y;
-        const float *src = a.part_acc + at * D + lane * V;
-        float x[V];
-        if constexpr (V == 2) {
-            *reinterpret_cast<float2 *>(x) = __ldcg(reinterpret_cast<const float2 *>(src));
-        } else {
+        for (int i = 0; i < kFly; i++) {
+            const int p = p0 + 8 * i;
+            ml[i] = make_float2(-INFINITY, 0.0f);
+            if (p < parts) {
+                const size_t at = (size_t)(2 * (c0 + p) + (p == 0 && late)) * a.part_rows + r % kRows;
+                const float *src = a.part_acc + at * D + lane * V;
+                ml[i] = __ldcg(a.part_ml + at);
+                if constexpr (V == 2) {
+                    *reinterpret_cast<float2 *>(x[i]) = __ldcg(reinterpret_cast<const float2 *>(src));
+                } else {
 #pragma unroll
-            for (int e = 0; e < V; e += 4) *reinterpret_cast<float4 *>(x + e) = __ldcg(reinterpret_cast<const float4 *>(src + e));
+                    for (int e = 0; e < V; e += 4) *reinterpret_cast<float4 *>(x[i] + e) = __ldcg(reinterpret_cast<const float4 *>(src + e));
+                }
+            }
         }
 #pragma unroll
-        for (int e = 0; e < V; e++) acc[e] = fmaf(f, x[e], acc[e]);
+        for (int i = 0; i < kFly; i++) top = fmaxf(top, ml[i].x);
+        const float keep = m == -INFINITY ? 1.0f : ex2(m - top);  // (what there is without a maximum is 0 or NaN)
+        m = top;
+        l *= keep;
+#pragma unroll
+        for (int e = 0; e < V; e++) acc[e] *= keep;
+#pragma unroll
+        for (int i = 0; i < kFly; i++) {
+            if (p0 + 8 * i >= parts) continue;
+            const float f = ml[i].x == -INFINITY ? ml[i].y : ex2(ml[i].x - m);  // its total is 0 (nothing seen) or NaN
+            l += f * ml[i].y;
+#pragma unroll
+            for (int e = 0; e < V; e++) acc[e] = fmaf(f, x[i][e], acc[e]);
+        }
     }
 #pragma unroll
     for (int e = 0; e < V; e++) sums[warp][lane * V + e] = acc[e];
-    if (lane == 0) totals[warp] = l;
+    if (lane == 0) totals[warp] = make_float2(m, l);
     __syncthreads();
-    l = 0.0f;
-    for (int k = 0; k < 8; k++) l += totals[k];
+    m = -INFINITY, l = 0.0f;
+    float f[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) m = fmaxf(m, totals[k].x);
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        f[k] = totals[k].x == -INFINITY ? totals[k].y : ex2(totals[k].x - m);
+        l += f[k] * totals[k].y;
+    }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     for (int i = threadIdx.x; i < D; i += 256) {
         float v = 0.0f;
-        for (int k = 0; k < 8; k++) v += sums[k][i];
+#pragma unroll
+        for (int k = 0; k < 8; k++) v = fmaf(f[k], sums[k][i], v);
         out[i] = v * inv;
     }
 }
