@@ -71,13 +71,19 @@ struct Cfg {
     static constexpr int kQBufs = 4 * kPlane <= 131072 ? 2 : 1;
     static constexpr int kKStages = (232448 - 3072 - kQBufs * 2 * kPlane) / (2 * kStage), kVStages = kKStages;
     static constexpr int kSmem = kQBufs * 2 * kPlane + (kKStages + kVStages) * kStage + 3072;
-    static constexpr int kS = 256;  // tensor memory columns: O, then two of S (P takes its place)
+    static constexpr int kOBufs = D == 256 ? 1 : 2;
+    static constexpr int kS = 256;  // tensor memory columns: O (twice where it fits), then two of S (P takes its place)
+    // A warp that issued MMAs stalls at its next wait until they have read their operands, and the tensor cores run dry:
+    // so for heads of 128 the issuers wait for a unit's two pieces at once (16 single tokens 87.0 -> 84.5 us, 5 x 5 tokens
+    // 22.6 -> 20.8). Heads of 256 have no room in the rings for that (98k keys 92.8 -> 99.2 us). P comes in kParts
+    // parts of a unit.
+    static constexpr int kGroup = D == 128 ? 2 : 1, kParts = kChunks / kGroup, kPartKeys = kKeys / kParts;
 };
 
 struct Shared {
     float val[2][kRows];    // rescaling factors, and at an item's end the totals: softmax -> accumulators
     float q_scale[2][kRows];  // at an item's end the maxima
-    uint64_t k_full[7], k_empty[7], v_full[7], v_empty[7], s_full[2], p_full[2][kKeys / kChunk], pv_done[2], msg_full[2], msg_empty[2], o_full, o_empty, q_full[2], landed, clean, drain;
+    uint64_t k_full[7], k_empty[7], v_full[7], v_empty[7], s_full[2], p_full[2][4], pv_done[2], msg_full[2], msg_empty[2], o_full[2], o_empty[2], q_full[2], landed, clean, drain;
     int pages[2][2][8];     // of the units that the producers are at: keys, values
     uint64_t odd_nodes;     // nodes whose values are not finite
     long long unit0, unit1;
@@ -293,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                                                                      const __grid_constant__ CUtensorMap v_map) {
     using C = Cfg<D, MR>;
     const int copies = D == 256 ? 1 : a.copies;
-    constexpr int NC = C::kChunks, NK = C::kKStages, NV = C::kVStages, VK = C::kVKeys, QB = C::kQBufs;
+    constexpr int NC = C::kChunks, NK = C::kKStages, NV = C::kVStages, VK = C::kVKeys, QB = C::kQBufs, OB = C::kOBufs;
     extern __shared__ __align__(1024) unsigned char smem[];  // swizzled tiles start on multiples of 1024
     unsigned char *q_smem = smem, *k_ring = smem + QB * 2 * C::kPlane, *v_ring = k_ring + NK * kStage;
     Shared &s = *reinterpret_cast<Shared *>(v_ring + NV * kStage);
@@ -332,9 +338,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         for (int i = 0; i < 2; i++) {
             mbar_init(&s.s_full[i], 1), mbar_init(&s.pv_done[i], 1);
             mbar_init(&s.msg_full[i], 4), mbar_init(&s.msg_empty[i], 8);
-            for (int k = 0; k < kKeys / kChunk; k++) mbar_init(&s.p_full[i][k], 4);
+            for (int z = 0; z < C::kParts; z++) mbar_init(&s.p_full[i][z], 4);
+            mbar_init(&s.o_full[i], 1), mbar_init(&s.o_empty[i], 8), mbar_init(&s.q_full[i], 8);
         }
-        mbar_init(&s.o_full, 1), mbar_init(&s.o_empty, 8), mbar_init(&s.q_full[0], 8), mbar_init(&s.q_full[1], 8), mbar_init(&s.drain, 2);
+        mbar_init(&s.drain, 2);
         mbar_init(&s.landed, 1), mbar_init(&s.clean, 8);
         fence_mbar_init();
     } else if (warp == 3 && lane == 0) {
@@ -416,19 +423,26 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     const uint32_t buf = tile & 1, d = tmem + C::kS + buf * kKeys;
                     if (tile >= 2) ok = wait(&s.pv_done[buf], (tile / 2 - 1) & 1, abort, a.err);
 #pragma unroll 1
-                    for (int c = 0; ok && c < NC; c++) {
-                        ok = wait(&s.k_full[st], round & 1, abort, a.err);
+                    for (int c0 = 0; ok && c0 < NC; c0 += C::kGroup) {
+                        uint32_t at = st, turn = round;
+#pragma unroll
+                        for (int c = 0; c < C::kGroup; c++) {
+                            ok = ok && wait(&s.k_full[at], turn & 1, abort, a.err);
+                            if (++at == NK) at = 0, turn++;
+                        }
                         if (!ok) break;
                         tc_fence_after();
-                        const uint64_t kd = operand(smem_u32(k_ring + st * kStage), 16);
 #pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            mma_ss(d, q_lo + qb * (2 * C::kPlane / 16) + c * (C::kBlock / 16) + 2 * k, kd + 2 * k, idesc(kKeys, false), c + k > 0);
+                        for (int c = 0; c < C::kGroup; c++) {
+                            const uint64_t kd = operand(smem_u32(k_ring + st * kStage), 16);
+                            const uint64_t qd = qb * (2 * C::kPlane / 16) + (c0 + c) * (C::kBlock / 16);
 #pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            mma_ss(d, q_hi + qb * (2 * C::kPlane / 16) + c * (C::kBlock / 16) + 2 * k, kd + 2 * k, idesc(kKeys, false), true);
-                        commit(&s.k_empty[st]);
-                        if (++st == NK) st = 0, round++;
+                            for (int k = 0; k < 4; k++) mma_ss(d, q_lo + qd + 2 * k, kd + 2 * k, idesc(kKeys, false), c0 + c + k > 0);
+#pragma unroll
+                            for (int k = 0; k < 4; k++) mma_ss(d, q_hi + qd + 2 * k, kd + 2 * k, idesc(kKeys, false), true);
+                            commit(&s.k_empty[st]);
+                            if (++st == NK) st = 0, round++;
+                        }
                     }
                     if (ok) commit(&s.s_full[buf]);
                 }
@@ -442,41 +456,43 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             bool ok = true;
             while (ok && walk.next(a, it)) {
                 for (int j = 0; ok && j < it.count; j++, tile++) {
-                    const uint32_t buf = tile & 1, p0 = tmem + C::kS + buf * kKeys;
+                    const uint32_t buf = tile & 1, p0 = tmem + C::kS + buf * kKeys, ob = tile % OB, o = tmem + ob * D;
                     const int keys = keys_of(a, it, j), past = it.length - (it.first + j) * kKeys;
-                    if (tile >= 1) ok = wait(&s.o_empty, (tile - 1) & 1, abort, a.err);
-                    // 32 keys at a time, as the softmax delivers them. Past the last key there is nothing to multiply, but
-                    // the softmax writes there too, and must be done before S takes the place again.
+                    if (tile >= OB) ok = wait(&s.o_empty[ob], (tile / OB - 1) & 1, abort, a.err);
 #pragma unroll 1
-                    for (int h = 0; ok && h < kKeys / kChunk; h++) {
-                        if (h * kChunk >= keys) {
-                            ok = wait(&s.p_full[buf][h], (tile / 2) & 1, abort, a.err);
-                            continue;
+                    for (int z = 0; ok && z < C::kParts; z++) {
+                        // Past the last key there is nothing to multiply, but the softmax writes there too, and must be
+                        // done before S takes the place again.
+                        const int key0 = z * C::kPartKeys, n = min(C::kPartKeys, keys - key0), pieces = (n + VK - 1) / VK;
+                        uint32_t at = st, turn = round;
+                        for (int c = 0; c < pieces; c++) {
+                            ok = ok && wait(&s.v_full[at], turn & 1, abort, a.err);
+                            if (++at == NV) at = 0, turn++;
                         }
-                        const int row = h * kChunk % VK;
-                        if (row == 0) ok = wait(&s.v_full[st], round & 1, abort, a.err);
-                        if (ok && (h + 1) * kChunk > past) {  // nodes: the accumulator warps clean their values
+                        if (ok && n > 0 && key0 + C::kPartKeys > past) {  // nodes: the accumulator warps clean their values
                             arrive(&s.landed);
                             ok = wait(&s.clean, cleans++ & 1, abort, a.err);
                         }
-                        ok = ok && wait(&s.p_full[buf][h], (tile / 2) & 1, abort, a.err);
+                        ok = ok && wait(&s.p_full[buf][z], (tile / 2) & 1, abort, a.err);
                         if (!ok) break;
                         tc_fence_after();
-                        const uint32_t v0 = smem_u32(v_ring + st * kStage);
-                        const int steps = min(2, (keys - h * kChunk + 15) / 16);
-                        for (int k = 0; k < steps; k++) {
-                            const uint64_t vd = operand(v0 + value_at<NC>(a, row + 16 * k), a.v_box * 128);
-                            mma_ts(tmem, p0 + h * kChunk + 16 + k * 8, vd, idesc(D, true), h + k > 0);
-                            mma_ts(tmem, p0 + h * kChunk + k * 8, vd, idesc(D, true), true);
-                        }
-                        if (row + kChunk == VK || (h + 1) * kChunk >= keys) {
+                        for (int c = 0; c < pieces; c++) {
+                            const uint32_t v0 = smem_u32(v_ring + st * kStage);
+                            const int steps = min(VK, n - c * VK + 15) / 16;
+                            for (int k = 0; k < steps; k++) {
+                                const int key = key0 + c * VK + 16 * k;
+                                const uint64_t vd = operand(v0 + value_at<NC>(a, 16 * k), a.v_box * 128);
+                                const uint32_t p = p0 + (key & ~31) + (key & 16) / 2;  // 32 keys: 16 columns of hi, 16 of lo
+                                mma_ts(o, p + 16, vd, idesc(D, true), key > 0);
+                                mma_ts(o, p, vd, idesc(D, true), true);
+                            }
                             commit(&s.v_empty[st]);
                             if (++st == NV) st = 0, round++;
                         }
                     }
                     if (!ok) break;
                     commit(&s.pv_done[buf]);
-                    commit(&s.o_full);
+                    commit(&s.o_full[ob]);
                 }
             }
             commit(&s.drain);
@@ -508,6 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 const uint32_t buf = tile & 1, cols = tmem + lanes + C::kS + buf * kKeys;
                 const int past = it.length - (it.first + j) * kKeys;  // keys of this unit before the nodes
                 const bool tail = past < kKeys;
+                const int held = (keys_of(a, it, j) + kChunk - 1) / kChunk;  // chunks that hold keys; the product leaves out the others
                 // which of keys 32h .. 32h+31 the row sees, in a unit that holds nodes
                 auto seen = [&](int h) -> uint32_t {
                     const int at = past - 32 * h;  // keys of the chunk before the nodes
@@ -522,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 if (live) {
                     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
-                    for (int h = h0; h < h1; h++) {
+                    for (int h = h0; h < min(h1, held); h++) {
                         float x[32];
                         tmem_ld32(cols + 32 * h, x);
                         tmem_wait_ld();
@@ -553,7 +570,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 for (int h = 0; h < kKeys / kChunk; h++) {
                     // P takes the place of 32 scores: 16 columns of hi, 16 of lo
                     uint32_t hi[16], lo[16];
-                    if (h >= h0 && h < h1) {
+                    if (h >= held) {
+                    } else if (h >= h0 && h < h1) {
                         if (live) {
                             float x[32];
                             tmem_ld32(cols + 32 * h, x);
@@ -584,9 +602,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                         tmem_st16(cols + 32 * h + 16, hi);
                         tmem_wait_st();
                     }
+                    if ((h + 1) * kChunk % C::kPartKeys) continue;
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) arrive(&s.p_full[buf][h]);
+                    if (lane == 0) arrive(&s.p_full[buf][h * kChunk / C::kPartKeys]);
                 }
                 // the running total, with what its rounding lost
                 const float add = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
@@ -629,19 +648,29 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 }
                 const uint32_t qb = round % QB;
                 unsigned char *q_to = q_smem + qb * 2 * C::kPlane;
-#pragma unroll 1
-                for (int i0 = 0; w + 8 * i0 < rows; i0 += 4) {  // lane l holds values V*l .. V*l+V-1 of four rows
-                    float x[4][V];
+                // lane l holds values V*l .. V*l+V-1 of four rows; the next four are asked for meanwhile
+                float next[4][V];
+                auto ask = [&](int i0) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const float *src = a.q + __shfl_sync(0xffffffffu, where_nx, i0 + i) + lane * V;
+                        const float *src = a.q + __shfl_sync(0xffffffffu, where_nx, i0 + i & 15) + lane * V;
                         if constexpr (V == 2) {
-                            *reinterpret_cast<float2 *>(x[i]) = __ldg(reinterpret_cast<const float2 *>(src));
+                            *reinterpret_cast<float2 *>(next[i]) = __ldg(reinterpret_cast<const float2 *>(src));
                         } else {
 #pragma unroll
-                            for (int e = 0; e < V; e += 4) *reinterpret_cast<float4 *>(x[i] + e) = __ldg(reinterpret_cast<const float4 *>(src + e));
+                            for (int e = 0; e < V; e += 4) *reinterpret_cast<float4 *>(next[i] + e) = __ldg(reinterpret_cast<const float4 *>(src + e));
                         }
                     }
+                };
+                ask(0);
+#pragma unroll 1
+                for (int i0 = 0; w + 8 * i0 < rows; i0 += 4) {
+                    float x[4][V];
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int e = 0; e < V; e++) x[i][e] = next[i][e];
+                    if (w + 8 * (i0 + 4) < rows) ask(i0 + 4);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int r = w + 8 * (i0 + i);
@@ -715,24 +744,27 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     // Values past the last position become 0 up to a multiple of 32; those of nodes 0 where they are
                     // not finite.
                     const int end = min(kKeys, past + a.tokens);
-                    for (int k0 = max(past, 0) & ~31; ok && k0 < end; k0 += 32) {
+                    for (int z = max(past, 0) / C::kPartKeys; ok && z * C::kPartKeys < end; z++) {
                         ok = wait_warp(&s.landed, cleans++ & 1, abort, a.err);
                         if (!ok) break;
-                        unsigned char *v0 = v_ring + (piece0 + j * NC + k0 / VK) % NV * kStage;
+                        const int key0 = max(past, z * C::kPartKeys) & ~31, key1 = min(end, (z + 1) * C::kPartKeys);
                         uint64_t odd = 0;
+                        for (int k0 = key0; k0 < key1; k0 += 32) {
+                            unsigned char *v0 = v_ring + (piece0 + j * NC + k0 / VK) % NV * kStage;
 #pragma unroll 1
-                        for (int u = tid - 256; u < 32 * 8 * NC; u += 256) {
-                            const int key = k0 + ((u >> 3) & 31);
-                            if (key < past) continue;
-                            uint4 *p = reinterpret_cast<uint4 *>(v0 + value_at<NC>(a, key % VK) + (u >> 8) * a.v_box * 128 + (u & 7) * 16);
-                            uint4 v = key < end ? *p : make_uint4(0, 0, 0, 0);
-                            uint32_t *wd = &v.x;
+                            for (int u = tid - 256; u < 32 * 8 * NC; u += 256) {
+                                const int key = k0 + ((u >> 3) & 31);
+                                if (key < past) continue;
+                                uint4 *p = reinterpret_cast<uint4 *>(v0 + value_at<NC>(a, key % VK) + (u >> 8) * a.v_box * 128 + (u & 7) * 16);
+                                uint4 v = key < end ? *p : make_uint4(0, 0, 0, 0);
+                                uint32_t *wd = &v.x;
 #pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                if ((wd[e] & 0x7c00u) == 0x7c00u) wd[e] &= 0xffff0000u, odd |= 1ull << (key - past);
-                                if ((wd[e] & 0x7c000000u) == 0x7c000000u) wd[e] &= 0x0000ffffu, odd |= 1ull << (key - past);
+                                for (int e = 0; e < 4; e++) {
+                                    if ((wd[e] & 0x7c00u) == 0x7c00u) wd[e] &= 0xffff0000u, odd |= 1ull << (key - past);
+                                    if ((wd[e] & 0x7c000000u) == 0x7c000000u) wd[e] &= 0x0000ffffu, odd |= 1ull << (key - past);
+                                }
+                                *p = v;
                             }
-                            *p = v;
                         }
                         if (odd) atomicOr(reinterpret_cast<unsigned long long *>(&s.odd_nodes), (unsigned long long)odd);
                         fence_proxy_async();
@@ -741,7 +773,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     }
                     if (!ok) break;
                 }
-                ok = wait_warp(&s.o_full, tile & 1, abort, a.err);
+                const uint32_t ob = tile % OB;
+                ok = wait_warp(&s.o_full[ob], tile / OB & 1, abort, a.err);
                 if (!ok) break;
                 if (live) {
                     tc_fence_after();
@@ -749,7 +782,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
 #pragma unroll
                     for (int b = 0; b < H / 32; b++) {
                         float x[32];
-                        tmem_ld32(tmem + lanes + col0 + 32 * b, x);
+                        tmem_ld32(tmem + lanes + ob * D + col0 + 32 * b, x);
                         tmem_wait_ld();
 #pragma unroll
                         for (int i = 0; i < 16; i++) acc[16 * b + i] = __ffma2_rn(acc[16 * b + i], keep2, {x[2 * i], x[2 * i + 1]});
@@ -757,17 +790,23 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     tc_fence_before();
                 }
                 __syncwarp();
-                if (lane == 0) arrive(&s.o_empty);
+                if (lane == 0) arrive(&s.o_empty[ob]);
             }
             const uint32_t slot = msg & 1;
             if (ok) ok = wait_warp(&s.msg_full[slot], (msg / 2) & 1, abort, a.err);
+            const bool whole = it.count == it.units;
             // The rows go through Q's place, 16-byte units turned by the row's low bits, so that whole rows are stored.
             if (ok && live) {
                 unsigned char *mine = stage + (size_t)row * D * 4;
+                float mul = 1.0f;
+                if (copies == 1 && whole) {
+                    const float total = s.val[slot][row];
+                    mul = total == 0.0f ? 0.0f : 1.0f / total;
+                }
 #pragma unroll
                 for (int i = 0; i < H / 4; i++)
                     *reinterpret_cast<float4 *>(mine + (((col0 / 4 + i) ^ (row & 7)) << 4)) =
-                        make_float4(acc[2 * i].x, acc[2 * i].y, acc[2 * i + 1].x, acc[2 * i + 1].y);
+                        make_float4(acc[2 * i].x * mul, acc[2 * i].y * mul, acc[2 * i + 1].x * mul, acc[2 * i + 1].y * mul);
                 uint64_t odd = row % span < rows ? *(volatile uint64_t *)&s.odd_nodes : 0;
                 if (odd) {  // rare: values that are not finite, for the rows that see them
                     const int node = (it.tile * kRows + row % span) / a.group;
@@ -791,38 +830,54 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             ok = !group_any(4, 256, !ok);  // the eight warps stop together
             if (!ok) break;
             if (tid == 256) s.odd_nodes = 0;
-            const bool whole = it.count == it.units;
             const size_t part = (size_t)(2 * blockIdx.x + (it.start > s.unit0)) * a.part_rows;
-#pragma unroll 2
-            for (int i = 0; w + 8 * i < rows; i++) {
-                const int r = w + 8 * i;
-                const size_t at = __shfl_sync(0xffffffffu, where, i);
-                // the copies' maxima and totals become one
-                float m = -INFINITY, l = 0.0f, f[4];
-                for (int k = 0; k < copies; k++) m = fmaxf(m, s.q_scale[qb][r + k * span]);
+            const float nan = __int_as_float(0x7fc00000);
+            if (copies == 1) {
+                if (!whole && col0 == 0 && row < rows) a.part_ml[part + row] = make_float2(s.q_scale[qb][row], s.val[slot][row]);
+#pragma unroll 4
+                for (int i = 0; w + 8 * i < rows; i++) {
+                    const int r = w + 8 * i;
+                    const size_t at = __shfl_sync(0xffffffffu, where, i);
+                    float *dst = whole ? a.out + at : a.part_acc + (part + r) * D;
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    f[k] = 0.0f;
-                    if (k < copies) {
-                        const float mk = s.q_scale[qb][r + k * span], lk = s.val[slot][r + k * span];
-                        f[k] = mk == -INFINITY ? lk : ex2(mk - m);  // lk is 0 (nothing seen) or NaN
-                        l += f[k] * lk;
+                    for (int u = lane; u < D / 4; u += 32) {
+                        float4 v = *reinterpret_cast<const float4 *>(stage + (size_t)r * D * 4 + ((u ^ (r & 7)) << 4));
+                        if (bad) v = make_float4(nan, nan, nan, nan);
+                        reinterpret_cast<float4 *>(dst)[u] = v;
                     }
                 }
-                float mul = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
-                if (bad) mul = __int_as_float(0x7fc00000);
-                float *dst = whole ? a.out + at : a.part_acc + (part + r) * D;
-                if (!whole && lane == 0) a.part_ml[part + r] = make_float2(m, l);
+            } else {
+                // the copies' maxima and totals become one
+#pragma unroll 1
+                for (int i = 0; w + 8 * i < rows; i++) {
+                    const int r = w + 8 * i;
+                    const size_t at = __shfl_sync(0xffffffffu, where, i);
+                    float m = -INFINITY, l = 0.0f, f[4];
+                    for (int k = 0; k < copies; k++) m = fmaxf(m, s.q_scale[qb][r + k * span]);
 #pragma unroll
-                for (int u = lane; u < D / 4; u += 32) {
-                    float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
+                    for (int k = 0; k < 4; k++) {
+                        f[k] = 0.0f;
                         if (k < copies) {
-                            const float4 x = *reinterpret_cast<const float4 *>(stage + (size_t)(r + k * span) * D * 4 + ((u ^ (r & 7)) << 4));
-                            v.x += f[k] * x.x, v.y += f[k] * x.y, v.z += f[k] * x.z, v.w += f[k] * x.w;
+                            const float mk = s.q_scale[qb][r + k * span], lk = s.val[slot][r + k * span];
+                            f[k] = mk == -INFINITY ? lk : ex2(mk - m);  // lk is 0 (nothing seen) or NaN
+                            l += f[k] * lk;
                         }
-                    reinterpret_cast<float4 *>(dst)[u] = make_float4(v.x * mul, v.y * mul, v.z * mul, v.w * mul);
+                    }
+                    float mul = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+                    if (bad) mul = nan;
+                    float *dst = whole ? a.out + at : a.part_acc + (part + r) * D;
+                    if (!whole && lane == 0) a.part_ml[part + r] = make_float2(m, l);
+#pragma unroll
+                    for (int u = lane; u < D / 4; u += 32) {
+                        float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            if (k < copies) {
+                                const float4 x = *reinterpret_cast<const float4 *>(stage + (size_t)(r + k * span) * D * 4 + ((u ^ (r & 7)) << 4));
+                                v.x += f[k] * x.x, v.y += f[k] * x.y, v.z += f[k] * x.z, v.w += f[k] * x.w;
+                            }
+                        reinterpret_cast<float4 *>(dst)[u] = make_float4(v.x * mul, v.y * mul, v.z * mul, v.w * mul);
+                    }
                 }
             }
             __syncwarp();
