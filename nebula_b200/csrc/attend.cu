@@ -83,7 +83,7 @@ struct Cfg {
 struct Shared {
     float val[2][kRows];    // rescaling factors, and at an item's end the totals: softmax -> accumulators
     float q_scale[2][kRows];  // at an item's end the maxima
-    uint64_t k_full[7], k_empty[7], v_full[7], v_empty[7], s_full[2], p_full[2][4], pv_done[2], msg_full[2], msg_empty[2], o_full[2], o_empty[2], q_full[2], landed, clean, drain;
+    uint64_t k_full[7], k_empty[7], v_full[7], v_empty[7], s_full[2], p_full[2][4], pv_done[2], msg_full[2], msg_empty[2], o_full[2], o_empty[2], q_full[2], landed[2], clean[2], drain;
     int pages[2][2][8];     // of the units that the producers are at: keys, values
     uint64_t odd_nodes;     // nodes whose values are not finite
     long long unit0, unit1;
@@ -307,6 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     volatile int *abort = &s.abort;
 
     if (warp == 0) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
         const int per = a.c.kv_heads * a.row_tiles;
         const int len = lane < a.seqs ? a.c.committed(lane, a.tokens) : -1;
         long long w = (long long)units_of(a, len) * per, base = 0, u0 = 0, u1 = 0;
@@ -340,24 +341,25 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             mbar_init(&s.msg_full[i], 4), mbar_init(&s.msg_empty[i], 8);
             for (int z = 0; z < C::kParts; z++) mbar_init(&s.p_full[i][z], 4);
             mbar_init(&s.o_full[i], 1), mbar_init(&s.o_empty[i], 8), mbar_init(&s.q_full[i], 8);
+            mbar_init(&s.landed[i], 1), mbar_init(&s.clean[i], 8);
         }
         mbar_init(&s.drain, 2);
-        mbar_init(&s.landed, 1), mbar_init(&s.clean, 8);
         fence_mbar_init();
     } else if (warp == 3 && lane == 0) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map));
         asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map));
     }
+    // Every role goes to its code first and meets the others there: instructions that are not yet in the SM's caches
+    // arrive while the plan is made.
     tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const uint32_t tmem = s.tmem;
-    Walk walk(s);
-    Item it;
-
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
+        __syncthreads();
+        tc_fence_after();
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+        const uint32_t tmem = s.tmem;
+        Walk walk(s);
+        Item it;
         if (warp == 0 || warp == 3) {
             // ------------------------------------------------ producers: pages to the rings, keys (warp 0), values (warp 3)
             // A warp issues its copies one after the other (134 cycles for a 2 KB box, 440 for 8 KB, measured), 15-23
@@ -410,6 +412,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             if (!ok && lane == 0)  // the copies in flight land before the CTA ends
                 for (uint32_t i = 0; i < places; i++)
                     if (i < st || round) wait_drain(&full[i], (i < st ? round : round - 1) & 1);
+            if (!is_k)  // rows of refused sequences
+                for (int q = blockIdx.x; q < a.seqs; q += gridDim.x)
+                    if (a.c.committed(q, a.tokens) < 0)
+                        for (size_t i = lane; i < (size_t)a.tokens * a.q_heads * D; i += 32)
+                            a.out[(size_t)q * a.tokens * a.q_heads * D + i] = __int_as_float(0x7fc00000);
         } else if (warp == 1 && elect_one()) {
             // ------------------------------------------------ S = Q K^T
             uint32_t st = 0, round = 0, tile = 0, item = 0;
@@ -452,26 +459,34 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             wait_drain(&s.drain, 0);
         } else if (warp == 2 && elect_one()) {
             // ------------------------------------------------ O = P V
-            uint32_t st = 0, round = 0, tile = 0, cleans = 0;
+            uint32_t st = 0, round = 0, tile = 0, lands = 0, cleans = 0;  // (at most two parts between landed and clean)
             bool ok = true;
             while (ok && walk.next(a, it)) {
                 for (int j = 0; ok && j < it.count; j++, tile++) {
                     const uint32_t buf = tile & 1, p0 = tmem + C::kS + buf * kKeys, ob = tile % OB, o = tmem + ob * D;
                     const int keys = keys_of(a, it, j), past = it.length - (it.first + j) * kKeys;
                     if (tile >= OB) ok = wait(&s.o_empty[ob], (tile / OB - 1) & 1, abort, a.err);
+                    // the pieces of part z; where it holds nodes, the accumulator warps are told to clean their values
+                    uint32_t at = st, turn = round;
+                    auto take = [&](int z) {
+                        const int n = min(C::kPartKeys, keys - z * C::kPartKeys);
+                        for (int c = 0; c * VK < n; c++) {
+                            ok = ok && wait(&s.v_full[at], turn & 1, abort, a.err);
+                            if (++at == NV) at = 0, turn++;
+                        }
+                        if (ok && n > 0 && (z + 1) * C::kPartKeys > past) arrive(&s.landed[lands++ & 1]);
+                    };
+                    if (past < kKeys) take(0);
 #pragma unroll 1
                     for (int z = 0; ok && z < C::kParts; z++) {
                         // Past the last key there is nothing to multiply, but the softmax writes there too, and must be
                         // done before S takes the place again.
                         const int key0 = z * C::kPartKeys, n = min(C::kPartKeys, keys - key0), pieces = (n + VK - 1) / VK;
-                        uint32_t at = st, turn = round;
-                        for (int c = 0; c < pieces; c++) {
-                            ok = ok && wait(&s.v_full[at], turn & 1, abort, a.err);
-                            if (++at == NV) at = 0, turn++;
-                        }
-                        if (ok && n > 0 && key0 + C::kPartKeys > past) {  // nodes: the accumulator warps clean their values
-                            arrive(&s.landed);
-                            ok = wait(&s.clean, cleans++ & 1, abort, a.err);
+                        if (past >= kKeys) take(z);
+                        else if (z + 1 < C::kParts) take(z + 1);  // a part ahead, so that the cleaning is not waited for
+                        if (ok && n > 0 && key0 + C::kPartKeys > past) {
+                            ok = wait(&s.clean[cleans & 1], cleans / 2 & 1, abort, a.err);
+                            cleans++;
                         }
                         ok = ok && wait(&s.p_full[buf][z], (tile / 2) & 1, abort, a.err);
                         if (!ok) break;
@@ -503,6 +518,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         // With few rows (a.copies 2 or 4) Q lies in the tile several times, and each copy takes its share of a unit's
         // keys: a running maximum and total of its own, P = 0 for the others' keys, joined at the end of the item.
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+        __syncthreads();
+        tc_fence_after();
+        const uint32_t tmem = s.tmem;
+        Walk walk(s);
+        Item it;
         const int row = tid - 128, span = MR / copies, copy = row / span, chunks = kKeys / kChunk / copies;
         const int h0 = copy * chunks, h1 = h0 + chunks;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // tensor memory lane of the warp's first row, in bits 16+
@@ -629,6 +649,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     } else {
         // ---------------------------------------------------- Q, and the accumulators: rows x half of the columns
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsAcc));
+        __syncthreads();
+        tc_fence_after();
+        const uint32_t tmem = s.tmem;
+        Walk walk(s);
+        Item it;
         constexpr int H = D / 2, V = D / 32;
         const int w = warp - 8, row = (warp & 3) * 32 + lane, col0 = (w >> 2) * H, span = MR / copies;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
@@ -745,7 +770,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     // not finite.
                     const int end = min(kKeys, past + a.tokens);
                     for (int z = max(past, 0) / C::kPartKeys; ok && z * C::kPartKeys < end; z++) {
-                        ok = wait_warp(&s.landed, cleans++ & 1, abort, a.err);
+                        ok = wait_warp(&s.landed[cleans & 1], cleans / 2 & 1, abort, a.err);
                         if (!ok) break;
                         const int key0 = max(past, z * C::kPartKeys) & ~31, key1 = min(end, (z + 1) * C::kPartKeys);
                         uint64_t odd = 0;
@@ -769,7 +794,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                         if (odd) atomicOr(reinterpret_cast<unsigned long long *>(&s.odd_nodes), (unsigned long long)odd);
                         fence_proxy_async();
                         __syncwarp();
-                        if (lane == 0) arrive(&s.clean);
+                        if (lane == 0) arrive(&s.clean[cleans & 1]);
+                        cleans++;
                     }
                     if (!ok) break;
                 }
@@ -888,16 +914,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             if (QB == 2) it = nx, where = where_nx, left = more;
             more = more && walk.next(a, nx);
         }
-        // refused sequences
-        for (int q = blockIdx.x; q < a.seqs; q += gridDim.x)
-            if (a.c.committed(q, a.tokens) < 0)
-                for (size_t i = tid - 256; i < (size_t)a.tokens * a.q_heads * D; i += 256)
-                    a.out[(size_t)q * a.tokens * a.q_heads * D + i] = __int_as_float(0x7fc00000);
     }
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(s.tmem));
     }
 }
 
@@ -1024,17 +1045,20 @@ int launch(const AttendArgs &a, const CUtensorMap &k_map, const CUtensorMap &v_m
     const long long units = (((long long)a.c.table_pages << a.c.shift) + kKeys - 1) / kKeys;
     const long long most = (long long)a.seqs * a.c.kv_heads * a.row_tiles * units;
     const int ctas = (int)(most < kMaxCtas ? most : kMaxCtas);
-    tree_attention_kernel<D, MR><<<ctas, kThreads, C::kSmem, launch_stream>>>(a, k_map, v_map);
-    if (int rc = cudaGetLastError()) return rc;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.seqs * a.tokens * a.q_heads));
-    cfg.blockDim = dim3(256);
     cfg.stream = launch_stream;
     cudaLaunchAttribute pdl[1];
     pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     pdl[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = pdl;
     cfg.numAttrs = 1;
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = C::kSmem;
+    if (int rc = cudaLaunchKernelEx(&cfg, tree_attention_kernel<D, MR>, a, k_map, v_map)) return rc;
+    cfg.gridDim = dim3((unsigned)(a.seqs * a.tokens * a.q_heads));
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
     return cudaLaunchKernelEx(&cfg, join_kernel<D>, a, ctas);
 }
 
