@@ -86,8 +86,8 @@ struct Shared {
     uint64_t k_full[7], k_empty[7], v_full[7], v_empty[7], s_full[2], p_full[2][4], pv_done[2], msg_full[2], msg_empty[2], o_full[2], o_empty[2], q_full[2], landed[2], clean[2], drain;
     int pages[2][2][8];     // of the units that the producers are at: keys, values
     uint64_t odd_nodes;     // nodes whose values are not finite
-    long long unit0, unit1;
-    int seq0, length0, kv0, tile0, first0;
+    long long slot0, slot1;
+    int seq0, length0, kv0, tile0, pos0;
     uint32_t tmem;
     int abort;
 };
@@ -203,25 +203,36 @@ __device__ __forceinline__ bool group_any(int id, int n, bool x) {
 __device__ __forceinline__ int units_of(const AttendArgs &a, int length) {
     return length < 0 ? 0 : (length + a.tokens + kKeys - 1) / kKeys;
 }
+// What an item costs besides its units, in units: Q, the first unit's latency and the store (about 2 us). The ranges
+// divide the sum of both; an item's first kItemCost slots stand for it and hold no unit. (16 sequences of 512 to 8191
+// keys: CTAs with eight short items took 81 us and those with one 65 when only units counted.)
+template <int D>
+constexpr int kItemCost = D == 256 ? 1 : 2;
+template <int D>
+__device__ __forceinline__ int slots_of(const AttendArgs &a, int length) {
+    return length < 0 ? 0 : units_of(a, length) + kItemCost<D>;
+}
 __device__ __forceinline__ long long warp_sum(long long x) {
 #pragma unroll
     for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
     return x;
 }
-// One warp: units of the sequences before `seqs`.
-__device__ long long sum_units(const AttendArgs &a, int seqs, int per) {
+// One warp: slots of the sequences before `seqs`.
+template <int D>
+__device__ long long sum_slots(const AttendArgs &a, int seqs, int per) {
     long long sum = 0;
-    for (int s = threadIdx.x & 31; s < seqs; s += 32) sum += (long long)units_of(a, a.c.committed(s, a.tokens)) * per;
+    for (int s = threadIdx.x & 31; s < seqs; s += 32) sum += (long long)slots_of<D>(a, a.c.committed(s, a.tokens)) * per;
     return warp_sum(sum);
 }
-// One warp: the sequence that holds unit `at`, its length and the units before it. `len`: the lane's own sequence
+// One warp: the sequence that holds slot `at`, its length and the slots before it. `len`: the lane's own sequence
 // among the first 32.
-__device__ int find_unit(const AttendArgs &a, int per, long long at, int len, long long &base, int &length) {
+template <int D>
+__device__ int find_slot(const AttendArgs &a, int per, long long at, int len, long long &base, int &length) {
     const int lane = threadIdx.x & 31;
     base = 0;
     for (int s0 = 0; s0 < a.seqs; s0 += 32) {
         if (s0) len = s0 + lane < a.seqs ? a.c.committed(s0 + lane, a.tokens) : -1;
-        const long long mine = (long long)units_of(a, len) * per;
+        const long long mine = (long long)slots_of<D>(a, len) * per;
         long long upto = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -243,28 +254,31 @@ __device__ int find_unit(const AttendArgs &a, int per, long long at, int len, lo
 __device__ __forceinline__ long long quotient(long long x, long long y) {
     return (x | y) >> 32 ? x / y : (long long)((uint32_t)x / (uint32_t)y);
 }
-// CTA c of g takes units [c*w/g, (c+1)*w/g).
+// CTA c of g takes slots [c*w/g, (c+1)*w/g).
 __device__ __forceinline__ long long range_start(long long c, long long w, int g) { return quotient(c * w, g); }
-__device__ __forceinline__ int cta_of(long long unit, long long w, int g) { return (int)quotient((unit + 1) * g + w - 1, w) - 1; }
+__device__ __forceinline__ int cta_of(long long slot, long long w, int g) { return (int)quotient((slot + 1) * g + w - 1, w) - 1; }
 
 // One CTA's part of one item.
 struct Item {
     int seq, kv, tile, first, count, units, length;
-    long long start;  // the item's first unit
+    long long start;  // the slot of the item's first unit
 };
+template <int D>
 struct Walk {
     long long at, end;
-    int seq, length, kv, tile, first;
+    int seq, length, kv, tile, pos;  // pos: slot within the item
     __device__ Walk(const Shared &s)
-        : at(s.unit0), end(s.unit1), seq(s.seq0), length(s.length0), kv(s.kv0), tile(s.tile0), first(s.first0) {}
+        : at(s.slot0), end(s.slot1), seq(s.seq0), length(s.length0), kv(s.kv0), tile(s.tile0), pos(s.pos0) {}
     __device__ bool next(const AttendArgs &a, Item &it) {
-        if (at >= end) return false;
-        it.seq = seq, it.kv = kv, it.tile = tile, it.first = first, it.length = length;
+        const int from = max(pos, kItemCost<D>);
+        if (at + (from - pos) >= end) return false;
+        it.seq = seq, it.kv = kv, it.tile = tile, it.first = from - kItemCost<D>, it.length = length;
         it.units = units_of(a, length);
-        it.count = (int)min((long long)(it.units - first), end - at);
-        it.start = at - first;
+        it.start = at - pos + kItemCost<D>;
+        at += from - pos;
+        it.count = (int)min((long long)(it.units - it.first), end - at);
         at += it.count;
-        first = 0;  // the item after it, should there be one
+        pos = 0;  // the item after it, should there be one
         if (++tile == a.row_tiles) {
             tile = 0;
             if (++kv == a.c.kv_heads) {
@@ -310,23 +324,23 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         asm volatile("griddepcontrol.wait;" ::: "memory");
         const int per = a.c.kv_heads * a.row_tiles;
         const int len = lane < a.seqs ? a.c.committed(lane, a.tokens) : -1;
-        long long w = (long long)units_of(a, len) * per, base = 0, u0 = 0, u1 = 0;
+        long long w = (long long)slots_of<D>(a, len) * per, base = 0, u0 = 0, u1 = 0;
         int seq = 0, length = len;
         if (a.seqs > 1) {
-            for (int q = lane + 32; q < a.seqs; q += 32) w += (long long)units_of(a, a.c.committed(q, a.tokens)) * per;
+            for (int q = lane + 32; q < a.seqs; q += 32) w += (long long)slots_of<D>(a, a.c.committed(q, a.tokens)) * per;
             w = warp_sum(w);
         }
         const int g = (int)min((long long)gridDim.x, w);  // (one sequence: right in lane 0)
         if ((int)blockIdx.x < g) {
             u0 = range_start(blockIdx.x, w, g);
             u1 = range_start(blockIdx.x + 1, w, g);
-            if (a.seqs > 1) seq = find_unit(a, per, u0, len, base, length);
+            if (a.seqs > 1) seq = find_slot<D>(a, per, u0, len, base, length);
         }
         if (lane == 0) {
-            const int units = max(1, units_of(a, length)), index = (int)quotient(u0 - base, units);
-            s.unit0 = u0, s.unit1 = u1, s.seq0 = seq, s.length0 = length;
+            const int slots = max(1, slots_of<D>(a, length)), index = (int)quotient(u0 - base, slots);
+            s.slot0 = u0, s.slot1 = u1, s.seq0 = seq, s.length0 = length;
             s.kv0 = index / a.row_tiles, s.tile0 = index % a.row_tiles;
-            s.first0 = (int)(u0 - base - (long long)index * units);
+            s.pos0 = (int)(u0 - base - (long long)index * slots);
         }
     } else if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s.tmem)));
@@ -358,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         tc_fence_after();
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
         const uint32_t tmem = s.tmem;
-        Walk walk(s);
+        Walk<D> walk(s);
         Item it;
         if (warp == 0 || warp == 3) {
             // ------------------------------------------------ producers: pages to the rings, keys (warp 0), values (warp 3)
@@ -521,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         __syncthreads();
         tc_fence_after();
         const uint32_t tmem = s.tmem;
-        Walk walk(s);
+        Walk<D> walk(s);
         Item it;
         const int row = tid - 128, span = MR / copies, copy = row / span, chunks = kKeys / kChunk / copies;
         const int h0 = copy * chunks, h1 = h0 + chunks;
@@ -652,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         __syncthreads();
         tc_fence_after();
         const uint32_t tmem = s.tmem;
-        Walk walk(s);
+        Walk<D> walk(s);
         Item it;
         constexpr int H = D / 2, V = D / 32;
         const int w = warp - 8, row = (warp & 3) * 32 + lane, col0 = (w >> 2) * H, span = MR / copies;
@@ -856,7 +870,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             ok = !group_any(4, 256, !ok);  // the eight warps stop together
             if (!ok) break;
             if (tid == 256) s.odd_nodes = 0;
-            const size_t part = (size_t)(2 * blockIdx.x + (it.start > s.unit0)) * a.part_rows;
+            const size_t part = (size_t)(2 * blockIdx.x + (it.start > s.slot0)) * a.part_rows;
             const float nan = __int_as_float(0x7fc00000);
             if (copies == 1) {
                 if (!whole && col0 == 0 && row < rows) a.part_ml[part + row] = make_float2(s.q_scale[qb][row], s.val[slot][row]);
@@ -935,8 +949,8 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Atten
     const int kv = h / a.group, r = (row % a.tokens) * a.group + h % a.group, tile = r / kRows;
     const int per = a.c.kv_heads * a.row_tiles;
     const int units = units_of(a, a.c.committed(seq, a.tokens));
-    const long long w = sum_units(a, a.seqs, per);
-    const long long start = (seq ? sum_units(a, seq, per) : 0) + (long long)(kv * a.row_tiles + tile) * units;
+    const long long w = sum_slots<D>(a, a.seqs, per);
+    const long long start = (seq ? sum_slots<D>(a, seq, per) : 0) + (long long)(kv * a.row_tiles + tile) * (units + kItemCost<D>) + kItemCost<D>;
     const int g = (int)min((long long)ctas, w);
     const int c0 = units ? cta_of(start, w, g) : 0, parts = units ? cta_of(start + units - 1, w, g) - c0 + 1 : 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -1043,7 +1057,7 @@ int launch(const AttendArgs &a, const CUtensorMap &k_map, const CUtensorMap &v_m
     if (int rc = cudaFuncSetAttribute(tree_attention_kernel<D, MR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem)) return rc;
     // no more CTAs than the longest sequences that the table allows could use
     const long long units = (((long long)a.c.table_pages << a.c.shift) + kKeys - 1) / kKeys;
-    const long long most = (long long)a.seqs * a.c.kv_heads * a.row_tiles * units;
+    const long long most = (long long)a.seqs * a.c.kv_heads * a.row_tiles * (units + kItemCost<D>);
     const int ctas = (int)(most < kMaxCtas ? most : kMaxCtas);
     cudaLaunchConfig_t cfg = {};
     cfg.stream = launch_stream;
