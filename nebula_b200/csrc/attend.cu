@@ -50,40 +50,50 @@ struct AttendArgs {
     const uint64_t *tree;
     float scale;  // |scale| * log2(e)
     float sign;   // of scale, folded into Q
-    int seqs, tokens, q_heads, group, row_tiles, part_rows, copies;
+    int seqs, tokens, q_heads, group, row_tiles, tile_rows, part_rows, copies;
     int k_box, v_box;  // rows of one TMA box: a page, at most a piece's keys
+    int k_blocks;      // column blocks of a box of keys
     int *err;
     float *part_acc;   // [2 * kMaxCtas][part_rows][D]
     float2 *part_ml;   // [2 * kMaxCtas][part_rows]
 };
 
-constexpr int kStage = 16384;    // one piece of the ring
 constexpr int kChunk = 32;       // keys per step of the softmax
 
-template <int D, int MR>
+// D: values of a head. MR: rows of Q that are kept. PAIR: two CTAs on neighbouring SMs (a cluster) work on 256 rows with
+// MMAs that span both (cta_group::2): each has its 128 rows of Q, S, P and O, and half of the keys' rows and of the
+// values' columns, which the tensor cores of both read. The rings hold twice the keys, and L2 delivers each key once for
+// 256 rows: heads of 256 need 128 KB for 128 rows of Q, and the 96 KB left are too few for keys and values of one CTA
+// (98k keys x 204 rows: 92.5 us with two row tiles apart).
+template <int D, int MR, bool PAIR>
 struct Cfg {
     static constexpr int kChunks = D / 64;                  // 128-byte wide column blocks
     static constexpr int kBlock = MR * 128;                 // one of them, of one plane of Q
     static constexpr int kPlane = kChunks * kBlock;
-    // The rings' pieces: 64 columns of 128 keys, or all columns of kVKeys values; kChunks pieces for a unit's keys or values.
-    static constexpr int kVKeys = kStage / (2 * D);
+    // The rings' pieces: kKBlocks column blocks of kKeyRows keys, or kVBlocks column blocks of kVKeys values; kPieces for
+    // a unit's keys or values.
+    static constexpr int kPiece = 16384, kKeyRows = PAIR ? kKeys / 2 : kKeys, kKBlocks = kPiece / (128 * kKeyRows);
+    static constexpr int kVBlocks = PAIR ? kChunks / 2 : kChunks, kVKeys = kPiece / (128 * kVBlocks);
+    static constexpr int kPieces = kChunks / kKBlocks;
+    static_assert(kPieces * kVKeys == kKeys, "as many pieces of values as of keys");
     // Two places for Q where there is room: the next item's is prepared while this one's is in use.
     static constexpr int kQBufs = 4 * kPlane <= 131072 ? 2 : 1;
-    static constexpr int kKStages = (232448 - 3072 - kQBufs * 2 * kPlane) / (2 * kStage), kVStages = kKStages;
-    static constexpr int kSmem = kQBufs * 2 * kPlane + (kKStages + kVStages) * kStage + 3072;
+    static constexpr int kKStages = (232448 - 3072 - kQBufs * 2 * kPlane) / (2 * kPiece), kVStages = kKStages;
+    static constexpr int kSmem = kQBufs * 2 * kPlane + (kKStages + kVStages) * kPiece + 3072;
     static constexpr int kOBufs = D == 256 ? 1 : 2;
     static constexpr int kS = 256;  // tensor memory columns: O (twice where it fits), then two of S (P takes its place)
     // A warp that issued MMAs stalls at its next wait until they have read their operands, and the tensor cores run dry:
-    // so for heads of 128 the issuers wait for a unit's two pieces at once (16 single tokens 87.0 -> 84.5 us, 5 x 5 tokens
-    // 22.6 -> 20.8). Heads of 256 have no room in the rings for that (98k keys 92.8 -> 99.2 us). P comes in kParts
+    // so where the rings have room the issuers wait for two pieces at once (16 single tokens of heads of 128 87.0 -> 84.5
+    // us, 5 x 5 tokens 22.6 -> 20.8; one CTA with heads of 256 has not: 98k keys 92.8 -> 99.2 us). P comes in kParts
     // parts of a unit.
-    static constexpr int kGroup = D == 128 ? 2 : 1, kParts = kChunks / kGroup, kPartKeys = kKeys / kParts;
+    static constexpr int kGroup = D == 128 ? 2 : 1, kParts = kPieces / kGroup, kPartKeys = kKeys / kParts;
+    static constexpr int kTileRows = PAIR ? 2 * kRows : kRows;
 };
 
 struct Shared {
     float val[2][kRows];    // rescaling factors, and at an item's end the totals: softmax -> accumulators
     float q_scale[2][kRows];  // at an item's end the maxima
-    uint64_t k_full[7], k_empty[7], v_full[7], v_empty[7], s_full[2], p_full[2][4], pv_done[2], msg_full[2], msg_empty[2], o_full[2], o_empty[2], q_full[2], landed[2], clean[2], drain;
+    uint64_t k_full[7], k_empty[7], v_full[7], v_empty[7], s_full[2], p_full[2][4], pv_done[2], msg_full[2], msg_empty[2], o_full[2], o_empty[2], q_full[2], q_all, landed[2], clean[2], drain;
     int pages[2][2][8];     // of the units that the producers are at: keys, values
     uint64_t odd_nodes;     // nodes whose values are not finite
     long long slot0, slot1;
@@ -98,8 +108,47 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 __device__ __forceinline__ void arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// At the same place in the pair's leading CTA (its own, without a pair).
+template <bool PAIR>
+__device__ __forceinline__ void arrive_leader(uint64_t *bar) {
+    if constexpr (PAIR)
+        asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
+                     "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar)) : "memory");
+    else arrive(bar);
+}
+// In both CTAs of a pair.
+template <bool PAIR>
+__device__ __forceinline__ void arrive_both(uint64_t *bar) {
+    arrive_leader<PAIR>(bar);
+    if constexpr (PAIR)
+        asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 1;\n\t"
+                     "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar)) : "memory");
+}
+// When this thread's MMAs so far are done: an arrival here, or in both CTAs of a pair.
+template <bool PAIR>
 __device__ __forceinline__ void commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    if constexpr (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    else asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void commit_both(uint64_t *bar) {
+    if constexpr (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                         smem_u32(bar)),
+                     "h"((uint16_t)3)
+                     : "memory");
+    else commit<false>(bar);
+}
+// All threads of the CTA, or of the pair.
+template <bool PAIR>
+__device__ __forceinline__ void sync_all() {
+    if constexpr (PAIR) {
+        asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    } else {
+        __syncthreads();
+    }
 }
 // Every wait is bounded: 2^17 attempts of at most 20 us (about 2.6 s), then the
 // CTA stops and the workspace's error word makes every row NaN.
@@ -122,9 +171,16 @@ __device__ __forceinline__ void wait_drain(uint64_t *bar, uint32_t parity) {
     for (int i = 0; i < (1 << 17); i++)
         if (mbar_try_wait_sleep(bar, parity, kWaitHintNs)) return;
 }
-// Box at pool row y, 64-column block z.
+// Box at pool row y, 64-column block z, into this CTA's memory; its bytes count at the leading CTA's barrier.
+template <bool PAIR>
 __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap *map, int y, int z, uint32_t bar) {
-    asm volatile(
+    if constexpr (PAIR)  // bit 24 of a shared::cluster address tells the CTAs of a pair apart
+        asm volatile(
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+                "r"(dst),
+            "l"(map), "r"(0), "r"(y), "r"(z), "r"(bar & 0xFEFFFFFFu)
+            : "memory");
+    else asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
             "r"(dst),
         "l"(map), "r"(0), "r"(y), "r"(z), "r"(bar)
@@ -144,22 +200,39 @@ __device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead) {
            ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 // F16 operands, F32 accumulator; bit 16: B is MN-major.
+template <bool PAIR>
 constexpr uint32_t idesc(int n, bool b_mn) {
-    return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+    return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)((PAIR ? 2 : 1) * kRows >> 4) << 24);
 }
+template <bool PAIR>
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool acc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(id), "r"((uint32_t)acc)
-        : "memory");
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(id), "r"((uint32_t)acc)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(id), "r"((uint32_t)acc)
+            : "memory");
 }
+template <bool PAIR>
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, bool acc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(id), "r"((uint32_t)acc)
-        : "memory");
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+            "r"(a), "l"(b), "r"(id), "r"((uint32_t)acc)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+            "r"(a), "l"(b), "r"(id), "r"((uint32_t)acc)
+            : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&r)[32]) {
     asm volatile(
@@ -304,19 +377,36 @@ __device__ __forceinline__ uint32_t value_at(const AttendArgs &a, int row) {
 // Pieces of values of an item's part: a last unit that is not full has fewer.
 template <class C>
 __device__ __forceinline__ uint32_t value_pieces(const AttendArgs &a, const Item &it) {
-    return (it.count - 1) * C::kChunks + (keys_of(a, it, it.count - 1) + C::kVKeys - 1) / C::kVKeys;
+    return (it.count - 1) * C::kPieces + (keys_of(a, it, it.count - 1) + C::kVKeys - 1) / C::kVKeys;
 }
 
-template <int D, int MR>
+// Nodes whose values are not finite, in the notes of both CTAs of a pair: each sees half of the columns.
+template <bool PAIR>
+__device__ __forceinline__ void mark_odd(uint64_t *notes, uint64_t nodes) {
+    if constexpr (!PAIR) {
+        atomicOr(reinterpret_cast<unsigned long long *>(notes), (unsigned long long)nodes);
+    } else {
+#pragma unroll
+        for (int r = 0; r < 2; r++)
+            asm volatile("{\n\t.reg .b32 a;\n\t.reg .b64 x;\n\tmapa.shared::cluster.u32 a, %0, %2;\n\t"
+                         "atom.relaxed.cluster.shared::cluster.or.b64 x, [a], %1;\n\t}" ::"r"(smem_u32(notes)),
+                         "l"(nodes), "r"(r)
+                         : "memory");
+    }
+}
+
+template <int D, int MR, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __grid_constant__ AttendArgs a,
                                                                      const __grid_constant__ CUtensorMap k_map,
                                                                      const __grid_constant__ CUtensorMap v_map) {
-    using C = Cfg<D, MR>;
+    using C = Cfg<D, MR, PAIR>;
     const int copies = D == 256 ? 1 : a.copies;
-    constexpr int NC = C::kChunks, NK = C::kKStages, NV = C::kVStages, VK = C::kVKeys, QB = C::kQBufs, OB = C::kOBufs;
+    constexpr int NC = C::kChunks, NK = C::kKStages, NV = C::kVStages, VK = C::kVKeys, QB = C::kQBufs, OB = C::kOBufs, VB = C::kVBlocks, NP = C::kPieces, KB = C::kKBlocks;
+    constexpr int kPeers = PAIR ? 2 : 1;  // CTAs that work on one item
+    const int team = blockIdx.x / kPeers, rank = blockIdx.x % kPeers, teams = gridDim.x / kPeers;
     extern __shared__ __align__(1024) unsigned char smem[];  // swizzled tiles start on multiples of 1024
-    unsigned char *q_smem = smem, *k_ring = smem + QB * 2 * C::kPlane, *v_ring = k_ring + NK * kStage;
-    Shared &s = *reinterpret_cast<Shared *>(v_ring + NV * kStage);
+    unsigned char *q_smem = smem, *k_ring = smem + QB * 2 * C::kPlane, *v_ring = k_ring + NK * C::kPiece;
+    Shared &s = *reinterpret_cast<Shared *>(v_ring + NV * C::kPiece);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     volatile int *abort = &s.abort;
 
@@ -330,10 +420,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             for (int q = lane + 32; q < a.seqs; q += 32) w += (long long)slots_of<D>(a, a.c.committed(q, a.tokens)) * per;
             w = warp_sum(w);
         }
-        const int g = (int)min((long long)gridDim.x, w);  // (one sequence: right in lane 0)
-        if ((int)blockIdx.x < g) {
-            u0 = range_start(blockIdx.x, w, g);
-            u1 = range_start(blockIdx.x + 1, w, g);
+        const int g = (int)min((long long)teams, w);  // (one sequence: right in lane 0)
+        if (team < g) {
+            u0 = range_start(team, w, g);
+            u1 = range_start(team + 1, w, g);
             if (a.seqs > 1) seq = find_slot<D>(a, per, u0, len, base, length);
         }
         if (lane == 0) {
@@ -343,8 +433,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             s.pos0 = (int)(u0 - base - (long long)index * slots);
         }
     } else if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s.tmem)));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s.tmem)));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s.tmem)));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        }
     } else if (warp == 2 && lane == 0) {
         s.abort = 0;
         s.odd_nodes = 0;
@@ -353,10 +448,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         for (int i = 0; i < 2; i++) {
             mbar_init(&s.s_full[i], 1), mbar_init(&s.pv_done[i], 1);
             mbar_init(&s.msg_full[i], 4), mbar_init(&s.msg_empty[i], 8);
-            for (int z = 0; z < C::kParts; z++) mbar_init(&s.p_full[i][z], 4);
-            mbar_init(&s.o_full[i], 1), mbar_init(&s.o_empty[i], 8), mbar_init(&s.q_full[i], 8);
-            mbar_init(&s.landed[i], 1), mbar_init(&s.clean[i], 8);
+            for (int z = 0; z < C::kParts; z++) mbar_init(&s.p_full[i][z], 4 * kPeers);
+            mbar_init(&s.o_full[i], 1), mbar_init(&s.o_empty[i], 8 * kPeers), mbar_init(&s.q_full[i], 8);
+            mbar_init(&s.landed[i], 1), mbar_init(&s.clean[i], 8 * kPeers);
         }
+        mbar_init(&s.q_all, 8 * kPeers);
         mbar_init(&s.drain, 2);
         fence_mbar_init();
     } else if (warp == 3 && lane == 0) {
@@ -368,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     tc_fence_before();
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
-        __syncthreads();
+        sync_all<PAIR>();
         tc_fence_after();
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
         const uint32_t tmem = s.tmem;
@@ -378,11 +474,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             // ------------------------------------------------ producers: pages to the rings, keys (warp 0), values (warp 3)
             // A warp issues its copies one after the other (134 cycles for a 2 KB box, 440 for 8 KB, measured), 15-23
             // bytes per cycle and SM; HBM delivers 25, so it takes two of them.
-            // The warp looks a unit's pages up one unit ahead (a lane each); one lane issues the boxes. A box of keys has
-            // one block of 64 columns, a box of values all of them.
+            // The warp looks a unit's pages up one unit ahead (a lane each); one lane issues the boxes. A box of values has
+            // all its column blocks side by side; keys want all rows of a block together.
             const bool is_k = warp == 0;
             const int page = a.c.page_tokens(), per_unit = max(1, kKeys >> a.c.shift);
-            const int box = is_k ? a.k_box : a.v_box, piece = is_k ? kKeys : VK, bytes = box * 128 * (is_k ? 1 : NC);
+            const int box = is_k ? a.k_box : a.v_box, piece = is_k ? C::kKeyRows : VK, blocks = is_k ? a.k_blocks : VB, bytes = box * 128 * blocks;
             const uint32_t ring = smem_u32(is_k ? k_ring : v_ring), places = is_k ? NK : NV;
             uint64_t *full = is_k ? s.k_full : s.v_full, *empty = is_k ? s.k_empty : s.v_empty;
             const CUtensorMap *map = is_k ? &k_map : &v_map;
@@ -403,20 +499,26 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     __syncwarp();
                     if (j + 1 < it.count) ids = look_up(j + 1);
                     const int pos = (it.first + j) * kKeys, keys = keys_of(a, it, j);
-                    const int pieces = is_k ? NC : (keys + VK - 1) / VK;
+                    const int pieces = is_k ? NP : (keys + VK - 1) / VK;
                     for (int c = 0; c < pieces; c++) {
                         if (round) ok = wait_warp(&empty[st], (round - 1) & 1, abort, a.err);
                         if (!ok) break;
                         if (elect_one()) {
-                            const int key0 = is_k ? 0 : c * VK;  // the piece's first key within the unit
-                            const int boxes = (min(piece, keys - key0) + box - 1) / box;  // none past the last position
+                            const int key0 = is_k ? rank * C::kKeyRows : c * VK;  // the piece's first key within the unit
+                            auto boxes_from = [&](int key) { return (min(piece, keys - key) + box - 1) / box; };
+                            const int boxes = boxes_from(key0);  // none past the last position
                             const uint32_t bar = smem_u32(&full[st]);
-                            uint32_t dst = ring + st * kStage;
-                            mbar_arrive_expect_tx(&full[st], boxes * bytes);
-                            int p = pos + key0;
-                            for (int b = 0; b < boxes; b++, p += box, dst += bytes)
-                                tma_3d(dst, map, (pages[(p >> a.c.shift) - (pos >> a.c.shift)] << a.c.shift) + (p & (page - 1)),
-                                       it.kv * NC + (is_k ? c : 0), bar);
+                            const int sweeps = is_k ? KB / blocks : 1;  // over the piece's column blocks
+                            if (!PAIR) mbar_arrive_expect_tx(&full[st], sweeps * boxes * bytes);
+                            else if (rank == 0)  // what both CTAs will bring
+                                mbar_arrive_expect_tx(&full[st], sweeps * (boxes + (is_k ? max(0, boxes_from(C::kKeyRows)) : boxes)) * bytes);
+                            for (int sw = 0; sw < sweeps; sw++) {
+                                uint32_t dst = ring + st * C::kPiece + sw * C::kKeyRows * 128;
+                                int p = pos + key0;
+                                for (int b = 0; b < boxes; b++, p += box, dst += bytes)
+                                    tma_3d<PAIR>(dst, map, (pages[(p >> a.c.shift) - (pos >> a.c.shift)] << a.c.shift) + (p & (page - 1)),
+                                                 it.kv * NC + (is_k ? c * KB + sw * blocks : rank * VB), bar);
+                            }
                         }
                         __syncwarp();
                         if (++st == places) st = 0, round++;
@@ -425,13 +527,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             }
             if (!ok && lane == 0)  // the copies in flight land before the CTA ends
                 for (uint32_t i = 0; i < places; i++)
-                    if (i < st || round) wait_drain(&full[i], (i < st ? round : round - 1) & 1);
+                    if ((i < st || round) && rank == 0) wait_drain(&full[i], (i < st ? round : round - 1) & 1);
             if (!is_k)  // rows of refused sequences
                 for (int q = blockIdx.x; q < a.seqs; q += gridDim.x)
                     if (a.c.committed(q, a.tokens) < 0)
                         for (size_t i = lane; i < (size_t)a.tokens * a.q_heads * D; i += 32)
                             a.out[(size_t)q * a.tokens * a.q_heads * D + i] = __int_as_float(0x7fc00000);
-        } else if (warp == 1 && elect_one()) {
+        } else if (warp == 1 && rank == 0 && elect_one()) {
             // ------------------------------------------------ S = Q K^T
             uint32_t st = 0, round = 0, tile = 0, item = 0;
             bool ok = true;
@@ -439,12 +541,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             const uint64_t q_hi = operand(smem_u32(q_smem), 16);
             while (ok && walk.next(a, it)) {
                 const uint32_t qb = item % QB;
-                ok = wait(&s.q_full[qb], item / QB & 1, abort, a.err);
+                ok = PAIR ? wait(&s.q_all, item & 1, abort, a.err) : wait(&s.q_full[qb], item / QB & 1, abort, a.err);
                 for (int j = 0; ok && j < it.count; j++, tile++) {
                     const uint32_t buf = tile & 1, d = tmem + C::kS + buf * kKeys;
                     if (tile >= 2) ok = wait(&s.pv_done[buf], (tile / 2 - 1) & 1, abort, a.err);
 #pragma unroll 1
-                    for (int c0 = 0; ok && c0 < NC; c0 += C::kGroup) {
+                    for (int c0 = 0; ok && c0 < NP; c0 += C::kGroup) {
                         uint32_t at = st, turn = round;
 #pragma unroll
                         for (int c = 0; c < C::kGroup; c++) {
@@ -455,23 +557,27 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                         tc_fence_after();
 #pragma unroll
                         for (int c = 0; c < C::kGroup; c++) {
-                            const uint64_t kd = operand(smem_u32(k_ring + st * kStage), 16);
-                            const uint64_t qd = qb * (2 * C::kPlane / 16) + (c0 + c) * (C::kBlock / 16);
 #pragma unroll
-                            for (int k = 0; k < 4; k++) mma_ss(d, q_lo + qd + 2 * k, kd + 2 * k, idesc(kKeys, false), c0 + c + k > 0);
+                            for (int e = 0; e < KB; e++) {
+                                const uint64_t kd = operand(smem_u32(k_ring + st * C::kPiece + e * C::kKeyRows * 128), 16);
+                                const uint64_t qd = qb * (2 * C::kPlane / 16) + ((c0 + c) * KB + e) * (C::kBlock / 16);
 #pragma unroll
-                            for (int k = 0; k < 4; k++) mma_ss(d, q_hi + qd + 2 * k, kd + 2 * k, idesc(kKeys, false), true);
-                            commit(&s.k_empty[st]);
+                                for (int k = 0; k < 4; k++)
+                                    mma_ss<PAIR>(d, q_lo + qd + 2 * k, kd + 2 * k, idesc<PAIR>(kKeys, false), c0 + c + e + k > 0);
+#pragma unroll
+                                for (int k = 0; k < 4; k++) mma_ss<PAIR>(d, q_hi + qd + 2 * k, kd + 2 * k, idesc<PAIR>(kKeys, false), true);
+                            }
+                            commit_both<PAIR>(&s.k_empty[st]);
                             if (++st == NK) st = 0, round++;
                         }
                     }
-                    if (ok) commit(&s.s_full[buf]);
+                    if (ok) commit_both<PAIR>(&s.s_full[buf]);
                 }
                 item++;
             }
-            commit(&s.drain);
+            commit<PAIR>(&s.drain);
             wait_drain(&s.drain, 0);
-        } else if (warp == 2 && elect_one()) {
+        } else if (warp == 2 && rank == 0 && elect_one()) {
             // ------------------------------------------------ O = P V
             uint32_t st = 0, round = 0, tile = 0, lands = 0, cleans = 0;  // (at most two parts between landed and clean)
             bool ok = true;
@@ -488,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                             ok = ok && wait(&s.v_full[at], turn & 1, abort, a.err);
                             if (++at == NV) at = 0, turn++;
                         }
-                        if (ok && n > 0 && (z + 1) * C::kPartKeys > past) arrive(&s.landed[lands++ & 1]);
+                        if (ok && n > 0 && (z + 1) * C::kPartKeys > past) arrive_both<PAIR>(&s.landed[lands++ & 1]);
                     };
                     if (past < kKeys) take(0);
 #pragma unroll 1
@@ -506,25 +612,25 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                         if (!ok) break;
                         tc_fence_after();
                         for (int c = 0; c < pieces; c++) {
-                            const uint32_t v0 = smem_u32(v_ring + st * kStage);
+                            const uint32_t v0 = smem_u32(v_ring + st * C::kPiece);
                             const int steps = min(VK, n - c * VK + 15) / 16;
                             for (int k = 0; k < steps; k++) {
                                 const int key = key0 + c * VK + 16 * k;
-                                const uint64_t vd = operand(v0 + value_at<NC>(a, 16 * k), a.v_box * 128);
+                                const uint64_t vd = operand(v0 + value_at<VB>(a, 16 * k), a.v_box * 128);
                                 const uint32_t p = p0 + (key & ~31) + (key & 16) / 2;  // 32 keys: 16 columns of hi, 16 of lo
-                                mma_ts(o, p + 16, vd, idesc(D, true), key > 0);
-                                mma_ts(o, p, vd, idesc(D, true), true);
+                                mma_ts<PAIR>(o, p + 16, vd, idesc<PAIR>(D, true), key > 0);
+                                mma_ts<PAIR>(o, p, vd, idesc<PAIR>(D, true), true);
                             }
-                            commit(&s.v_empty[st]);
+                            commit_both<PAIR>(&s.v_empty[st]);
                             if (++st == NV) st = 0, round++;
                         }
                     }
                     if (!ok) break;
-                    commit(&s.pv_done[buf]);
-                    commit(&s.o_full[ob]);
+                    commit<PAIR>(&s.pv_done[buf]);
+                    commit_both<PAIR>(&s.o_full[ob]);
                 }
             }
-            commit(&s.drain);
+            commit<PAIR>(&s.drain);
             wait_drain(&s.drain, 0);
         }
     } else if (warp < 8) {
@@ -532,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         // With few rows (a.copies 2 or 4) Q lies in the tile several times, and each copy takes its share of a unit's
         // keys: a running maximum and total of its own, P = 0 for the others' keys, joined at the end of the item.
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-        __syncthreads();
+        sync_all<PAIR>();
         tc_fence_after();
         const uint32_t tmem = s.tmem;
         Walk<D> walk(s);
@@ -543,8 +649,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         uint32_t tile = 0, item = 0, msg = 0;
         bool ok = true;
         while (ok && walk.next(a, it)) {
-            const int r = it.tile * kRows + row % span, node = r / a.group;
-            const bool live = row < MR && (row & ~31) % span + it.tile * kRows < a.tokens * a.group;  // the warp has rows
+            const int row0 = it.tile * C::kTileRows + rank * kRows, node = (row0 + row % span) / a.group;
+            const bool live = row < MR && row0 + (row & ~31) % span < a.tokens * a.group;  // the warp has rows
             uint64_t mask = 0;
             if (node < a.tokens) {
                 mask = a.tree ? a.tree[(size_t)it.seq * a.tokens + node] : ~0ull >> (63 - node);
@@ -639,7 +745,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     if ((h + 1) * kChunk % C::kPartKeys) continue;
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) arrive(&s.p_full[buf][h * kChunk / C::kPartKeys]);
+                    if (lane == 0) arrive_leader<PAIR>(&s.p_full[buf][h * kChunk / C::kPartKeys]);
                 }
                 // the running total, with what its rounding lost
                 const float add = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
@@ -663,7 +769,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     } else {
         // ---------------------------------------------------- Q, and the accumulators: rows x half of the columns
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsAcc));
-        __syncthreads();
+        sync_all<PAIR>();
         tc_fence_after();
         const uint32_t tmem = s.tmem;
         Walk<D> walk(s);
@@ -680,9 +786,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             if (more) {
                 // Warp w prepares, and at the end stores, rows w, w+8, ...; lane i < 16 knows where row w+8i lies in q
                 // and out. Rows past the last are left as they are: no one reads their results.
-                const int rows = min(kRows, a.tokens * a.group - nx.tile * kRows);
+                const int row0 = nx.tile * C::kTileRows + rank * kRows, rows = min(kRows, a.tokens * a.group - row0);
                 {
-                    const int r = nx.tile * kRows + w + 8 * (lane & 15), node = r / a.group;
+                    const int r = row0 + w + 8 * (lane & 15), node = r / a.group;
                     where_nx = node < a.tokens ? (((size_t)nx.seq * a.tokens + node) * a.q_heads + nx.kv * a.group + (r - node * a.group)) * D : 0;
                 }
                 const uint32_t qb = round % QB;
@@ -750,6 +856,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) arrive(&s.q_full[qb]);
+                if (PAIR && lane == 0) arrive_leader<PAIR>(&s.q_all);
             }
             if (QB == 2 && !left) {  // the first round only prepares
                 it = nx, where = where_nx, left = more;
@@ -758,7 +865,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             }
             if (QB == 1) it = nx, where = where_nx;
             const uint32_t qb = QB == 2 ? (round - 1) % 2 : 0;
-            const int rows = min(kRows, a.tokens * a.group - it.tile * kRows);
+            const int row0 = it.tile * C::kTileRows + rank * kRows, rows = min(kRows, a.tokens * a.group - row0);
             const bool live = (row & ~31) % span < rows && row < MR;  // the warp has rows
             unsigned char *stage = q_smem + qb * 2 * C::kPlane;
             // pages of the item, checked
@@ -789,12 +896,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                         const int key0 = max(past, z * C::kPartKeys) & ~31, key1 = min(end, (z + 1) * C::kPartKeys);
                         uint64_t odd = 0;
                         for (int k0 = key0; k0 < key1; k0 += 32) {
-                            unsigned char *v0 = v_ring + (piece0 + j * NC + k0 / VK) % NV * kStage;
+                            unsigned char *v0 = v_ring + (piece0 + j * NP + k0 / VK) % NV * C::kPiece;
 #pragma unroll 1
-                            for (int u = tid - 256; u < 32 * 8 * NC; u += 256) {
+                            for (int u = tid - 256; u < 32 * 8 * VB; u += 256) {
                                 const int key = k0 + ((u >> 3) & 31);
                                 if (key < past) continue;
-                                uint4 *p = reinterpret_cast<uint4 *>(v0 + value_at<NC>(a, key % VK) + (u >> 8) * a.v_box * 128 + (u & 7) * 16);
+                                uint4 *p = reinterpret_cast<uint4 *>(v0 + value_at<VB>(a, key % VK) + (u >> 8) * a.v_box * 128 + (u & 7) * 16);
                                 uint4 v = key < end ? *p : make_uint4(0, 0, 0, 0);
                                 uint32_t *wd = &v.x;
 #pragma unroll
@@ -805,10 +912,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                                 *p = v;
                             }
                         }
-                        if (odd) atomicOr(reinterpret_cast<unsigned long long *>(&s.odd_nodes), (unsigned long long)odd);
+                        if (odd) mark_odd<PAIR>(&s.odd_nodes, odd);
                         fence_proxy_async();
                         __syncwarp();
-                        if (lane == 0) arrive(&s.clean[cleans & 1]);
+                        if (lane == 0) arrive_leader<PAIR>(&s.clean[cleans & 1]);
                         cleans++;
                     }
                     if (!ok) break;
@@ -830,7 +937,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     tc_fence_before();
                 }
                 __syncwarp();
-                if (lane == 0) arrive(&s.o_empty[ob]);
+                if (lane == 0) arrive_leader<PAIR>(&s.o_empty[ob]);
             }
             const uint32_t slot = msg & 1;
             if (ok) ok = wait_warp(&s.msg_full[slot], (msg / 2) & 1, abort, a.err);
@@ -849,7 +956,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                         make_float4(acc[2 * i].x * mul, acc[2 * i].y * mul, acc[2 * i + 1].x * mul, acc[2 * i + 1].y * mul);
                 uint64_t odd = row % span < rows ? *(volatile uint64_t *)&s.odd_nodes : 0;
                 if (odd) {  // rare: values that are not finite, for the rows that see them
-                    const int node = (it.tile * kRows + row % span) / a.group;
+                    const int node = (row0 + row % span) / a.group;
                     odd &= a.tree ? a.tree[(size_t)it.seq * a.tokens + node] : ~0ull >> (63 - node);
                     while (odd) {
                         const int nd = __ffsll((long long)odd) - 1;
@@ -870,7 +977,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             ok = !group_any(4, 256, !ok);  // the eight warps stop together
             if (!ok) break;
             if (tid == 256) s.odd_nodes = 0;
-            const size_t part = (size_t)(2 * blockIdx.x + (it.start > s.slot0)) * a.part_rows;
+            const size_t part = (size_t)(2 * team + (it.start > s.slot0)) * a.part_rows + rank * kRows;
             const float nan = __int_as_float(0x7fc00000);
             if (copies == 1) {
                 if (!whole && col0 == 0 && row < rows) a.part_ml[part + row] = make_float2(s.q_scale[qb][row], s.val[slot][row]);
@@ -929,10 +1036,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             more = more && walk.next(a, nx);
         }
     }
-    __syncthreads();
+    sync_all<PAIR>();  // (a pair's CTA stays until the other's MMAs and arrivals are over)
     if (warp == 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(s.tmem));
+        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(s.tmem));
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(s.tmem));
     }
 }
 
@@ -940,18 +1048,18 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
 // after an error: one CTA per (row, head). Warps take every eighth part, so all
 // loads of a row are in flight at once; their sums join in order.
 template <int D>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttendArgs a, int ctas) {
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttendArgs a, int teams) {
     constexpr int V = D / 32;
     __shared__ float sums[8][D];
     __shared__ float2 totals[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int id = blockIdx.x, h = id % a.q_heads, row = id / a.q_heads, seq = row / a.tokens;
-    const int kv = h / a.group, r = (row % a.tokens) * a.group + h % a.group, tile = r / kRows;
+    const int kv = h / a.group, r = (row % a.tokens) * a.group + h % a.group, tile = r / a.tile_rows;
     const int per = a.c.kv_heads * a.row_tiles;
     const int units = units_of(a, a.c.committed(seq, a.tokens));
     const long long w = sum_slots<D>(a, a.seqs, per);
     const long long start = (seq ? sum_slots<D>(a, seq, per) : 0) + (long long)(kv * a.row_tiles + tile) * (units + kItemCost<D>) + kItemCost<D>;
-    const int g = (int)min((long long)ctas, w);
+    const int g = (int)min((long long)teams, w);
     const int c0 = units ? cta_of(start, w, g) : 0, parts = units ? cta_of(start + units - 1, w, g) - c0 + 1 : 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     float *out = a.out + (size_t)id * D;
@@ -974,7 +1082,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Atten
             const int p = p0 + 8 * i;
             ml[i] = make_float2(-INFINITY, 0.0f);
             if (p < parts) {
-                const size_t at = (size_t)(2 * (c0 + p) + (p == 0 && late)) * a.part_rows + r % kRows;
+                const size_t at = (size_t)(2 * (c0 + p) + (p == 0 && late)) * a.part_rows + r % a.tile_rows;
                 const float *src = a.part_acc + at * D + lane * V;
                 ml[i] = __ldcg(a.part_ml + at);
                 if constexpr (V == 2) {
@@ -1051,29 +1159,34 @@ int part_rows(int tokens, int group) { return tokens * group < kRows ? tokens * 
 
 size_t ml_bytes(int rows) { return (size_t)2 * kMaxCtas * rows * sizeof(float2); }
 
-template <int D, int MR>
+template <int D, int MR, bool PAIR>
 int launch(const AttendArgs &a, const CUtensorMap &k_map, const CUtensorMap &v_map) {
-    using C = Cfg<D, MR>;
-    if (int rc = cudaFuncSetAttribute(tree_attention_kernel<D, MR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem)) return rc;
+    using C = Cfg<D, MR, PAIR>;
+    constexpr int kPeers = PAIR ? 2 : 1;
+    if (int rc = cudaFuncSetAttribute(tree_attention_kernel<D, MR, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem)) return rc;
     // no more CTAs than the longest sequences that the table allows could use
     const long long units = (((long long)a.c.table_pages << a.c.shift) + kKeys - 1) / kKeys;
     const long long most = (long long)a.seqs * a.c.kv_heads * a.row_tiles * (units + kItemCost<D>);
-    const int ctas = (int)(most < kMaxCtas ? most : kMaxCtas);
+    const int teams = (int)(most < kMaxCtas / kPeers ? most : kMaxCtas / kPeers);
     cudaLaunchConfig_t cfg = {};
     cfg.stream = launch_stream;
-    cudaLaunchAttribute pdl[1];
-    pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    pdl[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = pdl;
-    cfg.numAttrs = 1;
-    cfg.gridDim = dim3(ctas);
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = kPeers;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = PAIR ? 2 : 1;
+    cfg.gridDim = dim3(teams * kPeers);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = C::kSmem;
-    if (int rc = cudaLaunchKernelEx(&cfg, tree_attention_kernel<D, MR>, a, k_map, v_map)) return rc;
+    if (int rc = cudaLaunchKernelEx(&cfg, tree_attention_kernel<D, MR, PAIR>, a, k_map, v_map)) return rc;
+    cfg.numAttrs = 1;
     cfg.gridDim = dim3((unsigned)(a.seqs * a.tokens * a.q_heads));
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
-    return cudaLaunchKernelEx(&cfg, join_kernel<D>, a, ctas);
+    return cudaLaunchKernelEx(&cfg, join_kernel<D>, a, teams);
 }
 
 }  // namespace
@@ -1104,26 +1217,27 @@ extern "C" int qg_tree_attention(float *out, const float *q, const qg_kv_cache *
     a.tokens = tokens;
     a.q_heads = q_heads;
     a.group = q_heads / a.c.kv_heads;
-    a.row_tiles = (tokens * a.group + kRows - 1) / kRows;
-    a.part_rows = part_rows(tokens, a.group);
-    a.k_box = a.c.page_tokens() < kKeys ? a.c.page_tokens() : kKeys;
-    const int v_keys = kStage / (2 * a.c.head_dim);
-    a.v_box = a.c.page_tokens() < v_keys ? a.c.page_tokens() : v_keys;
+    // Few rows: heads of 64 and 128 values, whose units take little time, share a unit's keys among copies of Q; heads of
+    // 256 keep only 64 rows of Q, and the room goes to the rings. Many rows of heads of 256: pairs of CTAs.
+    const int rows = tokens * a.group;
+    const bool pair = a.c.head_dim == 256 && rows > kRows;
+    a.copies = a.c.head_dim == 256 || rows > 64 ? 1 : a.c.head_dim == 128 || rows > 32 ? 2 : 4;
+    a.tile_rows = pair ? 2 * kRows : kRows;
+    a.row_tiles = (rows + a.tile_rows - 1) / a.tile_rows;
+    a.part_rows = rows < a.tile_rows ? rows : a.tile_rows;
+    const int page = a.c.page_tokens(), k_rows = pair ? kKeys / 2 : kKeys, v_blocks = a.c.head_dim / (pair ? 128 : 64);
+    const int v_rows = 16384 / (128 * v_blocks);
+    a.k_box = page < k_rows ? page : k_rows;
+    a.k_blocks = pair && a.k_box == k_rows ? 2 : 1;
+    a.v_box = page < v_rows ? page : v_rows;
     a.err = static_cast<int *>(workspace);
     a.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + 256);
-    a.part_acc = reinterpret_cast<float *>(static_cast<char *>(workspace) + 256 + ml_bytes(a.part_rows));
+    a.part_acc = reinterpret_cast<float *>(static_cast<char *>(workspace) + 256 + ml_bytes(part_rows(tokens, a.group)));
     CUtensorMap k_map, v_map;
-    if (int rc = pool_map(&k_map, a.c, a.c.k, a.k_box, 1)) return rc;
-    if (int rc = pool_map(&v_map, a.c, a.c.v, a.v_box, a.c.head_dim / 64)) return rc;
-    // Few rows: heads of 64 and 128 values, whose units take little time, share a unit's keys among copies of Q; heads of
-    // 256 keep only 64 rows of Q, and the room goes to the ring.
-    const int rows = tokens * a.group;
-    a.copies = a.c.head_dim == 256 || rows > 64 ? 1 : rows > 32 ? 2 : 4;
-    if (a.c.head_dim == 64) return launch<64, 128>(a, k_map, v_map);
-    if (a.c.head_dim == 128 && rows <= 32) {
-        a.copies = 2;
-        return launch<128, 64>(a, k_map, v_map);
-    }
-    if (a.c.head_dim == 128) return launch<128, 128>(a, k_map, v_map);
-    return rows <= 64 ? launch<256, 64>(a, k_map, v_map) : launch<256, 128>(a, k_map, v_map);
+    if (int rc = pool_map(&k_map, a.c, a.c.k, a.k_box, a.k_blocks)) return rc;
+    if (int rc = pool_map(&v_map, a.c, a.c.v, a.v_box, v_blocks)) return rc;
+    if (a.c.head_dim == 64) return launch<64, 128, false>(a, k_map, v_map);
+    if (a.c.head_dim == 128) return rows <= 32 ? launch<128, 64, false>(a, k_map, v_map) : launch<128, 128, false>(a, k_map, v_map);
+    if (pair) return launch<256, 128, true>(a, k_map, v_map);
+    return rows <= 64 ? launch<256, 64, false>(a, k_map, v_map) : launch<256, 128, false>(a, k_map, v_map);
 }
