@@ -580,6 +580,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         } else if (warp == 2 && rank == 0 && elect_one()) {
             // ------------------------------------------------ O = P V
             uint32_t st = 0, round = 0, tile = 0, lands = 0, cleans = 0;  // (at most two parts between landed and clean)
+            // descriptor steps for 16 and 32 keys within a piece: a box of 16 or 32 keys ends with them
+            const uint32_t step16 = value_at<VB>(a, 16) / 16, step32 = value_at<VB>(a, 32) / 16;
             bool ok = true;
             while (ok && walk.next(a, it)) {
                 for (int j = 0; ok && j < it.count; j++, tile++) {
@@ -601,28 +603,32 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     for (int z = 0; ok && z < C::kParts; z++) {
                         // Past the last key there is nothing to multiply, but the softmax writes there too, and must be
                         // done before S takes the place again.
-                        const int key0 = z * C::kPartKeys, n = min(C::kPartKeys, keys - key0), pieces = (n + VK - 1) / VK;
+                        const int key0 = z * C::kPartKeys, end = min(key0 + C::kPartKeys, keys);
                         if (past >= kKeys) take(z);
                         else if (z + 1 < C::kParts) take(z + 1);  // a part ahead, so that the cleaning is not waited for
-                        if (ok && n > 0 && key0 + C::kPartKeys > past) {
+                        if (ok && key0 < end && key0 + C::kPartKeys > past) {
                             ok = wait(&s.clean[cleans & 1], cleans / 2 & 1, abort, a.err);
                             cleans++;
                         }
                         ok = ok && wait(&s.p_full[buf][z], (tile / 2) & 1, abort, a.err);
                         if (!ok) break;
                         tc_fence_after();
-                        for (int c = 0; c < pieces; c++) {
-                            const uint32_t v0 = smem_u32(v_ring + st * C::kPiece);
-                            const int steps = min(VK, n - c * VK + 15) / 16;
-                            for (int k = 0; k < steps; k++) {
-                                const int key = key0 + c * VK + 16 * k;
-                                const uint64_t vd = operand(v0 + value_at<VB>(a, 16 * k), a.v_box * 128);
-                                const uint32_t p = p0 + (key & ~31) + (key & 16) / 2;  // 32 keys: 16 columns of hi, 16 of lo
-                                mma_ts<PAIR>(o, p + 16, vd, idesc<PAIR>(D, true), key > 0);
-                                mma_ts<PAIR>(o, p, vd, idesc<PAIR>(D, true), true);
+                        uint64_t vd = operand(smem_u32(v_ring + st * C::kPiece), a.v_box * 128);
+                        uint32_t p = p0 + key0;  // 32 keys: 16 columns of hi, 16 of lo
+#pragma unroll 1
+                        for (int key = key0; key < end; key += 32) {
+                            mma_ts<PAIR>(o, p + 16, vd, idesc<PAIR>(D, true), key > 0);
+                            mma_ts<PAIR>(o, p, vd, idesc<PAIR>(D, true), true);
+                            if (key + 16 < end) {
+                                mma_ts<PAIR>(o, p + 24, vd + step16, idesc<PAIR>(D, true), true);
+                                mma_ts<PAIR>(o, p + 8, vd + step16, idesc<PAIR>(D, true), true);
                             }
-                            commit_both<PAIR>(&s.v_empty[st]);
-                            if (++st == NV) st = 0, round++;
+                            p += 32, vd += step32;
+                            if ((key + 32) % VK == 0 || key + 32 >= keys) {
+                                commit_both<PAIR>(&s.v_empty[st]);
+                                if (++st == NV) st = 0, round++;
+                                vd = operand(smem_u32(v_ring + st * C::kPiece), a.v_box * 128);
+                            }
                         }
                     }
                     if (!ok) break;
