@@ -54,9 +54,14 @@ __device__ __forceinline__ float split(float x, float scale, float &frac) {
     frac = t - n;
     return n;
 }
+__device__ __forceinline__ float ex2(float x) {  // the instruction: |x| <= 1 here, which needs no scaling
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // 2^f * 2^rel for 0 <= f <= 1 and rel <= 0: the power of two goes into the exponent; weights below 2^-126 are zero.
 __device__ __forceinline__ float weigh(float f, float rel) {
-    return rel < -126.0f ? 0.0f : exp2f(f) * __int_as_float(((int)rel + 127) << 23);
+    return rel < -126.0f ? 0.0f : ex2(f) * __int_as_float(((int)rel + 127) << 23);
 }
 // 2^rel for rel <= 0 (0 below the range), to bring a sum to another M.
 __device__ __forceinline__ double shift_down(float rel) {
@@ -103,8 +108,8 @@ __device__ __forceinline__ float warp_max(float x) {
 
 // Of 8 values of a thread: the largest n, and the sum of the weights relative to it. Conversions and floor run at an
 // eighth of the rate of additions here and would bound the kernel (50 us instead of the copy's 17 for 12 x 17 x
-// 131072 logits), so for |t| < 2^21 floor comes from rounding by an addition, n is read from that sum's bits, and 2^f
-// 2^(n - top) is put together as the bits of a double.
+// 131072 logits), so for |t| < 2^21 floor comes from an addition that rounds down, n is read from that sum's bits, and
+// 2^f 2^(n - top) is put together as the bits of a double.
 __device__ __forceinline__ void weigh8(const float (&x)[8], float scale, float &top, double &sum) {
     constexpr float kMagic = 12582912.0f, kRange = 2097152.0f;  // 1.5 * 2^23, 2^21
     float t[8], most = -INFINITY;
@@ -120,17 +125,16 @@ __device__ __forceinline__ void weigh8(const float (&x)[8], float scale, float &
         float f[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const float tc = fmaxf(t[i], -kRange), u = __fadd_rn(tc, kMagic), d = __fsub_rn(tc, __fsub_rn(u, kMagic));
-            const bool up = d < 0.0f;  // u rounded up
-            n[i] = __float_as_int(u) - (up ? 1 : 0);
-            f[i] = up ? __fadd_rn(d, 1.0f) : d;
+            const float tc = fmaxf(t[i], -kRange), u = __fadd_rd(tc, kMagic);  // the sum's last bit is a one
+            n[i] = __float_as_int(u);
+            f[i] = __fsub_rn(tc, __fsub_rn(u, kMagic));
             m = max(m, n[i]);
         }
+        const int scale_down = ((1023 - 127) << 20) - (m << 20), least = m - 900;  // 2^-900 is nothing beside the largest
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const unsigned g = __float_as_uint(exp2f(f[i]));  // in [1, 2]
-            const int rel = max(n[i] - m, -900);              // 2^-900 is nothing beside the largest
-            sum += __hiloint2double((int)((g >> 3) + ((1023 - 127) << 20)) + (rel << 20), (int)(g << 29));
+            const unsigned g = __float_as_uint(ex2(f[i]));  // in [1, 2]
+            sum += __hiloint2double((int)(g >> 3) + (max(n[i], least) << 20) + scale_down, (int)(g << 29));
         }
         top = (float)(m - __float_as_int(kMagic));
     } else {
@@ -153,6 +157,7 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_kernel(const VerifyArgs a
     __shared__ double sums[kWarps];
     __shared__ float tops[kWarps];
     __shared__ int bests[kWarps];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int c = blockIdx.x % a.chunks, r = blockIdx.x / a.chunks, warp = threadIdx.x / 32;
     const float *row = a.logits + (size_t)r * a.vocab;
@@ -477,8 +482,15 @@ extern "C" int qg_verify_tree(int *path, int *accepted, int *next, const float *
     const VerifyArgs a = {path, accepted, next, logits, draft, parents, draft_probs, uniforms, scale, tokens, vocab, chunks, stats,
                           reinterpret_cast<double *>(stats + (size_t)seqs * tokens * chunks)};
     const unsigned grid = (unsigned)((size_t)seqs * tokens * chunks);
-    if (scale == 0.0f) chunk_kernel<true><<<grid, kChunkThreads, 0, launch_stream>>>(a);
-    else chunk_kernel<false><<<grid, kChunkThreads, 0, launch_stream>>>(a);
-    if (int rc = cudaGetLastError()) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kChunkThreads);
+    cfg.stream = launch_stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (int rc = cudaLaunchKernelEx(&cfg, scale == 0.0f ? chunk_kernel<true> : chunk_kernel<false>, a)) return rc;
     return draft_probs ? launch_walk<true>(a, seqs) : launch_walk<false>(a, seqs);
 }
