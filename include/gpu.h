@@ -284,7 +284,9 @@ int qg_qk_norm_rope(float *q_out, const qg_kv_cache *cache, int layer, const flo
  * node i sees nodes 0..i. A row that sees nothing is zero. What a row does not
  * see has no effect on it, whatever its bits (NaN and infinities included).
  * q and out: [row][q_heads][head_dim] F32, 16-byte aligned. The workspace is
- * zero-filled once; calls sharing it must not overlap on the device.
+ * zero-filled once; calls sharing it must not overlap on the device. Waits in
+ * the kernel are bounded: should one run out, every row is NaN, in this call
+ * and later ones, until the workspace is zero-filled again.
  * Deterministic, graph-capturable, no host synchronisation. */
 int qg_attention_workspace_bytes(int seqs, int tokens, int q_heads, int kv_heads, int head_dim, size_t *bytes);
 int qg_tree_attention(float *out, const float *q, const qg_kv_cache *cache, int layer, const uint64_t *tree, float scale,

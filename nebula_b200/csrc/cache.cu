@@ -171,7 +171,7 @@ constexpr int kCommitCtas = 8;  // one cluster per sequence
 // ascends, so path[i] >= i: a destination is never a later node's source, and
 // a thread that reads nodes in ascending order before it writes them moves
 // them as if at once. Eight are read before they are written: with one at a
-// time each move waits for its own load (48 sequences x 24 layers: 45 us). Nodes
+// time each move waits for its own load (48 sequences x 24 layers: 45 us, so 32). Nodes
 // already in place are a prefix. The length is written after the cluster's
 // barrier, when every CTA has read it, so lengths_out may be the cache's own.
 // Bound by HBM for many sequences, by the chain length - page - row for one.

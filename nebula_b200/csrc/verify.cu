@@ -75,6 +75,25 @@ __device__ __forceinline__ float weight(float scale, const Stats &r, float x, in
     return weigh(f, n - r.top);
 }
 
+// The weights of 8 neighbouring values from v on. Conversions and floor run at an eighth of the rate of additions, so for
+// |M| < 2^20 floor comes from an addition that rounds down, and n is read from that sum's bits.
+constexpr float kMagic = 12582912.0f, kRange = 2097152.0f;  // 1.5 * 2^23, 2^21
+__device__ __forceinline__ void weights8(float scale, const Stats &r, float (&x)[8], int v) {
+    if (scale > 0.0f && fabsf(r.top) < kRange / 2) {  // and no t is above the row's M + 1
+        const int top = __float_as_int(kMagic) + (int)r.top;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float tc = fmaxf(__fmul_rn(x[i], scale), -kRange), u = __fadd_rd(tc, kMagic);
+            const int rel = __float_as_int(u) - top;
+            const float g = ex2(__fsub_rn(tc, __fsub_rn(u, kMagic)));
+            x[i] = rel < -126 ? 0.0f : g * __int_as_float((rel + 127) << 23);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = weight(scale, r, x[i], v + i);
+    }
+}
+
 // A part of a row brought to the row's M.
 __device__ __forceinline__ double brought(const Stats &s, float top) { return s.sum * shift_down(s.top - top); }
 
@@ -106,12 +125,10 @@ __device__ __forceinline__ float warp_max(float x) {
     return __int_as_float(m < 0 ? m ^ 0x7fffffff : m);
 }
 
-// Of 8 values of a thread: the largest n, and the sum of the weights relative to it. Conversions and floor run at an
-// eighth of the rate of additions here and would bound the kernel (50 us instead of the copy's 17 for 12 x 17 x
-// 131072 logits), so for |t| < 2^21 floor comes from an addition that rounds down, n is read from that sum's bits, and
-// 2^f 2^(n - top) is put together as the bits of a double.
+// Of 8 values of a thread: the largest n, and the sum of the weights relative to it, floor as in weights8 (|t| < 2^21); 2^f 2^(n - top)
+// is put together as the bits of a double. (With conversions, which would bound the kernel, 50 us for 12 x 17 x 131072
+// logits.)
 __device__ __forceinline__ void weigh8(const float (&x)[8], float scale, float &top, double &sum) {
-    constexpr float kMagic = 12582912.0f, kRange = 2097152.0f;  // 1.5 * 2^23, 2^21
     float t[8], most = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
@@ -223,95 +240,117 @@ template <bool DRAWN>
 __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) {
     constexpr int kWarps = kWalkThreads / 32, kCtas = DRAWN ? kDrawnCtas : 1;
     static_assert(kWalkThreads * 8 == kChunk, "eight values of a chunk to a thread");
+    // Chunks whose loads are in flight together (7 x 6 x 50001 logits 12.4 us, 12 x 17 x 131072 39.7; four: 13.0, 39.0).
+    constexpr int kBatch = 2;
     __shared__ Stats rows[kMaxNodes];
-    constexpr int kBatch = 8;  // chunks between two barriers
     __shared__ double sums[kWarps], batch[DRAWN ? kBatch : 1][kWarps];
-    __shared__ float mine[kMaxNodes], guess[kMaxNodes], uniform[kMaxNodes];
-    __shared__ int draft[kMaxNodes], parent[kMaxNodes], gone[kMaxNodes], path[kMaxNodes], n_gone, count, at_node, refused;
+    __shared__ unsigned long long kids[kMaxNodes];     // of a node: its children
+    __shared__ float held[kMaxNodes];                  // the target's weight of a draft, 0 after an older sibling's equal
+    __shared__ unsigned takes[2], bads[2], sane[2], weighty[2];  // nodes as bits
+    __shared__ int draft[kMaxNodes], parent[kMaxNodes], path[kMaxNodes], count, at_node, refused;
+    __shared__ float first_uniform;
     const int seq = blockIdx.x / kCtas, rank = blockIdx.x % kCtas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const size_t base = (size_t)seq * a.tokens;
-    const bool greedy = a.scale == 0.0f;
+    const bool greedy = a.scale == 0.0f, node = tid < a.tokens;
     bool sound = true;
-    if (tid < a.tokens) {
+    float u = 0.0f;
+    if (tid < kMaxNodes) kids[tid] = 0;
+    if (node) {
         parent[tid] = a.parents[base + tid];
         draft[tid] = a.draft[base + tid];
-        uniform[tid] = a.uniforms[base + tid];
+        u = a.uniforms[base + tid];
         sound = tid == 0 || (parent[tid] >= -1 && parent[tid] < tid);
     }
+    if (tid == 0) first_uniform = u;
     sound = __syncthreads_and(sound);
-    const bool tries = sound && tid > 0 && tid < a.tokens && parent[tid] >= 0 && (unsigned)draft[tid] < (unsigned)a.vocab;
+    const bool used = sound && tid > 0 && node && parent[tid] >= 0, tries = used && (unsigned)draft[tid] < (unsigned)a.vocab;
     const size_t above = tries ? base + parent[tid] : 0;
     const float x = tries ? a.logits[above * a.vocab + draft[tid]] : 0.0f;
-    if (DRAWN && tries) guess[tid] = a.probs[(base + tid) * a.vocab + draft[tid]];
+    const float guess = DRAWN && tries ? a.probs[(base + tid) * a.vocab + draft[tid]] : 0.0f;
+    if (used) atomicOr(&kids[parent[tid]], 1ull << tid);
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    // ---- the rows' M and total: a warp per row
-    for (int r = warp; r < a.tokens; r += kWarps) {
-        const Stats *part = a.stats + (base + r) * a.chunks;
-        float top = -INFINITY;
-        int best = 0x7fffffff, bad = 0;
-        double sum = 0.0;
-        for (int c = lane; c < a.chunks; c += 32) {
-            const Stats s = part[c];
-            bad |= s.best == kBad;
-            if (s.best < 0) continue;
-            if (s.top > top) {
-                sum *= shift_down(top - s.top);
-                top = s.top, best = s.best;
-            } else if (s.top == top && s.best < best) {
-                best = s.best;
-            }
-            sum += brought(s, top);
+    // ---- the rows' M and total: a warp per row, two rows' first 64 chunks asked for together
+    for (int r0 = warp; r0 < a.tokens; r0 += 2 * kWarps) {
+        Stats ahead[2][2];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = r0 + i / 2 * kWarps, c = lane + i % 2 * 32;
+            ahead[i / 2][i % 2] = r < a.tokens && c < a.chunks ? a.stats[(base + r) * a.chunks + c] : Stats{0.0, -INFINITY, kNone};
         }
-        const float m = warp_max(top);
-        sum = m > -INFINITY ? warp_sum(sum * shift_down(top - m)) : 0.0;
-        best = __reduce_min_sync(0xffffffffu, top == m ? best : 0x7fffffff);
-        bad = __any_sync(0xffffffffu, bad);
-        if (lane == 0) rows[r] = {greedy ? 1.0 : sum, m, bad ? kBad : m > -INFINITY ? best : kNone};
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int r = r0 + j * kWarps;
+            if (r >= a.tokens) break;
+            float top = -INFINITY;
+            int best = 0x7fffffff, bad = 0;
+            double sum = 0.0;
+            auto join = [&](const Stats &s) {
+                bad |= s.best == kBad;
+                if (s.best < 0) return;
+                if (s.top > top) {
+                    sum *= shift_down(top - s.top);
+                    top = s.top, best = s.best;
+                } else if (s.top == top && s.best < best) {
+                    best = s.best;
+                }
+                sum += brought(s, top);
+            };
+            join(ahead[j][0]);
+            join(ahead[j][1]);
+            for (int c = lane + 64; c < a.chunks; c += 32) join(a.stats[(base + r) * a.chunks + c]);
+            const float m = warp_max(top);
+            sum = m > -INFINITY ? warp_sum(sum * shift_down(top - m)) : 0.0;
+            best = __reduce_min_sync(0xffffffffu, top == m ? best : 0x7fffffff);
+            bad = __any_sync(0xffffffffu, bad);
+            if (lane == 0) rows[r] = {greedy ? 1.0 : sum, m, bad ? kBad : m > -INFINITY ? best : kNone};
+        }
     }
     __syncthreads();
-    // ---- the walk
+    // ---- the walk: a thread per node decides whether it would be taken were it reached with all older siblings
+    // refused, so that what is left to do one after the other is to follow bits
     if (warp < kMaxNodes / 32) {
-        if (tries) mine[tid] = weight(a.scale, rows[parent[tid]], x, draft[tid]);  // the target's weight of each draft
+        float w = tries ? weight(a.scale, rows[parent[tid]], x, draft[tid]) : 0.0f;
+        const unsigned long long older = tries ? kids[parent[tid]] & ((1ull << tid) - 1) : 0;
+        if constexpr (!DRAWN)
+            for (unsigned long long m = older; m; m &= m - 1)
+                if (draft[__ffsll(m) - 1] == draft[tid]) w = 0.0f;  // a token leaves p once
+        held[tid] = w;
         asm volatile("bar.sync 1, 64;" ::: "memory");
-    }
-    if (tid == 0) {
-        int cur = 0, n = 0, child = -1, left_out = 0;
-        bool ok = sound && rows[0].best >= 0;
-        double left = rows[0].sum;
-        path[0] = 0;
-        for (int c = 1; ok && c < a.tokens; c++) {  // children come after their parent
-            if (parent[c] != cur) continue;
-            if ((unsigned)draft[c] >= (unsigned)a.vocab || (DRAWN && child >= 0)) {
-                ok = false;
-                break;
-            }
-            float w = mine[c];
-            bool take;
+        bool take = false;
+        if (tries) {
+            double left = rows[parent[tid]].sum;
             if constexpr (DRAWN) {
-                take = __fmul_rn(uniform[c], guess[c]) < w / (float)left;
+                take = __fmul_rn(u, guess) < w / (float)left;
             } else {
-                for (int g = 0; g < left_out; g++)
-                    if (gone[g] == draft[c]) w = 0.0f;
-                take = (double)uniform[c] * left < (double)w;
-            }
-            if (take) {
-                cur = c;
-                path[++n] = c;
-                child = -1;
-                left_out = 0;
-                ok = rows[c].best >= 0;
-                left = rows[c].sum;
-            } else {
-                child = c;
-                if constexpr (!DRAWN) {
-                    if (w > 0.0f) gone[left_out++] = draft[c];
-                    left -= (double)w;
-                }
+                for (unsigned long long m = older; m; m &= m - 1) left -= (double)held[__ffsll(m) - 1];
+                take = (double)u * left < (double)w;
             }
         }
+        const unsigned t = __ballot_sync(0xffffffffu, take), b = __ballot_sync(0xffffffffu, used && !tries);
+        const unsigned s = __ballot_sync(0xffffffffu, node && rows[node ? tid : 0].best >= 0), h = __ballot_sync(0xffffffffu, w > 0.0f);
+        if (lane == 0) takes[warp] = t, bads[warp] = b, sane[warp] = s, weighty[warp] = h;
+        asm volatile("bar.sync 1, 64;" ::: "memory");
+    }
+    auto bits = [](const unsigned (&m)[2]) { return m[0] | (unsigned long long)m[1] << 32; };
+    if (tid == 0) {
+        const unsigned long long taken = bits(takes), bad = bits(bads), good = bits(sane);
+        int cur = 0, n = 0;
+        bool ok = sound && (good & 1);
+        refused = -1;
+        path[0] = 0;
+        while (ok) {
+            const unsigned long long k = kids[cur], first = DRAWN ? k & (~k + 1) : k, t = first & taken;
+            if (!t) {
+                ok = !(bad & k) && !(DRAWN && (k & (k - 1)));
+                refused = __ffsll(k) - 1;
+                break;
+            }
+            const unsigned long long c = t & (~t + 1);
+            ok = !(bad & k & (c - 1)) && (good & c);
+            cur = __ffsll(c) - 1;
+            path[++n] = cur;
+        }
         at_node = ok ? cur : -1;
-        refused = child;
-        n_gone = left_out;
         count = ok ? n : -1;
     }
     __syncthreads();
@@ -325,29 +364,53 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) 
     // ---- what is left of the last node's row
     const float *row = a.logits + (base + at_node) * a.vocab;
     const Stats r = rows[at_node];
-    const float total = (float)r.sum;
+    const float total = (float)r.sum, inverse = __frcp_rn(total);
     const float *q = DRAWN && refused >= 0 ? a.probs + (base + refused) * a.vocab : nullptr;
     const int lead = chunk_lead(row);
+    const unsigned long long gone = DRAWN ? 0 : kids[at_node] & bits(weighty);  // nodes whose drafts have left p
     // the thread's eight neighbouring values of chunk c
-    auto left8 = [&](int c, float (&w)[8]) {
+    // (q's rows may lie otherwise on the 16-byte boundaries: twelve values from the boundary before, of which eight from
+    // `off` on are the thread's)
+    constexpr int kY = DRAWN ? 12 : 8;
+    const int off = DRAWN && q ? (chunk_lead(q) - lead) & 3 : 0;
+    auto fetch = [&](int c, float (&w)[8], float (&y)[kY]) {
         const int v = c * kChunk - lead + 8 * tid;
-        float y[8];
         load4(row, a.vocab, v, *reinterpret_cast<float(*)[4]>(&w[0]));
         load4(row, a.vocab, v + 4, *reinterpret_cast<float(*)[4]>(&w[4]));
         if (DRAWN && q) {
-            load4(q, a.vocab, v, *reinterpret_cast<float(*)[4]>(&y[0]));
-            load4(q, a.vocab, v + 4, *reinterpret_cast<float(*)[4]>(&y[4]));
+            load4(q, a.vocab, v - off, *reinterpret_cast<float(*)[4]>(&y[0]));
+            load4(q, a.vocab, v - off + 4, *reinterpret_cast<float(*)[4]>(&y[4]));
+            if (off) load4(q, a.vocab, v - off + 8, *reinterpret_cast<float(*)[4]>(&y[8]));
         }
+    };
+    auto left8 = [&](int c, float (&w)[8], float (&y)[kY]) {
+        const int v = c * kChunk - lead + 8 * tid;
+        if constexpr (DRAWN) {
+            if (off & 1) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            w[i] = weight(a.scale, r, w[i], v + i);  // none outside the row
-            if constexpr (DRAWN) {
-                w[i] /= total;
-                if (q) w[i] = v + i >= 0 && v + i < a.vocab ? fmaxf(w[i] - y[i], 0.0f) : 0.0f;
-            } else {
-                for (int g = 0; g < n_gone; g++)
-                    if (gone[g] == v + i) w[i] = 0.0f;
+                for (int i = 0; i < kY - 1; i++) y[i] = y[i + 1];
             }
+            if (off & 2) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) y[i] = y[i + 2];
+            }
+        }
+        weights8(a.scale, r, w, v);  // none outside the row
+        if constexpr (DRAWN) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                // w/total with one reciprocal for all: from a correctly rounded reciprocal one step on the remainder
+                // leads to the correctly rounded quotient (P. Markstein, 1990), w < 2^-100 aside
+                const float p = w[i] * inverse;
+                w[i] = fmaf(fmaf(-p, total, w[i]), inverse, p);
+                if (q) w[i] = v + i >= 0 && v + i < a.vocab ? fmaxf(w[i] - y[i], 0.0f) : 0.0f;
+            }
+        }
+        for (unsigned long long m = gone; m; m &= m - 1) {
+            const int g = draft[__ffsll(m) - 1] - v;
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (g == i) w[i] = 0.0f;
         }
     };
     double *rest = a.rest + (size_t)seq * a.chunks;
@@ -358,39 +421,51 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) 
             const Stats s = a.stats[(base + at_node) * a.chunks + c];
             if (greedy) return s.best == r.best ? 1.0 : 0.0;
             double w = s.best >= 0 ? brought(s, r.top) : 0.0;
-            for (int g = 0; g < n_gone; g++)
-                if ((gone[g] + lead) / kChunk == c) w -= (double)weight(a.scale, r, row[gone[g]], gone[g]);
+            for (unsigned long long m = gone; m; m &= m - 1) {
+                const int g = __ffsll(m) - 1;
+                if ((draft[g] + lead) / kChunk == c) w -= (double)held[g];
+            }
             return fmax(w, 0.0);
         }
     };
     // ---- the chunk that holds the aim: every warp finds it for itself, a lane takes neighbouring chunks
     const int per = (a.chunks + 31) / 32, c0 = min(lane * per, a.chunks), c1 = min(c0 + per, a.chunks);
-    double whole = 0.0, upto = 0.0, sum = 0.0;
+    constexpr int kKept = 4;  // a lane's first chunks, whose sums stay in registers
+    double whole = 0.0, upto = 0.0, sum = 0.0, kept[kKept];
     for (;;) {
         if constexpr (DRAWN) {
-            for (int c0 = rank; c0 < a.chunks; c0 += kBatch * kCtas) {
-#pragma unroll 1
-                for (int i = 0; i < kBatch && c0 + i * kCtas < a.chunks; i++) {
-                    float w[8];
-                    left8(c0 + i * kCtas, w);
+            const int full = (a.vocab + lead + kChunk - 1) / kChunk;  // chunks that hold values: all, or all but the last
+            for (int b0 = rank; b0 < full; b0 += kBatch * kCtas) {
+                float w[kBatch][8], y[kBatch][kY];
+#pragma unroll
+                for (int i = 0; i < kBatch; i++) fetch(b0 + i * kCtas, w[i], y[i]);  // -infinity past the row's end
+#pragma unroll
+                for (int i = 0; i < kBatch; i++) {
+                    if (b0 + i * kCtas >= full) break;
+                    left8(b0 + i * kCtas, w[i], y[i]);
                     double part = 0.0;
 #pragma unroll
-                    for (int k = 0; k < 8; k++) part += (double)w[k];
+                    for (int k = 0; k < 8; k++) part += (double)w[i][k];
                     part = warp_sum(part);
                     if (lane == 0) batch[i][warp] = part;
                 }
                 __syncthreads();
-                if (tid < kBatch && c0 + tid * kCtas < a.chunks) {
+                if (tid < kBatch && b0 + tid * kCtas < full) {
                     double all = 0.0;
                     for (int k = 0; k < kWarps; k++) all += batch[tid][k];
-                    __stcg(rest + c0 + tid * kCtas, all);
+                    __stcg(rest + b0 + tid * kCtas, all);
                 }
                 __syncthreads();
             }
+            if (rank == 0 && tid == 0 && full < a.chunks) __stcg(rest + full, 0.0);
             cg::this_cluster().sync();  // the sums are there
         }
         sum = 0.0;
-        for (int c = c0; c < c1; c++) sum += chunk_sum(c);
+#pragma unroll
+        for (int k = 0; k < kKept; k++) kept[k] = c0 + k < c1 ? chunk_sum(c0 + k) : 0.0;
+#pragma unroll
+        for (int k = 0; k < kKept; k++) sum += kept[k];
+        for (int c = c0 + kKept; c < c1; c++) sum += chunk_sum(c);
         upto = warp_scan(sum);
         whole = __shfl_sync(0xffffffffu, upto, 31);
         if (!DRAWN || whole > 0.0 || !q) break;
@@ -398,7 +473,7 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) 
         cg::this_cluster().sync();  // the sums were read
     }
     if (rank) return;
-    const double aim = (double)uniform[0] * whole;
+    const double aim = (double)first_uniform * whole;
     const int owner = claim(sum, upto, aim);
     if (owner < 0) {  // not met: a row with a distribution has weight left, for what was refused was not all of it
         if (tid == 0) a.next[seq] = -1;
@@ -408,18 +483,22 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) 
     double before = upto - sum;
     if (lane == owner) {
         double run = before;
-        for (int k = c0; k < c1; k++) {
-            const double w = chunk_sum(k);
-            if (w > 0.0) c = k, before = run;
+        bool past = false;
+        auto look = [&](int k, double w) {
+            if (!past && w > 0.0) c = k, before = run;
             run += w;
-            if (run > aim) break;
-        }
+            past |= run > aim;
+        };
+#pragma unroll
+        for (int k = 0; k < kKept; k++) look(c0 + k, kept[k]);
+        for (int k = c0 + kKept; k < c1 && !past; k++) look(k, chunk_sum(k));
     }
     c = __shfl_sync(0xffffffffu, c, owner);
     before = __shfl_sync(0xffffffffu, before, owner);
     // ---- the place in the chunk
-    float w[8];
-    left8(c, w);
+    float w[8], y[kY];
+    fetch(c, w, y);
+    left8(c, w, y);
     double part = 0.0;
 #pragma unroll
     for (int i = 0; i < 8; i++) part += (double)w[i];

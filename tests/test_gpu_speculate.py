@@ -469,6 +469,48 @@ def test_acceptance_malformed_trees(L):
         assert nxt[0] == (2 if first == 2 else -1)
 
 
+@pytest.mark.parametrize("tokens", [6, 64])
+def test_acceptance_of_equal_siblings(L, tokens):
+    """A star whose drafts repeat: a refused token leaves p once, and its equals are refused after it."""
+    rng = np.random.default_rng(tokens)
+    vocab = 9
+    logits = rng.normal(size=(4, tokens, vocab)).astype(np.float32)
+    parents = np.array([[-1] + [0] * (tokens - 1)] * 4)
+    draft = rng.integers(0, 5, (4, tokens))
+    want, uniforms = [], np.zeros((4, tokens), np.float32)
+    for s in range(4):
+        while True:
+            uniforms[s] = rng.random(tokens, dtype=np.float32)
+            uniforms[s, 1:] = 0.75 + uniforms[s, 1:] / 4  # most are refused
+            p, n, margin = S.verify(logits[s], draft[s], parents[s], None, uniforms[s], 1.0)
+            if margin > 1e-5:
+                break
+        want.append((len(p) - 1, n))
+    _, accepted, nxt = verify(L, logits, draft, parents, None, uniforms, 1.0)
+    assert list(zip(accepted, nxt)) == want
+
+
+@pytest.mark.parametrize("sampled", [False, True])
+def test_acceptance_far_from_zero(L, sampled):
+    """Logits at which t is beyond 2^21; with this temperature t is the logit, so 32 bits hold it."""
+    rng = np.random.default_rng(77)
+    seqs, tokens, vocab, temperature = 3, 5, 5003, 1.4426950408889634
+    logits = (rng.integers(-40, 1, (seqs, tokens, vocab)) / 4 + 2.0 ** 21).astype(np.float32)
+    parents = np.array([list(range(-1, tokens - 1))] * seqs)
+    draft = rng.integers(0, vocab, (seqs, tokens))
+    probs = np.full((seqs, tokens, vocab), 1 / vocab, np.float32) if sampled else None
+    want, uniforms = [], np.zeros((seqs, tokens), np.float32)
+    for s in range(seqs):
+        while True:
+            uniforms[s] = rng.random(tokens, dtype=np.float32)
+            p, n, margin = S.verify(logits[s], draft[s], parents[s], None if probs is None else probs[s], uniforms[s], temperature)
+            if margin > 1e-5:
+                break
+        want.append((len(p) - 1, n))
+    _, accepted, nxt = verify(L, logits, draft, parents, probs, uniforms, temperature)
+    assert list(zip(accepted, nxt)) == want
+
+
 def test_acceptance_of_the_targets_own_drafts(L):
     """Drafts drawn from the target itself are all accepted; a draft distribution that covers the target leaves the target."""
     vocab, tokens = 64, 5
