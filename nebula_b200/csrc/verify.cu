@@ -47,8 +47,7 @@ struct VerifyArgs {
     double *rest;   // [seqs][chunks]: sums of max(p - q, 0)
 };
 
-// t = n + f. The product is rounded before the floor (no fused multiply-add), so that f is the same everywhere; one
-// past the finite range counts as the range's end.
+// t = n + f, the product rounded before the floor; one past the finite range counts as the range's end.
 __device__ __forceinline__ float split(float x, float scale, float &frac) {
     const float t = fminf(fmaxf(__fmul_rn(x, scale), -FLT_MAX), FLT_MAX), n = floorf(t);
     frac = t - n;
@@ -67,30 +66,33 @@ __device__ __forceinline__ float weigh(float f, float rel) {
 __device__ __forceinline__ double shift_down(float rel) {
     return rel < -1000.0f ? 0.0 : __longlong_as_double((long long)((int)rel + 1023) << 52);
 }
-__device__ __forceinline__ float weight(float scale, const Stats &r, float x, int v) {
+// Conversions and floor run at an eighth of the rate of additions. Where |M| < 2^20, x*scale + (1.5 * 2^23 - M + b) that
+// rounds down is an integer of the last bit, floor(x*scale) - M + b stands in its low bits, and what it leaves of x*scale
+// is f: not even x*scale is rounded. Far below M the sum's bits are any, but it compares below.
+constexpr float kMagic = 12582912.0f, kNear = 1048576.0f;  // 1.5 * 2^23, 2^20
+__device__ __forceinline__ float near_weight(float scale, float k, float x) {  // k: kMagic + 127 - M
+    const float u = __fmaf_rd(x, scale, k), g = ex2(__fmaf_rn(x, scale, __fsub_rn(k, u)));
+    return u >= kMagic + 1.0f ? g * __int_as_float(__float_as_int(u) << 23) : 0.0f;
+}
+__device__ __forceinline__ float far_weight(float scale, const Stats &r, float x, int v) {
     if (scale == 0.0f) return v == r.best ? 1.0f : 0.0f;
     if (x == -INFINITY) return 0.0f;
     float f;
     const float n = split(x, scale, f);
     return weigh(f, n - r.top);
 }
-
-// The weights of 8 neighbouring values from v on. Conversions and floor run at an eighth of the rate of additions, so for
-// |M| < 2^20 floor comes from an addition that rounds down, and n is read from that sum's bits.
-constexpr float kMagic = 12582912.0f, kRange = 2097152.0f;  // 1.5 * 2^23, 2^21
+__device__ __forceinline__ bool is_near(float scale, const Stats &r) { return scale > 0.0f && fabsf(r.top) < kNear; }
+__device__ __forceinline__ float weight(float scale, const Stats &r, float x, int v) {
+    return is_near(scale, r) ? near_weight(scale, kMagic + 127.0f - r.top, x) : far_weight(scale, r, x, v);
+}
+// Of 8 neighbouring values from v on.
 __device__ __forceinline__ void weights8(float scale, const Stats &r, float (&x)[8], int v) {
-    if (scale > 0.0f && fabsf(r.top) < kRange / 2) {  // and no t is above the row's M + 1
-        const int top = __float_as_int(kMagic) + (int)r.top;
+    if (is_near(scale, r)) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float tc = fmaxf(__fmul_rn(x[i], scale), -kRange), u = __fadd_rd(tc, kMagic);
-            const int rel = __float_as_int(u) - top;
-            const float g = ex2(__fsub_rn(tc, __fsub_rn(u, kMagic)));
-            x[i] = rel < -126 ? 0.0f : g * __int_as_float((rel + 127) << 23);
-        }
+        for (int i = 0; i < 8; i++) x[i] = near_weight(scale, kMagic + 127.0f - r.top, x[i]);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = weight(scale, r, x[i], v + i);
+        for (int i = 0; i < 8; i++) x[i] = far_weight(scale, r, x[i], v + i);
     }
 }
 
@@ -125,84 +127,87 @@ __device__ __forceinline__ float warp_max(float x) {
     return __int_as_float(m < 0 ? m ^ 0x7fffffff : m);
 }
 
-// Of 8 values of a thread: the largest n, and the sum of the weights relative to it, floor as in weights8 (|t| < 2^21); 2^f 2^(n - top)
-// is put together as the bits of a double. (With conversions, which would bound the kernel, 50 us for 12 x 17 x 131072
-// logits.)
-__device__ __forceinline__ void weigh8(const float (&x)[8], float scale, float &top, double &sum) {
-    float t[8], most = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        t[i] = __fmul_rn(x[i], scale);
-        most = fmaxf(most, t[i]);
-    }
-    top = -INFINITY;
+// NaN if one of them is.
+__device__ __forceinline__ float max_nan(float x, float y) {
+    float z;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+    return z;
+}
+
+// The values of a thread, `most` the largest: the largest n, and the sum of the weights relative to it.
+template <int N>
+__device__ __forceinline__ void weigh_all(const float (&x)[N], float most, float scale, float &top, double &sum) {
     sum = 0.0;
-    if (most < kRange && most > -kRange / 2) {
-        int n[8], m = -0x7fffffff;
-        float f[8];
+    const float t = __fmul_rn(most, scale);
+    if (t > -kNear && t < kNear) {
+        // As near_weight, and 2^f 2^(n - top) put together as the bits of a double: 896 more make the exponent's bias.
+        // What is far below (2^f any there, 0, infinity and NaN too) comes to less than 2^-511: nothing beside the largest.
+        top = __fsub_rn(__fmaf_rd(most, scale, kMagic), kMagic);
+        const float k = kMagic + 896.0f - top;
+        const int least = __float_as_int(kMagic);
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float tc = fmaxf(t[i], -kRange), u = __fadd_rd(tc, kMagic);  // the sum's last bit is a one
-            n[i] = __float_as_int(u);
-            f[i] = __fsub_rn(tc, __fsub_rn(u, kMagic));
-            m = max(m, n[i]);
+        for (int i = 0; i < N; i++) {
+            const float u = __fmaf_rd(x[i], scale, k);
+            const unsigned g = __float_as_uint(ex2(__fmaf_rn(x[i], scale, __fsub_rn(k, u))));  // in [1, 2]
+            sum += __hiloint2double((int)(g >> 3) + (max(__float_as_int(u), least) << 20), (int)(g << 29));
         }
-        const int scale_down = ((1023 - 127) << 20) - (m << 20), least = m - 900;  // 2^-900 is nothing beside the largest
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const unsigned g = __float_as_uint(ex2(f[i]));  // in [1, 2]
-            sum += __hiloint2double((int)(g >> 3) + (max(n[i], least) << 20) + scale_down, (int)(g << 29));
-        }
-        top = (float)(m - __float_as_int(kMagic));
     } else {
-        float n[8];
+        float f;
+        top = most > -INFINITY ? split(most, scale, f) : -INFINITY;
+#pragma unroll 1
+        for (int i = 0; i < N; i++) {
+            float y = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            n[i] = -INFINITY;
-            if (x[i] > -INFINITY) n[i] = split(x[i], scale, t[i]);
-            top = fmaxf(top, n[i]);
+            for (int j = 0; j < N; j++) y = j == i ? x[j] : y;
+            if (y > -INFINITY) {
+                const float n = split(y, scale, f);
+                sum += (double)weigh(f, n - top);
+            }
         }
-#pragma unroll
-        for (int i = 0; i < 8; i++) sum += (double)(n[i] > -INFINITY ? weigh(t[i], n[i] - top) : 0.0f);
     }
 }
 
 // GREEDY: temperature 0, only the largest logit and its lowest index.
-// One chunk to a CTA: many short CTAs, eight to an SM, keep more loads in flight than fewer that go on to a next chunk
-// (12 x 17 x 131072 logits: 29 us against 33 with the next chunk's loads ahead).
+// One chunk to a CTA: many short CTAs keep more loads in flight than fewer that go on to a next chunk (all of a step, 12 x
+// 17 x 131072 logits: 46 us against 50 with the next chunk's loads ahead). The warps' instructions count next to the
+// bytes: at 26 a logit (with the last bit of floor taken by conversions and a maximum per eight) the step took 39.5 us,
+// like this 33.8; 128 threads with twice the logits 36.9.
 template <bool GREEDY>
 __global__ void __launch_bounds__(kChunkThreads) chunk_kernel(const __grid_constant__ VerifyArgs a) {
-    constexpr int kWarps = kChunkThreads / 32;
+    constexpr int kWarps = kChunkThreads / 32, kQuads = kChunk / (4 * kChunkThreads);
     __shared__ Stats part[kWarps];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const unsigned id = blockIdx.x;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const float *row = a.logits + (size_t)(id / (unsigned)a.chunks) * a.vocab;
-    const int first = (int)(id % (unsigned)a.chunks) * kChunk - chunk_lead(row) + 4 * (int)threadIdx.x;
-    float x[2][8];
+    const float *row = a.logits + (size_t)blockIdx.x * a.vocab;
+    const int start = (int)blockIdx.y * kChunk - chunk_lead(row), first = start + 4 * (int)threadIdx.x;
+    float x[4 * kQuads];
+    if (start >= 0 && start + kChunk <= a.vocab) {
+        const float4 *at = reinterpret_cast<const float4 *>(row + first);
 #pragma unroll
-    for (int i = 0; i < 4; i++) load4(row, a.vocab, first + 4 * kChunkThreads * i, *reinterpret_cast<float(*)[4]>(&x[i / 2][i % 2 * 4]));
-    bool bad = false;
+        for (int i = 0; i < kQuads; i++) *reinterpret_cast<float4 *>(&x[4 * i]) = __ldg(at + kChunkThreads * i);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 16; i++) bad |= !(x[i / 8][i % 8] < INFINITY);
-    bad = __any_sync(0xffffffffu, bad);
+        for (int i = 0; i < kQuads; i++) load4(row, a.vocab, first + 4 * kChunkThreads * i, *reinterpret_cast<float(*)[4]>(&x[4 * i]));
+    }
+    float most = x[0];
+#pragma unroll
+    for (int i = 1; i < 4 * kQuads; i++) most = max_nan(most, x[i]);
+    bool bad = __any_sync(0xffffffffu, !(most < INFINITY));
     Stats s = {0.0, -INFINITY, 0};
     if constexpr (GREEDY) {
         int best = 0x7fffffff;
 #pragma unroll
-        for (int i = 0; i < 16; i++)
-            if (x[i / 8][i % 8] > s.top) s.top = x[i / 8][i % 8], best = first + 4 * kChunkThreads * (i / 4) + i % 4;
-        const float m = warp_max(s.top + 0.0f);  // -0 and 0 are equals
-        s.best = __reduce_min_sync(0xffffffffu, s.top == m ? best : 0x7fffffff);
-        s.top = m;
+        for (int i = 4 * kQuads - 1; i >= 0; i--)
+            if (x[i] == most) best = first + 4 * kChunkThreads * (i / 4) + i % 4;
+        s.top = warp_max(most + 0.0f);  // -0 and 0 are equals
+        s.best = __reduce_min_sync(0xffffffffu, s.top == most ? best : 0x7fffffff);
     } else {
-        float t0, t1;
-        double s0, s1;
-        weigh8(x[0], a.scale, t0, s0);
-        weigh8(x[1], a.scale, t1, s1);
-        s.top = warp_max(fmaxf(t0, t1));
-        if (s.top > -INFINITY) s.sum = warp_sum(s0 * shift_down(t0 - s.top) + s1 * shift_down(t1 - s.top));
+        float top = -INFINITY;
+        double sum = 0.0;
+        if (!bad) weigh_all(x, most, a.scale, top, sum);
+        s.top = warp_max(top);
+        if (s.top > -INFINITY) s.sum = warp_sum(sum * shift_down(top - s.top));
     }
     if (!(s.top > -INFINITY)) s.best = kNone;
     if (bad) s.best = kBad;
@@ -214,7 +219,7 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_kernel(const __grid_const
         const float m = warp_max(s.best >= 0 ? s.top : -INFINITY);
         const int best = __reduce_min_sync(0xffffffffu, s.best >= 0 && s.top == m ? s.best : 0x7fffffff);
         const double sum = m > -INFINITY && !GREEDY ? warp_sum(s.best >= 0 ? s.sum * shift_down(s.top - m) : 0.0) : 0.0;
-        if (lane == 0) a.stats[id] = {sum, m, bad ? kBad : m > -INFINITY ? best : kNone};
+        if (lane == 0) a.stats[(size_t)blockIdx.x * a.chunks + blockIdx.y] = {sum, m, bad ? kBad : m > -INFINITY ? best : kNone};
     }
 }
 
@@ -563,9 +568,8 @@ extern "C" int qg_verify_tree(int *path, int *accepted, int *next, const float *
     Stats *stats = static_cast<Stats *>(workspace);
     const VerifyArgs a = {path, accepted, next, logits, draft, parents, draft_probs, uniforms, scale, tokens, vocab, chunks, stats,
                           reinterpret_cast<double *>(stats + (size_t)seqs * tokens * chunks)};
-    const unsigned grid = (unsigned)((size_t)seqs * tokens * chunks);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
+    cfg.gridDim = dim3(seqs * tokens, chunks);
     cfg.blockDim = dim3(kChunkThreads);
     cfg.stream = launch_stream;
     cudaLaunchAttribute attr[1];

@@ -511,6 +511,32 @@ def test_acceptance_far_from_zero(L, sampled):
     assert list(zip(accepted, nxt)) == want
 
 
+@pytest.mark.parametrize("mask", [-np.inf, -1e9, -1e30, np.finfo(np.float32).min])
+@pytest.mark.parametrize("sampled", [False, True])
+def test_acceptance_of_masked_logits(L, mask, sampled):
+    """Tokens taken out by very low logits: next to the others, in whole runs, and at nearly every place."""
+    rng = np.random.default_rng(13)
+    seqs, tokens, vocab = 3, 3, 9001
+    logits = rng.normal(size=(seqs, tokens, vocab)).astype(np.float32)
+    logits[0, :, ::2] = mask
+    logits[1, :, 1000:8000] = mask
+    logits[2] = mask
+    logits[2, :, [5, 4500, 9000]] = 1.0
+    parents = np.array([[-1, 0, 1]] * seqs)
+    draft = np.array([[0, 3, 5], [0, 10, 2000], [0, 5, 9000]])
+    probs = np.full((seqs, tokens, vocab), 1 / vocab, np.float32) if sampled else None
+    want, uniforms = [], np.zeros((seqs, tokens), np.float32)
+    for s in range(seqs):
+        while True:
+            uniforms[s] = rng.random(tokens, dtype=np.float32)
+            p, n, margin = S.verify(logits[s], draft[s], parents[s], None if probs is None else probs[s], uniforms[s], 0.7)
+            if margin > 1e-5:
+                break
+        want.append((len(p) - 1, n))
+    _, accepted, nxt = verify(L, logits, draft, parents, probs, uniforms, 0.7)
+    assert list(zip(accepted, nxt)) == want
+
+
 def test_acceptance_of_the_targets_own_drafts(L):
     """Drafts drawn from the target itself are all accepted; a draft distribution that covers the target leaves the target."""
     vocab, tokens = 64, 5
