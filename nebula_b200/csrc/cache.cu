@@ -23,17 +23,16 @@ struct PrepArgs {
     const float *q, *k, *v, *q_weight, *k_weight;
     const float2 *rope;
     const int *offsets;
-    int q_stride, k_stride, v_stride, rope_positions, half, tokens, q_heads, rows;
+    int q_stride, k_stride, v_stride, rope_positions, half, tokens, q_heads;
     float eps;
-    bool aligned;  // all rows of q, k, v, q_out and the weights start on 16-byte boundaries
 };
 
-// W neighbouring floats; aligned: in one load. (Not through the read-only path: q may be q_out.)
-template <int W>
-__device__ __forceinline__ void load(float (&x)[W], const float *p, bool aligned) {
-    if (W == 4 && aligned) {
+// W neighbouring floats; WIDE: in one load. (Not through the read-only path: q may be q_out.)
+template <bool WIDE, int W>
+__device__ __forceinline__ void load(float (&x)[W], const float *p) {
+    if constexpr (W == 4 && WIDE) {
         *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(p);
-    } else if (W == 2 && aligned) {
+    } else if constexpr (W == 2 && WIDE) {
         *reinterpret_cast<float2 *>(x) = *reinterpret_cast<const float2 *>(p);
     } else {
 #pragma unroll
@@ -45,22 +44,24 @@ __device__ __forceinline__ void load(float (&x)[W], const float *p, bool aligned
 // value heads. Lane l holds values W*l .. W*l+W-1 of each 128 (64 for heads of
 // 64) of a head. The heads' values are asked for first; the length, the page and
 // the table's angles, each of which depends on the one before, arrive meanwhile
-// and serve both heads (96 x 17 rows of 24 + 4 heads of 256: 24.6 us; one head to
-// a warp 28.9, four 24.9, each with the registers that keep five CTAs on an SM or
-// without, whichever was faster). The partner of a rotated value sits in
-// another lane, so the rotated part of the normalised head goes through the
-// warp's part of shared memory. Bound by HBM (by the launch for one verify batch).
+// and serve both heads (96 x 17 rows of 24 + 4 heads of 256: 22.6 us; one head to a warp 24.6, four 26.7; with the chained
+// launch 20.6). The partner of a rotated value sits in another lane, so the rotated part of the normalised head goes through
+// the warp's part of shared memory. Bound by HBM (by the launch for one verify batch).
 constexpr int kHeads = 2;
 
-template <int D>
-__global__ void __launch_bounds__(256, 5) qk_norm_rope_kernel(const __grid_constant__ PrepArgs a) {
+// WIDE: all rows of q, k, v, q_out and the weights start on 16-byte boundaries, and the rotated halves and the table's
+// rows are whole loads of a lane. The instructions count next to the bytes (two thirds of the issue slots).
+template <int D, bool WIDE>
+__global__ void __launch_bounds__(256, 4) qk_norm_rope_kernel(const __grid_constant__ PrepArgs a) {
     constexpr int W = D == 64 ? 2 : 4, N = D / (32 * W);
     __shared__ __align__(16) float head[8][D];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int heads = a.q_heads + 2 * a.c.kv_heads;
-    const unsigned groups = (heads + kHeads - 1) / kHeads, item = blockIdx.x * 8 + warp;
-    if (item >= (unsigned)a.rows * groups) return;
-    const int row = item / groups, h0 = (item - row * groups) * kHeads, seq = row / a.tokens, node = row - seq * a.tokens;
+    const int row = blockIdx.x, h0 = ((int)(blockIdx.y * blockDim.x / 32) + warp) * kHeads;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (h0 >= heads) return;
+    const int seq = row / a.tokens, node = row - seq * a.tokens;
     float x[kHeads][N][W];
 #pragma unroll
     for (int g = 0; g < kHeads; g++) {
@@ -69,21 +70,28 @@ __global__ void __launch_bounds__(256, 5) qk_norm_rope_kernel(const __grid_const
                            : v < 0 ? a.k + (size_t)row * a.k_stride + (size_t)k * D
                                    : a.v + (size_t)row * a.v_stride + (size_t)v * D;
 #pragma unroll
-        for (int j = 0; j < N; j++) load(x[g][j], src + 32 * W * j + W * lane, a.aligned);
+        for (int j = 0; j < N; j++) load<WIDE>(x[g][j], src + 32 * W * j + W * lane);
     }
     const int length = a.c.committed(seq, a.tokens);
     const int pos = length + (a.offsets ? a.offsets[row] : node);
     long long at = length < 0 ? -1 : a.c.row(seq, length + node);
     if (a.half && (unsigned)pos >= (unsigned)a.rope_positions) at = -1;
     float2 turn[N][W];
+    const float2 *angles = a.rope + (size_t)pos * a.half;
 #pragma unroll
-    for (int j = 0; j < N; j++)
+    for (int j = 0; j < N; j++) {
+        const int i0 = 32 * W * j + W * lane;
+        if (at < 0 || i0 >= 2 * a.half) continue;
+        if constexpr (WIDE) {
 #pragma unroll
-        for (int e = 0; e < W; e++) {
-            const int i = 32 * W * j + W * lane + e;
-            turn[j][e] = make_float2(1.0f, 0.0f);
-            if (at >= 0 && i < 2 * a.half) turn[j][e] = __ldg(a.rope + (size_t)pos * a.half + (i < a.half ? i : i - a.half));
+            for (int e = 0; e < W; e += 2)
+                *reinterpret_cast<float4 *>(&turn[j][e]) = __ldg(reinterpret_cast<const float4 *>(angles + (i0 < a.half ? i0 : i0 - a.half) + e));
+        } else {
+#pragma unroll
+            for (int e = 0; e < W; e++)
+                if (i0 + e < 2 * a.half) turn[j][e] = __ldg(angles + (i0 + e < a.half ? i0 + e : i0 + e - a.half));
         }
+    }
 #pragma unroll
     for (int g = 0; g < kHeads; g++) {
         const int h = h0 + g, k = h - a.q_heads, v = k - a.c.kv_heads;
@@ -93,7 +101,7 @@ __global__ void __launch_bounds__(256, 5) qk_norm_rope_kernel(const __grid_const
             float w[N][W], sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < N; j++) {
-                load(w[j], weight + 32 * W * j, a.aligned);
+                load<WIDE>(w[j], weight + 32 * W * j);
 #pragma unroll
                 for (int e = 0; e < W; e++) sum = fmaf(x[g][j][e], x[g][j][e], sum);
             }
@@ -116,11 +124,20 @@ __global__ void __launch_bounds__(256, 5) qk_norm_rope_kernel(const __grid_const
             __syncwarp();
 #pragma unroll
             for (int j = 0; j < N; j++) {
-                if (32 * W * j >= 2 * a.half) continue;
+                const int i0 = 32 * W * j + W * lane;
+                if (i0 >= 2 * a.half) continue;
+                if constexpr (WIDE) {
+                    const bool low = i0 < a.half;
+                    float other[W];
+                    load<true>(other, &head[warp][low ? i0 + a.half : i0 - a.half]);
 #pragma unroll
-                for (int e = 0; e < W; e++) {
-                    const int i = 32 * W * j + W * lane + e;
-                    if (i < 2 * a.half) {
+                    for (int e = 0; e < W; e++)
+                        x[g][j][e] = fmaf(other[e], low ? -turn[j][e].y : turn[j][e].y, x[g][j][e] * turn[j][e].x);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < W; e++) {
+                        const int i = i0 + e;
+                        if (i >= 2 * a.half) continue;
                         const bool low = i < a.half;
                         const float other = head[warp][low ? i + a.half : i - a.half];
                         const float2 t = turn[j][e];
@@ -136,7 +153,7 @@ __global__ void __launch_bounds__(256, 5) qk_norm_rope_kernel(const __grid_const
                 if (at < 0)  // the header's refusals: NaN queries, no store
 #pragma unroll
                     for (int e = 0; e < W; e++) x[g][j][e] = __int_as_float(0x7fc00000);
-                if (W == 4 && a.aligned) *reinterpret_cast<float4 *>(out + 32 * W * j) = *reinterpret_cast<float4 *>(x[g][j]);
+                if constexpr (W == 4 && WIDE) *reinterpret_cast<float4 *>(out + 32 * W * j) = *reinterpret_cast<float4 *>(x[g][j]);
                 else
 #pragma unroll
                     for (int e = 0; e < W; e++) out[32 * W * j + e] = x[g][j][e];
@@ -179,6 +196,7 @@ __global__ void __cluster_dims__(kCommitCtas, 1, 1) __launch_bounds__(256) cache
     __shared__ long long from[kMaxNodes], to[kMaxNodes];
     cg::cluster_group cluster = cg::this_cluster();
     const int seq = blockIdx.x / kCommitCtas, part = blockIdx.x % kCommitCtas, i = threadIdx.x;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int n = a.accepted[seq];
     const int p = i < a.tokens ? a.path[(size_t)seq * a.tokens + i] : 0;
     const int before = i > 0 && i < a.tokens ? a.path[(size_t)seq * a.tokens + i - 1] : -1;
@@ -214,6 +232,7 @@ __global__ void __cluster_dims__(kCommitCtas, 1, 1) __launch_bounds__(256) cache
             }
         }
     }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     cluster.sync();
     if (part == 0 && i == 0) a.lengths_out[seq] = sound ? length + n + 1 : a.c.lengths[seq];
 }
@@ -250,17 +269,20 @@ extern "C" int qg_qk_norm_rope(float *q_out, const qg_kv_cache *cache, int layer
     a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride;
     a.rope_positions = rope_positions;
     a.half = rotary / 2;
-    a.tokens = tokens, a.q_heads = q_heads, a.rows = seqs * tokens;
+    a.tokens = tokens, a.q_heads = q_heads;
     a.eps = eps;
-    a.aligned = !((reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
-                   reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(q_weight) | reinterpret_cast<uintptr_t>(k_weight)) & 15) &&
-                !((q_stride | k_stride | v_stride) & 3);
-    const long long items = (long long)a.rows * ((q_heads + 2 * a.c.kv_heads + kHeads - 1) / kHeads);
-    const unsigned grid = (unsigned)((items + 7) / 8);
-    if (D == 64) qk_norm_rope_kernel<64><<<grid, 256, 0, launch_stream>>>(a);
-    else if (D == 128) qk_norm_rope_kernel<128><<<grid, 256, 0, launch_stream>>>(a);
-    else qk_norm_rope_kernel<256><<<grid, 256, 0, launch_stream>>>(a);
-    NB_CHECK_LAUNCH();
+    const bool wide = !((reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
+                         reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(q_weight) | reinterpret_cast<uintptr_t>(k_weight) |
+                         reinterpret_cast<uintptr_t>(rope)) & 15) &&
+                      !((q_stride | k_stride | v_stride | a.half) & 3);
+    // the warps of a row in as few blocks as hold them, evenly
+    const int groups = (q_heads + 2 * a.c.kv_heads + kHeads - 1) / kHeads, blocks = (groups + 7) / 8;
+    const dim3 grid(seqs * tokens, blocks);
+    const int threads = 32 * ((groups + blocks - 1) / blocks);
+    const auto kernel = D == 64    ? wide ? qk_norm_rope_kernel<64, true> : qk_norm_rope_kernel<64, false>
+                        : D == 128 ? wide ? qk_norm_rope_kernel<128, true> : qk_norm_rope_kernel<128, false>
+                                   : wide ? qk_norm_rope_kernel<256, true> : qk_norm_rope_kernel<256, false>;
+    return launch_chained(kernel, grid, threads, a);
 }
 
 extern "C" int qg_cache_commit(const qg_kv_cache *cache, int *lengths_out, const int *path, const int *accepted, int seqs,
@@ -274,6 +296,9 @@ extern "C" int qg_cache_commit(const qg_kv_cache *cache, int *lengths_out, const
     a.lengths_out = lengths_out;
     a.path = path;
     a.accepted = accepted;
+    // A chained launch hides what the kernel before leaves of the launch (one sequence 3.6 us in place of 4.4 to 5.1); with
+    // more clusters than the GPU takes at once it only adds (48 sequences 32.6 us in place of 31.4).
+    if (seqs * kCommitCtas <= 148) return launch_chained(cache_commit_kernel, dim3(seqs * kCommitCtas), 256, a);
     cache_commit_kernel<<<seqs * kCommitCtas, 256, 0, launch_stream>>>(a);
     NB_CHECK_LAUNCH();
 }

@@ -27,6 +27,22 @@ struct CacheView {
     }
 };
 
+// A launch that may begin while the stream's previous kernel ends; the kernel waits (griddepcontrol.wait) before it touches
+// memory.
+template <typename Args>
+inline int launch_chained(void (*kernel)(Args), dim3 grid, int threads, const Args &args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = launch_stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args);
+}
+
 // Checks what the header asks of a cache and a batch; cudaErrorInvalidValue before any launch.
 inline int cache_view(const qg_kv_cache *c, int layer, int seqs, int tokens, CacheView &view) {
     if (!c || !c->k || !c->v || !c->page_table || !c->lengths || seqs < 1 || seqs > kMaxSeqs || tokens < 1 ||

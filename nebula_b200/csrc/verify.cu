@@ -568,15 +568,7 @@ extern "C" int qg_verify_tree(int *path, int *accepted, int *next, const float *
     Stats *stats = static_cast<Stats *>(workspace);
     const VerifyArgs a = {path, accepted, next, logits, draft, parents, draft_probs, uniforms, scale, tokens, vocab, chunks, stats,
                           reinterpret_cast<double *>(stats + (size_t)seqs * tokens * chunks)};
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(seqs * tokens, chunks);
-    cfg.blockDim = dim3(kChunkThreads);
-    cfg.stream = launch_stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (int rc = cudaLaunchKernelEx(&cfg, scale == 0.0f ? chunk_kernel<true> : chunk_kernel<false>, a)) return rc;
+    if (int rc = launch_chained(scale == 0.0f ? chunk_kernel<true> : chunk_kernel<false>, dim3(seqs * tokens, chunks), kChunkThreads, a))
+        return rc;
     return draft_probs ? launch_walk<true>(a, seqs) : launch_walk<false>(a, seqs);
 }
