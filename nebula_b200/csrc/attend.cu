@@ -365,6 +365,32 @@ struct Walk {
     }
 };
 
+// One warp: the slots of CTA (or pair) `team`.
+template <int D>
+__device__ __forceinline__ void plan(const AttendArgs &a, Shared &s, int team, int teams) {
+    const int lane = threadIdx.x & 31;
+    const int per = a.c.kv_heads * a.row_tiles;
+    const int len = lane < a.seqs ? a.c.committed(lane, a.tokens) : -1;
+    long long w = (long long)slots_of<D>(a, len) * per, base = 0, u0 = 0, u1 = 0;
+    int seq = 0, length = len;
+    if (a.seqs > 1) {
+        for (int q = lane + 32; q < a.seqs; q += 32) w += (long long)slots_of<D>(a, a.c.committed(q, a.tokens)) * per;
+        w = warp_sum(w);
+    }
+    const int g = (int)min((long long)teams, w);  // (one sequence: right in lane 0)
+    if (team < g) {
+        u0 = range_start(team, w, g);
+        u1 = range_start(team + 1, w, g);
+        if (a.seqs > 1) seq = find_slot<D>(a, per, u0, len, base, length);
+    }
+    if (lane == 0) {
+        const int slots = max(1, slots_of<D>(a, length)), index = (int)quotient(u0 - base, slots);
+        s.slot0 = u0, s.slot1 = u1, s.seq0 = seq, s.length0 = length;
+        s.kv0 = index / a.row_tiles, s.tile0 = index % a.row_tiles;
+        s.pos0 = (int)(u0 - base - (long long)index * slots);
+    }
+}
+
 // Keys that unit j of an item's part holds.
 __device__ __forceinline__ int keys_of(const AttendArgs &a, const Item &it, int j) {
     return min(kKeys, it.length + a.tokens - (it.first + j) * kKeys);
@@ -412,26 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
 
     if (warp == 0) {
         asm volatile("griddepcontrol.wait;" ::: "memory");
-        const int per = a.c.kv_heads * a.row_tiles;
-        const int len = lane < a.seqs ? a.c.committed(lane, a.tokens) : -1;
-        long long w = (long long)slots_of<D>(a, len) * per, base = 0, u0 = 0, u1 = 0;
-        int seq = 0, length = len;
-        if (a.seqs > 1) {
-            for (int q = lane + 32; q < a.seqs; q += 32) w += (long long)slots_of<D>(a, a.c.committed(q, a.tokens)) * per;
-            w = warp_sum(w);
-        }
-        const int g = (int)min((long long)teams, w);  // (one sequence: right in lane 0)
-        if (team < g) {
-            u0 = range_start(team, w, g);
-            u1 = range_start(team + 1, w, g);
-            if (a.seqs > 1) seq = find_slot<D>(a, per, u0, len, base, length);
-        }
-        if (lane == 0) {
-            const int slots = max(1, slots_of<D>(a, length)), index = (int)quotient(u0 - base, slots);
-            s.slot0 = u0, s.slot1 = u1, s.seq0 = seq, s.length0 = length;
-            s.kv0 = index / a.row_tiles, s.tile0 = index % a.row_tiles;
-            s.pos0 = (int)(u0 - base - (long long)index * slots);
-        }
+        plan<D>(a, s, team, teams);
     } else if (warp == 1) {
         if constexpr (PAIR) {
             asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s.tmem)));
@@ -1050,6 +1057,201 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     }
 }
 
+// ---- one token and at most four heads to a key head ---------------------------
+
+// So few rows need no tensor cores: a value of the cache costs five instructions or so, and the SM has time for them while
+// HBM delivers it. Warp w of 16 takes keys 8w .. 8w+7 of every unit, on its own from memory to registers: its copies go to
+// its own part of shared memory, kStages units ahead, and a lane reads only what it copied itself, so there is no barrier
+// before an item's end. Lane l holds 8 values of a key, D/8 lanes a key. The 8 x 4 partial products of a lane are added up
+// over the lanes in a butterfly that leaves one score to a lane; softmax runs per warp, and an item's 16 maxima, totals and
+// sums become one at its end. The division of the work and the join are the other kernel's. Bound by HBM (16 single tokens
+// of 32 heads, 8 key heads of 128: XX us, on the tensor cores 87).
+constexpr int kFewWarps = 16, kFewRows = 4;
+template <int D>
+struct Few {
+    static constexpr int kLanes = D / 8, kPer = 32 / kLanes, kLoads = 8 / kPer;  // lanes a key, keys a load, loads of 8 keys
+    static constexpr int kStage = 2 * kLoads * 512, kStages = D == 128 ? 3 : 6;
+    static constexpr int kRing = kFewWarps * kStages * kStage, kSmem = kRing + kFewWarps * kFewRows * D * 4;
+    static_assert(kLoads * kFewRows == kLanes, "a score to a lane");
+    static_assert(kSmem + 2048 <= 232448, "shared memory");
+};
+
+__device__ __forceinline__ void eight(const unsigned char *p, float (&x)[8], bool none = false) {
+    const uint4 y = none ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4 *>(p);
+    const uint32_t z[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&z[i]));
+        x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    }
+}
+
+template <int D>
+__global__ void __launch_bounds__(32 * kFewWarps, 1) token_attention_kernel(const __grid_constant__ AttendArgs a) {
+    using C = Few<D>;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    __shared__ Shared s;
+    __shared__ float2 ml[kFewWarps][kFewRows];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, team = blockIdx.x;
+    const int key = lane / C::kLanes, dim = lane % C::kLanes * 8;
+    const float nan = __int_as_float(0x7fc00000);
+    if (warp == 0) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        plan<D>(a, s, team, gridDim.x);
+    }
+    __syncthreads();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    for (int q = team; q < a.seqs; q += gridDim.x)  // rows of refused sequences
+        if (a.c.committed(q, 1) < 0)
+            for (int i = tid; i < a.q_heads * D; i += 32 * kFewWarps) a.out[(size_t)q * a.q_heads * D + i] = nan;
+    unsigned char *const ring = smem + warp * C::kStages * C::kStage + lane * 16;
+    float *const sums = reinterpret_cast<float *>(smem + C::kRing);
+    const size_t width = (size_t)a.c.kv_heads * D;
+    Walk<D> walk(s);
+    Item it;
+    while (walk.next(a, it)) {
+        const int all = it.length + 1, n = it.length + (a.tree ? (int)(a.tree[it.seq] & 1) : 1);  // keys there, keys seen
+        const int first = it.first * kKeys + 8 * warp;
+        const int *table = a.c.table + (size_t)it.seq * a.c.table_pages;
+        bool bad = false;
+        int page = 0;
+        auto issue = [&](int t) {
+            if (t < it.count) {
+                if (!(t & 31)) {  // the pages of the next 32 units, a lane each
+                    const int at = first + (t + lane) * kKeys;
+                    page = t + lane < it.count && at < all ? table[at >> a.c.shift] : 0;
+                    if ((unsigned)page >= (unsigned)a.c.pages) bad = true, page = 0;
+                }
+                const int p = __shfl_sync(0xffffffffu, page, t & 31), base = first + t * kKeys;
+                if (base < all) {  // (the 8 rows lie in one page)
+                    const size_t row = ((size_t)p << a.c.shift) + (base & (a.c.page_tokens() - 1)) + key;
+                    const size_t off = row * width + (size_t)it.kv * D + dim;
+                    const uint32_t to = smem_u32(ring + t % C::kStages * C::kStage);
+#pragma unroll
+                    for (int i = 0; i < C::kLoads; i++)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i * 512), "l"(a.c.k + off + i * C::kPer * width) : "memory");
+#pragma unroll
+                    for (int i = 0; i < C::kLoads; i++)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (C::kLoads + i) * 512), "l"(a.c.v + off + i * C::kPer * width) : "memory");
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int t = 0; t < C::kStages - 1; t++) issue(t);
+        float q[kFewRows][8], acc[kFewRows][8], m = -INFINITY, l = 0.0f;  // m and l: of row lane % 4
+#pragma unroll
+        for (int r = 0; r < kFewRows; r++) {
+            const float *src = a.q + ((size_t)it.seq * a.q_heads + it.kv * a.group + min(r, a.group - 1)) * D + dim;
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) *reinterpret_cast<float4 *>(&q[r][e]) = *reinterpret_cast<const float4 *>(src + e);
+#pragma unroll
+            for (int e = 0; e < 8; e++) q[r][e] *= a.scale * a.sign, acc[r][e] = 0.0f;
+        }
+#pragma unroll 1
+        for (int t = 0; t < it.count; t++) {
+            __syncwarp();  // what was read from the place of the unit before is read
+            issue(t + C::kStages - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
+            const int base = first + t * kKeys;
+            if (base >= all) break;  // and so are the units after it
+            const unsigned char *k = ring + t % C::kStages * C::kStage, *v = k + C::kLoads * 512;
+            float x[C::kLanes];
+#pragma unroll
+            for (int i = 0; i < C::kLoads; i++) {
+                float f[8];
+                eight(k + i * 512, f);
+#pragma unroll
+                for (int r = 0; r < kFewRows; r++) {
+                    float dot = q[r][0] * f[0];
+#pragma unroll
+                    for (int e = 1; e < 8; e++) dot = fmaf(q[r][e], f[e], dot);
+                    x[i * kFewRows + r] = dot;
+                }
+            }
+#pragma unroll
+            for (int o = C::kLanes / 2; o; o >>= 1) {
+#pragma unroll
+                for (int j = 0; j < o; j++) {
+                    const float mine = lane & o ? x[j + o] : x[j], other = lane & o ? x[j] : x[j + o];
+                    x[j] = mine + __shfl_xor_sync(0xffffffffu, other, o);
+                }
+            }
+            // the lane's score: row lane % 4 and key
+            const int at = base + lane % C::kLanes / kFewRows * C::kPer + key;
+            const float score = at < n ? x[0] : -INFINITY;
+            float top = score;
+#pragma unroll
+            for (int o = kFewRows; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            top = fmaxf(m, top);
+            if (__any_sync(0xffffffffu, top > m)) {
+                const float keep = m == -INFINITY ? 0.0f : ex2(m - top);
+                l *= keep;
+                m = top;
+#pragma unroll
+                for (int r = 0; r < kFewRows; r++) {
+                    const float f = __shfl_sync(0xffffffffu, keep, r);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) acc[r][e] *= f;
+                }
+            }
+            const float p = ex2(score - (m == -INFINITY ? 0.0f : m));
+            l += p;
+#pragma unroll
+            for (int i = 0; i < C::kLoads; i++) {
+                float f[8];
+                eight(v + i * 512, f, base + i * C::kPer + key >= n);  // unseen values are any: P = 0 would not keep a NaN out
+#pragma unroll
+                for (int r = 0; r < kFewRows; r++) {
+                    const float w = __shfl_sync(0xffffffffu, p, key * C::kLanes + i * kFewRows + r);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) acc[r][e] = fmaf(w, f[e], acc[r][e]);
+                }
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        // ---- the warps' parts become one
+#pragma unroll
+        for (int o = kFewRows; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+#pragma unroll
+        for (int r = 0; r < kFewRows; r++) {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+#pragma unroll
+                for (int o = C::kLanes; o < 32; o <<= 1) acc[r][e] += __shfl_xor_sync(0xffffffffu, acc[r][e], o);
+            if (key == 0)
+#pragma unroll
+                for (int e = 0; e < 8; e += 4)
+                    *reinterpret_cast<float4 *>(&sums[(warp * kFewRows + r) * D + dim + e]) = *reinterpret_cast<float4 *>(&acc[r][e]);
+        }
+        if (lane < kFewRows) ml[warp][lane] = make_float2(m, l);
+        bad = __syncthreads_or(bad);
+        const bool whole = it.count == it.units;
+        const size_t part = (size_t)(2 * team + (it.start > s.slot0)) * a.part_rows;
+        for (int i = tid; i < a.group * D; i += 32 * kFewWarps) {
+            const int r = i / D, d = i % D;
+            float most = -INFINITY, total = 0.0f, sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kFewWarps; w++) most = fmaxf(most, ml[w][r].x);
+#pragma unroll
+            for (int w = 0; w < kFewWarps; w++) {
+                const float2 x = ml[w][r];
+                const float f = x.x == -INFINITY ? x.y : ex2(x.x - most);  // its total is 0 (nothing seen) or NaN
+                total += f * x.y;
+                sum = fmaf(f, sums[(w * kFewRows + r) * D + d], sum);
+            }
+            if (bad) sum = nan;
+            if (whole) {
+                a.out[((size_t)it.seq * a.q_heads + it.kv * a.group + r) * D + d] = total == 0.0f && !bad ? 0.0f : sum / total;
+            } else {
+                a.part_acc[(part + r) * D + d] = sum;
+                if (d == 0) a.part_ml[part + r] = make_float2(most, total);
+            }
+        }
+        __syncthreads();
+    }
+}
+
 // Joins the parts of items that several CTAs share, and makes every row NaN
 // after an error: one CTA per (row, head). Warps take every eighth part, so all
 // loads of a row are in flight at once; their sums join in order.
@@ -1165,34 +1367,41 @@ int part_rows(int tokens, int group) { return tokens * group < kRows ? tokens * 
 
 size_t ml_bytes(int rows) { return (size_t)2 * kMaxCtas * rows * sizeof(float2); }
 
-template <int D, int MR, bool PAIR>
-int launch(const AttendArgs &a, const CUtensorMap &k_map, const CUtensorMap &v_map) {
-    using C = Cfg<D, MR, PAIR>;
-    constexpr int kPeers = PAIR ? 2 : 1;
-    if (int rc = cudaFuncSetAttribute(tree_attention_kernel<D, MR, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem)) return rc;
+// The attention kernel and the join, chained to what runs before. Peers: CTAs that work on one item.
+template <int D, typename... A>
+int launch(const AttendArgs &a, void (*kernel)(A...), int peers, int threads, int smem, const A &...args) {
+    if (int rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return rc;
     // no more CTAs than the longest sequences that the table allows could use
     const long long units = (((long long)a.c.table_pages << a.c.shift) + kKeys - 1) / kKeys;
     const long long most = (long long)a.seqs * a.c.kv_heads * a.row_tiles * (units + kItemCost<D>);
-    const int teams = (int)(most < kMaxCtas / kPeers ? most : kMaxCtas / kPeers);
+    const int teams = (int)(most < kMaxCtas / peers ? most : kMaxCtas / peers);
     cudaLaunchConfig_t cfg = {};
     cfg.stream = launch_stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = kPeers;
+    attr[1].val.clusterDim.x = peers;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = PAIR ? 2 : 1;
-    cfg.gridDim = dim3(teams * kPeers);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = C::kSmem;
-    if (int rc = cudaLaunchKernelEx(&cfg, tree_attention_kernel<D, MR, PAIR>, a, k_map, v_map)) return rc;
+    cfg.numAttrs = peers > 1 ? 2 : 1;
+    cfg.gridDim = dim3(teams * peers);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    if (int rc = cudaLaunchKernelEx(&cfg, kernel, args...)) return rc;
     cfg.numAttrs = 1;
     cfg.gridDim = dim3((unsigned)(a.seqs * a.tokens * a.q_heads));
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
     return cudaLaunchKernelEx(&cfg, join_kernel<D>, a, teams);
+}
+template <int D, int MR, bool PAIR>
+int launch_tiles(const AttendArgs &a, const CUtensorMap &k_map, const CUtensorMap &v_map) {
+    return launch<D>(a, tree_attention_kernel<D, MR, PAIR>, PAIR ? 2 : 1, kThreads, Cfg<D, MR, PAIR>::kSmem, a, k_map, v_map);
+}
+template <int D>
+int launch_token(const AttendArgs &a) {
+    return launch<D>(a, token_attention_kernel<D>, 1, 32 * kFewWarps, Few<D>::kSmem, a);
 }
 
 }  // namespace
@@ -1239,11 +1448,12 @@ extern "C" int qg_tree_attention(float *out, const float *q, const qg_kv_cache *
     a.err = static_cast<int *>(workspace);
     a.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + 256);
     a.part_acc = reinterpret_cast<float *>(static_cast<char *>(workspace) + 256 + ml_bytes(part_rows(tokens, a.group)));
+    if (rows <= kFewRows && tokens == 1 && a.c.head_dim <= 128) return a.c.head_dim == 64 ? launch_token<64>(a) : launch_token<128>(a);
     CUtensorMap k_map, v_map;
     if (int rc = pool_map(&k_map, a.c, a.c.k, a.k_box, a.k_blocks)) return rc;
     if (int rc = pool_map(&v_map, a.c, a.c.v, a.v_box, v_blocks)) return rc;
-    if (a.c.head_dim == 64) return launch<64, 128, false>(a, k_map, v_map);
-    if (a.c.head_dim == 128) return rows <= 32 ? launch<128, 64, false>(a, k_map, v_map) : launch<128, 128, false>(a, k_map, v_map);
-    if (pair) return launch<256, 128, true>(a, k_map, v_map);
-    return rows <= 64 ? launch<256, 64, false>(a, k_map, v_map) : launch<256, 128, false>(a, k_map, v_map);
+    if (a.c.head_dim == 64) return launch_tiles<64, 128, false>(a, k_map, v_map);
+    if (a.c.head_dim == 128) return rows <= 32 ? launch_tiles<128, 64, false>(a, k_map, v_map) : launch_tiles<128, 128, false>(a, k_map, v_map);
+    if (pair) return launch_tiles<256, 128, true>(a, k_map, v_map);
+    return rows <= 64 ? launch_tiles<256, 64, false>(a, k_map, v_map) : launch_tiles<256, 128, false>(a, k_map, v_map);
 }

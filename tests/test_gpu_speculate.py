@@ -117,6 +117,41 @@ def test_attention_many_short_sequences(L, hq, hkv, d, tokens):
     assert_parity(got, expected(cache, q, None, d ** -0.5))
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(4, 4, 64), (6, 2, 64), (4, 1, 128), (4, 2, 128), (32, 8, 128)])
+@pytest.mark.parametrize("page", [16, 128])
+def test_attention_single_tokens_of_few_heads(L, hq, hkv, d, page):
+    """Lengths around the eight keys of a warp, the unit and the page; the token may see itself or not."""
+    rng = np.random.default_rng(hq * d + page)
+    lengths = [0, 1, 6, 7, 8, 9, 119, 120, 127, 128, 129, 255, 1001, 5000, 33000]
+    cache = Cache(L, rng, lengths, 1, hkv, d, page)
+    q = (1.5 * rng.normal(size=(len(lengths), 1, hq, d))).astype(np.float32)
+    assert_parity(attend(L, cache, q, None, d ** -0.5, calls=3), expected(cache, q, None, d ** -0.5))
+    masks = [[s % 2] for s in range(len(lengths))]
+    ref = expected(cache, q, masks, d ** -0.5)
+    for s in range(0, len(lengths), 2):  # what is not seen may be anything
+        cache.k[0, cache.rows(s, lengths[s], 1)] = np.nan
+        cache.v[0, cache.rows(s, lengths[s], 1), :, ::2] = np.inf
+    cache.upload()
+    got = attend(L, cache, q, masks, d ** -0.5, calls=2)
+    assert_parity(got, ref)
+    assert np.array_equal(got[0], np.zeros_like(got[0]))
+    q[3, 0, hq - 1, 5] = np.nan
+    again = attend(L, cache, q, masks, d ** -0.5)
+    assert np.isnan(again[3, 0, hq - 1]).all()
+    again[3, 0, hq - 1] = got[3, 0, hq - 1]
+    np.testing.assert_array_equal(again, got)
+    table = cache.table.copy()
+    table[12, 1], table[14, 200] = cache.pages, -1
+    cache.dt.set(table)
+    now = np.array(lengths, np.int32)
+    now[2], now[5] = -1, 1 << 20
+    cache.dl.set(now)
+    again, bad = attend(L, cache, q, masks, d ** -0.5), [2, 5, 12, 14]
+    assert np.isnan(again[bad]).all()
+    keep = [s for s in range(len(lengths)) if s not in bad and s != 3]
+    assert_parity(again[keep], ref[keep])
+
+
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_attention_layers_and_large_scores(L, d):
     """The layer asked for is the one read; scores of some hundreds leave one key with all the weight."""
