@@ -24,6 +24,10 @@
 // value rows of the nodes' tiles are cleaned in shared memory (P = 0 would not
 // keep a NaN or infinity out of a product); nodes whose values are not finite
 // are added by hand to the rows that see them.
+//
+// One token whose query heads share a key head by four at most has a kernel
+// without tensor cores (token_attention_kernel): its arithmetic hides behind
+// HBM, and nothing is handed from one role to another.
 #include <cuda.h>
 #include <cstring>
 #include "cache.cuh"
@@ -1065,7 +1069,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
 // before an item's end. Lane l holds 8 values of a key, D/8 lanes a key. The 8 x 4 partial products of a lane are added up
 // over the lanes in a butterfly that leaves one score to a lane; softmax runs per warp, and an item's 16 maxima, totals and
 // sums become one at its end. The division of the work and the join are the other kernel's. Bound by HBM (16 single tokens
-// of 32 heads, 8 key heads of 128: XX us, on the tensor cores 87).
+// of 32 heads, 8 key heads of 128, 285 MB: 63.7 us, on the tensor cores 87).
 constexpr int kFewWarps = 16, kFewRows = 4;
 template <int D>
 struct Few {
@@ -1448,6 +1452,8 @@ extern "C" int qg_tree_attention(float *out, const float *q, const qg_kv_cache *
     a.err = static_cast<int *>(workspace);
     a.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + 256);
     a.part_acc = reinterpret_cast<float *>(static_cast<char *>(workspace) + 256 + ml_bytes(part_rows(tokens, a.group)));
+    // One token, at most four heads to a key head of up to 128 values: no tensor cores (16 tokens, 32/8 heads of 128: 63.7 us
+    // against 87). Heads of 256 leave no room for copies ahead.
     if (rows <= kFewRows && tokens == 1 && a.c.head_dim <= 128) return a.c.head_dim == 64 ? launch_token<64>(a) : launch_token<128>(a);
     CUtensorMap k_map, v_map;
     if (int rc = pool_map(&k_map, a.c, a.c.k, a.k_box, a.k_blocks)) return rc;
