@@ -170,7 +170,7 @@ __device__ __forceinline__ void weigh_all(const float (&x)[N], float most, float
 // GREEDY: temperature 0, only the largest logit and its lowest index.
 // One chunk to a CTA: many short CTAs keep more loads in flight than fewer that go on to a next chunk (all of a step, 12 x
 // 17 x 131072 logits: 46 us against 50 with the next chunk's loads ahead). The warps' instructions count next to the
-// bytes: at 26 a logit (with the last bit of floor taken by conversions and a maximum per eight) the step took 39.5 us,
+// bytes: at 26 a logit (guarded loads, the product rounded by itself, a maximum per eight) the step took 39.5 us,
 // like this 33.8; 128 threads with twice the logits 36.9.
 template <bool GREEDY>
 __global__ void __launch_bounds__(kChunkThreads) chunk_kernel(const __grid_constant__ VerifyArgs a) {
@@ -245,7 +245,8 @@ template <bool DRAWN>
 __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) {
     constexpr int kWarps = kWalkThreads / 32, kCtas = DRAWN ? kDrawnCtas : 1;
     static_assert(kWalkThreads * 8 == kChunk, "eight values of a chunk to a thread");
-    // Chunks whose loads are in flight together (7 x 6 x 50001 logits 12.4 us, 12 x 17 x 131072 39.7; four: 13.0, 39.0).
+    // Chunks whose loads are in flight together (four: 7 x 6 x 50001 logits 0.6 us slower, 12 x 17 x
+    // 131072 0.7 us faster).
     constexpr int kBatch = 2;
     __shared__ Stats rows[kMaxNodes];
     __shared__ double sums[kWarps], batch[DRAWN ? kBatch : 1][kWarps];
