@@ -41,6 +41,7 @@ constexpr int kRows = 128;       // rows per tile (MMA M)
 constexpr int kKeys = 128;       // keys per unit (MMA N of S: with 64 the re-reads of Q bound the shared memory)
 constexpr int kMaxCtas = 148;    // SMs of a B200: one CTA each
 constexpr int kThreads = 512;
+constexpr int kNotes = 3 * 1024;  // bytes for the roles' shared bookkeeping
 // Registers per thread after the split; the four warpgroups' sum is what the
 // CTA was launched with (4 * 128).
 constexpr int kRegsControl = 48, kRegsSoftmax = 112, kRegsAcc = 176;
@@ -82,8 +83,8 @@ struct Cfg {
     static_assert(kPieces * kVKeys == kKeys, "as many pieces of values as of keys");
     // Two places for Q where there is room: the next item's is prepared while this one's is in use.
     static constexpr int kQBufs = 4 * kPlane <= 131072 ? 2 : 1;
-    static constexpr int kKStages = (232448 - 3072 - kQBufs * 2 * kPlane) / (2 * kPiece), kVStages = kKStages;
-    static constexpr int kSmem = kQBufs * 2 * kPlane + (kKStages + kVStages) * kPiece + 3072;
+    static constexpr int kKStages = (232448 - kNotes - kQBufs * 2 * kPlane) / (2 * kPiece), kVStages = kKStages;
+    static constexpr int kSmem = kQBufs * 2 * kPlane + (kKStages + kVStages) * kPiece + kNotes;
     static constexpr int kOBufs = D == 256 ? 1 : 2;
     static constexpr int kS = 256;  // tensor memory columns: O (twice where it fits), then two of S (P takes its place)
     // A warp that issued MMAs stalls at its next wait until they have read their operands, and the tensor cores run dry:
@@ -105,7 +106,7 @@ struct Shared {
     uint32_t tmem;
     int abort;
 };
-static_assert(sizeof(Shared) <= 3072, "shared bookkeeping");
+static_assert(sizeof(Shared) <= kNotes, "shared bookkeeping");
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
