@@ -313,7 +313,8 @@ int qg_tree_attention(float *out, const float *q, const qg_kv_cache *cache, int 
  * NaN or +infinite logit or no finite one, a malformed tree or a draft outside
  * the vocabulary on its way gets accepted, next and path -1.
  * Sums over the vocabulary are held in 64 bits: the tokens do not depend on
- * how the work is split. vocab at most 2^24. The workspace is zero-filled once. */
+ * how the work is split. Tokens below 2^-900 of a row's largest probability
+ * count as having none. vocab at most 2^24. The workspace is zero-filled once. */
 int qg_verify_workspace_bytes(int seqs, int tokens, int vocab, size_t *bytes);
 int qg_verify_tree(int *path, int *accepted, int *next, const float *logits, const int *draft, const int *parents,
                    const float *draft_probs, const float *uniforms, double temperature, int seqs, int tokens, int vocab,

@@ -62,9 +62,11 @@ __device__ __forceinline__ float ex2(float x) {  // the instruction: |x| <= 1 he
 __device__ __forceinline__ float weigh(float f, float rel) {
     return rel < -126.0f ? 0.0f : ex2(f) * __int_as_float(((int)rel + 127) << 23);
 }
-// 2^rel for rel <= 0 (0 below the range), to bring a sum to another M.
-__device__ __forceinline__ double shift_down(float rel) {
-    return rel < -1000.0f ? 0.0 : __longlong_as_double((long long)((int)rel + 1023) << 52);
+// 2^rel for rel <= 0, 0 below `least`. Sums come to another M down to 2^-900, single weights are held in 64 bits down to
+// 2^-1000: a part of a row whose sum is not zero holds a weight that is not zero, and a uniform of 0 finds it.
+constexpr float kLeastSum = -900.0f, kLeastWeight = -1000.0f;
+__device__ __forceinline__ double shift_down(float rel, float least = kLeastSum) {
+    return rel < least ? 0.0 : __longlong_as_double((long long)((int)rel + 1023) << 52);
 }
 // Conversions and floor run at an eighth of the rate of additions. Where |M| < 2^20, x*scale + (1.5 * 2^23 - M + b) that
 // rounds down is an integer of the last bit, floor(x*scale) - M + b stands in its low bits, and what it leaves of x*scale
@@ -82,8 +84,22 @@ __device__ __forceinline__ float far_weight(float scale, const Stats &r, float x
     return weigh(f, n - r.top);
 }
 __device__ __forceinline__ bool is_near(float scale, const Stats &r) { return scale > 0.0f && fabsf(r.top) < kNear; }
-__device__ __forceinline__ float weight(float scale, const Stats &r, float x, int v) {
-    return is_near(scale, r) ? near_weight(scale, kMagic + 127.0f - r.top, x) : far_weight(scale, r, x, v);
+// The same weights in 64 bits, what is below 2^-126 too. `near`: 2^f 2^(n - M) put together as the bits of a double.
+__device__ __forceinline__ double near_fine(float scale, float k, float x) {  // k: kMagic + 127 - M
+    const float u = __fmaf_rd(x, scale, k);
+    const unsigned g = __float_as_uint(ex2(__fmaf_rn(x, scale, __fsub_rn(k, u))));  // in [1, 2] where it is used
+    const int n = __float_as_int(u) - __float_as_int(kMagic + 127.0f);
+    return u >= kMagic + 127.0f + kLeastWeight ? __hiloint2double((int)(g >> 3) + (n + 896) * (1 << 20), (int)(g << 29)) : 0.0;
+}
+__device__ __forceinline__ double far_fine(float scale, const Stats &r, float x, int v) {
+    if (scale == 0.0f) return v == r.best ? 1.0 : 0.0;
+    if (x == -INFINITY) return 0.0;
+    float f;
+    const float rel = split(x, scale, f) - r.top;
+    return rel < kLeastWeight ? 0.0 : (double)ex2(f) * shift_down(rel, kLeastWeight);
+}
+__device__ __forceinline__ double fine_weight(float scale, const Stats &r, float x, int v) {
+    return is_near(scale, r) ? near_fine(scale, kMagic + 127.0f - r.top, x) : far_fine(scale, r, x, v);
 }
 // Of 8 neighbouring values from v on.
 __device__ __forceinline__ void weights8(float scale, const Stats &r, float (&x)[8], int v) {
@@ -93,6 +109,16 @@ __device__ __forceinline__ void weights8(float scale, const Stats &r, float (&x)
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i] = far_weight(scale, r, x[i], v + i);
+    }
+}
+
+__device__ __forceinline__ void fine8(float scale, const Stats &r, const float (&x)[8], int v, double (&w)[8]) {
+    if (is_near(scale, r)) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i] = near_fine(scale, kMagic + 127.0f - r.top, x[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i] = far_fine(scale, r, x[i], v + i);
     }
 }
 
@@ -248,10 +274,11 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) 
     // Chunks whose loads are in flight together (four: 7 x 6 x 50001 logits 0.6 us slower, 12 x 17 x
     // 131072 0.7 us faster).
     constexpr int kBatch = 2;
+    constexpr double kVisible = 0x1p-126, kCoarse = 0x1p-60;  // weights that 32 bits hold; aims that need the others
     __shared__ Stats rows[kMaxNodes];
     __shared__ double sums[kWarps], batch[DRAWN ? kBatch : 1][kWarps];
     __shared__ unsigned long long kids[kMaxNodes];     // of a node: its children
-    __shared__ float held[kMaxNodes];                  // the target's weight of a draft, 0 after an older sibling's equal
+    __shared__ double held[kMaxNodes];                 // the target's weight of a draft, 0 after an older sibling's equal
     __shared__ unsigned takes[2], bads[2], sane[2], weighty[2];  // nodes as bits
     __shared__ int draft[kMaxNodes], parent[kMaxNodes], path[kMaxNodes], count, at_node, refused;
     __shared__ float first_uniform;
@@ -315,25 +342,25 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) 
     // ---- the walk: a thread per node decides whether it would be taken were it reached with all older siblings
     // refused, so that what is left to do one after the other is to follow bits
     if (warp < kMaxNodes / 32) {
-        float w = tries ? weight(a.scale, rows[parent[tid]], x, draft[tid]) : 0.0f;
+        double w = tries ? fine_weight(a.scale, rows[parent[tid]], x, draft[tid]) : 0.0;
         const unsigned long long older = tries ? kids[parent[tid]] & ((1ull << tid) - 1) : 0;
         if constexpr (!DRAWN)
             for (unsigned long long m = older; m; m &= m - 1)
-                if (draft[__ffsll(m) - 1] == draft[tid]) w = 0.0f;  // a token leaves p once
+                if (draft[__ffsll(m) - 1] == draft[tid]) w = 0.0;  // a token leaves p once
         held[tid] = w;
         asm volatile("bar.sync 1, 64;" ::: "memory");
         bool take = false;
         if (tries) {
             double left = rows[parent[tid]].sum;
             if constexpr (DRAWN) {
-                take = __fmul_rn(u, guess) < w / (float)left;
+                take = w < kVisible ? (double)u * (double)guess < w / left : __fmul_rn(u, guess) < (float)w / (float)left;
             } else {
-                for (unsigned long long m = older; m; m &= m - 1) left -= (double)held[__ffsll(m) - 1];
-                take = (double)u * left < (double)w;
+                for (unsigned long long m = older; m; m &= m - 1) left -= held[__ffsll(m) - 1];
+                take = (double)u * left < w;
             }
         }
         const unsigned t = __ballot_sync(0xffffffffu, take), b = __ballot_sync(0xffffffffu, used && !tries);
-        const unsigned s = __ballot_sync(0xffffffffu, node && rows[node ? tid : 0].best >= 0), h = __ballot_sync(0xffffffffu, w > 0.0f);
+        const unsigned s = __ballot_sync(0xffffffffu, node && rows[node ? tid : 0].best >= 0), h = __ballot_sync(0xffffffffu, w > 0.0);
         if (lane == 0) takes[warp] = t, bads[warp] = b, sane[warp] = s, weighty[warp] = h;
         asm volatile("bar.sync 1, 64;" ::: "memory");
     }
@@ -389,8 +416,7 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) 
             if (off) load4(q, a.vocab, v - off + 8, *reinterpret_cast<float(*)[4]>(&y[8]));
         }
     };
-    auto left8 = [&](int c, float (&w)[8], float (&y)[kY]) {
-        const int v = c * kChunk - lead + 8 * tid;
+    auto turn = [&](float (&y)[kY]) {
         if constexpr (DRAWN) {
             if (off & 1) {
 #pragma unroll
@@ -401,23 +427,53 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) 
                 for (int i = 0; i < 8; i++) y[i] = y[i + 2];
             }
         }
+    };
+    // With drawn drafts p is a 32-bit number, and weights below 2^-126 are left out: all of them come to less than 2^-102.
+    auto left8 = [&](int c, float (&w)[8], float (&y)[kY]) {
+        const int v = c * kChunk - lead + 8 * tid;
+        turn(y);
         weights8(a.scale, r, w, v);  // none outside the row
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            // w/total with one reciprocal for all: from a correctly rounded reciprocal one step on the remainder
+            // leads to the correctly rounded quotient (P. Markstein, 1990), w < 2^-100 aside
+            const float p = w[i] * inverse;
+            w[i] = fmaf(fmaf(-p, total, w[i]), inverse, p);
+            if (q) w[i] = v + i >= 0 && v + i < a.vocab ? fmaxf(w[i] - y[i], 0.0f) : 0.0f;
+        }
+    };
+    // Where nothing may be left out: 64-bit weights (with drawn drafts p, the same 32-bit number where it is one).
+    auto left8_fine = [&](int c, const float (&x)[8], float (&y)[kY], double (&w)[8]) {
+        const int v = c * kChunk - lead + 8 * tid;
+        turn(y);
+        fine8(a.scale, r, x, v, w);
         if constexpr (DRAWN) {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                // w/total with one reciprocal for all: from a correctly rounded reciprocal one step on the remainder
-                // leads to the correctly rounded quotient (P. Markstein, 1990), w < 2^-100 aside
-                const float p = w[i] * inverse;
-                w[i] = fmaf(fmaf(-p, total, w[i]), inverse, p);
-                if (q) w[i] = v + i >= 0 && v + i < a.vocab ? fmaxf(w[i] - y[i], 0.0f) : 0.0f;
+                w[i] = w[i] < kVisible ? w[i] / r.sum : (double)((float)w[i] / total);
+                if (q) w[i] = v + i >= 0 && v + i < a.vocab ? fmax(w[i] - (double)y[i], 0.0) : 0.0;
             }
         }
         for (unsigned long long m = gone; m; m &= m - 1) {
             const int g = draft[__ffsll(m) - 1] - v;
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                if (g == i) w[i] = 0.0f;
+                if (g == i) w[i] = 0.0;
         }
+    };
+    auto fine_sum = [&](int c) -> double {  // of chunk c, by the whole CTA
+        float x[8], y[kY];
+        double w[8], part = 0.0, all = 0.0;
+        fetch(c, x, y);
+        left8_fine(c, x, y, w);
+#pragma unroll
+        for (int i = 0; i < 8; i++) part += w[i];
+        part = warp_sum(part);
+        __syncthreads();
+        if (lane == 0) sums[warp] = part;
+        __syncthreads();
+        for (int k = 0; k < kWarps; k++) all += sums[k];
+        return all;
     };
     double *rest = a.rest + (size_t)seq * a.chunks;
     auto chunk_sum = [&](int c) -> double {
@@ -429,7 +485,7 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) 
             double w = s.best >= 0 ? brought(s, r.top) : 0.0;
             for (unsigned long long m = gone; m; m &= m - 1) {
                 const int g = __ffsll(m) - 1;
-                if ((draft[g] + lead) / kChunk == c) w -= (double)held[g];
+                if ((draft[g] + lead) / kChunk == c) w -= held[g];
             }
             return fmax(w, 0.0);
         }
@@ -438,10 +494,11 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) 
     const int per = (a.chunks + 31) / 32, c0 = min(lane * per, a.chunks), c1 = min(c0 + per, a.chunks);
     constexpr int kKept = 4;  // a lane's first chunks, whose sums stay in registers
     double whole = 0.0, upto = 0.0, sum = 0.0, kept[kKept];
+    bool fine = !DRAWN;
     for (;;) {
         if constexpr (DRAWN) {
             const int full = (a.vocab + lead + kChunk - 1) / kChunk;  // chunks that hold values: all, or all but the last
-            for (int b0 = rank; b0 < full; b0 += kBatch * kCtas) {
+            for (int b0 = rank; b0 < full && !fine; b0 += kBatch * kCtas) {
                 float w[kBatch][8], y[kBatch][kY];
 #pragma unroll
                 for (int i = 0; i < kBatch; i++) fetch(b0 + i * kCtas, w[i], y[i]);  // -infinity past the row's end
@@ -463,6 +520,10 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) 
                 }
                 __syncthreads();
             }
+            for (int b = rank; b < full && fine; b += kCtas) {
+                const double all = fine_sum(b);
+                if (tid == 0) __stcg(rest + b, all);
+            }
             if (rank == 0 && tid == 0 && full < a.chunks) __stcg(rest + full, 0.0);
             cg::this_cluster().sync();  // the sums are there
         }
@@ -474,9 +535,14 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) 
         for (int c = c0 + kKept; c < c1; c++) sum += chunk_sum(c);
         upto = warp_scan(sum);
         whole = __shfl_sync(0xffffffffu, upto, 31);
-        if (!DRAWN || whole > 0.0 || !q) break;
-        q = nullptr;  // the draft's distribution covers the target's: draw from the target's
-        cg::this_cluster().sync();  // the sums were read
+        if constexpr (!DRAWN) {
+            break;
+        } else {
+            if (!fine && !greedy && (double)first_uniform * whole < kCoarse) fine = true;  // the weights left out matter
+            else if (q && !(whole > 0.0)) q = nullptr;  // the draft's distribution covers the target's: draw from the target's
+            else break;
+            cg::this_cluster().sync();  // the sums were read
+        }
     }
     if (rank) return;
     const double aim = (double)first_uniform * whole;
@@ -502,12 +568,18 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) 
     c = __shfl_sync(0xffffffffu, c, owner);
     before = __shfl_sync(0xffffffffu, before, owner);
     // ---- the place in the chunk
-    float w[8], y[kY];
-    fetch(c, w, y);
-    left8(c, w, y);
-    double part = 0.0;
+    float x8[8], y[kY];
+    double w[8], part = 0.0;
+    fetch(c, x8, y);
+    if (fine) {
+        left8_fine(c, x8, y, w);
+    } else {
+        left8(c, x8, y);
 #pragma unroll
-    for (int i = 0; i < 8; i++) part += (double)w[i];
+        for (int i = 0; i < 8; i++) w[i] = x8[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) part += w[i];
     double end = warp_scan(part);
     __syncthreads();
     if (lane == 31) sums[warp] = end;
@@ -521,8 +593,8 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) 
     bool past = false;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        if (!past && w[i] > 0.0f) hit = i;
-        run += (double)w[i];
+        if (!past && w[i] > 0.0) hit = i;
+        run += w[i];
         past |= run > aim;
     }
     a.next[seq] = c * kChunk - lead + 8 * tid + hit;

@@ -1,0 +1,90 @@
+"""The verify step's operators on a B200 where their arithmetic runs out of room. Against the 64-bit definitions
+(oracle/speculate.py)."""
+import numpy as np
+import pytest
+
+from oracle import speculate as S
+from test_gpu_speculate import L  # noqa: F401  (a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+MARK = 123456789  # in next before the call: no token
+
+
+def accept(L, logits, draft, parents, probs, uniforms, temperature):  # noqa: F811
+    seqs, tokens, vocab = logits.shape
+    up = lambda x, t: L.Device(np.ascontiguousarray(x, t))  # noqa: E731
+    bufs = [up(logits, np.float32), up(draft, np.int32), up(parents, np.int32), up(uniforms, np.float32)]
+    dp = None if probs is None else up(probs, np.float32)
+    path, acc, nxt = (up(np.full(n, MARK), np.int32) for n in ((seqs, tokens), seqs, seqs))
+    ws = L.verify_workspace(seqs, tokens, vocab)
+    L.call("verify_tree", path.p, acc.p, nxt.p, bufs[0].p, bufs[1].p, bufs[2].p, dp.p if dp else None, bufs[3].p, temperature, seqs,
+           tokens, vocab, ws.p)
+    return path.get(), acc.get(), nxt.get()
+
+
+def check(L, logits, draft, parents, probs, uniforms, temperature):  # noqa: F811
+    logits, uniforms = np.asarray(logits, np.float32), np.asarray(uniforms, np.float32)
+    path, acc, nxt = accept(L, logits, np.asarray(draft), np.asarray(parents), probs, uniforms, temperature)
+    for s in range(len(logits)):
+        p, n, _ = S.verify(logits[s], draft[s], parents[s], None if probs is None else np.asarray(probs, np.float32)[s], uniforms[s],
+                           temperature)
+        assert list(path[s]) == p + [-1] * (len(parents[s]) - len(p)), s
+        assert acc[s] == len(p) - 1
+        assert nxt[s] == n, s
+
+
+# ---- weights far below the row's largest -----------------------------------
+
+
+def cliff(gap, vocab=9000, high=1000):
+    """A row whose first logits are `gap` below its last ones."""
+    row = np.full(vocab, -gap, np.float32)
+    row[-high:] = 0.0
+    return row
+
+
+@pytest.mark.parametrize("drawn", [False, True])
+@pytest.mark.parametrize("gap,temperature", [(60, 1.0), (100, 1.0), (10, 0.1), (140, 0.5), (420, 1.0), (5e5, 8e3)])
+def test_uniform_of_zero_takes_the_first_token_with_any_mass(L, drawn, gap, temperature):  # noqa: F811
+    """Chunks of the vocabulary up to 600 octaves below the largest weight; the row begins with tokens without any."""
+    row = cliff(gap)
+    row[:10] = -np.inf
+    rows = np.stack([[row, row], [np.roll(row, 4500), row]])
+    probs = np.full((2, 2, 9000), 1 / 9000) if drawn else None
+    # the draft has no mass, or is refused at no uniform; then the next token is drawn at uniform 0
+    check(L, rows, [[0, 3], [0, 20]], [[-1, 0]] * 2, probs, [[0, 0.5], [0, 1 - 2.0 ** -24]], temperature)
+
+
+def test_uniform_of_zero_where_the_logits_are_large(L):  # noqa: F811
+    """Logits at which t is beyond 2^22; with this temperature t is the logit, so 32 bits hold it."""
+    row = cliff(150) + np.float32(2.0 ** 22)
+    check(L, np.stack([[row], [np.roll(row, -500)]]), [[0]] * 2, [[-1]] * 2, None, [[0], [0]], 1.4426950408889634)
+
+
+@pytest.mark.parametrize("drawn", [False, True])
+def test_uniform_of_zero_accepts_a_draft_with_any_mass(L, drawn):  # noqa: F811
+    rows = np.stack([[cliff(110)] * 3])
+    probs = np.full((1, 3, 9000), 1 / 9000) if drawn else None
+    check(L, rows, [[0, 17, 4321]], [[-1, 0, 1]], probs, [[0, 0, 0]], 1.0)
+
+
+@pytest.mark.parametrize("drawn", [False, True])
+def test_uniforms_among_tiny_weights(L, drawn):  # noqa: F811
+    """Uniforms so small that the aim falls among weights of e^-100."""
+    tiny = np.exp(-100.0)
+    u = [np.float32(k * 2.0 ** -149) for k in range(1, 200)]
+    # the aim in units of the tiny weight, away from where the token changes
+    u = [x for x in u if 0.1 < float(x) * (1000 + 8000 * tiny) / tiny % 1 < 0.9 and float(x) * 1000 < 7990 * tiny][:40]
+    assert len(u) > 20
+    rows = np.stack([[cliff(100)]] * len(u))
+    probs = np.full((len(u), 1, 9000), 1 / 9000) if drawn else None
+    check(L, rows, [[0]] * len(u), [[-1]] * len(u), probs, [[x] for x in u], 1.0)
+
+
+def test_what_a_drafts_distribution_leaves_may_be_tiny(L):  # noqa: F811
+    """q is above p wherever p has visible mass: max(p - q, 0) has its mass on tokens of e^-100."""
+    probs = np.zeros((2, 2, 9000), np.float32)
+    probs[:, 1, 8000:] = 0.0011
+    check(L, np.stack([[cliff(100)] * 2] * 2), [[0, 8003]] * 2, [[-1, 0]] * 2, probs, [[0.50007, 1 - 2.0 ** -24], [0, 1 - 2.0 ** -24]], 1.0)
