@@ -266,9 +266,134 @@ __device__ __forceinline__ int claim(double part, double upto, double aim) {
     return passes ? __ffs(passes) - 1 : has ? 31 - __clz(has) : -1;
 }
 
+// What refused drafts leave of a row's or a chunk's mass is taken as a difference of 64-bit sums, which are off by some
+// 2^-50. Where it comes out below this share of the sum, walk_anew adds up what is there.
+constexpr double kSure = 0x1p-20;
+
+// The thread's eight weights of chunk c, without those of the nodes `gone`.
+__device__ void weights_without(const VerifyArgs &a, const float *row, const Stats &r, int c, unsigned long long gone,
+                                const int *draft, double (&w)[8]) {
+    const int v = c * kChunk - chunk_lead(row) + 8 * (int)threadIdx.x;
+    float x[8];
+    load4(row, a.vocab, v, *reinterpret_cast<float(*)[4]>(&x[0]));
+    load4(row, a.vocab, v + 4, *reinterpret_cast<float(*)[4]>(&x[4]));
+    fine8(a.scale, r, x, v, w);
+    for (unsigned long long m = gone; m; m &= m - 1) {
+        const int g = draft[__ffsll(m) - 1] - v;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (g == i) w[i] = 0.0;
+    }
+}
+// Their sum over chunks c0 .. c1-1, by one CTA.
+__device__ double sum_without(const VerifyArgs &a, const float *row, const Stats &r, int c0, int c1, unsigned long long gone,
+                              const int *draft, double *sums) {
+    double part = 0.0, all = 0.0;
+    for (int c = c0; c < c1; c++) {
+        double w[8];
+        weights_without(a, row, r, c, gone, draft, w);
+#pragma unroll
+        for (int i = 0; i < 8; i++) part += w[i];
+    }
+    part = warp_sum(part);
+    __syncthreads();
+    if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = part;
+    __syncthreads();
+    for (int k = 0; k < kWalkThreads / 32; k++) all += sums[k];
+    return all;
+}
+// The walk for given drafts and the draw of the next token, one step after the other and by sums of what is left. Rare (refused
+// drafts hold all but 2^-20 of p), and apart from the other walk: in the way of it 9.0 us became 9.7 (one tree of
+// 17 x 131072 logits).
+__noinline__ __device__ void walk_anew(const VerifyArgs &a, int seq, const Stats *rows, const unsigned long long *kids, const int *draft,
+                                       const double *held, int *path, double *sums) {
+    __shared__ int first, last;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const size_t base = (size_t)seq * a.tokens;
+    int cur = 0, n = 0;
+    unsigned long long gone;
+    bool ok = true;
+    path[0] = 0;
+    for (;;) {
+        int to = -1;
+        gone = 0;
+        double held_gone = 0.0;
+        for (unsigned long long k = kids[cur]; k; k &= k - 1) {
+            const int c = __ffsll(k) - 1;
+            ok = (unsigned)draft[c] < (unsigned)a.vocab;
+            if (!ok) break;
+            double left = rows[cur].sum - held_gone;
+            if (gone && left < kSure * rows[cur].sum)
+                left = sum_without(a, a.logits + (base + cur) * a.vocab, rows[cur], 0, a.chunks, gone, draft, sums);
+            if ((double)a.uniforms[base + c] * left < held[c]) {
+                to = c;
+                break;
+            }
+            gone |= 1ull << c;
+            held_gone += held[c];
+        }
+        if (to < 0) break;
+        ok = rows[to].best >= 0;
+        if (!ok) break;
+        cur = to;
+        n++;
+        path[n] = to;  // all threads write the same
+    }
+    __syncthreads();
+    if (tid < a.tokens) a.path[base + tid] = ok && tid <= n ? path[tid] : -1;
+    if (tid == 0) {
+        a.accepted[seq] = ok ? n : -1;
+        a.next[seq] = -1;
+        first = kWalkThreads, last = -1;
+    }
+    if (!ok) return;
+    const float *row = a.logits + (base + cur) * a.vocab;
+    const Stats r = rows[cur];
+    double *rest = a.rest + (size_t)seq * a.chunks, whole = 0.0, run = 0.0, before = 0.0;
+    for (int c = 0; c < a.chunks; c++) {
+        const double all = sum_without(a, row, r, c, c + 1, gone, draft, sums);
+        if (tid == 0) __stcg(rest + c, all);
+        whole += all;
+    }
+    __syncthreads();
+    const double aim = (double)a.uniforms[base] * whole;
+    int chunk = -1;
+    for (int c = 0; c < a.chunks && (chunk < 0 || run <= aim); c++) {
+        const double all = __ldcg(rest + c);
+        if (all > 0.0) chunk = c, before = run;
+        run += all;
+    }
+    if (chunk < 0) return;  // not with uniforms below 1
+    double w[8], part = 0.0;
+    weights_without(a, row, r, chunk, gone, draft, w);
+#pragma unroll
+    for (int i = 0; i < 8; i++) part += w[i];
+    double end = warp_scan(part);
+    if (lane == 31) sums[warp] = end;
+    __syncthreads();
+    end += before;
+    for (int k = 0; k < warp; k++) end += sums[k];
+    if (part > 0.0) {
+        if (aim < end) atomicMin(&first, tid);
+        atomicMax(&last, tid);
+    }
+    __syncthreads();
+    if (tid != (first < kWalkThreads ? first : last)) return;
+    run = end - part;
+    int hit = 0;
+    bool past = false;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        if (!past && w[i] > 0.0) hit = i;
+        run += w[i];
+        past |= run > aim;
+    }
+    a.next[seq] = chunk * kChunk - chunk_lead(row) + 8 * tid + hit;
+}
+
 // DRAWN: the drafts' distributions are given; a cluster of kDrawnCtas CTAs per sequence, otherwise one CTA.
 template <bool DRAWN>
-__global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kWalkThreads) walk_kernel(const __grid_constant__ VerifyArgs a) {
     constexpr int kWarps = kWalkThreads / 32, kCtas = DRAWN ? kDrawnCtas : 1;
     static_assert(kWalkThreads * 8 == kChunk, "eight values of a chunk to a thread");
     // Chunks whose loads are in flight together (four: 7 x 6 x 50001 logits 0.6 us slower, 12 x 17 x
@@ -279,8 +404,8 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) 
     __shared__ double sums[kWarps], batch[DRAWN ? kBatch : 1][kWarps];
     __shared__ unsigned long long kids[kMaxNodes];     // of a node: its children
     __shared__ double held[kMaxNodes];                 // the target's weight of a draft, 0 after an older sibling's equal
-    __shared__ unsigned takes[2], bads[2], sane[2], weighty[2];  // nodes as bits
-    __shared__ int draft[kMaxNodes], parent[kMaxNodes], path[kMaxNodes], count, at_node, refused;
+    __shared__ unsigned takes[2], bads[2], sane[2], weighty[2], unsure[2];  // nodes as bits
+    __shared__ int draft[kMaxNodes], parent[kMaxNodes], path[kMaxNodes], count, at_node, refused, doubt;
     __shared__ float first_uniform;
     const int seq = blockIdx.x / kCtas, rank = blockIdx.x % kCtas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const size_t base = (size_t)seq * a.tokens;
@@ -349,7 +474,7 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) 
                 if (draft[__ffsll(m) - 1] == draft[tid]) w = 0.0;  // a token leaves p once
         held[tid] = w;
         asm volatile("bar.sync 1, 64;" ::: "memory");
-        bool take = false;
+        bool take = false, close = false;  // close: the older siblings leave next to nothing
         if (tries) {
             double left = rows[parent[tid]].sum;
             if constexpr (DRAWN) {
@@ -357,16 +482,19 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) 
             } else {
                 for (unsigned long long m = older; m; m &= m - 1) left -= held[__ffsll(m) - 1];
                 take = (double)u * left < w;
+                close = older && left < kSure * rows[parent[tid]].sum;
             }
         }
         const unsigned t = __ballot_sync(0xffffffffu, take), b = __ballot_sync(0xffffffffu, used && !tries);
         const unsigned s = __ballot_sync(0xffffffffu, node && rows[node ? tid : 0].best >= 0), h = __ballot_sync(0xffffffffu, w > 0.0);
-        if (lane == 0) takes[warp] = t, bads[warp] = b, sane[warp] = s, weighty[warp] = h;
+        const unsigned z = __ballot_sync(0xffffffffu, close);
+        if (lane == 0) takes[warp] = t, bads[warp] = b, sane[warp] = s, weighty[warp] = h, unsure[warp] = z;
         asm volatile("bar.sync 1, 64;" ::: "memory");
     }
     auto bits = [](const unsigned (&m)[2]) { return m[0] | (unsigned long long)m[1] << 32; };
     if (tid == 0) {
-        const unsigned long long taken = bits(takes), bad = bits(bads), good = bits(sane);
+        const unsigned long long taken = bits(takes), bad = bits(bads), good = bits(sane), doubted = bits(unsure);
+        unsigned long long met = 0;  // nodes that were tried
         int cur = 0, n = 0;
         bool ok = sound && (good & 1);
         refused = -1;
@@ -374,19 +502,25 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) 
         while (ok) {
             const unsigned long long k = kids[cur], first = DRAWN ? k & (~k + 1) : k, t = first & taken;
             if (!t) {
+                met |= k;
                 ok = !(bad & k) && !(DRAWN && (k & (k - 1)));
                 refused = __ffsll(k) - 1;
                 break;
             }
             const unsigned long long c = t & (~t + 1);
+            met |= k & (c | (c - 1));
             ok = !(bad & k & (c - 1)) && (good & c);
             cur = __ffsll(c) - 1;
             path[++n] = cur;
         }
         at_node = ok ? cur : -1;
         count = ok ? n : -1;
+        doubt = (met & doubted) != 0;
     }
     __syncthreads();
+    if constexpr (!DRAWN) {
+        if (doubt) return walk_anew(a, seq, rows, kids, draft, held, path, sums);
+    }
     if (rank == 0) {
         if (tid < a.tokens) a.path[base + tid] = tid <= count ? path[tid] : -1;
         if (tid == 0) a.accepted[seq] = count;
@@ -476,18 +610,21 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) 
         return all;
     };
     double *rest = a.rest + (size_t)seq * a.chunks;
+    bool close = false;  // a chunk of refused drafts has next to nothing left
     auto chunk_sum = [&](int c) -> double {
         if constexpr (DRAWN) {
             return __ldcg(rest + c);
         } else {
             const Stats s = a.stats[(base + at_node) * a.chunks + c];
             if (greedy) return s.best == r.best ? 1.0 : 0.0;
-            double w = s.best >= 0 ? brought(s, r.top) : 0.0;
+            const double all = s.best >= 0 ? brought(s, r.top) : 0.0;
+            double w = all;
             for (unsigned long long m = gone; m; m &= m - 1) {
                 const int g = __ffsll(m) - 1;
                 if ((draft[g] + lead) / kChunk == c) w -= held[g];
             }
-            return fmax(w, 0.0);
+            close |= w < kSure * all;
+            return w;
         }
     };
     // ---- the chunk that holds the aim: every warp finds it for itself, a lane takes neighbouring chunks
@@ -536,6 +673,7 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyArgs a) 
         upto = warp_scan(sum);
         whole = __shfl_sync(0xffffffffu, upto, 31);
         if constexpr (!DRAWN) {
+            if (__any_sync(0xffffffffu, close)) return walk_anew(a, seq, rows, kids, draft, held, path, sums);  // all warps say the same
             break;
         } else {
             if (!fine && !greedy && (double)first_uniform * whole < kCoarse) fine = true;  // the weights left out matter

@@ -88,3 +88,50 @@ def test_what_a_drafts_distribution_leaves_may_be_tiny(L):  # noqa: F811
     probs = np.zeros((2, 2, 9000), np.float32)
     probs[:, 1, 8000:] = 0.0011
     check(L, np.stack([[cliff(100)] * 2] * 2), [[0, 8003]] * 2, [[-1, 0]] * 2, probs, [[0.50007, 1 - 2.0 ** -24], [0, 1 - 2.0 ** -24]], 1.0)
+
+
+# ---- what refused drafts leave ---------------------------------------------
+
+
+LAST = 1 - 2.0 ** -24
+
+
+@pytest.mark.parametrize("vocab", [40, 9000])
+def test_the_last_token_left_is_accepted(L, vocab):  # noqa: F811
+    """Two refused drafts hold all but 1e-14 of the mass: the third is the only token left and is taken at any uniform."""
+    seqs, places = 16, [3, 5, vocab - 9]
+    rows = np.full((seqs, 4, vocab), -np.inf, np.float32)
+    for s in range(seqs):
+        rows[s, :, places] = np.array([0.0, -15.5, -31.0 - 0.06 * s], np.float32)[:, None]
+    check(L, rows, [[0, *places]] * seqs, [[-1, 0, 0, 0]] * seqs, None, np.full((seqs, 4), LAST), 1.0)
+
+
+@pytest.mark.parametrize("first", [0.0, 0.25, LAST])
+def test_a_chunk_whose_tokens_were_all_refused_is_not_drawn_from(L, first):  # noqa: F811
+    seqs = 16
+    rows = np.full((seqs, 3, 9000), -np.inf, np.float32)
+    for s in range(seqs):
+        rows[s, :, [3, 5, 8000]] = np.array([0.0, -22.0 - 0.1 * s, -15.5], np.float32)[:, None]
+    check(L, rows, [[0, 3, 5]] * seqs, [[-1, 0, 0]] * seqs, None, [[first, LAST, LAST]] * seqs, 1.0)
+
+
+def test_what_is_left_beside_a_refused_draft(L):  # noqa: F811
+    """The refused draft holds all but 1e-10 of its chunk: the others of the chunk are drawn by their own weights."""
+    seqs, vocab = 32, 9000
+    rng = np.random.default_rng(3)
+    rows = np.full((seqs, 2, vocab), -np.inf, np.float32)
+    rows[:, :, 100:140] = -28.0 + rng.normal(size=(seqs, 1, 40))
+    rows[:, :, 7] = 0.0
+    rows[:, :, 8000] = -15.5
+    u = np.full((seqs, 2), LAST, np.float32)
+    draft = [[0, 7]] * seqs
+    for s in range(seqs):  # an aim among the 40, and away from where the token changes
+        while True:
+            u[s, 0] = rng.random() * 1e-4
+            _, n, _ = S.verify(rows[s], draft[s], [-1, 0], None, u[s], 1.0)
+            p = S.target(rows[s, 0], 1.0)
+            p[7] = 0.0
+            run = np.cumsum(p)
+            if 100 <= n < 140 and np.abs(run[99:140] - u[s, 0] * run[-1]).min() > 1e-5 * run[139]:
+                break
+    check(L, rows, draft, [[-1, 0]] * seqs, None, u, 1.0)
