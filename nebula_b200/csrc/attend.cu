@@ -47,6 +47,9 @@ constexpr int kNotes = 3 * 1024;  // bytes for the roles' shared bookkeeping
 constexpr int kRegsControl = 48, kRegsSoftmax = 112, kRegsAcc = 176;
 static_assert(kRegsControl + kRegsSoftmax + 2 * kRegsAcc <= 4 * (65536 / kThreads), "register split");
 constexpr float kPScale = 32768.0f;  // P as F16: 2^15 at the maximum, so that small weights keep their bits
+// c x - m is one instruction whose product is not rounded; m is. Up to this |m| the two differ by 2^-4 at most; far above it
+// P at the maximum would be beyond F16, or nothing. There the scores are taken relative to the largest before they are scaled.
+constexpr float kFar = 1048576.0f;  // 2^20
 
 struct AttendArgs {
     CacheView c;
@@ -677,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             const uint32_t qb = item % QB;
             ok = wait_warp(&s.q_full[qb], item / QB & 1, abort, a.err);
             const float c = s.q_scale[qb][row];
-            float m = -INFINITY, l = 0.0f, l_low = 0.0f;
+            float most = -INFINITY, m = -INFINITY, l = 0.0f, l_low = 0.0f;  // most: the largest score as it is; m = c * most
             for (int j = 0; ok && j < it.count; j++, tile++) {
                 const uint32_t buf = tile & 1, cols = tmem + lanes + C::kS + buf * kKeys;
                 const int past = it.length - (it.first + j) * kKeys;  // keys of this unit before the nodes
@@ -709,7 +712,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
 #pragma unroll
                         for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], x[i]);
                     }
-                    const float m_new = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c);
+                    const float here = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), m_new = fmaxf(m, here * c);
+                    most = fmaxf(most, here);
                     keep = m == -INFINITY ? 0.0f : ex2(m - m_new);
                     off = m_new == -INFINITY ? 0.0f : m_new;
                     m = m_new;
@@ -722,6 +726,21 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 __syncwarp();
                 if (lane == 0) arrive(&s.msg_full[slot]);
                 msg++;
+                if (__builtin_expect(__any_sync(0xffffffffu, fabsf(off) >= kFar), 0)) {  // (in the chunks' way instead: 98k keys 103 -> 105 us)
+                    float base = 0.0f;
+                    if (fabsf(off) >= kFar) base = most, off = 0.0f;
+#pragma unroll 1
+                    for (int h = h0; h < min(h1, held); h++) {
+                        float x[32];
+                        tmem_ld32(cols + 32 * h, x);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) x[i] -= base;
+                        tmem_st16(cols + 32 * h, reinterpret_cast<const uint32_t(&)[16]>(x[0]));
+                        tmem_st16(cols + 32 * h + 16, reinterpret_cast<const uint32_t(&)[16]>(x[16]));
+                    }
+                    tmem_wait_st();
+                }
                 float2 sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
                 const float2 c2 = {c, c}, off2 = {-off, -off}, up2 = {kPScale, kPScale};
 #pragma unroll 1

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from oracle import speculate as S
-from test_gpu_speculate import L  # noqa: F401  (a fixture)
+from test_gpu_speculate import L, Cache, attend, expected  # noqa: F401  (L is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -135,3 +135,30 @@ def test_what_is_left_beside_a_refused_draft(L):  # noqa: F811
             if 100 <= n < 140 and np.abs(run[99:140] - u[s, 0] * run[-1]).min() > 1e-5 * run[139]:
                 break
     check(L, rows, draft, [[-1, 0]] * seqs, None, u, 1.0)
+
+
+# ---- large scores ----------------------------------------------------------
+
+
+@pytest.mark.parametrize("hq,hkv,d,tokens", [(4, 1, 64, 1), (4, 1, 64, 3), (16, 4, 64, 25), (32, 8, 128, 1), (8, 1, 128, 1),
+                                             (32, 8, 128, 17), (24, 2, 256, 1), (24, 2, 256, 9), (24, 2, 256, 17)])
+@pytest.mark.parametrize("size", [1e6, 1e8, 1e11])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_attention_of_scores_far_beyond_a_unit(L, hq, hkv, d, tokens, size, sign):  # noqa: F811
+    """One key of each sequence is far above the others (by a tenth of the scores' size): the row is its value."""
+    rng = np.random.default_rng(d + tokens)
+    lengths = [40, 300, 2500]
+    cache = Cache(L, rng, lengths, tokens, hkv, d, 32)
+    cache.k[:] = np.where(np.isnan(cache.k), cache.k, 0)
+    for s, n in enumerate(lengths):
+        rows = cache.rows(s, 0, n + tokens)
+        cache.k[0, rows, :, 0] = rng.integers(900, 1000, (n + tokens, 1)) if sign > 0 else rng.integers(1300, 1400, (n + tokens, 1))
+        cache.k[0, rows[n // 3], :, 0] = 1200
+    cache.upload()
+    q = np.zeros((len(lengths), tokens, hq, d), np.float32)
+    q[..., 0] = sign * size / 1000 * (1 + rng.random(q.shape[:3]))
+    got = attend(L, cache, q, None, 1.0)
+    want = expected(cache, q, None, 1.0)
+    assert np.isfinite(got).all()
+    # all other weights are below 2^-1000 of the largest; P is 2^15 and V an F16
+    np.testing.assert_array_equal(got, want.astype(np.float32))
