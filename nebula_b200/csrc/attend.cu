@@ -98,14 +98,18 @@ struct Cfg {
     static constexpr int kTileRows = PAIR ? 2 * kRows : kRows;
 };
 
-struct Shared {
+// The slots of one CTA (or pair), and where the first of them lies.
+struct Plan {
+    long long slot0, slot1;
+    int seq0, length0, kv0, tile0, pos0;
+};
+
+struct Shared : Plan {
     float val[2][kRows];    // rescaling factors, and at an item's end the totals: softmax -> accumulators
     float q_scale[2][kRows];  // at an item's end the maxima
     uint64_t k_full[7], k_empty[7], v_full[7], v_empty[7], s_full[2], p_full[2][4], pv_done[2], msg_full[2], msg_empty[2], o_full[2], o_empty[2], q_full[2], q_all, landed[2], clean[2], drain;
     int pages[2][2][8];     // of the units that the producers are at: keys, values
     uint64_t odd_nodes;     // nodes whose values are not finite
-    long long slot0, slot1;
-    int seq0, length0, kv0, tile0, pos0;
     uint32_t tmem;
     int abort;
 };
@@ -348,7 +352,7 @@ template <int D>
 struct Walk {
     long long at, end;
     int seq, length, kv, tile, pos;  // pos: slot within the item
-    __device__ Walk(const Shared &s)
+    __device__ Walk(const Plan &s)
         : at(s.slot0), end(s.slot1), seq(s.seq0), length(s.length0), kv(s.kv0), tile(s.tile0), pos(s.pos0) {}
     __device__ bool next(const AttendArgs &a, Item &it) {
         const int from = max(pos, kItemCost<D>);
@@ -375,7 +379,7 @@ struct Walk {
 
 // One warp: the slots of CTA (or pair) `team`.
 template <int D>
-__device__ __forceinline__ void plan(const AttendArgs &a, Shared &s, int team, int teams) {
+__device__ __forceinline__ void plan(const AttendArgs &a, Plan &s, int team, int teams) {
     const int lane = threadIdx.x & 31;
     const int per = a.c.kv_heads * a.row_tiles;
     const int len = lane < a.seqs ? a.c.committed(lane, a.tokens) : -1;
@@ -1097,7 +1101,8 @@ struct Few {
     static constexpr int kStage = 2 * kLoads * 512, kStages = D == 128 ? 3 : 6;
     static constexpr int kRing = kFewWarps * kStages * kStage, kSmem = kRing + kFewWarps * kFewRows * D * 4;
     static_assert(kLoads * kFewRows == kLanes, "a score to a lane");
-    static_assert(kSmem + 2048 <= 232448, "shared memory");
+    // the kernel's own variables lie before, up to the next multiple of 1024
+    static_assert(kSmem + (sizeof(Plan) + kFewWarps * kFewRows * sizeof(float2) + 1023) / 1024 * 1024 <= 232448, "shared memory");
 };
 
 __device__ __forceinline__ void eight(const unsigned char *p, float (&x)[8], bool none = false) {
@@ -1114,7 +1119,7 @@ template <int D>
 __global__ void __launch_bounds__(32 * kFewWarps, 1) token_attention_kernel(const __grid_constant__ AttendArgs a) {
     using C = Few<D>;
     extern __shared__ __align__(1024) unsigned char smem[];
-    __shared__ Shared s;
+    __shared__ Plan s;
     __shared__ float2 ml[kFewWarps][kFewRows];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, team = blockIdx.x;
     const int key = lane / C::kLanes, dim = lane % C::kLanes * 8;
