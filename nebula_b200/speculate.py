@@ -19,10 +19,10 @@ Q4_K, F32 = 12, 0
 
 
 def tree_masks(parents) -> np.ndarray:
-    """One 64-bit mask per node: the node and its ancestors."""
+    """One 64-bit mask per node: the node and its ancestors (parent -1: none)."""
     masks = np.zeros(len(parents), np.uint64)
     for i, p in enumerate(parents):
-        masks[i] = (masks[p] if i else np.uint64(0)) | np.uint64(1 << i)
+        masks[i] = (masks[p] if i and p >= 0 else np.uint64(0)) | np.uint64(1 << i)
     return masks
 
 
@@ -30,12 +30,13 @@ def depths(parents) -> np.ndarray:
     """The nodes' distances from the root: their positions after the committed tokens."""
     d = np.zeros(len(parents), np.int32)
     for i, p in enumerate(parents):
-        d[i] = d[p] + 1 if i else 0
+        d[i] = d[p] + 1 if i and p >= 0 else 0
     return d
 
 
 class Speculator:
-    """One sequence. ``nodes``: the largest tree (the last token and its drafts), at most 64."""
+    """One sequence. ``nodes``: the largest tree (the last token and its drafts), at most 64. ``capacity``: tokens that the
+    cache has room for, drafts of the last step included; ``committed``: those it holds."""
 
     def __init__(self, layers=2, vocab=1024, capacity=512, nodes=9, q_heads=24, kv_heads=2, head_dim=256, rotary=64, page=64,
                  hidden=2048, ffn=512, seed=1):
@@ -58,7 +59,7 @@ class Speculator:
 
         # the cache: one page table for all layers, pages in any order
         pages = -(-(capacity + nodes) // page)
-        self.capacity = pages * page
+        self.capacity, self.committed = pages * page, 0
         layer_bytes = pages * page * kv_heads * head_dim * 2
         self.k, self.v = L.Device(nbytes=layers * layer_bytes), L.Device(nbytes=layers * layer_bytes)
         self.table = L.Device(np.random.default_rng(seed).permutation(pages).astype(np.int32))
@@ -84,8 +85,21 @@ class Speculator:
         values = np.ascontiguousarray(values, dtype)
         L.call("write", buf.p, values.ctypes.data, values.nbytes)
 
+    def _check(self, tokens, parents) -> None:
+        """The buffers hold ``nodes`` rows and the embedding ``vocab``: nothing outside them may reach an entry point."""
+        t = len(tokens)
+        if not 1 <= t <= self.nodes or len(parents) != t:
+            raise ValueError(f"{t} tokens and {len(parents)} parents: one parent each, at most {self.nodes}")
+        if not all(0 <= int(x) < self.vocab for x in tokens):
+            raise ValueError(f"a token outside the vocabulary of {self.vocab}")
+        if not all(-1 <= int(p) < i for i, p in enumerate(parents) if i):
+            raise ValueError("a node's parent comes before it")
+        if self.committed + t > self.capacity:
+            raise ValueError(f"{self.committed} tokens committed, {t} more: the cache holds {self.capacity}")
+
     def forward(self, tokens, parents) -> None:
         """The nodes through every layer; their keys and values follow the committed ones in the cache."""
+        self._check(tokens, parents)
         t, d = len(tokens), self.head_dim
         self._put(self.masks, tree_masks(parents), np.uint64)
         self._put(self.offsets, depths(parents), np.int32)
@@ -108,28 +122,38 @@ class Speculator:
 
     def prefill(self, tokens) -> None:
         """Tokens that are given: all of them are kept."""
+        if self.committed + len(tokens) > self.capacity:
+            raise ValueError(f"{self.committed} tokens committed, {len(tokens)} more: the cache holds {self.capacity}")
+        if not all(0 <= int(x) < self.vocab for x in tokens):
+            raise ValueError(f"a token outside the vocabulary of {self.vocab}")
         for at in range(0, len(tokens), self.nodes):
             part = tokens[at : at + self.nodes]
             self.forward(part, range(-1, len(part) - 1))
             self._put(self.path, range(len(part)), np.int32)
             self._put(self.accepted, [len(part) - 1], np.int32)
             L.call("cache_commit", C.byref(self.cache), self.lengths.p, self.path.p, self.accepted.p, 1, len(part))
+            self.committed += len(part)
 
     def step(self, tokens, parents, uniforms=None, temperature=0.0):
         """``tokens[0]`` is the last token chosen, the others are drafts. Returns the accepted nodes (the root first) and
         the token after them; the accepted nodes' keys and values stay in the cache."""
         t = len(tokens)
+        self._check(tokens, parents)
+        uniforms = np.zeros(t) if uniforms is None else np.asarray(uniforms, np.float64)
+        if uniforms.shape != (t,) or not ((uniforms >= 0) & (uniforms < 1)).all():
+            raise ValueError(f"{t} uniforms in [0, 1)")
         self.forward(tokens, parents)
         L.call("matmul", self.logits.p, self.head.p, F32, self.vocab, self.hidden, self.x.p, t)
         self._put(self.draft, tokens, np.int32)
         self._put(self.parents, list(parents), np.int32)
-        self._put(self.uniforms, np.zeros(t) if uniforms is None else uniforms, np.float32)
+        self._put(self.uniforms, np.minimum(uniforms, 1 - 2.0 ** -24), np.float32)  # none is rounded to 1
         L.call("verify_tree", self.path.p, self.accepted.p, self.next.p, self.logits.p, self.draft.p, self.parents.p, None,
                self.uniforms.p, temperature, 1, t, self.vocab, self.verify_ws.p)
         L.call("cache_commit", C.byref(self.cache), self.lengths.p, self.path.p, self.accepted.p, 1, t)
         accepted = int(self.accepted.get()[0])
         if accepted < 0:
             raise RuntimeError("the target gave no distribution")
+        self.committed += accepted + 1
         return [int(n) for n in self.path.get()[: accepted + 1]], int(self.next.get()[0])
 
 
@@ -165,7 +189,8 @@ def main() -> None:
     a = ap.parse_args()
     rng = np.random.default_rng(0)
     prompt = [int(t) for t in rng.integers(0, 1024, 20)]
-    plain = greedy(Speculator(layers=a.layers), prompt, a.count)
+    size = dict(layers=a.layers, capacity=len(prompt) + a.count)
+    plain = greedy(Speculator(**size), prompt, a.count)
 
     def drafter(chosen):  # a stand-in for a draft model: often right; two candidates for each of three positions
         drafts, parents, at = [], [], 0
@@ -176,7 +201,7 @@ def main() -> None:
             at = len(drafts)
         return drafts, parents
 
-    text, steps = speculative(Speculator(layers=a.layers), prompt, a.count, drafter)
+    text, steps = speculative(Speculator(**size), prompt, a.count, drafter)
     if text != plain:
         raise SystemExit("the texts differ")
     print(f"{a.count} tokens: {a.count} steps one at a time, {steps} steps with drafted trees, the same text")
