@@ -109,7 +109,7 @@ struct Shared : Plan {
     float q_scale[2][kRows];  // at an item's end the maxima
     uint64_t k_full[7], k_empty[7], v_full[7], v_empty[7], s_full[2], p_full[2][4], pv_done[2], msg_full[2], msg_empty[2], o_full[2], o_empty[2], q_full[2], q_all, landed[2], clean[2], drain;
     int pages[2][2][8];     // of the units that the producers are at: keys, values
-    uint64_t odd_nodes;     // nodes whose values are not finite
+    uint64_t odd_nodes[2];  // nodes whose values are not finite: of this item, and of the next (a pair's other CTA may be there)
     uint32_t tmem;
     int abort;
 };
@@ -418,7 +418,10 @@ __device__ __forceinline__ uint32_t value_pieces(const AttendArgs &a, const Item
     return (it.count - 1) * C::kPieces + (keys_of(a, it, it.count - 1) + C::kVKeys - 1) / C::kVKeys;
 }
 
-// Nodes whose values are not finite, in the notes of both CTAs of a pair: each sees half of the columns.
+// Nodes whose values are not finite, in the notes of both CTAs of a pair: each sees half of the columns. The other CTA may
+// still be at the item before (it has given O back, but not yet read and cleared its notes), so notes are kept by the item's
+// parity; two items apart they cannot be, for the unit between them takes both CTAs' O. The fence brings the note to the
+// other CTA before the values are reported clean.
 template <bool PAIR>
 __device__ __forceinline__ void mark_odd(uint64_t *notes, uint64_t nodes) {
     if constexpr (!PAIR) {
@@ -430,6 +433,7 @@ __device__ __forceinline__ void mark_odd(uint64_t *notes, uint64_t nodes) {
                          "atom.relaxed.cluster.shared::cluster.or.b64 x, [a], %1;\n\t}" ::"r"(smem_u32(notes)),
                          "l"(nodes), "r"(r)
                          : "memory");
+        asm volatile("fence.acq_rel.cluster;" ::: "memory");
     }
 }
 
@@ -438,6 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                                                                      const __grid_constant__ CUtensorMap k_map,
                                                                      const __grid_constant__ CUtensorMap v_map) {
     using C = Cfg<D, MR, PAIR>;
+    static_assert(!PAIR || C::kOBufs == 1, "mark_odd: a unit takes both CTAs' O of the unit before");
     const int copies = D == 256 ? 1 : a.copies;
     constexpr int NC = C::kChunks, NK = C::kKStages, NV = C::kVStages, VK = C::kVKeys, QB = C::kQBufs, OB = C::kOBufs, VB = C::kVBlocks, NP = C::kPieces, KB = C::kKBlocks;
     constexpr int kPeers = PAIR ? 2 : 1;  // CTAs that work on one item
@@ -461,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         }
     } else if (warp == 2 && lane == 0) {
         s.abort = 0;
-        s.odd_nodes = 0;
+        s.odd_nodes[0] = s.odd_nodes[1] = 0;
         for (int i = 0; i < NK; i++) mbar_init(&s.k_full[i], 1), mbar_init(&s.k_empty[i], 1);
         for (int i = 0; i < NV; i++) mbar_init(&s.v_full[i], 1), mbar_init(&s.v_empty[i], 1);
         for (int i = 0; i < 2; i++) {
@@ -818,7 +823,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         constexpr int H = D / 2, V = D / 32;
         const int w = warp - 8, row = (warp & 3) * 32 + lane, col0 = (w >> 2) * H, span = MR / copies;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
-        uint32_t piece0 = 0, tile = 0, msg = 0, cleans = 0;
+        uint32_t piece0 = 0, tile = 0, msg = 0, cleans = 0, items = 0;
         // Every round prepares Q of one item and works through one: the same, or with two places for Q the one before.
         Item nx;
         size_t where_nx = 0, where = 0;
@@ -953,7 +958,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                                 *p = v;
                             }
                         }
-                        if (odd) mark_odd<PAIR>(&s.odd_nodes, odd);
+                        if (odd) mark_odd<PAIR>(&s.odd_nodes[PAIR ? items & 1 : 0], odd);
                         fence_proxy_async();
                         __syncwarp();
                         if (lane == 0) arrive_leader<PAIR>(&s.clean[cleans & 1]);
@@ -995,7 +1000,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 for (int i = 0; i < H / 4; i++)
                     *reinterpret_cast<float4 *>(mine + (((col0 / 4 + i) ^ (row & 7)) << 4)) =
                         make_float4(acc[2 * i].x * mul, acc[2 * i].y * mul, acc[2 * i + 1].x * mul, acc[2 * i + 1].y * mul);
-                uint64_t odd = row % span < rows ? *(volatile uint64_t *)&s.odd_nodes : 0;
+                uint64_t odd = row % span < rows ? *(volatile uint64_t *)&s.odd_nodes[PAIR ? items & 1 : 0] : 0;
                 if (odd) {  // rare: values that are not finite, for the rows that see them
                     const int node = (row0 + row % span) / a.group;
                     odd &= a.tree ? a.tree[(size_t)it.seq * a.tokens + node] : ~0ull >> (63 - node);
@@ -1017,7 +1022,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             bad = group_any(3, 256, bad);
             ok = !group_any(4, 256, !ok);  // the eight warps stop together
             if (!ok) break;
-            if (tid == 256) s.odd_nodes = 0;
+            if (tid == 256) s.odd_nodes[PAIR ? items & 1 : 0] = 0;
             const size_t part = (size_t)(2 * team + (it.start > s.slot0)) * a.part_rows + rank * kRows;
             const float nan = __int_as_float(0x7fc00000);
             if (copies == 1) {
@@ -1070,7 +1075,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             }
             __syncwarp();
             if (lane == 0) arrive(&s.msg_empty[slot]);
-            msg++;
+            msg++, items++;
             piece0 += value_pieces<C>(a, it);
             group_sync(4, 256);  // Q's place is free again
             if (QB == 2) it = nx, where = where_nx, left = more;

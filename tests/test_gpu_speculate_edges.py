@@ -162,3 +162,28 @@ def test_attention_of_scores_far_beyond_a_unit(L, hq, hkv, d, tokens, size, sign
     assert np.isfinite(got).all()
     # all other weights are below 2^-1000 of the largest; P is 2^15 and V an F16
     np.testing.assert_array_equal(got, want.astype(np.float32))
+
+
+# ---- values that are not finite --------------------------------------------
+
+
+@pytest.mark.parametrize("hq,hkv,tokens", [(24, 2, 17), (16, 2, 33), (24, 2, 5)])
+def test_attention_values_of_nodes_that_are_not_finite_in_every_sequence(L, hq, hkv, tokens):  # noqa: F811
+    """Many short sequences to a CTA, or to a pair of CTAs of which one may be an item ahead: each finds its own nodes."""
+    rng = np.random.default_rng(hq + tokens)
+    lengths = [int(n) for n in rng.integers(0, 200, 150)]
+    cache = Cache(L, rng, lengths, tokens, hkv, 256, 16)
+    q = rng.normal(size=(len(lengths), tokens, hq, 256)).astype(np.float32)
+    masks = [S.tree_masks([-1] + [int(rng.integers(0, i)) for i in range(1, tokens)]) for _ in lengths]
+    clean = expected(cache, q, masks, 0.1)
+    odd = np.zeros(clean.shape, bool)
+    for s, n in enumerate(lengths):
+        node, col = int(rng.integers(1, tokens)), int(rng.integers(256))
+        cache.v[0, cache.rows(s, n + node, 1), s % hkv, col] = np.nan
+        sees = [t for t in range(tokens) if masks[s][t] >> node & 1]
+        odd[s, sees, s % hkv * (hq // hkv) : (s % hkv + 1) * (hq // hkv), col] = True
+    cache.upload()
+    got = attend(L, cache, q, masks, 0.1, calls=3)
+    assert np.isnan(got[odd]).all()
+    assert np.isfinite(got[~odd]).all()
+    np.testing.assert_allclose(got[~odd], clean[~odd], rtol=0, atol=1e-4 * np.abs(clean).max())
