@@ -1008,7 +1008,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                         const int nd = __ffsll((long long)odd) - 1;
                         odd &= odd - 1;
                         const long long at = a.c.row(it.seq, it.length + nd);
-                        if (at < 0) continue;
+                        // (only in the copy of Q that has the key: another may see nothing, and its sums be left out by a 0)
+                        if (at < 0 || (it.length + nd) % kKeys * copies / kKeys != row / span) continue;
                         const __half *v = a.c.v + ((size_t)at * a.c.kv_heads + it.kv) * D + col0;
 #pragma unroll 1
                         for (int i = 0; i < H; i++) {

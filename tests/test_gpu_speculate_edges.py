@@ -187,3 +187,21 @@ def test_attention_values_of_nodes_that_are_not_finite_in_every_sequence(L, hq, 
     assert np.isnan(got[odd]).all()
     assert np.isfinite(got[~odd]).all()
     np.testing.assert_allclose(got[~odd], clean[~odd], rtol=0, atol=1e-4 * np.abs(clean).max())
+
+
+@pytest.mark.parametrize("hq,hkv,d,tokens", [(4, 1, 64, 3), (16, 4, 64, 10), (8, 2, 128, 4), (4, 4, 128, 1), (24, 2, 256, 5), (24, 2, 256, 17)])
+@pytest.mark.parametrize("value", [np.inf, -np.inf])
+def test_attention_of_infinite_values_of_nodes(L, hq, hkv, d, tokens, value):  # noqa: F811
+    """An infinity in a node's value is what the rows that see it have in its column, whatever the other keys are."""
+    rng = np.random.default_rng(d + tokens)
+    lengths = [0, 20, 77, 100, 126]
+    cache = Cache(L, rng, lengths, tokens, hkv, d, 16)
+    q = rng.normal(size=(len(lengths), tokens, hq, d)).astype(np.float32)
+    for s, n in enumerate(lengths):
+        cache.v[0, cache.rows(s, n + tokens // 2, 1), :, 5] = value
+    cache.upload()
+    got, want = attend(L, cache, q, None, 0.1), expected(cache, q, None, 0.1)
+    odd = ~np.isfinite(want)
+    assert odd.any()
+    np.testing.assert_array_equal(got[odd], want[odd])
+    np.testing.assert_allclose(got[~odd], want[~odd], rtol=0, atol=1e-4 * np.abs(want[~odd]).max())
