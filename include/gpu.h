@@ -243,7 +243,8 @@ int qg_moe_profile_read(int phase, double *total_ms, int *launches);
  * p / page_tokens]. lengths[s] positions are committed; a step's nodes take
  * the positions after them, so the caller's table covers lengths[s] + tokens
  * positions. Entries of page_table past those are never read. page_tokens:
- * 16, 32, 64, 128 or 256. head_dim: 64, 128 or 256.
+ * 16, 32, 64, 128 or 256. head_dim: 64, 128 or 256. pages*page_tokens is at
+ * most 2^31 - 1, table_pages*page_tokens at most 2^31 - 128.
  *
  * A sequence whose length is negative or leaves no room for its nodes, or
  * whose table names a page outside the pool, gets NaN rows and no store;

@@ -54,8 +54,8 @@ inline int cache_view(const qg_kv_cache *c, int layer, int seqs, int tokens, Cac
     int shift = 4;
     while (shift <= 8 && (1 << shift) != c->page_tokens) shift++;
     if (shift > 8) return cudaErrorInvalidValue;
-    // positions and pool rows are 32-bit coordinates
-    if (((long long)c->pages << shift) > 0x7fffffffll || ((long long)c->table_pages << shift) > 0x7fffffffll)
+    // pool rows are 32-bit coordinates, and so is the end of the 128 keys that a sequence's last position lies in
+    if (((long long)c->pages << shift) > 0x7fffffffll || ((long long)c->table_pages << shift) > 0x7fffff80ll)
         return cudaErrorInvalidValue;
     const size_t pool = ((size_t)c->pages << shift) * c->kv_heads * c->head_dim * sizeof(__half);
     if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15) return cudaErrorInvalidValue;
