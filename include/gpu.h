@@ -284,7 +284,8 @@ int qg_qk_norm_rope(float *q_out, const qg_kv_cache *cache, int layer, const flo
  * of tree[row] is node j (its own bit is not implied). tree NULL: a chain,
  * node i sees nodes 0..i. A row that sees nothing is zero. What a row does not
  * see has no effect on it, whatever its bits (NaN and infinities included).
- * q and out: [row][q_heads][head_dim] F32, 16-byte aligned. The workspace is
+ * q and out: [row][q_heads][head_dim] F32, 16-byte aligned. scale: finite, and
+ * so is scale*log2(e). The workspace is
  * zero-filled once; calls sharing it must not overlap on the device. Waits in
  * the kernel are bounded: should one run out, every row is NaN, in this call
  * and later ones, until the workspace is zero-filled again.

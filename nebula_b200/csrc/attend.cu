@@ -1463,6 +1463,7 @@ extern "C" int qg_tree_attention(float *out, const float *q, const qg_kv_cache *
     a.tree = tree;
     a.sign = scale < 0 ? -1.0f : 1.0f;
     a.scale = (scale < 0 ? -scale : scale) * 1.4426950408889634f;
+    if (!(a.scale < INFINITY)) return cudaErrorInvalidValue;
     a.seqs = seqs;
     a.tokens = tokens;
     a.q_heads = q_heads;

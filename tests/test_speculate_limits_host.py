@@ -14,3 +14,9 @@ def test_positions_end_before_a_units_end_passes_31_bits(page, table_pages):
     assert attention(cache(**c)) == INVALID
     assert prep(cache(**c)) == INVALID
     assert commit(cache(**c)) == INVALID
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf"), 3e38, -3e38])
+def test_attention_refuses_a_scale_that_is_not_finite(scale):
+    """Also one that is not finite any more in units of powers of two (times log2(e))."""
+    assert attention(cache(), scale=scale) == INVALID
