@@ -91,7 +91,7 @@ def verify(logits, draft, parents, probs, uniforms, temperature):
                 p[draft[c]] = 0.0
             else:
                 left = np.maximum(p - np.asarray(probs[c], np.float64), 0.0)
-                p = left if left.sum() > 0 else p
+                p = left / left.sum() if left.sum() > 0 else p
         if chosen is None:
             break
         at = chosen
