@@ -1,8 +1,11 @@
 """The verify step's operators on a B200 where their arithmetic runs out of room. Against the 64-bit definitions
 (oracle/speculate.py)."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
+from conftest import assert_parity
 from oracle import speculate as S
 from test_gpu_speculate import L, Cache, attend, expected  # noqa: F401  (L is a fixture)
 
@@ -205,3 +208,30 @@ def test_attention_of_infinite_values_of_nodes(L, hq, hkv, d, tokens, value):  #
     assert odd.any()
     np.testing.assert_array_equal(got[odd], want[odd])
     np.testing.assert_allclose(got[~odd], want[~odd], rtol=0, atol=1e-4 * np.abs(want[~odd]).max())
+
+
+# ---- after a wait that ran out ---------------------------------------------
+
+
+@pytest.mark.parametrize("hq,hkv,d,tokens", [(8, 8, 128, 1), (16, 4, 64, 5), (32, 8, 128, 17), (24, 2, 256, 1), (24, 2, 256, 17)])
+def test_attention_after_an_error_every_row_is_nan_until_the_workspace_is_cleared(L, hq, hkv, d, tokens):  # noqa: F811
+    """The error word (the workspace's first) is written from the host, as a wait that ran out would leave it."""
+    rng = np.random.default_rng(d + tokens)
+    lengths = [20, 700]
+    cache = Cache(L, rng, lengths, tokens, hkv, d, 32)
+    q = rng.normal(size=(2, tokens, hq, d)).astype(np.float32)
+    dq, out = L.Device(q), L.Device(np.zeros(q.shape, np.float32))
+    ws = L.attention_workspace(2, tokens, hq, hkv, d)
+
+    def call():
+        L.call("tree_attention", out.p, dq.p, C.byref(cache.c), 0, None, 0.1, 2, tokens, hq, ws.p)
+        return out.get()
+
+    want = expected(cache, q, None, 0.1)
+    assert_parity(call(), want)
+    word = np.array([4], np.int32)
+    L.call("write", ws.p, word.ctypes.data, 4)
+    for _ in range(2):
+        assert np.isnan(call()).all()
+    L.call("zero", ws.p, ws.nbytes)
+    assert_parity(call(), want)
