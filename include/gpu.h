@@ -246,9 +246,12 @@ int qg_moe_profile_read(int phase, double *total_ms, int *launches);
  * 16, 32, 64, 128 or 256. head_dim: 64, 128 or 256. pages*page_tokens is at
  * most 2^31 - 1, table_pages*page_tokens at most 2^31 - 128.
  *
- * A sequence whose length is negative or leaves no room for its nodes, or
- * whose table names a page outside the pool, gets NaN rows and no store;
- * other sequences are not affected. */
+ * A sequence whose length is negative or leaves no room for its nodes gets NaN
+ * rows and no store. Where its table names a page outside the pool,
+ * qg_tree_attention gives all its rows NaN, qg_qk_norm_rope the rows whose own
+ * position is on that page (they are not stored; its other rows are), and
+ * qg_cache_commit leaves it as it is when a row would move from or to that page.
+ * Other sequences are not affected. */
 typedef struct {
     void *k, *v;
     const int *page_table;  /* device [seqs][table_pages] */
@@ -284,11 +287,14 @@ int qg_qk_norm_rope(float *q_out, const qg_kv_cache *cache, int layer, const flo
  * of tree[row] is node j (its own bit is not implied). tree NULL: a chain,
  * node i sees nodes 0..i. A row that sees nothing is zero. What a row does not
  * see has no effect on it, whatever its bits (NaN and infinities included).
+ * What it sees and is not finite: a value makes its column NaN or infinite (of a
+ * committed position NaN where the sum is an infinity), a key the row NaN
+ * (where its score is -infinity, the row may also be what the others give).
  * q and out: [row][q_heads][head_dim] F32, 16-byte aligned. scale: finite, and
- * so is scale*log2(e). The workspace is
- * zero-filled once; calls sharing it must not overlap on the device. Waits in
- * the kernel are bounded: should one run out, every row is NaN, in this call
- * and later ones, until the workspace is zero-filled again.
+ * so is scale*log2(e). The workspace is zero-filled once; calls sharing it must
+ * not overlap on the device. Waits in the kernel are bounded: should one run
+ * out, every row is NaN, in this call and later ones, until the workspace is
+ * zero-filled again.
  * Deterministic, graph-capturable, no host synchronisation. */
 int qg_attention_workspace_bytes(int seqs, int tokens, int q_heads, int kv_heads, int head_dim, size_t *bytes);
 int qg_tree_attention(float *out, const float *q, const qg_kv_cache *cache, int layer, const uint64_t *tree, float scale,
@@ -304,9 +310,12 @@ int qg_tree_attention(float *out, const float *q, const qg_kv_cache *cache, int 
  *  - draft_probs NULL (drafts taken as they are): child c is accepted when
  *    uniforms[c] * (p's mass left) < p(draft[c]), otherwise draft[c] leaves p;
  *  - draft_probs [row][vocab], the distribution each draft was drawn from
- *    (chains: a node with two children is refused): accepted when
+ *    (chains): accepted when
  *    uniforms[c] * draft_probs[c](draft[c]) < p(draft[c]), otherwise p becomes
- *    max(p - draft_probs[c], 0) (p itself where that is zero everywhere).
+ *    max(p - draft_probs[c], 0) (p itself where that is zero everywhere). A
+ *    second child is never tried: after an accepted first one it does not
+ *    matter, after a refused first one the sequence is refused like one with a
+ *    malformed tree.
  * When no child is accepted, next[seq] is drawn from what is left of p with
  * uniforms[root]: the first token at which p's running sum exceeds
  * uniforms[root] * its total. So the tokens follow the target's distribution.
@@ -316,7 +325,9 @@ int qg_tree_attention(float *out, const float *q, const qg_kv_cache *cache, int 
  * the vocabulary on its way gets accepted, next and path -1.
  * Sums over the vocabulary are held in 64 bits: the tokens do not depend on
  * how the work is split. Tokens below 2^-900 of a row's largest probability
- * count as having none. vocab at most 2^24. The workspace is zero-filled once. */
+ * count as having none. logit*log2(e)/temperature is held in 32 bits, and what
+ * passes their range counts as its end. vocab at most 2^24. The workspace is
+ * zero-filled once. */
 int qg_verify_workspace_bytes(int seqs, int tokens, int vocab, size_t *bytes);
 int qg_verify_tree(int *path, int *accepted, int *next, const float *logits, const int *draft, const int *parents,
                    const float *draft_probs, const float *uniforms, double temperature, int seqs, int tokens, int vocab,
