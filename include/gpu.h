@@ -325,7 +325,7 @@ int qg_tree_attention(float *out, const float *q, const qg_kv_cache *cache, int 
  * the vocabulary on its way gets accepted, next and path -1.
  * Sums over the vocabulary are held in 64 bits: the tokens do not depend on
  * how the work is split. Tokens below 2^-900 of a row's largest probability
- * count as having none. logit*log2(e)/temperature is held in 32 bits, and what
+ * may count as having none. logit*log2(e)/temperature is held in 32 bits, and what
  * passes their range counts as its end. vocab at most 2^24. The workspace is
  * zero-filled once. */
 int qg_verify_workspace_bytes(int seqs, int tokens, int vocab, size_t *bytes);

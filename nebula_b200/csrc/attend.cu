@@ -39,7 +39,7 @@ namespace {
 
 constexpr int kRows = 128;       // rows per tile (MMA M)
 constexpr int kKeys = 128;       // keys per unit (MMA N of S: with 64 the re-reads of Q bound the shared memory)
-constexpr int kMaxCtas = 148;    // SMs of a B200: one CTA each
+constexpr int kMaxCtas = kSms;   // one CTA each
 constexpr int kThreads = 512;
 constexpr int kNotes = 3 * 1024;  // bytes for the roles' shared bookkeeping
 // Registers per thread after the split; the four warpgroups' sum is what the

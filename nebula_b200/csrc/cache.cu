@@ -298,7 +298,7 @@ extern "C" int qg_cache_commit(const qg_kv_cache *cache, int *lengths_out, const
     a.accepted = accepted;
     // A chained launch hides what the kernel before leaves of the launch (one sequence 3.6 us in place of 4.4 to 5.1); with
     // more clusters than the GPU takes at once it only adds (48 sequences 32.6 us in place of 31.4).
-    if (seqs * kCommitCtas <= 148) return launch_chained(cache_commit_kernel, dim3(seqs * kCommitCtas), 256, a);
+    if (seqs * kCommitCtas <= kSms) return launch_chained(cache_commit_kernel, dim3(seqs * kCommitCtas), 256, a);
     cache_commit_kernel<<<seqs * kCommitCtas, 256, 0, launch_stream>>>(a);
     NB_CHECK_LAUNCH();
 }

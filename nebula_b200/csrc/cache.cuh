@@ -6,6 +6,7 @@ namespace nb {
 
 constexpr int kMaxSeqs = 1024;
 constexpr int kMaxNodes = 64;  // one 64-bit mask per node
+constexpr int kSms = 148;      // of a B200; no kernel needs its CTAs to run at the same time beyond a cluster
 
 struct CacheView {
     __half *k, *v;  // one layer's pools
