@@ -72,7 +72,8 @@ constexpr int kChunk = 32;       // keys per step of the softmax
 // MMAs that span both (cta_group::2): each has its 128 rows of Q, S, P and O, and half of the keys' rows and of the
 // values' columns, which the tensor cores of both read. The rings hold twice the keys, and L2 delivers each key once for
 // 256 rows: heads of 256 need 128 KB for 128 rows of Q, and the 96 KB left are too few for keys and values of one CTA
-// (98k keys x 204 rows: 86.5 us, with two row tiles apart 92.5).
+// (98k keys x 204 rows in a sustained loop, power-capped at 1.59 GHz: 102 us, with two row tiles apart 109.5; at the first
+// calls' 1.97 GHz 88 and 95).
 template <int D, int MR, bool PAIR>
 struct Cfg {
     static constexpr int kChunks = D / 64;                  // 128-byte wide column blocks
@@ -91,8 +92,9 @@ struct Cfg {
     static constexpr int kOBufs = D == 256 ? 1 : 2;
     static constexpr int kS = 256;  // tensor memory columns: O (twice where it fits), then two of S (P takes its place)
     // A warp that issued MMAs stalls at its next wait until they have read their operands, and the tensor cores run dry:
-    // so where the rings have room the issuers wait for two pieces at once (16 single tokens of heads of 128 87.0 -> 84.5
-    // us, 5 x 5 tokens 22.6 -> 20.8; one CTA with heads of 256 has not: 98k keys 92.8 -> 99.2 us). P comes in kParts
+    // so where the rings have room the issuers wait for two pieces at once (16 x 2 tokens, up to 8191 keys of heads of 128:
+    // 85.2 -> 83.6 us at full clock, no difference under the power cap; heads of 256 have no room: 98k keys 102 -> 105 us,
+    // 4097 keys 23.8 -> 24.4). P comes in kParts
     // parts of a unit.
     static constexpr int kGroup = D == 128 ? 2 : 1, kParts = kPieces / kGroup, kPartKeys = kKeys / kParts;
     static constexpr int kTileRows = PAIR ? 2 * kRows : kRows;
@@ -289,8 +291,8 @@ __device__ __forceinline__ int units_of(const AttendArgs &a, int length) {
     return length < 0 ? 0 : (length + a.tokens + kKeys - 1) / kKeys;
 }
 // What an item costs besides its units, in units: Q, the first unit's latency and the store (about 2 us). The ranges
-// divide the sum of both; an item's first kItemCost slots stand for it and hold no unit. (16 sequences of 512 to 8191
-// keys: CTAs with eight short items took 81 us and those with one 65 when only units counted.)
+// divide the sum of both; an item's first kItemCost slots stand for it and hold no unit. (When only units counted: 16 x 2
+// tokens, 512 to 8191 keys of heads of 128 92.1 -> 97.3 us, 5 x 5 tokens of heads of 64 18.5 -> 19.5.)
 template <int D>
 constexpr int kItemCost = D == 256 ? 1 : 2;
 template <int D>
@@ -1099,7 +1101,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
 // before an item's end. Lane l holds 8 values of a key, D/8 lanes a key. The 8 x 4 partial products of a lane are added up
 // over the lanes in a butterfly that leaves one score to a lane; softmax runs per warp, and an item's 16 maxima, totals and
 // sums become one at its end. The division of the work and the join are the other kernel's. Bound by HBM (16 single tokens
-// of 32 heads, 8 key heads of 128, 285 MB: 63.7 us, on the tensor cores 87).
+// of 32 heads, 8 key heads of 128, 285 MB: 62 us, on the tensor cores 88).
 constexpr int kFewWarps = 16, kFewRows = 4;
 template <int D>
 struct Few {
@@ -1484,8 +1486,8 @@ extern "C" int qg_tree_attention(float *out, const float *q, const qg_kv_cache *
     a.err = static_cast<int *>(workspace);
     a.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + 256);
     a.part_acc = reinterpret_cast<float *>(static_cast<char *>(workspace) + 256 + ml_bytes(part_rows(tokens, a.group)));
-    // One token, at most four heads to a key head of up to 128 values: no tensor cores (16 tokens, 32/8 heads of 128: 63.7 us
-    // against 87). Heads of 256 leave no room for copies ahead.
+    // One token, at most four heads to a key head of up to 128 values: no tensor cores (16 tokens, 32/8 heads of 128: 62 us
+    // against 88). Heads of 256 leave no room for copies ahead.
     if (rows <= kFewRows && tokens == 1 && a.c.head_dim <= 128) return a.c.head_dim == 64 ? launch_token<64>(a) : launch_token<128>(a);
     CUtensorMap k_map, v_map;
     if (int rc = pool_map(&k_map, a.c, a.c.k, a.k_box, a.k_blocks)) return rc;

@@ -46,11 +46,12 @@ __device__ __forceinline__ void load(float (&x)[W], const float *p) {
 // the table's angles, each of which depends on the one before, arrive meanwhile
 // and serve both heads (96 x 17 rows of 24 + 4 heads of 256: 22.6 us; one head to a warp 24.6, four 26.7; with the chained
 // launch 20.6). The partner of a rotated value sits in another lane, so the rotated part of the normalised head goes through
-// the warp's part of shared memory. Bound by HBM (by the launch for one verify batch).
+// the warp's part of shared memory. For many rows bound by the latency of its loads: 64 registers leave 37 % of the warps, which
+// wait for memory most of the time (issue slots 48 %, HBM 30 %); for one verify batch by the launch.
 constexpr int kHeads = 2;
 
 // WIDE: all rows of q, k, v, q_out and the weights start on 16-byte boundaries, and the rotated halves and the table's
-// rows are whole loads of a lane. The instructions count next to the bytes (two thirds of the issue slots).
+// rows are whole loads of a lane (before, the instructions took two thirds of the issue slots).
 template <int D, bool WIDE>
 __global__ void __launch_bounds__(256, 4) qk_norm_rope_kernel(const __grid_constant__ PrepArgs a) {
     constexpr int W = D == 64 ? 2 : 4, N = D / (32 * W);

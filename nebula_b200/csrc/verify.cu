@@ -5,7 +5,8 @@
 // on M, and the power of two is exact, so sums over parts of a row, each
 // relative to its own M, come to a common M without rounding, and one pass over
 // the logits is enough. Sums are held in 64 bits: a token is a whole number
-// that must not depend on their order.
+// that must not depend on their order. So are the weights of drafts and of the
+// chunk that the next token is drawn from, down to 2^-1000 of the largest.
 //
 // Two kernels, the second chained to the first (programmatic launch):
 //  - chunk_kernel reads all logits once, 4096 to a CTA, and leaves each chunk's
