@@ -268,7 +268,7 @@ __device__ __forceinline__ int claim(double part, double upto, double aim) {
 }
 
 // What refused drafts leave of a row's or a chunk's mass is taken as a difference of 64-bit sums, which are off by some
-// 2^-50. Where it comes out below this share of the sum, walk_anew adds up what is there.
+// 2^-50. Where it comes out below this share of the sum and matters, walk_anew adds up what is there.
 constexpr double kSure = 0x1p-20;
 
 // The thread's eight weights of chunk c, without those of the nodes `gone`.
@@ -611,7 +611,10 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const __grid_constan
         return all;
     };
     double *rest = a.rest + (size_t)seq * a.chunks;
-    bool close = false;  // a chunk of refused drafts has next to nothing left
+    // ---- the chunk that holds the aim: every warp finds it for itself, a lane takes neighbouring chunks
+    const int per = (a.chunks + 31) / 32, c0 = min(lane * per, a.chunks), c1 = min(c0 + per, a.chunks);
+    constexpr int kKept = 4;  // a lane's first chunks, whose sums stay in registers
+    unsigned close = 0;       // those of which refused drafts leave next to nothing, as bits (the others: bit kKept)
     auto chunk_sum = [&](int c) -> double {
         if constexpr (DRAWN) {
             return __ldcg(rest + c);
@@ -624,13 +627,10 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const __grid_constan
                 const int g = __ffsll(m) - 1;
                 if ((draft[g] + lead) / kChunk == c) w -= held[g];
             }
-            close |= w < kSure * all;
-            return w;
+            close |= (unsigned)(w < kSure * all) << min(c - c0, kKept);
+            return fmax(w, 0.0);
         }
     };
-    // ---- the chunk that holds the aim: every warp finds it for itself, a lane takes neighbouring chunks
-    const int per = (a.chunks + 31) / 32, c0 = min(lane * per, a.chunks), c1 = min(c0 + per, a.chunks);
-    constexpr int kKept = 4;  // a lane's first chunks, whose sums stay in registers
     double whole = 0.0, upto = 0.0, sum = 0.0, kept[kKept];
     bool fine = !DRAWN;
     for (;;) {
@@ -674,7 +674,6 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const __grid_constan
         upto = warp_scan(sum);
         whole = __shfl_sync(0xffffffffu, upto, 31);
         if constexpr (!DRAWN) {
-            if (__any_sync(0xffffffffu, close)) return walk_anew(a, seq, rows, kids, draft, held, path, sums);  // all warps say the same
             break;
         } else {
             if (!fine && !greedy && (double)first_uniform * whole < kCoarse) fine = true;  // the weights left out matter
@@ -686,6 +685,11 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const __grid_constan
     if (rank) return;
     const double aim = (double)first_uniform * whole;
     const int owner = claim(sum, upto, aim);
+    // Chunks with next to nothing left do not count beside the others, unless the aim is as small (or one is chosen, below).
+    // All warps say the same.
+    if constexpr (!DRAWN) {
+        if (aim < kSure * r.sum && __any_sync(0xffffffffu, close)) return walk_anew(a, seq, rows, kids, draft, held, path, sums);
+    }
     if (owner < 0) {  // not met: a row with a distribution has weight left, for what was refused was not all of it
         if (tid == 0) a.next[seq] = -1;
         return;
@@ -703,6 +707,10 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const __grid_constan
 #pragma unroll
         for (int k = 0; k < kKept; k++) look(c0 + k, kept[k]);
         for (int k = c0 + kKept; k < c1 && !past; k++) look(k, chunk_sum(k));
+    }
+    if constexpr (!DRAWN) {
+        if (__any_sync(0xffffffffu, lane == owner && close >> min(c - c0, kKept) & 1))
+            return walk_anew(a, seq, rows, kids, draft, held, path, sums);
     }
     c = __shfl_sync(0xffffffffu, c, owner);
     before = __shfl_sync(0xffffffffu, before, owner);
