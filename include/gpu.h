@@ -340,6 +340,70 @@ int qg_verify_tree(int *path, int *accepted, int *next, const float *logits, con
  * ascending) keeps its length and its rows. */
 int qg_cache_commit(const qg_kv_cache *cache, int *lengths_out, const int *path, const int *accepted, int seqs, int tokens);
 
+/* ---- a batch of users on one paged cache (no counterpart in the reference, which
+ * serves one) */
+
+/* The next token of each row of logits [row][vocab], drawn with the given random
+ * number uniforms[row] in [0, 1) from what the user's settings leave of
+ * p = softmax(logits/temperature). User row/per's settings are temperature[],
+ * top_k[], top_p[] and min_p[] (device; each may be NULL: 1, 0, 1 and 0). In the
+ * order of the logits, the lowest index of equals first:
+ *  - the first top_k tokens are kept (0 or less: all),
+ *  - of these, as many as it takes until their probabilities' sum is at least
+ *    top_p of the sum of all these (1 or more: all),
+ *  - of these, those with at least min_p of the largest's probability;
+ * the first token is always kept, tokens at -infinity never.
+ * token[row] is the first index at which the running sum of what is kept exceeds
+ * uniforms[row] * its total (a uniform below 0 counts as 0, one of 1 or more as
+ * the largest below 1). Temperature 0: the largest logit, the lowest index of
+ * equals. A row with a NaN or +infinite logit or no finite one, a temperature
+ * that is negative or not finite, or a NaN among its settings or its uniform
+ * gets token -1.
+ * Probabilities are taken relative to the largest, as whole multiples of 2^-44
+ * of it, and their sums are exact: equal inputs give equal tokens. vocab at most
+ * 393213, rows at most 2^20, logits 4-byte aligned. */
+int qg_sample(int *token, const float *logits, const float *uniforms, const float *temperature, const int *top_k, const float *top_p,
+              const float *min_p, int per, int rows, int vocab);
+/* The same logits with -infinity in place of what is not kept, so that
+ * qg_verify_tree (with the same temperature) accepts and draws from what the
+ * user's settings leave: per is then the nodes of a sequence. Temperature 0 keeps one
+ * token. A row that qg_sample would refuse for its logits or settings is NaN
+ * throughout. out may be logits, and overlaps them in no other way. */
+int qg_truncate_logits(float *out, const float *logits, const float *temperature, const int *top_k, const float *top_p,
+                       const float *min_p, int per, int rows, int vocab);
+
+/* The pages of a paged cache for sequences that come, grow and go, without the
+ * host. A stack of free pages: free_pages[0 .. *free_count), the last one on
+ * top; held[s] entries of sequence s's row of the page table are its pages. Shared pages
+ * are entries that the host writes into several rows (and counts in their
+ * held). A call uses seqs rows of the table; calls on one pool must not overlap on the device. */
+typedef struct {
+    int *page_table;  /* device [seqs][table_pages]: the cache's */
+    int *held;        /* device [seqs] */
+    int *free_pages;  /* device [pages] */
+    int *free_count;  /* device */
+    int pages, page_tokens, table_pages;
+} qg_page_pool;
+
+/* Room for counts[s] (0..tokens; NULL: tokens) new positions after lengths[s] of each
+ * sequence. In the order of the sequences, the pages that lengths[s] + counts[s]
+ * positions need beyond held[s] come off the stack and are appended to the row;
+ * a sequence for which there are not enough, and all later ones that need any,
+ * get none. taken[s]: pages taken, -2: none for want of pages, -1: refused (a
+ * negative length, a count outside 0..tokens, positions past the table, held
+ * outside 0..table_pages). slots [seq][tokens] (may be NULL): the pool row of
+ * each new position, -1 behind counts[s], for sequences that were refused
+ * or got none, and where the row names a page outside the pool. A *free_count
+ * outside 0..pages counts as 0. */
+int qg_pages_reserve(const qg_page_pool *pool, int *slots, int *taken, const int *lengths, const int *counts, int seqs, int tokens);
+/* Gives back what sequence s's first lengths[s] positions do not need (a negative
+ * length: all), its first shared_pages entries excepted: the pages of the first
+ * sequence end on top of the stack, each sequence's first one uppermost, so that reserving
+ * again hands them out as before. freed[s]: pages given back, -1: refused (held outside
+ * 0..table_pages; and every sequence with pages to give back where the stack would
+ * hold more than the pool, or *free_count is negative: then nothing changes). */
+int qg_pages_release(const qg_page_pool *pool, int *freed, const int *lengths, int shared_pages, int seqs);
+
 /* ---- loading an all-resident model (no counterpart in the reference
  * header; the reference's loader is qwen/qwen.c:108-146,324-369) -------- */
 

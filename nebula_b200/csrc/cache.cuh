@@ -44,6 +44,17 @@ inline int launch_chained(void (*kernel)(Args), dim3 grid, int threads, const Ar
     return cudaLaunchKernelEx(&cfg, kernel, args);
 }
 
+// log2 of a page's tokens: 16, 32, 64, 128 or 256; -1 for others.
+inline int page_shift(int page_tokens) {
+    for (int shift = 4; shift <= 8; shift++)
+        if (1 << shift == page_tokens) return shift;
+    return -1;
+}
+// Pool rows are 32-bit coordinates, and so is the end of the 128 keys that a sequence's last position lies in.
+inline bool pool_too_large(int pages, int table_pages, int shift) {
+    return ((long long)pages << shift) > 0x7fffffffll || ((long long)table_pages << shift) > 0x7fffff80ll;
+}
+
 // Checks what the header asks of a cache and a batch; cudaErrorInvalidValue before any launch.
 inline int cache_view(const qg_kv_cache *c, int layer, int seqs, int tokens, CacheView &view) {
     if (!c || !c->k || !c->v || !c->page_table || !c->lengths || seqs < 1 || seqs > kMaxSeqs || tokens < 1 ||
@@ -52,12 +63,8 @@ inline int cache_view(const qg_kv_cache *c, int layer, int seqs, int tokens, Cac
     if (c->layers < 1 || layer < 0 || layer >= c->layers || c->pages < 1 || c->table_pages < 1 || c->kv_heads < 1 ||
         c->kv_heads > 1024 || (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256))
         return cudaErrorInvalidValue;
-    int shift = 4;
-    while (shift <= 8 && (1 << shift) != c->page_tokens) shift++;
-    if (shift > 8) return cudaErrorInvalidValue;
-    // pool rows are 32-bit coordinates, and so is the end of the 128 keys that a sequence's last position lies in
-    if (((long long)c->pages << shift) > 0x7fffffffll || ((long long)c->table_pages << shift) > 0x7fffff80ll)
-        return cudaErrorInvalidValue;
+    const int shift = page_shift(c->page_tokens);
+    if (shift < 0 || pool_too_large(c->pages, c->table_pages, shift)) return cudaErrorInvalidValue;
     const size_t pool = ((size_t)c->pages << shift) * c->kv_heads * c->head_dim * sizeof(__half);
     if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15) return cudaErrorInvalidValue;
     if (c->layers > 1 && (c->layer_bytes < pool || c->layer_bytes % 16)) return cudaErrorInvalidValue;

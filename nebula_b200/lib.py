@@ -52,6 +52,8 @@ SIGNATURES = {
     "verify_workspace_bytes": ([I, I, I, C.POINTER(Z)], I),
     "verify_tree": ([P, P, P, P, P, P, P, P, D, I, I, I, P], I),
     "cache_commit": ([P, P, P, P, I, I], I),
+    "sample": ([P, P, P, P, P, P, P, I, I, I], I), "truncate_logits": ([P, P, P, P, P, P, I, I, I], I),
+    "pages_reserve": ([P, P, P, P, P, I, I], I), "pages_release": ([P, P, P, I, I], I),
     "synth_weights": ([P, I, I, I, U64, F], I), "synth_normal": ([P, Z, U64, F], I),
     "index_open": ([C.c_char_p, C.POINTER(P), C.c_char_p, Z], I), "index_close": ([P], None),
     "index_tensor": ([P, C.c_char_p, C.POINTER(P), C.POINTER(I), C.POINTER(U64), C.POINTER(U64)], I),
@@ -67,6 +69,13 @@ class KvCache(C.Structure):
 
     _fields_ = [("k", P), ("v", P), ("page_table", P), ("lengths", P), ("layer_bytes", Z), ("layers", I), ("pages", I),
                 ("page_tokens", I), ("table_pages", I), ("kv_heads", I), ("head_dim", I)]
+
+
+class PagePool(C.Structure):
+    """qg_page_pool: the page tables of a paged cache and its stack of free pages (pass C.byref of it)."""
+
+    _fields_ = [("page_table", P), ("held", P), ("free_pages", P), ("free_count", P), ("pages", I), ("page_tokens", I),
+                ("table_pages", I)]
 
 
 _LIB = None
