@@ -341,7 +341,24 @@ int qg_verify_tree(int *path, int *accepted, int *next, const float *logits, con
 int qg_cache_commit(const qg_kv_cache *cache, int *lengths_out, const int *path, const int *accepted, int seqs, int tokens);
 
 /* ---- a batch of users on one paged cache (no counterpart in the reference, which
- * serves one) */
+ * serves one) ------------------------------------------------------------
+ *
+ * Attention as qg_tree_attention where all sequences begin alike (one system
+ * prompt, one document), reading what they share once for all of them. *shared
+ * (device) positions are common: the pages wholly below them have the same
+ * entries in every sequence's row of the page table, and hold the same committed
+ * tokens. Of these pages the entries are read in the row of the first sequence
+ * that is not refused, and only there (the largest multiple of
+ * max(128, page_tokens) up to *shared counts; less than that is read like the
+ * rest). *shared 0 or less: nothing is common. A sequence shorter than *shared is
+ * refused like one whose length is negative. Sequences, rows, masks, values that are not
+ * finite and waits: as qg_tree_attention says, for which out is the same up to
+ * rounding; a page outside the pool among the common ones makes every row NaN. The
+ * workspace is zero-filled once, and is not that of qg_tree_attention.
+ * seqs*tokens*q_heads is at most 2^24. */
+int qg_shared_attention_workspace_bytes(int seqs, int tokens, int q_heads, int kv_heads, int head_dim, size_t *bytes);
+int qg_shared_attention(float *out, const float *q, const qg_kv_cache *cache, int layer, const int *shared, const uint64_t *tree,
+                        float scale, int seqs, int tokens, int q_heads, void *workspace);
 
 /* The next token of each row of logits [row][vocab], drawn with the given random
  * number uniforms[row] in [0, 1) from what the user's settings leave of

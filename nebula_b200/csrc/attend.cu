@@ -64,6 +64,12 @@ struct AttendArgs {
     int *err;
     float *part_acc;   // [2 * kMaxCtas][part_rows][D]
     float2 *part_ml;   // [2 * kMaxCtas][part_rows]
+    // with a shared prefix:
+    const int *shared;
+    int all_tiles;       // row tiles of all sequences' rows together
+    float *prefix_acc;   // [row][q_heads][D], [row][q_heads]: of prefix items that one CTA did as a whole
+    float2 *prefix_ml;
+    float2 *own_ml;      // the same of sequences' items, whose sums are in out
 };
 
 constexpr int kChunk = 32;       // keys per step of the softmax
@@ -104,6 +110,7 @@ struct Cfg {
 struct Plan {
     long long slot0, slot1;
     int seq0, length0, kv0, tile0, pos0;
+    int common, source;  // positions that are read once for all sequences, and the sequence whose pages tell where
 };
 
 struct Shared : Plan {
@@ -286,6 +293,45 @@ __device__ __forceinline__ bool group_any(int id, int n, bool x) {
 
 // ---- the division of the work ---------------------------------------------
 
+// With a shared prefix (SHARED) the line of work begins with the prefix, as one more sequence (-1) whose rows are those of all
+// sequences and whose keys are `common` positions, a whole number of units and pages; the sequences' own items hold what
+// comes after. Their lengths below count from there.
+__device__ __forceinline__ long long warp_sum(long long x) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    return x;
+}
+// Positions that all sequences share as asked for, 0: none, -1: more than a table has (every sequence is refused).
+template <bool SHARED>
+__device__ __forceinline__ int asked_shared(const AttendArgs &a) {
+    if constexpr (!SHARED) return 0;
+    const int n = *a.shared;
+    return n > a.c.table_pages << a.c.shift ? -1 : max(n, 0);
+}
+template <bool SHARED>
+__device__ __forceinline__ int committed(const AttendArgs &a, int seq, int shared) {
+    const int n = a.c.committed(seq, a.tokens);
+    return SHARED && (shared < 0 || n < shared) ? -1 : n;
+}
+// One warp: the first sequence that is not refused, or -1.
+__device__ __forceinline__ int first_live(const AttendArgs &a, int shared) {
+    for (int s0 = 0; s0 < a.seqs; s0 += 32) {
+        const int s = s0 + (threadIdx.x & 31);
+        const unsigned live = __ballot_sync(0xffffffffu, s < a.seqs && committed<true>(a, s, shared) >= 0);
+        if (live) return s0 + __ffs(live) - 1;
+    }
+    return -1;
+}
+__device__ __forceinline__ int common_of(const AttendArgs &a, int shared, int source) {
+    return shared <= 0 || source < 0 ? 0 : shared & ~(max(kKeys, a.c.page_tokens()) - 1);
+}
+// A sequence's committed positions after the common ones.
+template <bool SHARED>
+__device__ __forceinline__ int own_length(const AttendArgs &a, int seq, int shared, int common) {
+    const int n = committed<SHARED>(a, seq, shared);
+    return n < 0 ? -1 : n - common;
+}
+
 // Units of one (sequence, head, row tile); 0: the sequence is refused (length -1).
 __device__ __forceinline__ int units_of(const AttendArgs &a, int length) {
     return length < 0 ? 0 : (length + a.tokens + kKeys - 1) / kKeys;
@@ -299,26 +345,28 @@ template <int D>
 __device__ __forceinline__ int slots_of(const AttendArgs &a, int length) {
     return length < 0 ? 0 : units_of(a, length) + kItemCost<D>;
 }
-__device__ __forceinline__ long long warp_sum(long long x) {
-#pragma unroll
-    for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-    return x;
+// Slots of the prefix, and those of one of its items.
+template <int D>
+__device__ __forceinline__ int prefix_slots(int common) { return common / kKeys + kItemCost<D>; }
+template <int D>
+__device__ __forceinline__ long long prefix_line(const AttendArgs &a, int common) {
+    return common ? (long long)prefix_slots<D>(common) * a.c.kv_heads * a.all_tiles : 0;
 }
 // One warp: slots of the sequences before `seqs`.
-template <int D>
-__device__ long long sum_slots(const AttendArgs &a, int seqs, int per) {
+template <int D, bool SHARED>
+__device__ long long sum_slots(const AttendArgs &a, int seqs, int per, int shared, int common) {
     long long sum = 0;
-    for (int s = threadIdx.x & 31; s < seqs; s += 32) sum += (long long)slots_of<D>(a, a.c.committed(s, a.tokens)) * per;
+    for (int s = threadIdx.x & 31; s < seqs; s += 32) sum += (long long)slots_of<D>(a, own_length<SHARED>(a, s, shared, common)) * per;
     return warp_sum(sum);
 }
 // One warp: the sequence that holds slot `at`, its length and the slots before it. `len`: the lane's own sequence
 // among the first 32.
-template <int D>
-__device__ int find_slot(const AttendArgs &a, int per, long long at, int len, long long &base, int &length) {
+template <int D, bool SHARED>
+__device__ int find_slot(const AttendArgs &a, int per, long long at, int len, int shared, int common, long long &base, int &length) {
     const int lane = threadIdx.x & 31;
     base = 0;
     for (int s0 = 0; s0 < a.seqs; s0 += 32) {
-        if (s0) len = s0 + lane < a.seqs ? a.c.committed(s0 + lane, a.tokens) : -1;
+        if (s0) len = s0 + lane < a.seqs ? own_length<SHARED>(a, s0 + lane, shared, common) : -1;
         const long long mine = (long long)slots_of<D>(a, len) * per;
         long long upto = mine;
 #pragma unroll
@@ -350,28 +398,29 @@ struct Item {
     int seq, kv, tile, first, count, units, length;
     long long start;  // the slot of the item's first unit
 };
-template <int D>
+template <int D, bool SHARED>
 struct Walk {
     long long at, end;
     int seq, length, kv, tile, pos;  // pos: slot within the item
+    const Plan &p;
     __device__ Walk(const Plan &s)
-        : at(s.slot0), end(s.slot1), seq(s.seq0), length(s.length0), kv(s.kv0), tile(s.tile0), pos(s.pos0) {}
+        : at(s.slot0), end(s.slot1), seq(s.seq0), length(s.length0), kv(s.kv0), tile(s.tile0), pos(s.pos0), p(s) {}
     __device__ bool next(const AttendArgs &a, Item &it) {
         const int from = max(pos, kItemCost<D>);
         if (at + (from - pos) >= end) return false;
         it.seq = seq, it.kv = kv, it.tile = tile, it.first = from - kItemCost<D>, it.length = length;
-        it.units = units_of(a, length);
+        it.units = SHARED && seq < 0 ? length / kKeys : units_of(a, length);
         it.start = at - pos + kItemCost<D>;
         at += from - pos;
         it.count = (int)min((long long)(it.units - it.first), end - at);
         at += it.count;
         pos = 0;  // the item after it, should there be one
-        if (++tile == a.row_tiles) {
+        if (++tile == (SHARED && seq < 0 ? a.all_tiles : a.row_tiles)) {
             tile = 0;
             if (++kv == a.c.kv_heads) {
                 kv = 0;
                 do
-                    if (++seq < a.seqs) length = a.c.committed(seq, a.tokens);
+                    if (++seq < a.seqs) length = own_length<SHARED>(a, seq, SHARED ? asked_shared<SHARED>(a) : 0, SHARED ? p.common : 0);
                 while (seq < a.seqs && length < 0);
             }
         }
@@ -380,34 +429,60 @@ struct Walk {
 };
 
 // One warp: the slots of CTA (or pair) `team`.
-template <int D>
+template <int D, bool SHARED>
 __device__ __forceinline__ void plan(const AttendArgs &a, Plan &s, int team, int teams) {
     const int lane = threadIdx.x & 31;
     const int per = a.c.kv_heads * a.row_tiles;
-    const int len = lane < a.seqs ? a.c.committed(lane, a.tokens) : -1;
+    const int shared = asked_shared<SHARED>(a), source = SHARED ? first_live(a, shared) : 0, common = SHARED ? common_of(a, shared, source) : 0;
+    const int len = lane < a.seqs ? own_length<SHARED>(a, lane, shared, common) : -1;
+    const long long line = SHARED ? prefix_line<D>(a, common) : 0;
     long long w = (long long)slots_of<D>(a, len) * per, base = 0, u0 = 0, u1 = 0;
     int seq = 0, length = len;
     if (a.seqs > 1) {
-        for (int q = lane + 32; q < a.seqs; q += 32) w += (long long)slots_of<D>(a, a.c.committed(q, a.tokens)) * per;
+        for (int q = lane + 32; q < a.seqs; q += 32) w += (long long)slots_of<D>(a, own_length<SHARED>(a, q, shared, common)) * per;
         w = warp_sum(w);
     }
+    w += line;
     const int g = (int)min((long long)teams, w);  // (one sequence: right in lane 0)
     if (team < g) {
         u0 = range_start(team, w, g);
         u1 = range_start(team + 1, w, g);
-        if (a.seqs > 1) seq = find_slot<D>(a, per, u0, len, base, length);
+        if (u0 < line) seq = -1, length = common;
+        else if (a.seqs > 1) seq = find_slot<D, SHARED>(a, per, u0 - line, len, shared, common, base, length), base += line;
+        else base = line;
     }
     if (lane == 0) {
-        const int slots = max(1, slots_of<D>(a, length)), index = (int)quotient(u0 - base, slots);
+        const int slots = SHARED && seq < 0 ? prefix_slots<D>(common) : max(1, slots_of<D>(a, length)), index = (int)quotient(u0 - base, slots);
+        const int tiles = SHARED && seq < 0 ? a.all_tiles : a.row_tiles;
         s.slot0 = u0, s.slot1 = u1, s.seq0 = seq, s.length0 = length;
-        s.kv0 = index / a.row_tiles, s.tile0 = index % a.row_tiles;
+        s.kv0 = index / tiles, s.tile0 = index % tiles;
         s.pos0 = (int)(u0 - base - (long long)index * slots);
+        s.common = common, s.source = source;
     }
 }
 
+// Of an item: the rows of q that are its own, counted from its first sequence's; where its keys begin; whose pages they are on.
+template <bool SHARED>
+__device__ __forceinline__ int rows_of(const AttendArgs &a, const Item &it) {
+    return (SHARED && it.seq < 0 ? a.seqs * a.tokens : a.tokens) * a.group;
+}
+template <bool SHARED>
+__device__ __forceinline__ int base_of(const Plan &s, const Item &it) { return SHARED && it.seq >= 0 ? s.common : 0; }
+template <bool SHARED>
+__device__ __forceinline__ int pages_of(const Plan &s, const Item &it) { return SHARED && it.seq < 0 ? s.source : it.seq; }
+template <bool SHARED>
+__device__ __forceinline__ int nodes_of(const AttendArgs &a, const Item &it) { return SHARED && it.seq < 0 ? 0 : a.tokens; }
+// Row r of the item in q and out, in heads.
+template <bool SHARED>
+__device__ __forceinline__ size_t head_of(const AttendArgs &a, const Item &it, int r) {
+    const int node = r / a.group;
+    return ((size_t)(SHARED ? max(it.seq, 0) : it.seq) * a.tokens + node) * a.q_heads + it.kv * a.group + (r - node * a.group);
+}
+
 // Keys that unit j of an item's part holds.
+template <bool SHARED>
 __device__ __forceinline__ int keys_of(const AttendArgs &a, const Item &it, int j) {
-    return min(kKeys, it.length + a.tokens - (it.first + j) * kKeys);
+    return min(kKeys, it.length + nodes_of<SHARED>(a, it) - (it.first + j) * kKeys);
 }
 // Where key `row` of a piece of values starts: boxes of v_box keys, in each the column blocks one after the other.
 template <int NC>
@@ -415,9 +490,9 @@ __device__ __forceinline__ uint32_t value_at(const AttendArgs &a, int row) {
     return ((row & ~(a.v_box - 1)) * NC + (row & (a.v_box - 1))) * 128;
 }
 // Pieces of values of an item's part: a last unit that is not full has fewer.
-template <class C>
+template <class C, bool SHARED>
 __device__ __forceinline__ uint32_t value_pieces(const AttendArgs &a, const Item &it) {
-    return (it.count - 1) * C::kPieces + (keys_of(a, it, it.count - 1) + C::kVKeys - 1) / C::kVKeys;
+    return (it.count - 1) * C::kPieces + (keys_of<SHARED>(a, it, it.count - 1) + C::kVKeys - 1) / C::kVKeys;
 }
 
 // Nodes whose values are not finite, in the notes of both CTAs of a pair: each sees half of the columns. The other CTA may
@@ -439,13 +514,13 @@ __device__ __forceinline__ void mark_odd(uint64_t *notes, uint64_t nodes) {
     }
 }
 
-template <int D, int MR, bool PAIR>
+template <int D, int MR, bool PAIR, bool SHARED>
 __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __grid_constant__ AttendArgs a,
                                                                      const __grid_constant__ CUtensorMap k_map,
                                                                      const __grid_constant__ CUtensorMap v_map) {
     using C = Cfg<D, MR, PAIR>;
     static_assert(!PAIR || C::kOBufs == 1, "mark_odd: a unit takes both CTAs' O of the unit before");
-    const int copies = D == 256 ? 1 : a.copies;
+    const int copies = D == 256 || SHARED ? 1 : a.copies;
     constexpr int NC = C::kChunks, NK = C::kKStages, NV = C::kVStages, VK = C::kVKeys, QB = C::kQBufs, OB = C::kOBufs, VB = C::kVBlocks, NP = C::kPieces, KB = C::kKBlocks;
     constexpr int kPeers = PAIR ? 2 : 1;  // CTAs that work on one item
     const int team = blockIdx.x / kPeers, rank = blockIdx.x % kPeers, teams = gridDim.x / kPeers;
@@ -457,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
 
     if (warp == 0) {
         asm volatile("griddepcontrol.wait;" ::: "memory");
-        plan<D>(a, s, team, teams);
+        plan<D, SHARED>(a, s, team, teams);
     } else if (warp == 1) {
         if constexpr (PAIR) {
             asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s.tmem)));
@@ -494,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         tc_fence_after();
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
         const uint32_t tmem = s.tmem;
-        Walk<D> walk(s);
+        Walk<D, SHARED> walk(s);
         Item it;
         if (warp == 0 || warp == 3) {
             // ------------------------------------------------ producers: pages to the rings, keys (warp 0), values (warp 3)
@@ -511,10 +586,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             uint32_t st = 0, round = 0, unit = 0;
             bool ok = true;
             while (ok && walk.next(a, it)) {
-                const int n = it.length + a.tokens;
-                const int *table = a.c.table + (size_t)it.seq * a.c.table_pages;
+                const int base = base_of<SHARED>(s, it), n = base + it.length + nodes_of<SHARED>(a, it);
+                const int *table = a.c.table + (size_t)pages_of<SHARED>(s, it) * a.c.table_pages;
                 auto look_up = [&](int j) {  // page of keys l*page.. of unit j, for lane l
-                    const int p = (((it.first + j) * kKeys) >> a.c.shift) + lane;
+                    const int p = ((base + (it.first + j) * kKeys) >> a.c.shift) + lane;
                     const int id = lane < per_unit && p <= (n - 1) >> a.c.shift ? table[p] : 0;
                     return (unsigned)id < (unsigned)a.c.pages ? id : 0;  // the accumulators make the row NaN
                 };
@@ -524,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                     if (lane < 8) pages[lane] = ids;
                     __syncwarp();
                     if (j + 1 < it.count) ids = look_up(j + 1);
-                    const int pos = (it.first + j) * kKeys, keys = keys_of(a, it, j);
+                    const int pos = base + (it.first + j) * kKeys, keys = keys_of<SHARED>(a, it, j);
                     const int pieces = is_k ? NP : (keys + VK - 1) / VK;
                     for (int c = 0; c < pieces; c++) {
                         if (round) ok = wait_warp(&empty[st], (round - 1) & 1, abort, a.err);
@@ -554,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             if (!ok && lane == 0)  // the copies in flight land before the CTA ends
                 for (uint32_t i = 0; i < places; i++)
                     if ((i < st || round) && rank == 0) wait_drain(&full[i], (i < st ? round : round - 1) & 1);
-            if (!is_k)  // rows of refused sequences
+            if (!SHARED && !is_k)  // rows of refused sequences (with a shared prefix, the join's)
                 for (int q = blockIdx.x; q < a.seqs; q += gridDim.x)
                     if (a.c.committed(q, a.tokens) < 0)
                         for (size_t i = lane; i < (size_t)a.tokens * a.q_heads * D; i += 32)
@@ -612,7 +687,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             while (ok && walk.next(a, it)) {
                 for (int j = 0; ok && j < it.count; j++, tile++) {
                     const uint32_t buf = tile & 1, p0 = tmem + C::kS + buf * kKeys, ob = tile % OB, o = tmem + ob * D;
-                    const int keys = keys_of(a, it, j), past = it.length - (it.first + j) * kKeys;
+                    const int keys = keys_of<SHARED>(a, it, j), past = it.length - (it.first + j) * kKeys;
                     if (tile >= OB) ok = wait(&s.o_empty[ob], (tile / OB - 1) & 1, abort, a.err);
                     // the pieces of part z; where it holds nodes, the accumulator warps are told to clean their values
                     uint32_t at = st, turn = round;
@@ -673,7 +748,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         sync_all<PAIR>();
         tc_fence_after();
         const uint32_t tmem = s.tmem;
-        Walk<D> walk(s);
+        Walk<D, SHARED> walk(s);
         Item it;
         const int row = tid - 128, span = MR / copies, copy = row / span, chunks = kKeys / kChunk / copies;
         const int h0 = copy * chunks, h1 = h0 + chunks;
@@ -682,9 +757,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         bool ok = true;
         while (ok && walk.next(a, it)) {
             const int row0 = it.tile * C::kTileRows + rank * kRows, node = (row0 + row % span) / a.group;
-            const bool live = row < MR && row0 + (row & ~31) % span < a.tokens * a.group;  // the warp has rows
+            const bool live = row < MR && row0 + (row & ~31) % span < rows_of<SHARED>(a, it);  // the warp has rows
             uint64_t mask = 0;
-            if (node < a.tokens) {
+            if (!(SHARED && it.seq < 0) && node < a.tokens) {
                 mask = a.tree ? a.tree[(size_t)it.seq * a.tokens + node] : ~0ull >> (63 - node);
                 if (a.tokens < 64) mask &= (1ull << a.tokens) - 1;
             }
@@ -696,7 +771,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 const uint32_t buf = tile & 1, cols = tmem + lanes + C::kS + buf * kKeys;
                 const int past = it.length - (it.first + j) * kKeys;  // keys of this unit before the nodes
                 const bool tail = past < kKeys;
-                const int held = (keys_of(a, it, j) + kChunk - 1) / kChunk;  // chunks that hold keys; the product leaves out the others
+                const int held = (keys_of<SHARED>(a, it, j) + kChunk - 1) / kChunk;  // chunks that hold keys; the product leaves out the others
                 // which of keys 32h .. 32h+31 the row sees, in a unit that holds nodes
                 auto seen = [&](int h) -> uint32_t {
                     const int at = past - 32 * h;  // keys of the chunk before the nodes
@@ -820,7 +895,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         sync_all<PAIR>();
         tc_fence_after();
         const uint32_t tmem = s.tmem;
-        Walk<D> walk(s);
+        Walk<D, SHARED> walk(s);
         Item it;
         constexpr int H = D / 2, V = D / 32;
         const int w = warp - 8, row = (warp & 3) * 32 + lane, col0 = (w >> 2) * H, span = MR / copies;
@@ -834,10 +909,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             if (more) {
                 // Warp w prepares, and at the end stores, rows w, w+8, ...; lane i < 16 knows where row w+8i lies in q
                 // and out. Rows past the last are left as they are: no one reads their results.
-                const int row0 = nx.tile * C::kTileRows + rank * kRows, rows = min(kRows, a.tokens * a.group - row0);
+                const int row0 = nx.tile * C::kTileRows + rank * kRows, rows = min(kRows, rows_of<SHARED>(a, nx) - row0);
                 {
-                    const int r = row0 + w + 8 * (lane & 15), node = r / a.group;
-                    where_nx = node < a.tokens ? (((size_t)nx.seq * a.tokens + node) * a.q_heads + nx.kv * a.group + (r - node * a.group)) * D : 0;
+                    const int r = row0 + w + 8 * (lane & 15);
+                    where_nx = r < rows_of<SHARED>(a, nx) ? head_of<SHARED>(a, nx, r) * D : 0;
                 }
                 const uint32_t qb = round % QB;
                 unsigned char *q_to = q_smem + qb * 2 * C::kPlane;
@@ -913,15 +988,16 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             }
             if (QB == 1) it = nx, where = where_nx;
             const uint32_t qb = QB == 2 ? (round - 1) % 2 : 0;
-            const int row0 = it.tile * C::kTileRows + rank * kRows, rows = min(kRows, a.tokens * a.group - row0);
+            const int row0 = it.tile * C::kTileRows + rank * kRows, rows = min(kRows, rows_of<SHARED>(a, it) - row0);
             const bool live = (row & ~31) % span < rows && row < MR;  // the warp has rows
             unsigned char *stage = q_smem + qb * 2 * C::kPlane;
             // pages of the item, checked
             bool bad = false;
-            const int last = min((it.first + it.count) * kKeys, it.length + a.tokens) - 1;
+            const int base = base_of<SHARED>(s, it);
+            const int last = base + min((it.first + it.count) * kKeys, it.length + nodes_of<SHARED>(a, it)) - 1;
 #pragma unroll 1
-            for (int p = ((it.first * kKeys) >> a.c.shift) + (tid - 256); p <= last >> a.c.shift; p += 256)
-                bad |= (unsigned)a.c.table[(size_t)it.seq * a.c.table_pages + p] >= (unsigned)a.c.pages;
+            for (int p = ((base + it.first * kKeys) >> a.c.shift) + (tid - 256); p <= last >> a.c.shift; p += 256)
+                bad |= (unsigned)a.c.table[(size_t)pages_of<SHARED>(s, it) * a.c.table_pages + p] >= (unsigned)a.c.pages;
             float2 acc[H / 2];
 #pragma unroll
             for (int i = 0; i < H / 2; i++) acc[i] = make_float2(0.0f, 0.0f);
@@ -994,7 +1070,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             if (ok && live) {
                 unsigned char *mine = stage + (size_t)row * D * 4;
                 float mul = 1.0f;
-                if (copies == 1 && whole) {
+                if (!SHARED && copies == 1 && whole) {
                     const float total = s.val[slot][row];
                     mul = total == 0.0f ? 0.0f : 1.0f / total;
                 }
@@ -1002,14 +1078,14 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                 for (int i = 0; i < H / 4; i++)
                     *reinterpret_cast<float4 *>(mine + (((col0 / 4 + i) ^ (row & 7)) << 4)) =
                         make_float4(acc[2 * i].x * mul, acc[2 * i].y * mul, acc[2 * i + 1].x * mul, acc[2 * i + 1].y * mul);
-                uint64_t odd = row % span < rows ? *(volatile uint64_t *)&s.odd_nodes[PAIR ? items & 1 : 0] : 0;
+                uint64_t odd = row % span < rows && !(SHARED && it.seq < 0) ? *(volatile uint64_t *)&s.odd_nodes[PAIR ? items & 1 : 0] : 0;
                 if (odd) {  // rare: values that are not finite, for the rows that see them
                     const int node = (row0 + row % span) / a.group;
                     odd &= a.tree ? a.tree[(size_t)it.seq * a.tokens + node] : ~0ull >> (63 - node);
                     while (odd) {
                         const int nd = __ffsll((long long)odd) - 1;
                         odd &= odd - 1;
-                        const long long at = a.c.row(it.seq, it.length + nd);
+                        const long long at = a.c.row(it.seq, base + it.length + nd);
                         // (only in the copy of Q that has the key: another may see nothing, and its sums be left out by a 0)
                         if (at < 0 || (it.length + nd) % kKeys * copies / kKeys != row / span) continue;
                         const __half *v = a.c.v + ((size_t)at * a.c.kv_heads + it.kv) * D + col0;
@@ -1029,12 +1105,18 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             const size_t part = (size_t)(2 * team + (it.start > s.slot0)) * a.part_rows + rank * kRows;
             const float nan = __int_as_float(0x7fc00000);
             if (copies == 1) {
-                if (!whole && col0 == 0 && row < rows) a.part_ml[part + row] = make_float2(s.q_scale[qb][row], s.val[slot][row]);
+                // whole items with a shared prefix wait in out, or in the prefix's rows, for the join
+                float *const rows_to = SHARED && it.seq < 0 ? a.prefix_acc : a.out;
+                if ((SHARED || !whole) && col0 == 0 && row < rows) {
+                    float2 *ml = a.part_ml + part + row;
+                    if (SHARED && whole) ml = (it.seq < 0 ? a.prefix_ml : a.own_ml) + head_of<SHARED>(a, it, row0 + row);
+                    *ml = make_float2(s.q_scale[qb][row], s.val[slot][row]);
+                }
 #pragma unroll 4
                 for (int i = 0; w + 8 * i < rows; i++) {
                     const int r = w + 8 * i;
                     const size_t at = __shfl_sync(0xffffffffu, where, i);
-                    float *dst = whole ? a.out + at : a.part_acc + (part + r) * D;
+                    float *dst = whole ? rows_to + at : a.part_acc + (part + r) * D;
 #pragma unroll
                     for (int u = lane; u < D / 4; u += 32) {
                         float4 v = *reinterpret_cast<const float4 *>(stage + (size_t)r * D * 4 + ((u ^ (r & 7)) << 4));
@@ -1079,7 +1161,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             __syncwarp();
             if (lane == 0) arrive(&s.msg_empty[slot]);
             msg++, items++;
-            piece0 += value_pieces<C>(a, it);
+            piece0 += value_pieces<C, SHARED>(a, it);
             group_sync(4, 256);  // Q's place is free again
             if (QB == 2) it = nx, where = where_nx, left = more;
             more = more && walk.next(a, nx);
@@ -1134,7 +1216,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) token_attention_kernel(cons
     const float nan = __int_as_float(0x7fc00000);
     if (warp == 0) {
         asm volatile("griddepcontrol.wait;" ::: "memory");
-        plan<D>(a, s, team, gridDim.x);
+        plan<D, false>(a, s, team, gridDim.x);
     }
     __syncthreads();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -1144,7 +1226,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) token_attention_kernel(cons
     unsigned char *const ring = smem + warp * C::kStages * C::kStage + lane * 16;
     float *const sums = reinterpret_cast<float *>(smem + C::kRing);
     const size_t width = (size_t)a.c.kv_heads * D;
-    Walk<D> walk(s);
+    Walk<D, false> walk(s);
     Item it;
     while (walk.next(a, it)) {
         const int all = it.length + 1, n = it.length + (a.tree ? (int)(a.tree[it.seq] & 1) : 1);  // keys there, keys seen
@@ -1292,7 +1374,9 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) token_attention_kernel(cons
 // Joins the parts of items that several CTAs share, and makes every row NaN
 // after an error: one CTA per (row, head). Warps take every eighth part, so all
 // loads of a row are in flight at once; their sums join in order.
-template <int D>
+// With a shared prefix every row has parts: the prefix's, then its sequence's own. One that a CTA did as a whole is in the
+// rows of prefix_acc or out.
+template <int D, bool SHARED>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttendArgs a, int teams) {
     constexpr int V = D / 32;
     __shared__ float sums[8][D];
@@ -1301,35 +1385,56 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Atten
     const int id = blockIdx.x, h = id % a.q_heads, row = id / a.q_heads, seq = row / a.tokens;
     const int kv = h / a.group, r = (row % a.tokens) * a.group + h % a.group, tile = r / a.tile_rows;
     const int per = a.c.kv_heads * a.row_tiles;
-    const int units = units_of(a, a.c.committed(seq, a.tokens));
-    const long long w = sum_slots<D>(a, a.seqs, per);
-    const long long start = (seq ? sum_slots<D>(a, seq, per) : 0) + (long long)(kv * a.row_tiles + tile) * (units + kItemCost<D>) + kItemCost<D>;
+    const int shared = asked_shared<SHARED>(a), common = SHARED ? common_of(a, shared, first_live(a, shared)) : 0;
+    const int own = own_length<SHARED>(a, seq, shared, common), units = units_of(a, own);
+    const long long line = SHARED ? prefix_line<D>(a, common) : 0, w = line + sum_slots<D, SHARED>(a, a.seqs, per, shared, common);
+    const long long start = line + (seq ? sum_slots<D, SHARED>(a, seq, per, shared, common) : 0) +
+                            (long long)(kv * a.row_tiles + tile) * (units + kItemCost<D>) + kItemCost<D>;
     const int g = (int)min((long long)teams, w);
     const int c0 = units ? cta_of(start, w, g) : 0, parts = units ? cta_of(start + units - 1, w, g) - c0 + 1 : 0;
+    // the prefix's parts of this row
+    const int all_r = SHARED ? row * a.group + h % a.group : 0, all_tile = all_r / a.tile_rows;
+    const long long all_start = SHARED ? (long long)(kv * a.all_tiles + all_tile) * prefix_slots<D>(common) + kItemCost<D> : 0;
+    const int p0 = common ? cta_of(all_start, w, g) : 0, before = common ? cta_of(all_start + common / kKeys - 1, w, g) - p0 + 1 : 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     float *out = a.out + (size_t)id * D;
-    if (*(volatile int *)a.err) {
+    if (*(volatile int *)a.err || (SHARED && own < 0)) {
         for (int i = threadIdx.x; i < D; i += 256) out[i] = __int_as_float(0x7fc00000);
         return;
     }
-    if (parts < 2) return;
+    if (!SHARED && parts < 2) return;
+    const bool late = start > range_start(c0, w, g), all_late = SHARED && all_start > range_start(p0, w, g);  // the first part is its CTA's second
+    const int count = before + parts;
+    // where part p of the row is
+    auto part = [&](int p, const float *&acc, const float2 *&ml) {
+        const bool prefix = SHARED && p < before;
+        if (SHARED && (prefix ? before : parts) == 1) {
+            acc = (prefix ? a.prefix_acc : a.out) + (size_t)id * D, ml = (prefix ? a.prefix_ml : a.own_ml) + id;
+            return;
+        }
+        const int q = prefix ? p : p - before;
+        const size_t at = (size_t)(2 * ((prefix ? p0 : c0) + q) + (q == 0 && (prefix ? all_late : late))) * a.part_rows +
+                          (prefix ? all_r : r) % a.tile_rows;
+        acc = a.part_acc + at * D, ml = a.part_ml + at;
+    };
     // Every warp has its own maximum; kFly parts are asked for before the first is used.
     constexpr int kFly = 5;
     float m = -INFINITY, l = 0.0f, acc[V];
 #pragma unroll
     for (int e = 0; e < V; e++) acc[e] = 0.0f;
-    const bool late = start > range_start(c0, w, g);  // the first part is its CTA's second
-    for (int p0 = warp; p0 < parts; p0 += 8 * kFly) {
+    for (int from = warp; from < count; from += 8 * kFly) {
         float2 ml[kFly];
         float x[kFly][V], top = m;
 #pragma unroll
         for (int i = 0; i < kFly; i++) {
-            const int p = p0 + 8 * i;
+            const int p = from + 8 * i;
             ml[i] = make_float2(-INFINITY, 0.0f);
-            if (p < parts) {
-                const size_t at = (size_t)(2 * (c0 + p) + (p == 0 && late)) * a.part_rows + r % a.tile_rows;
-                const float *src = a.part_acc + at * D + lane * V;
-                ml[i] = __ldcg(a.part_ml + at);
+            if (p < count) {
+                const float *src;
+                const float2 *totals_at;
+                part(p, src, totals_at);
+                src += lane * V;
+                ml[i] = __ldcg(totals_at);
                 if constexpr (V == 2) {
                     *reinterpret_cast<float2 *>(x[i]) = __ldcg(reinterpret_cast<const float2 *>(src));
                 } else {
@@ -1347,7 +1452,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Atten
         for (int e = 0; e < V; e++) acc[e] *= keep;
 #pragma unroll
         for (int i = 0; i < kFly; i++) {
-            if (p0 + 8 * i >= parts) continue;
+            if (from + 8 * i >= count) continue;
             const float f = ml[i].x == -INFINITY ? ml[i].y : ex2(ml[i].x - m);  // its total is 0 (nothing seen) or NaN
             l += f * ml[i].y;
 #pragma unroll
@@ -1405,12 +1510,12 @@ int part_rows(int tokens, int group) { return tokens * group < kRows ? tokens * 
 size_t ml_bytes(int rows) { return (size_t)2 * kMaxCtas * rows * sizeof(float2); }
 
 // The attention kernel and the join, chained to what runs before. Peers: CTAs that work on one item.
-template <int D, typename... A>
+template <int D, bool SHARED, typename... A>
 int launch(const AttendArgs &a, void (*kernel)(A...), int peers, int threads, int smem, const A &...args) {
     if (int rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return rc;
     // no more CTAs than the longest sequences that the table allows could use
     const long long units = (((long long)a.c.table_pages << a.c.shift) + kKeys - 1) / kKeys;
-    const long long most = (long long)a.seqs * a.c.kv_heads * a.row_tiles * (units + kItemCost<D>);
+    const long long most = ((long long)a.seqs * a.row_tiles + (SHARED ? a.all_tiles : 0)) * a.c.kv_heads * (units + kItemCost<D>);
     const int teams = (int)(most < kMaxCtas / peers ? most : kMaxCtas / peers);
     cudaLaunchConfig_t cfg = {};
     cfg.stream = launch_stream;
@@ -1430,31 +1535,20 @@ int launch(const AttendArgs &a, void (*kernel)(A...), int peers, int threads, in
     cfg.gridDim = dim3((unsigned)(a.seqs * a.tokens * a.q_heads));
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
-    return cudaLaunchKernelEx(&cfg, join_kernel<D>, a, teams);
+    return cudaLaunchKernelEx(&cfg, join_kernel<D, SHARED>, a, teams);
 }
-template <int D, int MR, bool PAIR>
+template <int D, int MR, bool PAIR, bool SHARED>
 int launch_tiles(const AttendArgs &a, const CUtensorMap &k_map, const CUtensorMap &v_map) {
-    return launch<D>(a, tree_attention_kernel<D, MR, PAIR>, PAIR ? 2 : 1, kThreads, Cfg<D, MR, PAIR>::kSmem, a, k_map, v_map);
+    return launch<D, SHARED>(a, tree_attention_kernel<D, MR, PAIR, SHARED>, PAIR ? 2 : 1, kThreads, Cfg<D, MR, PAIR>::kSmem, a, k_map, v_map);
 }
 template <int D>
 int launch_token(const AttendArgs &a) {
-    return launch<D>(a, token_attention_kernel<D>, 1, 32 * kFewWarps, Few<D>::kSmem, a);
+    return launch<D, false>(a, token_attention_kernel<D>, 1, 32 * kFewWarps, Few<D>::kSmem, a);
 }
 
-}  // namespace
-
-extern "C" int qg_attention_workspace_bytes(int seqs, int tokens, int q_heads, int kv_heads, int head_dim, size_t *bytes) {
-    if (!bytes || seqs < 1 || seqs > kMaxSeqs || tokens < 1 || tokens > kMaxNodes || kv_heads < 1 || kv_heads > 1024 ||
-        q_heads < kv_heads || q_heads > 1024 || q_heads % kv_heads || (head_dim != 64 && head_dim != 128 && head_dim != 256))
-        return cudaErrorInvalidValue;
-    const int rows = part_rows(tokens, q_heads / kv_heads);
-    *bytes = 256 + ml_bytes(rows) + (size_t)2 * kMaxCtas * rows * head_dim * sizeof(float);
-    return cudaSuccess;
-}
-
-extern "C" int qg_tree_attention(float *out, const float *q, const qg_kv_cache *cache, int layer, const uint64_t *tree,
-                                 float scale, int seqs, int tokens, int q_heads, void *workspace) {
-    AttendArgs a;
+// Checks of both attentions' arguments, and what follows from them alone.
+int attend_args(AttendArgs &a, float *out, const float *q, const qg_kv_cache *cache, int layer, const uint64_t *tree, float scale, int seqs,
+                int tokens, int q_heads, void *workspace) {
     if (int rc = cache_view(cache, layer, seqs, tokens, a.c)) return rc;
     if (!out || !q || !workspace || q_heads < a.c.kv_heads || q_heads > 1024 || q_heads % a.c.kv_heads ||
         ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(workspace)) & 15) ||
@@ -1470,30 +1564,96 @@ extern "C" int qg_tree_attention(float *out, const float *q, const qg_kv_cache *
     a.tokens = tokens;
     a.q_heads = q_heads;
     a.group = q_heads / a.c.kv_heads;
-    // Few rows: heads of 64 and 128 values, whose units take little time, share a unit's keys among copies of Q; heads of
-    // 256 keep only 64 rows of Q, and the room goes to the rings. Many rows of heads of 256: pairs of CTAs.
-    const int rows = tokens * a.group;
-    const bool pair = a.c.head_dim == 256 && rows > kRows;
-    a.copies = a.c.head_dim == 256 || rows > 64 ? 1 : a.c.head_dim == 128 || rows > 32 ? 2 : 4;
+    a.shared = nullptr;
+    a.all_tiles = 0;
+    a.prefix_acc = nullptr;
+    a.prefix_ml = a.own_ml = nullptr;
+    a.err = static_cast<int *>(workspace);
+    a.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + 256);
+    return 0;
+}
+// Tiles of 128 rows, or of 256 for a pair, and the boxes of keys and values that go with them. `rows`: of the tallest item.
+void tiles(AttendArgs &a, int rows, bool pair) {
     a.tile_rows = pair ? 2 * kRows : kRows;
-    a.row_tiles = (rows + a.tile_rows - 1) / a.tile_rows;
+    a.row_tiles = (a.tokens * a.group + a.tile_rows - 1) / a.tile_rows;
     a.part_rows = rows < a.tile_rows ? rows : a.tile_rows;
     const int page = a.c.page_tokens(), k_rows = pair ? kKeys / 2 : kKeys, v_blocks = a.c.head_dim / (pair ? 128 : 64);
     const int v_rows = 16384 / (128 * v_blocks);
     a.k_box = page < k_rows ? page : k_rows;
     a.k_blocks = pair && a.k_box == k_rows ? 2 : 1;
     a.v_box = page < v_rows ? page : v_rows;
-    a.err = static_cast<int *>(workspace);
-    a.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + 256);
+}
+int maps(const AttendArgs &a, bool pair, CUtensorMap &k_map, CUtensorMap &v_map) {
+    if (int rc = pool_map(&k_map, a.c, a.c.k, a.k_box, a.k_blocks)) return rc;
+    return pool_map(&v_map, a.c, a.c.v, a.v_box, a.c.head_dim / (pair ? 128 : 64));
+}
+bool bad_sizes(int seqs, int tokens, int q_heads, int kv_heads, int head_dim) {
+    return seqs < 1 || seqs > kMaxSeqs || tokens < 1 || tokens > kMaxNodes || kv_heads < 1 || kv_heads > 1024 || q_heads < kv_heads ||
+           q_heads > 1024 || q_heads % kv_heads || (head_dim != 64 && head_dim != 128 && head_dim != 256);
+}
+constexpr long long kMaxShared = 1 << 24;  // rows and heads of a batch with a shared prefix
+
+}  // namespace
+
+extern "C" int qg_attention_workspace_bytes(int seqs, int tokens, int q_heads, int kv_heads, int head_dim, size_t *bytes) {
+    if (!bytes || bad_sizes(seqs, tokens, q_heads, kv_heads, head_dim)) return cudaErrorInvalidValue;
+    const int rows = part_rows(tokens, q_heads / kv_heads);
+    *bytes = 256 + ml_bytes(rows) + (size_t)2 * kMaxCtas * rows * head_dim * sizeof(float);
+    return cudaSuccess;
+}
+
+extern "C" int qg_tree_attention(float *out, const float *q, const qg_kv_cache *cache, int layer, const uint64_t *tree,
+                                 float scale, int seqs, int tokens, int q_heads, void *workspace) {
+    AttendArgs a;
+    if (int rc = attend_args(a, out, q, cache, layer, tree, scale, seqs, tokens, q_heads, workspace)) return rc;
+    // Few rows: heads of 64 and 128 values, whose units take little time, share a unit's keys among copies of Q; heads of
+    // 256 keep only 64 rows of Q, and the room goes to the rings. Many rows of heads of 256: pairs of CTAs.
+    const int rows = tokens * a.group;
+    const bool pair = a.c.head_dim == 256 && rows > kRows;
+    a.copies = a.c.head_dim == 256 || rows > 64 ? 1 : a.c.head_dim == 128 || rows > 32 ? 2 : 4;
+    tiles(a, rows, pair);
     a.part_acc = reinterpret_cast<float *>(static_cast<char *>(workspace) + 256 + ml_bytes(part_rows(tokens, a.group)));
     // One token, at most four heads to a key head of up to 128 values: no tensor cores (16 tokens, 32/8 heads of 128: 62 us
     // against 88). Heads of 256 leave no room for copies ahead.
     if (rows <= kFewRows && tokens == 1 && a.c.head_dim <= 128) return a.c.head_dim == 64 ? launch_token<64>(a) : launch_token<128>(a);
     CUtensorMap k_map, v_map;
-    if (int rc = pool_map(&k_map, a.c, a.c.k, a.k_box, a.k_blocks)) return rc;
-    if (int rc = pool_map(&v_map, a.c, a.c.v, a.v_box, v_blocks)) return rc;
-    if (a.c.head_dim == 64) return launch_tiles<64, 128, false>(a, k_map, v_map);
-    if (a.c.head_dim == 128) return rows <= 32 ? launch_tiles<128, 64, false>(a, k_map, v_map) : launch_tiles<128, 128, false>(a, k_map, v_map);
-    if (pair) return launch_tiles<256, 128, true>(a, k_map, v_map);
-    return rows <= 64 ? launch_tiles<256, 64, false>(a, k_map, v_map) : launch_tiles<256, 128, false>(a, k_map, v_map);
+    if (int rc = maps(a, pair, k_map, v_map)) return rc;
+    if (a.c.head_dim == 64) return launch_tiles<64, 128, false, false>(a, k_map, v_map);
+    if (a.c.head_dim == 128) return rows <= 32 ? launch_tiles<128, 64, false, false>(a, k_map, v_map) : launch_tiles<128, 128, false, false>(a, k_map, v_map);
+    if (pair) return launch_tiles<256, 128, true, false>(a, k_map, v_map);
+    return rows <= 64 ? launch_tiles<256, 64, false, false>(a, k_map, v_map) : launch_tiles<256, 128, false, false>(a, k_map, v_map);
+}
+
+extern "C" int qg_shared_attention_workspace_bytes(int seqs, int tokens, int q_heads, int kv_heads, int head_dim, size_t *bytes) {
+    if (!bytes || bad_sizes(seqs, tokens, q_heads, kv_heads, head_dim) || (long long)seqs * tokens * q_heads > kMaxShared)
+        return cudaErrorInvalidValue;
+    const int rows = part_rows(seqs * tokens, q_heads / kv_heads);
+    const size_t heads = ((size_t)seqs * tokens * q_heads + 1) & ~(size_t)1;
+    *bytes = 256 + ml_bytes(rows) + (size_t)2 * kMaxCtas * rows * head_dim * sizeof(float) + heads * (2 * sizeof(float2) + head_dim * sizeof(float));
+    return cudaSuccess;
+}
+
+extern "C" int qg_shared_attention(float *out, const float *q, const qg_kv_cache *cache, int layer, const int *shared, const uint64_t *tree,
+                                   float scale, int seqs, int tokens, int q_heads, void *workspace) {
+    AttendArgs a;
+    if (int rc = attend_args(a, out, q, cache, layer, tree, scale, seqs, tokens, q_heads, workspace)) return rc;
+    if (!shared || (long long)seqs * tokens * q_heads > kMaxShared) return cudaErrorInvalidValue;
+    const int rows = seqs * tokens * a.group, d = a.c.head_dim;  // of the prefix
+    const bool pair = d == 256 && rows > kRows;
+    a.copies = 1;
+    tiles(a, rows, pair);
+    a.shared = shared;
+    a.all_tiles = (rows + a.tile_rows - 1) / a.tile_rows;
+    const int held = part_rows(seqs * tokens, a.group);
+    const size_t heads = ((size_t)seqs * tokens * q_heads + 1) & ~(size_t)1;
+    a.part_acc = reinterpret_cast<float *>(static_cast<char *>(workspace) + 256 + ml_bytes(held));
+    a.prefix_acc = a.part_acc + (size_t)2 * kMaxCtas * held * d;
+    a.prefix_ml = reinterpret_cast<float2 *>(a.prefix_acc + heads * d);
+    a.own_ml = a.prefix_ml + heads;
+    CUtensorMap k_map, v_map;
+    if (int rc = maps(a, pair, k_map, v_map)) return rc;
+    if (d == 64) return launch_tiles<64, 128, false, true>(a, k_map, v_map);
+    if (d == 128) return launch_tiles<128, 128, false, true>(a, k_map, v_map);
+    if (pair) return launch_tiles<256, 128, true, true>(a, k_map, v_map);
+    return rows <= 64 ? launch_tiles<256, 64, false, true>(a, k_map, v_map) : launch_tiles<256, 128, false, true>(a, k_map, v_map);
 }

@@ -52,6 +52,8 @@ SIGNATURES = {
     "verify_workspace_bytes": ([I, I, I, C.POINTER(Z)], I),
     "verify_tree": ([P, P, P, P, P, P, P, P, D, I, I, I, P], I),
     "cache_commit": ([P, P, P, P, I, I], I),
+    "shared_attention_workspace_bytes": ([I, I, I, I, I, C.POINTER(Z)], I),
+    "shared_attention": ([P, P, P, I, P, P, F, I, I, I, P], I),
     "sample": ([P, P, P, P, P, P, P, I, I, I], I), "truncate_logits": ([P, P, P, P, P, P, I, I, I], I),
     "pages_reserve": ([P, P, P, P, P, I, I], I), "pages_release": ([P, P, P, I, I], I),
     "synth_weights": ([P, I, I, I, U64, F], I), "synth_normal": ([P, Z, U64, F], I),
@@ -233,6 +235,11 @@ def _zeroed(name: str, *sizes) -> Device:
 def attention_workspace(seqs: int, tokens: int, q_heads: int, kv_heads: int, head_dim: int) -> Device:
     """A zero-filled workspace for qg_tree_attention."""
     return _zeroed("attention_workspace_bytes", seqs, tokens, q_heads, kv_heads, head_dim)
+
+
+def shared_attention_workspace(seqs: int, tokens: int, q_heads: int, kv_heads: int, head_dim: int) -> Device:
+    """A zero-filled workspace for qg_shared_attention."""
+    return _zeroed("shared_attention_workspace_bytes", seqs, tokens, q_heads, kv_heads, head_dim)
 
 
 def verify_workspace(seqs: int, tokens: int, vocab: int) -> Device:

@@ -98,3 +98,42 @@ def test_definition_of_pages():
     assert p.reserve([40, 16], [2, 2], 2, 10)[0] == [0, 1]
     p.held[0] = 0
     assert p.reserve([40, 16], [2, 2], 2, 10)[0] == [-2, 0]
+
+
+def cache(**over):
+    f = dict(k=P4, v=P4, page_table=P4, lengths=P4, layer_bytes=64 * 16 * 2 * 128 * 2, layers=3, pages=64, page_tokens=16,
+             table_pages=8, kv_heads=2, head_dim=128)
+    f.update(over)
+    return C.byref(L.KvCache(**f))
+
+
+def attention(c, **over):
+    f = dict(out=P4, q=P4, layer=0, shared=P4, tree=P4, scale=0.1, seqs=2, tokens=4, q_heads=8, ws=P4)
+    f.update(over)
+    return L.code("shared_attention", f["out"], f["q"], c, f["layer"], f["shared"], f["tree"], f["scale"], f["seqs"], f["tokens"], f["q_heads"],
+                  f["ws"])
+
+
+@pytest.mark.parametrize("over", [dict(k=None), dict(v=None), dict(page_table=None), dict(lengths=None), dict(k=P4 + 8), dict(pages=0),
+                                  dict(page_tokens=8), dict(page_tokens=512), dict(table_pages=0), dict(kv_heads=0), dict(head_dim=96),
+                                  dict(layers=0), dict(layer_bytes=64), dict(pages=1 << 28), dict(table_pages=1 << 28)], ids=str)
+def test_shared_attention_refuses_caches(over):
+    assert attention(cache(**over)) == INVALID
+
+
+@pytest.mark.parametrize("over", [dict(out=None), dict(q=None), dict(shared=None), dict(ws=None), dict(layer=-1), dict(layer=3), dict(q_heads=0),
+                                  dict(q_heads=7), dict(q_heads=2048), dict(out=P4 + 8), dict(q=P4 + 4), dict(tree=P4 + 4), dict(ws=P4 + 8),
+                                  dict(seqs=0), dict(seqs=1025), dict(tokens=0), dict(tokens=65), dict(scale=float("inf")),
+                                  dict(scale=float("nan")), dict(seqs=1024, tokens=64, q_heads=258)], ids=str)
+def test_shared_attention_refuses(over):
+    assert attention(cache(), **over) == INVALID
+
+
+def test_shared_attention_workspace():
+    n = C.c_size_t(0)
+    for bad in ((0, 4, 8, 2, 128), (1025, 4, 8, 2, 128), (2, 65, 8, 2, 128), (2, 4, 7, 2, 128), (2, 4, 8, 0, 128), (2, 4, 8, 2, 80),
+                (1024, 64, 512, 2, 128)):
+        assert L.code("shared_attention_workspace_bytes", *bad, C.byref(n)) == INVALID
+    assert L.code("shared_attention_workspace_bytes", 2, 4, 8, 2, 128, None) == INVALID
+    assert L.code("shared_attention_workspace_bytes", 2, 4, 8, 2, 128, C.byref(n)) == 0 and n.value > 0
+    assert L.code("shared_attention_workspace_bytes", 1024, 64, 256, 2, 256, C.byref(n)) == 0 and n.value > 1 << 34
