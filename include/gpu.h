@@ -378,7 +378,7 @@ int qg_shared_attention(float *out, const float *q, const qg_kv_cache *cache, in
  * gets token -1.
  * Probabilities are taken relative to the largest, as whole multiples of 2^-44
  * of it, and their sums are exact: equal inputs give equal tokens. vocab at most
- * 393213, rows at most 2^20, logits 4-byte aligned. */
+ * 360445, rows at most 2^20, logits 4-byte aligned. */
 int qg_sample(int *token, const float *logits, const float *uniforms, const float *temperature, const int *top_k, const float *top_p,
               const float *min_p, int per, int rows, int vocab);
 /* The same logits with -infinity in place of what is not kept, so that

@@ -8,7 +8,8 @@
 //             until their sum reaches top_p of those, none below min_p of the largest
 //     token   the first index at which the running sum of the kept exceeds u times their sum
 // A set that is kept is always "all logits above a key, and those at the key up to an index". The key is found by counts (top-k)
-// or sums (top-p) over 1024 bins, first of the distance to the maximum, then of the bits of the keys that are left.
+// or sums (top-p) over 256 bins, first of the distance to the maximum, then of the bits of the keys that are left; as soon as
+// 1024 logits are left, every CTA reads them all and goes on alone.
 //
 // Weights are evaluated in 64 bits and summed as whole numbers: borders are compared exactly, and neither the cluster's
 // size nor the order of atomics has a say. With weights in 32 bits a running sum is off by some 1e-8, and a tail of 100,000
@@ -20,39 +21,40 @@ using namespace nb;
 namespace {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kBins = 1024;
-constexpr int kPiece = 128;                       // logits that a warp takes at a time: four to a lane
-constexpr int kStep = kWarps * kPiece;            // a CTA's part of a row is a multiple of this
-constexpr int kMaxPart = 24 * kStep;              // 192 KB
+constexpr int kBins = 256;
+constexpr int kFew = 256;                         // logits that are ordered one by one
+constexpr int kList = 1024;                       // logits that every CTA has a list of
+constexpr int kStep = kThreads * 4;               // a CTA's part of a row is a multiple of this: a thread has whole units of four
+constexpr int kMaxUnits = 22;                     // of a thread: 188 KB a CTA
 constexpr int kMaxRanks = 8;                      // CTAs of a cluster
-constexpr int kMaxVocab = kMaxRanks * kMaxPart;   // the sum of 2^44 for each still fits 63 bits
+constexpr int kMaxVocab = kMaxRanks * kMaxUnits * kStep;
 constexpr int kRowsAtOnce = 1 << 20;
-static_assert(kMaxVocab <= 1 << 19, "sums of weights");
+static_assert(kMaxVocab <= 1 << 19, "sums of weights, 2^44 at most, fit 63 bits");
+static_assert(2 * kFew <= kThreads && kBins <= kThreads, "two threads to a logit that is ordered, one to a bin");
 
 struct SampleArgs {
     const float *logits, *uniforms, *temperature, *top_p, *min_p;
     const int *top_k;
     float *out;
     int *token;
-    int per, vocab, part;  // part: logits of a CTA
+    int per, vocab, units;
 };
 
-struct Top {
-    float most;
-    int odd;  // a NaN or +infinity
-};
-// What the CTAs of a cluster tell each other.
+using Whole = unsigned long long;
+
+// What the CTAs of a cluster read of each other.
 struct Shared {
-    Top top[kMaxRanks];
-    unsigned long long total[2][kMaxRanks];  // by the parity of the exchange: a CTA may be one ahead
-    unsigned long long before;               // of the bin that was found
-    unsigned long long warp_sum[kWarps];
-    unsigned bin, count;
-    int index[kMaxRanks];
-    int last;                                // of the ties that are kept
-    float warp_most[kWarps];
-    int warp_odd[kWarps];
-    unsigned hist[4][kBins];                 // counts; sums as 15 + 15 + 14 bits
+    float most[kMaxRanks], least[kMaxRanks];
+    int index[kMaxRanks], last[2];
+    Whole total[2][kMaxRanks];         // by the parity of the exchange: a CTA may be one ahead
+    unsigned hist[2][4][kBins];        // by the parity of the pass: counts; sums as 15 + 15 + 14 bits
+    Whole list[kList];                 // key and inverted index: the larger is the better
+    int listed;
+    // a CTA's own
+    Whole warp_sum[kWarps], entry[kList], entry_weight[kFew];
+    Whole found, kept_sum;
+    int few;
+    float warp_most[kWarps], warp_least[kWarps];
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -80,9 +82,18 @@ __device__ __forceinline__ unsigned peer_load(uint32_t a) {
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(a) : "memory");
     return x;
 }
+__device__ __forceinline__ Whole peer_load64(uint32_t a) {
+    Whole x;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(x) : "r"(a) : "memory");
+    return x;
+}
 __device__ __forceinline__ void peer_store(uint32_t a, unsigned x) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(x) : "memory"); }
-__device__ __forceinline__ void peer_store(uint32_t a, unsigned long long x) {
-    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(x) : "memory");
+__device__ __forceinline__ void peer_store(uint32_t a, Whole x) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(x) : "memory"); }
+// The larger, or NaN if one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
 }
 
 // Whole numbers in the order of the floats.
@@ -92,401 +103,650 @@ __device__ __forceinline__ unsigned key_of(float x) {
 }
 __device__ __forceinline__ float of_key(unsigned k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 constexpr unsigned kNone = 0x007fffffu;  // key of -infinity
+constexpr float kLowest = -3.402823466e38f;
 
-// 2^44 * 2^((x - most) * c), rounded; c = log2(e) / T. The polynomial of degree 9 is 2^f's Chebyshev fit on [-1/2, 1/2]
-// (error 2^-46).
-__device__ __forceinline__ unsigned long long weight(float x, double most, double c) {
-    const double t = ((double)x - most) * c;
-    if (!(t > -46.0)) return 0;  // less than half a unit
-    constexpr double kRound = 6755399441055744.0, kUnit = 4503599627370496.0;  // 1.5 * 2^52, 2^52
-    const double n = t + kRound, f = t - (n - kRound);
-    double p = 1.0205905413765595e-07;
-    p = fma(p, f, 1.325964524488711e-06);
-    p = fma(p, f, 1.5252672924850737e-05);
-    p = fma(p, f, 1.540343375125101e-04);
-    p = fma(p, f, 1.3333558200794592e-03);
-    p = fma(p, f, 9.618129193934313e-03);
-    p = fma(p, f, 5.550410866465167e-02);
-    p = fma(p, f, 2.402265069564034e-01);
-    p = fma(p, f, 6.931471805599462e-01);
-    p = fma(p, f, 1.0000000000000135);
-    const double v = __hiloint2double(__double2hiint(p) + ((__double2loint(n) + 44) << 20), __double2loint(p)) + kUnit;
-    return (unsigned long long)__double_as_longlong(v) & 0xfffffffffffffull;
-}
-
-__device__ __forceinline__ unsigned long long warp_sum(unsigned long long x) {
+__device__ __forceinline__ Whole warp_sum(Whole x) {
 #pragma unroll
     for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
     return x;
 }
-__device__ __forceinline__ unsigned long long warp_scan(unsigned long long x) {
+__device__ __forceinline__ Whole warp_scan(Whole x) {
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const unsigned long long y = __shfl_up_sync(0xffffffffu, x, d);
+        const Whole y = __shfl_up_sync(0xffffffffu, x, d);
         if ((threadIdx.x & 31) >= d) x += y;
     }
     return x;
 }
 
-// One CTA's view of a row.
+// One CTA's view of a row. A thread has units of four neighbouring logits, all of its units next to each other, so the
+// threads' order is the indices' order; in shared memory threads are an odd number of units apart, which keeps their reads
+// off each other's banks.
 struct Row {
-    const float *part;  // its logits, in shared memory; what lies outside the row is -infinity
-    int pieces;         // of each warp
-    int start;          // index of the first logit (may be negative, where the row does not start on 16 bytes)
+    const float4 *mine;  // the thread's units; what lies outside the row is -infinity
+    int units;           // of a thread
+    int index;           // of its first logit (may be negative, where the row does not start on 16 bytes)
     uint32_t rank, ranks;
-    float most;
-    double top, c;
-    unsigned key;       // kept: logits above the key, and those at it up to index `last`
+    float most, zero;    // the largest logit; below `zero` weights are 0
+    double top, c;       // log2(e) / T
+    unsigned key;        // kept: logits above the key, and those at it up to index `last`
     int last;
 
+    // f(x, index) for every logit of the thread.
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll 2
-        for (int i = 0; i < pieces; i++) {
-            const int at = (warp * pieces + i) * kPiece + lane * 4;
-            const float4 x = *reinterpret_cast<const float4 *>(part + at);
-            f(x.x, start + at), f(x.y, start + at + 1), f(x.z, start + at + 2), f(x.w, start + at + 3);
+        for (int j = 0; j < units; j++) {
+            const float4 x = mine[j];
+            const int at = index + 4 * j;
+            f(x.x, at), f(x.y, at + 1), f(x.z, at + 2), f(x.w, at + 3);
         }
     }
-    __device__ __forceinline__ bool keeps(float x, int index) const {
-        const unsigned k = key_of(x);
-        return k > key || (k == key && index <= last);
+    // f(x, index, n) for those from low to high only, n of four at a time (the others are -infinity). They are looked for first,
+    // 32 logits at a time: a warp then takes as many turns as its fullest lane has logits, and not one for every place at which
+    // some lane has one; four at a time hide each other's latency.
+    template <typename F>
+    __device__ __forceinline__ void some(float low, float high, F f) const {
+        for (int j0 = 0; j0 < units; j0 += 8) {
+            unsigned found = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (j0 + j < units) {
+                    const float4 x = mine[j0 + j];
+                    found |= (unsigned)(x.x >= low && x.x <= high) << (4 * j) | (unsigned)(x.y >= low && x.y <= high) << (4 * j + 1) |
+                             (unsigned)(x.z >= low && x.z <= high) << (4 * j + 2) | (unsigned)(x.w >= low && x.w <= high) << (4 * j + 3);
+                }
+            while (found) {
+                float x[4];
+                int at[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int b = found ? __ffs(found) - 1 + 4 * j0 : 0;
+                    x[e] = found ? reinterpret_cast<const float *>(mine)[b] : -INFINITY;
+                    at[e] = index + b;
+                    found &= found - 1;
+                }
+                f(x, at);
+            }
+        }
     }
-    __device__ __forceinline__ unsigned long long weigh(float x) const { return weight(x, top, c); }
+    // The sum of the weights that are kept.
+    __device__ __forceinline__ Whole kept_sum() const {
+        Whole sum = 0;
+        if (key == kNone) {
+#pragma unroll 2
+            for (int j = 0; j < units; j++) {
+                const float4 x = mine[j];
+                if (__any_sync(0xffffffffu, fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)) >= zero)) sum += (weigh(x.x) + weigh(x.y)) + (weigh(x.z) + weigh(x.w));
+            }
+        } else {
+            some(fmaxf(floor(), zero), most, [&](const float (&x)[4], const int (&at)[4]) {
+                Whole w[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[e] = weigh(x[e]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) sum += keeps(x[e], at[e]) ? w[e] : 0;
+            });
+        }
+        return sum;
+    }
+    __device__ __forceinline__ bool keeps(float x, int i) const {
+        const unsigned k = key_of(x);
+        return k > key || (k == key && i <= last);
+    }
+    // The lowest logit that may be kept.
+    __device__ __forceinline__ float floor() const { return key == kNone ? kLowest : of_key(key); }
+
+    // 2^44 * 2^((x - most) * c), rounded. The polynomial of degree 9 is 2^f's Chebyshev fit on [-1/2, 1/2] (error 2^-46).
+    __device__ __forceinline__ Whole weigh(float x) const {
+        const double t = ((double)fmaxf(x, zero) - top) * c;
+        constexpr double kRound = 6755399441055744.0, kUnit = 4503599627370496.0;  // 1.5 * 2^52, 2^52
+        const double n = t + kRound, f = t - (n - kRound);
+        double p = 1.0205905413765595e-07;
+        p = fma(p, f, 1.325964524488711e-06);
+        p = fma(p, f, 1.5252672924850737e-05);
+        p = fma(p, f, 1.540343375125101e-04);
+        p = fma(p, f, 1.3333558200794592e-03);
+        p = fma(p, f, 9.618129193934313e-03);
+        p = fma(p, f, 5.550410866465167e-02);
+        p = fma(p, f, 2.402265069564034e-01);
+        p = fma(p, f, 6.931471805599462e-01);
+        p = fma(p, f, 1.0000000000000135);
+        const double v = __hiloint2double(__double2hiint(p) + ((__double2loint(n) + 44) << 20), __double2loint(p)) + kUnit;
+        return x >= zero ? (Whole)__double_as_longlong(v) & 0xfffffffffffffull : 0;
+    }
 };
 
-// Of 64-bit sums of the threads: the warps' to s.warp_sum, the CTAs' to s.total[turn] of all. Ends with a barrier of the
-// cluster.
-__device__ __forceinline__ void share_sums(Shared &s, const Row &r, unsigned long long x, int turn) {
+// Of the threads' sums: the warps' to s.warp_sum, the CTAs' to s.total of all. Ends with a barrier of the cluster.
+__device__ __forceinline__ void share_sums(Shared &s, const Row &r, Whole x, int turn) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     x = warp_sum(x);
     if (lane == 0) s.warp_sum[warp] = x;
     __syncthreads();
     if (warp == 0) {
-        const unsigned long long all = warp_sum(lane < kWarps ? s.warp_sum[lane] : 0);
+        const Whole all = warp_sum(lane < kWarps ? s.warp_sum[lane] : 0);
         if (lane < r.ranks) peer_store(at_rank(&s.total[turn & 1][r.rank], lane), all);
     }
     cluster_sync();
 }
 // Totals of the CTAs before this one, and of all.
-__device__ __forceinline__ unsigned long long sums_before(const Shared &s, const Row &r, int turn, unsigned long long &all) {
-    unsigned long long before = 0;
+__device__ __forceinline__ Whole sums_before(const Shared &s, const Row &r, int turn, Whole &all) {
+    Whole before = 0;
     all = 0;
     for (uint32_t i = 0; i < r.ranks; i++) {
-        const unsigned long long x = s.total[turn & 1][i];
+        const Whole x = s.total[turn & 1][i];
         if (i < r.rank) before += x;
         all += x;
     }
     return before;
 }
 // The index at which the running sum of f (in the order of indices) reaches `target`, for the one warp that holds it; -1 for
-// all others. After share_sums of the same f.
+// all others. `mine`: the thread's sum; after share_sums of it.
 template <typename F>
-__device__ int reach(const Shared &s, const Row &r, unsigned long long before, unsigned long long target, F f) {
+__device__ int reach(const Shared &s, const Row &r, Whole mine, Whole before, Whole target, F f) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const unsigned long long mine = lane < kWarps ? s.warp_sum[lane] : 0, upto = warp_scan(mine) + before;
+    const Whole of_warp = lane < kWarps ? s.warp_sum[lane] : 0, upto = warp_scan(of_warp) + before;
     const unsigned past = __ballot_sync(0xffffffffu, lane < kWarps && upto >= target);
     if (!past || __ffs(past) - 1 != warp) return -1;
-    unsigned long long base = __shfl_sync(0xffffffffu, upto - mine, warp);
+    const Whole base = __shfl_sync(0xffffffffu, upto - of_warp, warp);
     if (base >= target) return -1;  // (an earlier CTA's)
-    for (int i = 0; i < r.pieces; i++) {
-        const int at = (warp * r.pieces + i) * kPiece + lane * 4;
-        const float4 x = *reinterpret_cast<const float4 *>(r.part + at);
-        const unsigned long long w[4] = {f(x.x, r.start + at), f(x.y, r.start + at + 1), f(x.z, r.start + at + 2), f(x.w, r.start + at + 3)};
-        const unsigned long long four = w[0] + w[1] + w[2] + w[3], here = warp_scan(four) + base;
-        const unsigned hit = __ballot_sync(0xffffffffu, here >= target);
-        if (hit) {
-            const int l = __ffs(hit) - 1;
-            unsigned long long run = here - four;
-            int index = r.start + at;
-#pragma unroll
-            for (int e = 0; e < 3; e++) {
-                run += w[e];
-                if (run < target) index++;
-                else break;
-            }
-            return __shfl_sync(0xffffffffu, index, l);
-        }
-        base = __shfl_sync(0xffffffffu, here, 31);
+    const Whole here = warp_scan(mine) + base;
+    const int l = __ffs(__ballot_sync(0xffffffffu, here >= target)) - 1;
+    // the warp goes through that lane's logits, 32 at a time
+    Whole run = __shfl_sync(0xffffffffu, here - mine, l);
+    const float *x = reinterpret_cast<const float *>(r.mine + (l - lane) * (r.units | 1));
+    const int first = r.index + (l - lane) * 4 * r.units;
+    for (int i = 0; i < 4 * r.units; i += 32) {
+        const int at = i + lane;
+        const Whole w = at < 4 * r.units ? f(x[at], first + at) : 0, till = warp_scan(w) + run;
+        const unsigned hit = __ballot_sync(0xffffffffu, till >= target);
+        if (hit) return first + i + __ffs(hit) - 1;
+        run = __shfl_sync(0xffffffffu, till, 31);
     }
     return -1;
 }
 
-// The lowest key whose logit has a distance bin of at most `bin`. Each round, the lanes try 32 keys.
-__device__ unsigned lowest_key(float most, float scale, int bin) {
-    const int lane = threadIdx.x & 31;
-    const unsigned high = key_of(most);
-    unsigned a = 0;
-    for (int shift = 27; shift >= 0; shift = shift ? max(shift - 5, 0) : -1) {
-        const unsigned long long k = a + ((unsigned long long)lane << shift);
-        const bool below = lane == 0 || (k < high && (k <= kNone || min(kBins - 1, (int)((most - of_key((unsigned)k)) * scale)) > bin));
-        a += (unsigned)(__popc(__ballot_sync(0xffffffffu, below)) - 1) << shift;
-    }
-    return a + 1;
-}
-
-// Narrows the kept set to its largest logits: `target` of them (SUM: as many as it takes until their weights reach it).
-// `octaves`: bins of the first pass reach so far below the largest weight.
-template <bool SUM>
-__device__ void narrow(Shared &s, Row &r, unsigned long long target, float octaves, int &turn) {
+// The thread's bin of those in the order of threads (tid < kBins) at which the running sum of `mine` reaches `target`, and the
+// sum before it, to all threads; -1 where it is not reached. `count` is given along.
+struct Bin {
+    int bin, count;
+    Whole before;
+};
+__device__ __forceinline__ Bin reach_bin(Shared &s, Whole mine, unsigned count, Whole target) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int bins = kBins / r.ranks, bin0 = r.rank * bins;  // that this CTA adds up
-    const float scale = fminf((float)((kBins - 1) / (double)octaves * r.c), 1e30f);
-    const unsigned lowest = r.key;
-    unsigned low = r.key, high = key_of(r.most);
-    bool linear = true;
-    while (linear || low < high) {
-        const int shift = linear ? 0 : max(0, 22 - __clz(high - low));  // (high - low) >> shift < kBins
-        for (int i = tid; i < 4 * kBins; i += kThreads) s.hist[0][i] = 0;
-        __syncthreads();
-        r.each([&](float x, int index) {
-            const unsigned k = key_of(x);
-            if (k < low || k > high || !r.keeps(x, index)) return;
-            const int bin = linear ? min(kBins - 1, (int)((r.most - x) * scale)) : (int)((high - k) >> shift);
-            atomicAdd(&s.hist[0][bin], 1u);
-            if (SUM) {
-                const unsigned long long w = r.weigh(x);
-                atomicAdd(&s.hist[1][bin], (unsigned)w & 0x7fffu);
-                atomicAdd(&s.hist[2][bin], (unsigned)(w >> 15) & 0x7fffu);
-                atomicAdd(&s.hist[3][bin], (unsigned)(w >> 30));
+    const Whole upto_warp = warp_scan(mine);
+    if (lane == 31) s.warp_sum[warp] = upto_warp;
+    if (tid == 0) s.found = ~0ull;
+    __syncthreads();
+    const Whole of_warp = lane < kWarps ? s.warp_sum[lane] : 0, warps_upto = warp_scan(of_warp);
+    const Whole upto = upto_warp + __shfl_sync(0xffffffffu, warps_upto - of_warp, warp);
+    if (upto >= target && upto - mine < target) s.found = (Whole)count << 32 | (unsigned)tid, s.kept_sum = upto - mine;
+    __syncthreads();
+    const Whole found = s.found;
+    return {found == ~0ull ? -1 : (int)(found & 0xffffffffu), (int)(found >> 32), s.kept_sum};
+}
+// Adds a weight to a histogram's bin. Each part's sum over a CTA's logits (or a list's) fits 32 bits.
+__device__ __forceinline__ void add_weight(unsigned (&hist)[4][kBins], int bin, Whole w) {
+    atomicAdd(&hist[1][bin], (unsigned)w & 0x7fffu);
+    atomicAdd(&hist[2][bin], (unsigned)(w >> 15) & 0x7fffu);
+    atomicAdd(&hist[3][bin], (unsigned)(w >> 30));
+}
+// Keys from low to high, and of these the logits whose distance from the largest falls into `bin` (-1: any).
+struct Range {
+    unsigned low, high;
+    float most, scale;
+    int bin;
+    __device__ __forceinline__ int bin_of(float x) const { return min(kBins - 1, (int)((most - x) * scale)); }
+    __device__ __forceinline__ bool has(float x) const {
+        const unsigned k = key_of(x);
+        return k >= low && k <= high && (bin < 0 || bin_of(x) == bin);
+    }
+    // Only what is in distance bin b. The keys' limits are wider than the bin by more than bin_of rounds.
+    __device__ __forceinline__ void take_bin(int b) {
+        if (b < kBins - 1) low = max(low, key_of(__double2float_rd((double)most - (b + 1) * 1.000001 / (double)scale)));
+        if (b) high = min(high, key_of(__double2float_ru((double)most - b * 0.999999 / (double)scale)));
+        bin = b;
+    }
+    // Only key bin b of those that are 2^shift keys wide, from high on downwards.
+    __device__ __forceinline__ void take_keys(int b, int shift) {
+        high -= (unsigned)b << shift;
+        const unsigned span = (1u << shift) - 1;
+        low = high - low > span ? high - span : low;
+    }
+    __device__ __forceinline__ int shift() const { return max(0, 24 - __clz(high - low)); }  // (high - low) >> shift < kBins
+};
+
+// The kept logits in a range, of all CTAs and in any order, in s.entry. Returns their number; more than kList are not listed.
+// s.listed is zero before.
+__device__ int gather(Shared &s, const Row &r, const Range &in) {
+    const int tid = threadIdx.x;
+    r.some(of_key(max(in.low, kNone + 1)), of_key(in.high), [&](const float (&x)[4], const int (&at)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (r.keeps(x[e], at[e]) && in.has(x[e])) {
+                const int to = atomicAdd(&s.listed, 1);
+                if (to < kList) s.list[to] = (Whole)key_of(x[e]) << 32 | (unsigned)~at[e];
             }
-        });
-        cluster_sync();
-        // this CTA's bins over all CTAs, one bin to a thread and pass; warps' sums go through s.warp_sum
-        unsigned long long upto[2], mine[2];
-        unsigned count[2];
-        unsigned long long sum = 0;
+    });
+    cluster_sync();
+    int n[kMaxRanks], all = 0;
+#pragma unroll
+    for (int q = 0; q < kMaxRanks; q++) n[q] = q < r.ranks ? (int)peer_load(at_rank(&s.listed, q)) : 0;
+#pragma unroll
+    for (int q = 0; q < kMaxRanks; q++) all += n[q];
+    if (all > kList) return all;
+    for (int i = tid; i < all; i += kThreads) {
+        int q = 0, at = i;
+#pragma unroll
+        for (int e = 0; e < kMaxRanks - 1; e++)
+            if (q == e && at >= n[e]) at -= n[e], q++;
+        s.entry[i] = peer_load64(at_rank(&s.list[at], q));
+    }
+    __syncthreads();
+    return all;
+}
+// Weights of the n entries, and for entry tid/2 the number and the weights of the better ones. n is at most kFew.
+__device__ __forceinline__ int order(Shared &s, const Row &r, int n, Whole &above) {
+    const int tid = threadIdx.x;
+    if (tid < n) s.entry_weight[tid] = r.weigh(of_key((unsigned)(s.entry[tid] >> 32)));
+    __syncthreads();
+    int better = 0;
+    above = 0;
+    if ((tid & ~31) / 2 < n) {  // whole warps
+        const Whole me = s.entry[min(tid / 2, n - 1)];
+#pragma unroll 4
+        for (int j = tid & 1; j < n; j += 2) {
+            const bool b = s.entry[j] > me;
+            better += b;
+            above += b ? s.entry_weight[j] : 0;
+        }
+        better += __shfl_xor_sync(0xffffffffu, better, 1);
+        above += __shfl_xor_sync(0xffffffffu, above, 1);
+    }
+    return better;
+}
+// Of the n entries (they are the kept logits in a range): the one at which the running count, or sum, from the best on reaches
+// `target`. `hist` is zero before and after. In every CTA by itself.
+template <bool SUM>
+__device__ Whole nth_entry(Shared &s, const Row &r, int n, Range in, Whole target, unsigned (&hist)[4][kBins]) {
+    const int tid = threadIdx.x;
+    static_assert(kList == 2 * kThreads, "two entries to a thread");
+    while (n > kFew && in.low < in.high) {
+        Whole mine[2];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const int b = 2 * tid + i;
-            mine[i] = 0, count[i] = 0;
-            if (b < bins) {
-                unsigned long long part[3] = {0, 0, 0};
-                for (uint32_t q = 0; q < r.ranks; q++) {
-                    const uint32_t a = at_rank(&s.hist[0][bin0 + b], q);
-                    count[i] += peer_load(a);
-                    if (SUM)
-                        for (int e = 0; e < 3; e++) part[e] += peer_load(a + (e + 1) * kBins * 4);
-                }
-                mine[i] = SUM ? part[0] + (part[1] << 15) + (part[2] << 30) : count[i];
+            mine[i] = tid + i * kThreads < n ? s.entry[tid + i * kThreads] : 0;
+            if (mine[i]) {
+                const int bin = (int)((in.high - (unsigned)(mine[i] >> 32)) >> in.shift());
+                atomicAdd(&hist[0][bin], 1u);
+                if (SUM) add_weight(hist, bin, r.weigh(of_key((unsigned)(mine[i] >> 32))));
             }
-            sum += mine[i];
         }
-        share_sums(s, r, sum, turn);
-        unsigned long long all;
-        unsigned long long before = sums_before(s, r, turn, all);
-        turn++;
-        if (all < target) return;  // all of them
-        for (int i = 0; i < warp; i++) before += s.warp_sum[i];
-        before += warp_scan(sum) - sum;
-        upto[0] = before + mine[0], upto[1] = upto[0] + mine[1];
+        if (tid == 0) s.few = 0;
+        __syncthreads();
+        Whole sum = 0;
+        unsigned count = 0;
+        if (tid < kBins) {
+            count = hist[0][tid];
+            sum = SUM ? hist[1][tid] + ((Whole)hist[2][tid] << 15) + ((Whole)hist[3][tid] << 30) : count;
 #pragma unroll
-        for (int i = 0; i < 2; i++)
-            if (upto[i] >= target && upto[i] - mine[i] < target)
-                for (uint32_t q = 0; q < r.ranks; q++) {
-                    peer_store(at_rank(&s.bin, q), (unsigned)(bin0 + 2 * tid + i));
-                    peer_store(at_rank(&s.count, q), count[i]);
-                    peer_store(at_rank(&s.before, q), upto[i] - mine[i]);
-                }
-        cluster_sync();
-        const int bin = s.bin;
-        const bool whole = s.count == 1 || (!SUM && s.count == target - s.before);
-        target -= s.before;
-        if (linear) {
-            if (bin) high = min(high, lowest_key(r.most, scale, bin - 1) - 1);
-            low = max(low, lowest_key(r.most, scale, bin));
-            linear = false;
-        } else {
-            high -= (unsigned)bin << shift;
-            const unsigned span = (1u << shift) - 1;
-            low = high - low > span ? high - span : low;
+            for (int e = 0; e < 4; e++) hist[e][tid] = 0;
         }
-        if (whole) {  // the bin ends the set
-            if (low > lowest) r.last = 0x7fffffff;  // (at the lowest key fewer may have been kept before)
-            r.key = low;
+        const Bin b = reach_bin(s, sum, count, target);
+        const int shift = in.shift();
+        target -= b.before;
+        in.take_keys(b.bin, shift);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const unsigned k = (unsigned)(mine[i] >> 32);
+            if (mine[i] && k >= in.low && k <= in.high) s.entry[atomicAdd(&s.few, 1)] = mine[i];
+        }
+        __syncthreads();
+        n = b.count;
+    }
+    if (n <= kFew) {
+        Whole above;
+        const int better = order(s, r, n, above);
+        if (!(tid & 1) && tid / 2 < n && (SUM ? above < target && above + s.entry_weight[tid / 2] >= target : (Whole)better + 1 == target))
+            s.found = s.entry[tid / 2];
+        __syncthreads();
+        return s.found;
+    }
+    // equal logits: by their index alone
+    if (SUM) {
+        const Whole one = r.weigh(of_key(in.low));
+        target = (target + one - 1) / one;
+    }
+    for (int i = tid; i < n; i += kThreads) {
+        int better = 0;
+        const Whole me = s.entry[i];
+        for (int j = 0; j < n; j++) better += s.entry[j] > me;
+        if ((Whole)better + 1 == target) s.found = me;
+    }
+    __syncthreads();
+    return s.found;
+}
+
+// Narrows the kept set to its largest logits: `target` of them (SUM: as many as it takes until their weights reach it). None
+// that is wanted lies below `lowest`.
+template <bool SUM>
+__device__ void narrow(Shared &s, Row &r, Whole target, float lowest, int &pass, int &turn) {
+    const int tid = threadIdx.x, lane = tid & 31;
+    lowest = fmaxf(lowest, r.floor());
+    Range in = {key_of(lowest), key_of(r.most), r.most, fminf(kBins / (r.most - lowest), 1e30f), -1};
+    for (bool linear = true; linear || in.low < in.high; linear = false) {
+        const int shift = in.shift();
+        unsigned (&hist)[4][kBins] = s.hist[pass & 1], (&other)[4][kBins] = s.hist[~pass & 1];  // (zeros)
+        r.some(of_key(max(in.low, kNone + 1)), of_key(in.high), [&](const float (&x)[4], const int (&at)[4]) {
+            Whole w[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = SUM ? r.weigh(x[e]) : 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (r.keeps(x[e], at[e]) && in.has(x[e])) {
+                    const int bin = linear ? in.bin_of(x[e]) : (int)((in.high - key_of(x[e])) >> shift);
+                    atomicAdd(&hist[0][bin], 1u);
+                    if (SUM) add_weight(hist, bin, w[e]);
+                }
+        });
+        cluster_sync();
+        // every CTA adds up all bins of all, one bin to a thread
+        Whole mine = 0;
+        unsigned count = 0;
+        if (tid < kBins) {
+            unsigned part[SUM ? 4 : 1][kMaxRanks];
+#pragma unroll
+            for (int q = 0; q < kMaxRanks; q++)
+#pragma unroll
+                for (int e = 0; e < (SUM ? 4 : 1); e++) part[e][q] = q < r.ranks ? peer_load(at_rank(&hist[e][tid], q)) : 0;
+#pragma unroll
+            for (int q = 0; q < kMaxRanks; q++) {
+                count += part[0][q];
+                if constexpr (SUM) mine += part[1][q] + ((Whole)part[2][q] << 15) + ((Whole)part[3][q] << 30);
+            }
+            if (!SUM) mine = count;
+        }
+        // the other histogram, and the list, were read before this pass's barrier
+        for (int i = tid; i < 4 * kBins; i += kThreads) other[0][i] = 0;
+        if (tid == 0) s.listed = 0;
+        pass++;
+        const Bin b = reach_bin(s, mine, count, target);
+        if (b.bin < 0) return;  // all of them
+        target -= b.before;
+        if (linear) in.take_bin(b.bin);
+        else in.take_keys(b.bin, shift);
+        if (b.count <= kList) {
+            gather(s, r, in);
+            const Whole worst = nth_entry<SUM>(s, r, b.count, in, target, other);
+            r.key = (unsigned)(worst >> 32), r.last = (int)~(unsigned)worst;
             return;
         }
     }
-    // equal logits: the first ones
-    const unsigned long long each = SUM ? r.weigh(of_key(low)) : 1;
-    if (SUM) target = (target + each - 1) / each;
-    auto tie = [&](float x, int index) { return (unsigned long long)(key_of(x) == low && r.keeps(x, index)); };
-    unsigned long long n = 0;
+    // more equal logits than are listed: the first ones
+    const Whole one = SUM ? r.weigh(of_key(in.low)) : 1;
+    if (SUM) target = (target + one - 1) / one;
+    auto tie = [&](float x, int index) { return (Whole)(key_of(x) == in.low && r.keeps(x, index)); };
+    Whole n = 0, all;
     r.each([&](float x, int index) { n += tie(x, index); });
     share_sums(s, r, n, turn);
-    unsigned long long all;
-    const unsigned long long before = sums_before(s, r, turn, all);
+    const Whole before = sums_before(s, r, turn, all);
     turn++;
-    const int index = reach(s, r, before, target, tie);
-    if (index >= 0 && lane < r.ranks) peer_store(at_rank(&s.last, lane), (unsigned)index);
+    const int index = reach(s, r, n, before, target, tie);
+    if (index >= 0 && lane < r.ranks) peer_store(at_rank(&s.last[SUM], lane), (unsigned)index);
     cluster_sync();
-    r.key = low;
-    r.last = s.last;
+    r.key = in.low;
+    r.last = s.last[SUM];
+}
+
+// A lower bound of the k-th largest logit, from the largest of each thread's (k logits are at least as large as the k-th
+// largest of these); -infinity where there is none.
+__device__ float bound_of(Shared &s, const Row &r, int k, float threads_most, float least, int &pass) {
+    const int tid = threadIdx.x;
+    Range in = {kNone, key_of(r.most), r.most, fminf((kBins - 1) / (r.most - least), 1e30f), -1};
+    unsigned *hist = s.hist[pass & 1][0];
+    if (threads_most >= least) atomicAdd(&hist[in.bin_of(threads_most)], 1u);
+    cluster_sync();
+    unsigned count = 0;
+    if (tid < kBins) {
+        unsigned part[kMaxRanks];
+#pragma unroll
+        for (int q = 0; q < kMaxRanks; q++) part[q] = q < r.ranks ? peer_load(at_rank(&hist[tid], q)) : 0;
+#pragma unroll
+        for (int q = 0; q < kMaxRanks; q++) count += part[q];
+    }
+    pass++;  // (the next pass clears this histogram)
+    const Bin b = reach_bin(s, count, count, k);
+    if (b.bin < 0) return -INFINITY;
+    in.take_bin(b.bin);
+    return of_key(in.low);
 }
 
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a) {
     extern __shared__ __align__(16) unsigned char smem[];
-    float *const part = reinterpret_cast<float *>(smem);
-    Shared &s = *reinterpret_cast<Shared *>(part + a.part);
+    const int stride = a.units | 1;
+    float4 *const part = reinterpret_cast<float4 *>(smem);
+    Shared &s = *reinterpret_cast<Shared *>(part + kThreads * stride);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");  // a CTA's memory is there for others once it runs
     Row r;
-    r.part = part;
     r.rank = cluster_rank(), r.ranks = cluster_size();
-    r.pieces = a.part / kStep;
+    r.units = a.units;
+    r.mine = part + tid * stride;
     const int row = blockIdx.x / r.ranks, user = row / a.per;
     const float *const x0 = a.logits + (size_t)row * a.vocab;
     const int ahead = (int)(reinterpret_cast<uintptr_t>(x0) >> 2 & 3);  // logits between a multiple of 16 bytes and the row
-    r.start = (int)r.rank * a.part - ahead;
+    const int start = (int)r.rank * a.units * kStep - ahead;
+    r.index = start + tid * 4 * a.units;
+    for (int i = tid; i < 2 * 4 * kBins; i += kThreads) s.hist[0][0][i] = 0;
+    if (tid == 0) s.listed = 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const float t = a.temperature ? a.temperature[user] : 1.0f, p = a.top_p ? a.top_p[user] : 1.0f, least = a.min_p ? a.min_p[user] : 0.0f;
     const int k = a.top_k ? a.top_k[user] : 0;
     const float u = a.uniforms ? a.uniforms[row] : 0.0f;
 
-    // ---- the row, and its largest logit
+    // ---- the row, and its largest logit. A warp copies its threads' units, neighbouring ones at a time.
     float most = -INFINITY;
-    bool odd = false;
-#pragma unroll 8
-    for (int i = 0; i < r.pieces; i++) {
-        const int at = (warp * r.pieces + i) * kPiece + lane * 4, index = r.start + at;
-        float4 x = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        if (index >= 0 && index + 3 < a.vocab) x = __ldcs(reinterpret_cast<const float4 *>(x0 + index));
-        else {
-            if (index >= 0 && index < a.vocab) x.x = x0[index];
-            if (index + 1 >= 0 && index + 1 < a.vocab) x.y = x0[index + 1];
-            if (index + 2 >= 0 && index + 2 < a.vocab) x.z = x0[index + 2];
-            if (index + 3 >= 0 && index + 3 < a.vocab) x.w = x0[index + 3];
+    {
+        float4 *const to = part + warp * 32 * stride;
+        const int from = start + warp * 32 * 4 * a.units;
+        for (int j0 = 0; j0 < a.units; j0 += 8) {
+            float4 x[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int at = (j0 + j) * 32 + lane, i = from + 4 * at;
+                x[j] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                if (j0 + j < a.units) {
+                    if (i >= 0 && i + 3 < a.vocab) x[j] = __ldcs(reinterpret_cast<const float4 *>(x0 + i));
+                    else {
+                        if (i >= 0 && i < a.vocab) x[j].x = x0[i];
+                        if (i + 1 >= 0 && i + 1 < a.vocab) x[j].y = x0[i + 1];
+                        if (i + 2 >= 0 && i + 2 < a.vocab) x[j].z = x0[i + 2];
+                        if (i + 3 >= 0 && i + 3 < a.vocab) x[j].w = x0[i + 3];
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (j0 + j < a.units) {
+                    const int at = (j0 + j) * 32 + lane, owner = at / a.units;
+                    x[j].x += 0.0f, x[j].y += 0.0f, x[j].z += 0.0f, x[j].w += 0.0f;  // -0 is 0: equals go by their index
+                    to[owner * stride + (at - owner * a.units)] = x[j];
+                    most = max_nan(max_nan(max_nan(most, x[j].x), max_nan(x[j].y, x[j].z)), x[j].w);
+                }
         }
-        x.x += 0.0f, x.y += 0.0f, x.z += 0.0f, x.w += 0.0f;  // -0 is 0: equals go by their index
-        *reinterpret_cast<float4 *>(part + at) = x;
-        most = fmaxf(fmaxf(fmaxf(most, x.x), fmaxf(x.y, x.z)), x.w);
-        odd |= !(x.x < INFINITY && x.y < INFINITY && x.z < INFINITY && x.w < INFINITY);
     }
+    const float threads_most = most;
+    float lowest = most > -INFINITY ? most : INFINITY;  // of the threads' largest
 #pragma unroll
-    for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-    odd = __any_sync(0xffffffffu, odd);
-    if (lane == 0) s.warp_most[warp] = most, s.warp_odd[warp] = odd;
+    for (int d = 16; d; d >>= 1) {
+        most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, d));
+        lowest = fminf(lowest, __shfl_xor_sync(0xffffffffu, lowest, d));
+    }
+    if (lane == 0) s.warp_most[warp] = most, s.warp_least[warp] = lowest;
     __syncthreads();
-    if (warp == 0) {
-        most = lane < kWarps ? s.warp_most[lane] : -INFINITY;
-        odd = lane < kWarps && s.warp_odd[lane];
-#pragma unroll
-        for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-        odd = __any_sync(0xffffffffu, odd);
-    }
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     if (warp == 0) {
+        most = lane < kWarps ? s.warp_most[lane] : -INFINITY;
+        lowest = lane < kWarps ? s.warp_least[lane] : INFINITY;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) {
+            most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, d));
+            lowest = fminf(lowest, __shfl_xor_sync(0xffffffffu, lowest, d));
+        }
         if (lane < r.ranks) {
-            peer_store(at_rank(&s.top[r.rank].most, lane), __float_as_uint(most));
-            peer_store(at_rank(&s.top[r.rank].odd, lane), (unsigned)odd);
+            peer_store(at_rank(&s.most[r.rank], lane), __float_as_uint(most));
+            peer_store(at_rank(&s.least[r.rank], lane), __float_as_uint(lowest));
         }
     }
     cluster_sync();
-    most = -INFINITY, odd = false;
-    for (uint32_t i = 0; i < r.ranks; i++) most = fmaxf(most, s.top[i].most), odd |= s.top[i].odd != 0;
-    const bool refused = odd || most == -INFINITY || !(t >= 0.0f && t < INFINITY) || p != p || least != least || u != u;
+    most = -INFINITY, lowest = INFINITY;
+    for (uint32_t i = 0; i < r.ranks; i++) most = max_nan(most, s.most[i]), lowest = fminf(lowest, s.least[i]);
+    const bool refused = !(most > -INFINITY && most < INFINITY) || !(t >= 0.0f && t < INFINITY) || p != p || least != least || u != u;
 
     // ---- what is kept
-    int turn = 0;
+    int turn = 0, pass = 0;
     r.most = most;
     r.top = most;
     r.c = 1.4426950408889634 / (t > 0.0f ? (double)t : 1.0);
+    r.zero = fmaxf((float)(r.top - 46.0 / r.c), kLowest);
     r.key = kNone, r.last = -0x7fffffff;  // (what lies outside the row has indices from -3 on)
-    if (!refused) {
-        if (t == 0.0f) {  // the largest logit, the lowest index of equals
-            int index = 0x7fffffff;
-            r.each([&](float x, int at) { if (x == most) index = min(index, at); });
-            index = __reduce_min_sync(0xffffffffu, index);
-            if (lane == 0) s.warp_odd[warp] = index;
-            __syncthreads();
-            if (warp == 0) {
-                index = __reduce_min_sync(0xffffffffu, lane < kWarps ? s.warp_odd[lane] : 0x7fffffff);
-                if (lane < r.ranks) peer_store(at_rank(&s.index[r.rank], lane), (unsigned)index);
-            }
-            cluster_sync();
-            r.key = key_of(most), r.last = 0x7fffffff;
-            for (uint32_t i = 0; i < r.ranks; i++) r.last = min(r.last, s.index[i]);
-        } else {
-            if (k > 0 && k < a.vocab) narrow<false>(s, r, k, 32.0f, turn);
-            if (p < 1.0f) {
-                unsigned long long sum = 0, all;
-                r.each([&](float x, int index) { if (r.keeps(x, index)) sum += r.weigh(x); });
-                share_sums(s, r, sum, turn);
-                sums_before(s, r, turn, all);
-                turn++;
-                const unsigned long long share = p > 0.0f ? __double2ull_rz((double)p * 18446744073709551616.0) : 0;
-                const unsigned long long target = __umul64hi(share, all) + (share * all != 0);
-                // What lies a factor of vocab / (what may be left out) below the largest cannot reach into it.
-                const float left = (1.0f - fmaxf(p, 0.0f)) * (float)all * (1.0f / 17592186044416.0f);
-                const float octaves = fminf(fmaxf(log2f((float)a.vocab) - log2f(left) + 1.0f, 1.0f), 46.0f);
-                narrow<true>(s, r, target > 1 ? target : 1, octaves, turn);
-            }
-            if (least > 0.0f) {
-                const double border = r.top + (double)t * log((double)least);
-                const unsigned key = border >= r.top ? key_of(most) : key_of(__double2float_ru(border));
-                if (key > r.key) r.key = key, r.last = 0x7fffffff;
+    const unsigned min_key = [&]() -> unsigned {  // of the lowest logit that min_p leaves
+        if (!(least > 0.0f)) return 0;
+        const double border = r.top + (double)t * log((double)least);
+        return border >= r.top ? key_of(most) : key_of(__double2float_ru(border));
+    }();
+    int token = -1;  // where it is known already
+    if (refused) {
+    } else if (t == 0.0f) {  // the largest logit, the lowest index of equals
+        int index = 0x7fffffff;
+        r.some(most, most, [&](const float (&x)[4], const int (&at)[4]) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (x[e] == most) index = min(index, at[e]);
+        });
+        index = __reduce_min_sync(0xffffffffu, index);
+        if (lane == 0) s.warp_sum[warp] = index;
+        __syncthreads();
+        if (warp == 0) {
+            index = __reduce_min_sync(0xffffffffu, lane < kWarps ? (int)s.warp_sum[lane] : 0x7fffffff);
+            if (lane < r.ranks) peer_store(at_rank(&s.index[r.rank], lane), (unsigned)index);
+        }
+        cluster_sync();
+        r.key = key_of(most), r.last = 0x7fffffff;
+        for (uint32_t i = 0; i < r.ranks; i++) r.last = min(r.last, s.index[i]);
+        token = r.last;
+    } else {
+        bool done = false;
+        if (k > 0 && k < a.vocab) {
+            const float bound = bound_of(s, r, k, threads_most, lowest, pass);
+            const int n = k <= kFew ? gather(s, r, {key_of(fmaxf(bound, kLowest)), key_of(most), most, 0.0f, -1}) : kFew + 1;
+            if (n <= kFew) {
+                // few enough: all of the rest is in every CTA's own memory
+                Whole above;
+                const int better = order(s, r, n, above), held = min(k, n), me = tid / 2;
+                const bool one = !(tid & 1) && me < n;
+                if (one && better == held - 1) s.kept_sum = above + s.entry_weight[me];
+                __syncthreads();
+                bool stays = one && better < k;
+                if (p < 1.0f) {
+                    const Whole share = p > 0.0f ? __double2ull_rz((double)p * 18446744073709551616.0) : 0, all = s.kept_sum;
+                    const Whole target = __umul64hi(share, all) + (share * all != 0);
+                    stays = stays && (above < target || better == 0);
+                }
+                stays = stays && (unsigned)(s.entry[min(me, n - 1)] >> 32) >= min_key;
+                const int kept = __syncthreads_count(stays);
+                if (one && better == kept - 1) s.found = s.entry[me], s.kept_sum = above + s.entry_weight[me];
+                __syncthreads();
+                const Whole worst = s.found;
+                r.key = (unsigned)(worst >> 32), r.last = (int)~(unsigned)worst;
+                done = true;
+                if (a.token) {
+                    // among what is kept, the weights at lower indices
+                    const float v = fminf(fmaxf(u, 0.0f), 0.99999994f);
+                    const Whole aim = __umul64hi(__double2ull_rz((double)v * 18446744073709551616.0), s.kept_sum) + 1;
+                    if ((tid & ~31) / 2 < n) {
+                        const Whole entry = s.entry[min(me, n - 1)];
+                        Whole before = 0;
+                        for (int j = tid & 1; j < n; j += 2) {
+                            const Whole e = s.entry[j];
+                            if (e >= worst && (unsigned)e > (unsigned)entry) before += s.entry_weight[j];
+                        }
+                        before += __shfl_xor_sync(0xffffffffu, before, 1);
+                        if (one && entry >= worst && before < aim && before + s.entry_weight[me] >= aim && r.rank == 0)
+                            a.token[row] = (int)~(unsigned)entry;
+                    }
+                    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");  // no CTA ends while others read its list
+                    asm volatile("barrier.cluster.wait;" ::: "memory");
+                    return;
+                }
+            } else {
+                narrow<false>(s, r, k, bound, pass, turn);
             }
         }
+        if (!done && p < 1.0f) {
+            Whole all;
+            share_sums(s, r, r.kept_sum(), turn);
+            sums_before(s, r, turn, all);
+            turn++;
+            const Whole share = p > 0.0f ? __double2ull_rz((double)p * 18446744073709551616.0) : 0;
+            const Whole target = __umul64hi(share, all) + (share * all != 0);
+            // What lies a factor of vocab / (what may be left out) below the largest cannot reach into it.
+            const float left = (1.0f - fmaxf(p, 0.0f)) * (float)all * (1.0f / 17592186044416.0f);
+            const float octaves = fminf(fmaxf(log2f((float)a.vocab) - log2f(left) + 1.0f, 1.0f), 46.0f);
+            narrow<true>(s, r, target > 1 ? target : 1, fmaxf((float)(r.top - octaves / r.c), kLowest), pass, turn);
+        }
+        if (!done && min_key > r.key) r.key = min_key, r.last = 0x7fffffff;
     }
 
     // ---- the token, or the logits
     if (a.token) {
-        if (refused) {
-            if (r.rank == 0 && tid == 0) a.token[row] = -1;
-            return;
-        }
-        if (t == 0.0f) {
-            if (r.rank == 0 && tid == 0) a.token[row] = r.last;
+        if (refused || t == 0.0f) {
+            if (r.rank == 0 && tid == 0) a.token[row] = token;
             return;
         }
         auto mine = [&](float x, int index) { return r.keeps(x, index) ? r.weigh(x) : 0; };
-        unsigned long long sum = 0, all;
-        r.each([&](float x, int index) { sum += mine(x, index); });
+        const Whole sum = r.kept_sum();
+        Whole all;
         share_sums(s, r, sum, turn);
-        const unsigned long long before = sums_before(s, r, turn, all);
+        const Whole before = sums_before(s, r, turn, all);
         // the first running sum above u * all is the first that reaches the whole number after it
         const float v = fminf(fmaxf(u, 0.0f), 0.99999994f);
-        const unsigned long long aim = __umul64hi(__double2ull_rz((double)v * 18446744073709551616.0), all) + 1;
-        const int index = reach(s, r, before, aim, mine);
+        const Whole aim = __umul64hi(__double2ull_rz((double)v * 18446744073709551616.0), all) + 1;
+        const int index = reach(s, r, sum, before, aim, mine);
         if (index >= 0 && lane == 0) a.token[row] = index;
         return;
     }
+    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");  // no CTA ends while others read its memory
     float *const out = a.out + (size_t)row * a.vocab;
     const float other = refused ? __int_as_float(0x7fc00000) : -INFINITY;
-    if (!((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(x0)) & 15)) {
-        for (int i = 0; i < r.pieces; i++) {
-            const int at = (warp * r.pieces + i) * kPiece + lane * 4, index = r.start + at;
-            float4 x = *reinterpret_cast<const float4 *>(part + at);
-            x.x = !refused && r.keeps(x.x, index) ? x.x : other;
-            x.y = !refused && r.keeps(x.y, index + 1) ? x.y : other;
-            x.z = !refused && r.keeps(x.z, index + 2) ? x.z : other;
-            x.w = !refused && r.keeps(x.w, index + 3) ? x.w : other;
-            if (index >= 0 && index + 3 < a.vocab) __stcs(reinterpret_cast<float4 *>(out + index), x);
-            else {
-                if (index >= 0 && index < a.vocab) out[index] = x.x;
-                if (index + 1 >= 0 && index + 1 < a.vocab) out[index + 1] = x.y;
-                if (index + 2 >= 0 && index + 2 < a.vocab) out[index + 2] = x.z;
-                if (index + 3 >= 0 && index + 3 < a.vocab) out[index + 3] = x.w;
-            }
-        }
-    } else {
-        __syncwarp();
-        for (int i = 0; i < 4 * r.pieces; i++) {
-            const int at = warp * r.pieces * kPiece + i * 32 + lane, index = r.start + at;
-            const float x = part[at];
-            if (index >= 0 && index < a.vocab) out[index] = !refused && r.keeps(x, index) ? x : other;
+    const bool whole = !((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(x0)) & 15);
+    const float4 *const from = part + warp * 32 * stride;
+    for (int j = 0; j < a.units; j++) {
+        const int at = j * 32 + lane, owner = at / a.units, i = start + (warp * 32 * a.units + at) * 4;
+        float4 x = from[owner * stride + (at - owner * a.units)];
+        x.x = !refused && r.keeps(x.x, i) ? x.x : other;
+        x.y = !refused && r.keeps(x.y, i + 1) ? x.y : other;
+        x.z = !refused && r.keeps(x.z, i + 2) ? x.z : other;
+        x.w = !refused && r.keeps(x.w, i + 3) ? x.w : other;
+        if (whole && i >= 0 && i + 3 < a.vocab) __stcs(reinterpret_cast<float4 *>(out + i), x);
+        else {
+            if (i >= 0 && i < a.vocab) out[i] = x.x;
+            if (i + 1 >= 0 && i + 1 < a.vocab) out[i + 1] = x.y;
+            if (i + 2 >= 0 && i + 2 < a.vocab) out[i + 2] = x.z;
+            if (i + 3 >= 0 && i + 3 < a.vocab) out[i + 3] = x.w;
         }
     }
+    asm volatile("barrier.cluster.wait;" ::: "memory");
 }
 
 int launch(SampleArgs &a, int rows) {
-    // three logits may lie before a row that does not start on 16 bytes
-    const int long_row = a.vocab + 3;
+    // up to three logits may lie before a row that does not start on 16 bytes
+    const bool aligned = !(reinterpret_cast<uintptr_t>(a.logits) & 15) && a.vocab % 4 == 0;
+    const int long_row = a.vocab + (aligned ? 0 : 3);
     int ranks = 1;
     while (ranks < kMaxRanks && (long_row + ranks - 1) / ranks > kStep) ranks *= 2;
-    a.part = ((long_row + ranks - 1) / ranks + kStep - 1) / kStep * kStep;
-    const int smem = a.part * 4 + (int)sizeof(Shared);
+    a.units = ((long_row + ranks - 1) / ranks + kStep - 1) / kStep;
+    const int smem = kThreads * (a.units | 1) * 16 + (int)sizeof(Shared);
     if (int rc = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)rows * ranks);

@@ -24,7 +24,7 @@ def truncate(**over):
     return L.code("truncate_logits", *f.values())
 
 
-SIZES = [dict(rows=0), dict(rows=-1), dict(rows=(1 << 20) + 1), dict(vocab=0), dict(vocab=393214), dict(per=0), dict(per=-2)]
+SIZES = [dict(rows=0), dict(rows=-1), dict(rows=(1 << 20) + 1), dict(vocab=0), dict(vocab=360446), dict(per=0), dict(per=-2)]
 
 
 @pytest.mark.parametrize("over", [dict(token=None), dict(logits=None), dict(uniforms=None), dict(logits=P4 + 2), *SIZES], ids=str)

@@ -79,7 +79,7 @@ def peaked(rng, rows, vocab):
     return x
 
 
-@pytest.mark.parametrize("vocab", [1, 2, 3, 5, 31, 127, 1000, 2045, 2046, 4097, 16381, 50001, 131072, 393213])
+@pytest.mark.parametrize("vocab", [1, 2, 3, 5, 31, 127, 1000, 2045, 2046, 4097, 16381, 50001, 131072, 360445])
 def test_vocabularies(L, vocab):
     rng = np.random.default_rng(vocab)
     n = len(SETTINGS) if vocab <= 50001 else 6
