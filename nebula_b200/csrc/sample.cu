@@ -8,7 +8,7 @@
 //             until their sum reaches top_p of those, none below min_p of the largest
 //     token   the first index at which the running sum of the kept exceeds u times their sum
 // A set that is kept is always "all logits above a key, and those at the key up to an index". The key is found by counts (top-k)
-// or sums (top-p) over 256 bins, first of the distance to the maximum, then of the bits of the keys that are left; as soon as
+// or sums (top-p) over 128 bins, first of the distance to the maximum, then of the bits of the keys that are left; as soon as
 // 1024 logits are left, every CTA reads them all and goes on alone.
 //
 // Weights are evaluated in 64 bits and summed as whole numbers: borders are compared exactly, and neither the cluster's
@@ -21,7 +21,8 @@ using namespace nb;
 namespace {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kBins = 256;
+constexpr int kBins = 128;
+constexpr int kFine = 1024;                       // bins of the nucleus, in groups of 32
 constexpr int kFew = 256;                         // logits that are ordered one by one
 constexpr int kList = 1024;                       // logits that every CTA has a list of
 constexpr int kStep = kThreads * 4;               // a CTA's part of a row is a multiple of this: a thread has whole units of four
@@ -30,7 +31,7 @@ constexpr int kMaxRanks = 8;                      // CTAs of a cluster
 constexpr int kMaxVocab = kMaxRanks * kMaxUnits * kStep;
 constexpr int kRowsAtOnce = 1 << 20;
 static_assert(kMaxVocab <= 1 << 19, "sums of weights, 2^44 at most, fit 63 bits");
-static_assert(2 * kFew <= kThreads && kBins <= kThreads, "two threads to a logit that is ordered, one to a bin");
+static_assert(kMaxRanks == 8 && 2 * kFew <= kThreads && 4 * kBins == kThreads, "two threads to a logit that is ordered, four to a bin");
 
 struct SampleArgs {
     const float *logits, *uniforms, *temperature, *top_p, *min_p;
@@ -47,11 +48,19 @@ struct Shared {
     float most[kMaxRanks], least[kMaxRanks];
     int index[kMaxRanks], last[2];
     Whole total[2][kMaxRanks];         // by the parity of the exchange: a CTA may be one ahead
-    unsigned hist[2][4][kBins];        // by the parity of the pass: counts; sums as 15 + 15 + 14 bits
+    unsigned hist[2][3][kBins];        // by the parity of the pass: counts, or sums as 15 + 15 + 14 bits
     Whole list[kList];                 // key and inverted index: the larger is the better
     int listed;
+    unsigned fine[3][kFine];           // sums in the same parts
+    Whole coarse[kFine / 32];
     // a CTA's own
-    Whole warp_sum[kWarps], entry[kList], entry_weight[kFew];
+    Whole warp_sum[kWarps], entry_weight[kFew];
+    union {
+        Whole entry[kList];
+        struct {  // until a list is read
+            Whole bins[4][kBins], read[2][kMaxRanks][32];
+        };
+    };
     Whole found, kept_sum;
     int few;
     float warp_most[kWarps], warp_least[kWarps];
@@ -142,9 +151,10 @@ struct Row {
             f(x.x, at), f(x.y, at + 1), f(x.z, at + 2), f(x.w, at + 3);
         }
     }
-    // f(x, index, n) for those from low to high only, n of four at a time (the others are -infinity). They are looked for first,
-    // 32 logits at a time: a warp then takes as many turns as its fullest lane has logits, and not one for every place at which
-    // some lane has one; four at a time hide each other's latency.
+    // f(x, index) for two of those from low to high at a time (-infinity where there is none). They are looked for first, 32
+    // logits at a time: a warp then takes as many turns as its fullest lane has logits, and not one for every place at which
+    // some lane has one. (A list of a warp's logits that its lanes share evenly takes longer than it saves: nucleus of 0.98 at
+    // temperature 1, 34 us in all against 53.)
     template <typename F>
     __device__ __forceinline__ void some(float low, float high, F f) const {
         for (int j0 = 0; j0 < units; j0 += 8) {
@@ -153,49 +163,57 @@ struct Row {
             for (int j = 0; j < 8; j++)
                 if (j0 + j < units) {
                     const float4 x = mine[j0 + j];
-                    found |= (unsigned)(x.x >= low && x.x <= high) << (4 * j) | (unsigned)(x.y >= low && x.y <= high) << (4 * j + 1) |
-                             (unsigned)(x.z >= low && x.z <= high) << (4 * j + 2) | (unsigned)(x.w >= low && x.w <= high) << (4 * j + 3);
+                    if (x.x >= low && x.x <= high) found |= 1u << (4 * j);
+                    if (x.y >= low && x.y <= high) found |= 2u << (4 * j);
+                    if (x.z >= low && x.z <= high) found |= 4u << (4 * j);
+                    if (x.w >= low && x.w <= high) found |= 8u << (4 * j);
                 }
             while (found) {
-                float x[4];
-                int at[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int b = found ? __ffs(found) - 1 + 4 * j0 : 0;
-                    x[e] = found ? reinterpret_cast<const float *>(mine)[b] : -INFINITY;
-                    at[e] = index + b;
-                    found &= found - 1;
-                }
+                float x[2];
+                int at[2];
+                const int a = __ffs(found) - 1;
+                found &= found - 1;
+                const int b = found ? __ffs(found) - 1 : a;
+                const float *from = reinterpret_cast<const float *>(mine + j0);
+                x[0] = from[a], x[1] = found ? from[b] : -INFINITY;
+                found &= found - 1;
+                at[0] = index + 4 * j0 + a, at[1] = index + 4 * j0 + b;
                 f(x, at);
             }
         }
     }
-    // The sum of the weights that are kept.
+    // f(x, index, weight) for four neighbouring logits at a time, where some of the warp's are at or above low (and weigh something).
+    template <typename F>
+    __device__ __forceinline__ void each_weight(float low, F f) const {
+        low = fmaxf(low, zero);
+#pragma unroll 2
+        for (int j = 0; j < units; j++) {
+            const float4 x = mine[j];
+            if (!__any_sync(0xffffffffu, fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)) >= low)) continue;
+            const float y[4] = {x.x, x.y, x.z, x.w};
+            const Whole w[4] = {weigh(x.x), weigh(x.y), weigh(x.z), weigh(x.w)};
+            f(y, index + 4 * j, w);
+        }
+    }
+    // The thread's sum of the weights that are kept.
     __device__ __forceinline__ Whole kept_sum() const {
         Whole sum = 0;
-        if (key == kNone) {
-#pragma unroll 2
-            for (int j = 0; j < units; j++) {
-                const float4 x = mine[j];
-                if (__any_sync(0xffffffffu, fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)) >= zero)) sum += (weigh(x.x) + weigh(x.y)) + (weigh(x.z) + weigh(x.w));
-            }
-        } else {
-            some(fmaxf(floor(), zero), most, [&](const float (&x)[4], const int (&at)[4]) {
-                Whole w[4];
+        const float low = floor();
+        each_weight(low, [&](const float (&x)[4], int at, const Whole (&w)[4]) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) w[e] = weigh(x[e]);
-#pragma unroll
-                for (int e = 0; e < 4; e++) sum += keeps(x[e], at[e]) ? w[e] : 0;
-            });
-        }
+            for (int e = 0; e < 4; e++)
+                if (x[e] > low || (x[e] == low && at + e <= last)) sum += w[e];
+        });
         return sum;
     }
+    // Of logits from floor() up, and -infinity: those that are kept.
+    __device__ __forceinline__ bool kept_of_floor(float x, int i) const { return x > floor() || (x == floor() && i <= last); }
     __device__ __forceinline__ bool keeps(float x, int i) const {
         const unsigned k = key_of(x);
         return k > key || (k == key && i <= last);
     }
-    // The lowest logit that may be kept.
-    __device__ __forceinline__ float floor() const { return key == kNone ? kLowest : of_key(key); }
+    // The lowest logit that may be kept, or -infinity.
+    __device__ __forceinline__ float floor() const { return of_key(key); }
 
     // 2^44 * 2^((x - most) * c), rounded. The polynomial of degree 9 is 2^f's Chebyshev fit on [-1/2, 1/2] (error 2^-46).
     __device__ __forceinline__ Whole weigh(float x) const {
@@ -266,13 +284,13 @@ __device__ int reach(const Shared &s, const Row &r, Whole mine, Whole before, Wh
     return -1;
 }
 
-// The thread's bin of those in the order of threads (tid < kBins) at which the running sum of `mine` reaches `target`, and the
-// sum before it, to all threads; -1 where it is not reached. `count` is given along.
+// The bin, thread tid's for tid < kBins, at which the running sum of `mine` reaches `target`, and the sum before it, to all
+// threads; -1 where it is not reached.
 struct Bin {
-    int bin, count;
+    int bin;
     Whole before;
 };
-__device__ __forceinline__ Bin reach_bin(Shared &s, Whole mine, unsigned count, Whole target) {
+__device__ __forceinline__ Bin reach_bin(Shared &s, Whole mine, Whole target) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const Whole upto_warp = warp_scan(mine);
     if (lane == 31) s.warp_sum[warp] = upto_warp;
@@ -280,30 +298,50 @@ __device__ __forceinline__ Bin reach_bin(Shared &s, Whole mine, unsigned count, 
     __syncthreads();
     const Whole of_warp = lane < kWarps ? s.warp_sum[lane] : 0, warps_upto = warp_scan(of_warp);
     const Whole upto = upto_warp + __shfl_sync(0xffffffffu, warps_upto - of_warp, warp);
-    if (upto >= target && upto - mine < target) s.found = (Whole)count << 32 | (unsigned)tid, s.kept_sum = upto - mine;
+    if (upto >= target && upto - mine < target) s.found = tid, s.kept_sum = upto - mine;
     __syncthreads();
-    const Whole found = s.found;
-    return {found == ~0ull ? -1 : (int)(found & 0xffffffffu), (int)(found >> 32), s.kept_sum};
+    return {(int)s.found, s.kept_sum};
 }
-// Adds a weight to a histogram's bin. Each part's sum over a CTA's logits (or a list's) fits 32 bits.
-__device__ __forceinline__ void add_weight(unsigned (&hist)[4][kBins], int bin, Whole w) {
-    atomicAdd(&hist[1][bin], (unsigned)w & 0x7fffu);
-    atomicAdd(&hist[2][bin], (unsigned)(w >> 15) & 0x7fffu);
-    atomicAdd(&hist[3][bin], (unsigned)(w >> 30));
+// A histogram counts, or adds up weights in three parts: each part's sum over a CTA's logits fits 32 bits.
+using Hist = unsigned[3][kBins];
+template <bool SUM>
+__device__ __forceinline__ void add_to(Hist &hist, int bin, Whole w) {
+    if (SUM) {
+        atomicAdd(&hist[0][bin], (unsigned)w & 0x7fffu);
+        atomicAdd(&hist[1][bin], (unsigned)(w >> 15) & 0x7fffu);
+        atomicAdd(&hist[2][bin], (unsigned)(w >> 30));
+    } else {
+        atomicAdd(&hist[0][bin], 1u);
+    }
+}
+// One histogram of all CTAs' added up: bin tid's, for tid < kBins. Four threads to a bin read, two CTAs' each.
+template <bool SUM>
+__device__ __forceinline__ Whole all_bins(Shared &s, const Row &r, const Hist &hist) {
+    const int bin = threadIdx.x % kBins, group = threadIdx.x / kBins;
+    constexpr int N = SUM ? 3 : 1;
+    unsigned part[2][N];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const uint32_t q = 2 * group + i;
+#pragma unroll
+        for (int e = 0; e < N; e++) part[i][e] = q < r.ranks ? peer_load(at_rank(&hist[e][bin], q)) : 0;
+    }
+    Whole sum = (Whole)part[0][0] + part[1][0];
+    if constexpr (SUM) sum += (((Whole)part[0][1] + part[1][1]) << 15) + (((Whole)part[0][2] + part[1][2]) << 30);
+    s.bins[group][bin] = sum;
+    __syncthreads();
+    return threadIdx.x < kBins ? (s.bins[0][bin] + s.bins[1][bin]) + (s.bins[2][bin] + s.bins[3][bin]) : 0;
 }
 // Keys from low to high, and of these the logits whose distance from the largest falls into `bin` (-1: any).
 struct Range {
     unsigned low, high;
     float most, scale;
-    int bin;
-    __device__ __forceinline__ int bin_of(float x) const { return min(kBins - 1, (int)((most - x) * scale)); }
-    __device__ __forceinline__ bool has(float x) const {
-        const unsigned k = key_of(x);
-        return k >= low && k <= high && (bin < 0 || bin_of(x) == bin);
-    }
+    int last_bin, bin;
+    __device__ __forceinline__ int bin_of(float x) const { return min(last_bin, (int)((most - x) * scale)); }
+    __device__ __forceinline__ bool has(float x) const { return bin < 0 || bin_of(x) == bin; }  // of those between low and high
     // Only what is in distance bin b. The keys' limits are wider than the bin by more than bin_of rounds.
     __device__ __forceinline__ void take_bin(int b) {
-        if (b < kBins - 1) low = max(low, key_of(__double2float_rd((double)most - (b + 1) * 1.000001 / (double)scale)));
+        if (b < last_bin) low = max(low, key_of(__double2float_rd((double)most - (b + 1) * 1.000001 / (double)scale)));
         if (b) high = min(high, key_of(__double2float_ru((double)most - b * 0.999999 / (double)scale)));
         bin = b;
     }
@@ -313,17 +351,17 @@ struct Range {
         const unsigned span = (1u << shift) - 1;
         low = high - low > span ? high - span : low;
     }
-    __device__ __forceinline__ int shift() const { return max(0, 24 - __clz(high - low)); }  // (high - low) >> shift < kBins
+    __device__ __forceinline__ int shift() const { return max(0, 25 - __clz(high - low)); }  // (high - low) >> shift < kBins
 };
 
 // The kept logits in a range, of all CTAs and in any order, in s.entry. Returns their number; more than kList are not listed.
 // s.listed is zero before.
 __device__ int gather(Shared &s, const Row &r, const Range &in) {
     const int tid = threadIdx.x;
-    r.some(of_key(max(in.low, kNone + 1)), of_key(in.high), [&](const float (&x)[4], const int (&at)[4]) {
+    r.some(of_key(max(in.low, kNone + 1)), of_key(in.high), [&](const float (&x)[2], const int (&at)[2]) {
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (r.keeps(x[e], at[e]) && in.has(x[e])) {
+        for (int e = 0; e < 2; e++)
+            if (r.kept_of_floor(x[e], at[e]) && in.has(x[e])) {
                 const int to = atomicAdd(&s.listed, 1);
                 if (to < kList) s.list[to] = (Whole)key_of(x[e]) << 32 | (unsigned)~at[e];
             }
@@ -368,7 +406,7 @@ __device__ __forceinline__ int order(Shared &s, const Row &r, int n, Whole &abov
 // Of the n entries (they are the kept logits in a range): the one at which the running count, or sum, from the best on reaches
 // `target`. `hist` is zero before and after. In every CTA by itself.
 template <bool SUM>
-__device__ Whole nth_entry(Shared &s, const Row &r, int n, Range in, Whole target, unsigned (&hist)[4][kBins]) {
+__device__ Whole nth_entry(Shared &s, const Row &r, int n, Range in, Whole target, Hist &hist) {
     const int tid = threadIdx.x;
     static_assert(kList == 2 * kThreads, "two entries to a thread");
     while (n > kFew && in.low < in.high) {
@@ -378,21 +416,18 @@ __device__ Whole nth_entry(Shared &s, const Row &r, int n, Range in, Whole targe
             mine[i] = tid + i * kThreads < n ? s.entry[tid + i * kThreads] : 0;
             if (mine[i]) {
                 const int bin = (int)((in.high - (unsigned)(mine[i] >> 32)) >> in.shift());
-                atomicAdd(&hist[0][bin], 1u);
-                if (SUM) add_weight(hist, bin, r.weigh(of_key((unsigned)(mine[i] >> 32))));
+                add_to<SUM>(hist, bin, SUM ? r.weigh(of_key((unsigned)(mine[i] >> 32))) : 1);
             }
         }
-        if (tid == 0) s.few = 0;
         __syncthreads();
+        if (tid == 0) s.few = 0;
         Whole sum = 0;
-        unsigned count = 0;
         if (tid < kBins) {
-            count = hist[0][tid];
-            sum = SUM ? hist[1][tid] + ((Whole)hist[2][tid] << 15) + ((Whole)hist[3][tid] << 30) : count;
+            sum = hist[0][tid] + ((Whole)hist[1][tid] << 15) + ((Whole)hist[2][tid] << 30);  // (counts: the other parts are zero)
 #pragma unroll
-            for (int e = 0; e < 4; e++) hist[e][tid] = 0;
+            for (int e = 0; e < 3; e++) hist[e][tid] = 0;
         }
-        const Bin b = reach_bin(s, sum, count, target);
+        const Bin b = reach_bin(s, sum, target);
         const int shift = in.shift();
         target -= b.before;
         in.take_keys(b.bin, shift);
@@ -402,7 +437,7 @@ __device__ Whole nth_entry(Shared &s, const Row &r, int n, Range in, Whole targe
             if (mine[i] && k >= in.low && k <= in.high) s.entry[atomicAdd(&s.few, 1)] = mine[i];
         }
         __syncthreads();
-        n = b.count;
+        n = s.few;
     }
     if (n <= kFew) {
         Whole above;
@@ -427,57 +462,35 @@ __device__ Whole nth_entry(Shared &s, const Row &r, int n, Range in, Whole targe
     return s.found;
 }
 
-// Narrows the kept set to its largest logits: `target` of them (SUM: as many as it takes until their weights reach it). None
-// that is wanted lies below `lowest`.
+// Narrows the kept set to its largest logits: of those in a range, `target` (SUM: as many as it takes until their weights reach
+// it). linear: the first bins are distances.
 template <bool SUM>
-__device__ void narrow(Shared &s, Row &r, Whole target, float lowest, int &pass, int &turn) {
+__device__ void narrow(Shared &s, Row &r, Whole target, Range in, bool linear, int &pass, int &turn) {
     const int tid = threadIdx.x, lane = tid & 31;
-    lowest = fmaxf(lowest, r.floor());
-    Range in = {key_of(lowest), key_of(r.most), r.most, fminf(kBins / (r.most - lowest), 1e30f), -1};
-    for (bool linear = true; linear || in.low < in.high; linear = false) {
+    for (; linear || in.low < in.high; linear = false) {
         const int shift = in.shift();
-        unsigned (&hist)[4][kBins] = s.hist[pass & 1], (&other)[4][kBins] = s.hist[~pass & 1];  // (zeros)
-        r.some(of_key(max(in.low, kNone + 1)), of_key(in.high), [&](const float (&x)[4], const int (&at)[4]) {
-            Whole w[4];
+        Hist &hist = s.hist[pass & 1], &other = s.hist[~pass & 1];  // (zeros)
+        r.some(of_key(max(in.low, kNone + 1)), of_key(in.high), [&](const float (&x)[2], const int (&at)[2]) {
+            const Whole w[2] = {SUM ? r.weigh(x[0]) : 1, SUM ? r.weigh(x[1]) : 1};
 #pragma unroll
-            for (int e = 0; e < 4; e++) w[e] = SUM ? r.weigh(x[e]) : 0;
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (r.keeps(x[e], at[e]) && in.has(x[e])) {
-                    const int bin = linear ? in.bin_of(x[e]) : (int)((in.high - key_of(x[e])) >> shift);
-                    atomicAdd(&hist[0][bin], 1u);
-                    if (SUM) add_weight(hist, bin, w[e]);
-                }
+            for (int e = 0; e < 2; e++)
+                if (r.kept_of_floor(x[e], at[e]) && in.has(x[e]))
+                    add_to<SUM>(hist, linear ? in.bin_of(x[e]) : (int)((in.high - key_of(x[e])) >> shift), w[e]);
         });
         cluster_sync();
-        // every CTA adds up all bins of all, one bin to a thread
-        Whole mine = 0;
-        unsigned count = 0;
-        if (tid < kBins) {
-            unsigned part[SUM ? 4 : 1][kMaxRanks];
-#pragma unroll
-            for (int q = 0; q < kMaxRanks; q++)
-#pragma unroll
-                for (int e = 0; e < (SUM ? 4 : 1); e++) part[e][q] = q < r.ranks ? peer_load(at_rank(&hist[e][tid], q)) : 0;
-#pragma unroll
-            for (int q = 0; q < kMaxRanks; q++) {
-                count += part[0][q];
-                if constexpr (SUM) mine += part[1][q] + ((Whole)part[2][q] << 15) + ((Whole)part[3][q] << 30);
-            }
-            if (!SUM) mine = count;
-        }
+        const Whole mine = all_bins<SUM>(s, r, hist);
         // the other histogram, and the list, were read before this pass's barrier
-        for (int i = tid; i < 4 * kBins; i += kThreads) other[0][i] = 0;
+        for (int i = tid; i < 3 * kBins; i += kThreads) other[0][i] = 0;
         if (tid == 0) s.listed = 0;
         pass++;
-        const Bin b = reach_bin(s, mine, count, target);
+        const Bin b = reach_bin(s, mine, target);
         if (b.bin < 0) return;  // all of them
         target -= b.before;
         if (linear) in.take_bin(b.bin);
         else in.take_keys(b.bin, shift);
-        if (b.count <= kList) {
-            gather(s, r, in);
-            const Whole worst = nth_entry<SUM>(s, r, b.count, in, target, other);
+        const int n = gather(s, r, in);
+        if (n <= kList) {
+            const Whole worst = nth_entry<SUM>(s, r, n, in, target, other);
             r.key = (unsigned)(worst >> 32), r.last = (int)~(unsigned)worst;
             return;
         }
@@ -498,24 +511,89 @@ __device__ void narrow(Shared &s, Row &r, Whole target, float lowest, int &pass,
     r.last = s.last[SUM];
 }
 
+// The whole number that a sum must reach to be at least p of `all`.
+__device__ __forceinline__ Whole share_of(float p, Whole all) {
+    const Whole share = p > 0.0f ? __double2ull_rz((double)p * 18446744073709551616.0) : 0;
+    return max(__umul64hi(share, all) + (share * all != 0), 1ull);
+}
+// How far below the largest weight, in octaves, a logit must lie so that all of them there together are less than what top-p
+// leaves out. The sum is one largest weight at least.
+__device__ __forceinline__ float octaves_of(float p, int vocab) { return log2f((float)vocab) - log2f(1.0f - fmaxf(p, 0.0f)) + 1.0f; }
+
+// Top-p of a whole row: the sum of all weights and the bins of those that may matter, none of which lie below `end`, in one pass.
+__device__ void nucleus(Shared &s, Row &r, float p, float end, int &pass, int &turn) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    Range in = {key_of(end), key_of(r.most), r.most, fminf(kFine / (r.most - end), 1e30f), kFine - 1, -1};
+    for (int i = tid; i < 3 * kFine; i += kThreads) s.fine[0][i] = 0;
+    __syncthreads();
+    Whole sum = 0;
+    r.each_weight(-INFINITY, [&](const float (&x)[4], int, const Whole (&w)[4]) {
+        sum += (w[0] + w[1]) + (w[2] + w[3]);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (x[e] >= end) {
+                const int bin = in.bin_of(x[e]);
+                atomicAdd(&s.fine[0][bin], (unsigned)w[e] & 0x7fffu);
+                atomicAdd(&s.fine[1][bin], (unsigned)(w[e] >> 15) & 0x7fffu);
+                atomicAdd(&s.fine[2][bin], (unsigned)(w[e] >> 30));
+            }
+    });
+    __syncthreads();
+#pragma unroll
+    for (int g = warp; g < kFine / 32; g += kWarps) {
+        const int bin = 32 * g + lane;
+        const Whole of_group = warp_sum(s.fine[0][bin] + ((Whole)s.fine[1][bin] << 15) + ((Whole)s.fine[2][bin] << 30));
+        if (lane == 0) s.coarse[g] = of_group;
+    }
+    share_sums(s, r, sum, turn);
+    Whole all;
+    sums_before(s, r, turn, all);
+    turn++;
+    Whole target = share_of(p, all);
+    // the group, then the bin in it; a warp reads one CTA's, and every warp looks for it
+    auto find = [&](Whole (&from)[kMaxRanks][32], Whole &target) {
+        __syncthreads();
+        Whole mine = 0;
+#pragma unroll
+        for (int q = 0; q < kMaxRanks; q++) mine += from[q][lane];
+        const Whole upto = warp_scan(mine);
+        const unsigned past = __ballot_sync(0xffffffffu, upto >= target);
+        if (!past) return -1;
+        const int l = __ffs(past) - 1;
+        target -= __shfl_sync(0xffffffffu, upto - mine, l);
+        return l;
+    };
+    if (warp < kMaxRanks) s.read[0][warp][lane] = warp < r.ranks ? peer_load64(at_rank(&s.coarse[lane], warp)) : 0;
+    const int group = find(s.read[0], target);
+    if (group < 0) return;  // all of them
+    if (warp < kMaxRanks) {
+        unsigned part[3] = {0, 0, 0};
+        if (warp < r.ranks)
+#pragma unroll
+            for (int e = 0; e < 3; e++) part[e] = peer_load(at_rank(&s.fine[e][32 * group + lane], warp));
+        s.read[1][warp][lane] = part[0] + ((Whole)part[1] << 15) + ((Whole)part[2] << 30);
+    }
+    in.take_bin(32 * group + find(s.read[1], target));
+    const int n = gather(s, r, in);
+    if (n <= kList) {
+        const Whole worst = nth_entry<true>(s, r, n, in, target, s.hist[pass & 1]);
+        r.key = (unsigned)(worst >> 32), r.last = (int)~(unsigned)worst;
+    } else {
+        narrow<true>(s, r, target, in, false, pass, turn);
+    }
+}
+
 // A lower bound of the k-th largest logit, from the largest of each thread's (k logits are at least as large as the k-th
 // largest of these); -infinity where there is none.
 __device__ float bound_of(Shared &s, const Row &r, int k, float threads_most, float least, int &pass) {
     const int tid = threadIdx.x;
-    Range in = {kNone, key_of(r.most), r.most, fminf((kBins - 1) / (r.most - least), 1e30f), -1};
-    unsigned *hist = s.hist[pass & 1][0];
-    if (threads_most >= least) atomicAdd(&hist[in.bin_of(threads_most)], 1u);
+    Range in = {kNone, key_of(r.most), r.most, fminf((kBins - 1) / (r.most - least), 1e30f), kBins - 1, -1};
+    Hist &hist = s.hist[pass & 1];
+    if (threads_most >= least) add_to<false>(hist, in.bin_of(threads_most), 1);
     cluster_sync();
-    unsigned count = 0;
-    if (tid < kBins) {
-        unsigned part[kMaxRanks];
-#pragma unroll
-        for (int q = 0; q < kMaxRanks; q++) part[q] = q < r.ranks ? peer_load(at_rank(&hist[tid], q)) : 0;
-#pragma unroll
-        for (int q = 0; q < kMaxRanks; q++) count += part[q];
-    }
+    const Whole count = all_bins<false>(s, r, hist);
     pass++;  // (the next pass clears this histogram)
-    const Bin b = reach_bin(s, count, count, k);
+    const Bin b = reach_bin(s, count, k);
     if (b.bin < 0) return -INFINITY;
     in.take_bin(b.bin);
     return of_key(in.low);
@@ -537,7 +615,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     const int ahead = (int)(reinterpret_cast<uintptr_t>(x0) >> 2 & 3);  // logits between a multiple of 16 bytes and the row
     const int start = (int)r.rank * a.units * kStep - ahead;
     r.index = start + tid * 4 * a.units;
-    for (int i = tid; i < 2 * 4 * kBins; i += kThreads) s.hist[0][0][i] = 0;
+    for (int i = tid; i < 2 * 3 * kBins; i += kThreads) s.hist[0][0][i] = 0;
     if (tid == 0) s.listed = 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const float t = a.temperature ? a.temperature[user] : 1.0f, p = a.top_p ? a.top_p[user] : 1.0f, least = a.min_p ? a.min_p[user] : 0.0f;
@@ -604,6 +682,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     const bool refused = !(most > -INFINITY && most < INFINITY) || !(t >= 0.0f && t < INFINITY) || p != p || least != least || u != u;
 
     // ---- what is kept
+    auto bins_down_to = [&](float x) { return fminf(kBins / (most - x), 1e30f); };
     int turn = 0, pass = 0;
     r.most = most;
     r.top = most;
@@ -619,9 +698,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     if (refused) {
     } else if (t == 0.0f) {  // the largest logit, the lowest index of equals
         int index = 0x7fffffff;
-        r.some(most, most, [&](const float (&x)[4], const int (&at)[4]) {
+        r.some(most, most, [&](const float (&x)[2], const int (&at)[2]) {
 #pragma unroll
-            for (int e = 0; e < 4; e++)
+            for (int e = 0; e < 2; e++)
                 if (x[e] == most) index = min(index, at[e]);
         });
         index = __reduce_min_sync(0xffffffffu, index);
@@ -639,7 +718,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         bool done = false;
         if (k > 0 && k < a.vocab) {
             const float bound = bound_of(s, r, k, threads_most, lowest, pass);
-            const int n = k <= kFew ? gather(s, r, {key_of(fmaxf(bound, kLowest)), key_of(most), most, 0.0f, -1}) : kFew + 1;
+            const int n = k <= kFew ? gather(s, r, {key_of(fmaxf(bound, kLowest)), key_of(most), most, 0.0f, 0, -1}) : kFew + 1;
             if (n <= kFew) {
                 // few enough: all of the rest is in every CTA's own memory
                 Whole above;
@@ -649,9 +728,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
                 __syncthreads();
                 bool stays = one && better < k;
                 if (p < 1.0f) {
-                    const Whole share = p > 0.0f ? __double2ull_rz((double)p * 18446744073709551616.0) : 0, all = s.kept_sum;
-                    const Whole target = __umul64hi(share, all) + (share * all != 0);
-                    stays = stays && (above < target || better == 0);
+                    const Whole target = share_of(p, s.kept_sum);
+                    stays = stays && above < target;
                 }
                 stays = stays && (unsigned)(s.entry[min(me, n - 1)] >> 32) >= min_key;
                 const int kept = __syncthreads_count(stays);
@@ -680,20 +758,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
                     return;
                 }
             } else {
-                narrow<false>(s, r, k, bound, pass, turn);
+                narrow<false>(s, r, k, {key_of(bound), key_of(most), most, bins_down_to(fmaxf(bound, lowest)), kBins - 1, -1}, true, pass, turn);
             }
         }
         if (!done && p < 1.0f) {
-            Whole all;
-            share_sums(s, r, r.kept_sum(), turn);
-            sums_before(s, r, turn, all);
-            turn++;
-            const Whole share = p > 0.0f ? __double2ull_rz((double)p * 18446744073709551616.0) : 0;
-            const Whole target = __umul64hi(share, all) + (share * all != 0);
-            // What lies a factor of vocab / (what may be left out) below the largest cannot reach into it.
-            const float left = (1.0f - fmaxf(p, 0.0f)) * (float)all * (1.0f / 17592186044416.0f);
-            const float octaves = fminf(fmaxf(log2f((float)a.vocab) - log2f(left) + 1.0f, 1.0f), 46.0f);
-            narrow<true>(s, r, target > 1 ? target : 1, fmaxf((float)(r.top - octaves / r.c), kLowest), pass, turn);
+            const float octaves = fminf(octaves_of(p, a.vocab), 46.0f), end = fmaxf((float)(r.top - octaves / r.c), kLowest);
+            if (r.key == kNone) {
+                nucleus(s, r, p, end, pass, turn);
+            } else {
+                Whole all;
+                share_sums(s, r, r.kept_sum(), turn);
+                sums_before(s, r, turn, all);
+                turn++;
+                narrow<true>(s, r, share_of(p, all), {max(key_of(end), r.key), key_of(most), most, bins_down_to(fmaxf(end, r.floor())), kBins - 1, -1},
+                             true, pass, turn);
+            }
         }
         if (!done && min_key > r.key) r.key = min_key, r.last = 0x7fffffff;
     }
