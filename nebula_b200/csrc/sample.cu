@@ -23,7 +23,8 @@ namespace {
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 128;
 constexpr int kFine = 1024;                       // bins of the nucleus, in groups of 32
-constexpr int kFew = 256;                         // logits that are ordered one by one
+constexpr int kFew = 256;                         // logits of top-k that are ordered one by one
+constexpr int kFewer = 64;                        // the same where one of a list is looked for
 constexpr int kList = 1024;                       // logits that every CTA has a list of
 constexpr int kStep = kThreads * 4;               // a CTA's part of a row is a multiple of this: a thread has whole units of four
 constexpr int kMaxUnits = 22;                     // of a thread: 188 KB a CTA
@@ -38,7 +39,7 @@ struct SampleArgs {
     const int *top_k;
     float *out;
     int *token;
-    int per, vocab, units;
+    int per, rows, vocab, units;
 };
 
 using Whole = unsigned long long;
@@ -409,7 +410,7 @@ template <bool SUM>
 __device__ Whole nth_entry(Shared &s, const Row &r, int n, Range in, Whole target, Hist &hist) {
     const int tid = threadIdx.x;
     static_assert(kList == 2 * kThreads, "two entries to a thread");
-    while (n > kFew && in.low < in.high) {
+    while (n > kFewer && in.low < in.high) {
         Whole mine[2];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
@@ -439,7 +440,7 @@ __device__ Whole nth_entry(Shared &s, const Row &r, int n, Range in, Whole targe
         __syncthreads();
         n = s.few;
     }
-    if (n <= kFew) {
+    if (n <= kFewer) {
         Whole above;
         const int better = order(s, r, n, above);
         if (!(tid & 1) && tid / 2 < n && (SUM ? above < target && above + s.entry_weight[tid / 2] >= target : (Whole)better + 1 == target))
@@ -599,25 +600,16 @@ __device__ float bound_of(Shared &s, const Row &r, int k, float threads_most, fl
     return of_key(in.low);
 }
 
-__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a) {
-    extern __shared__ __align__(16) unsigned char smem[];
-    const int stride = a.units | 1;
-    float4 *const part = reinterpret_cast<float4 *>(smem);
-    Shared &s = *reinterpret_cast<Shared *>(part + kThreads * stride);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");  // a CTA's memory is there for others once it runs
-    Row r;
-    r.rank = cluster_rank(), r.ranks = cluster_size();
-    r.units = a.units;
-    r.mine = part + tid * stride;
-    const int row = blockIdx.x / r.ranks, user = row / a.per;
+// One row, by one cluster.
+__device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *part, Row &r, int row, int next) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, stride = a.units | 1;
+    const int user = row / a.per;
     const float *const x0 = a.logits + (size_t)row * a.vocab;
     const int ahead = (int)(reinterpret_cast<uintptr_t>(x0) >> 2 & 3);  // logits between a multiple of 16 bytes and the row
     const int start = (int)r.rank * a.units * kStep - ahead;
     r.index = start + tid * 4 * a.units;
     for (int i = tid; i < 2 * 3 * kBins; i += kThreads) s.hist[0][0][i] = 0;
     if (tid == 0) s.listed = 0;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     const float t = a.temperature ? a.temperature[user] : 1.0f, p = a.top_p ? a.top_p[user] : 1.0f, least = a.min_p ? a.min_p[user] : 0.0f;
     const int k = a.top_k ? a.top_k[user] : 0;
     const float u = a.uniforms ? a.uniforms[row] : 0.0f;
@@ -653,6 +645,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
                 }
         }
     }
+    if (next < a.rows) {  // the cluster's next row comes to L2 meanwhile
+        const float *const x1 = a.logits + (size_t)next * a.vocab;
+        for (int i = max(0, start) + tid * 32; i < min(a.vocab, start + a.units * kStep); i += kThreads * 32)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(x1 + i));
+    }
     const float threads_most = most;
     float lowest = most > -INFINITY ? most : INFINITY;  // of the threads' largest
 #pragma unroll
@@ -662,7 +659,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     }
     if (lane == 0) s.warp_most[warp] = most, s.warp_least[warp] = lowest;
     __syncthreads();
-    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     if (warp == 0) {
         most = lane < kWarps ? s.warp_most[lane] : -INFINITY;
         lowest = lane < kWarps ? s.warp_least[lane] : INFINITY;
@@ -753,8 +749,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
                         if (one && entry >= worst && before < aim && before + s.entry_weight[me] >= aim && r.rank == 0)
                             a.token[row] = (int)~(unsigned)entry;
                     }
-                    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");  // no CTA ends while others read its list
-                    asm volatile("barrier.cluster.wait;" ::: "memory");
                     return;
                 }
             } else {
@@ -795,7 +789,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         if (index >= 0 && lane == 0) a.token[row] = index;
         return;
     }
-    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");  // no CTA ends while others read its memory
     float *const out = a.out + (size_t)row * a.vocab;
     const float other = refused ? __int_as_float(0x7fc00000) : -INFINITY;
     const bool whole = !((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(x0)) & 15);
@@ -815,7 +808,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
             if (i + 3 >= 0 && i + 3 < a.vocab) out[i + 3] = x.w;
         }
     }
-    asm volatile("barrier.cluster.wait;" ::: "memory");
+}
+
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    float4 *const part = reinterpret_cast<float4 *>(smem);
+    Shared &s = *reinterpret_cast<Shared *>(part + kThreads * (a.units | 1));
+    Row r;
+    r.rank = cluster_rank(), r.ranks = cluster_size();
+    r.units = a.units;
+    r.mine = part + threadIdx.x * (a.units | 1);
+    cluster_sync();  // a CTA's memory is there for others once it runs
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int clusters = gridDim.x / r.ranks;
+    for (int row = blockIdx.x / r.ranks; row < a.rows; row += clusters) {
+        do_row(a, s, part, r, row, row + clusters);
+        cluster_sync();  // no CTA goes on, or ends, while others read its memory
+    }
 }
 
 int launch(SampleArgs &a, int rows) {
@@ -827,8 +836,8 @@ int launch(SampleArgs &a, int rows) {
     a.units = ((long_row + ranks - 1) / ranks + kStep - 1) / kStep;
     const int smem = kThreads * (a.units | 1) * 16 + (int)sizeof(Shared);
     if (int rc = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return rc;
+    a.rows = rows;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)rows * ranks);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = launch_stream;
@@ -840,6 +849,12 @@ int launch(SampleArgs &a, int rows) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
+    // as many clusters as fit at once
+    int clusters = 0;
+    cfg.gridDim = dim3(ranks);
+    if (rows > 1)
+        if (int rc = cudaOccupancyMaxActiveClusters(&clusters, sample_kernel, &cfg)) return rc;
+    cfg.gridDim = dim3((unsigned)(rows < clusters ? rows : clusters > 1 ? clusters : 1) * ranks);
     return cudaLaunchKernelEx(&cfg, sample_kernel, a);
 }
 
