@@ -70,6 +70,8 @@ struct AttendArgs {
     float *prefix_acc;   // [row][q_heads][D], [row][q_heads]: of prefix items that one CTA did as a whole
     float2 *prefix_ml;
     float2 *own_ml;      // the same of sequences' items, whose sums are in out
+    long long *starts;   // [seqs + 1]: the slots before each sequence's, and all
+    int *lengths;        // [seqs + 1]: own_length, and the common positions: for the join
 };
 
 constexpr int kChunk = 32;       // keys per step of the softmax
@@ -458,6 +460,22 @@ __device__ __forceinline__ void plan(const AttendArgs &a, Plan &s, int team, int
         s.kv0 = index / tiles, s.tile0 = index % tiles;
         s.pos0 = (int)(u0 - base - (long long)index * slots);
         s.common = common, s.source = source;
+    }
+    if (SHARED && team == 0 && blockIdx.x == 0) {  // what the join needs to find every row's parts
+        long long before = line;
+        for (int s0 = 0; s0 < a.seqs; s0 += 32) {
+            const int q = s0 + lane, own = q < a.seqs ? own_length<SHARED>(a, q, shared, common) : -1;
+            const long long mine = (long long)slots_of<D>(a, own) * per;
+            long long upto = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const long long x = __shfl_up_sync(0xffffffffu, upto, d);
+                if (lane >= d) upto += x;
+            }
+            if (q < a.seqs) a.starts[q] = before + upto - mine, a.lengths[q] = own;
+            before += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (lane == 0) a.starts[a.seqs] = before, a.lengths[a.seqs] = common;
     }
 }
 
@@ -1374,9 +1392,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) token_attention_kernel(cons
 // Joins the parts of items that several CTAs share, and makes every row NaN
 // after an error: one CTA per (row, head). Warps take every eighth part, so all
 // loads of a row are in flight at once; their sums join in order.
-// With a shared prefix every row has parts: the prefix's, then its sequence's own. One that a CTA did as a whole is in the
-// rows of prefix_acc or out.
-template <int D, bool SHARED>
+template <int D>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttendArgs a, int teams) {
     constexpr int V = D / 32;
     __shared__ float sums[8][D];
@@ -1385,49 +1401,129 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Atten
     const int id = blockIdx.x, h = id % a.q_heads, row = id / a.q_heads, seq = row / a.tokens;
     const int kv = h / a.group, r = (row % a.tokens) * a.group + h % a.group, tile = r / a.tile_rows;
     const int per = a.c.kv_heads * a.row_tiles;
-    const int shared = asked_shared<SHARED>(a), common = SHARED ? common_of(a, shared, first_live(a, shared)) : 0;
-    const int own = own_length<SHARED>(a, seq, shared, common), units = units_of(a, own);
-    const long long line = SHARED ? prefix_line<D>(a, common) : 0, w = line + sum_slots<D, SHARED>(a, a.seqs, per, shared, common);
-    const long long start = line + (seq ? sum_slots<D, SHARED>(a, seq, per, shared, common) : 0) +
-                            (long long)(kv * a.row_tiles + tile) * (units + kItemCost<D>) + kItemCost<D>;
+    const int units = units_of(a, a.c.committed(seq, a.tokens));
+    const long long w = sum_slots<D, false>(a, a.seqs, per, 0, 0);
+    const long long start = (seq ? sum_slots<D, false>(a, seq, per, 0, 0) : 0) + (long long)(kv * a.row_tiles + tile) * (units + kItemCost<D>) + kItemCost<D>;
     const int g = (int)min((long long)teams, w);
     const int c0 = units ? cta_of(start, w, g) : 0, parts = units ? cta_of(start + units - 1, w, g) - c0 + 1 : 0;
-    // the prefix's parts of this row
-    const int all_r = SHARED ? row * a.group + h % a.group : 0, all_tile = all_r / a.tile_rows;
-    const long long all_start = SHARED ? (long long)(kv * a.all_tiles + all_tile) * prefix_slots<D>(common) + kItemCost<D> : 0;
-    const int p0 = common ? cta_of(all_start, w, g) : 0, before = common ? cta_of(all_start + common / kKeys - 1, w, g) - p0 + 1 : 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     float *out = a.out + (size_t)id * D;
-    if (*(volatile int *)a.err || (SHARED && own < 0)) {
+    if (*(volatile int *)a.err) {
         for (int i = threadIdx.x; i < D; i += 256) out[i] = __int_as_float(0x7fc00000);
         return;
     }
-    if (!SHARED && parts < 2) return;
-    const bool late = start > range_start(c0, w, g), all_late = SHARED && all_start > range_start(p0, w, g);  // the first part is its CTA's second
-    const int count = before + parts;
-    // where part p of the row is
-    auto part = [&](int p, const float *&acc, const float2 *&ml) {
-        const bool prefix = SHARED && p < before;
-        if (SHARED && (prefix ? before : parts) == 1) {
-            acc = (prefix ? a.prefix_acc : a.out) + (size_t)id * D, ml = (prefix ? a.prefix_ml : a.own_ml) + id;
-            return;
-        }
-        const int q = prefix ? p : p - before;
-        const size_t at = (size_t)(2 * ((prefix ? p0 : c0) + q) + (q == 0 && (prefix ? all_late : late))) * a.part_rows +
-                          (prefix ? all_r : r) % a.tile_rows;
-        acc = a.part_acc + at * D, ml = a.part_ml + at;
-    };
+    if (parts < 2) return;
     // Every warp has its own maximum; kFly parts are asked for before the first is used.
     constexpr int kFly = 5;
     float m = -INFINITY, l = 0.0f, acc[V];
 #pragma unroll
     for (int e = 0; e < V; e++) acc[e] = 0.0f;
-    for (int from = warp; from < count; from += 8 * kFly) {
+    const bool late = start > range_start(c0, w, g);  // the first part is its CTA's second
+    for (int p0 = warp; p0 < parts; p0 += 8 * kFly) {
         float2 ml[kFly];
         float x[kFly][V], top = m;
 #pragma unroll
         for (int i = 0; i < kFly; i++) {
-            const int p = from + 8 * i;
+            const int p = p0 + 8 * i;
+            ml[i] = make_float2(-INFINITY, 0.0f);
+            if (p < parts) {
+                const size_t at = (size_t)(2 * (c0 + p) + (p == 0 && late)) * a.part_rows + r % a.tile_rows;
+                const float *src = a.part_acc + at * D + lane * V;
+                ml[i] = __ldcg(a.part_ml + at);
+                if constexpr (V == 2) {
+                    *reinterpret_cast<float2 *>(x[i]) = __ldcg(reinterpret_cast<const float2 *>(src));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < V; e += 4) *reinterpret_cast<float4 *>(x[i] + e) = __ldcg(reinterpret_cast<const float4 *>(src + e));
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kFly; i++) top = fmaxf(top, ml[i].x);
+        const float keep = m == -INFINITY ? 1.0f : ex2(m - top);  // (what there is without a maximum is 0 or NaN)
+        m = top;
+        l *= keep;
+#pragma unroll
+        for (int e = 0; e < V; e++) acc[e] *= keep;
+#pragma unroll
+        for (int i = 0; i < kFly; i++) {
+            if (p0 + 8 * i >= parts) continue;
+            const float f = ml[i].x == -INFINITY ? ml[i].y : ex2(ml[i].x - m);  // its total is 0 (nothing seen) or NaN
+            l += f * ml[i].y;
+#pragma unroll
+            for (int e = 0; e < V; e++) acc[e] = fmaf(f, x[i][e], acc[e]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < V; e++) sums[warp][lane * V + e] = acc[e];
+    if (lane == 0) totals[warp] = make_float2(m, l);
+    __syncthreads();
+    m = -INFINITY, l = 0.0f;
+    float f[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) m = fmaxf(m, totals[k].x);
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        f[k] = totals[k].x == -INFINITY ? totals[k].y : ex2(totals[k].x - m);
+        l += f[k] * totals[k].y;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    for (int i = threadIdx.x; i < D; i += 256) {
+        float v = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) v = fmaf(f[k], sums[k][i], v);
+        out[i] = v * inv;
+    }
+}
+
+// With a shared prefix every row has parts: the prefix's, then its sequence's own. What a CTA did as a whole is in the rows of
+// prefix_acc or out. WARPS warps to a (row, head): eight where there are so few rows that each may have many parts, otherwise one,
+// so that all rows are under way at once (48 x 5 rows of 24 heads of 256: 85 us with eight, @ with one).
+template <int D, int WARPS>
+__global__ void __launch_bounds__(256) join_shared_kernel(const __grid_constant__ AttendArgs a, int teams) {
+    constexpr int V = D / 32, kFly = 4;  // parts that are asked for before the first is used
+    __shared__ float sums[8][D];
+    __shared__ float2 totals[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int id = WARPS == 1 ? blockIdx.x * 8 + warp : blockIdx.x;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (id >= a.seqs * a.tokens * a.q_heads) return;  // (whole warps, and no barrier with WARPS 1)
+    const int h = id % a.q_heads, row = id / a.q_heads, seq = row / a.tokens, kv = h / a.group, r = (row - seq * a.tokens) * a.group + h % a.group;
+    const long long w = a.starts[a.seqs], first = a.starts[seq];
+    const int own = a.lengths[seq], common = a.lengths[a.seqs], units = units_of(a, own), g = (int)min((long long)teams, w);
+    float *out = a.out + (size_t)id * D;
+    if (*(volatile int *)a.err || own < 0) {
+        for (int i = WARPS == 1 ? lane : threadIdx.x; i < D; i += 32 * WARPS) out[i] = __int_as_float(0x7fc00000);
+        return;
+    }
+    const long long start = first + (long long)(kv * a.row_tiles + r / a.tile_rows) * (units + kItemCost<D>) + kItemCost<D>;
+    const int c0 = cta_of(start, w, g), parts = cta_of(start + units - 1, w, g) - c0 + 1;
+    // the prefix's parts of this row
+    const int all_r = row * a.group + h % a.group;
+    const long long all_start = (long long)(kv * a.all_tiles + all_r / a.tile_rows) * prefix_slots<D>(common) + kItemCost<D>;
+    const int p0 = common ? cta_of(all_start, w, g) : 0, before = common ? cta_of(all_start + common / kKeys - 1, w, g) - p0 + 1 : 0;
+    const bool late = start > range_start(c0, w, g), all_late = all_start > range_start(p0, w, g);  // the first part is its CTA's second
+    const int count = before + parts;
+    // where part p of the row is
+    auto part = [&](int p, const float *&acc, const float2 *&ml) {
+        const bool prefix = p < before;
+        if ((prefix ? before : parts) == 1) {
+            acc = (prefix ? a.prefix_acc : a.out) + (size_t)id * D, ml = (prefix ? a.prefix_ml : a.own_ml) + id;
+            return;
+        }
+        const int q = prefix ? p : p - before;
+        const size_t at = (size_t)(2 * ((prefix ? p0 : c0) + q) + (q == 0 && (prefix ? all_late : late))) * a.part_rows + (prefix ? all_r : r) % a.tile_rows;
+        acc = a.part_acc + at * D, ml = a.part_ml + at;
+    };
+    float m = -INFINITY, l = 0.0f, acc[V];
+#pragma unroll
+    for (int e = 0; e < V; e++) acc[e] = 0.0f;
+    for (int from = WARPS == 1 ? 0 : warp; from < count; from += WARPS * kFly) {
+        float2 ml[kFly];
+        float x[kFly][V], top = m;
+#pragma unroll
+        for (int i = 0; i < kFly; i++) {
+            const int p = from + WARPS * i;
             ml[i] = make_float2(-INFINITY, 0.0f);
             if (p < count) {
                 const float *src;
@@ -1452,12 +1548,25 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Atten
         for (int e = 0; e < V; e++) acc[e] *= keep;
 #pragma unroll
         for (int i = 0; i < kFly; i++) {
-            if (from + 8 * i >= count) continue;
+            if (from + WARPS * i >= count) continue;
             const float f = ml[i].x == -INFINITY ? ml[i].y : ex2(ml[i].x - m);  // its total is 0 (nothing seen) or NaN
             l += f * ml[i].y;
 #pragma unroll
             for (int e = 0; e < V; e++) acc[e] = fmaf(f, x[i][e], acc[e]);
         }
+    }
+    if constexpr (WARPS == 1) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int e = 0; e < V; e++) acc[e] *= inv;
+        float *to = out + lane * V;
+        if constexpr (V == 2) {
+            *reinterpret_cast<float2 *>(to) = *reinterpret_cast<float2 *>(acc);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; e += 4) *reinterpret_cast<float4 *>(to + e) = *reinterpret_cast<float4 *>(acc + e);
+        }
+        return;
     }
 #pragma unroll
     for (int e = 0; e < V; e++) sums[warp][lane * V + e] = acc[e];
@@ -1507,6 +1616,8 @@ int pool_map(CUtensorMap *m, const CacheView &c, const __half *pool, int box, in
 
 int part_rows(int tokens, int group) { return tokens * group < kRows ? tokens * group : kRows; }
 
+constexpr unsigned kFewJoined = 4 * kSms;  // rows that get eight warps each
+
 size_t ml_bytes(int rows) { return (size_t)2 * kMaxCtas * rows * sizeof(float2); }
 
 // The attention kernel and the join, chained to what runs before. Peers: CTAs that work on one item.
@@ -1532,10 +1643,14 @@ int launch(const AttendArgs &a, void (*kernel)(A...), int peers, int threads, in
     cfg.dynamicSmemBytes = smem;
     if (int rc = cudaLaunchKernelEx(&cfg, kernel, args...)) return rc;
     cfg.numAttrs = 1;
-    cfg.gridDim = dim3((unsigned)(a.seqs * a.tokens * a.q_heads));
+    const unsigned rows = (unsigned)(a.seqs * a.tokens * a.q_heads);
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
-    return cudaLaunchKernelEx(&cfg, join_kernel<D, SHARED>, a, teams);
+    cfg.gridDim = dim3(rows);
+    if (!SHARED) return cudaLaunchKernelEx(&cfg, join_kernel<D>, a, teams);
+    if (rows <= kFewJoined) return cudaLaunchKernelEx(&cfg, join_shared_kernel<D, 8>, a, teams);
+    cfg.gridDim = dim3((rows + 7) / 8);
+    return cudaLaunchKernelEx(&cfg, join_shared_kernel<D, 1>, a, teams);
 }
 template <int D, int MR, bool PAIR, bool SHARED>
 int launch_tiles(const AttendArgs &a, const CUtensorMap &k_map, const CUtensorMap &v_map) {
@@ -1568,6 +1683,8 @@ int attend_args(AttendArgs &a, float *out, const float *q, const qg_kv_cache *ca
     a.all_tiles = 0;
     a.prefix_acc = nullptr;
     a.prefix_ml = a.own_ml = nullptr;
+    a.starts = nullptr;
+    a.lengths = nullptr;
     a.err = static_cast<int *>(workspace);
     a.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + 256);
     return 0;
@@ -1629,7 +1746,8 @@ extern "C" int qg_shared_attention_workspace_bytes(int seqs, int tokens, int q_h
         return cudaErrorInvalidValue;
     const int rows = part_rows(seqs * tokens, q_heads / kv_heads);
     const size_t heads = ((size_t)seqs * tokens * q_heads + 1) & ~(size_t)1;
-    *bytes = 256 + ml_bytes(rows) + (size_t)2 * kMaxCtas * rows * head_dim * sizeof(float) + heads * (2 * sizeof(float2) + head_dim * sizeof(float));
+    *bytes = 256 + ml_bytes(rows) + (size_t)2 * kMaxCtas * rows * head_dim * sizeof(float) + heads * (2 * sizeof(float2) + head_dim * sizeof(float)) +
+             (kMaxSeqs + 1) * (sizeof(long long) + sizeof(int));
     return cudaSuccess;
 }
 
@@ -1641,6 +1759,11 @@ extern "C" int qg_shared_attention(float *out, const float *q, const qg_kv_cache
     const int rows = seqs * tokens * a.group, d = a.c.head_dim;  // of the prefix
     const bool pair = d == 256 && rows > kRows;
     a.copies = 1;
+    // The tensor cores cut off what does not fit when they add to S: two planes of d/16 steps each take half a unit in the last
+    // place, 0.72 * 2^-24 on average over the mantissas, of a running sum that is half of the final one on average. So scores
+    // are too small by d/16 * 0.72 * 2^-24, which the scale makes up for (24/2 heads of 256, 8,192 shared: errors against 64
+    // bits 1.8e-6 -> 0.95e-6; 32/8 of 128 0.94 -> 0.57e-6; 16/4 of 64 0.58 -> 0.39e-6).
+    a.scale = (float)((double)a.scale * (1.0 + d / 16 * 0.72 / 16777216.0));
     tiles(a, rows, pair);
     a.shared = shared;
     a.all_tiles = (rows + a.tile_rows - 1) / a.tile_rows;
@@ -1650,6 +1773,8 @@ extern "C" int qg_shared_attention(float *out, const float *q, const qg_kv_cache
     a.prefix_acc = a.part_acc + (size_t)2 * kMaxCtas * held * d;
     a.prefix_ml = reinterpret_cast<float2 *>(a.prefix_acc + heads * d);
     a.own_ml = a.prefix_ml + heads;
+    a.starts = reinterpret_cast<long long *>(a.own_ml + heads);
+    a.lengths = reinterpret_cast<int *>(a.starts + kMaxSeqs + 1);
     CUtensorMap k_map, v_map;
     if (int rc = maps(a, pair, k_map, v_map)) return rc;
     if (d == 64) return launch_tiles<64, 128, false, true>(a, k_map, v_map);
