@@ -70,8 +70,10 @@ struct AttendArgs {
     float *prefix_acc;   // [row][q_heads][D], [row][q_heads]: of prefix items that one CTA did as a whole
     float2 *prefix_ml;
     float2 *own_ml;      // the same of sequences' items, whose sums are in out
-    long long *starts;   // [seqs + 1]: the slots before each sequence's, and all
-    int *lengths;        // [seqs + 1]: own_length, and the common positions: for the join
+    // for the join: the slots before each sequence's, all of the sequences' line, all of the prefix's (the same line, or one of its
+    // own); own_length of each sequence, the common positions, the CTAs of both lines, the first CTA of the sequences' line
+    long long *starts;   // [seqs + 2]
+    int *lengths;        // [seqs + 4]
 };
 
 constexpr int kChunk = 32;       // keys per step of the softmax
@@ -430,6 +432,30 @@ struct Walk {
     }
 };
 
+// One warp: what the join needs to find every row's parts. `line`: slots before the first sequence's.
+template <int D>
+__device__ void tell_join(const AttendArgs &a, int shared, int common, long long line, long long own_w, long long prefix_w, int own_g, int prefix_g,
+                          int first) {
+    const int lane = threadIdx.x & 31;
+    for (int s0 = 0; s0 < a.seqs; s0 += 32) {
+        const int q = s0 + lane, own = q < a.seqs ? own_length<true>(a, q, shared, common) : -1;
+        const long long mine = (long long)slots_of<D>(a, own) * a.c.kv_heads * a.row_tiles;
+        long long upto = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += x;
+        }
+        if (q < a.seqs) a.starts[q] = line + upto - mine, a.lengths[q] = own;
+        line += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (lane == 0) {
+        a.starts[a.seqs] = own_w, a.starts[a.seqs + 1] = prefix_w;
+        int *to = a.lengths + a.seqs;
+        to[0] = common, to[1] = own_g, to[2] = prefix_g, to[3] = first;
+    }
+}
+
 // One warp: the slots of CTA (or pair) `team`.
 template <int D, bool SHARED>
 __device__ __forceinline__ void plan(const AttendArgs &a, Plan &s, int team, int teams) {
@@ -461,22 +487,7 @@ __device__ __forceinline__ void plan(const AttendArgs &a, Plan &s, int team, int
         s.pos0 = (int)(u0 - base - (long long)index * slots);
         s.common = common, s.source = source;
     }
-    if (SHARED && team == 0 && blockIdx.x == 0) {  // what the join needs to find every row's parts
-        long long before = line;
-        for (int s0 = 0; s0 < a.seqs; s0 += 32) {
-            const int q = s0 + lane, own = q < a.seqs ? own_length<SHARED>(a, q, shared, common) : -1;
-            const long long mine = (long long)slots_of<D>(a, own) * per;
-            long long upto = mine;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const long long x = __shfl_up_sync(0xffffffffu, upto, d);
-                if (lane >= d) upto += x;
-            }
-            if (q < a.seqs) a.starts[q] = before + upto - mine, a.lengths[q] = own;
-            before += __shfl_sync(0xffffffffu, upto, 31);
-        }
-        if (lane == 0) a.starts[a.seqs] = before, a.lengths[a.seqs] = common;
-    }
+    if (SHARED && team == 0 && blockIdx.x == 0) tell_join<D>(a, shared, common, line, w, w, g, g, 0);
 }
 
 // Of an item: the rows of q that are its own, counted from its first sequence's; where its keys begin; whose pages they are on.
@@ -532,10 +543,9 @@ __device__ __forceinline__ void mark_odd(uint64_t *notes, uint64_t nodes) {
     }
 }
 
-template <int D, int MR, bool PAIR, bool SHARED>
-__global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __grid_constant__ AttendArgs a,
-                                                                     const __grid_constant__ CUtensorMap k_map,
-                                                                     const __grid_constant__ CUtensorMap v_map) {
+// PLANNED: the plan is in shared memory already.
+template <int D, int MR, bool PAIR, bool SHARED, bool PLANNED>
+__device__ __forceinline__ void attend_tiles(const AttendArgs &a, const CUtensorMap &k_map, const CUtensorMap &v_map) {
     using C = Cfg<D, MR, PAIR>;
     static_assert(!PAIR || C::kOBufs == 1, "mark_odd: a unit takes both CTAs' O of the unit before");
     const int copies = D == 256 || SHARED ? 1 : a.copies;
@@ -549,8 +559,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     volatile int *abort = &s.abort;
 
     if (warp == 0) {
-        asm volatile("griddepcontrol.wait;" ::: "memory");
-        plan<D, SHARED>(a, s, team, teams);
+        if constexpr (!PLANNED) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            plan<D, SHARED>(a, s, team, teams);
+        }
     } else if (warp == 1) {
         if constexpr (PAIR) {
             asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s.tmem)));
@@ -1193,6 +1205,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     }
 }
 
+template <int D, int MR, bool PAIR, bool SHARED>
+__global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __grid_constant__ AttendArgs a,
+                                                                     const __grid_constant__ CUtensorMap k_map,
+                                                                     const __grid_constant__ CUtensorMap v_map) {
+    attend_tiles<D, MR, PAIR, SHARED, false>(a, k_map, v_map);
+}
+
 // ---- one token and at most four heads to a key head ---------------------------
 
 // So few rows need no tensor cores: a value of the cache costs five instructions or so, and the SM has time for them while
@@ -1223,28 +1242,26 @@ __device__ __forceinline__ void eight(const unsigned char *p, float (&x)[8], boo
     }
 }
 
-template <int D>
-__global__ void __launch_bounds__(32 * kFewWarps, 1) token_attention_kernel(const __grid_constant__ AttendArgs a) {
+struct FewNotes : Plan {
+    float2 ml[kFewWarps][kFewRows];
+};
+// What the CTA's plan says.
+template <int D, bool SHARED>
+__device__ __forceinline__ void attend_token(const AttendArgs &a, unsigned char *smem, FewNotes &s) {
     using C = Few<D>;
-    extern __shared__ __align__(1024) unsigned char smem[];
-    __shared__ Plan s;
-    __shared__ float2 ml[kFewWarps][kFewRows];
+    float2 (&ml)[kFewWarps][kFewRows] = s.ml;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, team = blockIdx.x;
     const int key = lane / C::kLanes, dim = lane % C::kLanes * 8;
     const float nan = __int_as_float(0x7fc00000);
-    if (warp == 0) {
-        asm volatile("griddepcontrol.wait;" ::: "memory");
-        plan<D, false>(a, s, team, gridDim.x);
-    }
-    __syncthreads();
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    for (int q = team; q < a.seqs; q += gridDim.x)  // rows of refused sequences
-        if (a.c.committed(q, 1) < 0)
-            for (int i = tid; i < a.q_heads * D; i += 32 * kFewWarps) a.out[(size_t)q * a.q_heads * D + i] = nan;
+    if constexpr (!SHARED)  // (with a shared prefix, the join's)
+        for (int q = team; q < a.seqs; q += gridDim.x)  // rows of refused sequences
+            if (a.c.committed(q, 1) < 0)
+                for (int i = tid; i < a.q_heads * D; i += 32 * kFewWarps) a.out[(size_t)q * a.q_heads * D + i] = nan;
     unsigned char *const ring = smem + warp * C::kStages * C::kStage + lane * 16;
     float *const sums = reinterpret_cast<float *>(smem + C::kRing);
     const size_t width = (size_t)a.c.kv_heads * D;
-    Walk<D, false> walk(s);
+    const int base0 = SHARED ? s.common : 0;  // where the items' positions begin
+    Walk<D, SHARED> walk(s);
     Item it;
     while (walk.next(a, it)) {
         const int all = it.length + 1, n = it.length + (a.tree ? (int)(a.tree[it.seq] & 1) : 1);  // keys there, keys seen
@@ -1256,7 +1273,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) token_attention_kernel(cons
             if (t < it.count) {
                 if (!(t & 31)) {  // the pages of the next 32 units, a lane each
                     const int at = first + (t + lane) * kKeys;
-                    page = t + lane < it.count && at < all ? table[at >> a.c.shift] : 0;
+                    page = t + lane < it.count && at < all ? table[(base0 + at) >> a.c.shift] : 0;
                     if ((unsigned)page >= (unsigned)a.c.pages) bad = true, page = 0;
                 }
                 const int p = __shfl_sync(0xffffffffu, page, t & 31), base = first + t * kKeys;
@@ -1377,15 +1394,81 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) token_attention_kernel(cons
                 total += f * x.y;
                 sum = fmaf(f, sums[(w * kFewRows + r) * D + d], sum);
             }
+            if (SHARED) sum *= kPScale, total *= kPScale;  // as the prefix's parts are
             if (bad) sum = nan;
-            if (whole) {
-                a.out[((size_t)it.seq * a.q_heads + it.kv * a.group + r) * D + d] = total == 0.0f && !bad ? 0.0f : sum / total;
+            const size_t at = (size_t)it.seq * a.q_heads + it.kv * a.group + r;
+            if (SHARED && whole) {  // for the join
+                a.out[at * D + d] = sum;
+                if (d == 0) a.own_ml[at] = make_float2(most, total);
+            } else if (whole) {
+                a.out[at * D + d] = total == 0.0f && !bad ? 0.0f : sum / total;
             } else {
                 a.part_acc[(part + r) * D + d] = sum;
                 if (d == 0) a.part_ml[part + r] = make_float2(most, total);
             }
         }
         __syncthreads();
+    }
+}
+
+template <int D>
+__global__ void __launch_bounds__(32 * kFewWarps, 1) token_attention_kernel(const __grid_constant__ AttendArgs a) {
+    extern __shared__ __align__(1024) unsigned char smem[];
+    __shared__ FewNotes s;
+    if (threadIdx.x < 32) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        plan<D, false>(a, s, blockIdx.x, gridDim.x);
+    }
+    __syncthreads();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    attend_token<D, false>(a, smem, s);
+}
+
+// With a shared prefix: the first CTAs do the prefix on the tensor cores, the others the sequences without them. Each has a line
+// of its own, and they share the GPU by what the lines take.
+constexpr int kPrefixUnit = 3, kTokenUnit = 2;  // time of a slot of either line, relatively
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1) shared_token_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap k_map,
+                                                                   const __grid_constant__ CUtensorMap v_map) {
+    using C = Cfg<D, 128, false>;
+    static_assert(kThreads == 32 * kFewWarps && sizeof(FewNotes) <= kNotes && Few<D>::kSmem <= C::kSmem - kNotes, "one CTA for both");
+    extern __shared__ __align__(1024) unsigned char smem[];
+    FewNotes &s = *reinterpret_cast<FewNotes *>(smem + C::kSmem - kNotes);  // (both keep the plan in the same place)
+    if (threadIdx.x < 32) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        const int lane = threadIdx.x, cta = blockIdx.x, ctas = gridDim.x, per = a.c.kv_heads;
+        const int shared = asked_shared<true>(a), source = first_live(a, shared), common = common_of(a, shared, source);
+        const int len = lane < a.seqs ? own_length<true>(a, lane, shared, common) : -1;
+        const long long prefix = prefix_line<D>(a, common), own = sum_slots<D, true>(a, a.seqs, per, shared, common);
+        const long long c1 = prefix * kPrefixUnit, c2 = own * kTokenUnit;
+        const int split = prefix ? max(1, min(ctas - 1, (int)((ctas * c1 + (c1 + c2) / 2) / (c1 + c2)))) : 0;
+        const int prefix_g = (int)min((long long)split, prefix), own_g = (int)min((long long)(ctas - split), own);
+        const bool first = cta < split;
+        const int team = first ? cta : cta - split, g = first ? prefix_g : own_g;
+        const long long w = first ? prefix : own;
+        long long base = 0, u0 = 0, u1 = 0;
+        int seq = first ? -1 : 0, length = common;
+        if (team < g) {
+            u0 = range_start(team, w, g);
+            u1 = range_start(team + 1, w, g);
+            if (!first) seq = find_slot<D, true>(a, per, u0, len, shared, common, base, length);
+        }
+        if (lane == 0) {
+            const int slots = first ? prefix_slots<D>(common) : max(1, slots_of<D>(a, length)), index = (int)quotient(u0 - base, slots);
+            const int tiles = first ? a.all_tiles : 1;
+            s.slot0 = u0, s.slot1 = u1, s.seq0 = seq, s.length0 = length;
+            s.kv0 = index / tiles, s.tile0 = index % tiles;
+            s.pos0 = (int)(u0 - base - (long long)index * slots);
+            s.common = common, s.source = first ? source : -1;
+        }
+        if (cta == 0) tell_join<D>(a, shared, common, 0, own, prefix, own_g, prefix_g, split);
+    }
+    __syncthreads();
+    if (s.seq0 < 0) {
+        attend_tiles<D, 128, false, true, true>(a, k_map, v_map);
+    } else {
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+        attend_token<D, true>(a, smem, s);
     }
 }
 
@@ -1480,7 +1563,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Atten
 // prefix_acc or out. WARPS warps to a (row, head): eight where there are so few rows that each may have many parts, otherwise one,
 // so that all rows are under way at once (48 x 5 rows of 24 heads of 256: 85 us with eight, @ with one).
 template <int D, int WARPS>
-__global__ void __launch_bounds__(256) join_shared_kernel(const __grid_constant__ AttendArgs a, int teams) {
+__global__ void __launch_bounds__(256) join_shared_kernel(const __grid_constant__ AttendArgs a) {
     constexpr int V = D / 32, kFly = 4;  // parts that are asked for before the first is used
     __shared__ float sums[8][D];
     __shared__ float2 totals[8];
@@ -1489,8 +1572,9 @@ __global__ void __launch_bounds__(256) join_shared_kernel(const __grid_constant_
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (id >= a.seqs * a.tokens * a.q_heads) return;  // (whole warps, and no barrier with WARPS 1)
     const int h = id % a.q_heads, row = id / a.q_heads, seq = row / a.tokens, kv = h / a.group, r = (row - seq * a.tokens) * a.group + h % a.group;
-    const long long w = a.starts[a.seqs], first = a.starts[seq];
-    const int own = a.lengths[seq], common = a.lengths[a.seqs], units = units_of(a, own), g = (int)min((long long)teams, w);
+    const long long w = a.starts[a.seqs], all_w = a.starts[a.seqs + 1], first = a.starts[seq];
+    const int *said = a.lengths + a.seqs;
+    const int own = a.lengths[seq], common = said[0], g = said[1], all_g = said[2], first_cta = said[3], units = units_of(a, own);
     float *out = a.out + (size_t)id * D;
     if (*(volatile int *)a.err || own < 0) {
         for (int i = WARPS == 1 ? lane : threadIdx.x; i < D; i += 32 * WARPS) out[i] = __int_as_float(0x7fc00000);
@@ -1501,8 +1585,9 @@ __global__ void __launch_bounds__(256) join_shared_kernel(const __grid_constant_
     // the prefix's parts of this row
     const int all_r = row * a.group + h % a.group;
     const long long all_start = (long long)(kv * a.all_tiles + all_r / a.tile_rows) * prefix_slots<D>(common) + kItemCost<D>;
-    const int p0 = common ? cta_of(all_start, w, g) : 0, before = common ? cta_of(all_start + common / kKeys - 1, w, g) - p0 + 1 : 0;
-    const bool late = start > range_start(c0, w, g), all_late = all_start > range_start(p0, w, g);  // the first part is its CTA's second
+    const int p0 = common ? cta_of(all_start, all_w, all_g) : 0, before = common ? cta_of(all_start + common / kKeys - 1, all_w, all_g) - p0 + 1 : 0;
+    // the first part is its CTA's second
+    const bool late = start > range_start(c0, w, g), all_late = common && all_start > range_start(p0, all_w, all_g);
     const int count = before + parts;
     // where part p of the row is
     auto part = [&](int p, const float *&acc, const float2 *&ml) {
@@ -1512,7 +1597,7 @@ __global__ void __launch_bounds__(256) join_shared_kernel(const __grid_constant_
             return;
         }
         const int q = prefix ? p : p - before;
-        const size_t at = (size_t)(2 * ((prefix ? p0 : c0) + q) + (q == 0 && (prefix ? all_late : late))) * a.part_rows + (prefix ? all_r : r) % a.tile_rows;
+        const size_t at = (size_t)(2 * ((prefix ? p0 : first_cta + c0) + q) + (q == 0 && (prefix ? all_late : late))) * a.part_rows + (prefix ? all_r : r) % a.tile_rows;
         acc = a.part_acc + at * D, ml = a.part_ml + at;
     };
     float m = -INFINITY, l = 0.0f, acc[V];
@@ -1627,7 +1712,7 @@ int launch(const AttendArgs &a, void (*kernel)(A...), int peers, int threads, in
     // no more CTAs than the longest sequences that the table allows could use
     const long long units = (((long long)a.c.table_pages << a.c.shift) + kKeys - 1) / kKeys;
     const long long most = ((long long)a.seqs * a.row_tiles + (SHARED ? a.all_tiles : 0)) * a.c.kv_heads * (units + kItemCost<D>);
-    const int teams = (int)(most < kMaxCtas / peers ? most : kMaxCtas / peers);
+    const int teams = (int)(most < kMaxCtas / peers ? most : kMaxCtas / peers);  // (two at least with SHARED: items cost more than a slot)
     cudaLaunchConfig_t cfg = {};
     cfg.stream = launch_stream;
     cudaLaunchAttribute attr[2];
@@ -1648,9 +1733,9 @@ int launch(const AttendArgs &a, void (*kernel)(A...), int peers, int threads, in
     cfg.dynamicSmemBytes = 0;
     cfg.gridDim = dim3(rows);
     if (!SHARED) return cudaLaunchKernelEx(&cfg, join_kernel<D>, a, teams);
-    if (rows <= kFewJoined) return cudaLaunchKernelEx(&cfg, join_shared_kernel<D, 8>, a, teams);
+    if (rows <= kFewJoined) return cudaLaunchKernelEx(&cfg, join_shared_kernel<D, 8>, a);
     cfg.gridDim = dim3((rows + 7) / 8);
-    return cudaLaunchKernelEx(&cfg, join_shared_kernel<D, 1>, a, teams);
+    return cudaLaunchKernelEx(&cfg, join_shared_kernel<D, 1>, a);
 }
 template <int D, int MR, bool PAIR, bool SHARED>
 int launch_tiles(const AttendArgs &a, const CUtensorMap &k_map, const CUtensorMap &v_map) {
@@ -1747,7 +1832,7 @@ extern "C" int qg_shared_attention_workspace_bytes(int seqs, int tokens, int q_h
     const int rows = part_rows(seqs * tokens, q_heads / kv_heads);
     const size_t heads = ((size_t)seqs * tokens * q_heads + 1) & ~(size_t)1;
     *bytes = 256 + ml_bytes(rows) + (size_t)2 * kMaxCtas * rows * head_dim * sizeof(float) + heads * (2 * sizeof(float2) + head_dim * sizeof(float)) +
-             (kMaxSeqs + 1) * (sizeof(long long) + sizeof(int));
+             (kMaxSeqs + 2) * sizeof(long long) + (kMaxSeqs + 4) * sizeof(int);
     return cudaSuccess;
 }
 
@@ -1774,9 +1859,15 @@ extern "C" int qg_shared_attention(float *out, const float *q, const qg_kv_cache
     a.prefix_ml = reinterpret_cast<float2 *>(a.prefix_acc + heads * d);
     a.own_ml = a.prefix_ml + heads;
     a.starts = reinterpret_cast<long long *>(a.own_ml + heads);
-    a.lengths = reinterpret_cast<int *>(a.starts + kMaxSeqs + 1);
+    a.lengths = reinterpret_cast<int *>(a.starts + kMaxSeqs + 2);
     CUtensorMap k_map, v_map;
     if (int rc = maps(a, pair, k_map, v_map)) return rc;
+    // One token, at most four heads to a key head of up to 128 values: as without a prefix, the sequences' own keys need no
+    // tensor cores.
+    if (tokens == 1 && a.group <= kFewRows && d == 64)
+        return launch<64, true>(a, shared_token_kernel<64>, 1, kThreads, Cfg<64, 128, false>::kSmem, a, k_map, v_map);
+    if (tokens == 1 && a.group <= kFewRows && d == 128)
+        return launch<128, true>(a, shared_token_kernel<128>, 1, kThreads, Cfg<128, 128, false>::kSmem, a, k_map, v_map);
     if (d == 64) return launch_tiles<64, 128, false, true>(a, k_map, v_map);
     if (d == 128) return launch_tiles<128, 128, false, true>(a, k_map, v_map);
     if (pair) return launch_tiles<256, 128, true, true>(a, k_map, v_map);
