@@ -343,15 +343,17 @@ __device__ __forceinline__ int units_of(const AttendArgs &a, int length) {
 // What an item costs besides its units, in units: Q, the first unit's latency and the store (about 2 us). The ranges
 // divide the sum of both; an item's first kItemCost slots stand for it and hold no unit. (When only units counted: 16 x 2
 // tokens, 512 to 8191 keys of heads of 128 92.1 -> 97.3 us, 5 x 5 tokens of heads of 64 18.5 -> 19.5.)
-template <int D>
-constexpr int kItemCost = D == 256 ? 1 : 2;
-template <int D>
+// With a shared prefix a CTA of heads of 256 often goes from one item to another, with one place for Q (in units, 1, 3 and 5:
+// 8 x 17 rows, 8,192 shared 92, 70, 68 us; 48 x 5, 32,768 shared 380, 329, 337; 32 single tokens, 4,096 shared 44, 41, 57).
+template <int D, bool SHARED>
+constexpr int kItemCost = D == 256 ? (SHARED ? 3 : 1) : 2;
+template <int D, bool SHARED>
 __device__ __forceinline__ int slots_of(const AttendArgs &a, int length) {
-    return length < 0 ? 0 : units_of(a, length) + kItemCost<D>;
+    return length < 0 ? 0 : units_of(a, length) + kItemCost<D, SHARED>;
 }
 // Slots of the prefix, and those of one of its items.
 template <int D>
-__device__ __forceinline__ int prefix_slots(int common) { return common / kKeys + kItemCost<D>; }
+__device__ __forceinline__ int prefix_slots(int common) { return common / kKeys + kItemCost<D, true>; }
 template <int D>
 __device__ __forceinline__ long long prefix_line(const AttendArgs &a, int common) {
     return common ? (long long)prefix_slots<D>(common) * a.c.kv_heads * a.all_tiles : 0;
@@ -360,7 +362,7 @@ __device__ __forceinline__ long long prefix_line(const AttendArgs &a, int common
 template <int D, bool SHARED>
 __device__ long long sum_slots(const AttendArgs &a, int seqs, int per, int shared, int common) {
     long long sum = 0;
-    for (int s = threadIdx.x & 31; s < seqs; s += 32) sum += (long long)slots_of<D>(a, own_length<SHARED>(a, s, shared, common)) * per;
+    for (int s = threadIdx.x & 31; s < seqs; s += 32) sum += (long long)slots_of<D, SHARED>(a, own_length<SHARED>(a, s, shared, common)) * per;
     return warp_sum(sum);
 }
 // One warp: the sequence that holds slot `at`, its length and the slots before it. `len`: the lane's own sequence
@@ -371,7 +373,7 @@ __device__ int find_slot(const AttendArgs &a, int per, long long at, int len, in
     base = 0;
     for (int s0 = 0; s0 < a.seqs; s0 += 32) {
         if (s0) len = s0 + lane < a.seqs ? own_length<SHARED>(a, s0 + lane, shared, common) : -1;
-        const long long mine = (long long)slots_of<D>(a, len) * per;
+        const long long mine = (long long)slots_of<D, SHARED>(a, len) * per;
         long long upto = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -410,11 +412,11 @@ struct Walk {
     __device__ Walk(const Plan &s)
         : at(s.slot0), end(s.slot1), seq(s.seq0), length(s.length0), kv(s.kv0), tile(s.tile0), pos(s.pos0), p(s) {}
     __device__ bool next(const AttendArgs &a, Item &it) {
-        const int from = max(pos, kItemCost<D>);
+        const int from = max(pos, kItemCost<D, SHARED>);
         if (at + (from - pos) >= end) return false;
-        it.seq = seq, it.kv = kv, it.tile = tile, it.first = from - kItemCost<D>, it.length = length;
+        it.seq = seq, it.kv = kv, it.tile = tile, it.first = from - kItemCost<D, SHARED>, it.length = length;
         it.units = SHARED && seq < 0 ? length / kKeys : units_of(a, length);
-        it.start = at - pos + kItemCost<D>;
+        it.start = at - pos + kItemCost<D, SHARED>;
         at += from - pos;
         it.count = (int)min((long long)(it.units - it.first), end - at);
         at += it.count;
@@ -439,7 +441,7 @@ __device__ void tell_join(const AttendArgs &a, int shared, int common, long long
     const int lane = threadIdx.x & 31;
     for (int s0 = 0; s0 < a.seqs; s0 += 32) {
         const int q = s0 + lane, own = q < a.seqs ? own_length<true>(a, q, shared, common) : -1;
-        const long long mine = (long long)slots_of<D>(a, own) * a.c.kv_heads * a.row_tiles;
+        const long long mine = (long long)slots_of<D, true>(a, own) * a.c.kv_heads * a.row_tiles;
         long long upto = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -464,10 +466,10 @@ __device__ __forceinline__ void plan(const AttendArgs &a, Plan &s, int team, int
     const int shared = asked_shared<SHARED>(a), source = SHARED ? first_live(a, shared) : 0, common = SHARED ? common_of(a, shared, source) : 0;
     const int len = lane < a.seqs ? own_length<SHARED>(a, lane, shared, common) : -1;
     const long long line = SHARED ? prefix_line<D>(a, common) : 0;
-    long long w = (long long)slots_of<D>(a, len) * per, base = 0, u0 = 0, u1 = 0;
+    long long w = (long long)slots_of<D, SHARED>(a, len) * per, base = 0, u0 = 0, u1 = 0;
     int seq = 0, length = len;
     if (a.seqs > 1) {
-        for (int q = lane + 32; q < a.seqs; q += 32) w += (long long)slots_of<D>(a, own_length<SHARED>(a, q, shared, common)) * per;
+        for (int q = lane + 32; q < a.seqs; q += 32) w += (long long)slots_of<D, SHARED>(a, own_length<SHARED>(a, q, shared, common)) * per;
         w = warp_sum(w);
     }
     w += line;
@@ -480,7 +482,7 @@ __device__ __forceinline__ void plan(const AttendArgs &a, Plan &s, int team, int
         else base = line;
     }
     if (lane == 0) {
-        const int slots = SHARED && seq < 0 ? prefix_slots<D>(common) : max(1, slots_of<D>(a, length)), index = (int)quotient(u0 - base, slots);
+        const int slots = SHARED && seq < 0 ? prefix_slots<D>(common) : max(1, slots_of<D, SHARED>(a, length)), index = (int)quotient(u0 - base, slots);
         const int tiles = SHARED && seq < 0 ? a.all_tiles : a.row_tiles;
         s.slot0 = u0, s.slot1 = u1, s.seq0 = seq, s.length0 = length;
         s.kv0 = index / tiles, s.tile0 = index % tiles;
@@ -1426,7 +1428,9 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) token_attention_kernel(cons
 
 // With a shared prefix: the first CTAs do the prefix on the tensor cores, the others the sequences without them. Each has a line
 // of its own, and they share the GPU by what the lines take.
-constexpr int kPrefixUnit = 3, kTokenUnit = 2;  // time of a slot of either line, relatively
+// Time of a slot of either line, relatively (64 users, 32/8 heads of 128, 4,112 shared, in us: 1 to 1 73, 3 to 2 59, 2 to 1 55,
+// 3 to 1 60; 16,384 shared: 82, 73, 72, 87).
+constexpr int kPrefixUnit = 2, kTokenUnit = 1;
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1) shared_token_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap k_map,
                                                                    const __grid_constant__ CUtensorMap v_map) {
@@ -1454,7 +1458,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_token_kernel(const __grid_
             if (!first) seq = find_slot<D, true>(a, per, u0, len, shared, common, base, length);
         }
         if (lane == 0) {
-            const int slots = first ? prefix_slots<D>(common) : max(1, slots_of<D>(a, length)), index = (int)quotient(u0 - base, slots);
+            const int slots = first ? prefix_slots<D>(common) : max(1, slots_of<D, true>(a, length)), index = (int)quotient(u0 - base, slots);
             const int tiles = first ? a.all_tiles : 1;
             s.slot0 = u0, s.slot1 = u1, s.seq0 = seq, s.length0 = length;
             s.kv0 = index / tiles, s.tile0 = index % tiles;
@@ -1486,7 +1490,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Atten
     const int per = a.c.kv_heads * a.row_tiles;
     const int units = units_of(a, a.c.committed(seq, a.tokens));
     const long long w = sum_slots<D, false>(a, a.seqs, per, 0, 0);
-    const long long start = (seq ? sum_slots<D, false>(a, seq, per, 0, 0) : 0) + (long long)(kv * a.row_tiles + tile) * (units + kItemCost<D>) + kItemCost<D>;
+    const long long start = (seq ? sum_slots<D, false>(a, seq, per, 0, 0) : 0) + (long long)(kv * a.row_tiles + tile) * (units + kItemCost<D, false>) + kItemCost<D, false>;
     const int g = (int)min((long long)teams, w);
     const int c0 = units ? cta_of(start, w, g) : 0, parts = units ? cta_of(start + units - 1, w, g) - c0 + 1 : 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -1580,11 +1584,11 @@ __global__ void __launch_bounds__(256) join_shared_kernel(const __grid_constant_
         for (int i = WARPS == 1 ? lane : threadIdx.x; i < D; i += 32 * WARPS) out[i] = __int_as_float(0x7fc00000);
         return;
     }
-    const long long start = first + (long long)(kv * a.row_tiles + r / a.tile_rows) * (units + kItemCost<D>) + kItemCost<D>;
+    const long long start = first + (long long)(kv * a.row_tiles + r / a.tile_rows) * (units + kItemCost<D, true>) + kItemCost<D, true>;
     const int c0 = cta_of(start, w, g), parts = cta_of(start + units - 1, w, g) - c0 + 1;
     // the prefix's parts of this row
     const int all_r = row * a.group + h % a.group;
-    const long long all_start = (long long)(kv * a.all_tiles + all_r / a.tile_rows) * prefix_slots<D>(common) + kItemCost<D>;
+    const long long all_start = (long long)(kv * a.all_tiles + all_r / a.tile_rows) * prefix_slots<D>(common) + kItemCost<D, true>;
     const int p0 = common ? cta_of(all_start, all_w, all_g) : 0, before = common ? cta_of(all_start + common / kKeys - 1, all_w, all_g) - p0 + 1 : 0;
     // the first part is its CTA's second
     const bool late = start > range_start(c0, w, g), all_late = common && all_start > range_start(p0, all_w, all_g);
@@ -1651,27 +1655,27 @@ __global__ void __launch_bounds__(256) join_shared_kernel(const __grid_constant_
 #pragma unroll
             for (int e = 0; e < V; e += 4) *reinterpret_cast<float4 *>(to + e) = *reinterpret_cast<float4 *>(acc + e);
         }
-        return;
-    }
+    } else {
 #pragma unroll
-    for (int e = 0; e < V; e++) sums[warp][lane * V + e] = acc[e];
-    if (lane == 0) totals[warp] = make_float2(m, l);
-    __syncthreads();
-    m = -INFINITY, l = 0.0f;
-    float f[8];
+        for (int e = 0; e < V; e++) sums[warp][lane * V + e] = acc[e];
+        if (lane == 0) totals[warp] = make_float2(m, l);
+        __syncthreads();
+        m = -INFINITY, l = 0.0f;
+        float f[8];
 #pragma unroll
-    for (int k = 0; k < 8; k++) m = fmaxf(m, totals[k].x);
+        for (int k = 0; k < 8; k++) m = fmaxf(m, totals[k].x);
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
-        f[k] = totals[k].x == -INFINITY ? totals[k].y : ex2(totals[k].x - m);
-        l += f[k] * totals[k].y;
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    for (int i = threadIdx.x; i < D; i += 256) {
-        float v = 0.0f;
+        for (int k = 0; k < 8; k++) {
+            f[k] = totals[k].x == -INFINITY ? totals[k].y : ex2(totals[k].x - m);
+            l += f[k] * totals[k].y;
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        for (int i = threadIdx.x; i < D; i += 256) {
+            float v = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 8; k++) v = fmaf(f[k], sums[k][i], v);
-        out[i] = v * inv;
+            for (int k = 0; k < 8; k++) v = fmaf(f[k], sums[k][i], v);
+            out[i] = v * inv;
+        }
     }
 }
 
@@ -1711,7 +1715,7 @@ int launch(const AttendArgs &a, void (*kernel)(A...), int peers, int threads, in
     if (int rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return rc;
     // no more CTAs than the longest sequences that the table allows could use
     const long long units = (((long long)a.c.table_pages << a.c.shift) + kKeys - 1) / kKeys;
-    const long long most = ((long long)a.seqs * a.row_tiles + (SHARED ? a.all_tiles : 0)) * a.c.kv_heads * (units + kItemCost<D>);
+    const long long most = ((long long)a.seqs * a.row_tiles + (SHARED ? a.all_tiles : 0)) * a.c.kv_heads * (units + kItemCost<D, SHARED>);
     const int teams = (int)(most < kMaxCtas / peers ? most : kMaxCtas / peers);  // (two at least with SHARED: items cost more than a slot)
     cudaLaunchConfig_t cfg = {};
     cfg.stream = launch_stream;
@@ -1731,11 +1735,13 @@ int launch(const AttendArgs &a, void (*kernel)(A...), int peers, int threads, in
     const unsigned rows = (unsigned)(a.seqs * a.tokens * a.q_heads);
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
-    cfg.gridDim = dim3(rows);
-    if (!SHARED) return cudaLaunchKernelEx(&cfg, join_kernel<D>, a, teams);
-    if (rows <= kFewJoined) return cudaLaunchKernelEx(&cfg, join_shared_kernel<D, 8>, a);
-    cfg.gridDim = dim3((rows + 7) / 8);
-    return cudaLaunchKernelEx(&cfg, join_shared_kernel<D, 1>, a);
+    if constexpr (!SHARED) {
+        cfg.gridDim = dim3(rows);
+        return cudaLaunchKernelEx(&cfg, join_kernel<D>, a, teams);
+    } else {
+        cfg.gridDim = dim3(rows <= kFewJoined ? rows : (rows + 7) / 8);
+        return rows <= kFewJoined ? cudaLaunchKernelEx(&cfg, join_shared_kernel<D, 8>, a) : cudaLaunchKernelEx(&cfg, join_shared_kernel<D, 1>, a);
+    }
 }
 template <int D, int MR, bool PAIR, bool SHARED>
 int launch_tiles(const AttendArgs &a, const CUtensorMap &k_map, const CUtensorMap &v_map) {
