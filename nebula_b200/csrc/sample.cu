@@ -46,13 +46,16 @@ using Whole = unsigned long long;
 
 // What the CTAs of a cluster read of each other.
 struct Shared {
-    float most[kMaxRanks], least[kMaxRanks];
+    Whole ends[kMaxRanks];             // keys of the largest logit, and of the threads' lowest
     int index[kMaxRanks], last[2];
     Whole total[2][kMaxRanks];         // by the parity of the exchange: a CTA may be one ahead
     unsigned hist[2][3][kBins];        // by the parity of the pass: counts, or sums as 15 + 15 + 14 bits
     Whole list[kList];                 // key and inverted index: the larger is the better
     int listed;
-    unsigned fine[3][kFine];           // sums in the same parts
+    union {
+        unsigned fine[3][kFine];       // sums in the same parts
+        Whole extra[kThreads];         // (once the bins are read) a CTA's own
+    };
     Whole coarse[kFine / 32];
     // a CTA's own
     Whole warp_sum[kWarps], entry_weight[kFew];
@@ -64,7 +67,7 @@ struct Shared {
     };
     Whole found, kept_sum;
     int few;
-    float warp_most[kWarps], warp_least[kWarps];
+    unsigned warp_most[kWarps], warp_least[kWarps];
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -355,18 +358,9 @@ struct Range {
     __device__ __forceinline__ int shift() const { return max(0, 25 - __clz(high - low)); }  // (high - low) >> shift < kBins
 };
 
-// The kept logits in a range, of all CTAs and in any order, in s.entry. Returns their number; more than kList are not listed.
-// s.listed is zero before.
-__device__ int gather(Shared &s, const Row &r, const Range &in) {
+// What all CTAs have listed, in any order, in s.entry. Returns its number; more than kList are not there.
+__device__ int read_lists(Shared &s, const Row &r) {
     const int tid = threadIdx.x;
-    r.some(of_key(max(in.low, kNone + 1)), of_key(in.high), [&](const float (&x)[2], const int (&at)[2]) {
-#pragma unroll
-        for (int e = 0; e < 2; e++)
-            if (r.kept_of_floor(x[e], at[e]) && in.has(x[e])) {
-                const int to = atomicAdd(&s.listed, 1);
-                if (to < kList) s.list[to] = (Whole)key_of(x[e]) << 32 | (unsigned)~at[e];
-            }
-    });
     cluster_sync();
     int n[kMaxRanks], all = 0;
 #pragma unroll
@@ -383,6 +377,19 @@ __device__ int gather(Shared &s, const Row &r, const Range &in) {
     }
     __syncthreads();
     return all;
+}
+__device__ __forceinline__ void list(Shared &s, float x, int index) {
+    const int to = atomicAdd(&s.listed, 1);
+    if (to < kList) s.list[to] = (Whole)key_of(x) << 32 | (unsigned)~index;
+}
+// The kept logits in a range, listed and read. s.listed is zero before.
+__device__ int gather(Shared &s, const Row &r, const Range &in) {
+    r.some(of_key(max(in.low, kNone + 1)), of_key(in.high), [&](const float (&x)[2], const int (&at)[2]) {
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+            if (r.kept_of_floor(x[e], at[e]) && in.has(x[e])) list(s, x[e], at[e]);
+    });
+    return read_lists(s, r);
 }
 // Weights of the n entries, and for entry tid/2 the number and the weights of the better ones. n is at most kFew.
 __device__ __forceinline__ int order(Shared &s, const Row &r, int n, Whole &above) {
@@ -522,7 +529,9 @@ __device__ __forceinline__ Whole share_of(float p, Whole all) {
 __device__ __forceinline__ float octaves_of(float p, int vocab) { return log2f((float)vocab) - log2f(1.0f - fmaxf(p, 0.0f)) + 1.0f; }
 
 // Top-p of a whole row: the sum of all weights and the bins of those that may matter, none of which lie below `end`, in one pass.
-__device__ void nucleus(Shared &s, Row &r, float p, float end, int &pass, int &turn) {
+// SUMS: also the thread's sum of the weights that are kept. False where it has none.
+template <bool SUMS>
+__device__ bool nucleus(Shared &s, Row &r, float p, float end, Whole &kept, int &pass, int &turn) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     Range in = {key_of(end), key_of(r.most), r.most, fminf(kFine / (r.most - end), 1e30f), kFine - 1, -1};
     for (int i = tid; i < 3 * kFine; i += kThreads) s.fine[0][i] = 0;
@@ -566,7 +575,7 @@ __device__ void nucleus(Shared &s, Row &r, float p, float end, int &pass, int &t
     };
     if (warp < kMaxRanks) s.read[0][warp][lane] = warp < r.ranks ? peer_load64(at_rank(&s.coarse[lane], warp)) : 0;
     const int group = find(s.read[0], target);
-    if (group < 0) return;  // all of them
+    if (group < 0) return false;  // all of them
     if (warp < kMaxRanks) {
         unsigned part[3] = {0, 0, 0};
         if (warp < r.ranks)
@@ -575,13 +584,40 @@ __device__ void nucleus(Shared &s, Row &r, float p, float end, int &pass, int &t
         s.read[1][warp][lane] = part[0] + ((Whole)part[1] << 15) + ((Whole)part[2] << 30);
     }
     in.take_bin(32 * group + find(s.read[1], target));
-    const int n = gather(s, r, in);
-    if (n <= kList) {
-        const Whole worst = nth_entry<true>(s, r, n, in, target, s.hist[pass & 1]);
-        r.key = (unsigned)(worst >> 32), r.last = (int)~(unsigned)worst;
+    int n;
+    if (SUMS) {  // what is in better bins stays, whatever comes of this one
+        kept = 0;
+        const float low = of_key(max(in.low, kNone + 1));
+        r.each_weight(low, [&](const float (&x)[4], int at, const Whole (&w)[4]) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (x[e] >= low) {
+                    const int bin = in.bin_of(x[e]);
+                    if (bin < in.bin) kept += w[e];
+                    if (bin == in.bin) list(s, x[e], at + e);
+                }
+        });
+        n = read_lists(s, r);
+        s.extra[tid] = 0;
     } else {
-        narrow<true>(s, r, target, in, false, pass, turn);
+        n = gather(s, r, in);
     }
+    if (n > kList) {
+        narrow<true>(s, r, target, in, false, pass, turn);
+        return false;
+    }
+    const Whole worst = nth_entry<true>(s, r, n, in, target, s.hist[pass & 1]);
+    r.key = (unsigned)(worst >> 32), r.last = (int)~(unsigned)worst;
+    if (SUMS) {
+        const int first = r.index - tid * 4 * r.units;  // of the CTA
+        for (int i = tid; i < s.listed; i += kThreads) {
+            const Whole e = s.list[i];
+            if (e >= worst) atomicAdd(&s.extra[((int)~(unsigned)e - first) / (4 * r.units)], r.weigh(of_key((unsigned)(e >> 32))));
+        }
+        __syncthreads();
+        kept += s.extra[tid];
+    }
+    return true;
 }
 
 // A lower bound of the k-th largest logit, from the largest of each thread's (k logits are at least as large as the k-th
@@ -651,30 +687,24 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
             asm volatile("prefetch.global.L2 [%0];" ::"l"(x1 + i));
     }
     const float threads_most = most;
-    float lowest = most > -INFINITY ? most : INFINITY;  // of the threads' largest
-#pragma unroll
-    for (int d = 16; d; d >>= 1) {
-        most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, d));
-        lowest = fminf(lowest, __shfl_xor_sync(0xffffffffu, lowest, d));
-    }
-    if (lane == 0) s.warp_most[warp] = most, s.warp_least[warp] = lowest;
+    // (as keys: a NaN's is above all)
+    unsigned top = key_of(most), low = most > -INFINITY ? top : ~0u;  // the lowest: of the threads' largest, for top-k
+    top = __reduce_max_sync(0xffffffffu, top);
+    low = __reduce_min_sync(0xffffffffu, low);
+    if (lane == 0) s.warp_most[warp] = top, s.warp_least[warp] = low;
     __syncthreads();
     if (warp == 0) {
-        most = lane < kWarps ? s.warp_most[lane] : -INFINITY;
-        lowest = lane < kWarps ? s.warp_least[lane] : INFINITY;
-#pragma unroll
-        for (int d = 16; d; d >>= 1) {
-            most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, d));
-            lowest = fminf(lowest, __shfl_xor_sync(0xffffffffu, lowest, d));
-        }
-        if (lane < r.ranks) {
-            peer_store(at_rank(&s.most[r.rank], lane), __float_as_uint(most));
-            peer_store(at_rank(&s.least[r.rank], lane), __float_as_uint(lowest));
-        }
+        top = __reduce_max_sync(0xffffffffu, lane < kWarps ? s.warp_most[lane] : 0);
+        low = __reduce_min_sync(0xffffffffu, lane < kWarps ? s.warp_least[lane] : ~0u);
+        if (lane < r.ranks) peer_store(at_rank(&s.ends[r.rank], lane), (Whole)top << 32 | low);
     }
     cluster_sync();
-    most = -INFINITY, lowest = INFINITY;
-    for (uint32_t i = 0; i < r.ranks; i++) most = max_nan(most, s.most[i]), lowest = fminf(lowest, s.least[i]);
+    top = 0, low = ~0u;
+#pragma unroll
+    for (int i = 0; i < kMaxRanks; i++)
+        if (i < r.ranks) top = max(top, (unsigned)(s.ends[i] >> 32)), low = min(low, (unsigned)s.ends[i]);
+    most = of_key(top);
+    const float lowest = low == ~0u ? most : of_key(low);
     const bool refused = !(most > -INFINITY && most < INFINITY) || !(t >= 0.0f && t < INFINITY) || p != p || least != least || u != u;
 
     // ---- what is kept
@@ -691,6 +721,8 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
         return border >= r.top ? key_of(most) : key_of(__double2float_ru(border));
     }();
     int token = -1;  // where it is known already
+    bool summed = false;  // kept: the thread's sum of what is kept
+    Whole kept = 0;
     if (refused) {
     } else if (t == 0.0f) {  // the largest logit, the lowest index of equals
         int index = 0x7fffffff;
@@ -758,7 +790,9 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
         if (!done && p < 1.0f) {
             const float octaves = fminf(octaves_of(p, a.vocab), 46.0f), end = fmaxf((float)(r.top - octaves / r.c), kLowest);
             if (r.key == kNone) {
-                nucleus(s, r, p, end, pass, turn);
+                // (only a draw needs sums; and min_p may leave out more)
+                if (a.token && !min_key) summed = nucleus<true>(s, r, p, end, kept, pass, turn);
+                else nucleus<false>(s, r, p, end, kept, pass, turn);
             } else {
                 Whole all;
                 share_sums(s, r, r.kept_sum(), turn);
@@ -778,7 +812,7 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
             return;
         }
         auto mine = [&](float x, int index) { return r.keeps(x, index) ? r.weigh(x) : 0; };
-        const Whole sum = r.kept_sum();
+        const Whole sum = summed ? kept : r.kept_sum();
         Whole all;
         share_sums(s, r, sum, turn);
         const Whole before = sums_before(s, r, turn, all);
@@ -831,9 +865,19 @@ int launch(SampleArgs &a, int rows) {
     // up to three logits may lie before a row that does not start on 16 bytes
     const bool aligned = !(reinterpret_cast<uintptr_t>(a.logits) & 15) && a.vocab % 4 == 0;
     const int long_row = a.vocab + (aligned ? 0 : 3);
-    int ranks = 1;
-    while (ranks < kMaxRanks && (long_row + ranks - 1) / ranks > kStep) ranks *= 2;
-    a.units = ((long_row + ranks - 1) / ranks + kStep - 1) / kStep;
+    // Clusters of more CTAs take less time for a row, but fewer of them fit. A row takes about as long for its fixed steps
+    // as for seven units of a thread, and the GPU takes 33, 71, 148 or 296 clusters of 8, 4, 2 or 1 CTAs (15, 33, 74 and 148 where a
+    // CTA has more than half an SM's memory) at once.
+    int ranks = 1, clusters = 1;
+    long long best = 0;
+    for (int n = 1; n <= kMaxRanks; n *= 2) {
+        const int units = ((long_row + n - 1) / n + kStep - 1) / kStep;
+        if (units > kMaxUnits) continue;
+        const bool half = kThreads * (units | 1) * 16 + (int)sizeof(Shared) <= 115200;
+        const int fit = n == 8 ? (half ? 33 : 15) : n == 4 ? (half ? 71 : 33) : (half ? 296 : 148) / n;
+        const long long time = (long long)((rows + fit - 1) / fit) * (7 + units);
+        if (!best || time < best) best = time, ranks = n, clusters = rows < fit ? rows : fit, a.units = units;
+    }
     const int smem = kThreads * (a.units | 1) * 16 + (int)sizeof(Shared);
     if (int rc = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return rc;
     a.rows = rows;
@@ -849,12 +893,7 @@ int launch(SampleArgs &a, int rows) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    // as many clusters as fit at once
-    int clusters = 0;
-    cfg.gridDim = dim3(ranks);
-    if (rows > 1)
-        if (int rc = cudaOccupancyMaxActiveClusters(&clusters, sample_kernel, &cfg)) return rc;
-    cfg.gridDim = dim3((unsigned)(rows < clusters ? rows : clusters > 1 ? clusters : 1) * ranks);
+    cfg.gridDim = dim3((unsigned)(clusters * ranks));
     return cudaLaunchKernelEx(&cfg, sample_kernel, a);
 }
 
