@@ -52,10 +52,7 @@ struct Shared {
     unsigned hist[2][3][kBins];        // by the parity of the pass: counts, or sums as 15 + 15 + 14 bits
     Whole list[kList];                 // key and inverted index: the larger is the better
     int listed;
-    union {
-        unsigned fine[3][kFine];       // sums in the same parts
-        Whole extra[kThreads];         // (once the bins are read) a CTA's own
-    };
+    unsigned fine[3][kFine];           // sums in the same parts
     Whole coarse[kFine / 32];
     // a CTA's own
     Whole warp_sum[kWarps], entry_weight[kFew];
@@ -222,7 +219,7 @@ struct Row {
     // 2^44 * 2^((x - most) * c), rounded. The polynomial of degree 9 is 2^f's Chebyshev fit on [-1/2, 1/2] (error 2^-46).
     __device__ __forceinline__ Whole weigh(float x) const {
         const double t = ((double)fmaxf(x, zero) - top) * c;
-        constexpr double kRound = 6755399441055744.0, kUnit = 4503599627370496.0;  // 1.5 * 2^52, 2^52
+        constexpr double kRound = 6755399441055744.0 + 44.0, kUnit = 4503599627370496.0;  // 1.5 * 2^52 (the last bits: n + 44), 2^52
         const double n = t + kRound, f = t - (n - kRound);
         double p = 1.0205905413765595e-07;
         p = fma(p, f, 1.325964524488711e-06);
@@ -234,7 +231,7 @@ struct Row {
         p = fma(p, f, 2.402265069564034e-01);
         p = fma(p, f, 6.931471805599462e-01);
         p = fma(p, f, 1.0000000000000135);
-        const double v = __hiloint2double(__double2hiint(p) + ((__double2loint(n) + 44) << 20), __double2loint(p)) + kUnit;
+        const double v = __hiloint2double(__double2hiint(p) + (__double2loint(n) << 20), __double2loint(p)) + kUnit;
         return x >= zero ? (Whole)__double_as_longlong(v) & 0xfffffffffffffull : 0;
     }
 };
@@ -358,9 +355,17 @@ struct Range {
     __device__ __forceinline__ int shift() const { return max(0, 25 - __clz(high - low)); }  // (high - low) >> shift < kBins
 };
 
-// What all CTAs have listed, in any order, in s.entry. Returns its number; more than kList are not there.
-__device__ int read_lists(Shared &s, const Row &r) {
-    const int tid = threadIdx.x;
+// The kept logits in a range, of all CTAs and in any order, in s.entry. Returns their number; more than kList are not listed.
+// s.listed is zero before.
+__device__ int gather(Shared &s, const Row &r, const Range &in) {
+    r.some(of_key(max(in.low, kNone + 1)), of_key(in.high), [&](const float (&x)[2], const int (&at)[2]) {
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+            if (r.kept_of_floor(x[e], at[e]) && in.has(x[e])) {
+                const int to = atomicAdd(&s.listed, 1);
+                if (to < kList) s.list[to] = (Whole)key_of(x[e]) << 32 | (unsigned)~at[e];
+            }
+    });
     cluster_sync();
     int n[kMaxRanks], all = 0;
 #pragma unroll
@@ -368,7 +373,7 @@ __device__ int read_lists(Shared &s, const Row &r) {
 #pragma unroll
     for (int q = 0; q < kMaxRanks; q++) all += n[q];
     if (all > kList) return all;
-    for (int i = tid; i < all; i += kThreads) {
+    for (int i = threadIdx.x; i < all; i += kThreads) {
         int q = 0, at = i;
 #pragma unroll
         for (int e = 0; e < kMaxRanks - 1; e++)
@@ -377,19 +382,6 @@ __device__ int read_lists(Shared &s, const Row &r) {
     }
     __syncthreads();
     return all;
-}
-__device__ __forceinline__ void list(Shared &s, float x, int index) {
-    const int to = atomicAdd(&s.listed, 1);
-    if (to < kList) s.list[to] = (Whole)key_of(x) << 32 | (unsigned)~index;
-}
-// The kept logits in a range, listed and read. s.listed is zero before.
-__device__ int gather(Shared &s, const Row &r, const Range &in) {
-    r.some(of_key(max(in.low, kNone + 1)), of_key(in.high), [&](const float (&x)[2], const int (&at)[2]) {
-#pragma unroll
-        for (int e = 0; e < 2; e++)
-            if (r.kept_of_floor(x[e], at[e]) && in.has(x[e])) list(s, x[e], at[e]);
-    });
-    return read_lists(s, r);
 }
 // Weights of the n entries, and for entry tid/2 the number and the weights of the better ones. n is at most kFew.
 __device__ __forceinline__ int order(Shared &s, const Row &r, int n, Whole &above) {
@@ -529,9 +521,7 @@ __device__ __forceinline__ Whole share_of(float p, Whole all) {
 __device__ __forceinline__ float octaves_of(float p, int vocab) { return log2f((float)vocab) - log2f(1.0f - fmaxf(p, 0.0f)) + 1.0f; }
 
 // Top-p of a whole row: the sum of all weights and the bins of those that may matter, none of which lie below `end`, in one pass.
-// SUMS: also the thread's sum of the weights that are kept. False where it has none.
-template <bool SUMS>
-__device__ bool nucleus(Shared &s, Row &r, float p, float end, Whole &kept, int &pass, int &turn) {
+__device__ void nucleus(Shared &s, Row &r, float p, float end, int &pass, int &turn) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     Range in = {key_of(end), key_of(r.most), r.most, fminf(kFine / (r.most - end), 1e30f), kFine - 1, -1};
     for (int i = tid; i < 3 * kFine; i += kThreads) s.fine[0][i] = 0;
@@ -575,7 +565,7 @@ __device__ bool nucleus(Shared &s, Row &r, float p, float end, Whole &kept, int 
     };
     if (warp < kMaxRanks) s.read[0][warp][lane] = warp < r.ranks ? peer_load64(at_rank(&s.coarse[lane], warp)) : 0;
     const int group = find(s.read[0], target);
-    if (group < 0) return false;  // all of them
+    if (group < 0) return;  // all of them
     if (warp < kMaxRanks) {
         unsigned part[3] = {0, 0, 0};
         if (warp < r.ranks)
@@ -584,40 +574,13 @@ __device__ bool nucleus(Shared &s, Row &r, float p, float end, Whole &kept, int 
         s.read[1][warp][lane] = part[0] + ((Whole)part[1] << 15) + ((Whole)part[2] << 30);
     }
     in.take_bin(32 * group + find(s.read[1], target));
-    int n;
-    if (SUMS) {  // what is in better bins stays, whatever comes of this one
-        kept = 0;
-        const float low = of_key(max(in.low, kNone + 1));
-        r.each_weight(low, [&](const float (&x)[4], int at, const Whole (&w)[4]) {
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (x[e] >= low) {
-                    const int bin = in.bin_of(x[e]);
-                    if (bin < in.bin) kept += w[e];
-                    if (bin == in.bin) list(s, x[e], at + e);
-                }
-        });
-        n = read_lists(s, r);
-        s.extra[tid] = 0;
-    } else {
-        n = gather(s, r, in);
-    }
+    const int n = gather(s, r, in);
     if (n > kList) {
         narrow<true>(s, r, target, in, false, pass, turn);
-        return false;
+        return;
     }
     const Whole worst = nth_entry<true>(s, r, n, in, target, s.hist[pass & 1]);
     r.key = (unsigned)(worst >> 32), r.last = (int)~(unsigned)worst;
-    if (SUMS) {
-        const int first = r.index - tid * 4 * r.units;  // of the CTA
-        for (int i = tid; i < s.listed; i += kThreads) {
-            const Whole e = s.list[i];
-            if (e >= worst) atomicAdd(&s.extra[((int)~(unsigned)e - first) / (4 * r.units)], r.weigh(of_key((unsigned)(e >> 32))));
-        }
-        __syncthreads();
-        kept += s.extra[tid];
-    }
-    return true;
 }
 
 // A lower bound of the k-th largest logit, from the largest of each thread's (k logits are at least as large as the k-th
@@ -721,8 +684,6 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
         return border >= r.top ? key_of(most) : key_of(__double2float_ru(border));
     }();
     int token = -1;  // where it is known already
-    bool summed = false;  // kept: the thread's sum of what is kept
-    Whole kept = 0;
     if (refused) {
     } else if (t == 0.0f) {  // the largest logit, the lowest index of equals
         int index = 0x7fffffff;
@@ -790,9 +751,7 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
         if (!done && p < 1.0f) {
             const float octaves = fminf(octaves_of(p, a.vocab), 46.0f), end = fmaxf((float)(r.top - octaves / r.c), kLowest);
             if (r.key == kNone) {
-                // (only a draw needs sums; and min_p may leave out more)
-                if (a.token && !min_key) summed = nucleus<true>(s, r, p, end, kept, pass, turn);
-                else nucleus<false>(s, r, p, end, kept, pass, turn);
+                nucleus(s, r, p, end, pass, turn);
             } else {
                 Whole all;
                 share_sums(s, r, r.kept_sum(), turn);
@@ -812,7 +771,7 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
             return;
         }
         auto mine = [&](float x, int index) { return r.keeps(x, index) ? r.weigh(x) : 0; };
-        const Whole sum = summed ? kept : r.kept_sum();
+        const Whole sum = r.kept_sum();
         Whole all;
         share_sums(s, r, sum, turn);
         const Whole before = sums_before(s, r, turn, all);
