@@ -4,7 +4,8 @@
 // Free pages are a stack. One cluster does a call: a thread per sequence, so every CTA makes the same prefix sum of what the
 // sequences need (or give back) in its own shared memory, then takes its share of the entries to write. What the call
 // changes and all CTAs read (pages held, the stack's height) is written after a barrier of the cluster. Bound by latency:
-// launch, one trip for the lengths, one for the stack or the table, the barrier.
+// launch, one trip for the lengths, one for the stack or the table, the barrier. Where there are many slots to write a second
+// kernel does it on the whole GPU, from the page tables that the first one has left.
 #include "cache.cuh"
 
 using namespace nb;
@@ -15,6 +16,7 @@ constexpr int kThreads = 1024;      // one per sequence
 constexpr int kPagesCluster = 8;    // CTAs where there is more than kOneCta to write
 constexpr long long kOneCta = 4096;
 constexpr int kChunk = 256;         // slots that a warp takes at a time
+constexpr long long kWide = 65536;  // slots that get a kernel of their own
 static_assert(kThreads >= kMaxSeqs, "a thread per sequence");
 
 struct PagesArgs {
@@ -177,6 +179,34 @@ __global__ void __launch_bounds__(kThreads, 1) release_kernel(const __grid_const
     }
 }
 
+// The slots alone, four at a time where that is how they lie, after reserve_kernel.
+__global__ void __launch_bounds__(256) slots_kernel(const __grid_constant__ PagesArgs a) {
+    const int lane = threadIdx.x & 31, chunks = (a.tokens + kChunk - 1) / kChunk, u = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int q = u / chunks, from = (u - q * chunks) * kChunk, to = min(from + kChunk, a.tokens), mask = (1 << a.shift) - 1;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (q >= a.seqs) return;
+    const int fresh = a.out[q] < 0 ? 0 : a.counts ? a.counts[q] : a.tokens, length = fresh ? a.lengths[q] : 0;
+    const int *row = a.table + (size_t)q * a.table_pages;
+    int *slots = a.slots + (size_t)q * a.tokens;
+    auto slot = [&](int page, int at) { return (unsigned)page < (unsigned)a.pages ? page << a.shift | (at & mask) : -1; };
+    if (!(a.tokens & 3) && !(reinterpret_cast<uintptr_t>(a.slots) & 15)) {
+#pragma unroll
+        for (int i = from + 4 * lane; i < to; i += 128) {
+            int4 x = {-1, -1, -1, -1};
+            if (i < fresh) {
+                const int at = length + i, last = length + min(i + 3, fresh - 1);  // (on two pages at most)
+                const int first_page = at >> a.shift, p0 = row[first_page], p1 = row[last >> a.shift];
+                auto one = [&](int k) { return at + k > last ? -1 : slot((at + k) >> a.shift == first_page ? p0 : p1, at + k); };
+                x = make_int4(one(0), one(1), one(2), one(3));
+            }
+            *reinterpret_cast<int4 *>(slots + i) = x;
+        }
+    } else {
+#pragma unroll 4
+        for (int i = from + lane; i < to; i += 32) slots[i] = i < fresh ? slot(row[(length + i) >> a.shift], length + i) : -1;
+    }
+}
+
 int pages_args(const qg_page_pool *p, int *out, const int *lengths, int seqs, PagesArgs &a) {
     if (!p || !p->page_table || !p->held || !p->free_pages || !p->free_count || !out || !lengths || seqs < 1 || seqs > kMaxSeqs ||
         p->pages < 1 || p->table_pages < 1)
@@ -224,10 +254,15 @@ extern "C" int qg_pages_reserve(const qg_page_pool *pool, int *slots, int *taken
     PagesArgs a;
     if (int rc = pages_args(pool, taken, lengths, seqs, a)) return rc;
     if (tokens < 1 || (long long)seqs * tokens > 0x7fffffffll) return cudaErrorInvalidValue;
-    a.slots = slots;
+    const bool wide = slots && (long long)seqs * tokens > kWide;
+    a.slots = wide ? nullptr : slots;
     a.counts = counts;
     a.tokens = tokens;
-    return launch(reserve_kernel, a, (long long)seqs * tokens);
+    if (int rc = launch(reserve_kernel, a, slots && !wide ? (long long)seqs * tokens : (long long)seqs * 16)) return rc;
+    if (!wide) return cudaSuccess;
+    a.slots = slots;
+    const long long warps = (long long)seqs * ((tokens + kChunk - 1) / kChunk);
+    return launch_chained(slots_kernel, dim3((unsigned)((warps + 7) / 8)), 256, a);
 }
 
 extern "C" int qg_pages_release(const qg_page_pool *pool, int *freed, const int *lengths, int shared_pages, int seqs) {
