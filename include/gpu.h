@@ -354,8 +354,8 @@ int qg_cache_commit(const qg_kv_cache *cache, int *lengths_out, const int *path,
  * refused like one whose length is negative. Sequences, rows, masks, values that are not
  * finite and waits: as qg_tree_attention says, for which out is the same up to
  * rounding; a page outside the pool among the common ones makes every row NaN. The
- * workspace is zero-filled once, and is not that of qg_tree_attention.
- * seqs*tokens*q_heads is at most 2^24. */
+ * workspace is zero-filled once, and is not that of qg_tree_attention. out and q
+ * do not overlap. seqs*tokens*q_heads is at most 2^24. */
 int qg_shared_attention_workspace_bytes(int seqs, int tokens, int q_heads, int kv_heads, int head_dim, size_t *bytes);
 int qg_shared_attention(float *out, const float *q, const qg_kv_cache *cache, int layer, const int *shared, const uint64_t *tree,
                         float scale, int seqs, int tokens, int q_heads, void *workspace);
@@ -377,7 +377,8 @@ int qg_shared_attention(float *out, const float *q, const qg_kv_cache *cache, in
  * that is negative or not finite, or a NaN among its settings or its uniform
  * gets token -1.
  * Probabilities are taken relative to the largest, as whole multiples of 2^-44
- * of it, and their sums are exact: equal inputs give equal tokens. vocab at most
+ * of it (below 2^-45 of it they count as none), and their sums are exact: equal
+ * inputs give equal tokens. vocab at most
  * 360445, rows at most 2^20, logits 4-byte aligned. */
 int qg_sample(int *token, const float *logits, const float *uniforms, const float *temperature, const int *top_k, const float *top_p,
               const float *min_p, int per, int rows, int vocab);
@@ -411,14 +412,16 @@ typedef struct {
  * outside 0..table_pages). slots [seq][tokens] (may be NULL): the pool row of
  * each new position, -1 behind counts[s], for sequences that were refused
  * or got none, and where the row names a page outside the pool. A *free_count
- * outside 0..pages counts as 0. */
+ * outside 0..pages counts as 0. tokens at most 2^30, seqs*tokens below 2^31; taken
+ * is neither lengths nor counts. */
 int qg_pages_reserve(const qg_page_pool *pool, int *slots, int *taken, const int *lengths, const int *counts, int seqs, int tokens);
 /* Gives back what sequence s's first lengths[s] positions do not need (a negative
  * length: all), its first shared_pages entries excepted: the pages of the first
  * sequence end on top of the stack, each sequence's first one uppermost, so that reserving
  * again hands them out as before. freed[s]: pages given back, -1: refused (held outside
  * 0..table_pages; and every sequence with pages to give back where the stack would
- * hold more than the pool, or *free_count is negative: then nothing changes). */
+ * hold more than the pool, or *free_count is negative: then nothing changes).
+ * freed is not lengths. */
 int qg_pages_release(const qg_page_pool *pool, int *freed, const int *lengths, int shared_pages, int seqs);
 
 /* ---- loading an all-resident model (no counterpart in the reference

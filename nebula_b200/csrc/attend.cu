@@ -1846,7 +1846,9 @@ extern "C" int qg_shared_attention(float *out, const float *q, const qg_kv_cache
                                    float scale, int seqs, int tokens, int q_heads, void *workspace) {
     AttendArgs a;
     if (int rc = attend_args(a, out, q, cache, layer, tree, scale, seqs, tokens, q_heads, workspace)) return rc;
-    if (!shared || (long long)seqs * tokens * q_heads > kMaxShared) return cudaErrorInvalidValue;
+    if (!shared || (reinterpret_cast<uintptr_t>(shared) & 3) || (long long)seqs * tokens * q_heads > kMaxShared) return cudaErrorInvalidValue;
+    const float *const q_end = q + (size_t)seqs * tokens * q_heads * a.c.head_dim, *const out_end = out + (q_end - q);
+    if (out < q_end && q < out_end) return cudaErrorInvalidValue;  // out holds parts of rows while others' queries are read
     const int rows = seqs * tokens * a.group, d = a.c.head_dim;  // of the prefix
     const bool pair = d == 256 && rows > kRows;
     a.copies = 1;

@@ -207,9 +207,12 @@ __global__ void __launch_bounds__(256) slots_kernel(const __grid_constant__ Page
     }
 }
 
+template <typename... T>
+bool unaligned(const T *...p) { return ((reinterpret_cast<uintptr_t>(p) | ...) & 3) != 0; }
+
 int pages_args(const qg_page_pool *p, int *out, const int *lengths, int seqs, PagesArgs &a) {
     if (!p || !p->page_table || !p->held || !p->free_pages || !p->free_count || !out || !lengths || seqs < 1 || seqs > kMaxSeqs ||
-        p->pages < 1 || p->table_pages < 1)
+        p->pages < 1 || p->table_pages < 1 || out == lengths || unaligned(p->page_table, p->held, p->free_pages, p->free_count, out, lengths))
         return cudaErrorInvalidValue;
     a.shift = page_shift(p->page_tokens);
     if (a.shift < 0 || pool_too_large(p->pages, p->table_pages, a.shift)) return cudaErrorInvalidValue;
@@ -253,7 +256,8 @@ extern "C" int qg_pages_reserve(const qg_page_pool *pool, int *slots, int *taken
                                 int tokens) {
     PagesArgs a;
     if (int rc = pages_args(pool, taken, lengths, seqs, a)) return rc;
-    if (tokens < 1 || (long long)seqs * tokens > 0x7fffffffll) return cudaErrorInvalidValue;
+    if (tokens < 1 || tokens > 1 << 30 || (long long)seqs * tokens > 0x7fffffffll || (counts && counts == taken) || unaligned(slots, counts))
+        return cudaErrorInvalidValue;
     const bool wide = slots && (long long)seqs * tokens > kWide;
     a.slots = wide ? nullptr : slots;
     a.counts = counts;

@@ -856,11 +856,12 @@ int launch(SampleArgs &a, int rows) {
     return cudaLaunchKernelEx(&cfg, sample_kernel, a);
 }
 
-bool unaligned(const void *p) { return reinterpret_cast<uintptr_t>(p) & 3; }
+template <typename... T>
+bool unaligned(const T *...p) { return ((reinterpret_cast<uintptr_t>(p) | ...) & 3) != 0; }
 
 int settings(SampleArgs &a, const float *logits, const float *temperature, const int *top_k, const float *top_p, const float *min_p, int per,
              int rows, int vocab) {
-    if (!logits || unaligned(logits) || per < 1 || rows < 1 || rows > kRowsAtOnce || vocab < 1 || vocab > kMaxVocab - 3)
+    if (!logits || unaligned(logits, temperature, top_k, top_p, min_p) || per < 1 || rows < 1 || rows > kRowsAtOnce || vocab < 1 || vocab > kMaxVocab - 3)
         return cudaErrorInvalidValue;
     a.logits = logits;
     a.temperature = temperature;
@@ -881,7 +882,7 @@ extern "C" int qg_sample(int *token, const float *logits, const float *uniforms,
                          const float *min_p, int per, int rows, int vocab) {
     SampleArgs a;
     if (int rc = settings(a, logits, temperature, top_k, top_p, min_p, per, rows, vocab)) return rc;
-    if (!token || !uniforms) return cudaErrorInvalidValue;
+    if (!token || !uniforms || unaligned(token, uniforms)) return cudaErrorInvalidValue;
     a.token = token;
     a.uniforms = uniforms;
     return launch(a, rows);

@@ -76,6 +76,7 @@ class Speculator:
         self.masks, self.offsets = L.Device.empty(nodes, np.uint64), i(nodes)
         self.draft, self.parents, self.uniforms = i(nodes), i(nodes), f(nodes)
         self.path, self.accepted, self.next = i(nodes), i(1), i(1)
+        self.temperature, self.top_k, self.top_p, self.min_p = f(1), i(1), f(1), f(1)
         self.ids, self.route = i(nodes, 10), f(nodes, 10)
         self.moe_ws = L.workspace(nodes, hidden, ffn)
         self.attention_ws = L.attention_workspace(1, nodes, q_heads, kv_heads, head_dim)
@@ -103,6 +104,13 @@ class Speculator:
         t, d = len(tokens), self.head_dim
         self._put(self.masks, tree_masks(parents), np.uint64)
         self._put(self.offsets, depths(parents), np.int32)
+        self.layers_of(tokens, lambda layer: L.call(
+            "tree_attention", self.attended.p, self.q.p, C.byref(self.cache), layer, self.masks.p, d ** -0.5, 1, t, self.q_heads,
+            self.attention_ws.p), self.offsets.p, 1)
+
+    def layers_of(self, tokens, attend, offsets, seqs) -> None:
+        """The tokens' rows through every layer; ``attend(layer)`` is the attention."""
+        t, d = len(tokens), self.head_dim
         for n, token in enumerate(tokens):
             L.call("gather", self.x.p + 4 * n * self.hidden, self.embed.p, F32, self.hidden, int(token))
         for layer, w in enumerate(self.weights):
@@ -110,9 +118,8 @@ class Speculator:
             k = self.qkv.p + 4 * self.q_heads * d
             L.call("qk_norm_rope", self.q.p, C.byref(self.cache), layer, self.qkv.p, self.width, k, self.width,
                    k + 4 * self.kv_heads * d, self.width, self.q_weight.p, self.k_weight.p, 1e-6, self.rope.p, self.capacity,
-                   self.rotary, self.offsets.p, 1, t, self.q_heads)
-            L.call("tree_attention", self.attended.p, self.q.p, C.byref(self.cache), layer, self.masks.p, d ** -0.5, 1, t,
-                   self.q_heads, self.attention_ws.p)
+                   self.rotary, offsets, seqs, t // seqs, self.q_heads)
+            attend(layer)
             L.call("matmul", self.y.p, w["out"].p, F32, self.hidden, self.q_heads * d, self.attended.p, t)
             L.call("binary", self.x.p, self.x.p, self.y.p, t * self.hidden, 0)
             L.call("moe_layer", self.y.p, self.ids.p, self.route.p, self.x.p, t, w["router"].p, None, w["gate"].p, Q4_K, w["up"].p, Q4_K,
@@ -134,9 +141,10 @@ class Speculator:
             L.call("cache_commit", C.byref(self.cache), self.lengths.p, self.path.p, self.accepted.p, 1, len(part))
             self.committed += len(part)
 
-    def step(self, tokens, parents, uniforms=None, temperature=0.0):
+    def step(self, tokens, parents, uniforms=None, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0):
         """``tokens[0]`` is the last token chosen, the others are drafts. Returns the accepted nodes (the root first) and
-        the token after them; the accepted nodes' keys and values stay in the cache."""
+        the token after them; the accepted nodes' keys and values stay in the cache. ``top_k``, ``top_p`` and ``min_p`` truncate
+        the target's distribution first (0, 1 and 0: not at all)."""
         t = len(tokens)
         self._check(tokens, parents)
         uniforms = np.zeros(t) if uniforms is None else np.asarray(uniforms, np.float64)
@@ -144,6 +152,11 @@ class Speculator:
             raise ValueError(f"{t} uniforms in [0, 1)")
         self.forward(tokens, parents)
         L.call("matmul", self.logits.p, self.head.p, F32, self.vocab, self.hidden, self.x.p, t)
+        if top_k > 0 or top_p < 1 or min_p > 0:
+            for buf, value, kind in ((self.temperature, temperature, np.float32), (self.top_k, top_k, np.int32), (self.top_p, top_p, np.float32),
+                                     (self.min_p, min_p, np.float32)):
+                self._put(buf, [value], kind)
+            L.call("truncate_logits", self.logits.p, self.logits.p, self.temperature.p, self.top_k.p, self.top_p.p, self.min_p.p, t, t, self.vocab)
         self._put(self.draft, tokens, np.int32)
         self._put(self.parents, list(parents), np.int32)
         self._put(self.uniforms, np.minimum(uniforms, 1 - 2.0 ** -24), np.float32)  # none is rounded to 1

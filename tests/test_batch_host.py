@@ -27,12 +27,16 @@ def truncate(**over):
 SIZES = [dict(rows=0), dict(rows=-1), dict(rows=(1 << 20) + 1), dict(vocab=0), dict(vocab=360446), dict(per=0), dict(per=-2)]
 
 
-@pytest.mark.parametrize("over", [dict(token=None), dict(logits=None), dict(uniforms=None), dict(logits=P4 + 2), *SIZES], ids=str)
+UNALIGNED = [dict(logits=P4 + 2), dict(temperature=P4 + 1), dict(top_k=P4 + 2), dict(top_p=P4 + 3), dict(min_p=P4 + 2)]
+
+
+@pytest.mark.parametrize("over", [dict(token=None), dict(logits=None), dict(uniforms=None), dict(token=P4 + 2), dict(uniforms=P4 + 1), *UNALIGNED,
+                                  *SIZES], ids=str)
 def test_sample_refuses(over):
     assert sample(**over) == INVALID
 
 
-@pytest.mark.parametrize("over", [dict(out=None), dict(logits=None), dict(out=P4 + 1), dict(logits=P4 + 2), dict(out=P4 + 4),
+@pytest.mark.parametrize("over", [dict(out=None), dict(logits=None), dict(out=P4 + 1), *UNALIGNED, dict(out=P4 + 4),
                                   dict(out=P4 + 4 * 4 * 1000 - 4), dict(out=P4 - 4 * 4 * 1000 + 4), *SIZES], ids=str)
 def test_truncate_refuses(over):
     assert truncate(**over) == INVALID
@@ -45,20 +49,21 @@ def pool(**over):
 
 
 def reserve(p, **over):
-    f = dict(slots=P4, taken=P4, lengths=P4, counts=P4, seqs=3, tokens=5)
+    f = dict(slots=P4, taken=P4 + 4096, lengths=P4, counts=P4, seqs=3, tokens=5)
     f.update(over)
     return L.code("pages_reserve", p, *f.values())
 
 
 def release(p, **over):
-    f = dict(freed=P4, lengths=P4, shared=0, seqs=3)
+    f = dict(freed=P4 + 4096, lengths=P4, shared=0, seqs=3)
     f.update(over)
     return L.code("pages_release", p, *f.values())
 
 
 @pytest.mark.parametrize("over", [dict(page_table=None), dict(held=None), dict(free_pages=None), dict(free_count=None), dict(pages=0),
                                   dict(page_tokens=8), dict(page_tokens=20), dict(page_tokens=512), dict(table_pages=0),
-                                  dict(pages=1 << 27), dict(table_pages=1 << 27)], ids=str)
+                                  dict(pages=1 << 27), dict(table_pages=1 << 27), dict(page_table=P4 + 2), dict(held=P4 + 1),
+                                  dict(free_pages=P4 + 2), dict(free_count=P4 + 3)], ids=str)
 def test_pools_are_refused(over):
     assert reserve(pool(**over)) == INVALID
     assert release(pool(**over)) == INVALID
@@ -66,9 +71,11 @@ def test_pools_are_refused(over):
 
 def test_pages_refuse():
     assert reserve(None) == INVALID and release(None) == INVALID
-    for over in (dict(taken=None), dict(lengths=None), dict(seqs=0), dict(seqs=1025), dict(tokens=0), dict(seqs=1024, tokens=1 << 21)):
+    for over in (dict(taken=None), dict(lengths=None), dict(seqs=0), dict(seqs=1025), dict(tokens=0), dict(seqs=1024, tokens=1 << 21),
+                 dict(seqs=1, tokens=(1 << 30) + 1), dict(taken=P4 + 2), dict(slots=P4 + 1), dict(lengths=P4 + 2), dict(counts=P4 + 1),
+                 dict(taken=P4, lengths=P4, counts=None), dict(taken=P4 + 64, lengths=P4, counts=P4 + 64)):
         assert reserve(pool(), **over) == INVALID, over
-    for over in (dict(freed=None), dict(lengths=None), dict(seqs=0), dict(seqs=1025), dict(shared=-1), dict(shared=21)):
+    for over in (dict(freed=P4, lengths=P4), dict(freed=P4 + 2), dict(freed=None), dict(lengths=None), dict(seqs=0), dict(seqs=1025), dict(shared=-1), dict(shared=21)):
         assert release(pool(), **over) == INVALID, over
 
 
@@ -108,7 +115,7 @@ def cache(**over):
 
 
 def attention(c, **over):
-    f = dict(out=P4, q=P4, layer=0, shared=P4, tree=P4, scale=0.1, seqs=2, tokens=4, q_heads=8, ws=P4)
+    f = dict(out=P4 + (1 << 24), q=P4, layer=0, shared=P4, tree=P4, scale=0.1, seqs=2, tokens=4, q_heads=8, ws=P4)
     f.update(over)
     return L.code("shared_attention", f["out"], f["q"], c, f["layer"], f["shared"], f["tree"], f["scale"], f["seqs"], f["tokens"], f["q_heads"],
                   f["ws"])
@@ -123,6 +130,7 @@ def test_shared_attention_refuses_caches(over):
 
 @pytest.mark.parametrize("over", [dict(out=None), dict(q=None), dict(shared=None), dict(ws=None), dict(layer=-1), dict(layer=3), dict(q_heads=0),
                                   dict(q_heads=7), dict(q_heads=2048), dict(out=P4 + 8), dict(q=P4 + 4), dict(tree=P4 + 4), dict(ws=P4 + 8),
+                                  dict(out=P4), dict(out=P4 + 2 * 4 * 8 * 128 * 4 - 16), dict(out=P4, q=P4 + 16), dict(shared=P4 + 2),
                                   dict(seqs=0), dict(seqs=1025), dict(tokens=0), dict(tokens=65), dict(scale=float("inf")),
                                   dict(scale=float("nan")), dict(seqs=1024, tokens=64, q_heads=258)], ids=str)
 def test_shared_attention_refuses(over):

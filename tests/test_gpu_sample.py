@@ -201,3 +201,45 @@ def test_captured_and_replayed(L):
         for r in range(3):
             assert got[r] == B.sample(x[r], v[r], top_k=30, top_p=float(np.float32(0.9)))[0]
     L.graph_destroy(g)
+
+
+def test_fewer_logits_than_asked_for(L):
+    """top_k above the number of finite logits leaves them all, to top-p and min_p too."""
+    rng = np.random.default_rng(11)
+    x = np.full((6, 40000), -np.inf)
+    for r, n in enumerate((1, 2, 100, 300, 2000, 9000)):
+        x[r, rng.choice(40000, n, replace=False)] = rng.normal(size=n)
+    for k in (3, 200, 257, 1000, 5000, 39999):
+        check(L, x, rng.random(6), None, [k] * 6, [0.7] * 6)
+        check(L, x, rng.random(6), None, [k] * 6, None, [0.2] * 6)
+        check(L, x, rng.random(6), None, [k] * 6)
+
+
+def test_two_graphs_at_once(L):
+    """Calls share no memory but their arguments: graphs of both entry points replayed one after the other without a wait."""
+    import ctypes as C
+    rng = np.random.default_rng(12)
+    graphs, bufs = [], []
+    for n in range(2):
+        x = peaked(rng, 9, 30000).astype(np.float32)
+        u = rng.random(9).astype(np.float32)
+        d, out, token, du = L.Device(x), L.Device(np.zeros_like(x)), L.Device(np.zeros(9, np.int32)), L.Device(u)
+        p = L.Device(np.full(9, 0.9, np.float32))
+        g = C.c_void_p()
+        L.call("graph_begin", C.byref(g))
+        L.call("truncate_logits", out.p, d.p, None, None, p.p, None, 1, 9, 30000)
+        L.call("sample", token.p, d.p, du.p, None, None, p.p, None, 1, 9, 30000)
+        L.call("graph_end", g)
+        graphs.append(g)
+        bufs.append((x, u, d, out, token, du, p))
+    for _ in range(5):
+        for g in graphs:
+            L.call("graph_launch", g)
+    for x, u, _, out, token, _, _ in bufs:
+        cut, got = out.get(), token.get()
+        for r in range(9):
+            best, _, _ = B.kept(x[r], top_p=float(np.float32(0.9)))
+            assert set(np.flatnonzero(cut[r] > -np.inf)) == set(int(b) for b in best)
+            assert got[r] == B.sample(x[r], u[r], top_p=float(np.float32(0.9)))[0]
+    for g in graphs:
+        L.graph_destroy(g)

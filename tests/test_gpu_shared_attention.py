@@ -266,3 +266,85 @@ def test_attention_captured_and_replayed(L):  # noqa: F811
         L.call("graph_launch", g)
         assert_parity(out.get(), expected(cache, q, None, 0.1))
     L.graph_destroy(g)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(4, 4, 64), (6, 2, 64), (16, 4, 64), (4, 1, 128), (4, 2, 128), (32, 8, 128)])
+@pytest.mark.parametrize("page", [16, 256])
+def test_attention_single_tokens_of_few_heads(L, hq, hkv, d, page):  # noqa: F811
+    """The sequences' own keys without tensor cores: lengths around the eight keys of a warp, the unit and the page; tokens that see
+    themselves or not, refused sequences, bad pages, infinite queries."""
+    rng = np.random.default_rng(hq * d + page)
+    own = [0, 1, 6, 7, 8, 9, 119, 120, 127, 128, 129, 255, 1001, 3000]
+    cache = SharedCache(L, rng, 512, own, 1, hkv, d, page, layers=2)
+    q = (1.5 * rng.normal(size=(len(own), 1, hq, d))).astype(np.float32)
+    assert_parity(attend_shared(L, cache, q, None, d ** -0.5, layer=1, calls=3), expected(cache, q, None, d ** -0.5, layer=1))
+    masks = [[s % 2] for s in range(len(own))]
+    ref = expected(cache, q, masks, d ** -0.5)
+    for s in range(0, len(own), 2):  # what is not seen may be anything
+        at = cache.rows(s, cache.lengths[s], 1)
+        cache.k[0, at] = np.nan
+        cache.v[0, at, :, ::2] = np.inf
+    cache.upload()
+    got = attend_shared(L, cache, q, masks, d ** -0.5, calls=2)
+    assert_parity(got, ref)
+    q[3, 0, hq - 1, 5] = np.inf
+    again = attend_shared(L, cache, q, masks, d ** -0.5)
+    assert np.isnan(again[3, 0, hq - 1]).all()
+    again[3, 0, hq - 1] = got[3, 0, hq - 1]
+    np.testing.assert_array_equal(again, got)
+    table = cache.upload_table.copy()
+    table[12, 512 // page], table[13, 2048 // page] = cache.pages, -1
+    cache.dt.set(table)
+    now = np.array(cache.lengths, np.int32)
+    now[2], now[5], now[6] = -1, 1 << 20, 511
+    cache.dl.set(now)
+    again, bad = attend_shared(L, cache, q, masks, d ** -0.5), [2, 5, 6, 12, 13]
+    assert np.isnan(again[bad]).all()
+    keep = [s for s in range(len(own)) if s not in bad and s != 3]
+    assert_parity(again[keep], ref[keep])
+    table[0, 0] = -5  # a page of the prefix
+    cache.dt.set(table)
+    assert np.isnan(attend_shared(L, cache, q, masks, d ** -0.5)).all()
+
+
+def test_attention_single_tokens_of_few_heads_and_any_prefix(L):  # noqa: F811
+    """No prefix, one that is less than a unit, longer than some sequences, changed between replays of a graph."""
+    rng = np.random.default_rng(2)
+    cache = SharedCache(L, rng, 1024, [300, 0, 17, 900], 1, 8, 128, 32, hide=False)
+    q = rng.normal(size=(4, 1, 32, 128)).astype(np.float32)
+    ref = expected(cache, q, None, 0.1)
+    dq, out, ws = L.Device(q), L.Device.empty(q.shape, np.float32), L.shared_attention_workspace(4, 1, 32, 8, 128)
+    g = C.c_void_p()
+    L.call("graph_begin", C.byref(g))
+    L.call("shared_attention", out.p, dq.p, C.byref(cache.c), 0, cache.shared.p, None, 0.1, 4, 1, 32, ws.p)
+    L.call("graph_end", g)
+    for n, refused in ((1024, []), (0, []), (-7, []), (100, []), (1000, []), (128, []), (1025, [1]), (1 << 30, [0, 1, 2, 3]), (1024, [])):
+        cache.shared.set(np.array([n], np.int32))
+        L.call("graph_launch", g)
+        got, keep = out.get(), [s for s in range(4) if s not in refused]
+        assert np.isnan(got[refused]).all()
+        if keep:
+            assert_parity(got[keep], ref[keep])
+    L.graph_destroy(g)
+    # a row of zeros where nothing is there to see
+    cache = SharedCache(L, rng, 0, [0, 5], 1, 8, 128, 32)
+    got = attend_shared(L, cache, q[:2], [[0], [1]], 0.1)
+    assert np.array_equal(got[0], np.zeros_like(got[0]))
+    assert_parity(got[1], expected(cache, q[:2], [[0], [1]], 0.1)[1])
+
+
+def test_attention_spread_of_magnitudes(L):  # noqa: F811
+    """Maxima that lie thousands apart between the prefix and a sequence's own keys, either way."""
+    rng = np.random.default_rng(11)
+    for hq, tokens in ((8, 1), (32, 3)):
+        cache = SharedCache(L, rng, 256, [40, 300], tokens, 8, 128, 64)
+        cache.k[0, cache.rows(0, 0, 256), :, 0] = np.float16(2000.0)
+        cache.k[0, cache.rows(1, 300, 1), :, 1] = np.float16(30000.0)
+        cache.upload()
+        q = rng.normal(size=(2, tokens, hq, 128)).astype(np.float32)
+        q[..., :2] = 1.0
+        got, ref = attend_shared(L, cache, q, None, 1.0), expected(cache, q, None, 1.0)
+        # scores of up to 30,000 are off by some 30,000 * 2^-20 = 0.03 (22 bits of Q, sums cut off), and so are the weights: next to
+        # these far maxima all the weight lies on one key, or on 256 keys whose scores differ by their small values alone
+        assert np.abs(got - ref).max() <= 0.1 * np.abs(ref).max()
+        assert_parity(got[1], ref[1])
