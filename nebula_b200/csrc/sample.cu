@@ -46,8 +46,8 @@ using Whole = unsigned long long;
 
 // What the CTAs of a cluster read of each other.
 struct Shared {
-    Whole ends[kMaxRanks];             // keys of the largest logit, and of the threads' lowest
-    int index[kMaxRanks], last[2];
+    Whole ends[kMaxRanks];             // key of the largest logit; inverted, the lowest of the threads' largest, or its index
+    int last[2];
     Whole total[2][kMaxRanks];         // by the parity of the exchange: a CTA may be one ahead
     unsigned hist[2][3][kBins];        // by the parity of the pass: counts, or sums as 15 + 15 + 14 bits
     Whole list[kList];                 // key and inverted index: the larger is the better
@@ -583,20 +583,18 @@ __device__ void nucleus(Shared &s, Row &r, float p, float end, int &pass, int &t
     r.key = (unsigned)(worst >> 32), r.last = (int)~(unsigned)worst;
 }
 
-// A lower bound of the k-th largest logit, from the largest of each thread's (k logits are at least as large as the k-th
-// largest of these); -infinity where there is none.
-__device__ float bound_of(Shared &s, const Row &r, int k, float threads_most, float least, int &pass) {
-    const int tid = threadIdx.x;
-    Range in = {kNone, key_of(r.most), r.most, fminf((kBins - 1) / (r.most - least), 1e30f), kBins - 1, -1};
-    Hist &hist = s.hist[pass & 1];
-    if (threads_most >= least) add_to<false>(hist, in.bin_of(threads_most), 1);
-    cluster_sync();
-    const Whole count = all_bins<false>(s, r, hist);
+// Bins a quarter wide around the logits that models give, and the lowest logit of one. They serve to leave out most logits
+// early, before the largest is known: others take a pass more.
+__device__ __forceinline__ int plain_bin(float x) { return (int)fminf(fmaxf((24.0f - x) * 4.0f, 0.0f), (float)(kBins - 1)); }
+__device__ __forceinline__ float plain_edge(int bin) { return 24.0f - 0.25f * (bin + 1) - 1e-4f; }
+// A lower bound of the k-th largest logit, from bins of each thread's largest, in s.hist[0] (k logits are at least as large as
+// the k-th largest of these); -infinity where there is none. many: more than kFew logits are above it for sure.
+__device__ float bound_of(Shared &s, const Row &r, int k, bool &many, int &pass) {
+    const Whole count = all_bins<false>(s, r, s.hist[pass & 1]);
     pass++;  // (the next pass clears this histogram)
     const Bin b = reach_bin(s, count, k);
-    if (b.bin < 0) return -INFINITY;
-    in.take_bin(b.bin);
-    return of_key(in.low);
+    many = __syncthreads_or((int)threadIdx.x == b.bin && b.before + count > kFew);
+    return b.bin < 0 || b.bin == kBins - 1 ? -INFINITY : plain_edge(b.bin);
 }
 
 // One row, by one cluster.
@@ -607,14 +605,13 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
     const int ahead = (int)(reinterpret_cast<uintptr_t>(x0) >> 2 & 3);  // logits between a multiple of 16 bytes and the row
     const int start = (int)r.rank * a.units * kStep - ahead;
     r.index = start + tid * 4 * a.units;
-    for (int i = tid; i < 2 * 3 * kBins; i += kThreads) s.hist[0][0][i] = 0;
-    if (tid == 0) s.listed = 0;
     const float t = a.temperature ? a.temperature[user] : 1.0f, p = a.top_p ? a.top_p[user] : 1.0f, least = a.min_p ? a.min_p[user] : 0.0f;
     const int k = a.top_k ? a.top_k[user] : 0;
     const float u = a.uniforms ? a.uniforms[row] : 0.0f;
 
     // ---- the row, and its largest logit. A warp copies its threads' units, neighbouring ones at a time.
     float most = -INFINITY;
+    __syncwarp();  // (its lanes are done with the row before)
     {
         float4 *const to = part + warp * 32 * stride;
         const int from = start + warp * 32 * 4 * a.units;
@@ -650,24 +647,44 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
             asm volatile("prefetch.global.L2 [%0];" ::"l"(x1 + i));
     }
     const float threads_most = most;
-    // (as keys: a NaN's is above all)
-    unsigned top = key_of(most), low = most > -INFINITY ? top : ~0u;  // the lowest: of the threads' largest, for top-k
+    // ---- the largest logit of all (as a key: a NaN's is above all), with temperature 0 its lowest index too. For top-k, bins of the
+    // threads' largest go along.
+    unsigned top = key_of(most), low = most > -INFINITY ? top : ~0u;  // the lowest: of the threads' largest
     top = __reduce_max_sync(0xffffffffu, top);
     low = __reduce_min_sync(0xffffffffu, low);
     if (lane == 0) s.warp_most[warp] = top, s.warp_least[warp] = low;
+    // (what this CTA's memory held of the row before is read by others until they are here)
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    for (int i = tid; i < 2 * 3 * kBins; i += kThreads) s.hist[0][0][i] = 0;
+    if (tid == 0) s.listed = 0;
     __syncthreads();
-    if (warp == 0) {
-        top = __reduce_max_sync(0xffffffffu, lane < kWarps ? s.warp_most[lane] : 0);
-        low = __reduce_min_sync(0xffffffffu, lane < kWarps ? s.warp_least[lane] : ~0u);
-        if (lane < r.ranks) peer_store(at_rank(&s.ends[r.rank], lane), (Whole)top << 32 | low);
+    top = __reduce_max_sync(0xffffffffu, lane < kWarps ? s.warp_most[lane] : 0);
+    low = __reduce_min_sync(0xffffffffu, lane < kWarps ? s.warp_least[lane] : ~0u);
+    const bool cut_k = k > 0 && k < a.vocab && t > 0.0f;
+    if (t == 0.0f) {
+        unsigned index = 0x7fffffff;
+        r.some(of_key(top), of_key(top), [&](const float (&x)[2], const int (&at)[2]) {
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+                if (x[e] == of_key(top)) index = min(index, (unsigned)at[e]);
+        });
+        index = __reduce_min_sync(0xffffffffu, index);
+        if (lane == 0) s.warp_sum[warp] = index;
+        __syncthreads();
+        low = __reduce_min_sync(0xffffffffu, lane < kWarps ? (unsigned)s.warp_sum[lane] : 0x7fffffffu);
+    } else if (cut_k && threads_most > -INFINITY) {
+        atomicAdd(&s.hist[0][0][plain_bin(threads_most)], 1u);
     }
+    if (warp == 0 && lane < r.ranks) peer_store(at_rank(&s.ends[r.rank], lane), (Whole)top << 32 | ~low);
     cluster_sync();
-    top = 0, low = ~0u;
+    // of equal keys the lowest index; without temperature 0, the lowest of all
+    Whole end = 0;
+    unsigned least_key = ~0u;
 #pragma unroll
     for (int i = 0; i < kMaxRanks; i++)
-        if (i < r.ranks) top = max(top, (unsigned)(s.ends[i] >> 32)), low = min(low, (unsigned)s.ends[i]);
-    most = of_key(top);
-    const float lowest = low == ~0u ? most : of_key(low);
+        if (i < r.ranks) end = max(end, s.ends[i]), least_key = min(least_key, ~(unsigned)s.ends[i]);
+    most = of_key((unsigned)(end >> 32));
+    const float lowest = least_key == ~0u ? most : of_key(least_key);
     const bool refused = !(most > -INFINITY && most < INFINITY) || !(t >= 0.0f && t < INFINITY) || p != p || least != least || u != u;
 
     // ---- what is kept
@@ -686,28 +703,15 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
     int token = -1;  // where it is known already
     if (refused) {
     } else if (t == 0.0f) {  // the largest logit, the lowest index of equals
-        int index = 0x7fffffff;
-        r.some(most, most, [&](const float (&x)[2], const int (&at)[2]) {
-#pragma unroll
-            for (int e = 0; e < 2; e++)
-                if (x[e] == most) index = min(index, at[e]);
-        });
-        index = __reduce_min_sync(0xffffffffu, index);
-        if (lane == 0) s.warp_sum[warp] = index;
-        __syncthreads();
-        if (warp == 0) {
-            index = __reduce_min_sync(0xffffffffu, lane < kWarps ? (int)s.warp_sum[lane] : 0x7fffffff);
-            if (lane < r.ranks) peer_store(at_rank(&s.index[r.rank], lane), (unsigned)index);
-        }
-        cluster_sync();
-        r.key = key_of(most), r.last = 0x7fffffff;
-        for (uint32_t i = 0; i < r.ranks; i++) r.last = min(r.last, s.index[i]);
+        r.key = key_of(most), r.last = (int)~(unsigned)end;
         token = r.last;
     } else {
         bool done = false;
-        if (k > 0 && k < a.vocab) {
-            const float bound = bound_of(s, r, k, threads_most, lowest, pass);
-            const int n = k <= kFew ? gather(s, r, {key_of(fmaxf(bound, kLowest)), key_of(most), most, 0.0f, 0, -1}) : kFew + 1;
+        if (cut_k) {
+            int n = kFew + 1;
+            bool many;
+            const float bound = bound_of(s, r, k, many, pass);
+            if (!many && bound > -INFINITY) n = gather(s, r, {key_of(bound), key_of(most), most, 0.0f, 0, -1});
             if (n <= kFew) {
                 // few enough: all of the rest is in every CTA's own memory
                 Whole above;
@@ -811,13 +815,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     r.rank = cluster_rank(), r.ranks = cluster_size();
     r.units = a.units;
     r.mine = part + threadIdx.x * (a.units | 1);
-    cluster_sync();  // a CTA's memory is there for others once it runs
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");  // a CTA's memory is there for others once it runs
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int clusters = gridDim.x / r.ranks;
     for (int row = blockIdx.x / r.ranks; row < a.rows; row += clusters) {
         do_row(a, s, part, r, row, row + clusters);
-        cluster_sync();  // no CTA goes on, or ends, while others read its memory
+        asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     }
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // no CTA ends while others read its memory
 }
 
 int launch(SampleArgs &a, int rows) {
