@@ -815,12 +815,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     r.rank = cluster_rank(), r.ranks = cluster_size();
     r.units = a.units;
     r.mine = part + threadIdx.x * (a.units | 1);
-    asm volatile("barrier.cluster.arrive.release;" ::: "memory");  // a CTA's memory is there for others once it runs
+    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");  // a CTA's memory is there for others once it runs
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int clusters = gridDim.x / r.ranks;
     for (int row = blockIdx.x / r.ranks; row < a.rows; row += clusters) {
         do_row(a, s, part, r, row, row + clusters);
-        asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+        // (nothing is handed over: others' memory was read, and what was read is used. A release would wait for the row's stores.)
+        asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
     }
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // no CTA ends while others read its memory
 }
