@@ -28,11 +28,11 @@ constexpr int kFewer = 64;                        // the same where one of a lis
 constexpr int kList = 1024;                       // logits that every CTA has a list of
 constexpr int kStep = kThreads * 4;               // a CTA's part of a row is a multiple of this: a thread has whole units of four
 constexpr int kMaxUnits = 22;                     // of a thread: 188 KB a CTA
-constexpr int kMaxRanks = 8;                      // CTAs of a cluster
-constexpr int kMaxVocab = kMaxRanks * kMaxUnits * kStep;
+constexpr int kMaxRanks = 16;                     // CTAs of a cluster
+constexpr int kMaxVocab = 8 * kMaxUnits * kStep;
 constexpr int kRowsAtOnce = 1 << 20;
 static_assert(kMaxVocab <= 1 << 19, "sums of weights, 2^44 at most, fit 63 bits");
-static_assert(kMaxRanks == 8 && 2 * kFew <= kThreads && 4 * kBins == kThreads, "two threads to a logit that is ordered, four to a bin");
+static_assert(kMaxRanks == kWarps && kMaxRanks % 4 == 0 && 2 * kFew <= kThreads && 4 * kBins == kThreads, "two threads to a logit that is ordered, four to a bin");
 
 struct SampleArgs {
     const float *logits, *uniforms, *temperature, *top_p, *min_p;
@@ -58,9 +58,7 @@ struct Shared {
     Whole warp_sum[kWarps], entry_weight[kFew];
     union {
         Whole entry[kList];
-        struct {  // until a list is read
-            Whole bins[4][kBins], read[2][kMaxRanks][32];
-        };
+        Whole bins[4][kBins], read[2][kMaxRanks][32];  // until a list is read
     };
     Whole found, kept_sum;
     int few;
@@ -315,20 +313,22 @@ __device__ __forceinline__ void add_to(Hist &hist, int bin, Whole w) {
         atomicAdd(&hist[0][bin], 1u);
     }
 }
-// One histogram of all CTAs' added up: bin tid's, for tid < kBins. Four threads to a bin read, two CTAs' each.
+// One histogram of all CTAs' added up: bin tid's, for tid < kBins. Four threads to a bin read, a quarter of the CTAs' each.
 template <bool SUM>
 __device__ __forceinline__ Whole all_bins(Shared &s, const Row &r, const Hist &hist) {
     const int bin = threadIdx.x % kBins, group = threadIdx.x / kBins;
     constexpr int N = SUM ? 3 : 1;
-    unsigned part[2][N];
+    Whole sum = 0;
+#pragma unroll 1
+    for (uint32_t q0 = group; q0 < r.ranks; q0 += 8) {
+        unsigned part[2][N];
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const uint32_t q = 2 * group + i;
+        for (int i = 0; i < 2; i++)
 #pragma unroll
-        for (int e = 0; e < N; e++) part[i][e] = q < r.ranks ? peer_load(at_rank(&hist[e][bin], q)) : 0;
+            for (int e = 0; e < N; e++) part[i][e] = q0 + 4 * i < r.ranks ? peer_load(at_rank(&hist[e][bin], q0 + 4 * i)) : 0;
+        sum += (Whole)part[0][0] + part[1][0];
+        if constexpr (SUM) sum += (((Whole)part[0][1] + part[1][1]) << 15) + (((Whole)part[0][2] + part[1][2]) << 30);
     }
-    Whole sum = (Whole)part[0][0] + part[1][0];
-    if constexpr (SUM) sum += (((Whole)part[0][1] + part[1][1]) << 15) + (((Whole)part[0][2] + part[1][2]) << 30);
     s.bins[group][bin] = sum;
     __syncthreads();
     return threadIdx.x < kBins ? (s.bins[0][bin] + s.bins[1][bin]) + (s.bins[2][bin] + s.bins[3][bin]) : 0;
@@ -367,18 +367,25 @@ __device__ int gather(Shared &s, const Row &r, const Range &in) {
             }
     });
     cluster_sync();
-    int n[kMaxRanks], all = 0;
+    // a lane has a CTA's number, and where its part of the list begins
+    const int lane = threadIdx.x & 31, n = lane < r.ranks ? (int)peer_load(at_rank(&s.listed, lane)) : 0;
+    int upto = n;
 #pragma unroll
-    for (int q = 0; q < kMaxRanks; q++) n[q] = q < r.ranks ? (int)peer_load(at_rank(&s.listed, q)) : 0;
-#pragma unroll
-    for (int q = 0; q < kMaxRanks; q++) all += n[q];
+    for (int d = 1; d < kMaxRanks; d <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += x;
+    }
+    const int all = __shfl_sync(0xffffffffu, upto, kMaxRanks - 1);
     if (all > kList) return all;
-    for (int i = threadIdx.x; i < all; i += kThreads) {
-        int q = 0, at = i;
+    for (int i0 = threadIdx.x & ~31; i0 < all; i0 += kThreads) {
+        const int i = i0 + lane;
+        int q = 0, from = 0;
 #pragma unroll
-        for (int e = 0; e < kMaxRanks - 1; e++)
-            if (q == e && at >= n[e]) at -= n[e], q++;
-        s.entry[i] = peer_load64(at_rank(&s.list[at], q));
+        for (int e = 0; e < kMaxRanks - 1; e++) {
+            const int end = __shfl_sync(0xffffffffu, upto, e);
+            if (i >= end) q = e + 1, from = end;
+        }
+        if (i < all) s.entry[i] = peer_load64(at_rank(&s.list[i - from], q));
     }
     __syncthreads();
     return all;
@@ -554,8 +561,10 @@ __device__ void nucleus(Shared &s, Row &r, float p, float end, int &pass, int &t
     auto find = [&](Whole (&from)[kMaxRanks][32], Whole &target) {
         __syncthreads();
         Whole mine = 0;
+#pragma unroll 1
+        for (uint32_t q0 = 0; q0 < r.ranks; q0 += 8)  // (zeros where there is no CTA)
 #pragma unroll
-        for (int q = 0; q < kMaxRanks; q++) mine += from[q][lane];
+            for (int q = 0; q < 8; q++) mine += from[q0 + q][lane];
         const Whole upto = warp_scan(mine);
         const unsigned past = __ballot_sync(0xffffffffu, upto >= target);
         if (!past) return -1;
@@ -563,16 +572,14 @@ __device__ void nucleus(Shared &s, Row &r, float p, float end, int &pass, int &t
         target -= __shfl_sync(0xffffffffu, upto - mine, l);
         return l;
     };
-    if (warp < kMaxRanks) s.read[0][warp][lane] = warp < r.ranks ? peer_load64(at_rank(&s.coarse[lane], warp)) : 0;
+    s.read[0][warp][lane] = warp < r.ranks ? peer_load64(at_rank(&s.coarse[lane], warp)) : 0;
     const int group = find(s.read[0], target);
     if (group < 0) return;  // all of them
-    if (warp < kMaxRanks) {
-        unsigned part[3] = {0, 0, 0};
-        if (warp < r.ranks)
+    unsigned part[3] = {0, 0, 0};
+    if (warp < r.ranks)
 #pragma unroll
-            for (int e = 0; e < 3; e++) part[e] = peer_load(at_rank(&s.fine[e][32 * group + lane], warp));
-        s.read[1][warp][lane] = part[0] + ((Whole)part[1] << 15) + ((Whole)part[2] << 30);
-    }
+        for (int e = 0; e < 3; e++) part[e] = peer_load(at_rank(&s.fine[e][32 * group + lane], warp));
+    s.read[1][warp][lane] = part[0] + ((Whole)part[1] << 15) + ((Whole)part[2] << 30);
     in.take_bin(32 * group + find(s.read[1], target));
     const int n = gather(s, r, in);
     if (n > kList) {
@@ -680,9 +687,8 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
     // of equal keys the lowest index; without temperature 0, the lowest of all
     Whole end = 0;
     unsigned least_key = ~0u;
-#pragma unroll
-    for (int i = 0; i < kMaxRanks; i++)
-        if (i < r.ranks) end = max(end, s.ends[i]), least_key = min(least_key, ~(unsigned)s.ends[i]);
+#pragma unroll 1
+    for (int i = 0; i < r.ranks; i++) end = max(end, s.ends[i]), least_key = min(least_key, ~(unsigned)s.ends[i]);
     most = of_key((unsigned)(end >> 32));
     const float lowest = least_key == ~0u ? most : of_key(least_key);
     const bool refused = !(most > -INFINITY && most < INFINITY) || !(t >= 0.0f && t < INFINITY) || p != p || least != least || u != u;
@@ -831,20 +837,22 @@ int launch(SampleArgs &a, int rows) {
     const bool aligned = !(reinterpret_cast<uintptr_t>(a.logits) & 15) && a.vocab % 4 == 0;
     const int long_row = a.vocab + (aligned ? 0 : 3);
     // Clusters of more CTAs take less time for a row, but fewer of them fit. A row takes about as long for its fixed steps
-    // as for seven units of a thread, and the GPU takes 33, 71, 148 or 296 clusters of 8, 4, 2 or 1 CTAs (15, 33, 74 and 148 where a
-    // CTA has more than half an SM's memory) at once.
+    // as for seven units of a thread (eight with 16 CTAs, which should have an SM each), and the GPU takes 33, 71, 148 or 296 clusters
+    // of 8, 4, 2 or 1 CTAs (15, 33, 74 and 148 where a CTA has more than half an SM's memory) at once. A nucleus among 131,072, one
+    // row: 23 us with 8, 19 with 16; 14 rows: 24 and 26. 37 rows of 50,001 with top-k 40: 18 us with 8, 13 with 4.
     int ranks = 1, clusters = 1;
     long long best = 0;
     for (int n = 1; n <= kMaxRanks; n *= 2) {
         const int units = ((long_row + n - 1) / n + kStep - 1) / kStep;
         if (units > kMaxUnits) continue;
         const bool half = kThreads * (units | 1) * 16 + (int)sizeof(Shared) <= 115200;
-        const int fit = n == 8 ? (half ? 33 : 15) : n == 4 ? (half ? 71 : 33) : (half ? 296 : 148) / n;
-        const long long time = (long long)((rows + fit - 1) / fit) * (7 + units);
+        const int fit = n == 16 ? 7 : n == 8 ? (half ? 33 : 15) : n == 4 ? (half ? 71 : 33) : (half ? 296 : 148) / n;
+        const long long time = (long long)((rows + fit - 1) / fit) * (7 + (n == 16) + units);
         if (!best || time < best) best = time, ranks = n, clusters = rows < fit ? rows : fit, a.units = units;
     }
     const int smem = kThreads * (a.units | 1) * 16 + (int)sizeof(Shared);
     if (int rc = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return rc;
+    if (int rc = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) return rc;
     a.rows = rows;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(kThreads);
