@@ -70,10 +70,13 @@ struct AttendArgs {
     float *prefix_acc;   // [row][q_heads][D], [row][q_heads]: of prefix items that one CTA did as a whole
     float2 *prefix_ml;
     float2 *own_ml;      // the same of sequences' items, whose sums are in out
+    float *own_part_acc;  // parts of sequences' items: part_acc, or where their line is one of its own
+    float2 *own_part_ml;  // [2 * kGroups * kMaxCtas][kFewRows]
+    int own_part_rows;
     // for the join: the slots before each sequence's, all of the sequences' line, all of the prefix's (the same line, or one of its
-    // own); own_length of each sequence, the common positions, the CTAs of both lines, the first CTA of the sequences' line
+    // own); own_length of each sequence, the common positions, the CTAs (or groups) of both lines
     long long *starts;   // [seqs + 2]
-    int *lengths;        // [seqs + 4]
+    int *lengths;        // [seqs + 3]
 };
 
 constexpr int kChunk = 32;       // keys per step of the softmax
@@ -436,8 +439,7 @@ struct Walk {
 
 // One warp: what the join needs to find every row's parts. `line`: slots before the first sequence's.
 template <int D>
-__device__ void tell_join(const AttendArgs &a, int shared, int common, long long line, long long own_w, long long prefix_w, int own_g, int prefix_g,
-                          int first) {
+__device__ void tell_join(const AttendArgs &a, int shared, int common, long long line, long long own_w, long long prefix_w, int own_g, int prefix_g) {
     const int lane = threadIdx.x & 31;
     for (int s0 = 0; s0 < a.seqs; s0 += 32) {
         const int q = s0 + lane, own = q < a.seqs ? own_length<true>(a, q, shared, common) : -1;
@@ -454,7 +456,7 @@ __device__ void tell_join(const AttendArgs &a, int shared, int common, long long
     if (lane == 0) {
         a.starts[a.seqs] = own_w, a.starts[a.seqs + 1] = prefix_w;
         int *to = a.lengths + a.seqs;
-        to[0] = common, to[1] = own_g, to[2] = prefix_g, to[3] = first;
+        to[0] = common, to[1] = own_g, to[2] = prefix_g;
     }
 }
 
@@ -489,7 +491,7 @@ __device__ __forceinline__ void plan(const AttendArgs &a, Plan &s, int team, int
         s.pos0 = (int)(u0 - base - (long long)index * slots);
         s.common = common, s.source = source;
     }
-    if (SHARED && team == 0 && blockIdx.x == 0) tell_join<D>(a, shared, common, line, w, w, g, g, 0);
+    if (SHARED && team == 0 && blockIdx.x == 0) tell_join<D>(a, shared, common, line, w, w, g, g);
 }
 
 // Of an item: the rows of q that are its own, counted from its first sequence's; where its keys begin; whose pages they are on.
@@ -1244,26 +1246,28 @@ __device__ __forceinline__ void eight(const unsigned char *p, float (&x)[8], boo
     }
 }
 
-struct FewNotes : Plan {
-    float2 ml[kFewWarps][kFewRows];
-};
-// What the CTA's plan says.
-template <int D, bool SHARED>
-__device__ __forceinline__ void attend_token(const AttendArgs &a, unsigned char *smem, FewNotes &s) {
+template <int D>
+__global__ void __launch_bounds__(32 * kFewWarps, 1) token_attention_kernel(const __grid_constant__ AttendArgs a) {
     using C = Few<D>;
-    float2 (&ml)[kFewWarps][kFewRows] = s.ml;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    __shared__ Plan s;
+    __shared__ float2 ml[kFewWarps][kFewRows];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, team = blockIdx.x;
     const int key = lane / C::kLanes, dim = lane % C::kLanes * 8;
     const float nan = __int_as_float(0x7fc00000);
-    if constexpr (!SHARED)  // (with a shared prefix, the join's)
-        for (int q = team; q < a.seqs; q += gridDim.x)  // rows of refused sequences
-            if (a.c.committed(q, 1) < 0)
-                for (int i = tid; i < a.q_heads * D; i += 32 * kFewWarps) a.out[(size_t)q * a.q_heads * D + i] = nan;
+    if (warp == 0) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        plan<D, false>(a, s, team, gridDim.x);
+    }
+    __syncthreads();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    for (int q = team; q < a.seqs; q += gridDim.x)  // rows of refused sequences
+        if (a.c.committed(q, 1) < 0)
+            for (int i = tid; i < a.q_heads * D; i += 32 * kFewWarps) a.out[(size_t)q * a.q_heads * D + i] = nan;
     unsigned char *const ring = smem + warp * C::kStages * C::kStage + lane * 16;
     float *const sums = reinterpret_cast<float *>(smem + C::kRing);
     const size_t width = (size_t)a.c.kv_heads * D;
-    const int base0 = SHARED ? s.common : 0;  // where the items' positions begin
-    Walk<D, SHARED> walk(s);
+    Walk<D, false> walk(s);
     Item it;
     while (walk.next(a, it)) {
         const int all = it.length + 1, n = it.length + (a.tree ? (int)(a.tree[it.seq] & 1) : 1);  // keys there, keys seen
@@ -1275,7 +1279,7 @@ __device__ __forceinline__ void attend_token(const AttendArgs &a, unsigned char 
             if (t < it.count) {
                 if (!(t & 31)) {  // the pages of the next 32 units, a lane each
                     const int at = first + (t + lane) * kKeys;
-                    page = t + lane < it.count && at < all ? table[(base0 + at) >> a.c.shift] : 0;
+                    page = t + lane < it.count && at < all ? table[at >> a.c.shift] : 0;
                     if ((unsigned)page >= (unsigned)a.c.pages) bad = true, page = 0;
                 }
                 const int p = __shfl_sync(0xffffffffu, page, t & 31), base = first + t * kKeys;
@@ -1396,14 +1400,9 @@ __device__ __forceinline__ void attend_token(const AttendArgs &a, unsigned char 
                 total += f * x.y;
                 sum = fmaf(f, sums[(w * kFewRows + r) * D + d], sum);
             }
-            if (SHARED) sum *= kPScale, total *= kPScale;  // as the prefix's parts are
             if (bad) sum = nan;
-            const size_t at = (size_t)it.seq * a.q_heads + it.kv * a.group + r;
-            if (SHARED && whole) {  // for the join
-                a.out[at * D + d] = sum;
-                if (d == 0) a.own_ml[at] = make_float2(most, total);
-            } else if (whole) {
-                a.out[at * D + d] = total == 0.0f && !bad ? 0.0f : sum / total;
+            if (whole) {
+                a.out[((size_t)it.seq * a.q_heads + it.kv * a.group + r) * D + d] = total == 0.0f && !bad ? 0.0f : sum / total;
             } else {
                 a.part_acc[(part + r) * D + d] = sum;
                 if (d == 0) a.part_ml[part + r] = make_float2(most, total);
@@ -1413,42 +1412,195 @@ __device__ __forceinline__ void attend_token(const AttendArgs &a, unsigned char 
     }
 }
 
+// The same with a shared prefix, for the sequences' own keys: these are few, and an item's start and end would be most of its
+// time. So a CTA works on four items at once: a group of four warps on one, warp w of them on keys 8w .. 8w+7 of every 32.
+constexpr int kGroups = 4, kGroupWarps = kFewWarps / kGroups, kGroupKeys = 8 * kGroupWarps;
+struct GroupNotes {
+    Plan plan[kGroups];
+    float2 ml[kFewWarps][kFewRows];
+};
 template <int D>
-__global__ void __launch_bounds__(32 * kFewWarps, 1) token_attention_kernel(const __grid_constant__ AttendArgs a) {
-    extern __shared__ __align__(1024) unsigned char smem[];
-    __shared__ FewNotes s;
-    if (threadIdx.x < 32) {
-        asm volatile("griddepcontrol.wait;" ::: "memory");
-        plan<D, false>(a, s, blockIdx.x, gridDim.x);
+__device__ __forceinline__ void attend_tokens(const AttendArgs &a, unsigned char *smem, GroupNotes &notes, int team) {
+    using C = Few<D>;
+    constexpr int kSteps = kKeys / kGroupKeys;  // to a unit
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = warp / kGroupWarps, tid = threadIdx.x % (32 * kGroupWarps);
+    const int key = lane / C::kLanes, dim = lane % C::kLanes * 8;
+    const float nan = __int_as_float(0x7fc00000);
+    const Plan &s = notes.plan[group];
+    float2 (*const ml)[kFewRows] = notes.ml + group * kGroupWarps;
+    unsigned char *const ring = smem + warp * C::kStages * C::kStage + lane * 16;
+    float *const sums = reinterpret_cast<float *>(smem + C::kRing) + group * kGroupWarps * kFewRows * D;
+    const size_t width = (size_t)a.c.kv_heads * D;
+    const int base0 = s.common;  // where the items' positions begin
+    Walk<D, true> walk(s);
+    Item it;
+    while (walk.next(a, it)) {
+        const int all = it.length + 1, n = it.length + (a.tree ? (int)(a.tree[it.seq] & 1) : 1);  // keys there, keys seen
+        const int first = it.first * kKeys + 8 * (warp % kGroupWarps), steps = it.count * kSteps;
+        const int *table = a.c.table + (size_t)it.seq * a.c.table_pages;
+        bool bad = false;
+        int page = 0;
+        auto issue = [&](int t) {
+            if (t < steps) {
+                if (!(t & 31)) {  // the pages of the next 32 steps, a lane each
+                    const int at = first + (t + lane) * kGroupKeys;
+                    page = t + lane < steps && at < all ? table[(base0 + at) >> a.c.shift] : 0;
+                    if ((unsigned)page >= (unsigned)a.c.pages) bad = true, page = 0;
+                }
+                const int p = __shfl_sync(0xffffffffu, page, t & 31), base = first + t * kGroupKeys;
+                if (base < all) {  // (the 8 rows lie in one page)
+                    const size_t row = ((size_t)p << a.c.shift) + (base & (a.c.page_tokens() - 1)) + key;
+                    const size_t off = row * width + (size_t)it.kv * D + dim;
+                    const uint32_t to = smem_u32(ring + t % C::kStages * C::kStage);
+#pragma unroll
+                    for (int i = 0; i < C::kLoads; i++)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i * 512), "l"(a.c.k + off + i * C::kPer * width) : "memory");
+#pragma unroll
+                    for (int i = 0; i < C::kLoads; i++)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (C::kLoads + i) * 512), "l"(a.c.v + off + i * C::kPer * width) : "memory");
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int t = 0; t < C::kStages - 1; t++) issue(t);
+        float q[kFewRows][8], acc[kFewRows][8], m = -INFINITY, l = 0.0f;  // m and l: of row lane % 4
+#pragma unroll
+        for (int r = 0; r < kFewRows; r++) {
+            const float *src = a.q + ((size_t)it.seq * a.q_heads + it.kv * a.group + min(r, a.group - 1)) * D + dim;
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) *reinterpret_cast<float4 *>(&q[r][e]) = *reinterpret_cast<const float4 *>(src + e);
+#pragma unroll
+            for (int e = 0; e < 8; e++) q[r][e] *= a.scale * a.sign, acc[r][e] = 0.0f;
+        }
+#pragma unroll 1
+        for (int t = 0; t < steps; t++) {
+            __syncwarp();  // what was read from the place of the unit before is read
+            issue(t + C::kStages - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
+            const int base = first + t * kGroupKeys;
+            if (base >= all) break;  // and so are the steps after it
+            const unsigned char *k = ring + t % C::kStages * C::kStage, *v = k + C::kLoads * 512;
+            float x[C::kLanes];
+#pragma unroll
+            for (int i = 0; i < C::kLoads; i++) {
+                float f[8];
+                eight(k + i * 512, f);
+#pragma unroll
+                for (int r = 0; r < kFewRows; r++) {
+                    float dot = q[r][0] * f[0];
+#pragma unroll
+                    for (int e = 1; e < 8; e++) dot = fmaf(q[r][e], f[e], dot);
+                    x[i * kFewRows + r] = dot;
+                }
+            }
+#pragma unroll
+            for (int o = C::kLanes / 2; o; o >>= 1) {
+#pragma unroll
+                for (int j = 0; j < o; j++) {
+                    const float mine = lane & o ? x[j + o] : x[j], other = lane & o ? x[j] : x[j + o];
+                    x[j] = mine + __shfl_xor_sync(0xffffffffu, other, o);
+                }
+            }
+            // the lane's score: row lane % 4 and key
+            const int at = base + lane % C::kLanes / kFewRows * C::kPer + key;
+            const float score = at < n ? x[0] : -INFINITY;
+            float top = score;
+#pragma unroll
+            for (int o = kFewRows; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            top = fmaxf(m, top);
+            if (__any_sync(0xffffffffu, top > m)) {
+                const float keep = m == -INFINITY ? 0.0f : ex2(m - top);
+                l *= keep;
+                m = top;
+#pragma unroll
+                for (int r = 0; r < kFewRows; r++) {
+                    const float f = __shfl_sync(0xffffffffu, keep, r);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) acc[r][e] *= f;
+                }
+            }
+            const float p = ex2(score - (m == -INFINITY ? 0.0f : m));
+            l += p;
+#pragma unroll
+            for (int i = 0; i < C::kLoads; i++) {
+                float f[8];
+                eight(v + i * 512, f, base + i * C::kPer + key >= n);  // unseen values are any: P = 0 would not keep a NaN out
+#pragma unroll
+                for (int r = 0; r < kFewRows; r++) {
+                    const float w = __shfl_sync(0xffffffffu, p, key * C::kLanes + i * kFewRows + r);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) acc[r][e] = fmaf(w, f[e], acc[r][e]);
+                }
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        // ---- the group's parts become one
+#pragma unroll
+        for (int o = kFewRows; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+#pragma unroll
+        for (int r = 0; r < kFewRows; r++) {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+#pragma unroll
+                for (int o = C::kLanes; o < 32; o <<= 1) acc[r][e] += __shfl_xor_sync(0xffffffffu, acc[r][e], o);
+            if (key == 0)
+#pragma unroll
+                for (int e = 0; e < 8; e += 4)
+                    *reinterpret_cast<float4 *>(&sums[(warp % kGroupWarps * kFewRows + r) * D + dim + e]) = *reinterpret_cast<float4 *>(&acc[r][e]);
+        }
+        if (lane < kFewRows) ml[warp % kGroupWarps][lane] = make_float2(m, l);
+        bad = group_any(1 + group, 32 * kGroupWarps, bad);
+        const bool whole = it.count == it.units;
+        const size_t part = (size_t)(2 * (team + group) + (it.start > s.slot0)) * kFewRows;
+        for (int i = tid; i < a.group * D; i += 32 * kGroupWarps) {
+            const int r = i / D, d = i % D;
+            float most = -INFINITY, total = 0.0f, sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kGroupWarps; w++) most = fmaxf(most, ml[w][r].x);
+#pragma unroll
+            for (int w = 0; w < kGroupWarps; w++) {
+                const float2 x = ml[w][r];
+                const float f = x.x == -INFINITY ? x.y : ex2(x.x - most);  // its total is 0 (nothing seen) or NaN
+                total += f * x.y;
+                sum = fmaf(f, sums[(w * kFewRows + r) * D + d], sum);
+            }
+            sum *= kPScale, total *= kPScale;  // as the prefix's parts are
+            if (bad) sum = nan;
+            // all of it is for the join
+            const size_t at = (size_t)it.seq * a.q_heads + it.kv * a.group + r;
+            *((whole ? a.out + at * D : a.own_part_acc + (part + r) * D) + d) = sum;
+            if (d == 0) *(whole ? a.own_ml + at : a.own_part_ml + part + r) = make_float2(most, total);
+        }
+        group_sync(1 + group, 32 * kGroupWarps);
     }
-    __syncthreads();
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    attend_token<D, false>(a, smem, s);
 }
 
 // With a shared prefix: the first CTAs do the prefix on the tensor cores, the others the sequences without them. Each has a line
 // of its own, and they share the GPU by what the lines take.
-// Time of a slot of either line, relatively (64 users, 32/8 heads of 128, 4,112 shared, in us: 1 to 1 73, 3 to 2 59, 2 to 1 55,
-// 3 to 1 60; 16,384 shared: 82, 73, 72, 87).
-constexpr int kPrefixUnit = 2, kTokenUnit = 1;
+// Time of a slot of either line, relatively (64 users, 32/8 heads of 128, 4,112 shared, in us: 1 to 1 72, 3 to 2 60, 2 to 1 53,
+// 3 to 1 52; 16,384 shared: 83, 73, 71, 66).
+constexpr int kPrefixUnit = 3, kTokenUnit = 1;
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1) shared_token_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap k_map,
                                                                    const __grid_constant__ CUtensorMap v_map) {
     using C = Cfg<D, 128, false>;
-    static_assert(kThreads == 32 * kFewWarps && sizeof(FewNotes) <= kNotes && Few<D>::kSmem <= C::kSmem - kNotes, "one CTA for both");
+    static_assert(kThreads == 32 * kFewWarps && sizeof(GroupNotes) <= kNotes && Few<D>::kSmem <= C::kSmem - kNotes, "one CTA for both");
     extern __shared__ __align__(1024) unsigned char smem[];
-    FewNotes &s = *reinterpret_cast<FewNotes *>(smem + C::kSmem - kNotes);  // (both keep the plan in the same place)
-    if (threadIdx.x < 32) {
+    GroupNotes &notes = *reinterpret_cast<GroupNotes *>(smem + C::kSmem - kNotes);  // (the first plan is where the tiles' plan is, too)
+    const int warp = threadIdx.x >> 5, group = warp / kGroupWarps;
+    if (warp % kGroupWarps == 0) {  // a plan for each group, or for the CTA
         asm volatile("griddepcontrol.wait;" ::: "memory");
-        const int lane = threadIdx.x, cta = blockIdx.x, ctas = gridDim.x, per = a.c.kv_heads;
+        const int lane = threadIdx.x & 31, cta = blockIdx.x, ctas = gridDim.x, per = a.c.kv_heads;
         const int shared = asked_shared<true>(a), source = first_live(a, shared), common = common_of(a, shared, source);
         const int len = lane < a.seqs ? own_length<true>(a, lane, shared, common) : -1;
         const long long prefix = prefix_line<D>(a, common), own = sum_slots<D, true>(a, a.seqs, per, shared, common);
         const long long c1 = prefix * kPrefixUnit, c2 = own * kTokenUnit;
         const int split = prefix ? max(1, min(ctas - 1, (int)((ctas * c1 + (c1 + c2) / 2) / (c1 + c2)))) : 0;
-        const int prefix_g = (int)min((long long)split, prefix), own_g = (int)min((long long)(ctas - split), own);
+        const int prefix_g = (int)min((long long)split, prefix), own_g = (int)min((long long)(ctas - split) * kGroups, own);
         const bool first = cta < split;
-        const int team = first ? cta : cta - split, g = first ? prefix_g : own_g;
+        const int g = first ? prefix_g : own_g;
+        const int team = first ? cta : (cta - split) * kGroups + group;
         const long long w = first ? prefix : own;
         long long base = 0, u0 = 0, u1 = 0;
         int seq = first ? -1 : 0, length = common;
@@ -1457,22 +1609,23 @@ __global__ void __launch_bounds__(kThreads, 1) shared_token_kernel(const __grid_
             u1 = range_start(team + 1, w, g);
             if (!first) seq = find_slot<D, true>(a, per, u0, len, shared, common, base, length);
         }
-        if (lane == 0) {
+        if (lane == 0 && (!first || group == 0)) {
+            Plan &s = notes.plan[group];
             const int slots = first ? prefix_slots<D>(common) : max(1, slots_of<D, true>(a, length)), index = (int)quotient(u0 - base, slots);
             const int tiles = first ? a.all_tiles : 1;
             s.slot0 = u0, s.slot1 = u1, s.seq0 = seq, s.length0 = length;
             s.kv0 = index / tiles, s.tile0 = index % tiles;
             s.pos0 = (int)(u0 - base - (long long)index * slots);
-            s.common = common, s.source = first ? source : -1;
+            s.common = common, s.source = first ? source : split;
         }
-        if (cta == 0) tell_join<D>(a, shared, common, 0, own, prefix, own_g, prefix_g, split);
+        if (cta == 0 && warp == 0) tell_join<D>(a, shared, common, 0, own, prefix, own_g, prefix_g);
     }
     __syncthreads();
-    if (s.seq0 < 0) {
+    if (notes.plan[0].seq0 < 0) {
         attend_tiles<D, 128, false, true, true>(a, k_map, v_map);
     } else {
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-        attend_token<D, true>(a, smem, s);
+        attend_tokens<D>(a, smem, notes, ((int)blockIdx.x - notes.plan[0].source) * kGroups);
     }
 }
 
@@ -1578,7 +1731,7 @@ __global__ void __launch_bounds__(256) join_shared_kernel(const __grid_constant_
     const int h = id % a.q_heads, row = id / a.q_heads, seq = row / a.tokens, kv = h / a.group, r = (row - seq * a.tokens) * a.group + h % a.group;
     const long long w = a.starts[a.seqs], all_w = a.starts[a.seqs + 1], first = a.starts[seq];
     const int *said = a.lengths + a.seqs;
-    const int own = a.lengths[seq], common = said[0], g = said[1], all_g = said[2], first_cta = said[3], units = units_of(a, own);
+    const int own = a.lengths[seq], common = said[0], g = said[1], all_g = said[2], units = units_of(a, own);
     float *out = a.out + (size_t)id * D;
     if (*(volatile int *)a.err || own < 0) {
         for (int i = WARPS == 1 ? lane : threadIdx.x; i < D; i += 32 * WARPS) out[i] = __int_as_float(0x7fc00000);
@@ -1601,8 +1754,9 @@ __global__ void __launch_bounds__(256) join_shared_kernel(const __grid_constant_
             return;
         }
         const int q = prefix ? p : p - before;
-        const size_t at = (size_t)(2 * ((prefix ? p0 : first_cta + c0) + q) + (q == 0 && (prefix ? all_late : late))) * a.part_rows + (prefix ? all_r : r) % a.tile_rows;
-        acc = a.part_acc + at * D, ml = a.part_ml + at;
+        const size_t at = (size_t)(2 * ((prefix ? p0 : c0) + q) + (q == 0 && (prefix ? all_late : late))) * (prefix ? a.part_rows : a.own_part_rows) +
+                          (prefix ? all_r : r) % a.tile_rows;
+        acc = (prefix ? a.part_acc : a.own_part_acc) + at * D, ml = (prefix ? a.part_ml : a.own_part_ml) + at;
     };
     float m = -INFINITY, l = 0.0f, acc[V];
 #pragma unroll
@@ -1774,6 +1928,9 @@ int attend_args(AttendArgs &a, float *out, const float *q, const qg_kv_cache *ca
     a.all_tiles = 0;
     a.prefix_acc = nullptr;
     a.prefix_ml = a.own_ml = nullptr;
+    a.own_part_acc = nullptr;
+    a.own_part_ml = nullptr;
+    a.own_part_rows = 0;
     a.starts = nullptr;
     a.lengths = nullptr;
     a.err = static_cast<int *>(workspace);
@@ -1799,6 +1956,7 @@ bool bad_sizes(int seqs, int tokens, int q_heads, int kv_heads, int head_dim) {
     return seqs < 1 || seqs > kMaxSeqs || tokens < 1 || tokens > kMaxNodes || kv_heads < 1 || kv_heads > 1024 || q_heads < kv_heads ||
            q_heads > 1024 || q_heads % kv_heads || (head_dim != 64 && head_dim != 128 && head_dim != 256);
 }
+constexpr size_t kFewParts = (size_t)2 * kGroups * kMaxCtas * kFewRows;  // rows of the parts of sequences' own lines
 constexpr long long kMaxShared = 1 << 24;  // rows and heads of a batch with a shared prefix
 
 }  // namespace
@@ -1838,7 +1996,7 @@ extern "C" int qg_shared_attention_workspace_bytes(int seqs, int tokens, int q_h
     const int rows = part_rows(seqs * tokens, q_heads / kv_heads);
     const size_t heads = ((size_t)seqs * tokens * q_heads + 1) & ~(size_t)1;
     *bytes = 256 + ml_bytes(rows) + (size_t)2 * kMaxCtas * rows * head_dim * sizeof(float) + heads * (2 * sizeof(float2) + head_dim * sizeof(float)) +
-             (kMaxSeqs + 2) * sizeof(long long) + (kMaxSeqs + 4) * sizeof(int);
+             (kMaxSeqs + 2) * sizeof(long long) + (kMaxSeqs + 4) * sizeof(int) + kFewParts * (sizeof(float2) + head_dim * sizeof(float));
     return cudaSuccess;
 }
 
@@ -1870,11 +2028,20 @@ extern "C" int qg_shared_attention(float *out, const float *q, const qg_kv_cache
     a.lengths = reinterpret_cast<int *>(a.starts + kMaxSeqs + 2);
     CUtensorMap k_map, v_map;
     if (int rc = maps(a, pair, k_map, v_map)) return rc;
+    a.own_part_acc = a.part_acc;
+    a.own_part_ml = a.part_ml;
+    a.own_part_rows = a.part_rows;
     // One token, at most four heads to a key head of up to 128 values: as without a prefix, the sequences' own keys need no
     // tensor cores.
-    if (tokens == 1 && a.group <= kFewRows && d == 64)
+    const bool few = tokens == 1 && a.group <= kFewRows && d <= 128;
+    if (few) {
+        a.own_part_ml = reinterpret_cast<float2 *>(a.lengths + kMaxSeqs + 4);
+        a.own_part_acc = reinterpret_cast<float *>(a.own_part_ml + kFewParts);
+        a.own_part_rows = kFewRows;
+    }
+    if (few && d == 64)
         return launch<64, true>(a, shared_token_kernel<64>, 1, kThreads, Cfg<64, 128, false>::kSmem, a, k_map, v_map);
-    if (tokens == 1 && a.group <= kFewRows && d == 128)
+    if (few)
         return launch<128, true>(a, shared_token_kernel<128>, 1, kThreads, Cfg<128, 128, false>::kSmem, a, k_map, v_map);
     if (d == 64) return launch_tiles<64, 128, false, true>(a, k_map, v_map);
     if (d == 128) return launch_tiles<128, 128, false, true>(a, k_map, v_map);
