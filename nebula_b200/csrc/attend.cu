@@ -28,6 +28,14 @@
 // One token whose query heads share a key head by four at most has a kernel
 // without tensor cores (token_attention_kernel): its arithmetic hides behind
 // HBM, and nothing is handed from one role to another.
+//
+// Sequences that begin alike (qg_shared_attention): the prefix is one more
+// sequence at the head of the line, whose rows are those of all sequences, and
+// the join adds its parts to each sequence's own. A key of the prefix is read
+// once for 128 or 256 rows, so the tensor cores bound it: with both planes of
+// Q and P 4 rows heads keys values FLOP count twice (48 x 5 rows, 32,768 shared,
+// heads of 256: 243 us at the rate of one library product, 334 measured, 382
+// in a loop under the power cap).
 #include <cuda.h>
 #include <cstring>
 #include "cache.cuh"
@@ -1718,7 +1726,8 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Atten
 
 // With a shared prefix every row has parts: the prefix's, then its sequence's own. What a CTA did as a whole is in the rows of
 // prefix_acc or out. WARPS warps to a (row, head): eight where there are so few rows that each may have many parts, otherwise one,
-// so that all rows are under way at once (48 x 5 rows of 24 heads of 256: 85 us with eight, @ with one).
+// so that all rows are under way at once (the whole call, in us, with eight and with one: 8 x 17 rows of 24 heads, 8,192 shared
+// 88 and 70; two single tokens of 24 heads, 30,016 shared 39 and 69; eight of 32 heads, 8,192 shared 39 and 47).
 template <int D, int WARPS>
 __global__ void __launch_bounds__(256) join_shared_kernel(const __grid_constant__ AttendArgs a) {
     constexpr int V = D / 32, kFly = 4;  // parts that are asked for before the first is used

@@ -5,7 +5,8 @@
 // sequences need (or give back) in its own shared memory, then takes its share of the entries to write. What the call
 // changes and all CTAs read (pages held, the stack's height) is written after a barrier of the cluster. Bound by latency:
 // launch, one trip for the lengths, one for the stack or the table, the barrier. Where there are many slots to write a second
-// kernel does it on the whole GPU, from the page tables that the first one has left.
+// kernel does it on the whole GPU, from the page tables that the first one has left (700 sequences of up to 512 new positions:
+// releasing and reserving 17 us with one kernel each, 12 with the third). Four sequences of 17: 7 us for both calls.
 #include "cache.cuh"
 
 using namespace nb;
@@ -231,8 +232,8 @@ int pages_args(const qg_page_pool *p, int *out, const int *lengths, int seqs, Pa
     return 0;
 }
 
-// `entries`: what there may be to write. A cluster's barrier and its CTAs' launch cost more than one CTA's writes up to some
-// thousands of them.
+// `entries`: what there may be to write. A cluster's barrier and its CTAs' launch cost as much as one CTA's writes of some
+// thousands of them (both calls, one CTA and eight: 64 sequences of 17 slots 10.2 and 11.3 us, 300 of 17 12.9 and 8.6).
 int launch(void (*kernel)(PagesArgs), const PagesArgs &a, long long entries) {
     const int ranks = entries > kOneCta ? kPagesCluster : 1;
     cudaLaunchConfig_t cfg = {};

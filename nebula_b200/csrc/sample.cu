@@ -14,6 +14,11 @@
 // Weights are evaluated in 64 bits and summed as whole numbers: borders are compared exactly, and neither the cluster's
 // size nor the order of atomics has a say. With weights in 32 bits a running sum is off by some 1e-8, and a tail of 100,000
 // tokens of 1e-6 each is off by a token once in a hundred draws.
+//
+// What bounds it: one row is a chain of barriers of its cluster (some 0.7 us each with what they wait for) and passes over
+// 8 to 32 logits a thread; of many rows, some 30 are on the GPU at a time, as many as its shared memory holds, so their chains
+// and the 64-bit weights (15 instructions, 7.5 clocks a warp and SM) are the time, not HBM. 256 rows of 131,072 (20.5 us of
+// HBM): temperature 0 62 us, top-k 40 100, no truncation 120, a nucleus of 0.9 260; one row 7.5, 10.5, 9 and 19.
 #include "cache.cuh"
 
 using namespace nb;
