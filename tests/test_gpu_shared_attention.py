@@ -348,3 +348,19 @@ def test_attention_spread_of_magnitudes(L):  # noqa: F811
         # these far maxima all the weight lies on one key, or on 256 keys whose scores differ by their small values alone
         assert np.abs(got - ref).max() <= 0.1 * np.abs(ref).max()
         assert_parity(got[1], ref[1])
+
+
+@pytest.mark.parametrize("hq,hkv,d,tokens", [(8, 2, 64, 1), (32, 8, 128, 1), (8, 2, 128, 5), (8, 2, 256, 3), (24, 2, 256, 17)])
+def test_attention_rows_are_nan_while_the_error_word_is_set(L, hq, hkv, d, tokens):  # noqa: F811
+    """A wait that ran out leaves its mark in the workspace: every row is NaN until the workspace is cleared."""
+    rng = np.random.default_rng(d)
+    cache = SharedCache(L, rng, 256, [40, 7], tokens, hkv, d, 32)
+    q = rng.normal(size=(2, tokens, hq, d)).astype(np.float32)
+    ws = L.shared_attention_workspace(2, tokens, hq, hkv, d)
+    ref = expected(cache, q, None, 0.1)
+    mark = np.array([4], np.int32)
+    L.call("write", ws.p, mark.ctypes.data, 4)
+    for _ in range(2):
+        assert np.isnan(attend_shared(L, cache, q, None, 0.1, ws=ws)).all()
+    L.call("zero", ws.p, ws.nbytes)
+    assert_parity(attend_shared(L, cache, q, None, 0.1, ws=ws), ref)
