@@ -54,10 +54,10 @@ struct Shared {
     Whole ends[kMaxRanks];             // key of the largest logit; inverted, the lowest of the threads' largest, or its index
     int last[2];
     Whole total[2][kMaxRanks];         // by the parity of the exchange: a CTA may be one ahead
-    unsigned hist[2][3][kBins];        // by the parity of the pass: counts, or sums as 15 + 15 + 14 bits
+    unsigned hist[2][2][kBins];        // by the parity of the pass: counts, or the low and high words of sums
     Whole list[kList];                 // key and inverted index: the larger is the better
     int listed;
-    unsigned fine[3][kFine];           // sums in the same parts
+    unsigned fine[2][kFine];           // words of sums
     Whole coarse[kFine / 32];
     // a CTA's own
     Whole warp_sum[kWarps], entry_weight[kFew];
@@ -306,23 +306,25 @@ __device__ __forceinline__ Bin reach_bin(Shared &s, Whole mine, Whole target) {
     __syncthreads();
     return {(int)s.found, s.kept_sum};
 }
-// A histogram counts, or adds up weights in three parts: each part's sum over a CTA's logits fits 32 bits.
-using Hist = unsigned[3][kBins];
+// Adds to a sum of two words. Shared memory has no addition of 64 bits of its own (one that tries again and again takes 61
+// clocks a warp over 64 bins, two words 5.6, three parts that need no carry 7.5).
+__device__ __forceinline__ void add_words(unsigned &low, unsigned &high, Whole w) {
+    const unsigned before = atomicAdd(&low, (unsigned)w);
+    atomicAdd(&high, (unsigned)(w >> 32) + (before + (unsigned)w < before));
+}
+__device__ __forceinline__ Whole words(unsigned low, unsigned high) { return (Whole)high << 32 | low; }
+// A histogram counts, or adds up weights.
+using Hist = unsigned[2][kBins];
 template <bool SUM>
 __device__ __forceinline__ void add_to(Hist &hist, int bin, Whole w) {
-    if (SUM) {
-        atomicAdd(&hist[0][bin], (unsigned)w & 0x7fffu);
-        atomicAdd(&hist[1][bin], (unsigned)(w >> 15) & 0x7fffu);
-        atomicAdd(&hist[2][bin], (unsigned)(w >> 30));
-    } else {
-        atomicAdd(&hist[0][bin], 1u);
-    }
+    if (SUM) add_words(hist[0][bin], hist[1][bin], w);
+    else atomicAdd(&hist[0][bin], 1u);
 }
 // One histogram of all CTAs' added up: bin tid's, for tid < kBins. Four threads to a bin read, a quarter of the CTAs' each.
 template <bool SUM>
 __device__ __forceinline__ Whole all_bins(Shared &s, const Row &r, const Hist &hist) {
     const int bin = threadIdx.x % kBins, group = threadIdx.x / kBins;
-    constexpr int N = SUM ? 3 : 1;
+    constexpr int N = SUM ? 2 : 1;
     Whole sum = 0;
 #pragma unroll 1
     for (uint32_t q0 = group; q0 < r.ranks; q0 += 8) {
@@ -332,7 +334,7 @@ __device__ __forceinline__ Whole all_bins(Shared &s, const Row &r, const Hist &h
 #pragma unroll
             for (int e = 0; e < N; e++) part[i][e] = q0 + 4 * i < r.ranks ? peer_load(at_rank(&hist[e][bin], q0 + 4 * i)) : 0;
         sum += (Whole)part[0][0] + part[1][0];
-        if constexpr (SUM) sum += (((Whole)part[0][1] + part[1][1]) << 15) + (((Whole)part[0][2] + part[1][2]) << 30);
+        if constexpr (SUM) sum += (Whole)(part[0][1] + part[1][1]) << 32;
     }
     s.bins[group][bin] = sum;
     __syncthreads();
@@ -435,9 +437,8 @@ __device__ Whole nth_entry(Shared &s, const Row &r, int n, Range in, Whole targe
         if (tid == 0) s.few = 0;
         Whole sum = 0;
         if (tid < kBins) {
-            sum = hist[0][tid] + ((Whole)hist[1][tid] << 15) + ((Whole)hist[2][tid] << 30);  // (counts: the other parts are zero)
-#pragma unroll
-            for (int e = 0; e < 3; e++) hist[e][tid] = 0;
+            sum = words(hist[0][tid], hist[1][tid]);  // (counts: the high words are zero)
+            hist[0][tid] = hist[1][tid] = 0;
         }
         const Bin b = reach_bin(s, sum, target);
         const int shift = in.shift();
@@ -492,7 +493,7 @@ __device__ void narrow(Shared &s, Row &r, Whole target, Range in, bool linear, i
         cluster_sync();
         const Whole mine = all_bins<SUM>(s, r, hist);
         // the other histogram, and the list, were read before this pass's barrier
-        for (int i = tid; i < 3 * kBins; i += kThreads) other[0][i] = 0;
+        for (int i = tid; i < 2 * kBins; i += kThreads) other[0][i] = 0;
         if (tid == 0) s.listed = 0;
         pass++;
         const Bin b = reach_bin(s, mine, target);
@@ -536,7 +537,7 @@ __device__ __forceinline__ float octaves_of(float p, int vocab) { return log2f((
 __device__ void nucleus(Shared &s, Row &r, float p, float end, int &pass, int &turn) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     Range in = {key_of(end), key_of(r.most), r.most, fminf(kFine / (r.most - end), 1e30f), kFine - 1, -1};
-    for (int i = tid; i < 3 * kFine; i += kThreads) s.fine[0][i] = 0;
+    for (int i = tid; i < 2 * kFine; i += kThreads) s.fine[0][i] = 0;
     __syncthreads();
     Whole sum = 0;
     r.each_weight(-INFINITY, [&](const float (&x)[4], int, const Whole (&w)[4]) {
@@ -545,16 +546,14 @@ __device__ void nucleus(Shared &s, Row &r, float p, float end, int &pass, int &t
         for (int e = 0; e < 4; e++)
             if (x[e] >= end) {
                 const int bin = in.bin_of(x[e]);
-                atomicAdd(&s.fine[0][bin], (unsigned)w[e] & 0x7fffu);
-                atomicAdd(&s.fine[1][bin], (unsigned)(w[e] >> 15) & 0x7fffu);
-                atomicAdd(&s.fine[2][bin], (unsigned)(w[e] >> 30));
+                add_words(s.fine[0][bin], s.fine[1][bin], w[e]);
             }
     });
     __syncthreads();
 #pragma unroll
     for (int g = warp; g < kFine / 32; g += kWarps) {
         const int bin = 32 * g + lane;
-        const Whole of_group = warp_sum(s.fine[0][bin] + ((Whole)s.fine[1][bin] << 15) + ((Whole)s.fine[2][bin] << 30));
+        const Whole of_group = warp_sum(words(s.fine[0][bin], s.fine[1][bin]));
         if (lane == 0) s.coarse[g] = of_group;
     }
     share_sums(s, r, sum, turn);
@@ -580,11 +579,9 @@ __device__ void nucleus(Shared &s, Row &r, float p, float end, int &pass, int &t
     s.read[0][warp][lane] = warp < r.ranks ? peer_load64(at_rank(&s.coarse[lane], warp)) : 0;
     const int group = find(s.read[0], target);
     if (group < 0) return;  // all of them
-    unsigned part[3] = {0, 0, 0};
-    if (warp < r.ranks)
-#pragma unroll
-        for (int e = 0; e < 3; e++) part[e] = peer_load(at_rank(&s.fine[e][32 * group + lane], warp));
-    s.read[1][warp][lane] = part[0] + ((Whole)part[1] << 15) + ((Whole)part[2] << 30);
+    unsigned low = 0, high = 0;
+    if (warp < r.ranks) low = peer_load(at_rank(&s.fine[0][32 * group + lane], warp)), high = peer_load(at_rank(&s.fine[1][32 * group + lane], warp));
+    s.read[1][warp][lane] = words(low, high);
     in.take_bin(32 * group + find(s.read[1], target));
     const int n = gather(s, r, in);
     if (n > kList) {
@@ -667,7 +664,7 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
     if (lane == 0) s.warp_most[warp] = top, s.warp_least[warp] = low;
     // (what this CTA's memory held of the row before is read by others until they are here)
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-    for (int i = tid; i < 2 * 3 * kBins; i += kThreads) s.hist[0][0][i] = 0;
+    for (int i = tid; i < 2 * 2 * kBins; i += kThreads) s.hist[0][0][i] = 0;
     if (tid == 0) s.listed = 0;
     __syncthreads();
     top = __reduce_max_sync(0xffffffffu, lane < kWarps ? s.warp_most[lane] : 0);
