@@ -30,6 +30,7 @@ constexpr int kBins = 128;
 constexpr int kFine = 1024;                       // bins of the nucleus, in groups of 32
 constexpr int kFew = 256;                         // logits of top-k that are ordered one by one
 constexpr int kFewer = 64;                        // the same where one of a list is looked for
+constexpr int kSparse = 16;                       // of a lane's 32 logits: with more than these in a lane, all of the warp's are weighed
 constexpr int kList = 1024;                       // logits that every CTA has a list of
 constexpr int kStep = kThreads * 4;               // a CTA's part of a row is a multiple of this: a thread has whole units of four
 constexpr int kMaxUnits = 22;                     // of a thread: 188 KB a CTA
@@ -57,14 +58,17 @@ struct Shared {
     unsigned hist[2][2][kBins];        // by the parity of the pass: counts, or the low and high words of sums
     Whole list[kList];                 // key and inverted index: the larger is the better
     int listed;
-    unsigned fine[2][kFine];           // words of sums
     Whole coarse[kFine / 32];
-    // a CTA's own
-    Whole warp_sum[kWarps], entry_weight[kFew];
     union {
-        Whole entry[kList];
-        Whole bins[4][kBins], read[2][kMaxRanks][32];  // until a list is read
+        unsigned fine[2][kFine];       // words of sums
+        Whole entry[kList];            // from here on a CTA's own: these once all have read the bins, with a barrier between
+        Whole bins[4][kBins];
     };
+    union {
+        Whole entry_weight[kFew];
+        Whole read[kMaxRanks][32];     // until entries are ordered
+    };
+    Whole warp_sum[kWarps];
     Whole found, kept_sum;
     int few;
     unsigned warp_most[kWarps], warp_least[kWarps];
@@ -144,6 +148,8 @@ struct Row {
     double top, c;       // log2(e) / T
     unsigned key;        // kept: logits above the key, and those at it up to index `last`
     int last;
+    bool known;          // whether all threads' shares add up to the weights that this CTA keeps
+    Whole share;
 
     // f(x, index) for every logit of the thread.
     template <typename F>
@@ -161,37 +167,50 @@ struct Row {
     // temperature 1, 34 us in all against 53.)
     template <typename F>
     __device__ __forceinline__ void some(float low, float high, F f) const {
-        for (int j0 = 0; j0 < units; j0 += 8) {
-            unsigned found = 0;
+        for (int j0 = 0; j0 < units; j0 += 8) two_by_two(between(j0, low, high), j0, f);
+    }
+    // Which of the 32 logits from unit j0 on lie between low and high. With low alone: up to the largest.
+    __device__ __forceinline__ unsigned between(int j0, float low, float high) const {
+        return which(j0, [=](float x) { return x >= low && x <= high; });
+    }
+    __device__ __forceinline__ unsigned from(int j0, float low) const {
+        return which(j0, [=](float x) { return x >= low; });
+    }
+    template <typename P>
+    __device__ __forceinline__ unsigned which(int j0, P is) const {
+        unsigned found = 0;
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (j0 + j < units) {
-                    const float4 x = mine[j0 + j];
-                    if (x.x >= low && x.x <= high) found |= 1u << (4 * j);
-                    if (x.y >= low && x.y <= high) found |= 2u << (4 * j);
-                    if (x.z >= low && x.z <= high) found |= 4u << (4 * j);
-                    if (x.w >= low && x.w <= high) found |= 8u << (4 * j);
-                }
-            while (found) {
-                float x[2];
-                int at[2];
-                const int a = __ffs(found) - 1;
-                found &= found - 1;
-                const int b = found ? __ffs(found) - 1 : a;
-                const float *from = reinterpret_cast<const float *>(mine + j0);
-                x[0] = from[a], x[1] = found ? from[b] : -INFINITY;
-                found &= found - 1;
-                at[0] = index + 4 * j0 + a, at[1] = index + 4 * j0 + b;
-                f(x, at);
+        for (int j = 0; j < 8; j++)
+            if (j0 + j < units) {
+                const float4 x = mine[j0 + j];
+                found |= (is(x.x) ? 1u << (4 * j) : 0) | (is(x.y) ? 2u << (4 * j) : 0) | (is(x.z) ? 4u << (4 * j) : 0) | (is(x.w) ? 8u << (4 * j) : 0);
             }
+        return found;
+    }
+    template <typename F>
+    __device__ __forceinline__ void two_by_two(unsigned found, int j0, F f) const {
+        while (found) {
+            float x[2];
+            int at[2];
+            const int a = __ffs(found) - 1;
+            found &= found - 1;
+            const int b = found ? __ffs(found) - 1 : a;
+            const float *from = reinterpret_cast<const float *>(mine + j0);
+            x[0] = from[a], x[1] = found ? from[b] : -INFINITY;
+            found &= found - 1;
+            at[0] = index + 4 * j0 + a, at[1] = index + 4 * j0 + b;
+            f(x, at);
         }
     }
     // f(x, index, weight) for four neighbouring logits at a time, where some of the warp's are at or above low (and weigh something).
     template <typename F>
     __device__ __forceinline__ void each_weight(float low, F f) const {
-        low = fmaxf(low, zero);
+        weights_of(0, units, fmaxf(low, zero), f);
+    }
+    template <typename F>
+    __device__ __forceinline__ void weights_of(int j0, int j1, float low, F f) const {
 #pragma unroll 2
-        for (int j = 0; j < units; j++) {
+        for (int j = j0; j < j1; j++) {
             const float4 x = mine[j];
             if (!__any_sync(0xffffffffu, fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)) >= low)) continue;
             const float y[4] = {x.x, x.y, x.z, x.w};
@@ -202,12 +221,23 @@ struct Row {
     // The thread's sum of the weights that are kept.
     __device__ __forceinline__ Whole kept_sum() const {
         Whole sum = 0;
-        const float low = floor();
-        each_weight(low, [&](const float (&x)[4], int at, const Whole (&w)[4]) {
+        const float low = floor(), weighs = fmaxf(low, zero);
+        for (int j0 = 0; j0 < units; j0 += 8) {
+            const unsigned found = key == kNone ? ~0u : from(j0, weighs);
+            if (__reduce_max_sync(0xffffffffu, __popc(found)) <= kSparse)
+                two_by_two(found, j0, [&](const float (&x)[2], const int (&at)[2]) {
+                    const Whole w[2] = {weigh(x[0]), weigh(x[1])};
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (x[e] > low || (x[e] == low && at + e <= last)) sum += w[e];
-        });
+                    for (int e = 0; e < 2; e++)
+                        if (kept_of_floor(x[e], at[e])) sum += w[e];
+                });
+            else
+                weights_of(j0, min(units, j0 + 8), weighs, [&](const float (&x)[4], int at, const Whole (&w)[4]) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (kept_of_floor(x[e], at + e)) sum += w[e];
+                });
+        }
         return sum;
     }
     // Of logits from floor() up, and -infinity: those that are kept.
@@ -475,6 +505,18 @@ __device__ Whole nth_entry(Shared &s, const Row &r, int n, Range in, Whole targe
     return s.found;
 }
 
+// The kept set ends at a listed entry. SUM: the threads' shares of what this CTA has in better bins are summed up; its own
+// list is the rest.
+template <bool SUM>
+__device__ __forceinline__ void keep_to(const Shared &s, Row &r, Whole worst) {
+    r.key = (unsigned)(worst >> 32), r.last = (int)~(unsigned)worst;
+    if constexpr (SUM) {
+        for (int i = threadIdx.x; i < s.listed; i += kThreads)
+            if (s.list[i] >= worst) r.share += r.weigh(of_key((unsigned)(s.list[i] >> 32)));
+        r.known = true;
+    }
+}
+
 // Narrows the kept set to its largest logits: of those in a range, `target` (SUM: as many as it takes until their weights reach
 // it). linear: the first bins are distances.
 template <bool SUM>
@@ -499,12 +541,12 @@ __device__ void narrow(Shared &s, Row &r, Whole target, Range in, bool linear, i
         const Bin b = reach_bin(s, mine, target);
         if (b.bin < 0) return;  // all of them
         target -= b.before;
+        if (SUM && tid < b.bin) r.share += words(hist[0][tid], hist[1][tid]);
         if (linear) in.take_bin(b.bin);
         else in.take_keys(b.bin, shift);
         const int n = gather(s, r, in);
         if (n <= kList) {
-            const Whole worst = nth_entry<SUM>(s, r, n, in, target, other);
-            r.key = (unsigned)(worst >> 32), r.last = (int)~(unsigned)worst;
+            keep_to<SUM>(s, r, nth_entry<SUM>(s, r, n, in, target, other));
             return;
         }
     }
@@ -562,13 +604,14 @@ __device__ void nucleus(Shared &s, Row &r, float p, float end, int &pass, int &t
     turn++;
     Whole target = share_of(p, all);
     // the group, then the bin in it; a warp reads one CTA's, and every warp looks for it
-    auto find = [&](Whole (&from)[kMaxRanks][32], Whole &target) {
+    auto find = [&](Whole &target) {
         __syncthreads();
         Whole mine = 0;
 #pragma unroll 1
         for (uint32_t q0 = 0; q0 < r.ranks; q0 += 8)  // (zeros where there is no CTA)
 #pragma unroll
-            for (int q = 0; q < 8; q++) mine += from[q0 + q][lane];
+            for (int q = 0; q < 8; q++) mine += s.read[q0 + q][lane];
+        __syncthreads();
         const Whole upto = warp_scan(mine);
         const unsigned past = __ballot_sync(0xffffffffu, upto >= target);
         if (!past) return -1;
@@ -576,20 +619,21 @@ __device__ void nucleus(Shared &s, Row &r, float p, float end, int &pass, int &t
         target -= __shfl_sync(0xffffffffu, upto - mine, l);
         return l;
     };
-    s.read[0][warp][lane] = warp < r.ranks ? peer_load64(at_rank(&s.coarse[lane], warp)) : 0;
-    const int group = find(s.read[0], target);
+    s.read[warp][lane] = warp < r.ranks ? peer_load64(at_rank(&s.coarse[lane], warp)) : 0;
+    const int group = find(target);
     if (group < 0) return;  // all of them
     unsigned low = 0, high = 0;
     if (warp < r.ranks) low = peer_load(at_rank(&s.fine[0][32 * group + lane], warp)), high = peer_load(at_rank(&s.fine[1][32 * group + lane], warp));
-    s.read[1][warp][lane] = words(low, high);
-    in.take_bin(32 * group + find(s.read[1], target));
+    s.read[warp][lane] = words(low, high);
+    const int bin = 32 * group + find(target);
+    for (int i = tid; i < bin; i += kThreads) r.share += words(s.fine[0][i], s.fine[1][i]);
+    in.take_bin(bin);
     const int n = gather(s, r, in);
     if (n > kList) {
         narrow<true>(s, r, target, in, false, pass, turn);
         return;
     }
-    const Whole worst = nth_entry<true>(s, r, n, in, target, s.hist[pass & 1]);
-    r.key = (unsigned)(worst >> 32), r.last = (int)~(unsigned)worst;
+    keep_to<true>(s, r, nth_entry<true>(s, r, n, in, target, s.hist[pass & 1]));
 }
 
 // Bins a quarter wide around the logits that models give, and the lowest logit of one. They serve to leave out most logits
@@ -702,6 +746,7 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
     r.top = most;
     r.c = 1.4426950408889634 / (t > 0.0f ? (double)t : 1.0);
     r.zero = fmaxf((float)(r.top - 46.0 / r.c), kLowest);
+    r.share = 0, r.known = false;
     r.key = kNone, r.last = -0x7fffffff;  // (what lies outside the row has indices from -3 on)
     const unsigned min_key = [&]() -> unsigned {  // of the lowest logit that min_p leaves
         if (!(least > 0.0f)) return 0;
@@ -773,7 +818,7 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
                              true, pass, turn);
             }
         }
-        if (!done && min_key > r.key) r.key = min_key, r.last = 0x7fffffff;
+        if (!done && min_key > r.key) r.key = min_key, r.last = 0x7fffffff, r.known = false;
     }
 
     // ---- the token, or the logits
@@ -783,13 +828,19 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
             return;
         }
         auto mine = [&](float x, int index) { return r.keeps(x, index) ? r.weigh(x) : 0; };
-        const Whole sum = r.kept_sum();
-        Whole all;
+        Whole sum = r.known ? r.share : r.kept_sum(), all;
         share_sums(s, r, sum, turn);
         const Whole before = sums_before(s, r, turn, all);
         // the first running sum above u * all is the first that reaches the whole number after it
         const float v = fminf(fmaxf(u, 0.0f), 0.99999994f);
         const Whole aim = __umul64hi(__double2ull_rz((double)v * 18446744073709551616.0), all) + 1;
+        if (r.known) {  // by index, in the one CTA that has the token
+            if (before >= aim || before + s.total[turn & 1][r.rank] < aim) return;
+            sum = r.kept_sum();
+            const Whole of_warp = warp_sum(sum);
+            if (lane == 0) s.warp_sum[warp] = of_warp;
+            __syncthreads();
+        }
         const int index = reach(s, r, sum, before, aim, mine);
         if (index >= 0 && lane == 0) a.token[row] = index;
         return;
