@@ -379,8 +379,9 @@ struct Range {
     __device__ __forceinline__ bool has(float x) const { return bin < 0 || bin_of(x) == bin; }  // of those between low and high
     // Only what is in distance bin b. The keys' limits are wider than the bin by more than bin_of rounds.
     __device__ __forceinline__ void take_bin(int b) {
-        if (b < last_bin) low = max(low, key_of(__double2float_rd((double)most - (b + 1) * 1.000001 / (double)scale)));
-        if (b) high = min(high, key_of(__double2float_ru((double)most - b * 0.999999 / (double)scale)));
+        const double width = 1.0f / scale;
+        if (b < last_bin) low = max(low, key_of(__double2float_rd((double)most - (b + 1) * 1.000001 * width)));
+        if (b) high = min(high, key_of(__double2float_ru((double)most - b * 0.999999 * width)));
         bin = b;
     }
     // Only key bin b of those that are 2^shift keys wide, from high on downwards.
