@@ -37,6 +37,7 @@ constexpr int kMaxUnits = 22;                     // of a thread: 188 KB a CTA
 constexpr int kMaxRanks = 16;                     // CTAs of a cluster
 constexpr int kMaxVocab = 8 * kMaxUnits * kStep;
 constexpr int kRowsAtOnce = 1 << 20;
+static_assert(32 * kMaxUnits * kMaxUnits < 65536, "a unit's owner by multiplication");
 static_assert(kMaxVocab <= 1 << 19, "sums of weights, 2^44 at most, fit 63 bits");
 static_assert(kMaxRanks == kWarps && kMaxRanks % 4 == 0 && 2 * kFew <= kThreads && 4 * kBins == kThreads, "two threads to a logit that is ordered, four to a bin");
 
@@ -46,6 +47,8 @@ struct SampleArgs {
     float *out;
     int *token;
     int per, rows, vocab, units;
+    unsigned inverse;  // of units, in 65536ths and rounded up: right for all of a warp's 32 * units, since 32 * 22 * 22 < 65536
+    __device__ __forceinline__ int owner_of(int unit) const { return (int)(unit * inverse >> 16); }
 };
 
 using Whole = unsigned long long;
@@ -265,7 +268,8 @@ struct Row {
         p = fma(p, f, 6.931471805599462e-01);
         p = fma(p, f, 1.0000000000000135);
         const double v = __hiloint2double(__double2hiint(p) + (__double2loint(n) << 20), __double2loint(p)) + kUnit;
-        return x >= zero ? (Whole)__double_as_longlong(v) & 0xfffffffffffffull : 0;
+        const Whole w = (Whole)__double_as_longlong(v) & 0xfffffffffffffull;
+        return x >= zero ? w : 0;
     }
 };
 
@@ -688,7 +692,7 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
 #pragma unroll
             for (int j = 0; j < 8; j++)
                 if (j0 + j < a.units) {
-                    const int at = (j0 + j) * 32 + lane, owner = at / a.units;
+                    const int at = (j0 + j) * 32 + lane, owner = a.owner_of(at);
                     x[j].x += 0.0f, x[j].y += 0.0f, x[j].z += 0.0f, x[j].w += 0.0f;  // -0 is 0: equals go by their index
                     to[owner * stride + (at - owner * a.units)] = x[j];
                     most = max_nan(max_nan(max_nan(most, x[j].x), max_nan(x[j].y, x[j].z)), x[j].w);
@@ -851,7 +855,7 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
     const bool whole = !((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(x0)) & 15);
     const float4 *const from = part + warp * 32 * stride;
     for (int j = 0; j < a.units; j++) {
-        const int at = j * 32 + lane, owner = at / a.units, i = start + (warp * 32 * a.units + at) * 4;
+        const int at = j * 32 + lane, owner = a.owner_of(at), i = start + (warp * 32 * a.units + at) * 4;
         float4 x = from[owner * stride + (at - owner * a.units)];
         x.x = !refused && r.keeps(x.x, i) ? x.x : other;
         x.y = !refused && r.keeps(x.y, i + 1) ? x.y : other;
@@ -907,6 +911,7 @@ int launch(SampleArgs &a, int rows) {
     const int smem = kThreads * (a.units | 1) * 16 + (int)sizeof(Shared);
     if (int rc = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return rc;
     if (int rc = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) return rc;
+    a.inverse = 65535 / a.units + 1;
     a.rows = rows;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(kThreads);
