@@ -705,6 +705,8 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
             asm volatile("prefetch.global.L2 [%0];" ::"l"(x1 + i));
     }
     const float threads_most = most;
+    const double octaves_per_logit = 1.4426950408889634 / (t > 0.0f ? (double)t : 1.0), logits_per_octave = 0.6931471805599453 * (t > 0.0f ? (double)t : 1.0);
+    const double min_below = least > 0.0f ? (double)t * log((double)least) : 0.0;
     // ---- the largest logit of all (as a key: a NaN's is above all), with temperature 0 its lowest index too. For top-k, bins of the
     // threads' largest go along.
     unsigned top = key_of(most), low = most > -INFINITY ? top : ~0u;  // the lowest: of the threads' largest
@@ -749,13 +751,13 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
     int turn = 0, pass = 0;
     r.most = most;
     r.top = most;
-    r.c = 1.4426950408889634 / (t > 0.0f ? (double)t : 1.0);
-    r.zero = fmaxf((float)(r.top - 46.0 / r.c), kLowest);
+    r.c = octaves_per_logit;
+    r.zero = fmaxf((float)(r.top - 46.0 * logits_per_octave), kLowest);
     r.share = 0, r.known = false;
     r.key = kNone, r.last = -0x7fffffff;  // (what lies outside the row has indices from -3 on)
     const unsigned min_key = [&]() -> unsigned {  // of the lowest logit that min_p leaves
         if (!(least > 0.0f)) return 0;
-        const double border = r.top + (double)t * log((double)least);
+        const double border = r.top + min_below;
         return border >= r.top ? key_of(most) : key_of(__double2float_ru(border));
     }();
     int token = -1;  // where it is known already
@@ -811,7 +813,7 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
             }
         }
         if (!done && p < 1.0f) {
-            const float octaves = fminf(octaves_of(p, a.vocab), 46.0f), end = fmaxf((float)(r.top - octaves / r.c), kLowest);
+            const float octaves = fminf(octaves_of(p, a.vocab), 46.0f), end = fmaxf((float)(r.top - octaves * logits_per_octave), kLowest);
             if (r.key == kNone) {
                 nucleus(s, r, p, end, pass, turn);
             } else {
