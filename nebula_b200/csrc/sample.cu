@@ -60,8 +60,7 @@ struct Shared {
     Whole total[2][kMaxRanks];         // by the parity of the exchange: a CTA may be one ahead
     unsigned hist[2][2][kBins];        // by the parity of the pass: counts, or the low and high words of sums
     Whole list[kList];                 // key and inverted index: the larger is the better
-    int listed;
-    Whole coarse[kFine / 32];
+    int listed, lists[kMaxRanks];      // of this CTA's list and of all
     union {
         unsigned fine[2][kFine];       // words of sums
         Whole entry[kList];            // from here on a CTA's own: these once all have read the bins, with a barrier between
@@ -69,7 +68,7 @@ struct Shared {
     };
     union {
         Whole entry_weight[kFew];
-        Whole read[kMaxRanks][32];     // until entries are ordered
+        Whole read[kMaxRanks][kFine / 32];  // sums of the CTAs' groups of bins, then of a group's bins; until entries are ordered
     };
     Whole warp_sum[kWarps];
     Whole found, kept_sum;
@@ -151,9 +150,14 @@ struct Row {
     double top, c;       // log2(e) / T
     unsigned key;        // kept: logits above the key, and those at it up to index `last`
     int last;
-    bool known;          // whether all threads' shares add up to the weights that this CTA keeps
+    bool settled;        // whether it is known already what the CTAs' kept weights add up to
+    bool known;          // whether all threads' shares add up to those that this CTA keeps
     Whole share;
+    int ahead;           // logits of the first CTA that lie before the row
+    unsigned inverse;    // of units
 
+    // The CTA that has a logit.
+    __device__ __forceinline__ int rank_of(int i) const { return (int)(((unsigned)(i + ahead) / kStep) * inverse >> 16); }
     // f(x, index) for every logit of the thread.
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
@@ -274,26 +278,35 @@ struct Row {
 };
 
 // Of the threads' sums: the warps' to s.warp_sum, the CTAs' to s.total of all. Ends with a barrier of the cluster.
-__device__ __forceinline__ void share_sums(Shared &s, const Row &r, Whole x, int turn) {
+// `along` is called by all threads once all are here, before that barrier.
+template <typename F>
+__device__ __forceinline__ void share_sums(Shared &s, const Row &r, Whole x, int turn, F along) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     x = warp_sum(x);
     if (lane == 0) s.warp_sum[warp] = x;
     __syncthreads();
+    along();
     if (warp == 0) {
         const Whole all = warp_sum(lane < kWarps ? s.warp_sum[lane] : 0);
         if (lane < r.ranks) peer_store(at_rank(&s.total[turn & 1][r.rank], lane), all);
     }
     cluster_sync();
 }
+__device__ __forceinline__ void share_sums(Shared &s, const Row &r, Whole x, int turn) {
+    share_sums(s, r, x, turn, [] {});
+}
 // Totals of the CTAs before this one, and of all.
 __device__ __forceinline__ Whole sums_before(const Shared &s, const Row &r, int turn, Whole &all) {
     Whole before = 0;
     all = 0;
-    for (uint32_t i = 0; i < r.ranks; i++) {
-        const Whole x = s.total[turn & 1][i];
-        if (i < r.rank) before += x;
-        all += x;
-    }
+#pragma unroll 1
+    for (uint32_t i0 = 0; i0 < r.ranks; i0 += 4)
+#pragma unroll
+        for (uint32_t i = i0; i < i0 + 4; i++) {
+            const Whole x = i < r.ranks ? s.total[turn & 1][i] : 0;
+            if (i < r.rank) before += x;
+            all += x;
+        }
     return before;
 }
 // The index at which the running sum of f (in the order of indices) reaches `target`, for the one warp that holds it; -1 for
@@ -408,9 +421,11 @@ __device__ int gather(Shared &s, const Row &r, const Range &in) {
                 if (to < kList) s.list[to] = (Whole)key_of(x[e]) << 32 | (unsigned)~at[e];
             }
     });
+    __syncthreads();
+    if (threadIdx.x < r.ranks) peer_store(at_rank(&s.lists[r.rank], threadIdx.x), (unsigned)s.listed);
     cluster_sync();
     // a lane has a CTA's number, and where its part of the list begins
-    const int lane = threadIdx.x & 31, n = lane < r.ranks ? (int)peer_load(at_rank(&s.listed, lane)) : 0;
+    const int lane = threadIdx.x & 31, n = lane < r.ranks ? s.lists[lane] : 0;
     int upto = n;
 #pragma unroll
     for (int d = 1; d < kMaxRanks; d <<= 1) {
@@ -581,11 +596,10 @@ __device__ __forceinline__ Whole share_of(float p, Whole all) {
 __device__ __forceinline__ float octaves_of(float p, int vocab) { return log2f((float)vocab) - log2f(1.0f - fmaxf(p, 0.0f)) + 1.0f; }
 
 // Top-p of a whole row: the sum of all weights and the bins of those that may matter, none of which lie below `end`, in one pass.
-__device__ void nucleus(Shared &s, Row &r, float p, float end, int &pass, int &turn) {
+// s.fine is zero before. Where it comes down to a list, what the CTAs keep is in s.total[turn & 1] (for `settle`).
+__device__ void nucleus(Shared &s, Row &r, float p, float end, bool settle, int &pass, int &turn) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     Range in = {key_of(end), key_of(r.most), r.most, fminf(kFine / (r.most - end), 1e30f), kFine - 1, -1};
-    for (int i = tid; i < 2 * kFine; i += kThreads) s.fine[0][i] = 0;
-    __syncthreads();
     Whole sum = 0;
     r.each_weight(-INFINITY, [&](const float (&x)[4], int, const Whole (&w)[4]) {
         sum += (w[0] + w[1]) + (w[2] + w[3]);
@@ -596,27 +610,24 @@ __device__ void nucleus(Shared &s, Row &r, float p, float end, int &pass, int &t
                 add_words(s.fine[0][bin], s.fine[1][bin], w[e]);
             }
     });
-    __syncthreads();
+    share_sums(s, r, sum, turn, [&] {  // and the sums of groups of 32 bins
 #pragma unroll
-    for (int g = warp; g < kFine / 32; g += kWarps) {
-        const int bin = 32 * g + lane;
-        const Whole of_group = warp_sum(words(s.fine[0][bin], s.fine[1][bin]));
-        if (lane == 0) s.coarse[g] = of_group;
-    }
-    share_sums(s, r, sum, turn);
+        for (int g = warp; g < kFine / 32; g += kWarps) {
+            const Whole of_group = warp_sum(words(s.fine[0][32 * g + lane], s.fine[1][32 * g + lane]));
+            if (lane < r.ranks) peer_store(at_rank(&s.read[r.rank][g], lane), of_group);
+        }
+    });
     Whole all;
     sums_before(s, r, turn, all);
     turn++;
     Whole target = share_of(p, all);
-    // the group, then the bin in it; a warp reads one CTA's, and every warp looks for it
-    auto find = [&](Whole &target) {
-        __syncthreads();
+    // the group, then the bin in it, by every warp
+    auto find = [&]() {
         Whole mine = 0;
 #pragma unroll 1
-        for (uint32_t q0 = 0; q0 < r.ranks; q0 += 8)  // (zeros where there is no CTA)
+        for (uint32_t q0 = 0; q0 < r.ranks; q0 += 8)
 #pragma unroll
-            for (int q = 0; q < 8; q++) mine += s.read[q0 + q][lane];
-        __syncthreads();
+            for (uint32_t q = q0; q < q0 + 8; q++) mine += q < r.ranks ? s.read[q][lane] : 0;
         const Whole upto = warp_scan(mine);
         const unsigned past = __ballot_sync(0xffffffffu, upto >= target);
         if (!past) return -1;
@@ -624,21 +635,47 @@ __device__ void nucleus(Shared &s, Row &r, float p, float end, int &pass, int &t
         target -= __shfl_sync(0xffffffffu, upto - mine, l);
         return l;
     };
-    s.read[warp][lane] = warp < r.ranks ? peer_load64(at_rank(&s.coarse[lane], warp)) : 0;
-    const int group = find(target);
+    const int group = find();
     if (group < 0) return;  // all of them
-    unsigned low = 0, high = 0;
-    if (warp < r.ranks) low = peer_load(at_rank(&s.fine[0][32 * group + lane], warp)), high = peer_load(at_rank(&s.fine[1][32 * group + lane], warp));
-    s.read[warp][lane] = words(low, high);
-    const int bin = 32 * group + find(target);
-    for (int i = tid; i < bin; i += kThreads) r.share += words(s.fine[0][i], s.fine[1][i]);
-    in.take_bin(bin);
+    // a warp reads one CTA's
+    Whole better = 0, of_bin = 0;
+    if (warp < r.ranks) {
+        better = lane < group ? s.read[warp][lane] : 0;
+        const unsigned low = peer_load(at_rank(&s.fine[0][32 * group + lane], warp)), high = peer_load(at_rank(&s.fine[1][32 * group + lane], warp));
+        of_bin = words(low, high);
+    }
+    __syncthreads();
+    if (warp < r.ranks) s.read[warp][lane] = of_bin;
+    __syncthreads();
+    const int bin = find();
+    if (settle && warp < r.ranks) {
+        better = warp_sum(better + (lane < bin ? of_bin : 0));
+        if (lane == 0) s.total[turn & 1][warp] = better;
+    }
+    in.take_bin(32 * group + bin);
     const int n = gather(s, r, in);
     if (n > kList) {
+        if (settle && tid == 0) r.share = s.total[turn & 1][r.rank];
         narrow<true>(s, r, target, in, false, pass, turn);
         return;
     }
-    keep_to<true>(s, r, nth_entry<true>(s, r, n, in, target, s.hist[pass & 1]));
+    Whole mine[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) mine[i] = tid + i * kThreads < n ? s.entry[tid + i * kThreads] : 0;
+    Hist &hist = s.hist[pass & 1];
+    const Whole worst = nth_entry<true>(s, r, n, in, target, hist);
+    r.key = (unsigned)(worst >> 32), r.last = (int)~(unsigned)worst;
+    if (!settle) return;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        if (mine[i] >= worst) {
+            const int q = r.rank_of((int)~(unsigned)mine[i]);
+            add_words(hist[0][q], hist[1][q], r.weigh(of_key((unsigned)(mine[i] >> 32))));
+        }
+    __syncthreads();
+    if (tid < r.ranks) s.total[turn & 1][tid] += words(hist[0][tid], hist[1][tid]);
+    __syncthreads();
+    r.settled = true;
 }
 
 // Bins a quarter wide around the logits that models give, and the lowest logit of one. They serve to leave out most logits
@@ -663,6 +700,7 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
     const int ahead = (int)(reinterpret_cast<uintptr_t>(x0) >> 2 & 3);  // logits between a multiple of 16 bytes and the row
     const int start = (int)r.rank * a.units * kStep - ahead;
     r.index = start + tid * 4 * a.units;
+    r.ahead = ahead, r.inverse = a.inverse;
     const float t = a.temperature ? a.temperature[user] : 1.0f, p = a.top_p ? a.top_p[user] : 1.0f, least = a.min_p ? a.min_p[user] : 0.0f;
     const int k = a.top_k ? a.top_k[user] : 0;
     const float u = a.uniforms ? a.uniforms[row] : 0.0f;
@@ -706,6 +744,7 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
     }
     const float threads_most = most;
     const double octaves_per_logit = 1.4426950408889634 / (t > 0.0f ? (double)t : 1.0), logits_per_octave = 0.6931471805599453 * (t > 0.0f ? (double)t : 1.0);
+    const double nucleus_below = p < 1.0f ? fminf(octaves_of(p, a.vocab), 46.0f) * logits_per_octave : 0.0;
     const double min_below = least > 0.0f ? (double)t * log((double)least) : 0.0;
     // ---- the largest logit of all (as a key: a NaN's is above all), with temperature 0 its lowest index too. For top-k, bins of the
     // threads' largest go along.
@@ -715,12 +754,14 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
     if (lane == 0) s.warp_most[warp] = top, s.warp_least[warp] = low;
     // (what this CTA's memory held of the row before is read by others until they are here)
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    const bool cut_k = k > 0 && k < a.vocab && t > 0.0f;
     for (int i = tid; i < 2 * 2 * kBins; i += kThreads) s.hist[0][0][i] = 0;
+    if (!cut_k && p < 1.0f)
+        for (int i = tid; i < 2 * kFine; i += kThreads) s.fine[0][i] = 0;
     if (tid == 0) s.listed = 0;
     __syncthreads();
     top = __reduce_max_sync(0xffffffffu, lane < kWarps ? s.warp_most[lane] : 0);
     low = __reduce_min_sync(0xffffffffu, lane < kWarps ? s.warp_least[lane] : ~0u);
-    const bool cut_k = k > 0 && k < a.vocab && t > 0.0f;
     if (t == 0.0f) {
         unsigned index = 0x7fffffff;
         r.some(of_key(top), of_key(top), [&](const float (&x)[2], const int (&at)[2]) {
@@ -738,11 +779,9 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
     if (warp == 0 && lane < r.ranks) peer_store(at_rank(&s.ends[r.rank], lane), (Whole)top << 32 | ~low);
     cluster_sync();
     // of equal keys the lowest index; without temperature 0, the lowest of all
-    Whole end = 0;
-    unsigned least_key = ~0u;
-#pragma unroll 1
-    for (int i = 0; i < r.ranks; i++) end = max(end, s.ends[i]), least_key = min(least_key, ~(unsigned)s.ends[i]);
-    most = of_key((unsigned)(end >> 32));
+    const Whole of_rank = lane < r.ranks ? s.ends[lane] : 0;
+    const unsigned most_key = __reduce_max_sync(0xffffffffu, (unsigned)(of_rank >> 32)), least_key = __reduce_min_sync(0xffffffffu, ~(unsigned)of_rank);
+    most = of_key(most_key);
     const float lowest = least_key == ~0u ? most : of_key(least_key);
     const bool refused = !(most > -INFINITY && most < INFINITY) || !(t >= 0.0f && t < INFINITY) || p != p || least != least || u != u;
 
@@ -753,7 +792,7 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
     r.top = most;
     r.c = octaves_per_logit;
     r.zero = fmaxf((float)(r.top - 46.0 * logits_per_octave), kLowest);
-    r.share = 0, r.known = false;
+    r.share = 0, r.known = r.settled = false;
     r.key = kNone, r.last = -0x7fffffff;  // (what lies outside the row has indices from -3 on)
     const unsigned min_key = [&]() -> unsigned {  // of the lowest logit that min_p leaves
         if (!(least > 0.0f)) return 0;
@@ -763,7 +802,7 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
     int token = -1;  // where it is known already
     if (refused) {
     } else if (t == 0.0f) {  // the largest logit, the lowest index of equals
-        r.key = key_of(most), r.last = (int)~(unsigned)end;
+        r.key = most_key, r.last = (int)~__reduce_max_sync(0xffffffffu, (unsigned)(of_rank >> 32) == most_key ? (unsigned)of_rank : 0);
         token = r.last;
     } else {
         bool done = false;
@@ -813,9 +852,13 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
             }
         }
         if (!done && p < 1.0f) {
-            const float octaves = fminf(octaves_of(p, a.vocab), 46.0f), end = fmaxf((float)(r.top - octaves * logits_per_octave), kLowest);
+            const float end = fmaxf((float)(r.top - nucleus_below), kLowest);
             if (r.key == kNone) {
-                nucleus(s, r, p, end, pass, turn);
+                if (cut_k) {
+                    for (int i = tid; i < 2 * kFine; i += kThreads) s.fine[0][i] = 0;
+                    __syncthreads();
+                }
+                nucleus(s, r, p, end, a.token, pass, turn);
             } else {
                 Whole all;
                 share_sums(s, r, r.kept_sum(), turn);
@@ -825,7 +868,11 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
                              true, pass, turn);
             }
         }
-        if (!done && min_key > r.key) r.key = min_key, r.last = 0x7fffffff, r.known = false;
+        if (!done && min_key > r.key) {
+            r.key = min_key, r.last = 0x7fffffff;
+            turn += r.settled;  // (others may be at the next exchange already)
+            r.known = r.settled = false;
+        }
     }
 
     // ---- the token, or the logits
@@ -835,13 +882,16 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
             return;
         }
         auto mine = [&](float x, int index) { return r.keeps(x, index) ? r.weigh(x) : 0; };
-        Whole sum = r.known ? r.share : r.kept_sum(), all;
-        share_sums(s, r, sum, turn);
+        Whole sum = 0, all;
+        if (!r.settled) {
+            sum = r.known ? r.share : r.kept_sum();
+            share_sums(s, r, sum, turn);
+        }
         const Whole before = sums_before(s, r, turn, all);
         // the first running sum above u * all is the first that reaches the whole number after it
         const float v = fminf(fmaxf(u, 0.0f), 0.99999994f);
         const Whole aim = __umul64hi(__double2ull_rz((double)v * 18446744073709551616.0), all) + 1;
-        if (r.known) {  // by index, in the one CTA that has the token
+        if (r.settled || r.known) {  // by index, in the one CTA that has the token
             if (before >= aim || before + s.total[turn & 1][r.rank] < aim) return;
             sum = r.kept_sum();
             const Whole of_warp = warp_sum(sum);
