@@ -357,7 +357,9 @@ __device__ __forceinline__ Bin reach_bin(Shared &s, Whole mine, Whole target) {
 // clocks a warp over 64 bins, two words 5.6, three parts that need no carry 7.5).
 __device__ __forceinline__ void add_words(unsigned &low, unsigned &high, Whole w) {
     const unsigned before = atomicAdd(&low, (unsigned)w);
-    atomicAdd(&high, (unsigned)(w >> 32) + (before + (unsigned)w < before));
+    unsigned carried;
+    asm("{.reg .u32 t;\n add.cc.u32 t, %1, %2;\n addc.u32 %0, %3, 0;}" : "=r"(carried) : "r"(before), "r"((unsigned)w), "r"((unsigned)(w >> 32)));
+    atomicAdd(&high, carried);
 }
 __device__ __forceinline__ Whole words(unsigned low, unsigned high) { return (Whole)high << 32 | low; }
 // A histogram counts, or adds up weights.
@@ -599,14 +601,14 @@ __device__ __forceinline__ float octaves_of(float p, int vocab) { return log2f((
 // s.fine is zero before. Where it comes down to a list, what the CTAs keep is in s.total[turn & 1] (for `settle`).
 __device__ void nucleus(Shared &s, Row &r, float p, float end, bool settle, int &pass, int &turn) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    Range in = {key_of(end), key_of(r.most), r.most, fminf(kFine / (r.most - end), 1e30f), kFine - 1, -1};
+    Range in = {key_of(end), key_of(r.most), r.most, fminf((kFine - 0.001f) / (r.most - end), 1e30f), kFine - 1, -1};
     Whole sum = 0;
     r.each_weight(-INFINITY, [&](const float (&x)[4], int, const Whole (&w)[4]) {
         sum += (w[0] + w[1]) + (w[2] + w[3]);
 #pragma unroll
         for (int e = 0; e < 4; e++)
             if (x[e] >= end) {
-                const int bin = in.bin_of(x[e]);
+                const int bin = (int)((in.most - x[e]) * in.scale);  // bin_of: kFine is not reached
                 add_words(s.fine[0][bin], s.fine[1][bin], w[e]);
             }
     });
@@ -946,18 +948,21 @@ int launch(SampleArgs &a, int rows) {
     // up to three logits may lie before a row that does not start on 16 bytes
     const bool aligned = !(reinterpret_cast<uintptr_t>(a.logits) & 15) && a.vocab % 4 == 0;
     const int long_row = a.vocab + (aligned ? 0 : 3);
-    // Clusters of more CTAs take less time for a row, but fewer of them fit. A row takes about as long for its fixed steps
-    // as for seven units of a thread (eight with 16 CTAs, which should have an SM each), and the GPU takes 33, 71, 148 or 296 clusters
-    // of 8, 4, 2 or 1 CTAs (15, 33, 74 and 148 where a CTA has more than half an SM's memory) at once. A nucleus among 131,072, one
-    // row: 23 us with 8, 19 with 16; 14 rows: 24 and 26. 37 rows of 50,001 with top-k 40: 18 us with 8, 13 with 4.
+    // Clusters of more CTAs take less time for a row, but fewer of them fit: as many as these, by what cudaOccupancyMaxActiveClusters
+    // says, two CTAs to an SM (up to half its memory each) or one. A row takes about as long for its fixed steps as for seven units
+    // of a thread, and 1.4 times as long where CTAs share an SM. A nucleus of 0.9 with the number of CTAs that this takes, and
+    // with others: 14 rows of 131,072 8 (21.7 us) or 16 (24.3); 17 rows 13 (26) or 8 (27.9); 256 rows 6 (200) or 8 (209);
+    // 37 rows of 50,001 7 (22.4) or 4 (25.4); 60 rows of 200,000 9 (75) or 8 (103).
+    static constexpr short kTwo[kMaxRanks] = {296, 148, 93, 71, 56, 45, 37, 33, 30, 26, 21, 21, 17, 14, 14, 14};
+    static constexpr short kOne[kMaxRanks] = {148, 74, 45, 33, 26, 22, 15, 15, 15, 11, 7, 7, 7, 7, 7, 7};
     int ranks = 1, clusters = 1;
     long long best = 0;
-    for (int n = 1; n <= kMaxRanks; n *= 2) {
+    for (int n = 1; n <= kMaxRanks; n++) {
         const int units = ((long_row + n - 1) / n + kStep - 1) / kStep;
         if (units > kMaxUnits) continue;
         const bool half = kThreads * (units | 1) * 16 + (int)sizeof(Shared) <= 115200;
-        const int fit = n == 16 ? 7 : n == 8 ? (half ? 33 : 15) : n == 4 ? (half ? 71 : 33) : (half ? 296 : 148) / n;
-        const long long time = (long long)((rows + fit - 1) / fit) * (7 + (n == 16) + units);
+        const int one = kOne[n - 1], fit = half ? kTwo[n - 1] : one, rest = rows % fit;
+        const long long time = (long long)(7 + units) * ((long long)(rows / fit) * (half ? 7 : 5) + (rest > one ? 7 : rest ? 5 : 0));
         if (!best || time < best) best = time, ranks = n, clusters = rows < fit ? rows : fit, a.units = units;
     }
     const int smem = kThreads * (a.units | 1) * 16 + (int)sizeof(Shared);
