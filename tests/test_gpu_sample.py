@@ -243,3 +243,25 @@ def test_two_graphs_at_once(L):
             assert got[r] == B.sample(x[r], u[r], top_p=float(np.float32(0.9)))[0]
     for g in graphs:
         L.graph_destroy(g)
+
+
+@pytest.mark.parametrize("rows,vocab", [(60, 4097), (6, 10001), (100, 12288), (6, 12288), (13, 40001), (9, 50001), (6, 20000), (6, 65537),
+                                        (6, 24576), (6, 50001), (6, 200000)])
+def test_clusters_of_any_size(L, rows, vocab):
+    """Rows and lengths for which a row has 2, 5, 1, 6, 7, 9, 10, 11, 12, 13 and 14 CTAs: with borders that come out of a list, of more
+    than a list, of min-p within what top-p keeps, and of top-k where it leaves all that is finite."""
+    rng = np.random.default_rng(rows * vocab)
+    x = peaked(rng, rows, vocab).astype(np.float32)
+    chosen = [(1.0, 0, 0.9, 0.0), (1.0, 0, 0.9, 0.002), (3.0, 1000, 0.8, 0.0), (25.0, 0, 0.7, 0.0), (1.5, 2000, 0.9, 0.0), (1.0, 0, 0.98, 1e-4)]
+    t, k, p, m = zip(*[chosen[r % 6] for r in range(rows)])
+    for r in range(4, rows, 6):
+        x[r, rng.permutation(vocab)[:-700]] = -np.inf
+    check(L, x, rng.random(rows), t, k, p, m)
+
+
+def test_min_p_within_a_nucleus_row_after_row(L):
+    """More rows than clusters, of one kind, with a border that is found twice."""
+    rng = np.random.default_rng(8)
+    x = peaked(rng, 400, 8191)
+    for least in (0.0005, 0.01):
+        check(L, x, rng.random(400), [1.0] * 400, [0] * 400, [0.97] * 400, [least] * 400)
