@@ -597,6 +597,47 @@ __device__ __forceinline__ Whole share_of(float p, Whole all) {
 // leaves out. The sum is one largest weight at least.
 __device__ __forceinline__ float octaves_of(float p, int vocab) { return log2f((float)vocab) - log2f(1.0f - fmaxf(p, 0.0f)) + 1.0f; }
 
+// The kept set ends where the n entries' weights, from the best on, reach `target`. With `settle`, s.total[turn & 1] has what the
+// CTAs keep besides, and has all of it after.
+__device__ __forceinline__ void cut_list(Shared &s, Row &r, int n, const Range &in, Whole target, bool settle, int pass, int turn) {
+    const int tid = threadIdx.x;
+    Whole mine[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) mine[i] = tid + i * kThreads < n ? s.entry[tid + i * kThreads] : 0;
+    Hist &hist = s.hist[pass & 1];
+    const Whole worst = nth_entry<true>(s, r, n, in, target, hist);
+    r.key = (unsigned)(worst >> 32), r.last = (int)~(unsigned)worst;
+    if (!settle) return;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        if (mine[i] >= worst) {
+            const int q = r.rank_of((int)~(unsigned)mine[i]);
+            add_words(hist[0][q], hist[1][q], r.weigh(of_key((unsigned)(mine[i] >> 32))));
+        }
+    __syncthreads();
+    if (tid < r.ranks) s.total[turn & 1][tid] += words(hist[0][tid], hist[1][tid]);
+    __syncthreads();
+    r.settled = true;
+}
+
+// Top-p of a kept set of kList logits at most, all of which every CTA then has.
+__device__ void listed_nucleus(Shared &s, Row &r, float p, bool settle, int pass, int turn) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    cluster_sync();  // others have read this CTA's list
+    if (tid == 0) s.listed = 0;
+    if (tid < r.ranks) s.total[turn & 1][tid] = 0;
+    __syncthreads();
+    const Range in = {r.key, key_of(r.most), r.most, 0.0f, 0, -1};
+    const int n = gather(s, r, in);
+    Whole sum = 0;
+    for (int i = tid; i < n; i += kThreads) sum += r.weigh(of_key((unsigned)(s.entry[i] >> 32)));
+    sum = warp_sum(sum);
+    if (lane == 0) s.warp_sum[warp] = sum;
+    __syncthreads();
+    const Whole all = warp_sum(lane < kWarps ? s.warp_sum[lane] : 0);
+    cut_list(s, r, n, in, share_of(p, all), settle, pass, turn);
+}
+
 // Top-p of a whole row: the sum of all weights and the bins of those that may matter, none of which lie below `end`, in one pass.
 // s.fine is zero before. Where it comes down to a list, what the CTAs keep is in s.total[turn & 1] (for `settle`).
 __device__ void nucleus(Shared &s, Row &r, float p, float end, bool settle, int &pass, int &turn) {
@@ -661,23 +702,7 @@ __device__ void nucleus(Shared &s, Row &r, float p, float end, bool settle, int 
         narrow<true>(s, r, target, in, false, pass, turn);
         return;
     }
-    Whole mine[2];
-#pragma unroll
-    for (int i = 0; i < 2; i++) mine[i] = tid + i * kThreads < n ? s.entry[tid + i * kThreads] : 0;
-    Hist &hist = s.hist[pass & 1];
-    const Whole worst = nth_entry<true>(s, r, n, in, target, hist);
-    r.key = (unsigned)(worst >> 32), r.last = (int)~(unsigned)worst;
-    if (!settle) return;
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-        if (mine[i] >= worst) {
-            const int q = r.rank_of((int)~(unsigned)mine[i]);
-            add_words(hist[0][q], hist[1][q], r.weigh(of_key((unsigned)(mine[i] >> 32))));
-        }
-    __syncthreads();
-    if (tid < r.ranks) s.total[turn & 1][tid] += words(hist[0][tid], hist[1][tid]);
-    __syncthreads();
-    r.settled = true;
+    cut_list(s, r, n, in, target, settle, pass, turn);
 }
 
 // Bins a quarter wide around the logits that models give, and the lowest logit of one. They serve to leave out most logits
@@ -861,6 +886,8 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
                     __syncthreads();
                 }
                 nucleus(s, r, p, end, a.token, pass, turn);
+            } else if (k <= kList) {
+                listed_nucleus(s, r, p, a.token, pass, turn);
             } else {
                 Whole all;
                 share_sums(s, r, r.kept_sum(), turn);

@@ -265,3 +265,12 @@ def test_min_p_within_a_nucleus_row_after_row(L):
     x = peaked(rng, 400, 8191)
     for least in (0.0005, 0.01):
         check(L, x, rng.random(400), [1.0] * 400, [0] * 400, [0.97] * 400, [least] * 400)
+
+
+@pytest.mark.parametrize("steps", [1e-6, 0.25])
+def test_top_p_of_as_many_as_a_list_holds(L, steps):
+    """Where top-p goes through a list of top-k's logits, and through passes over the row: 1,024 of them, and one more; equals at the border."""
+    rng = np.random.default_rng(9)
+    k = [257, 1023, 1024, 1025, 700, 1024]
+    x = np.round(2 * rng.normal(size=(6, 30011)) / steps) * steps
+    check(L, x, rng.random(6), [1.0, 2.0, 1.0, 1.0, 0.7, 1e6], k, [0.9, 0.99, 0.5, 0.5, 1e-7, 0.999], [0.0, 0.0, 0.0, 0.0, 0.0, 0.0])
