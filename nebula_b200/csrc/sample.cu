@@ -710,12 +710,13 @@ __device__ void nucleus(Shared &s, Row &r, float p, float end, bool settle, int 
 __device__ __forceinline__ int plain_bin(float x) { return (int)fminf(fmaxf((24.0f - x) * 4.0f, 0.0f), (float)(kBins - 1)); }
 __device__ __forceinline__ float plain_edge(int bin) { return 24.0f - 0.25f * (bin + 1) - 1e-4f; }
 // A lower bound of the k-th largest logit, from bins of each thread's largest, in s.hist[0] (k logits are at least as large as
-// the k-th largest of these); -infinity where there is none. many: more than kFew logits are above it for sure.
+// the k-th largest of these); -infinity where there is none. many: so many logits are above it for sure that a list
+// will hardly do.
 __device__ float bound_of(Shared &s, const Row &r, int k, bool &many, int &pass) {
     const Whole count = all_bins<false>(s, r, s.hist[pass & 1]);
     pass++;  // (the next pass clears this histogram)
     const Bin b = reach_bin(s, count, k);
-    many = __syncthreads_or((int)threadIdx.x == b.bin && b.before + count > kFew);
+    many = __syncthreads_or((int)threadIdx.x == b.bin && b.before + count > kList / 2);
     return b.bin < 0 || b.bin == kBins - 1 ? -INFINITY : plain_edge(b.bin);
 }
 
@@ -834,10 +835,11 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
     } else {
         bool done = false;
         if (cut_k) {
-            int n = kFew + 1;
+            int n = kList + 1;
             bool many;
             const float bound = bound_of(s, r, k, many, pass);
-            if (!many && bound > -INFINITY) n = gather(s, r, {key_of(bound), key_of(most), most, 0.0f, 0, -1});
+            const Range upward = {key_of(bound), key_of(most), most, 0.0f, 0, -1};
+            if (!many && bound > -INFINITY) n = gather(s, r, upward);
             if (n <= kFew) {
                 // few enough: all of the rest is in every CTA's own memory
                 Whole above;
@@ -874,6 +876,8 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
                     }
                     return;
                 }
+            } else if (n <= kList) {
+                keep_to<false>(s, r, nth_entry<false>(s, r, n, upward, min(k, n), s.hist[pass & 1]));
             } else {
                 narrow<false>(s, r, k, {key_of(bound), key_of(most), most, bins_down_to(fmaxf(bound, lowest)), kBins - 1, -1}, true, pass, turn);
             }
