@@ -25,6 +25,7 @@ class User:
     uniforms: object  # an iterator of numbers in [0, 1)
     settings: tuple = (0.0, 0, 1.0, 0.0)  # temperature, top_k, top_p, min_p
     text: list = field(default_factory=list)
+    drawn: float | None = None  # the number for the next token, until that is there
 
 
 class Batch(Speculator):
@@ -112,27 +113,33 @@ class Batch(Speculator):
         L.call("cache_commit", C.byref(self.cache), self.lengths.p, self.path.p, self.accepted.p, self.users, 1)
 
     def step(self) -> None:
-        """Every user reads a token that waits, or gets the next one of its text."""
+        """Every user reads a token that waits, or gets the next one of its text. Where a row is refused the step raises, names the
+        places and keeps nothing: without those users it can be made again."""
         users = self.places
+        last = [u is not None and len(u.waiting) <= 1 for u in users]  # a token is chosen after what the user reads
+        for user, chosen in zip(users, last):
+            if chosen and user.drawn is None:
+                user.drawn = next(user.uniforms)
         self._reserve([int(u is not None) for u in users])
         self._forward([0 if u is None else u.waiting[0] if u.waiting else u.text[-1] for u in users])
         L.call("matmul", self.logits.p, self.head.p, F32, self.vocab, self.hidden, self.x.p, self.users)
-        last = [u is not None and len(u.waiting) <= 1 for u in users]  # a token is chosen after what the user reads
         asked = [u.settings if u is not None else (0.0, 0, 1.0, 0.0) for u in users]
         for buf, values, kind in zip((self.temperature, self.top_k, self.top_p, self.min_p), zip(*asked), (np.float32, np.int32, np.float32, np.float32)):
             self._put(buf, values, kind)
-        self._put(self.uniforms, [next(u.uniforms) if chosen else 0.0 for u, chosen in zip(users, last)], np.float32)
+        self._put(self.uniforms, [u.drawn if chosen else 0.0 for u, chosen in zip(users, last)], np.float32)
         L.call("sample", self.sampled.p, self.logits.p, self.uniforms.p, self.temperature.p, self.top_k.p, self.top_p.p, self.min_p.p, 1,
                self.users, self.vocab)
+        tokens = self.sampled.get()
+        if none := [at for at, (chosen, token) in enumerate(zip(last, tokens)) if chosen and token < 0]:
+            raise RuntimeError(f"the model gave no distribution for places {none}")
         self._commit()
-        for user, chosen, token in zip(users, last, self.sampled.get()):
+        for user, chosen, token in zip(users, last, tokens):
             if user is None:
                 continue
             user.waiting = user.waiting[1:]
-            if chosen and token < 0:
-                raise RuntimeError("the model gave no distribution")
             if chosen:
                 user.text.append(int(token))
+                user.drawn = None
 
     def pages_in_use(self) -> int:
         return self.cache.pages - int(self.free_count.get()[0])
