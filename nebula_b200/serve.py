@@ -117,9 +117,11 @@ class Batch(Speculator):
         places and keeps nothing: without those users it can be made again."""
         users = self.places
         last = [u is not None and len(u.waiting) <= 1 for u in users]  # a token is chosen after what the user reads
-        for user, chosen in zip(users, last):
+        for at, (user, chosen) in enumerate(zip(users, last)):
             if chosen and user.drawn is None:
-                user.drawn = next(user.uniforms)
+                user.drawn = next(user.uniforms, None)
+            if chosen and (user.drawn is None or user.drawn != user.drawn):
+                raise ValueError(f"place {at} has no number in [0, 1) for its next token")
         self._reserve([int(u is not None) for u in users])
         self._forward([0 if u is None else u.waiting[0] if u.waiting else u.text[-1] for u in users])
         L.call("matmul", self.logits.p, self.head.p, F32, self.vocab, self.hidden, self.x.p, self.users)

@@ -74,3 +74,24 @@ def test_a_user_without_a_distribution_stops_no_other(V, place):
     for n in others:
         assert users[n].text[:8] == texts[n], n
     assert users[place].text == []
+
+
+@pytest.mark.parametrize("numbers", [[0.5, 0.25], [0.5, 0.25, float("nan")]])
+def test_a_user_without_uniforms_stops_no_other(V, numbers):
+    """Numbers that end, or are none, take no number from the other users."""
+    settings = (1.0, 0, 1.0, 0.0)
+    texts = [alone(V, [7 + n], n, settings, 8) for n in range(3)]
+    batch = V.Batch(3, **SIZE)
+    rest = batch.read_prompt([3, 4, 5])
+    users = [V.User(rest + [7 + n], V.uniforms(n), settings) for n in range(3)]
+    users[1].uniforms = iter(numbers)
+    for user in users:
+        batch.join(user)
+    with pytest.raises(ValueError, match="1"):
+        for _ in range(20):
+            batch.step()
+    assert len(users[1].text) == 2
+    batch.leave(1)
+    while len(users[0].text) < 8:
+        batch.step()
+    assert [users[0].text[:8], users[2].text[:8]] == [texts[0], texts[2]]
