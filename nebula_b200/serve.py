@@ -14,7 +14,7 @@ from dataclasses import dataclass, field
 import numpy as np
 
 from . import lib as L
-from .speculate import F32, Speculator
+from .speculate import F32, Speculator, check_settings
 
 
 @dataclass
@@ -78,6 +78,9 @@ class Batch(Speculator):
         """A user takes a free place, with the prompt's pages in its row of the table. Returns the place."""
         if not user.waiting or not all(0 <= int(t) < self.vocab for t in user.waiting):
             raise ValueError("a user begins with at least one token of the vocabulary")
+        if not isinstance(user.settings, (tuple, list)) or len(user.settings) != 4:
+            raise ValueError("settings are temperature, top_k, top_p and min_p")
+        check_settings(*user.settings)
         if None not in self.places:
             raise ValueError("no free place")
         at, n = self.places.index(None), len(self.prompt_pages)

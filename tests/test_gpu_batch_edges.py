@@ -95,3 +95,19 @@ def test_a_user_without_uniforms_stops_no_other(V, numbers):
     while len(users[0].text) < 8:
         batch.step()
     assert [users[0].text[:8], users[2].text[:8]] == [texts[0], texts[2]]
+
+
+BAD = [(-1.0, 0, 1.0, 0.0), (float("nan"), 0, 1.0, 0.0), (float("inf"), 0, 1.0, 0.0), (1e39, 0, 1.0, 0.0), (1.0, 0, float("nan"), 0.0),
+       (1.0, 0, 1.0, float("nan")), (1.0, 1 << 31, 1.0, 0.0), (1.0, 0.5, 1.0, 0.0), (1.0, 0, 1.0), None]
+
+
+def test_settings_that_no_row_can_have_are_refused(V):
+    batch = V.Batch(2, **SIZE)
+    for settings in BAD:
+        with pytest.raises(ValueError):
+            batch.join(V.User([1], V.uniforms(0), settings))
+    assert batch.places == [None, None]
+    user = V.User([1], V.uniforms(0), (0.5, -3, 1.5, -1.0))
+    batch.join(user)
+    batch.step()
+    assert len(user.text) == 1
