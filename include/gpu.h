@@ -246,8 +246,14 @@ int qg_moe_profile_read(int phase, double *total_ms, int *launches);
  * 16, 32, 64, 128 or 256. head_dim: 64, 128 or 256. pages*page_tokens is at
  * most 2^31 - 1, table_pages*page_tokens at most 2^31 - 128.
  *
- * A sequence whose length is negative or leaves no room for its nodes gets NaN
- * rows and no store. Where its table names a page outside the pool,
+ * held (device [seqs], NULL: the whole row) says how many entries of a
+ * sequence's row are its pages; those behind them may name pages that are
+ * another's by now and are never read. A cache whose pages come from a
+ * qg_page_pool has the pool's.
+ *
+ * A sequence whose length is negative or leaves no room for its nodes, in the
+ * table or on the pages held, or whose held is outside 0..table_pages, gets NaN
+ * rows and no store, and qg_cache_commit leaves its length as it is. Where its table names a page outside the pool,
  * qg_tree_attention gives all its rows NaN, qg_qk_norm_rope the rows whose own
  * position is on that page (they are not stored; its other rows are), and
  * qg_cache_commit leaves it as it is when a row would move from or to that page.
@@ -258,6 +264,7 @@ typedef struct {
     int *lengths;           /* device [seqs] */
     size_t layer_bytes;     /* from one layer's pool to the next's */
     int layers, pages, page_tokens, table_pages, kv_heads, head_dim;
+    const int *held;        /* device [seqs], or NULL */
 } qg_kv_cache;
 
 /* table [positions][rotary/2][2]: cos and sin of position*base^(-2i/rotary),
@@ -394,7 +401,11 @@ int qg_truncate_logits(float *out, const float *logits, const float *temperature
  * host. A stack of free pages: free_pages[0 .. *free_count), the last one on
  * top; held[s] entries of sequence s's row of the page table are its pages. Shared pages
  * are entries that the host writes into several rows (and counts in their
- * held). A call uses seqs rows of the table; calls on one pool must not overlap on the device. */
+ * held). Entries behind held keep whatever page they named last, which may be
+ * another sequence's now: the cache that the step runs on is given this held
+ * (qg_kv_cache), so that a sequence which got no page is left out of it on the
+ * device, with NaN rows and its length as it was, and no other is touched.
+ * A call uses seqs rows of the table; calls on one pool must not overlap on the device. */
 typedef struct {
     int *page_table;  /* device [seqs][table_pages]: the cache's */
     int *held;        /* device [seqs] */
@@ -404,7 +415,9 @@ typedef struct {
 } qg_page_pool;
 
 /* Room for counts[s] (0..tokens; NULL: tokens) new positions after lengths[s] of each
- * sequence. In the order of the sequences, the pages that lengths[s] + counts[s]
+ * sequence. A verify step stores and reads all of its nodes: a sequence that takes
+ * part in a step of `tokens` has that count however few of them it uses, and one that
+ * sits out has 0 (with accepted -1 for qg_cache_commit). In the order of the sequences, the pages that lengths[s] + counts[s]
  * positions need beyond held[s] come off the stack and are appended to the row;
  * a sequence for which there are not enough, and all later ones that need any,
  * get none. taken[s]: pages taken, -2: none for want of pages, -1: refused (a

@@ -12,13 +12,15 @@ struct CacheView {
     __half *k, *v;  // one layer's pools
     const int *table;
     const int *lengths;
+    const int *held;  // entries of a row that are its sequence's pages, or NULL: all
     int pages, shift, table_pages, kv_heads, head_dim;
 
     __host__ __device__ int page_tokens() const { return 1 << shift; }
-    // Committed tokens of a sequence, or -1 when its length leaves no room for its nodes.
+    // Committed tokens of a sequence, or -1 when its length leaves no room for its nodes: in the table, or on the pages that it
+    // has. What its row names behind those may be another sequence's by now.
     __device__ int committed(int seq, int tokens) const {
-        const int n = lengths[seq];
-        return n >= 0 && n <= (table_pages << shift) - tokens ? n : -1;
+        const int n = lengths[seq], room = held ? held[seq] : table_pages;
+        return n >= 0 && (unsigned)room <= (unsigned)table_pages && n <= (room << shift) - tokens ? n : -1;
     }
     // Pool row of a position (64 bits: a pool may hold more than 2^31 values), or -1 for a page outside the pool.
     __device__ long long row(int seq, int pos) const {
@@ -67,11 +69,13 @@ inline int cache_view(const qg_kv_cache *c, int layer, int seqs, int tokens, Cac
     if (shift < 0 || pool_too_large(c->pages, c->table_pages, shift)) return cudaErrorInvalidValue;
     const size_t pool = ((size_t)c->pages << shift) * c->kv_heads * c->head_dim * sizeof(__half);
     if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15) return cudaErrorInvalidValue;
+    if (reinterpret_cast<uintptr_t>(c->held) & 3) return cudaErrorInvalidValue;
     if (c->layers > 1 && (c->layer_bytes < pool || c->layer_bytes % 16)) return cudaErrorInvalidValue;
     view.k = reinterpret_cast<__half *>(static_cast<char *>(c->k) + layer * c->layer_bytes);
     view.v = reinterpret_cast<__half *>(static_cast<char *>(c->v) + layer * c->layer_bytes);
     view.table = c->page_table;
     view.lengths = c->lengths;
+    view.held = c->held;
     view.pages = c->pages;
     view.shift = shift;
     view.table_pages = c->table_pages;

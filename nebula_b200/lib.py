@@ -67,10 +67,11 @@ SIGNATURES = {
 
 
 class KvCache(C.Structure):
-    """qg_kv_cache: the paged key/value cache of the verify step (pass C.byref of it)."""
+    """qg_kv_cache: the paged key/value cache of the verify step (pass C.byref of it). ``held``: that of the pool which
+    the pages come from, if they do."""
 
     _fields_ = [("k", P), ("v", P), ("page_table", P), ("lengths", P), ("layer_bytes", Z), ("layers", I), ("pages", I),
-                ("page_tokens", I), ("table_pages", I), ("kv_heads", I), ("head_dim", I)]
+                ("page_tokens", I), ("table_pages", I), ("kv_heads", I), ("head_dim", I), ("held", P)]
 
 
 class PagePool(C.Structure):

@@ -1,8 +1,14 @@
 """Operators for a batch of users on a B200, at the edges of what their header allows and next to each other."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
+from conftest import assert_parity
+from oracle import speculate as S
 from test_gpu_sample import L, check  # noqa: F401  (L is a fixture)
+from test_gpu_shared_attention import SharedCache, attend_shared
+from test_gpu_speculate import attend, expected, random_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -20,6 +26,169 @@ def test_min_p_above_one_leaves_the_first_of_equals(L, least):  # noqa: F811
     u = np.array([0.0, 0.9, 0.99, 0.3, 0.7, 0.999, 0.5, 0.6])
     for k, p in ((0, 1.0), (50, 1.0), (400, 1.0), (2000, 1.0), (5002, 0.9), (0, 0.9), (0, 0.0), (1, 1.0)):
         check(L, x, u, [1.0] * 8, [k] * 8, [p] * 8, [least] * 8)
+
+
+# ---- pages that a sequence no longer has -------------------------------------
+
+
+def prepared(L, cache, seqs, tokens, q_heads, rows, ones):  # noqa: F811
+    """Keys and values of one step into the cache, without rotation; their normalised queries."""
+    hkv, d = cache.kv_heads, cache.head_dim
+    x = L.Device(np.ascontiguousarray(rows, np.float32))
+    width = (q_heads + 2 * hkv) * d
+    out = L.Device.empty((seqs * tokens, q_heads, d), np.float32)
+    L.call("qk_norm_rope", out.p, C.byref(cache), 0, x.p, width, x.p + 4 * q_heads * d, width, x.p + 4 * (q_heads + hkv) * d, width, ones.p, ones.p,
+           1e-6, None, 0, 0, None, seqs, tokens, q_heads)
+    return out
+
+
+class Paged:
+    """A cache of one layer whose pages come from a pool."""
+
+    def __init__(self, L, seqs, pages, table_pages, hkv=2, d=64, page=16):  # noqa: F811
+        self.L, self.seqs, self.page, self.hkv, self.d, self.pages = L, seqs, page, hkv, d, pages
+        self.k, self.v = (L.Device(np.full((pages * page, hkv, d), 0.5, np.float16)) for _ in range(2))
+        self.table, self.held = L.Device(np.zeros((seqs, table_pages), np.int32)), L.Device(np.zeros(seqs, np.int32))
+        self.free, self.count = L.Device(np.arange(pages, dtype=np.int32)), L.Device(np.array([pages], np.int32))
+        self.lengths, self.taken, self.freed = (L.Device(np.zeros(seqs, np.int32)) for _ in range(3))
+        self.pool = L.PagePool(self.table.p, self.held.p, self.free.p, self.count.p, pages, page, table_pages)
+        self.cache = L.KvCache(k=self.k.p, v=self.v.p, page_table=self.table.p, lengths=self.lengths.p, layer_bytes=self.k.nbytes, layers=1, pages=pages,
+                               page_tokens=page, table_pages=table_pages, kv_heads=hkv, head_dim=d, held=self.held.p)
+        self.ones = L.Device(np.ones(d, np.float32))
+
+    def reserve(self, counts, tokens):
+        n = None if counts is None else self.L.Device(np.array(counts, np.int32))
+        self.L.call("pages_reserve", C.byref(self.pool), None, self.taken.p, self.lengths.p, n.p if n else None, self.seqs, tokens)
+        return list(self.taken.get())
+
+    def release(self):
+        self.L.call("pages_release", C.byref(self.pool), self.freed.p, self.lengths.p, 0, self.seqs)
+        return list(self.freed.get())
+
+    def rows(self, s, start, count):
+        return S.positions_rows(self.table.get()[s], self.page, start, count)
+
+
+def test_a_sequence_that_got_no_page_writes_into_no_other(L):  # noqa: F811
+    """A pool of one page: sequence 0 has it, ends, and sequence 1 gets it. Sequence 0's row of the table still names the page when it
+    begins anew and gets none: nothing of the step may reach sequence 1's keys, and sequence 0 waits."""
+    rng = np.random.default_rng(41)
+    p = Paged(L, 2, 1, 4)
+    p.lengths.set(np.array([0, -1], np.int32))
+    assert p.reserve([1, 0], 1) == [1, -1]
+    p.lengths.set(np.array([-1, -1], np.int32))
+    assert p.release() == [1, 0]
+    p.lengths.set(np.array([-1, 0], np.int32))
+    assert p.reserve([0, 5], 5) == [-1, 1]
+    k, v = rng.normal(size=(2, 16, 2, 64)).astype(np.float16)
+    p.k.set(k)
+    p.v.set(v)
+    p.lengths.set(np.array([0, 5], np.int32))
+    assert p.reserve([1, 1], 1) == [-2, 0]
+    q = prepared(L, p.cache, 2, 1, 4, rng.normal(size=(2, 8 * 64)), p.ones)
+    now = p.k.get(), p.v.get()
+    for a, b in zip(now, (k, v)):
+        np.testing.assert_array_equal(np.delete(a, 5, 0), np.delete(b, 5, 0))
+    out, shared = L.Device.empty((2, 4, 64), np.float32), L.Device(np.zeros(1, np.int32))
+    for name, ws in (("tree", L.attention_workspace(2, 1, 4, 2, 64)), ("shared", L.shared_attention_workspace(2, 1, 4, 2, 64))):
+        prefix = (shared.p,) if name == "shared" else ()
+        L.call(name + "_attention", out.p, q.p, C.byref(p.cache), 0, *prefix, None, 0.125, 2, 1, 4, ws.p)
+        got = out.get()
+        assert np.isnan(got[0]).all()
+        ref = S.attention(q.get()[1:], now[0][:6], now[1][:6], S.chain_masks(1), 0.125)
+        assert_parity(got[1], ref[0])
+    path, accepted = L.Device(np.zeros(2, np.int32)), L.Device(np.zeros(2, np.int32))
+    L.call("cache_commit", C.byref(p.cache), p.lengths.p, path.p, accepted.p, 2, 1)
+    assert list(p.lengths.get()) == [0, 6]
+
+
+@pytest.mark.parametrize("hq,hkv,d,tokens", [(8, 2, 64, 1), (8, 2, 128, 1), (8, 2, 128, 4), (24, 2, 256, 1), (24, 2, 256, 7)])
+def test_pages_held_bound_what_a_step_reaches(L, hq, hkv, d, tokens):  # noqa: F811
+    """Sequences whose pages do not reach their last node are refused, whatever their row of the table says behind them."""
+    rng = np.random.default_rng(42)
+    lengths = [30, 32 - tokens, 33 - tokens, 100, 0, 70, 40]
+    cache = SharedCache(L, rng, 0, lengths, tokens, hkv, d, 16)
+    table = cache.table.copy()
+    table[table == 1 << 30] = 0
+    cache.dt.set(table)
+    need = [-(-(n + tokens) // 16) for n in lengths]
+    assert need[1] == 2 and need[2] == 3
+    held = [need[0], 2, 2, need[3] - 1, 0, -(1 << 31), cache.table_pages + 1]
+    cache.c.held = (keep := L.Device(np.array(held, np.int32))).p
+    q = rng.normal(size=(7, tokens, hq, d)).astype(np.float32)
+    ref, good, bad = expected(cache, q, None, 0.1), [0, 1], [2, 3, 4, 5, 6]
+    for got in (attend(L, cache, q, None, 0.1, calls=2), attend_shared(L, cache, q, None, 0.1, calls=2)):
+        assert np.isnan(got[bad]).all()
+        assert_parity(got[good], ref[good])
+    path, accepted, out = L.Device(np.zeros((7, tokens), np.int32)), L.Device(np.zeros(7, np.int32)), L.Device(np.zeros(7, np.int32))
+    L.call("cache_commit", C.byref(cache.c), out.p, path.p, accepted.p, 7, tokens)
+    assert list(out.get()) == [n + (s in good) for s, n in enumerate(lengths)]
+    before = cache.dk.get()
+    width = (hq + 2 * hkv) * d
+    ones = L.Device(np.ones(d, np.float32))
+    prep = prepared(L, cache.c, 7, tokens, hq, rng.normal(size=(7 * tokens, width)), ones).get().reshape(7, tokens, hq, d)
+    assert np.isnan(prep[bad]).all() and np.isfinite(prep[good]).all()
+    changed = np.flatnonzero((before[0].view(np.uint16) != cache.dk.get()[0].view(np.uint16)).any(axis=(1, 2)))
+    assert set(changed) <= {int(r) for s in good for r in cache.rows(s, lengths[s], tokens)}
+    assert keep.get()[0] == held[0]
+
+
+@pytest.mark.parametrize("pages", [6, 60])
+def test_steps_of_users_with_drafts_of_different_number(L, pages):  # noqa: F811
+    """Pages, preparation, attention of trees, truncation, acceptance, commit and the pages given back, step after step, from one graph's worth of
+    calls without the host: a sequence sits out with a count of 0, has all of the step's nodes otherwise, waits where the pool has
+    nothing left, and every sequence's committed keys and values are the ones that its accepted nodes had."""
+    seqs, tokens, hq, hkv, d, vocab = 6, 5, 4, 2, 64, 97
+    rng = np.random.default_rng(pages)
+    p = Paged(L, seqs, pages, 8)
+    want = [np.zeros((0, 2, hkv, d), np.float16) for _ in range(seqs)]
+    shared, aws, vws = L.Device(np.zeros(1, np.int32)), L.shared_attention_workspace(seqs, tokens, hq, hkv, d), L.verify_workspace(seqs, tokens, vocab)
+    out, weights = L.Device.empty((seqs, tokens, hq * d), np.float32), L.Device(rng.normal(size=(vocab, hq * d)).astype(np.float32))
+    logits = L.Device.empty((seqs, tokens, vocab), np.float32)
+    path, accepted, after = L.Device.empty((seqs, tokens), np.int32), L.Device.empty(seqs, np.int32), L.Device.empty(seqs, np.int32)
+    lengths, refused, advanced = np.zeros(seqs, np.int32), 0, 0
+    for step in range(24):
+        ended = rng.random(seqs) < 0.15
+        for s in np.flatnonzero(ended):
+            want[s] = want[s][:0]
+        p.lengths.set(np.where(ended, -1, lengths).astype(np.int32))
+        p.release()
+        lengths[ended] = 0
+        p.lengths.set(lengths)
+        counts = np.where(rng.random(seqs) < 0.25, 0, tokens)
+        counts[lengths + tokens > 8 * 16] = 0
+        taken = p.reserve(counts, tokens)
+        sits = counts == 0
+        parents = np.array([random_tree(rng, tokens) for _ in range(seqs)], np.int32)
+        drafts, u = rng.integers(0, vocab, (seqs, tokens)).astype(np.int32), rng.random((seqs, tokens)).astype(np.float32)
+        masks = L.Device(np.array([S.tree_masks(list(r)) for r in parents], np.uint64))
+        q = prepared(L, p.cache, seqs, tokens, hq, rng.normal(size=(seqs * tokens, (hq + 2 * hkv) * d)), p.ones)
+        stored = [np.stack([x.get()[p.rows(s, lengths[s], tokens)] for x in (p.k, p.v)], axis=1) if taken[s] >= 0 and not sits[s] else None for s in range(seqs)]
+        L.call("shared_attention", out.p, q.p, C.byref(p.cache), 0, shared.p, masks.p, 0.125, seqs, tokens, hq, aws.p)
+        L.call("matmul", logits.p, weights.p, 0, vocab, hq * d, out.p, seqs * tokens)
+        t, k = L.Device(np.full(seqs, 0.9, np.float32)), L.Device(np.full(seqs, 20, np.int32))
+        L.call("truncate_logits", logits.p, logits.p, t.p, k.p, None, None, tokens, seqs * tokens, vocab)
+        dd, dp, du = L.Device(drafts), L.Device(parents), L.Device(u)
+        L.call("verify_tree", path.p, accepted.p, after.p, logits.p, dd.p, dp.p, None, du.p, float(np.float32(0.9)), seqs, tokens, vocab, vws.p)
+        took = accepted.get()
+        took[sits] = -1  # (who sits out has no say, whether or not its last page has room)
+        accepted.set(took)
+        L.call("cache_commit", C.byref(p.cache), p.lengths.p, path.p, accepted.p, seqs, tokens)
+        steps, now = path.get(), p.lengths.get()
+        for s in range(seqs):
+            if sits[s] or taken[s] < 0:
+                refused += taken[s] == -2
+                assert now[s] == lengths[s] and (sits[s] or (took[s] == -1 and after.get()[s] == -1))
+                continue
+            assert took[s] >= 0 and now[s] == lengths[s] + took[s] + 1
+            want[s] = np.concatenate([want[s], stored[s][steps[s, : took[s] + 1]]])
+            advanced += 1
+        lengths = now.copy()
+        keys, values = p.k.get(), p.v.get()
+        for s in range(seqs):
+            rows = p.rows(s, 0, lengths[s])
+            np.testing.assert_array_equal(np.stack([keys[rows], values[rows]], axis=1), want[s], err_msg=f"step {step}, sequence {s}")
+    assert advanced > 20 and (refused > 0) == (pages == 6)
 
 
 # ---- users ---------------------------------------------------------------------
