@@ -979,6 +979,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // no CTA ends while others read its memory
 }
 
+constexpr int smem_of(int units) { return kThreads * (units | 1) * 16 + (int)sizeof(Shared); }
+static_assert(smem_of(kMaxUnits) <= 232448, "shared memory");
+
 int launch(SampleArgs &a, int rows) {
     // up to three logits may lie before a row that does not start on 16 bytes
     const bool aligned = !(reinterpret_cast<uintptr_t>(a.logits) & 15) && a.vocab % 4 == 0;
@@ -995,13 +998,14 @@ int launch(SampleArgs &a, int rows) {
     for (int n = 1; n <= kMaxRanks; n++) {
         const int units = ((long_row + n - 1) / n + kStep - 1) / kStep;
         if (units > kMaxUnits) continue;
-        const bool half = kThreads * (units | 1) * 16 + (int)sizeof(Shared) <= 115200;
+        const bool half = smem_of(units) <= 115200;
         const int one = kOne[n - 1], fit = half ? kTwo[n - 1] : one, rest = rows % fit;
         const long long time = (long long)(7 + units) * ((long long)(rows / fit) * (half ? 7 : 5) + (rest > one ? 7 : rest ? 5 : 0));
         if (!best || time < best) best = time, ranks = n, clusters = rows < fit ? rows : fit, a.units = units;
     }
-    const int smem = kThreads * (a.units | 1) * 16 + (int)sizeof(Shared);
-    if (int rc = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return rc;
+    const int smem = smem_of(a.units);
+    // (the kernel's limits are the same in every call: another thread's, for a row of another length, may come before this launch)
+    if (int rc = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_of(kMaxUnits))) return rc;
     if (int rc = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) return rc;
     a.inverse = 65535 / a.units + 1;
     a.rows = rows;

@@ -1,12 +1,14 @@
 """Operators for a batch of users on a B200, at the edges of what their header allows and next to each other."""
 import ctypes as C
+import threading
 
 import numpy as np
 import pytest
 
 from conftest import assert_parity
+from oracle import batch as B
 from oracle import speculate as S
-from test_gpu_sample import L, check  # noqa: F401  (L is a fixture)
+from test_gpu_sample import L, check, peaked  # noqa: F401  (L is a fixture)
 from test_gpu_shared_attention import SharedCache, attend_shared
 from test_gpu_speculate import attend, expected, random_tree
 
@@ -26,6 +28,57 @@ def test_min_p_above_one_leaves_the_first_of_equals(L, least):  # noqa: F811
     u = np.array([0.0, 0.9, 0.99, 0.3, 0.7, 0.999, 0.5, 0.6])
     for k, p in ((0, 1.0), (50, 1.0), (400, 1.0), (2000, 1.0), (5002, 0.9), (0, 0.9), (0, 0.0), (1, 1.0)):
         check(L, x, u, [1.0] * 8, [k] * 8, [p] * 8, [least] * 8)
+
+
+def test_threads_that_sample_different_vocabularies(L):  # noqa: F811
+    """Entry points are called by several host threads; what one call asks of the kernel is not another's."""
+    rng = np.random.default_rng(22)
+    work = []
+    for vocab, rows in ((1000, 2), (360445, 1), (131072, 1), (50001, 3)):
+        x, u = peaked(rng, rows, vocab).astype(np.float32), rng.random(rows).astype(np.float32)
+        work.append((x, u, L.Device(x), L.Device(u), L.Device(np.zeros(rows, np.int32)), L.Device(np.full(rows, 40, np.int32)), L.Device(x)))
+    failed = []
+
+    def go(n):
+        x, u, dx, du, token, k, out = work[n]
+        try:
+            for _ in range(1500):
+                L.call("sample", token.p, dx.p, du.p, None, k.p, None, None, 1, *x.shape)
+                L.call("truncate_logits", out.p, dx.p, None, k.p, None, None, 1, *x.shape)
+        except Exception as e:  # (an assertion in a thread would be lost)
+            failed.append((n, e))
+
+    threads = [threading.Thread(target=go, args=(n,)) for n in range(len(work))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for x, u, _, _, token, _, out in work:
+        got, cut = token.get(), out.get()
+        for r in range(len(x)):
+            assert got[r] == B.sample(x[r], u[r], top_k=40)[0]
+            assert sorted(np.flatnonzero(cut[r] > -np.inf)) == sorted(int(b) for b in B.kept(x[r], top_k=40)[0])
+
+
+def test_one_graph_of_different_vocabularies(L):  # noqa: F811
+    rng = np.random.default_rng(23)
+    work = []
+    for vocab in (360445, 1000, 131072):
+        x, u = peaked(rng, 2, vocab).astype(np.float32), rng.random(2).astype(np.float32)
+        work.append((x, u, L.Device(x), L.Device(u), L.Device(np.zeros(2, np.int32)), L.Device(np.full(2, 0.7, np.float32))))
+    g = C.c_void_p()
+    L.call("graph_begin", C.byref(g))
+    for x, _, dx, du, token, t in work:
+        L.call("sample", token.p, dx.p, du.p, t.p, None, None, None, 1, *x.shape)
+    L.call("graph_end", g)
+    for _ in range(3):
+        L.call("graph_launch", g)
+    for x, u, _, _, token, _ in work:
+        got = token.get()
+        for r in range(2):
+            assert got[r] == B.sample(x[r], u[r], temperature=float(np.float32(0.7)))[0]
+    L.graph_destroy(g)
 
 
 # ---- pages that a sequence no longer has -------------------------------------
