@@ -73,6 +73,7 @@ struct AttendArgs {
     float *part_acc;   // [2 * kMaxCtas][part_rows][D]
     float2 *part_ml;   // [2 * kMaxCtas][part_rows]
     // with a shared prefix:
+    float tile_scale;    // scale, and what makes up for the tensor cores' sums
     const int *shared;
     int all_tiles;       // row tiles of all sequences' rows together
     float *prefix_acc;   // [row][q_heads][D], [row][q_heads]: of prefix items that one CTA did as a whole
@@ -1003,7 +1004,7 @@ __device__ __forceinline__ void attend_tiles(const AttendArgs &a, const CUtensor
                         }
                         const int at = lane * V, unit = (at % 64) / 8;
                         for (int rr = r; rr < MR; rr += span) {
-                            if (lane == 0) s.q_scale[qb][rr] = fmaxf(a.scale * inv, 1e-44f);  // never 0: -infinity stays what it is
+                            if (lane == 0) s.q_scale[qb][rr] = fmaxf((SHARED ? a.tile_scale : a.scale) * inv, 1e-44f);  // never 0: -infinity stays what it is
                             unsigned char *dst = q_to + (at / 64) * C::kBlock + rr * 128 + ((unit ^ (rr & 7)) << 4) + (at % 8) * 2;
                             if constexpr (V == 8) {
                                 *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
@@ -1933,6 +1934,7 @@ int attend_args(AttendArgs &a, float *out, const float *q, const qg_kv_cache *ca
     a.tokens = tokens;
     a.q_heads = q_heads;
     a.group = q_heads / a.c.kv_heads;
+    a.tile_scale = a.scale;
     a.shared = nullptr;
     a.all_tiles = 0;
     a.prefix_acc = nullptr;
@@ -2020,10 +2022,11 @@ extern "C" int qg_shared_attention(float *out, const float *q, const qg_kv_cache
     const bool pair = d == 256 && rows > kRows;
     a.copies = 1;
     // The tensor cores cut off what does not fit when they add to S: two planes of d/16 steps each take half a unit in the last
-    // place, 0.72 * 2^-24 on average over the mantissas, of a running sum that is half of the final one on average. So scores
-    // are too small by d/16 * 0.72 * 2^-24, which the scale makes up for (24/2 heads of 256, 8,192 shared: errors against 64
-    // bits 1.8e-6 -> 0.95e-6; 32/8 of 128 0.94 -> 0.57e-6; 16/4 of 64 0.58 -> 0.39e-6).
-    a.scale = (float)((double)a.scale * (1.0 + d / 16 * 0.72 / 16777216.0));
+    // place, 0.72 * 2^-24 on average over the mantissas, of a running sum that is half of the final one on average (both of random
+    // keys and queries; sums that cancel lose less). So their scores are too small by d/16 * 0.72 * 2^-24, which their scale makes
+    // up for (24/2 heads of 256, 8,192 shared: errors against 64 bits 1.8e-6 -> 0.95e-6; 16/4 of 64 0.58 -> 0.39e-6). Scores that
+    // attend_tokens adds up lose nothing and have the scale as it is.
+    a.tile_scale = (float)((double)a.scale * (1.0 + d / 16 * 0.72 / 16777216.0));
     tiles(a, rows, pair);
     a.shared = shared;
     a.all_tiles = (rows + a.tile_rows - 1) / a.tile_rows;

@@ -81,6 +81,31 @@ def test_one_graph_of_different_vocabularies(L):  # noqa: F811
     L.graph_destroy(g)
 
 
+# ---- attention with a shared prefix ------------------------------------------
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(2, 2, 64), (8, 2, 64), (4, 2, 128), (32, 8, 128)])
+@pytest.mark.parametrize("shared", [0, 128])
+def test_scores_of_single_tokens_of_few_heads_are_not_stretched(L, hq, hkv, d, shared):  # noqa: F811
+    """One key at score 0 and one at -64, both of the sequence's own: the second's share is e^-64 to within what the roundings on its way can do.
+    The score is exact but for log2(e) as a float (2^-24 of 64); beside it ex2 (2^-22) and a dozen roundings (2^-24 each). With a
+    prefix, its keys are at -512 and weigh nothing."""
+    rng = np.random.default_rng(d)
+    cache = SharedCache(L, rng, shared, [1, 1, 1], 1, hkv, d, 16)
+    cache.k[:], cache.v[:] = 0.0, 0.0
+    for s in range(3):
+        if shared:
+            cache.k[0, cache.rows(s, 0, shared), :, 0] = -64.0
+        at = cache.rows(s, shared + 1, 1)
+        cache.k[0, at, :, 0], cache.v[0, at] = -8.0, 1.0
+    cache.upload()
+    q = np.zeros((3, 1, hq, d), np.float32)
+    q[..., 0] = 8.0
+    got = attend_shared(L, cache, q, None, 1.0).astype(np.float64)
+    ref = np.exp(-64.0) / (1 + np.exp(-64.0))
+    assert np.abs(got / ref - 1).max() <= (64 + 4 + 12) * 2.0 ** -24
+
+
 # ---- pages that a sequence no longer has -------------------------------------
 
 
