@@ -123,7 +123,8 @@ __device__ __forceinline__ unsigned key_of(float x) {
     return b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float of_key(unsigned k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
-constexpr unsigned kNone = 0x007fffffu;  // key of -infinity
+constexpr unsigned kNone = 0x007fffffu;       // key of -infinity
+constexpr unsigned kMinusZero = 0x7fffffffu;  // of -0, which no logit is
 constexpr float kLowest = -3.402823466e38f;
 
 __device__ __forceinline__ Whole warp_sum(Whole x) {
@@ -397,6 +398,8 @@ struct Range {
     unsigned low, high;
     float most, scale;
     int last_bin, bin;
+    // Up to where its logits are looked for. Keys that end at -0's end below 0, which as a float is not above it.
+    __device__ __forceinline__ float highest() const { return of_key(high == kMinusZero ? high - 1 : high); }
     __device__ __forceinline__ int bin_of(float x) const { return min(last_bin, (int)((most - x) * scale)); }
     __device__ __forceinline__ bool has(float x) const { return bin < 0 || bin_of(x) == bin; }  // of those between low and high
     // Only what is in distance bin b. The keys' limits are wider than the bin by more than bin_of rounds.
@@ -418,7 +421,7 @@ struct Range {
 // The kept logits in a range, of all CTAs and in any order, in s.entry. Returns their number; more than kList are not listed.
 // s.listed is zero before.
 __device__ int gather(Shared &s, const Row &r, const Range &in) {
-    r.some(of_key(max(in.low, kNone + 1)), of_key(in.high), [&](const float (&x)[2], const int (&at)[2]) {
+    r.some(of_key(max(in.low, kNone + 1)), in.highest(), [&](const float (&x)[2], const int (&at)[2]) {
 #pragma unroll
         for (int e = 0; e < 2; e++)
             if (r.kept_of_floor(x[e], at[e]) && in.has(x[e])) {
@@ -550,7 +553,7 @@ __device__ void narrow(Shared &s, Row &r, Whole target, Range in, bool linear, i
     for (; linear || in.low < in.high; linear = false) {
         const int shift = in.shift();
         Hist &hist = s.hist[pass & 1], &other = s.hist[~pass & 1];  // (zeros)
-        r.some(of_key(max(in.low, kNone + 1)), of_key(in.high), [&](const float (&x)[2], const int (&at)[2]) {
+        r.some(of_key(max(in.low, kNone + 1)), in.highest(), [&](const float (&x)[2], const int (&at)[2]) {
             const Whole w[2] = {SUM ? r.weigh(x[0]) : 1, SUM ? r.weigh(x[1]) : 1};
 #pragma unroll
             for (int e = 0; e < 2; e++)

@@ -30,6 +30,22 @@ def test_min_p_above_one_leaves_the_first_of_equals(L, least):  # noqa: F811
         check(L, x, u, [1.0] * 8, [k] * 8, [p] * 8, [least] * 8)
 
 
+@pytest.mark.parametrize("zeros,small", [(1500, 1500), (300, 500), (1200, 40), (40, 1200)])
+def test_keys_of_zero_and_of_the_numbers_next_to_it(L, zeros, small):  # noqa: F811
+    """Borders among logits just below 0 (multiples of 2^-149) with zeros above them, where the range of keys that is left ends between the two:
+    the largest logit's mantissa is all ones, so that bins of keys begin there."""
+    rng = np.random.default_rng(1)
+    row = np.full(20000, -300.0, np.float32)
+    below = -(rng.integers(1, 100000, small).astype(np.uint32).view(np.float32))
+    some = np.concatenate([rng.uniform(0.3, 0.99, 3999), [np.float32(0.99999994)], np.zeros(zeros), below]).astype(np.float32)
+    row[: len(some)] = rng.permutation(some)
+    k = 4000 + zeros + small // 2
+    w = np.sort(np.exp((row.astype(np.float64) - row.max()) / 60))[::-1]
+    p = float((np.cumsum(w)[k - 1] - w[k - 1] / 2) / w.sum())  # as many as k, with a temperature of 60
+    x, u = np.tile(row, (4, 1)), rng.random(4)
+    check(L, x, u, [1.0, 60.0, 60.0, 60.0], [k, k, 0, 15000], [1.0, 1.0, p, p])
+
+
 def test_threads_that_sample_different_vocabularies(L):  # noqa: F811
     """Entry points are called by several host threads; what one call asks of the kernel is not another's."""
     rng = np.random.default_rng(22)
