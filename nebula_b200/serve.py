@@ -95,6 +95,8 @@ class Batch(Speculator):
 
     def leave(self, at: int) -> User:
         """The user's pages go back to the pool, but for the prompt's."""
+        if not isinstance(at, (int, np.integer)) or not 0 <= at < self.users or self.places[at] is None:
+            raise ValueError(f"place {at} has no user")
         user, self.places[at] = self.places[at], None
         one = np.array([-1], np.int32)
         L.call("write", self.lengths.p + 4 * at, one.ctypes.data, 4)

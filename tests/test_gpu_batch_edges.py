@@ -374,3 +374,15 @@ def test_settings_that_no_row_can_have_are_refused(V):
     batch.join(user)
     batch.step()
     assert len(user.text) == 1
+
+
+def test_places_that_no_one_has(V):
+    batch = V.Batch(2, **SIZE)
+    batch.join(V.User([1], V.uniforms(0)))
+    for at in (-1, -2, 1, 2, 0.0, None):
+        with pytest.raises(ValueError):
+            batch.leave(at)
+    batch.leave(0)
+    with pytest.raises(ValueError):
+        batch.leave(0)
+    assert batch.pages_in_use() == 0
