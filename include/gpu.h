@@ -425,8 +425,8 @@ typedef struct {
  * outside 0..table_pages). slots [seq][tokens] (may be NULL): the pool row of
  * each new position, -1 behind counts[s], for sequences that were refused
  * or got none, and where the row names a page outside the pool. A *free_count
- * outside 0..pages counts as 0. tokens at most 2^30, seqs*tokens below 2^31; taken
- * is neither lengths nor counts. */
+ * outside 0..pages counts as 0. tokens at most 2^30, seqs*tokens below 2^31. taken
+ * and slots overlap nothing else that the call reads or writes. */
 int qg_pages_reserve(const qg_page_pool *pool, int *slots, int *taken, const int *lengths, const int *counts, int seqs, int tokens);
 /* Gives back what sequence s's first lengths[s] positions do not need (a negative
  * length: all), its first shared_pages entries excepted: the pages of the first
@@ -434,7 +434,7 @@ int qg_pages_reserve(const qg_page_pool *pool, int *slots, int *taken, const int
  * again hands them out as before. freed[s]: pages given back, -1: refused (held outside
  * 0..table_pages; and every sequence with pages to give back where the stack would
  * hold more than the pool, or *free_count is negative: then nothing changes).
- * freed is not lengths. */
+ * freed overlaps nothing else that the call reads or writes. */
 int qg_pages_release(const qg_page_pool *pool, int *freed, const int *lengths, int shared_pages, int seqs);
 
 /* ---- loading an all-resident model (no counterpart in the reference

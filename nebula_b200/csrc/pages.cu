@@ -211,12 +211,27 @@ __global__ void __launch_bounds__(256) slots_kernel(const __grid_constant__ Page
 template <typename... T>
 bool unaligned(const T *...p) { return ((reinterpret_cast<uintptr_t>(p) | ...) & 3) != 0; }
 
+// n values at p.
+struct Span {
+    const int *p;
+    size_t n;
+    bool meets(const Span &o) const { return p && o.p && p < o.p + o.n && o.p < p + n; }
+};
+// What a call writes besides the pool's arrays must not be one of these or of the inputs, not even in part: sequences' results are
+// written while others' inputs are read.
+bool meets_pool(const Span &x, const qg_page_pool *p, int seqs) {
+    return x.meets({p->page_table, (size_t)seqs * p->table_pages}) || x.meets({p->held, (size_t)seqs}) || x.meets({p->free_pages, (size_t)p->pages}) ||
+           x.meets({p->free_count, 1});
+}
+
 int pages_args(const qg_page_pool *p, int *out, const int *lengths, int seqs, PagesArgs &a) {
     if (!p || !p->page_table || !p->held || !p->free_pages || !p->free_count || !out || !lengths || seqs < 1 || seqs > kMaxSeqs ||
-        p->pages < 1 || p->table_pages < 1 || out == lengths || unaligned(p->page_table, p->held, p->free_pages, p->free_count, out, lengths))
+        p->pages < 1 || p->table_pages < 1 || unaligned(p->page_table, p->held, p->free_pages, p->free_count, out, lengths))
         return cudaErrorInvalidValue;
     a.shift = page_shift(p->page_tokens);
     if (a.shift < 0 || pool_too_large(p->pages, p->table_pages, a.shift)) return cudaErrorInvalidValue;
+    const Span results = {out, (size_t)seqs};
+    if (results.meets({lengths, (size_t)seqs}) || meets_pool(results, p, seqs)) return cudaErrorInvalidValue;
     a.table = p->page_table;
     a.held = p->held;
     a.stack = p->free_pages;
@@ -257,7 +272,9 @@ extern "C" int qg_pages_reserve(const qg_page_pool *pool, int *slots, int *taken
                                 int tokens) {
     PagesArgs a;
     if (int rc = pages_args(pool, taken, lengths, seqs, a)) return rc;
-    if (tokens < 1 || tokens > 1 << 30 || (long long)seqs * tokens > 0x7fffffffll || (counts && counts == taken) || unaligned(slots, counts))
+    if (tokens < 1 || tokens > 1 << 30 || (long long)seqs * tokens > 0x7fffffffll || unaligned(slots, counts)) return cudaErrorInvalidValue;
+    const Span results = {taken, (size_t)seqs}, places = {slots, (size_t)seqs * tokens}, asked = {counts, (size_t)seqs};
+    if (results.meets(asked) || places.meets(asked) || places.meets(results) || places.meets({lengths, (size_t)seqs}) || meets_pool(places, pool, seqs))
         return cudaErrorInvalidValue;
     const bool wide = slots && (long long)seqs * tokens > kWide;
     a.slots = wide ? nullptr : slots;

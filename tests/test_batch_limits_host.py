@@ -13,3 +13,24 @@ def test_pages_held_are_whole_numbers(off):
     assert batch.attention(batch.cache(held=P4 + off)) == INVALID
     for entry in (verify.attention, verify.prep, verify.commit):
         assert entry(verify.cache(held=P4 + off)) == INVALID
+
+
+POOL = dict(page_table=P4 + (1 << 16), held=P4 + (2 << 16), free_pages=P4 + (3 << 16), free_count=P4 + (4 << 16))
+FREE = dict(slots=P4 + (5 << 16), taken=P4 + (6 << 16), lengths=P4 + (7 << 16), counts=P4 + (8 << 16))
+
+
+@pytest.mark.parametrize("what", ["page_table", "held", "free_pages", "free_count", "lengths", "counts", "slots", "taken"])
+def test_results_of_pages_overlap_nothing(what):
+    """Not in part either: a sequence's result is written while another's lengths, counts or pages are read. Three sequences, 20 entries of
+    the table each, 100 pages, 5 slots a sequence."""
+    size = dict(page_table=60, held=3, free_pages=100, free_count=1, lengths=3, counts=3, slots=15, taken=3)
+    at = {**POOL, **FREE}[what]
+    for name in ("taken", "slots"):
+        if name == what:
+            continue
+        for p in {at, at + 4 * (size[what] - 1), at - 4 * (size[name] - 1)}:
+            assert batch.reserve(batch.pool(**POOL), **{**FREE, name: p}) == INVALID, (name, p - at)
+    if what in ("counts", "slots", "taken"):
+        return
+    for p in {at, at + 4 * (size[what] - 1), at - 8}:
+        assert batch.release(batch.pool(**POOL), freed=p, lengths=FREE["lengths"]) == INVALID, p - at
