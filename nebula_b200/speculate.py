@@ -160,9 +160,12 @@ class Speculator:
         uniforms = np.zeros(t) if uniforms is None else np.asarray(uniforms, np.float64)
         if uniforms.shape != (t,) or not ((uniforms >= 0) & (uniforms < 1)).all():
             raise ValueError(f"{t} uniforms in [0, 1)")
+        truncates = top_k > 0 or top_p < 1 or min_p > 0
+        check_settings(temperature if truncates else 0.0, top_k, top_p, min_p)
         self.forward(tokens, parents)
         L.call("matmul", self.logits.p, self.head.p, F32, self.vocab, self.hidden, self.x.p, t)
-        if top_k > 0 or top_p < 1 or min_p > 0:
+        if truncates:
+            temperature = float(np.float32(temperature))  # one temperature for what is kept and what is accepted
             for buf, value, kind in ((self.temperature, temperature, np.float32), (self.top_k, top_k, np.int32), (self.top_p, top_p, np.float32),
                                      (self.min_p, min_p, np.float32)):
                 self._put(buf, [value], kind)

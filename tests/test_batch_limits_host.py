@@ -4,6 +4,7 @@ import pytest
 
 import test_batch_host as batch
 import test_speculate_host as verify
+from test_speculator_limits import model  # noqa: F401  (a fixture)
 
 INVALID, P4 = batch.INVALID, batch.P4
 
@@ -34,3 +35,11 @@ def test_results_of_pages_overlap_nothing(what):
         return
     for p in {at, at + 4 * (size[what] - 1), at - 8}:
         assert batch.release(batch.pool(**POOL), freed=p, lengths=FREE["lengths"]) == INVALID, p - at
+
+
+@pytest.mark.parametrize("settings", [dict(top_p=float("nan")), dict(min_p=float("nan")), dict(top_k=0.5), dict(top_k=1 << 31), dict(top_k=float("nan")),
+                                      dict(temperature=1e39, top_k=5), dict(temperature=float("nan"), min_p=0.1), dict(temperature=-1.0, top_p=0.9)], ids=str)
+def test_steps_refuse_settings_that_no_row_can_have(model, settings):  # noqa: F811
+    """NaN is neither below 1 nor above 0: the target would have been left as it is."""
+    with pytest.raises(ValueError):
+        model.step([1, 2], [-1, 0], [0.5, 0.5], **{"temperature": 1.0, **settings})
