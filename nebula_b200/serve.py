@@ -55,6 +55,11 @@ class Batch(Speculator):
         self.shared_ws = L.shared_attention_workspace(users, 1, self.q_heads, self.kv_heads, self.head_dim)
         self.prompt_pages, self.places = np.zeros(0, np.int32), [None] * users
 
+    def forward(self, *_) -> None:
+        raise NotImplementedError("one sequence's: a batch reads with read_prompt, join and step")
+
+    prefill = forward
+
     def read_prompt(self, tokens) -> list:
         """The prompt's whole pages are read once, for all users that come. Returns the tokens after them: each user's first."""
         if any(self.places) or len(self.prompt_pages):

@@ -43,3 +43,13 @@ def test_steps_refuse_settings_that_no_row_can_have(model, settings):  # noqa: F
     """NaN is neither below 1 nor above 0: the target would have been left as it is."""
     with pytest.raises(ValueError):
         model.step([1, 2], [-1, 0], [0.5, 0.5], **{"temperature": 1.0, **settings})
+
+
+def test_a_batch_reads_no_single_sequence():
+    """What Speculator does to one sequence of its own cache would go to the first user's pages."""
+    from nebula_b200 import serve
+    b = serve.Batch.__new__(serve.Batch)
+    with pytest.raises(NotImplementedError):
+        b.forward([1], [-1])
+    with pytest.raises(NotImplementedError):
+        b.prefill([1])
