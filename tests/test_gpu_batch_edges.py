@@ -9,7 +9,7 @@ from conftest import assert_parity
 from oracle import batch as B
 from oracle import speculate as S
 from test_gpu_sample import L, check, peaked  # noqa: F401  (L is a fixture)
-from test_gpu_shared_attention import SharedCache, attend_shared
+from test_gpu_shared_attention import SharedCache, attend_shared, scores_off
 from test_gpu_speculate import attend, expected, random_tree
 
 pytestmark = pytest.mark.gpu
@@ -120,6 +120,41 @@ def test_scores_of_single_tokens_of_few_heads_are_not_stretched(L, hq, hkv, d, s
     got = attend_shared(L, cache, q, None, 1.0).astype(np.float64)
     ref = np.exp(-64.0) / (1 + np.exp(-64.0))
     assert np.abs(got / ref - 1).max() <= (64 + 4 + 12) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("hq,hkv,d,tokens", [(8, 2, 64, 1), (32, 8, 128, 1), (8, 2, 128, 3), (24, 2, 256, 5)])
+def test_a_prefix_that_weighs_a_little_more_or_less(L, hq, hkv, d, tokens):  # noqa: F811
+    """Maxima of a thousand that lie 2 apart between the prefix and a sequence's own keys: neither part may be lost, nor scaled by the
+    other's. The bound is the first order's, as for scores of some hundreds."""
+    rng = np.random.default_rng(31)
+    cache = SharedCache(L, rng, 256, [40, 300], tokens, hkv, d, 64)
+    for s, (far, near) in enumerate(((1000.0, 998.0), (1000.0, 1002.0))):
+        if s == 0:
+            cache.k[0, cache.rows(s, 0, 256), :, 0] = np.float16(far)
+        n = cache.lengths[s] + tokens - 256
+        cache.k[0, cache.rows(s, 256, n), :, 0] = np.float16(near)
+    cache.upload()
+    q = (0.1 * rng.normal(size=(2, tokens, hq, d))).astype(np.float32)
+    q[..., 0] = 1.0
+    got, ref = attend_shared(L, cache, q, None, 1.0), expected(cache, q, None, 1.0)
+    told = 0
+    for s, n in enumerate(cache.lengths):
+        rows = cache.rows(s, 0, n + tokens)
+        for t in range(tokens):
+            for h in range(hq):
+                k, v = (x[0, rows[: n + t + 1], h // (hq // hkv)].astype(np.float64) for x in (cache.k, cache.v))
+                score = k @ q[s, t, h].astype(np.float64)
+                w = np.exp(score - score.max())
+                w /= w.sum()
+                off = float(scores_off(q[s, t, h][None], k)[0])
+                assert off < 0.05
+                bound = 1.1 * off * (w @ np.abs(v - ref[s, t, h])) + 1e-5 * np.abs(ref[s, t, h]).max()
+                assert (np.abs(got[s, t, h] - ref[s, t, h]) <= bound).all(), (s, t, h)
+                lost = w[256:] if s == 0 else w[:256]  # the lighter part
+                other = slice(0, 256) if s == 0 else slice(256, None)
+                without = w[other] @ v[other] / w[other].sum()
+                told += bool(lost.sum() > 0 and (np.abs(without - ref[s, t, h]) > bound).any())
+    assert told == 2 * tokens * hq  # the inputs would show a part that is missing
 
 
 # ---- pages that a sequence no longer has -------------------------------------
