@@ -13,13 +13,20 @@ struct CacheView {
     const int *table;
     const int *lengths;
     const int *held;  // entries of a row that are its sequence's pages, or NULL: all
-    int pages, shift, table_pages, kv_heads, head_dim;
+    int pages, shift, table_pages;
+    short kv_heads, head_dim;  // 16 bits: 8 bytes more of arguments cost a commit of one sequence 0.35 of 3.9 us
 
     __host__ __device__ int page_tokens() const { return 1 << shift; }
     // Committed tokens of a sequence, or -1 when its length leaves no room for its nodes: in the table, or on the pages that it
     // has. What its row names behind those may be another sequence's by now.
     __device__ int committed(int seq, int tokens) const {
-        const int n = lengths[seq], room = held ? held[seq] : table_pages;
+        // (A load under a predicate: as a branch it takes registers that the attention's roles do not have. One sequence of 98k
+        // keys and heads of 256 106.5 us, so 102.9, and 103.1 without the check.)
+        const int n = lengths[seq];
+        int room;
+        asm volatile("{.reg .pred p;\n setp.ne.u64 p, %1, 0;\n mov.b32 %0, %3;\n @p ld.global.b32 %0, [%2];}"
+                     : "=r"(room)
+                     : "l"(held), "l"(held + seq), "r"(table_pages));
         return n >= 0 && (unsigned)room <= (unsigned)table_pages && n <= (room << shift) - tokens ? n : -1;
     }
     // Pool row of a position (64 bits: a pool may hold more than 2^31 values), or -1 for a page outside the pool.
@@ -79,8 +86,8 @@ inline int cache_view(const qg_kv_cache *c, int layer, int seqs, int tokens, Cac
     view.pages = c->pages;
     view.shift = shift;
     view.table_pages = c->table_pages;
-    view.kv_heads = c->kv_heads;
-    view.head_dim = c->head_dim;
+    view.kv_heads = (short)c->kv_heads;
+    view.head_dim = (short)c->head_dim;
     return 0;
 }
 
