@@ -737,7 +737,7 @@ __device__ __forceinline__ void do_row(const SampleArgs &a, Shared &s, float4 *p
     r.ahead = ahead, r.inverse = a.inverse;
     const float t = a.temperature ? a.temperature[user] : 1.0f, p = a.top_p ? a.top_p[user] : 1.0f, least = a.min_p ? a.min_p[user] : 0.0f;
     // (min-p above 1 leaves the token that is always kept, and of equals that is the first: what top-k leaves with 1)
-    const int k = least > 1.0f ? 1 : a.top_k ? a.top_k[user] : 0;
+    const int asked = a.top_k ? a.top_k[user] : 0, k = least > 1.0f ? 1 : asked;
     const float u = a.uniforms ? a.uniforms[row] : 0.0f;
 
     // ---- the row, and its largest logit. A warp copies its threads' units, neighbouring ones at a time.
