@@ -68,10 +68,15 @@ class Batch(Speculator):
         if whole + 1 > self.capacity or not all(0 <= int(t) < self.vocab for t in tokens):
             raise ValueError("a prompt that fits the cache, of the vocabulary's tokens")
         self._put(self.lengths, [0] + [-1] * (self.users - 1), np.int32)
-        for at in range(whole):
-            self._reserve([1] + [0] * (self.users - 1))
-            self._forward([int(tokens[at])] + [0] * (self.users - 1))
-            self._commit()
+        try:
+            for at in range(whole):
+                self._reserve([1] + [0] * (self.users - 1))
+                self._forward([int(tokens[at])] + [0] * (self.users - 1))
+                self._commit()
+        except RuntimeError:  # no page of what there is may stay behind
+            self._put(self.lengths, [-1] * self.users, np.int32)
+            L.call("pages_release", C.byref(self.pool), self.freed.p, self.lengths.p, 0, self.users)
+            raise
         n = whole // self.page
         self.prompt_pages = self.table.get()[0, :n].copy()
         self._put(self.held, [0] * self.users, np.int32)  # the prompt's pages are no one user's

@@ -421,3 +421,20 @@ def test_places_that_no_one_has(V):
     with pytest.raises(ValueError):
         batch.leave(0)
     assert batch.pages_in_use() == 0
+
+
+def test_a_prompt_that_the_pool_has_no_room_for(V):
+    """Its pages go back, and the batch is as it was: a shorter prompt, and users, find all of the pool."""
+    batch = V.Batch(2, **dict(SIZE, pages=2))
+    for _ in range(3):
+        with pytest.raises(RuntimeError):
+            batch.read_prompt(list(range(63)))  # three whole pages
+        assert batch.pages_in_use() == 0
+    rest = batch.read_prompt(list(range(20)))
+    assert batch.pages_in_use() == 1 and rest == [16, 17, 18, 19]
+    full = V.User(rest + [7], V.uniforms(0))
+    batch.join(full)
+    while len(full.text) < 3:
+        batch.step()
+    batch.leave(0)
+    assert batch.pages_in_use() == 1
