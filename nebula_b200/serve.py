@@ -116,8 +116,8 @@ class Batch(Speculator):
     def _reserve(self, counts) -> None:
         self._put(self.counts, counts, np.int32)
         L.call("pages_reserve", C.byref(self.pool), None, self.taken.p, self.lengths.p, self.counts.p, self.users, 1)
-        if any(c and t < 0 for c, t in zip(counts, self.taken.get())):
-            raise RuntimeError("the pool has no pages left, or a sequence is as long as the table")
+        if none := [at for at, (c, t) in enumerate(zip(counts, self.taken.get())) if c and t < 0]:
+            raise RuntimeError(f"places {none}: the pool has no pages left, or the sequence is as long as the table")
 
     def _forward(self, tokens) -> None:
         self.layers_of(tokens, lambda layer: L.call(

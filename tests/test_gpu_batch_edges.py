@@ -438,3 +438,22 @@ def test_a_prompt_that_the_pool_has_no_room_for(V):
         batch.step()
     batch.leave(0)
     assert batch.pages_in_use() == 1
+
+
+def test_those_who_get_no_page_are_named(V):
+    """Without them the others go on, and get the texts that they get alone."""
+    texts = [alone(V, [7 + n], n, (0.8, 40, 0.95, 0.0), 40) for n in (0, 2)]
+    batch = V.Batch(3, **dict(SIZE, pages=6))
+    rest = batch.read_prompt([3, 4, 5])
+    users = [V.User(rest + [7 + n], V.uniforms(n), (0.8, 40, 0.95, 0.0)) for n in range(3)]
+    users[1].waiting *= 8  # 32 tokens to read
+    for user in users:
+        batch.join(user)
+    with pytest.raises(RuntimeError, match=r"\[0, 1, 2\]"):
+        for _ in range(64):
+            batch.step()
+    assert batch.pages_in_use() == 6
+    batch.leave(1)
+    while min(len(users[n].text) for n in (0, 2)) < 40:
+        batch.step()
+    assert [users[n].text[:40] for n in (0, 2)] == texts
