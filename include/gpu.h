@@ -362,7 +362,8 @@ int qg_cache_commit(const qg_kv_cache *cache, int *lengths_out, const int *path,
  * finite and waits: as qg_tree_attention says, for which out is the same up to
  * rounding; a page outside the pool among the common ones makes every row NaN. The
  * workspace is zero-filled once, and is not that of qg_tree_attention. out and q
- * do not overlap. seqs*tokens*q_heads is at most 2^24. */
+ * do not overlap. seqs*tokens*q_heads is at most 2^24. Two to four sequences take about
+ * the time of qg_tree_attention or up to a tenth more, eight and more less. */
 int qg_shared_attention_workspace_bytes(int seqs, int tokens, int q_heads, int kv_heads, int head_dim, size_t *bytes);
 int qg_shared_attention(float *out, const float *q, const qg_kv_cache *cache, int layer, const int *shared, const uint64_t *tree,
                         float scale, int seqs, int tokens, int q_heads, void *workspace);
@@ -391,7 +392,9 @@ int qg_sample(int *token, const float *logits, const float *uniforms, const floa
               const float *min_p, int per, int rows, int vocab);
 /* The same logits with -infinity in place of what is not kept, so that
  * qg_verify_tree (with the same temperature) accepts and draws from what the
- * user's settings leave: per is then the nodes of a sequence. Temperature 0 keeps one
+ * user's settings leave: per is then the nodes of a sequence. That call has one
+ * temperature for all of its sequences: users with others are verified in calls of
+ * their own (a sequence's rows lie together). Temperature 0 keeps one
  * token. A row that qg_sample would refuse for its logits or settings is NaN
  * throughout. out may be logits, and overlaps them in no other way. */
 int qg_truncate_logits(float *out, const float *logits, const float *temperature, const int *top_k, const float *top_p,

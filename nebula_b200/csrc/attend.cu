@@ -34,7 +34,7 @@
 // the join adds its parts to each sequence's own. A key of the prefix is read
 // once for 128 or 256 rows, so the tensor cores bound it: with both planes of
 // Q and P 4 rows heads keys values FLOP count twice (48 x 5 rows, 32,768 shared,
-// heads of 256: 243 us at the rate of one library product, 334 measured, 382
+// heads of 256: 243 us at the rate of one library product, 330 measured, 389
 // in a loop under the power cap).
 #include <cuda.h>
 #include <cstring>
@@ -1587,8 +1587,8 @@ __device__ __forceinline__ void attend_tokens(const AttendArgs &a, unsigned char
 
 // With a shared prefix: the first CTAs do the prefix on the tensor cores, the others the sequences without them. Each has a line
 // of its own, and they share the GPU by what the lines take.
-// Time of a slot of either line, relatively (64 users, 32/8 heads of 128, 4,112 shared, in us: 1 to 1 72, 3 to 2 60, 2 to 1 53,
-// 3 to 1 52; 16,384 shared: 83, 73, 71, 66).
+// Time of a slot of either line, relatively (64 users, 4,112 shared, in us, 1 to 1, 2 to 1, 3 to 1 and 4 to 1: 32/8 heads of 128 71, 53,
+// 51, 55; 10/10 of 128 77, 53, 49, 54; 16/4 of 64 45, 37, 34, 34, with 16,384 shared 58, 51, 50, 48).
 constexpr int kPrefixUnit = 3, kTokenUnit = 1;
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1) shared_token_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap k_map,

@@ -20,7 +20,7 @@
 // What bounds it: one row is a chain of barriers of its cluster (some 0.7 us each with what they wait for) and passes over
 // 8 to 44 logits a thread; of many rows, some 45 are on the GPU at a time, as many as its shared memory holds, so their chains
 // and the 64-bit weights (15 instructions, 7.5 clocks a warp and SM) are the time, not HBM. 256 rows of 131,072 (20.5 us of
-// HBM): temperature 0 50 us, top-k 40 with top-p 79, no truncation 114, a nucleus of 0.9 198; one row 5, 9, 8 and 17.
+// HBM): temperature 0 48 us, top-k 40 with top-p 78, no truncation 113, a nucleus of 0.9 197; one row 4, 8, 8 and 15.
 #include "cache.cuh"
 
 using namespace nb;
@@ -260,7 +260,8 @@ struct Row {
     // The lowest logit that may be kept, or -infinity.
     __device__ __forceinline__ float floor() const { return of_key(key); }
 
-    // 2^44 * 2^((x - most) * c), rounded. The polynomial of degree 9 is 2^f's Chebyshev fit on [-1/2, 1/2] (error 2^-46).
+    // 2^44 * 2^((x - most) * c), rounded. The polynomial of degree 9 is 2^f's Chebyshev fit on [-1/2, 1/2] (off by less than
+    // 2^-46 there, and by 2^-45.6 of its value at most).
     __device__ __forceinline__ Whole weigh(float x) const {
         const double t = ((double)fmaxf(x, zero) - top) * c;
         constexpr double kRound = 6755399441055744.0 + 44.0, kUnit = 4503599627370496.0;  // 1.5 * 2^52 (the last bits: n + 44), 2^52
@@ -712,7 +713,9 @@ __device__ void nucleus(Shared &s, Row &r, float p, float end, bool settle, int 
 }
 
 // Bins a quarter wide around the logits that models give, and the lowest logit of one. They serve to leave out most logits
-// early, before the largest is known: others take a pass more.
+// early, before the largest is known: logits that lie elsewhere (log-probabilities, for instance) are passed over once more. 40 lower
+// or higher, 256 rows of 131,072 with top-k 40 and top-p 0.95 take 178 us for 78, with top-k 200 and min-p 154 for 121, with top-k 1000 and
+// top-p 0.8 209 for 178; one row 17 for 8.4, 14 for 11, 20 for 18.5.
 __device__ __forceinline__ int plain_bin(float x) { return (int)fminf(fmaxf((24.0f - x) * 4.0f, 0.0f), (float)(kBins - 1)); }
 __device__ __forceinline__ float plain_edge(int bin) { return 24.0f - 0.25f * (bin + 1) - 1e-4f; }
 // A lower bound of the k-th largest logit, from bins of each thread's largest, in s.hist[0] (k logits are at least as large as
@@ -990,7 +993,7 @@ int launch(SampleArgs &a, int rows) {
     const bool aligned = !(reinterpret_cast<uintptr_t>(a.logits) & 15) && a.vocab % 4 == 0;
     const int long_row = a.vocab + (aligned ? 0 : 3);
     // Clusters of more CTAs take less time for a row, but fewer of them fit: as many as these, by what cudaOccupancyMaxActiveClusters
-    // says, two CTAs to an SM (up to half its memory each) or one. A row takes about as long for its fixed steps as for seven units
+    // says of one B200 (another part's may be others, and then the choice is not the fastest), two CTAs to an SM (up to half its memory each) or one. A row takes about as long for its fixed steps as for seven units
     // of a thread, and 1.4 times as long where CTAs share an SM. A nucleus of 0.9 with the number of CTAs that this takes, and
     // with others: 14 rows of 131,072 8 (21.7 us) or 16 (24.3); 17 rows 13 (26) or 8 (27.9); 256 rows 6 (200) or 8 (209);
     // 37 rows of 50,001 7 (22.4) or 4 (25.4); 60 rows of 200,000 9 (75) or 8 (103).
