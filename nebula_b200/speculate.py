@@ -36,11 +36,13 @@ def depths(parents) -> np.ndarray:
 
 def check_settings(temperature, top_k, top_p, min_p) -> None:
     """What sampling takes: the entry points refuse the rows of other settings. (As the 32-bit numbers that they are there.)"""
-    if not all(isinstance(x, (int, float, np.integer, np.floating)) for x in (temperature, top_k, top_p, min_p)):
-        raise ValueError("temperature, top_k, top_p and min_p are numbers")
-    with np.errstate(over="ignore"):
-        t, p, m = (np.float32(x) for x in (temperature, top_p, min_p))
-    if not (0 <= t < np.inf) or np.isnan(p) or np.isnan(m) or not -(1 << 31) <= top_k < 1 << 31 or top_k != int(top_k):
+    try:
+        with np.errstate(over="ignore"):
+            t, p, m = (np.float32(x) for x in (temperature, top_p, min_p))
+        sound = 0 <= t < np.inf and p == p and m == m and -(1 << 31) <= top_k < 1 << 31 and top_k == int(top_k)
+    except (TypeError, ValueError, OverflowError):
+        sound = False
+    if not sound:
         raise ValueError(f"temperature {temperature}, top_k {top_k}, top_p {top_p}, min_p {min_p}")
 
 
