@@ -993,8 +993,9 @@ int launch(SampleArgs &a, int rows) {
     const bool aligned = !(reinterpret_cast<uintptr_t>(a.logits) & 15) && a.vocab % 4 == 0;
     const int long_row = a.vocab + (aligned ? 0 : 3);
     // Clusters of more CTAs take less time for a row, but fewer of them fit: as many as these, by what cudaOccupancyMaxActiveClusters
-    // says of one B200 (another part's may be others, and then the choice is not the fastest), two CTAs to an SM (up to half its memory each) or one. A row takes about as long for its fixed steps as for seven units
-    // of a thread, and 1.4 times as long where CTAs share an SM. A nucleus of 0.9 with the number of CTAs that this takes, and
+    // says of one B200 (another part's may be others, and then the choice is not the fastest), two CTAs to an SM (up to half its
+    // memory each) or one. A row takes about as long for its fixed steps as for seven units of a thread, and 1.4 times as long
+    // where CTAs share an SM. A nucleus of 0.9 with the number of CTAs that this takes, and
     // with others: 14 rows of 131,072 8 (21.7 us) or 16 (24.3); 17 rows 13 (26) or 8 (27.9); 256 rows 6 (200) or 8 (209);
     // 37 rows of 50,001 7 (22.4) or 4 (25.4); 60 rows of 200,000 9 (75) or 8 (103).
     static constexpr short kTwo[kMaxRanks] = {296, 148, 93, 71, 56, 45, 37, 33, 30, 26, 21, 21, 17, 14, 14, 14};
