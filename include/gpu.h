@@ -246,17 +246,19 @@ int qg_moe_profile_read(int phase, double *total_ms, int *launches);
  * 16, 32, 64, 128 or 256. head_dim: 64, 128 or 256. pages*page_tokens is at
  * most 2^31 - 1, table_pages*page_tokens at most 2^31 - 128.
  *
- * held (device [seqs], NULL: the whole row) says how many entries of a
- * sequence's row are its pages; those behind them may name pages that are
+ * held (with QG_CACHE_HELD in page_tokens: device [seqs]) says how many entries
+ * of a sequence's row are its pages; those behind them may name pages that are
  * another's by now and are never read. A cache whose pages come from a
- * qg_page_pool has the pool's.
+ * qg_page_pool has the pool's. Without QG_CACHE_HELD the whole row counts and the
+ * field is not looked at.
  *
  * A sequence whose length is negative or leaves no room for its nodes, in the
  * table or on the pages held, or whose held is outside 0..table_pages, gets NaN
- * rows and no store, and qg_cache_commit leaves its length as it is. Where its table names a page outside the pool,
- * qg_tree_attention gives all its rows NaN, qg_qk_norm_rope the rows whose own
- * position is on that page (they are not stored; its other rows are), and
- * qg_cache_commit leaves it as it is when a row would move from or to that page.
+ * rows and no store, and qg_cache_commit leaves its length as it is. Where its
+ * table names a page outside the pool, qg_tree_attention gives all its rows NaN,
+ * qg_qk_norm_rope the rows whose own position is on that page (they are not
+ * stored; its other rows are), and qg_cache_commit leaves it as it is when a row
+ * would move from or to that page.
  * Other sequences are not affected. */
 typedef struct {
     void *k, *v;
@@ -264,8 +266,9 @@ typedef struct {
     int *lengths;           /* device [seqs] */
     size_t layer_bytes;     /* from one layer's pool to the next's */
     int layers, pages, page_tokens, table_pages, kv_heads, head_dim;
-    const int *held;        /* device [seqs], or NULL */
+    const int *held;        /* device [seqs], with QG_CACHE_HELD in page_tokens */
 } qg_kv_cache;
+enum { QG_CACHE_HELD = 1 << 30 };
 
 /* table [positions][rotary/2][2]: cos and sin of position*base^(-2i/rotary),
  * evaluated in 64 bits and rounded once. rotary: even, 2..256. */
@@ -406,8 +409,8 @@ int qg_truncate_logits(float *out, const float *logits, const float *temperature
  * are entries that the host writes into several rows (and counts in their
  * held). Entries behind held keep whatever page they named last, which may be
  * another sequence's now: the cache that the step runs on is given this held
- * (qg_kv_cache), so that a sequence which got no page is left out of it on the
- * device, with NaN rows and its length as it was, and no other is touched.
+ * (QG_CACHE_HELD), so that a sequence which got no page is left out of the step on
+ * the device, with NaN rows and its length as it was, and no other is touched.
  * A call uses seqs rows of the table; calls on one pool must not overlap on the device. */
 typedef struct {
     int *page_table;  /* device [seqs][table_pages]: the cache's */
@@ -420,7 +423,8 @@ typedef struct {
 /* Room for counts[s] (0..tokens; NULL: tokens) new positions after lengths[s] of each
  * sequence. A verify step stores and reads all of its nodes: a sequence that takes
  * part in a step of `tokens` has that count however few of them it uses, and one that
- * sits out has 0 (with accepted -1 for qg_cache_commit). In the order of the sequences, the pages that lengths[s] + counts[s]
+ * sits out has 0 (with accepted -1 for qg_cache_commit).
+ * In the order of the sequences, the pages that lengths[s] + counts[s]
  * positions need beyond held[s] come off the stack and are appended to the row;
  * a sequence for which there are not enough, and all later ones that need any,
  * get none. taken[s]: pages taken, -2: none for want of pages, -1: refused (a

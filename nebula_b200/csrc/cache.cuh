@@ -72,17 +72,19 @@ inline int cache_view(const qg_kv_cache *c, int layer, int seqs, int tokens, Cac
     if (c->layers < 1 || layer < 0 || layer >= c->layers || c->pages < 1 || c->table_pages < 1 || c->kv_heads < 1 ||
         c->kv_heads > 1024 || (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256))
         return cudaErrorInvalidValue;
-    const int shift = page_shift(c->page_tokens);
+    // (a caller that knows nothing of held may not have set it)
+    const bool has_held = c->page_tokens & QG_CACHE_HELD;
+    const int shift = page_shift(c->page_tokens & ~QG_CACHE_HELD);
+    if (has_held && (!c->held || (reinterpret_cast<uintptr_t>(c->held) & 3))) return cudaErrorInvalidValue;
     if (shift < 0 || pool_too_large(c->pages, c->table_pages, shift)) return cudaErrorInvalidValue;
     const size_t pool = ((size_t)c->pages << shift) * c->kv_heads * c->head_dim * sizeof(__half);
     if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15) return cudaErrorInvalidValue;
-    if (reinterpret_cast<uintptr_t>(c->held) & 3) return cudaErrorInvalidValue;
     if (c->layers > 1 && (c->layer_bytes < pool || c->layer_bytes % 16)) return cudaErrorInvalidValue;
     view.k = reinterpret_cast<__half *>(static_cast<char *>(c->k) + layer * c->layer_bytes);
     view.v = reinterpret_cast<__half *>(static_cast<char *>(c->v) + layer * c->layer_bytes);
     view.table = c->page_table;
     view.lengths = c->lengths;
-    view.held = c->held;
+    view.held = has_held ? c->held : nullptr;
     view.pages = c->pages;
     view.shift = shift;
     view.table_pages = c->table_pages;

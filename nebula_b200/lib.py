@@ -68,10 +68,25 @@ SIGNATURES = {
 
 class KvCache(C.Structure):
     """qg_kv_cache: the paged key/value cache of the verify step (pass C.byref of it). ``held``: that of the pool which
-    the pages come from, if they do."""
+    the pages come from, if they do (None: the whole rows of the table); page_tokens says whether it is there."""
 
     _fields_ = [("k", P), ("v", P), ("page_table", P), ("lengths", P), ("layer_bytes", Z), ("layers", I), ("pages", I),
-                ("page_tokens", I), ("table_pages", I), ("kv_heads", I), ("head_dim", I), ("held", P)]
+                ("page_tokens", I), ("table_pages", I), ("kv_heads", I), ("head_dim", I), ("held_entries", P)]
+    HELD = 1 << 30  # QG_CACHE_HELD
+
+    def __init__(self, *args, held=None, **fields):
+        super().__init__(*args, **fields)
+        if held is not None:
+            self.held = held
+
+    @property
+    def held(self):
+        return self.held_entries
+
+    @held.setter
+    def held(self, p):
+        self.held_entries = p
+        self.page_tokens = self.page_tokens & ~self.HELD | (self.HELD if p else 0)
 
 
 class PagePool(C.Structure):

@@ -44,7 +44,7 @@ class Batch(Speculator):
         self.lengths = L.Device(np.full(users, -1, np.int32))
         self.held, self.free = L.Device(np.zeros(users, np.int32)), L.Device(np.arange(pages, dtype=np.int32))
         self.cache = L.KvCache(self.k.p, self.v.p, self.table.p, self.lengths.p, layer_bytes, self.layers, pages, page, table_pages,
-                               self.kv_heads, self.head_dim, self.held.p)
+                               self.kv_heads, self.head_dim, held=self.held.p)
         self.free_count = L.Device(np.array([pages], np.int32))
         self.pool = L.PagePool(self.table.p, self.held.p, self.free.p, self.free_count.p, pages, page, table_pages)
         i = lambda n: L.Device(np.zeros(n, np.int32))  # noqa: E731

@@ -16,6 +16,12 @@ def test_pages_held_are_whole_numbers(off):
         assert entry(verify.cache(held=P4 + off)) == INVALID
 
 
+def test_pages_held_that_are_announced_are_there():
+    assert batch.attention(batch.cache(page_tokens=16 | batch.L.KvCache.HELD)) == INVALID
+    for entry in (verify.attention, verify.prep, verify.commit):
+        assert entry(verify.cache(page_tokens=16 | batch.L.KvCache.HELD)) == INVALID
+
+
 POOL = dict(page_table=P4 + (1 << 16), held=P4 + (2 << 16), free_pages=P4 + (3 << 16), free_count=P4 + (4 << 16))
 FREE = dict(slots=P4 + (5 << 16), taken=P4 + (6 << 16), lengths=P4 + (7 << 16), counts=P4 + (8 << 16))
 

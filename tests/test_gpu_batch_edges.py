@@ -243,8 +243,10 @@ def test_pages_held_bound_what_a_step_reaches(L, hq, hkv, d, tokens):  # noqa: F
     need = [-(-(n + tokens) // 16) for n in lengths]
     assert need[1] == 2 and need[2] == 3
     held = [need[0], 2, 2, need[3] - 1, 0, -(1 << 31), cache.table_pages + 1]
-    cache.c.held = (keep := L.Device(np.array(held, np.int32))).p
+    cache.c.held_entries = 2  # without its flag in page_tokens: no address, and not looked at
     q = rng.normal(size=(7, tokens, hq, d)).astype(np.float32)
+    assert_parity(attend(L, cache, q, None, 0.1), expected(cache, q, None, 0.1))
+    cache.c.held = (keep := L.Device(np.array(held, np.int32))).p
     ref, good, bad = expected(cache, q, None, 0.1), [0, 1], [2, 3, 4, 5, 6]
     for got in (attend(L, cache, q, None, 0.1, calls=2), attend_shared(L, cache, q, None, 0.1, calls=2)):
         assert np.isnan(got[bad]).all()
