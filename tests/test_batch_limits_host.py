@@ -59,3 +59,13 @@ def test_a_batch_reads_no_single_sequence():
         b.forward([1], [-1])
     with pytest.raises(NotImplementedError):
         b.prefill([1])
+
+
+def test_settings_of_any_kind_of_number():
+    import numpy as np
+    from nebula_b200.speculate import check_settings
+    for settings in ((0.8, 40, 0.95, 0.0), (0, 0, 1, 0), (np.float32(1), np.int64(4), np.float64(2.0), float("inf")), (np.array(0.8), np.array(3), 1, 0), (1, 40.0, 1, 0)):
+        check_settings(*settings)
+    for settings in (("a", 0, 1, 0), (None, 0, 1, 0), (1, None, 1, 0), (1, 1 << 3000, 1, 0), (1, float("inf"), 1, 0)):
+        with pytest.raises(ValueError):
+            check_settings(*settings)
